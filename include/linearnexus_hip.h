@@ -396,6 +396,42 @@ int lnx_sigmoid_fwd(const float* x, float* y, int64_t n, void* hip_stream);
 int lnx_sigmoid_bwd(const float* y, const float* dy, float* dx, int64_t n, void* hip_stream);
 
 /*
+ * Element-wise gated linear recurrence over [B, T, D] tensors and its gradient:
+ *   h_t = e^{g_t} h_{t-1} + x_t,  y_t = h_t;   dh_t = dy_t + e^{g_{t+1}} dh_{t+1},  dx = dh,  dg_t = e^{g_t} h_{t-1} dh_t
+ * x, y, d_y, d_x in `dtype`, g and d_g in `g_dtype` (LNX_F32 or `dtype`; log-decays, <= 0, -inf drops what came before);
+ * states [B, D] ([nseq, D] packed) fp32.  x, g and d_y have a stride per row and per token in elements (last dimension
+ * contiguous); everything else is dense.  The forward call leaves in `kept` what the backward call reads (NULL: no backward
+ * pass will follow); `workspace` holds nothing between calls and may be NULL where its size is 0.  initial_state, d_y,
+ * d_final_state (zeros) and d_initial_state may be NULL.  lnx_linrec_step is one token on n = B D contiguous elements;
+ * new_state may be state.
+ */
+typedef struct lnx_linrec_args {
+  int32_t B, T, D, nseq;    /* nseq: number of packed sequences (B == 1), 0 for a dense batch */
+  int32_t dtype, g_dtype;
+  int64_t x_stride_b, x_stride_t, g_stride_b, g_stride_t, d_y_stride_b, d_y_stride_t;
+  const void* x;
+  const void* g;
+  const float* initial_state;
+  const int32_t* cu_seqlens;
+  void* y;
+  float* final_state;
+  float* kept;
+  void* workspace;
+  uint64_t workspace_bytes;
+  const void* d_y;          /* backward only, from here */
+  const float* d_final_state;
+  void* d_x;
+  void* d_g;
+  float* d_initial_state;
+} lnx_linrec_args;
+uint64_t lnx_linrec_workspace_bytes(const lnx_linrec_args* a);
+uint64_t lnx_linrec_kept_bytes(const lnx_linrec_args* a);
+int lnx_linrec_fwd(const lnx_linrec_args* a, void* hip_stream);
+int lnx_linrec_bwd(const lnx_linrec_args* a, void* hip_stream);
+int lnx_linrec_step(const void* x, const void* g, const float* state, void* y, float* new_state, int64_t n, int32_t dtype,
+                    int32_t g_dtype, void* hip_stream);
+
+/*
  * Optional per-kernel timing for benchmarks (no counterpart in the reference; its micro-benchmark
  * times whole jitted ops, bench_kda_kernels.py:216-249).  While enabled (process-wide),
  * every entry point records HIP events around each kernel it launches, on the caller's stream.

@@ -19,6 +19,7 @@ EXPORTS = (
     "lnx_chunk_workspace_bytes", "lnx_chunk_normalises_qk", "lnx_chunk_fuses_l2norm", "lnx_chunk_fwd", "lnx_chunk_fwd_segmented_bytes", "lnx_chunk_fwd_segmented", "lnx_chunk_fwd_segmented_final", "lnx_chunk_fwd_static", "lnx_chunk_fwd_static_init", "lnx_chunk_bwd", "lnx_chunk_bwd_d_o32", "lnx_chunk_rounds_d_o", "lnx_l2norm_fwd", "lnx_l2norm_bwd", "lnx_l2norm_pair_fwd", "lnx_l2norm_pair_bwd",
     "lnx_conv1d_fwd", "lnx_conv1d_bwd", "lnx_conv1d_cache_bwd", "lnx_conv1d_packed_fwd", "lnx_conv1d_packed_bwd", "lnx_conv1d_fwd_zero", "lnx_conv1d_bwd_add", "lnx_dplr_recurrent_fwd", "lnx_dplr_step", "lnx_dplr_recurrent_bwd", "lnx_dplr_recurrent_bwd_workspace_bytes", "lnx_dplr_chunk_fits", "lnx_dplr_chunk_bytes", "lnx_dplr_chunk_fwd", "lnx_dplr_chunk_bwd", "lnx_rmsnorm_gated_fwd", "lnx_rmsnorm_gated_bwd", "lnx_rmsnorm_gated_bwd_workspace_bytes",
     "lnx_gdn_gate_fwd", "lnx_gdn_gate_bwd", "lnx_gdn_gate_bwd_workspace_bytes", "lnx_kda_gate_fwd", "lnx_kda_gate_bwd", "lnx_kda_gate_bwd_workspace_bytes", "lnx_sigmoid_fwd", "lnx_sigmoid_bwd",
+    "lnx_linrec_workspace_bytes", "lnx_linrec_kept_bytes", "lnx_linrec_fwd", "lnx_linrec_bwd", "lnx_linrec_step",
     "lnx_profile_enable", "lnx_profile_read",
 )
 
@@ -62,6 +63,19 @@ class DplrBwdArgs(C.Structure):
         ("fwd", DplrArgs), ("d_o", C.c_void_p), ("d_final_state", C.c_void_p),
         ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p), ("da", C.c_void_p), ("db", C.c_void_p),
         ("dgk", C.c_void_p), ("d_initial_state", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
+    ]
+
+
+class LinrecArgs(C.Structure):
+    """Mirror of ``struct lnx_linrec_args``."""
+
+    _fields_ = [
+        ("B", C.c_int32), ("T", C.c_int32), ("D", C.c_int32), ("nseq", C.c_int32), ("dtype", C.c_int32), ("g_dtype", C.c_int32),
+        ("x_stride_b", C.c_int64), ("x_stride_t", C.c_int64), ("g_stride_b", C.c_int64), ("g_stride_t", C.c_int64),
+        ("d_y_stride_b", C.c_int64), ("d_y_stride_t", C.c_int64),
+        ("x", C.c_void_p), ("g", C.c_void_p), ("initial_state", C.c_void_p), ("cu_seqlens", C.c_void_p), ("y", C.c_void_p),
+        ("final_state", C.c_void_p), ("kept", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
+        ("d_y", C.c_void_p), ("d_final_state", C.c_void_p), ("d_x", C.c_void_p), ("d_g", C.c_void_p), ("d_initial_state", C.c_void_p),
     ]
 
 
@@ -140,6 +154,14 @@ def load() -> C.CDLL:
     lib.lnx_dplr_recurrent_bwd.argtypes = [C.POINTER(DplrBwdArgs), C.c_void_p]
     lib.lnx_dplr_recurrent_bwd_workspace_bytes.restype = C.c_uint64
     lib.lnx_dplr_recurrent_bwd_workspace_bytes.argtypes = [C.c_int32] * 5
+    for name in ("lnx_linrec_workspace_bytes", "lnx_linrec_kept_bytes"):
+        getattr(lib, name).restype = C.c_uint64
+        getattr(lib, name).argtypes = [C.POINTER(LinrecArgs)]
+    for name in ("lnx_linrec_fwd", "lnx_linrec_bwd"):
+        getattr(lib, name).restype = C.c_int
+        getattr(lib, name).argtypes = [C.POINTER(LinrecArgs), C.c_void_p]
+    lib.lnx_linrec_step.restype = C.c_int
+    lib.lnx_linrec_step.argtypes = [C.c_void_p] * 5 + [C.c_int64, C.c_int32, C.c_int32, C.c_void_p]
     lib.lnx_profile_enable.restype = C.c_int
     lib.lnx_profile_enable.argtypes = [C.c_int]
     lib.lnx_profile_read.restype = C.c_int

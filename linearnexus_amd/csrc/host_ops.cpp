@@ -11,6 +11,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
 #include <atomic>
@@ -1101,6 +1102,144 @@ PyObject* py_dplr_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   LNX_END
 }
 
+// ---------------------------------------------------------------------------------------------------------------
+// element-wise gated linear recurrence
+// ---------------------------------------------------------------------------------------------------------------
+
+// Tensors of one call lie on one GPU; a tensor that is absent is not asked.
+void check_devices(const char* op, const Tensor& first, std::initializer_list<std::pair<const char*, const Tensor*>> rest) {
+  for (const auto& [name, t] : rest)
+    TORCH_CHECK(!t->defined() || t->device() == first.device(), op, ": ", name, " is on ", t->defined() ? t->device().str() : "", ", expected ", first.device().str());
+}
+
+// What the kernels read in place: any strides over rows and tokens, channels next to each other
+Tensor channels_dense(const Tensor& x) { return x.size(-1) == 1 || x.stride(-1) == 1 ? x : x.contiguous(); }
+
+struct RecShape {
+  int64_t B, T, D, nseq, rows;
+};
+
+RecShape rec_shape(const char* op, const Tensor& x, const Tensor& g, const Tensor& s0, const Tensor& cu, int64_t dims) {
+  TORCH_CHECK(x.is_cuda(), op, ": x is on ", x.device().str(), "; the op runs on the GPU only");
+  TORCH_CHECK(known_dtype(x.scalar_type()), "unsupported dtype ", x.scalar_type(), ": use float32 or bfloat16");
+  TORCH_CHECK(x.dim() == dims && x.size(-1) > 0, op, ": x must be ", dims == 3 ? "[batch, seq, channels]" : "[batch, channels]", ", got ", shape_text(x));
+  TORCH_CHECK(g.sizes() == x.sizes(), op, ": g ", shape_text(g), " must have x's shape ", shape_text(x));
+  TORCH_CHECK(g.is_floating_point(), op, ": g must be a floating-point tensor, got ", g.scalar_type());
+  check_devices(op, x, {{"g", &g}, {"state", &s0}, {"cu_seqlens", &cu}});
+  RecShape s{x.size(0), dims == 3 ? x.size(1) : 1, x.size(-1), 0, x.size(0)};
+  TORCH_CHECK(s.B <= INT32_MAX && s.T <= INT32_MAX && s.D <= INT32_MAX, op, ": x is too large, got ", shape_text(x));
+  if (cu.defined()) {
+    TORCH_CHECK(s.B == 1, "cu_seqlens needs a packed batch with B == 1");
+    s.rows = s.nseq = cu.numel() - 1;
+  }
+  TORCH_CHECK(!s0.defined() || (s0.sizes() == at::IntArrayRef({s.rows, s.D}) && s0.is_floating_point()), op, ": the state must be a floating-point (", s.rows, ", ", s.D,
+              ") tensor, got ", s0.defined() ? shape_text(s0) : "");
+  return s;
+}
+
+Tensor gate_type(const Tensor& g, at::ScalarType x) { return g.scalar_type() == x ? g : g.to(at::kFloat); }
+
+lnx_linrec_args rec_args(const RecShape& s, const Tensor& x, const Tensor& g, const Tensor& s0, const Tensor& cu) {
+  lnx_linrec_args a{};
+  a.B = (int32_t)s.B, a.T = (int32_t)s.T, a.D = (int32_t)s.D, a.nseq = (int32_t)s.nseq;
+  a.dtype = code_of(x.scalar_type()), a.g_dtype = code_of(g.scalar_type());
+  a.x_stride_b = x.stride(0), a.x_stride_t = x.stride(1), a.g_stride_b = g.stride(0), a.g_stride_t = g.stride(1);
+  a.x = ptr(x), a.g = ptr(g), a.initial_state = fptr(s0), a.cu_seqlens = static_cast<const int32_t*>(ptr(cu));
+  return a;
+}
+
+std::pair<Tensor, Tensor> rec_forward(const RecShape& s, const Tensor& x, const Tensor& g, const Tensor& s0, const Tensor& cu, Tensor* kept) {
+  lnx_linrec_args a = rec_args(s, x, g, s0, cu);
+  const auto fo = x.options().dtype(at::kFloat);
+  const Tensor y = at::empty({s.B, s.T, s.D}, x.options()), sT = at::empty({s.rows, s.D}, fo);
+  if (kept) *kept = at::empty({(int64_t)(lnx_linrec_kept_bytes(&a) / sizeof(float))}, fo);
+  a.workspace_bytes = lnx_linrec_workspace_bytes(&a);
+  Tensor ws;
+  if (a.workspace_bytes) ws = at::empty({(int64_t)a.workspace_bytes}, x.options().dtype(at::kByte));
+  a.workspace = ptr(ws), a.kept = kept ? fptr(*kept) : nullptr, a.y = ptr(y), a.final_state = fptr(sT);
+  const c10::DeviceGuard guard(x.device());
+  check_status(lnx_linrec_fwd(&a, stream_of(x)), "lnx_linrec_fwd");
+  return {y, sT};
+}
+
+struct RecFn : Function<RecFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x0, const Tensor& g0, const OptT& s0, const OptT& cu, const RecShape& s) {
+    const Tensor x = channels_dense(x0), g = channels_dense(gate_type(g0, x0.scalar_type())), si = f32(undef(s0));
+    Tensor kept;
+    auto [y, sT] = rec_forward(s, x, g, si, undef(cu), &kept);
+    ctx->save_for_backward({x, g, undef(cu), kept});
+    ctx->saved_data["i"] = std::vector<int64_t>{s.B, s.T, s.D, s.nseq, s.rows, (int64_t)g0.scalar_type(), s0.has_value() && s0->requires_grad(),
+                                                (int64_t)(s0.has_value() ? s0->scalar_type() : at::kFloat)};
+    ctx->set_materialize_grads(false);
+    return {y, sT};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_tangents("the gradient of gated_linear_recurrence", grads);
+    const variable_list sv = ctx->get_saved_variables();
+    const std::vector<int64_t> m = ctx->saved_data["i"].toIntVector();
+    const Tensor &x = sv[0], &g = sv[1], &cu = sv[2], &kept = sv[3];
+    const RecShape s{m[0], m[1], m[2], m[3], m[4]};
+    lnx_linrec_args a = rec_args(s, x, g, Tensor(), cu);
+    const Tensor dy = grads[0].defined() ? channels_dense(grads[0].to(x.scalar_type())) : Tensor(), ds = f32(grads[1]);
+    Tensor dx = at::empty({s.B, s.T, s.D}, x.options()), dg = at::empty({s.B, s.T, s.D}, g.options()), d0;
+    if (m[6]) d0 = at::empty({s.rows, s.D}, x.options().dtype(at::kFloat));
+    if (dy.defined()) a.d_y = ptr(dy), a.d_y_stride_b = dy.stride(0), a.d_y_stride_t = dy.stride(1);
+    a.workspace_bytes = lnx_linrec_workspace_bytes(&a);
+    Tensor ws;
+    if (a.workspace_bytes) ws = at::empty({(int64_t)a.workspace_bytes}, x.options().dtype(at::kByte));
+    a.workspace = ptr(ws), a.kept = fptr(kept), a.d_final_state = fptr(ds), a.d_x = ptr(dx), a.d_g = ptr(dg), a.d_initial_state = fptr(d0);
+    const c10::DeviceGuard guard(x.device());
+    check_status(lnx_linrec_bwd(&a, stream_of(x)), "lnx_linrec_bwd");
+    return {dx, dg.to((at::ScalarType)m[5]), d0.defined() ? d0.to((at::ScalarType)m[7]) : d0, Tensor(), Tensor()};
+  }
+};
+
+std::pair<Tensor, Tensor> rec_scan(const RecShape& s, const Tensor& x, const Tensor& g, const Tensor& s0, const Tensor& cu) {
+  if (wants_grad({&x, &g, &s0})) {
+    const variable_list r = RecFn::apply(x, g, opt(s0), opt(cu), s);
+    return {r[0], r[1]};
+  }
+  return rec_forward(s, channels_dense(x), channels_dense(gate_type(g, x.scalar_type())), f32(s0), cu, nullptr);
+}
+
+// linrec(x, g, initial_state, cu): (y, final state)
+PyObject* py_linrec(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  LNX_BEGIN
+  Args in(args, nargs, 4, "linrec");
+  const Tensor x = in.tensor(0, "x"), g = in.tensor(1, "g"), s0 = in.maybe(2, "initial_state"), cu = in.maybe(3, "cu_seqlens");
+  const RecShape s = rec_shape("gated_linear_recurrence", x, g, s0, cu, 3);
+  refuse_tangents("gated_linear_recurrence", {&x, &g, &s0});
+  const auto r = without_lock([&] { return rec_scan(s, x, g, s0, cu); });
+  return pack(r.first, r.second);
+  LNX_END
+}
+
+// linrec_step(x, g, state, inplace): (y, state)
+PyObject* py_linrec_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  LNX_BEGIN
+  Args in(args, nargs, 4, "linrec_step");
+  const Tensor x = in.tensor(0, "x"), g = in.tensor(1, "g"), state = in.tensor(2, "state");
+  const bool inplace = in.flag(3);
+  const RecShape s = rec_shape("gated_linear_recurrence_step", x, g, state, Tensor(), 2);
+  refuse_tangents("gated_linear_recurrence_step", {&x, &g, &state});
+  const bool grad = wants_grad({&x, &g, &state});
+  TORCH_CHECK(!grad || !inplace, "cannot differentiate through a step that updates its state in place");
+  TORCH_CHECK(!inplace || (state.scalar_type() == at::kFloat && state.is_contiguous()), "inplace=True needs a contiguous float32 state");
+  const auto r = without_lock([&]() -> std::pair<Tensor, Tensor> {
+    if (grad) {
+      const auto r = rec_scan(s, x.unsqueeze(1), g.unsqueeze(1), state, Tensor());
+      return {r.first.squeeze(1), r.second};
+    }
+    const Tensor xc = x.contiguous(), gc = gate_type(g, x.scalar_type()).contiguous(), si = f32(state), so = inplace ? state : at::empty_like(si), y = at::empty_like(xc);
+    const c10::DeviceGuard guard(x.device());
+    check_status(lnx_linrec_step(ptr(xc), ptr(gc), fptr(si), ptr(y), fptr(so), xc.numel(), code_of(xc.scalar_type()), code_of(gc.scalar_type()), stream_of(xc)),
+                 "lnx_linrec_step");
+    return {y, so};
+  });
+  return pack(r.first, r.second);
+  LNX_END
+}
+
 // set_kernel_error(class): the exception a failed C-ABI call raises
 PyObject* py_set_kernel_error(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (nargs != 1 || !PyExceptionClass_Check(args[0])) {
@@ -1114,7 +1253,7 @@ PyObject* py_set_kernel_error(PyObject*, PyObject* const* args, Py_ssize_t nargs
 
 #define LNX_FN(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {LNX_FN(step),     LNX_FN(recurrent), LNX_FN(l2norm), LNX_FN(l2norm_bwd), LNX_FN(chunk), LNX_FN(chunk_segmented),     LNX_FN(conv1d),           LNX_FN(rmsnorm_gated), LNX_FN(gdn_gate),
-                         LNX_FN(kda_gate), LNX_FN(dplr),      LNX_FN(dplr_step), LNX_FN(set_kernel_error), {nullptr, nullptr, 0, nullptr}};
+                         LNX_FN(kda_gate), LNX_FN(dplr),      LNX_FN(dplr_step), LNX_FN(linrec), LNX_FN(linrec_step), LNX_FN(set_kernel_error), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_host", "Host path of the linearnexus_amd ops.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
