@@ -432,6 +432,43 @@ int lnx_linrec_step(const void* x, const void* g, const float* state, void* y, f
                     int32_t g_dtype, void* hip_stream);
 
 /*
+ * The norms around a block on its residual stream, rows of d columns (d <= 8192):
+ *   u = RMSNorm(x) post_weight sigmoid(gate)    out = residual + scale u    z = RMSNorm(out) weight
+ * post_weight NULL: x itself in place of its norm; gate NULL: no gate; residual NULL: out = scale u; z NULL: no second norm;
+ * scale_vector [d] takes the place of `scale`.  x, gate, z and their gradients in `dtype`, residual, out and theirs in
+ * `r_dtype` (LNX_F32 or `dtype`), weights and their gradients fp32.  z is the norm of the unrounded sum.  The backward call
+ * reads the forward call's inputs; d_z and d_out may be NULL (zeros), d_residual, d_weight, d_post_weight and d_scale (the
+ * vector's) may be NULL (not wanted); the last three are summed without atomics through the workspace.
+ */
+typedef struct lnx_rmsnorm_residual_args {
+  int64_t rows;
+  int32_t d, dtype, r_dtype;
+  float scale, eps;
+  int32_t reserved;
+  const void* x;
+  const void* residual;
+  const void* gate;
+  const float* weight;
+  const float* post_weight;
+  const float* scale_vector;
+  void* z;
+  void* out;
+  const void* d_z;          /* backward only, from here */
+  const void* d_out;
+  void* d_x;
+  void* d_residual;
+  void* d_gate;
+  float* d_weight;
+  float* d_post_weight;
+  float* d_scale;
+  void* workspace;
+  uint64_t workspace_bytes;
+} lnx_rmsnorm_residual_args;
+uint64_t lnx_rmsnorm_residual_bwd_workspace_bytes(int64_t rows, int32_t d, int32_t dtype);
+int lnx_rmsnorm_residual_fwd(const lnx_rmsnorm_residual_args* a, void* hip_stream);
+int lnx_rmsnorm_residual_bwd(const lnx_rmsnorm_residual_args* a, void* hip_stream);
+
+/*
  * Optional per-kernel timing for benchmarks (no counterpart in the reference; its micro-benchmark
  * times whole jitted ops, bench_kda_kernels.py:216-249).  While enabled (process-wide),
  * every entry point records HIP events around each kernel it launches, on the caller's stream.

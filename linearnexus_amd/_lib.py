@@ -20,6 +20,7 @@ EXPORTS = (
     "lnx_conv1d_fwd", "lnx_conv1d_bwd", "lnx_conv1d_cache_bwd", "lnx_conv1d_packed_fwd", "lnx_conv1d_packed_bwd", "lnx_conv1d_fwd_zero", "lnx_conv1d_bwd_add", "lnx_dplr_recurrent_fwd", "lnx_dplr_step", "lnx_dplr_recurrent_bwd", "lnx_dplr_recurrent_bwd_workspace_bytes", "lnx_dplr_chunk_fits", "lnx_dplr_chunk_bytes", "lnx_dplr_chunk_fwd", "lnx_dplr_chunk_bwd", "lnx_rmsnorm_gated_fwd", "lnx_rmsnorm_gated_bwd", "lnx_rmsnorm_gated_bwd_workspace_bytes",
     "lnx_gdn_gate_fwd", "lnx_gdn_gate_bwd", "lnx_gdn_gate_bwd_workspace_bytes", "lnx_kda_gate_fwd", "lnx_kda_gate_bwd", "lnx_kda_gate_bwd_workspace_bytes", "lnx_sigmoid_fwd", "lnx_sigmoid_bwd",
     "lnx_linrec_workspace_bytes", "lnx_linrec_kept_bytes", "lnx_linrec_fwd", "lnx_linrec_bwd", "lnx_linrec_step",
+    "lnx_rmsnorm_residual_bwd_workspace_bytes", "lnx_rmsnorm_residual_fwd", "lnx_rmsnorm_residual_bwd",
     "lnx_profile_enable", "lnx_profile_read",
 )
 
@@ -76,6 +77,19 @@ class LinrecArgs(C.Structure):
         ("x", C.c_void_p), ("g", C.c_void_p), ("initial_state", C.c_void_p), ("cu_seqlens", C.c_void_p), ("y", C.c_void_p),
         ("final_state", C.c_void_p), ("kept", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
         ("d_y", C.c_void_p), ("d_final_state", C.c_void_p), ("d_x", C.c_void_p), ("d_g", C.c_void_p), ("d_initial_state", C.c_void_p),
+    ]
+
+
+class RmsnormResidualArgs(C.Structure):
+    """Mirror of ``struct lnx_rmsnorm_residual_args``."""
+
+    _fields_ = [
+        ("rows", C.c_int64), ("d", C.c_int32), ("dtype", C.c_int32), ("r_dtype", C.c_int32), ("scale", C.c_float), ("eps", C.c_float),
+        ("reserved", C.c_int32),
+        ("x", C.c_void_p), ("residual", C.c_void_p), ("gate", C.c_void_p), ("weight", C.c_void_p), ("post_weight", C.c_void_p),
+        ("scale_vector", C.c_void_p), ("z", C.c_void_p), ("out", C.c_void_p), ("d_z", C.c_void_p), ("d_out", C.c_void_p), ("d_x", C.c_void_p),
+        ("d_residual", C.c_void_p), ("d_gate", C.c_void_p), ("d_weight", C.c_void_p), ("d_post_weight", C.c_void_p), ("d_scale", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
     ]
 
 
@@ -162,6 +176,11 @@ def load() -> C.CDLL:
         getattr(lib, name).argtypes = [C.POINTER(LinrecArgs), C.c_void_p]
     lib.lnx_linrec_step.restype = C.c_int
     lib.lnx_linrec_step.argtypes = [C.c_void_p] * 5 + [C.c_int64, C.c_int32, C.c_int32, C.c_void_p]
+    lib.lnx_rmsnorm_residual_bwd_workspace_bytes.restype = C.c_uint64
+    lib.lnx_rmsnorm_residual_bwd_workspace_bytes.argtypes = [C.c_int64, C.c_int32, C.c_int32]
+    for name in ("lnx_rmsnorm_residual_fwd", "lnx_rmsnorm_residual_bwd"):
+        getattr(lib, name).restype = C.c_int
+        getattr(lib, name).argtypes = [C.POINTER(RmsnormResidualArgs), C.c_void_p]
     lib.lnx_profile_enable.restype = C.c_int
     lib.lnx_profile_enable.argtypes = [C.c_int]
     lib.lnx_profile_read.restype = C.c_int

@@ -84,10 +84,18 @@ void refuse_tangents(const char* op, const variable_list& ts) {
   for (const Tensor& t : ts) refuse_tangents(op, {&t});
 }
 
+Tensor work_area(const Tensor& like, uint64_t bytes) { return at::empty({(int64_t)std::max<uint64_t>(bytes, 1)}, like.options().dtype(at::kByte)); }
+
 std::string shape_text(const Tensor& t) {
   std::string s = "(";
   for (int64_t i = 0; i < t.dim(); ++i) s += (i ? ", " : "") + std::to_string(t.size(i));
   return s + (t.dim() == 1 ? ",)" : ")");
+}
+
+// Tensors of one call lie on one GPU; a tensor that is absent is not asked.
+void check_devices(const char* op, const Tensor& first, std::initializer_list<std::pair<const char*, const Tensor*>> rest) {
+  for (const auto& [name, t] : rest)
+    TORCH_CHECK(!t->defined() || t->device() == first.device(), op, ": ", name, " is on ", t->defined() ? t->device().str() : "", ", expected ", first.device().str());
 }
 
 // Memory layout of the token tensors.  The ops take the reference's head-first [B, H, T, .] shapes; a caller whose data
@@ -795,6 +803,110 @@ PyObject* py_rmsnorm_gated(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------
+// norms around a block on its residual stream
+// ---------------------------------------------------------------------------------------------------------------
+
+// Inputs as the kernels read them: dense rows, fp32 vectors
+struct Around {
+  Tensor x, residual, gate, weight, post, scale_v;
+  double scale, eps;
+};
+
+lnx_rmsnorm_residual_args around_args(const Around& n) {
+  lnx_rmsnorm_residual_args a{};
+  const int64_t d = n.x.size(-1);
+  a.rows = n.x.numel() / d, a.d = (int32_t)d;
+  a.dtype = code_of(n.x.scalar_type()), a.r_dtype = n.residual.defined() ? code_of(n.residual.scalar_type()) : a.dtype;
+  a.scale = (float)n.scale, a.eps = (float)n.eps;
+  a.x = ptr(n.x), a.residual = ptr(n.residual), a.gate = ptr(n.gate), a.weight = fptr(n.weight), a.post_weight = fptr(n.post), a.scale_vector = fptr(n.scale_v);
+  return a;
+}
+
+std::pair<Tensor, Tensor> around_forward(const Around& n) {
+  const Tensor out = n.residual.defined() ? at::empty_like(n.residual) : at::empty_like(n.x), z = n.weight.defined() ? at::empty_like(n.x) : Tensor();
+  lnx_rmsnorm_residual_args a = around_args(n);
+  a.z = ptr(z), a.out = ptr(out);
+  const c10::DeviceGuard guard(n.x.device());
+  check_status(lnx_rmsnorm_residual_fwd(&a, stream_of(n.x)), "lnx_rmsnorm_residual_fwd");
+  return {z, out};
+}
+
+struct AroundFn : Function<AroundFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x0, const OptT& residual0, const OptT& weight0, const OptT& post0, const OptT& gate0, const OptT& scale0,
+                               double scale, double eps) {
+    auto dense = [&](const OptT& t, at::ScalarType type) { return t.has_value() ? t->to(type).contiguous() : Tensor(); };
+    const auto dt = x0.scalar_type();
+    const Around n{x0.contiguous(), residual0.has_value() ? residual0->contiguous() : Tensor(), dense(gate0, dt), dense(weight0, at::kFloat), dense(post0, at::kFloat),
+                   dense(scale0, at::kFloat), scale, eps};
+    auto [z, out] = around_forward(n);
+    ctx->save_for_backward({n.x, n.residual, n.gate, n.weight, n.post, n.scale_v});
+    auto kind = [](const OptT& t) { return (int64_t)(t.has_value() ? t->scalar_type() : at::kFloat); };
+    auto wants = [](const OptT& t) { return (int64_t)(t.has_value() && t->requires_grad()); };
+    ctx->saved_data["i"] = std::vector<int64_t>{kind(gate0), kind(weight0), kind(post0), kind(scale0), wants(residual0), wants(weight0), wants(post0), wants(scale0)};
+    ctx->saved_data["d"] = std::vector<double>{scale, eps};
+    ctx->set_materialize_grads(false);
+    if (!z.defined()) return {out};
+    return {out, z};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_tangents("the gradient of rmsnorm_residual", grads);
+    const variable_list s = ctx->get_saved_variables();
+    const std::vector<int64_t> m = ctx->saved_data["i"].toIntVector();
+    const std::vector<double> sc = ctx->saved_data["d"].toDoubleVector();
+    const Around n{s[0], s[1], s[2], s[3], s[4], s[5], sc[0], sc[1]};
+    lnx_rmsnorm_residual_args a = around_args(n);
+    auto like = [](const Tensor& t, bool want) { return t.defined() && want ? at::empty_like(t) : Tensor(); };
+    const auto rt = n.residual.defined() ? n.residual.scalar_type() : n.x.scalar_type();
+    const Tensor d_out = grads[0].defined() ? grads[0].to(rt).contiguous() : Tensor();
+    const Tensor d_z = grads.size() > 1 && grads[1].defined() ? grads[1].to(n.x.scalar_type()).contiguous() : Tensor();
+    Tensor dx = at::empty_like(n.x), dr = like(n.residual, m[4]), dg = like(n.gate, true), dw = like(n.weight, m[5]), dp = like(n.post, m[6]), dsc = like(n.scale_v, m[7]), ws;
+    if (dw.defined() || dp.defined() || dsc.defined()) {
+      a.workspace_bytes = lnx_rmsnorm_residual_bwd_workspace_bytes(a.rows, a.d, a.dtype);
+      ws = work_area(n.x, a.workspace_bytes);
+      a.workspace = ptr(ws);
+    }
+    a.d_z = ptr(d_z), a.d_out = ptr(d_out), a.d_x = ptr(dx), a.d_residual = ptr(dr), a.d_gate = ptr(dg);
+    a.d_weight = fptr(dw), a.d_post_weight = fptr(dp), a.d_scale = fptr(dsc);
+    const c10::DeviceGuard guard(n.x.device());
+    check_status(lnx_rmsnorm_residual_bwd(&a, stream_of(n.x)), "lnx_rmsnorm_residual_bwd");
+    auto to = [](const Tensor& t, int64_t type) { return t.defined() ? t.to((at::ScalarType)type) : t; };
+    return {dx, dr, to(dw, m[1]), to(dp, m[2]), to(dg, m[0]), to(dsc, m[3]), Tensor(), Tensor()};
+  }
+};
+
+// rmsnorm_residual(x, residual, weight, post_weight, gate, scale: number or vector, eps): (z or None, new residual)
+PyObject* py_rmsnorm_residual(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  LNX_BEGIN
+  Args in(args, nargs, 7, "rmsnorm_residual");
+  const char* op = "rmsnorm_residual";
+  const Tensor x = in.tensor(0, "x"), residual = in.maybe(1, "residual"), weight = in.maybe(2, "weight"), post = in.maybe(3, "post_weight"), gate = in.maybe(4, "gate"),
+               scale_v = in.is_tensor(5) ? in.tensor(5, "scale") : Tensor();
+  const double scale = scale_v.defined() ? 1.0 : in.number(5), eps = in.number(6);
+  TORCH_CHECK(x.is_cuda(), op, ": x is on ", x.device().str(), "; the op runs on the GPU only");
+  TORCH_CHECK(known_dtype(x.scalar_type()), "unsupported dtype ", x.scalar_type(), ": use float32 or bfloat16");
+  TORCH_CHECK(x.dim() > 0 && x.size(-1) > 0, op, ": x must have rows, got ", shape_text(x));
+  for (const auto& [name, t] : {std::make_pair("residual", &residual), std::make_pair("gate", &gate)})
+    TORCH_CHECK(!t->defined() || t->sizes() == x.sizes(), op, ": ", name, " ", t->defined() ? shape_text(*t) : "", " must have x's shape ", shape_text(x));
+  for (const auto& [name, t] : {std::make_pair("weight", &weight), std::make_pair("post_weight", &post), std::make_pair("scale", &scale_v)})
+    TORCH_CHECK(!t->defined() || (t->dim() == 1 && t->size(0) == x.size(-1)), op, ": ", name, " must be [", x.size(-1), "], got ", t->defined() ? shape_text(*t) : "");
+  TORCH_CHECK(!residual.defined() || residual.scalar_type() == at::kFloat || residual.scalar_type() == x.scalar_type(), op, ": the residual must be float32 or ",
+              x.scalar_type(), ", got ", residual.defined() ? residual.scalar_type() : at::kFloat);
+  for (const Tensor* t : {&gate, &weight, &post, &scale_v}) TORCH_CHECK(!t->defined() || t->is_floating_point(), op, ": gate, weights and scale must be floating-point tensors");
+  check_devices(op, x, {{"residual", &residual}, {"weight", &weight}, {"post_weight", &post}, {"gate", &gate}, {"scale", &scale_v}});
+  refuse_tangents(op, {&x, &residual, &weight, &post, &gate, &scale_v});
+  const auto r = without_lock([&]() -> std::pair<Tensor, Tensor> {
+    if (wants_grad({&x, &residual, &weight, &post, &gate, &scale_v})) {
+      const variable_list r = AroundFn::apply(x, opt(residual), opt(weight), opt(post), opt(gate), opt(scale_v), scale, eps);
+      return {r.size() > 1 ? r[1] : Tensor(), r[0]};
+    }
+    return around_forward({x.contiguous(), residual.defined() ? residual.contiguous() : residual, gate.defined() ? gate.to(x.scalar_type()).contiguous() : gate, f32(weight),
+                           f32(post), f32(scale_v), scale, eps});
+  });
+  return pack(r.first, r.second);
+  LNX_END
+}
+
+// ---------------------------------------------------------------------------------------------------------------
 // gate activations
 // ---------------------------------------------------------------------------------------------------------------
 
@@ -977,8 +1089,6 @@ Tensor dplr_call(bool step, const Tensor& q, const Tensor& k, const Tensor& v, c
   return o;
 }
 
-Tensor work_area(const Tensor& like, uint64_t bytes) { return at::empty({(int64_t)std::max<uint64_t>(bytes, 1)}, like.options().dtype(at::kByte)); }
-
 // Whether the chunked kernels take a scan (lnx_dplr_chunk_fits, and tensors that start on 16-byte boundaries)
 bool dplr_chunked(std::initializer_list<const Tensor*> ts, const Tensor& v) {
   const Tensor& q = **ts.begin();
@@ -1105,12 +1215,6 @@ PyObject* py_dplr_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 // ---------------------------------------------------------------------------------------------------------------
 // element-wise gated linear recurrence
 // ---------------------------------------------------------------------------------------------------------------
-
-// Tensors of one call lie on one GPU; a tensor that is absent is not asked.
-void check_devices(const char* op, const Tensor& first, std::initializer_list<std::pair<const char*, const Tensor*>> rest) {
-  for (const auto& [name, t] : rest)
-    TORCH_CHECK(!t->defined() || t->device() == first.device(), op, ": ", name, " is on ", t->defined() ? t->device().str() : "", ", expected ", first.device().str());
-}
 
 // What the kernels read in place: any strides over rows and tokens, channels next to each other
 Tensor channels_dense(const Tensor& x) { return x.size(-1) == 1 || x.stride(-1) == 1 ? x : x.contiguous(); }
@@ -1253,7 +1357,7 @@ PyObject* py_set_kernel_error(PyObject*, PyObject* const* args, Py_ssize_t nargs
 
 #define LNX_FN(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {LNX_FN(step),     LNX_FN(recurrent), LNX_FN(l2norm), LNX_FN(l2norm_bwd), LNX_FN(chunk), LNX_FN(chunk_segmented),     LNX_FN(conv1d),           LNX_FN(rmsnorm_gated), LNX_FN(gdn_gate),
-                         LNX_FN(kda_gate), LNX_FN(dplr),      LNX_FN(dplr_step), LNX_FN(linrec), LNX_FN(linrec_step), LNX_FN(set_kernel_error), {nullptr, nullptr, 0, nullptr}};
+                         LNX_FN(kda_gate), LNX_FN(dplr),      LNX_FN(dplr_step), LNX_FN(linrec), LNX_FN(linrec_step), LNX_FN(rmsnorm_residual), LNX_FN(set_kernel_error), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_host", "Host path of the linearnexus_amd ops.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
