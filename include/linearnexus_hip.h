@@ -469,6 +469,50 @@ int lnx_rmsnorm_residual_fwd(const lnx_rmsnorm_residual_args* a, void* hip_strea
 int lnx_rmsnorm_residual_bwd(const lnx_rmsnorm_residual_args* a, void* hip_stream);
 
 /*
+ * Causal softmax attention over whole prompts with grouped heads, and its gradient: query i of a sequence attends to its keys
+ * 0 .. i; query head h reads key head h / (H / Hkv).  q, o, d_o, d_q are [B, H, T, d], k, v, d_k, d_v [B, Hkv, T, d] in `dtype`,
+ * each with its own strides (in elements, rows contiguous, every stride and pointer a multiple of 16 bytes; an input's stride
+ * may be 0).  d <= 128 and a multiple of 8.  Packed batches as above.  lse [B, H, T] fp32 is written by the forward call if not
+ * NULL and read by the backward call, which also reads o; it holds nothing else between the calls.
+ */
+typedef struct lnx_tensor4 {
+  void* p;
+  int64_t stride_b, stride_h, stride_t;
+} lnx_tensor4;
+typedef struct lnx_attn_args {
+  int32_t B, H, Hkv, T, d, nseq, dtype;
+  float scale;
+  lnx_tensor4 q, k, v, o;
+  lnx_tensor4 d_o, d_q, d_k, d_v;  /* backward only */
+  float* lse;
+  const int32_t* cu_seqlens;
+  void* workspace;                 /* backward only */
+  uint64_t workspace_bytes;
+} lnx_attn_args;
+uint64_t lnx_attn_bwd_workspace_bytes(const lnx_attn_args* a);
+int lnx_attn_fwd(const lnx_attn_args* a, void* hip_stream);
+int lnx_attn_bwd(const lnx_attn_args* a, void* hip_stream);
+
+/*
+ * One token of the same attention against a cache: for sequence b the token's key and value are written to place lengths[b] of
+ * k_cache, v_cache [B, Hkv, S, d], and its queries attend to places 0 .. lengths[b].  q [B, H, d], k, v [B, Hkv, d] (stride_t
+ * unused), caches with their own strides, o [B, H, d] dense; lengths [B] int32 on the device, left as it is.  Places behind the
+ * token are not read.  A length outside 0 .. S - 1 writes nothing and gives NaN.  The workspace holds nothing between calls.
+ */
+typedef struct lnx_attn_step_args {
+  int32_t B, H, Hkv, S, d, dtype;
+  float scale;
+  int32_t reserved;
+  lnx_tensor4 q, k, v, k_cache, v_cache;
+  void* o;
+  const int32_t* lengths;
+  void* workspace;
+  uint64_t workspace_bytes;
+} lnx_attn_step_args;
+uint64_t lnx_attn_step_workspace_bytes(const lnx_attn_step_args* a);
+int lnx_attn_step(const lnx_attn_step_args* a, void* hip_stream);
+
+/*
  * Optional per-kernel timing for benchmarks (no counterpart in the reference; its micro-benchmark
  * times whole jitted ops, bench_kda_kernels.py:216-249).  While enabled (process-wide),
  * every entry point records HIP events around each kernel it launches, on the caller's stream.

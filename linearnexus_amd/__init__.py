@@ -1,4 +1,5 @@
 """MI355X-native delta-rule scan (DeltaNet / Gated DeltaNet / KDA) behind the reference's op names."""
+from .attention import causal_attention, causal_attention_step
 from .backend import KernelBackend, select_kernel_backend
 from .conv import depthwise_conv1d_causal
 from .gate import gated_deltanet_gate, kda_gate
@@ -30,4 +31,5 @@ __all__ = [
     "kda_recurrent", "kda_chunkwise", "kda_chunkwise_raw_gate", "kda_step", "l2norm_rows", "depthwise_conv1d_causal",
     "dplr_delta_rule_recurrent", "dplr_delta_rule_step", "rmsnorm_gated", "kda_gate", "gated_deltanet_gate",
     "gated_linear_recurrence", "gated_linear_recurrence_step", "rmsnorm_residual",
+    "causal_attention", "causal_attention_step",
 ]

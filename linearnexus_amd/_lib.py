@@ -21,6 +21,7 @@ EXPORTS = (
     "lnx_gdn_gate_fwd", "lnx_gdn_gate_bwd", "lnx_gdn_gate_bwd_workspace_bytes", "lnx_kda_gate_fwd", "lnx_kda_gate_bwd", "lnx_kda_gate_bwd_workspace_bytes", "lnx_sigmoid_fwd", "lnx_sigmoid_bwd",
     "lnx_linrec_workspace_bytes", "lnx_linrec_kept_bytes", "lnx_linrec_fwd", "lnx_linrec_bwd", "lnx_linrec_step",
     "lnx_rmsnorm_residual_bwd_workspace_bytes", "lnx_rmsnorm_residual_fwd", "lnx_rmsnorm_residual_bwd",
+    "lnx_attn_bwd_workspace_bytes", "lnx_attn_fwd", "lnx_attn_bwd", "lnx_attn_step_workspace_bytes", "lnx_attn_step",
     "lnx_profile_enable", "lnx_profile_read",
 )
 
@@ -90,6 +91,34 @@ class RmsnormResidualArgs(C.Structure):
         ("scale_vector", C.c_void_p), ("z", C.c_void_p), ("out", C.c_void_p), ("d_z", C.c_void_p), ("d_out", C.c_void_p), ("d_x", C.c_void_p),
         ("d_residual", C.c_void_p), ("d_gate", C.c_void_p), ("d_weight", C.c_void_p), ("d_post_weight", C.c_void_p), ("d_scale", C.c_void_p),
         ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
+    ]
+
+
+class Tensor4(C.Structure):
+    """Mirror of ``struct lnx_tensor4``."""
+
+    _fields_ = [("p", C.c_void_p), ("stride_b", C.c_int64), ("stride_h", C.c_int64), ("stride_t", C.c_int64)]
+
+
+class AttnArgs(C.Structure):
+    """Mirror of ``struct lnx_attn_args``."""
+
+    _fields_ = [
+        ("B", C.c_int32), ("H", C.c_int32), ("Hkv", C.c_int32), ("T", C.c_int32), ("d", C.c_int32), ("nseq", C.c_int32), ("dtype", C.c_int32),
+        ("scale", C.c_float),
+        ("q", Tensor4), ("k", Tensor4), ("v", Tensor4), ("o", Tensor4), ("d_o", Tensor4), ("d_q", Tensor4), ("d_k", Tensor4), ("d_v", Tensor4),
+        ("lse", C.c_void_p), ("cu_seqlens", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
+    ]
+
+
+class AttnStepArgs(C.Structure):
+    """Mirror of ``struct lnx_attn_step_args``."""
+
+    _fields_ = [
+        ("B", C.c_int32), ("H", C.c_int32), ("Hkv", C.c_int32), ("S", C.c_int32), ("d", C.c_int32), ("dtype", C.c_int32),
+        ("scale", C.c_float), ("reserved", C.c_int32),
+        ("q", Tensor4), ("k", Tensor4), ("v", Tensor4), ("k_cache", Tensor4), ("v_cache", Tensor4),
+        ("o", C.c_void_p), ("lengths", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
     ]
 
 
@@ -181,6 +210,15 @@ def load() -> C.CDLL:
     for name in ("lnx_rmsnorm_residual_fwd", "lnx_rmsnorm_residual_bwd"):
         getattr(lib, name).restype = C.c_int
         getattr(lib, name).argtypes = [C.POINTER(RmsnormResidualArgs), C.c_void_p]
+    lib.lnx_attn_bwd_workspace_bytes.restype = C.c_uint64
+    lib.lnx_attn_bwd_workspace_bytes.argtypes = [C.POINTER(AttnArgs)]
+    for name in ("lnx_attn_fwd", "lnx_attn_bwd"):
+        getattr(lib, name).restype = C.c_int
+        getattr(lib, name).argtypes = [C.POINTER(AttnArgs), C.c_void_p]
+    lib.lnx_attn_step_workspace_bytes.restype = C.c_uint64
+    lib.lnx_attn_step_workspace_bytes.argtypes = [C.POINTER(AttnStepArgs)]
+    lib.lnx_attn_step.restype = C.c_int
+    lib.lnx_attn_step.argtypes = [C.POINTER(AttnStepArgs), C.c_void_p]
     lib.lnx_profile_enable.restype = C.c_int
     lib.lnx_profile_enable.argtypes = [C.c_int]
     lib.lnx_profile_read.restype = C.c_int

@@ -1,0 +1,950 @@
+// Causal softmax attention over whole prompts, grouped heads, dense or packed, forward and backward on the matrix cores:
+//   s_ij = scale q_i . k_j   p_ij = exp(s_ij - lse_i)  (j <= i)   o_i = sum_j p_ij v_j
+//   delta_i = o_i . do_i   ds_ij = p_ij (do_i . v_j - delta_i)   dq_i = scale sum_j ds_ij k_j   dk_j = scale sum_i ds_ij q_i   dv_j = sum_i p_ij do_i
+// One pass over the keys with running maximum and sum; no score ever leaves the registers.  Every product is laid out so that its
+// result fragment is the next product's operand as it is: a wave owns 32 columns -- queries in the forward and the dq kernel, keys in
+// the dk / dv kernel -- whose vectors stay in registers as B operands, and the rows that it walks over lie in LDS, read by rows for
+// the products over the head dimension and through transposing reads for the products over the rows.  A score fragment holds one
+// column per lane and half, so maxima and sums are within the lane and one exchange of the wave's halves.
+// Tiles of 64 rows come in through loads that go straight to LDS, the next tile behind the one being multiplied, one barrier a tile.
+// bf16 takes v_mfma_f32_32x32x16_bf16 (probabilities and score gradients are rounded to bf16 as operands: 2^-9 of each term, what the
+// outputs are rounded to), fp32 takes v_mfma_f32_32x32x2_f32 throughout.  Sums, maxima and accumulators are fp32.
+// No atomics: dk and dv are summed over the group's query heads by the workgroup that owns the keys, dq by a kernel of its own.
+#include "lnx_common.h"
+#include "mma_tiles.h"
+
+namespace {
+
+constexpr int ROWS = 64;  // rows of a tile
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct Args {
+  const void *q, *k, *v, *dout;
+  void *o, *dq, *dk, *dv;
+  float *lse, *delta;  // [B, H, T]; lse in units of log 2
+  const int32_t* cu;
+  int64_t qs[3], ks[3], vs[3], os[3], gs[3], dqs[3], dks[3], dvs[3];  // strides of batch, head, token in elements
+  int B, H, Hkv, G, T, d, nseq, nblk;
+  float scale;
+};
+
+// Eight contraction slots of an operand
+template <typename T> struct Frag8;
+template <> struct Frag8<bf16_t> {
+  bf16x8 v;
+  __device__ __forceinline__ void zero() { v = vec_zero<bf16_t>(); }
+  __device__ __forceinline__ bf16_t get(int j) const { return v[j]; }
+};
+template <> struct Frag8<float> {
+  float v[8];
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+  }
+};
+__device__ __forceinline__ void mma(floatx16& c, const Frag8<bf16_t>& a, const Frag8<bf16_t>& b) { c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, b.v, c, 0, 0, 0); }
+__device__ __forceinline__ void mma(floatx16& c, const Frag8<float>& a, const Frag8<float>& b) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[e], b.v[e], c, 0, 0, 0);
+}
+// Elements 8 h .. 8 h + 7 of a result fragment as an operand in chain order (rows 16 h + 4 kg + 0 .. 3 and + 8 .. 11)
+__device__ __forceinline__ void from_acc(Frag8<bf16_t>& f, const floatx16& c, int h) { f.v = Mma<bf16_t>::from_acc(c, h); }
+__device__ __forceinline__ void from_acc(Frag8<float>& f, const floatx16& c, int h) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f.v[e] = c[8 * h + e];
+}
+// Eight consecutive elements from memory; `ok`: they exist
+template <typename T> __device__ __forceinline__ void from_global(Frag8<T>& f, const T* p, bool ok);
+template <> __device__ __forceinline__ void from_global<bf16_t>(Frag8<bf16_t>& f, const bf16_t* p, bool ok) {
+  f.zero();
+  if (ok) f.v = *reinterpret_cast<const bf16x8*>(p);
+}
+template <> __device__ __forceinline__ void from_global<float>(Frag8<float>& f, const float* p, bool ok) {
+  f.zero();
+  if (ok) {
+    const floatx4 a = load4(p), b = load4(p + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f.v[e] = a[e], f.v[e + 4] = b[e];
+  }
+}
+
+// A [R][D] tile in LDS, 16-byte granules of a row permuted by the row so that row reads and reads along the rows spread over the banks
+template <typename T, int D, int R = ROWS> struct Tile;
+template <int D, int R> struct Tile<bf16_t, D, R> {
+  typedef SwzTile<R, D> S;
+  static constexpr int BYTES = R * D * 2;
+  static __device__ __forceinline__ void src(int j, int lane, int& r, int& c) { S::src(j, lane, r, c); }
+  static __device__ __forceinline__ Frag8<bf16_t> by_row(const bf16_t* t, int r0, int k0, int lane) { return {S::load(t, r0 + (lane & 31), k0 + 8 * (lane >> 5))}; }
+  static __device__ __forceinline__ Frag8<bf16_t> by_col(const bf16_t* t, int k0, int c0, int lane) {
+    typedef short short8_ __attribute__((ext_vector_type(8)));
+    const int grp = lane >> 4;
+    const auto lo = S::tr4(t, k0 + 4 * (grp >> 1), c0 + 16 * (grp & 1), lane), hi = S::tr4(t, k0 + 8 + 4 * (grp >> 1), c0 + 16 * (grp & 1), lane);
+    const short8_ v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    return {__builtin_bit_cast(bf16x8, v)};
+  }
+  static __device__ __forceinline__ bool finite(const bf16_t* t, int j, int lane) {  // of the granule that instruction j's lane brought
+    typedef unsigned uint4_ __attribute__((ext_vector_type(4)));
+    const uint4_ x = *reinterpret_cast<const uint4_*>(t + (64 * j + lane) * 8);
+    bool ok = true;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ok = ok && (x[e] & 0x7f80u) != 0x7f80u && (x[e] & 0x7f800000u) != 0x7f800000u;
+    return ok;
+  }
+};
+template <int D, int R> struct Tile<float, D, R> {
+  static constexpr int BYTES = R * D * 4, G = D / 4;
+  static __device__ __forceinline__ int at(int r, int c) { return r * D + ((((c >> 2) ^ (r & 7)) << 2) | (c & 3)); }
+  static __device__ __forceinline__ void src(int j, int lane, int& r, int& c) {
+    const int p = 64 * j + lane;
+    r = p / G;
+    c = ((p % G) ^ (r & 7)) << 2;
+  }
+  static __device__ __forceinline__ Frag8<float> by_row(const float* t, int r0, int k0, int lane) {
+    const int r = r0 + (lane & 31), c = k0 + 8 * (lane >> 5);
+    const floatx4 a = load4(t + at(r, c)), b = load4(t + at(r, c + 4));
+    return {{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}};
+  }
+  static __device__ __forceinline__ Frag8<float> by_col(const float* t, int k0, int c0, int lane) {
+    Frag8<float> f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f.v[e] = t[at(k0 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3), c0 + (lane & 31))];
+    return f;
+  }
+  static __device__ __forceinline__ bool finite(const float* t, int j, int lane) {
+    const floatx4 x = load4(t + (64 * j + lane) * 4);
+    bool ok = true;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ok = ok && (__float_as_uint(x[e]) & 0x7f800000u) != 0x7f800000u;
+    return ok;
+  }
+};
+
+// Rows row0 .. row0 + 63 of a [len][d] matrix with row stride `st`, by the workgroup's four waves; rows behind the last are copies of
+// the last, columns behind d keep the zeros that clear_tiles left.
+template <typename T, int D> __device__ __forceinline__ void fetch_tile(T* tile, const T* base, int64_t st, int row0, int len, int d, int wave, int lane) {
+  typedef Tile<T, D> TL;
+  constexpr int N = TL::BYTES / 1024 / 4;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int j = wave * N + i;
+    int r, c;
+    TL::src(j, lane, r, c);
+    if (c < d) dma16(base + (int64_t)min(row0 + r, len - 1) * st + c, lds_byte_addr(tile) + 1024 * j);
+  }
+}
+template <typename T, int D> __device__ __forceinline__ bool tile_finite(const T* tile, int wave, int lane) {
+  constexpr int N = Tile<T, D>::BYTES / 1024 / 4;
+  bool ok = true;
+#pragma unroll
+  for (int i = 0; i < N; ++i) ok = ok && Tile<T, D>::finite(tile, wave * N + i, lane);
+  return ok;
+}
+__device__ __forceinline__ void clear_lds(char* p, int bytes) {
+  for (int i = threadIdx.x * 16; i < bytes; i += 256 * 16) *reinterpret_cast<floatx4*>(p + i) = floatx4{0.f, 0.f, 0.f, 0.f};
+}
+
+// max over the wave's two halves
+__device__ __forceinline__ float half_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// acc += (rows of a tile, turned) . B one row at a time, leaving out the (row, column) pairs that are masked: what the products over
+// the rows do when the tile holds values that are not finite, because 0 times those is not 0.  keep(row of the tile): this lane's column takes it.
+template <typename T, int D, typename F> __device__ __forceinline__ void add_rows_singly(floatx16 (&acc)[D / 32], const T* tile, int r0, const Frag8<T> (&b)[2], int lane, F keep) {
+#pragma unroll 1
+  for (int h = 0; h < 2; ++h)
+#pragma unroll 1
+    for (int e = 0; e < 16; ++e) {
+      const int row = r0 + 16 * h + e, slot = (e & 3) + 4 * (e >> 3), kg = (e >> 2) & 1;
+#pragma unroll
+      for (int m = 0; m < D / 32; ++m) {
+        Frag8<T> a = Tile<T, D>::by_col(tile, r0 + 16 * h, 32 * m, lane);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (j != slot || (lane >> 5) != kg) a.v[j] = from_f32<T>(0.f);
+        floatx16 t;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) t[i] = 0.f;
+        mma(t, a, h ? b[1] : b[0]);
+        const bool on = keep(row);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[m][i] += on ? t[i] : 0.f;
+      }
+    }
+}
+
+// Where a workgroup works: sequence (its first token, its length), block of `size` rows, heads
+struct Place {
+  int b, hkv, g, len, blk;
+  int64_t tok;
+  bool on;
+};
+// `per_group`: workgroups per (batch, key head, block) -- the query heads of a group, or one.  Heavy blocks first: of causal queries
+// the last ones (`last_first`), of keys the first ones.  Where the groups divide among the eight XCDs, workgroups of one group stay on
+// one, whose L2 then holds the group's keys and values.
+__device__ __forceinline__ Place place(const Args& a, int size, int per_group, bool last_first) {
+  Place p;
+  int w = blockIdx.x, group, blk;
+  const int groups = a.B * a.Hkv, per = a.nblk * per_group;
+  if (groups % 8 == 0) {
+    const int slot = w >> 3;
+    group = (w & 7) + 8 * (slot / per);
+    blk = slot % per / per_group;
+    p.g = slot % per_group;
+  } else {
+    blk = w / (groups * per_group);
+    w -= blk * groups * per_group;
+    group = w / per_group;
+    p.g = w % per_group;
+  }
+  p.b = group / a.Hkv;
+  p.hkv = group % a.Hkv;
+  p.tok = 0;
+  p.len = a.T;
+  p.on = true;
+  if (!a.nseq) {
+    p.blk = last_first ? a.nblk - 1 - blk : blk;
+    return p;
+  }
+  // packed: the sequence that holds block `blk` of all sequences' blocks, one lane per sequence
+  const int lane = threadIdx.x & 63;
+  p.on = false;
+  for (int s0 = 0, before = 0; s0 < a.nseq; s0 += 64) {
+    const int s = s0 + lane;
+    const int first = s < a.nseq ? seq_first(a.cu, s, a.T) : 0, len = s < a.nseq ? seq_end(a.cu, s, a.T) - first : 0;
+    const int n = (len + size - 1) / size;
+    int upto = n;
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) {
+      const int o = __shfl_up(upto, k, LNX_WAVE);
+      if (lane >= k) upto += o;
+    }
+    const uint64_t hit = __ballot(blk < before + upto);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      const int nb = __builtin_amdgcn_readlane(n, l), end = before + __builtin_amdgcn_readlane(upto, l);
+      p.tok = __builtin_amdgcn_readlane(first, l);
+      p.len = __builtin_amdgcn_readlane(len, l);
+      p.blk = blk - (end - nb);
+      if (last_first) p.blk = nb - 1 - p.blk;
+      p.on = true;
+      break;
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+  return p;
+}
+template <typename T> __device__ __forceinline__ T* at(const void* p, const int64_t (&s)[3], int64_t b, int64_t h, int64_t t) {
+  return const_cast<T*>(static_cast<const T*>(p)) + b * s[0] + h * s[1] + t * s[2];
+}
+
+// One column's D values from accumulators over rows, times f: the lane writes four consecutive elements at a time
+template <typename T, int D> __device__ __forceinline__ void store_column(T* p, const floatx16 (&acc)[D / 32], float f, int d, int lane) {
+#pragma unroll
+  for (int m = 0; m < D / 32; ++m)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int c = 32 * m + 8 * q + 4 * (lane >> 5);
+      if (c < d) store4(p + c, floatx4{acc[m][4 * q] * f, acc[m][4 * q + 1] * f, acc[m][4 * q + 2] * f, acc[m][4 * q + 3] * f});
+    }
+}
+
+// A wave owns 32 NQ queries, the workgroup 128 NQ.
+template <typename T, int D, int NQ> __global__ __launch_bounds__(256, sizeof(T) == 2 && NQ == 1 ? 2 : 1) void attn_fwd_kernel(Args a) {
+  typedef Tile<T, D> TL;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const auto kt = [](int buf) { return reinterpret_cast<T*>(lds + 2 * buf * TL::BYTES); };
+  const auto vt = [](int buf) { return reinterpret_cast<T*>(lds + (2 * buf + 1) * TL::BYTES); };
+  int* odd = reinterpret_cast<int*>(lds + 4 * TL::BYTES);
+  const Place p = place(a, 128 * NQ, a.G, true);
+  if (!p.on) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, kg = lane >> 5;
+  const int h = p.hkv * a.G + p.g, q_wg = p.blk * 128 * NQ, q0 = q_wg + wave * 32 * NQ;
+  const T* kb = at<T>(a.k, a.ks, p.b, p.hkv, p.tok);
+  const T* vb = at<T>(a.v, a.vs, p.b, p.hkv, p.tok);
+  const int q_end = min(q_wg + 128 * NQ, p.len), ntile = (q_end + ROWS - 1) / ROWS;
+  if (a.d < D) clear_lds(lds, 4 * TL::BYTES);
+  if (threadIdx.x < 2) odd[threadIdx.x] = 0;
+  lds_barrier();
+  fetch_tile<T, D>(kt(0), kb, a.ks[2], 0, p.len, a.d, wave, lane);
+  fetch_tile<T, D>(vt(0), vb, a.vs[2], 0, p.len, a.d, wave, lane);
+  // queries as B operands; a negative scale turns their sign, so that the largest product has the largest score
+  const float c = fmaxf(fabsf(a.scale) * LOG2E, 1e-30f);  // above 0: -inf stays what a masked score is
+  Frag8<T> qf[NQ][D / 16];
+#pragma unroll
+  for (int t = 0; t < NQ; ++t) {
+    const int row = q0 + 32 * t + n;
+    const T* qr = at<T>(a.q, a.qs, p.b, h, p.tok) + (int64_t)min(row, p.len - 1) * a.qs[2];
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+      from_global<T>(qf[t][s], qr + 16 * s + 8 * kg, 16 * s + 8 * kg < a.d);
+      if (a.scale < 0.f)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) qf[t][s].v[e] = -qf[t][s].v[e];
+    }
+  }
+  floatx16 acc[NQ][D / 32];
+  float m[NQ], l[NQ];
+#pragma unroll
+  for (int t = 0; t < NQ; ++t) {
+    m[t] = -INFINITY;
+    l[t] = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[t][i][e] = 0.f;
+  }
+  for (int it = 0; it < ntile; ++it) {
+    const int key0 = it * ROWS, buf = it & 1;
+    dma_wait<0>();
+    const bool edge = key0 + ROWS > q_wg;  // some pairs of this tile are masked
+    if (edge && !tile_finite<T, D>(vt(buf), wave, lane)) odd[buf] = 1;
+    lds_barrier();
+    if (it + 1 < ntile) {
+      fetch_tile<T, D>(kt(buf ^ 1), kb, a.ks[2], key0 + ROWS, p.len, a.d, wave, lane);
+      fetch_tile<T, D>(vt(buf ^ 1), vb, a.vs[2], key0 + ROWS, p.len, a.d, wave, lane);
+    }
+    if (key0 >= q0 + 32 * NQ) continue;  // behind all of this wave's queries
+    floatx16 sc[NQ][2];
+#pragma unroll
+    for (int t = 0; t < NQ; ++t)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc[t][i][e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s) {
+        const Frag8<T> kf = TL::by_row(kt(buf), 32 * i, 16 * s, lane);
+#pragma unroll
+        for (int t = 0; t < NQ; ++t) mma(sc[t][i], kf, qf[t][s]);
+      }
+    Frag8<T> pf[NQ][4];
+#pragma unroll
+    for (int t = 0; t < NQ; ++t) {
+      const int q = q0 + 32 * t + n;
+      if (key0 + ROWS - 1 > q0 + 32 * t) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (key0 + 32 * i + frag_row(e, lane) > q) sc[t][i][e] = -INFINITY;
+      }
+      float top = sc[t][0][0];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, sc[t][i][e]);
+      top = half_max(top);
+      // a new reference only where the old one is short by more than 2^8: sums and accumulators stay far inside fp32's range
+      const float far = 8.f / c;
+      if (__any(top > m[t] + far || (m[t] == -INFINITY && top > m[t]))) {
+        const float next = fmaxf(m[t], top);
+        const float f = m[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[t] - next) * c);
+        l[t] *= f;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[t][i][e] *= f;
+        m[t] = next;
+      }
+      const float ref = m[t] == -INFINITY ? 0.f : m[t] * c;
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          sc[t][i][e] = __builtin_amdgcn_exp2f(sc[t][i][e] * c - ref);
+          sum += sc[t][i][e];
+        }
+      l[t] += sum;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) from_acc(pf[t][s], sc[t][s >> 1], s & 1);
+    }
+    if (edge && odd[buf]) {
+#pragma unroll
+      for (int t = 0; t < NQ; ++t) {
+        const int q = q0 + 32 * t + n;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const Frag8<T> two[2] = {pf[t][2 * i], pf[t][2 * i + 1]};
+          add_rows_singly<T, D>(acc[t], vt(buf), 32 * i, two, lane, [&](int row) { return key0 + row <= q; });
+        }
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          const Frag8<T> vf = TL::by_col(vt(buf), 16 * s, 32 * i, lane);
+#pragma unroll
+          for (int t = 0; t < NQ; ++t) mma(acc[t][i], vf, pf[t][s]);
+        }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < NQ; ++t) {
+    const int q = q0 + 32 * t + n;
+    const float sum = xor32_sum(l[t]);
+    if (q < p.len) {
+      store_column<T, D>(at<T>(a.o, a.os, p.b, h, p.tok + q), acc[t], 1.f / sum, a.d, lane);
+      if (a.lse && kg == 0) a.lse[((int64_t)p.b * a.H + h) * a.T + p.tok + q] = m[t] * c + __builtin_amdgcn_logf(sum);
+    }
+  }
+}
+
+// delta_i = o_i . do_i, sixteen lanes a row
+template <typename T> __global__ __launch_bounds__(256) void attn_delta_kernel(Args a) {
+  const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+  const int li = threadIdx.x & 15;
+  float s = 0.f;
+  if (row < (int64_t)a.B * a.H * a.T) {
+    const int64_t t = row % a.T, bh = row / a.T;
+    const T* o = at<T>(a.o, a.os, bh / a.H, bh % a.H, t) + 8 * li;
+    const T* g = at<T>(a.dout, a.gs, bh / a.H, bh % a.H, t) + 8 * li;
+    Frag8<T> x, y;
+    from_global<T>(x, o, 8 * li < a.d);
+    from_global<T>(y, g, 8 * li < a.d);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s += to_f32(x.v[e]) * to_f32(y.v[e]);
+  }
+  s = row16_sum(s);
+  if (li == 0 && row < (int64_t)a.B * a.H * a.T) a.delta[row] = s;
+}
+
+// Queries as in the forward pass, their gradients beside them in registers.
+template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(Args a) {
+  typedef Tile<T, D> TL;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const auto kt = [](int buf) { return reinterpret_cast<T*>(lds + 2 * buf * TL::BYTES); };
+  const auto vt = [](int buf) { return reinterpret_cast<T*>(lds + (2 * buf + 1) * TL::BYTES); };
+  int* odd = reinterpret_cast<int*>(lds + 4 * TL::BYTES);
+  const Place p = place(a, 128, a.G, true);
+  if (!p.on) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, kg = lane >> 5;
+  const int h = p.hkv * a.G + p.g, q_wg = p.blk * 128, q0 = q_wg + wave * 32, q = q0 + n;
+  const T* kb = at<T>(a.k, a.ks, p.b, p.hkv, p.tok);
+  const T* vb = at<T>(a.v, a.vs, p.b, p.hkv, p.tok);
+  const int q_end = min(q_wg + 128, p.len), ntile = (q_end + ROWS - 1) / ROWS;
+  if (a.d < D) clear_lds(lds, 4 * TL::BYTES);
+  if (threadIdx.x < 2) odd[threadIdx.x] = 0;
+  lds_barrier();
+  fetch_tile<T, D>(kt(0), kb, a.ks[2], 0, p.len, a.d, wave, lane);
+  fetch_tile<T, D>(vt(0), vb, a.vs[2], 0, p.len, a.d, wave, lane);
+  const float c = a.scale * LOG2E;
+  const int64_t row = min(q, p.len - 1), stat = ((int64_t)p.b * a.H + h) * a.T + p.tok + row;
+  const float lse = a.lse[stat], delta = a.delta[stat];
+  const T* qr = at<T>(a.q, a.qs, p.b, h, p.tok + row);
+  const T* gr = at<T>(a.dout, a.gs, p.b, h, p.tok + row);
+  Frag8<T> qf[D / 16], gf[D / 16];
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s) {
+    from_global<T>(qf[s], qr + 16 * s + 8 * kg, 16 * s + 8 * kg < a.d);
+    from_global<T>(gf[s], gr + 16 * s + 8 * kg, 16 * s + 8 * kg < a.d);
+  }
+  floatx16 acc[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
+  for (int it = 0; it < ntile; ++it) {
+    const int key0 = it * ROWS, buf = it & 1;
+    dma_wait<0>();
+    const bool edge = key0 + ROWS > q_wg;
+    if (edge && !tile_finite<T, D>(kt(buf), wave, lane)) odd[buf] = 1;
+    lds_barrier();
+    if (it + 1 < ntile) {
+      fetch_tile<T, D>(kt(buf ^ 1), kb, a.ks[2], key0 + ROWS, p.len, a.d, wave, lane);
+      fetch_tile<T, D>(vt(buf ^ 1), vb, a.vs[2], key0 + ROWS, p.len, a.d, wave, lane);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (key0 + 32 * i > q0 + 31) continue;  // behind all of this wave's queries
+      floatx16 sc, dp;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sc[e] = dp[e] = 0.f;
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s) {
+        mma(sc, TL::by_row(kt(buf), 32 * i, 16 * s, lane), qf[s]);
+        mma(dp, TL::by_row(vt(buf), 32 * i, 16 * s, lane), gf[s]);
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float pe = __builtin_amdgcn_exp2f(sc[e] * c - lse);
+        sc[e] = key0 + 32 * i + frag_row(e, lane) <= q ? pe * (dp[e] - delta) : 0.f;
+      }
+      Frag8<T> ds[2];
+      from_acc(ds[0], sc, 0);
+      from_acc(ds[1], sc, 1);
+      if (edge && odd[buf]) {
+        add_rows_singly<T, D>(acc, kt(buf), 32 * i, ds, lane, [&](int r) { return key0 + r <= q; });
+      } else {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int m = 0; m < D / 32; ++m) mma(acc[m], TL::by_col(kt(buf), 32 * i + 16 * s, 32 * m, lane), ds[s]);
+      }
+    }
+  }
+  if (q < p.len) store_column<T, D>(at<T>(a.dq, a.dqs, p.b, h, p.tok + q), acc, a.scale, a.d, lane);
+}
+
+// A workgroup owns 64 keys: two waves of 32 take the first half of a tile's queries, two the second; their sums meet at the end.
+template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dkv_kernel(Args a) {
+  typedef Tile<T, D> TL;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const auto qt = [](int buf) { return reinterpret_cast<T*>(lds + 2 * buf * TL::BYTES); };
+  const auto gt = [](int buf) { return reinterpret_cast<T*>(lds + (2 * buf + 1) * TL::BYTES); };
+  float* stats = reinterpret_cast<float*>(lds + 4 * TL::BYTES);  // [buffer][lse, delta][64]
+  int* odd = reinterpret_cast<int*>(stats + 256);
+  const Place p = place(a, ROWS, 1, false);
+  if (!p.on) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, kg = lane >> 5;
+  const int kw = wave & 1, r0 = 32 * (wave >> 1), key0 = p.blk * ROWS + 32 * kw, key = key0 + n;
+  const int ntile = (p.len + ROWS - 1) / ROWS, per = ntile - p.blk, total = per * a.G;
+  if (a.d < D) clear_lds(lds, 4 * TL::BYTES);
+  if (threadIdx.x < 2) odd[threadIdx.x] = 0;
+  lds_barrier();
+  auto fetch = [&](int it, int buf) {
+    const int h = p.hkv * a.G + it / per, row0 = (p.blk + it % per) * ROWS;
+    fetch_tile<T, D>(qt(buf), at<T>(a.q, a.qs, p.b, h, p.tok), a.qs[2], row0, p.len, a.d, wave, lane);
+    fetch_tile<T, D>(gt(buf), at<T>(a.dout, a.gs, p.b, h, p.tok), a.gs[2], row0, p.len, a.d, wave, lane);
+    const int64_t stat = ((int64_t)p.b * a.H + h) * a.T + p.tok + min(row0 + lane, p.len - 1);
+    if (wave == 0) dma4(a.lse + stat, lds_byte_addr(stats + buf * 128));
+    if (wave == 1) dma4(a.delta + stat, lds_byte_addr(stats + buf * 128 + 64));
+  };
+  fetch(0, 0);
+  const float c = a.scale * LOG2E;
+  const int64_t krow = p.tok + min(key, p.len - 1);
+  const T* kr = at<T>(a.k, a.ks, p.b, p.hkv, krow);
+  const T* vr = at<T>(a.v, a.vs, p.b, p.hkv, krow);
+  Frag8<T> kf[D / 16], vf[D / 16];
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s) {
+    from_global<T>(kf[s], kr + 16 * s + 8 * kg, 16 * s + 8 * kg < a.d);
+    from_global<T>(vf[s], vr + 16 * s + 8 * kg, 16 * s + 8 * kg < a.d);
+  }
+  floatx16 dk[D / 32], dv[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) dk[i][e] = dv[i][e] = 0.f;
+  for (int it = 0; it < total; ++it) {
+    const int buf = it & 1, row0 = (p.blk + it % per) * ROWS;
+    dma_wait<0>();
+    const bool edge = it % per == 0 || row0 + ROWS > p.len;
+    if (edge && !(tile_finite<T, D>(qt(buf), wave, lane) && tile_finite<T, D>(gt(buf), wave, lane))) odd[buf] = 1;
+    lds_barrier();
+    if (it + 1 < total) fetch(it + 1, buf ^ 1);
+    if (row0 + r0 + 31 < key0 || row0 + r0 >= p.len) continue;  // queries before all of this wave's keys, or none
+    const float* st = stats + buf * 128 + r0;
+    floatx16 sc, dp;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sc[e] = dp[e] = 0.f;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) mma(sc, TL::by_row(qt(buf), r0, 16 * s, lane), kf[s]);
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) mma(dp, TL::by_row(gt(buf), r0, 16 * s, lane), vf[s]);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const floatx4 lse = load4(st + 8 * g + 4 * kg), delta = load4(st + 64 + 8 * g + 4 * kg);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int q = row0 + r0 + 8 * g + 4 * kg + e;
+        const bool on = q >= key && q < p.len;
+        const float pe = on ? __builtin_amdgcn_exp2f(sc[4 * g + e] * c - lse[e]) : 0.f;
+        sc[4 * g + e] = pe;
+        dp[4 * g + e] = on ? pe * (dp[4 * g + e] - delta[e]) : 0.f;
+      }
+    }
+    Frag8<T> pf[2], ds[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) from_acc(pf[s], sc, s), from_acc(ds[s], dp, s);
+    if (edge && odd[buf]) {
+      const auto keep = [&](int r) { return row0 + r >= key && row0 + r < p.len; };
+      add_rows_singly<T, D>(dv, gt(buf), r0, pf, lane, keep);
+      add_rows_singly<T, D>(dk, qt(buf), r0, ds, lane, keep);
+    } else {
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int m = 0; m < D / 32; ++m) {
+          mma(dv[m], TL::by_col(gt(buf), r0 + 16 * s, 32 * m, lane), pf[s]);
+          mma(dk[m], TL::by_col(qt(buf), r0 + 16 * s, 32 * m, lane), ds[s]);
+        }
+    }
+  }
+  lds_barrier();
+  float* sums = reinterpret_cast<float*>(lds) + kw * (2 * D / 32) * 16 * 64;
+  if (wave >= 2) {
+#pragma unroll
+    for (int m = 0; m < D / 32; ++m)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        sums[((2 * m) * 16 + e) * 64 + lane] = dk[m][e];
+        sums[((2 * m + 1) * 16 + e) * 64 + lane] = dv[m][e];
+      }
+  }
+  lds_barrier();
+  if (wave >= 2 || key >= p.len) return;
+#pragma unroll
+  for (int m = 0; m < D / 32; ++m)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      dk[m][e] += sums[((2 * m) * 16 + e) * 64 + lane];
+      dv[m][e] += sums[((2 * m + 1) * 16 + e) * 64 + lane];
+    }
+  store_column<T, D>(at<T>(a.dk, a.dks, p.b, p.hkv, krow), dk, a.scale, a.d, lane);
+  store_column<T, D>(at<T>(a.dv, a.dvs, p.b, p.hkv, krow), dv, 1.f, a.d, lane);
+}
+
+int64_t blocks_of(const lnx_attn_args* a, int size) { return a->nseq ? (int64_t)a->T / size + a->nseq : ((int64_t)a->T + size - 1) / size; }
+
+bool rows_fit(const lnx_tensor4* t, int64_t size) {
+  return reinterpret_cast<uintptr_t>(t->p) % 16 == 0 && t->stride_b * size % 16 == 0 && t->stride_h * size % 16 == 0 && t->stride_t * size % 16 == 0;
+}
+
+int check(const char* what, const lnx_attn_args* a, bool bwd) {
+  if (!a) return lnx_set_error(LNX_ERR_NULL, "%s: args is NULL", what);
+  if (a->B < 0 || a->H <= 0 || a->Hkv <= 0 || a->H % a->Hkv || a->T < 0 || a->d <= 0 || a->d > 128 || a->d % 8 || a->nseq < 0 || (a->nseq && a->B != 1))
+    return lnx_set_error(LNX_ERR_SHAPE, "%s: unsupported dimensions B=%d H=%d Hkv=%d T=%d d=%d nseq=%d (d a multiple of 8, at most 128; H a multiple of Hkv)", what, a->B, a->H,
+                         a->Hkv, a->T, a->d, a->nseq);
+  if (a->dtype != LNX_F32 && a->dtype != LNX_BF16) return lnx_set_error(LNX_ERR_DTYPE, "%s: dtype %d", what, a->dtype);
+  if (a->nseq && !a->cu_seqlens) return lnx_set_error(LNX_ERR_NULL, "%s: nseq without cu_seqlens", what);
+  if (a->B == 0 || a->T == 0) return LNX_OK;
+  if (!(a->scale == a->scale) || a->scale - a->scale != 0.f) return lnx_set_error(LNX_ERR_SHAPE, "%s: scale must be finite", what);
+  const lnx_tensor4* ts[] = {&a->q, &a->k, &a->v, &a->o, &a->d_o, &a->d_q, &a->d_k, &a->d_v};
+  for (int i = 0; i < (bwd ? 8 : 4); ++i) {
+    if (!ts[i]->p) return lnx_set_error(LNX_ERR_NULL, "%s: a tensor is missing", what);
+    if (!rows_fit(ts[i], a->dtype == LNX_BF16 ? 2 : 4)) return lnx_set_error(LNX_ERR_SHAPE, "%s: tensors must be 16-byte aligned, rows whole numbers of 16 bytes apart", what);
+  }
+  if (bwd && (!a->lse || !a->workspace || a->workspace_bytes < lnx_attn_bwd_workspace_bytes(a)))
+    return lnx_set_error(LNX_ERR_WORKSPACE, "%s: lse and a workspace of %llu bytes are required", what, (unsigned long long)lnx_attn_bwd_workspace_bytes(a));
+  if ((int64_t)a->B * a->H * blocks_of(a, ROWS) > 0x7fffffff || (int64_t)a->B * a->H * a->T / 16 >= 0x7fffffff)
+    return lnx_set_error(LNX_ERR_SHAPE, "%s: too many rows", what);
+  return LNX_OK;
+}
+
+Args kernel_args(const lnx_attn_args* a) {
+  Args k{};
+  auto strides = [](int64_t (&s)[3], const lnx_tensor4& t) { s[0] = t.stride_b, s[1] = t.stride_h, s[2] = t.stride_t; };
+  k.q = a->q.p, k.k = a->k.p, k.v = a->v.p, k.dout = a->d_o.p, k.o = a->o.p, k.dq = a->d_q.p, k.dk = a->d_k.p, k.dv = a->d_v.p;
+  strides(k.qs, a->q), strides(k.ks, a->k), strides(k.vs, a->v), strides(k.os, a->o), strides(k.gs, a->d_o), strides(k.dqs, a->d_q), strides(k.dks, a->d_k), strides(k.dvs, a->d_v);
+  k.lse = a->lse, k.delta = static_cast<float*>(a->workspace), k.cu = a->cu_seqlens;
+  k.B = a->B, k.H = a->H, k.Hkv = a->Hkv, k.G = a->H / a->Hkv, k.T = a->T, k.d = a->d, k.nseq = a->nseq, k.scale = a->scale;
+  return k;
+}
+
+template <typename K> int start(K kernel, const char* name, const Args& a, int64_t grid, size_t bytes, hipStream_t st) {
+  if (int rc = lnx_lds_limit(reinterpret_cast<const void*>(kernel), bytes)) return rc;
+  lnx_profile_mark(name, st);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), bytes, st, a);
+  return LNX_OK;
+}
+
+template <typename T, int D> int launch_fwd(const lnx_attn_args* a, hipStream_t st) {
+  Args k = kernel_args(a);
+  constexpr int NQ = 1;
+  k.nblk = (int)blocks_of(a, 128 * NQ);
+  return start(attn_fwd_kernel<T, D, NQ>, "attn_fwd", k, (int64_t)k.B * k.H * k.nblk, 4 * Tile<T, D>::BYTES + 16, st);
+}
+
+template <typename T, int D> int launch_bwd(const lnx_attn_args* a, hipStream_t st) {
+  Args k = kernel_args(a);
+  lnx_profile_mark("attn_delta", st);
+  attn_delta_kernel<T><<<dim3((unsigned)(((int64_t)k.B * k.H * k.T + 15) / 16)), 256, 0, st>>>(k);
+  k.nblk = (int)blocks_of(a, ROWS);
+  if (int rc = start(attn_dkv_kernel<T, D>, "attn_dkv", k, (int64_t)k.B * k.Hkv * k.nblk, 4 * Tile<T, D>::BYTES + 1024 + 16, st)) return rc;
+  k.nblk = (int)blocks_of(a, 128);
+  return start(attn_dq_kernel<T, D>, "attn_dq", k, (int64_t)k.B * k.H * k.nblk, 4 * Tile<T, D>::BYTES + 16, st);
+}
+
+int run(const char* what, const lnx_attn_args* a, bool bwd, hipStream_t st) {
+  if (int rc = check(what, a, bwd)) return rc;
+  if (a->B == 0 || a->T == 0) return LNX_OK;
+  int rc;
+  if (a->dtype == LNX_BF16) {
+    if (a->d <= 64) rc = bwd ? launch_bwd<bf16_t, 64>(a, st) : launch_fwd<bf16_t, 64>(a, st);
+    else rc = bwd ? launch_bwd<bf16_t, 128>(a, st) : launch_fwd<bf16_t, 128>(a, st);
+  } else {
+    if (a->d <= 64) rc = bwd ? launch_bwd<float, 64>(a, st) : launch_fwd<float, 64>(a, st);
+    else rc = bwd ? launch_bwd<float, 128>(a, st) : launch_fwd<float, 128>(a, st);
+  }
+  if (rc) return rc;
+  lnx_profile_mark(nullptr, st);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? LNX_OK : lnx_set_error(LNX_ERR_LAUNCH, "%s: %s", what, hipGetErrorString(e));
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// one token against a cache
+// ---------------------------------------------------------------------------------------------------------------
+
+struct StepArgs {
+  const void *q, *k, *v;
+  void *kc, *vc, *o;
+  const int32_t* len;
+  int64_t qs[2], ks[2], vs[2], kcs[3], vcs[3];  // strides of batch, head (and place) in elements; o is dense
+  float* part;  // [B H][splits][D + 2]: sums relative to a maximum, the maximum, the sum of weights
+  int B, H, Hkv, G, S, d, splits, ctiles;
+  float scale;
+};
+
+constexpr int SROWS = 32;  // keys of a wave's tile
+template <typename T> constexpr int step_waves() { return sizeof(T) == 2 ? 4 : 2; }  // two tiles of keys and values each in LDS
+
+// The queries that share a key head are the 32 columns, every wave walks over tiles of 32 cached tokens of its own: no barrier until
+// the waves' sums meet.  Bound by the bytes of the cache (the matrix products take a sixteenth of the time): the next tile is in
+// flight while one is multiplied.  The new token's key and value come from the call and are written to the cache by the wave whose
+// tile holds the place; what lies behind it is never read.
+template <typename T, int D> __global__ __launch_bounds__(64 * step_waves<T>(), 1) void attn_step_kernel(StepArgs a) {
+  constexpr int W = step_waves<T>();
+  typedef Tile<T, D, SROWS> TL;
+  constexpr int NI = TL::BYTES / 1024;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, kg = lane >> 5;
+  int w = blockIdx.x;
+  const int split = w % a.splits;
+  w /= a.splits;
+  const int ct = w % a.ctiles;
+  w /= a.ctiles;
+  const int hkv = w % a.Hkv, b = w / a.Hkv, cols = min(32, a.G - 32 * ct), h = hkv * a.G + 32 * ct + n;
+  const int len = a.len[b];
+  const bool good = len >= 0 && len < a.S;
+  const int ntile = good ? len / SROWS + 1 : 0;
+  const T* kc = static_cast<const T*>(a.kc) + b * a.kcs[0] + hkv * a.kcs[1];
+  const T* vc = static_cast<const T*>(a.vc) + b * a.vcs[0] + hkv * a.vcs[1];
+  const T* kn = static_cast<const T*>(a.k) + b * a.ks[0] + hkv * a.ks[1];
+  const T* vn = static_cast<const T*>(a.v) + b * a.vs[0] + hkv * a.vs[1];
+  char* mine = lds + wave * 4 * TL::BYTES;
+  const auto kt = [&](int buf) { return reinterpret_cast<T*>(mine + 2 * buf * TL::BYTES); };
+  const auto vt = [&](int buf) { return reinterpret_cast<T*>(mine + (2 * buf + 1) * TL::BYTES); };
+  const auto clear = [&](void* p, int bytes) {
+    for (int i = lane * 16; i < bytes; i += 1024) *reinterpret_cast<floatx4*>(static_cast<char*>(p) + i) = floatx4{0.f, 0.f, 0.f, 0.f};
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  };
+  if (a.d < D) clear(mine, 4 * TL::BYTES);
+  const auto fetch = [&](int tile, int buf) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the reads of the tile that lay here
+    if (tile == ntile - 1) clear(vt(buf), TL::BYTES);  // rows behind the new token: no value at all
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      int r, c;
+      TL::src(j, lane, r, c);
+      r += tile * SROWS;
+      if (c < a.d && r <= len) {
+        dma16(r < len ? kc + (int64_t)r * a.kcs[2] + c : kn + c, lds_byte_addr(kt(buf)) + 1024 * j);
+        dma16(r < len ? vc + (int64_t)r * a.vcs[2] + c : vn + c, lds_byte_addr(vt(buf)) + 1024 * j);
+      }
+    }
+  };
+  const int step = a.splits * W;
+  int tile = split * W + wave;
+  if (tile < ntile) fetch(tile, 0);
+  const float c = fmaxf(fabsf(a.scale) * LOG2E, 1e-30f);
+  const T* qr = static_cast<const T*>(a.q) + b * a.qs[0] + (int64_t)(n < cols ? h : hkv * a.G) * a.qs[1];
+  Frag8<T> qf[D / 16];
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s) {
+    from_global<T>(qf[s], qr + 16 * s + 8 * kg, 16 * s + 8 * kg < a.d && n < cols);
+    if (a.scale < 0.f)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) qf[s].v[e] = -qf[s].v[e];
+  }
+  floatx16 acc[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
+  float m = -INFINITY, l = 0.f;
+  for (int buf = 0; tile < ntile; tile += step, buf ^= 1) {
+    if (tile + step < ntile) fetch(tile + step, buf ^ 1);
+    if (tile + step < ntile - 1) dma_wait<2 * NI>();
+    else dma_wait<0>();  // the last tile may be short of rows, and of loads
+    if (tile == ntile - 1 && ct == 0) {  // the new token's place
+      T* kw = const_cast<T*>(kc) + (int64_t)len * a.kcs[2];
+      T* vw = const_cast<T*>(vc) + (int64_t)len * a.vcs[2];
+      for (int i = lane; i < a.d; i += 64) kw[i] = kn[i], vw[i] = vn[i];
+    }
+    floatx16 sc;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sc[e] = 0.f;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) mma(sc, TL::by_row(kt(buf), 0, 16 * s, lane), qf[s]);
+    float top = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      if (tile * SROWS + frag_row(e, lane) > len) sc[e] = -INFINITY;
+      top = fmaxf(top, sc[e]);
+    }
+    top = half_max(top);
+    const float next = fmaxf(m, top), ref = next == -INFINITY ? 0.f : next * c;
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m * c - ref);
+    m = next;
+    l *= f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      sc[e] = __builtin_amdgcn_exp2f(sc[e] * c - ref);
+      l += sc[e];
+    }
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][e] *= f;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      Frag8<T> pf;
+      from_acc(pf, sc, s);
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) mma(acc[i], TL::by_col(vt(buf), 16 * s, 32 * i, lane), pf);
+    }
+  }
+  // the waves' sums, and this workgroup's share of the result
+  __syncthreads();
+  float* sums = reinterpret_cast<float*>(lds);            // [W][D / 32][16][64]
+  float* stat = sums + W * (D / 32) * 16 * 64;            // [W][2][32]
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sums[((wave * (D / 32) + i) * 16 + e) * 64 + lane] = acc[i][e];
+  l = xor32_sum(l);
+  if (kg == 0) stat[wave * 64 + n] = m, stat[wave * 64 + 32 + n] = l;
+  __syncthreads();
+  float top = stat[n], sum = 0.f, f[W];
+#pragma unroll
+  for (int i = 1; i < W; ++i) top = fmaxf(top, stat[i * 64 + n]);
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    const float mi = stat[i * 64 + n];
+    f[i] = mi == -INFINITY && top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((mi - top) * c);
+    sum += stat[i * 64 + 32 + n] * f[i];
+  }
+  if (n >= cols) return;
+  const int64_t row = (int64_t)b * a.H + h;
+  if (!good) sum = NAN;  // no place for the token: no result either
+  for (int i = wave; i < D / 32; i += W)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      floatx4 t;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        t[e] = 0.f;
+#pragma unroll
+        for (int j = 0; j < W; ++j) t[e] += sums[((j * (D / 32) + i) * 16 + 4 * g + e) * 64 + lane] * f[j];
+      }
+      const int col = 32 * i + 8 * g + 4 * kg;
+      if (a.splits == 1) {
+        if (col < a.d) store4(static_cast<T*>(a.o) + row * a.d + col, floatx4{t[0] / sum, t[1] / sum, t[2] / sum, t[3] / sum});
+      } else {
+        store4(a.part + (row * a.splits + split) * (D + 4) + col, t);
+      }
+    }
+  if (a.splits > 1 && wave == 0 && kg == 0) {
+    float* q = a.part + (row * a.splits + split) * (D + 4) + D;
+    q[0] = top * c;
+    q[1] = sum;
+  }
+}
+
+// One wave per head joins its splits
+template <typename T, int D> __global__ __launch_bounds__(64) void attn_step_join_kernel(const float* part, T* o, int splits, int d) {
+  const int64_t row = blockIdx.x;
+  const int lane = threadIdx.x;
+  const float* p = part + row * splits * (D + 4);
+  float top = -INFINITY;
+  for (int s = 0; s < splits; ++s) top = fmaxf(top, p[s * (D + 4) + D]);
+  float sum = 0.f, t[D / 64];
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i) t[i] = 0.f;
+  for (int s = 0; s < splits; ++s) {
+    const float* q = p + s * (D + 4);
+    const float f = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(q[D] - top);
+    sum += q[D + 1] * f;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) t[i] += q[64 * i + lane] * f;
+  }
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i)
+    if (64 * i + lane < d) o[row * d + 64 * i + lane] = from_f32<T>(t[i] / sum);
+}
+
+// Splits of a cache: workgroups for four to a CU, but two tiles a wave at least of a cache that is full
+int step_splits(const lnx_attn_step_args* a) {
+  const int waves = a->dtype == LNX_BF16 ? step_waves<bf16_t>() : step_waves<float>();
+  const int64_t wgs = (int64_t)a->B * a->Hkv * ((a->H / a->Hkv + 31) / 32), tiles = (a->S + SROWS - 1) / SROWS;
+  int64_t s = (1024 + wgs - 1) / wgs;
+  const int64_t most = (tiles + 2 * waves - 1) / (2 * waves);
+  if (s > most) s = most;
+  return (int)(s < 1 ? 1 : s);
+}
+
+int check_step(const lnx_attn_step_args* a) {
+  const char* what = "attn_step";
+  if (!a) return lnx_set_error(LNX_ERR_NULL, "%s: args is NULL", what);
+  if (a->B < 0 || a->H <= 0 || a->Hkv <= 0 || a->H % a->Hkv || a->S <= 0 || a->d <= 0 || a->d > 128 || a->d % 8)
+    return lnx_set_error(LNX_ERR_SHAPE, "%s: unsupported dimensions B=%d H=%d Hkv=%d S=%d d=%d (d a multiple of 8, at most 128; H a multiple of Hkv)", what, a->B, a->H, a->Hkv,
+                         a->S, a->d);
+  if (a->dtype != LNX_F32 && a->dtype != LNX_BF16) return lnx_set_error(LNX_ERR_DTYPE, "%s: dtype %d", what, a->dtype);
+  if (a->B == 0) return LNX_OK;
+  if (!(a->scale == a->scale) || a->scale - a->scale != 0.f) return lnx_set_error(LNX_ERR_SHAPE, "%s: scale must be finite", what);
+  const lnx_tensor4* ts[] = {&a->q, &a->k, &a->v, &a->k_cache, &a->v_cache};
+  for (const lnx_tensor4* t : ts) {
+    if (!t->p) return lnx_set_error(LNX_ERR_NULL, "%s: a tensor is missing", what);
+    if (!rows_fit(t, a->dtype == LNX_BF16 ? 2 : 4)) return lnx_set_error(LNX_ERR_SHAPE, "%s: tensors must be 16-byte aligned, rows whole numbers of 16 bytes apart", what);
+  }
+  if (!a->o || !a->lengths) return lnx_set_error(LNX_ERR_NULL, "%s: o and lengths are required", what);
+  if (reinterpret_cast<uintptr_t>(a->o) % 16) return lnx_set_error(LNX_ERR_SHAPE, "%s: tensors must be 16-byte aligned, rows whole numbers of 16 bytes apart", what);
+  if ((int64_t)a->B * a->H * step_splits(a) > 0x7fffffff) return lnx_set_error(LNX_ERR_SHAPE, "%s: too many rows", what);
+  const uint64_t need = lnx_attn_step_workspace_bytes(a);
+  if (need && (!a->workspace || a->workspace_bytes < need)) return lnx_set_error(LNX_ERR_WORKSPACE, "%s: needs a workspace of %llu bytes", what, (unsigned long long)need);
+  return LNX_OK;
+}
+
+template <typename T, int D> int launch_step(const lnx_attn_step_args* a, hipStream_t st) {
+  constexpr int W = step_waves<T>();
+  StepArgs k{};
+  k.q = a->q.p, k.k = a->k.p, k.v = a->v.p, k.kc = a->k_cache.p, k.vc = a->v_cache.p, k.o = a->o, k.len = a->lengths, k.part = static_cast<float*>(a->workspace);
+  k.qs[0] = a->q.stride_b, k.qs[1] = a->q.stride_h, k.ks[0] = a->k.stride_b, k.ks[1] = a->k.stride_h, k.vs[0] = a->v.stride_b, k.vs[1] = a->v.stride_h;
+  k.kcs[0] = a->k_cache.stride_b, k.kcs[1] = a->k_cache.stride_h, k.kcs[2] = a->k_cache.stride_t;
+  k.vcs[0] = a->v_cache.stride_b, k.vcs[1] = a->v_cache.stride_h, k.vcs[2] = a->v_cache.stride_t;
+  k.B = a->B, k.H = a->H, k.Hkv = a->Hkv, k.G = a->H / a->Hkv, k.S = a->S, k.d = a->d, k.scale = a->scale;
+  k.splits = step_splits(a), k.ctiles = (k.G + 31) / 32;
+  const size_t tiles = W * 4 * Tile<T, D, SROWS>::BYTES, sums = W * ((D / 32) * 16 * 64 + 64) * sizeof(float), bytes = tiles > sums ? tiles : sums;
+  const auto kernel = attn_step_kernel<T, D>;
+  if (int rc = lnx_lds_limit(reinterpret_cast<const void*>(kernel), bytes)) return rc;
+  lnx_profile_mark("attn_step", st);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)((int64_t)k.B * k.Hkv * k.ctiles * k.splits)), dim3(64 * W), bytes, st, k);
+  if (k.splits > 1) {
+    lnx_profile_mark("attn_step_join", st);
+    attn_step_join_kernel<T, D><<<dim3((unsigned)((int64_t)k.B * k.H)), 64, 0, st>>>(k.part, static_cast<T*>(a->o), k.splits, k.d);
+  }
+  return LNX_OK;
+}
+
+}  // namespace
+
+extern "C" uint64_t lnx_attn_step_workspace_bytes(const lnx_attn_step_args* a) {
+  if (!a || a->B <= 0 || a->H <= 0 || a->Hkv <= 0 || a->S <= 0) return 0;
+  const int s = step_splits(a);
+  return s > 1 ? (uint64_t)a->B * a->H * s * ((a->d <= 64 ? 64 : 128) + 4) * sizeof(float) : 0;
+}
+extern "C" int lnx_attn_step(const lnx_attn_step_args* a, void* hip_stream) {
+  if (int rc = check_step(a)) return rc;
+  if (a->B == 0) return LNX_OK;
+  hipStream_t st = static_cast<hipStream_t>(hip_stream);
+  int rc;
+  if (a->dtype == LNX_BF16) rc = a->d <= 64 ? launch_step<bf16_t, 64>(a, st) : launch_step<bf16_t, 128>(a, st);
+  else rc = a->d <= 64 ? launch_step<float, 64>(a, st) : launch_step<float, 128>(a, st);
+  if (rc) return rc;
+  lnx_profile_mark(nullptr, st);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? LNX_OK : lnx_set_error(LNX_ERR_LAUNCH, "attn_step: %s", hipGetErrorString(e));
+}
+
+extern "C" uint64_t lnx_attn_bwd_workspace_bytes(const lnx_attn_args* a) {
+  return a && a->B > 0 && a->H > 0 && a->T > 0 ? (uint64_t)a->B * a->H * a->T * sizeof(float) : 0;
+}
+extern "C" int lnx_attn_fwd(const lnx_attn_args* a, void* hip_stream) { return run("attn_fwd", a, false, static_cast<hipStream_t>(hip_stream)); }
+extern "C" int lnx_attn_bwd(const lnx_attn_args* a, void* hip_stream) { return run("attn_bwd", a, true, static_cast<hipStream_t>(hip_stream)); }

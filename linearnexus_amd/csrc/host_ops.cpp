@@ -15,6 +15,7 @@
 #include <c10/hip/HIPStream.h>
 
 #include <atomic>
+#include <cmath>
 #include <optional>
 #include <stdexcept>
 #include <string>
@@ -1344,6 +1345,147 @@ PyObject* py_linrec_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   LNX_END
 }
 
+// ---------------------------------------------------------------------------------------------------------------
+// causal attention
+// ---------------------------------------------------------------------------------------------------------------
+
+// [B, H, T, d] (or [B, H, d]) tensors as the kernels read and write them: any strides that are whole numbers of 16 bytes
+bool vector_rows(const Tensor& t) {
+  if (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 || (t.size(-1) != 1 && t.stride(-1) != 1)) return false;
+  for (int64_t i = 0; i + 1 < t.dim(); ++i)
+    if (t.stride(i) * t.element_size() % 16) return false;
+  return true;
+}
+Tensor as_rows(const Tensor& t) {
+  if (vector_rows(t)) return t;
+  const Tensor c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 ? c.clone() : c;
+}
+lnx_tensor4 tensor4(const Tensor& t) { return {t.data_ptr(), t.stride(0), t.stride(1), t.dim() == 4 ? t.stride(2) : 0}; }
+
+void check_attention(const char* op, const Tensor& q, const Tensor& k, const Tensor& v, int64_t dims) {
+  const char* names = "qkv";
+  const Tensor* ts[3] = {&q, &k, &v};
+  for (int i = 0; i < 3; ++i) TORCH_CHECK(ts[i]->is_cuda(), op, ": ", names[i], " is on ", ts[i]->device().str(), "; the op runs on the GPU only");
+  TORCH_CHECK(known_dtype(q.scalar_type()), "unsupported dtype ", q.scalar_type(), ": use float32 or bfloat16");
+  TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), "q, k, v must share one dtype, got ", q.scalar_type(), ", ", k.scalar_type(), ", ",
+              v.scalar_type());
+  TORCH_CHECK(q.dim() == dims && k.dim() == dims && k.sizes() == v.sizes() && k.size(0) == q.size(0) && k.size(1) > 0 && q.size(1) > 0 && q.size(1) % k.size(1) == 0 &&
+                  k.sizes().slice(2) == q.sizes().slice(2),
+              op, ": expected q ", dims == 4 ? "[B, H, T, d] and k, v [B, Hkv, T, d]" : "[B, H, d] and k, v [B, Hkv, d]", " with H a multiple of Hkv, got q ", shape_text(q), " k ",
+              shape_text(k), " v ", shape_text(v));
+  TORCH_CHECK(q.size(-1) >= 1 && q.size(-1) <= 128, op, ": head dimension ", q.size(-1), " is not supported (1..128)");
+  for (int64_t i = 0; i < dims; ++i) TORCH_CHECK(q.size(i) <= INT32_MAX, op, ": q is too large, got ", shape_text(q));
+  check_devices(op, q, {{"k", &k}, {"v", &v}});
+}
+
+lnx_attn_args attention_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& cu, double scale) {
+  lnx_attn_args a{};
+  a.B = (int32_t)q.size(0), a.H = (int32_t)q.size(1), a.Hkv = (int32_t)k.size(1), a.T = (int32_t)q.size(2), a.d = (int32_t)q.size(3);
+  a.nseq = cu.defined() ? (int32_t)cu.numel() - 1 : 0, a.dtype = code_of(q.scalar_type()), a.scale = (float)scale;
+  a.q = tensor4(q), a.k = tensor4(k), a.v = tensor4(v), a.o = tensor4(o), a.cu_seqlens = static_cast<const int32_t*>(ptr(cu));
+  return a;
+}
+
+Tensor empty_rows(const Tensor& like, bool token_first) { return empty_layout(like.size(0), like.size(1), like.size(2), like.size(3), like.options(), token_first); }
+
+Tensor attention_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu, double scale, const Tensor& lse) {
+  const Tensor o = empty_rows(q, is_token_first(q));
+  lnx_attn_args a = attention_args(q, k, v, o, cu, scale);
+  a.lse = fptr(lse);
+  const c10::DeviceGuard guard(q.device());
+  check_status(lnx_attn_fwd(&a, stream_of(q)), "lnx_attn_fwd");
+  return o;
+}
+
+struct AttentionFn : Function<AttentionFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q0, const Tensor& k0, const Tensor& v0, const OptT& cu, double scale) {
+    const Tensor q = as_rows(q0), k = as_rows(k0), v = as_rows(v0), lse = at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
+    const Tensor o = attention_forward(q, k, v, undef(cu), scale, lse);
+    ctx->save_for_backward({q, k, v, o, lse, undef(cu)});
+    ctx->saved_data["d"] = scale;
+    return o;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_tangents("the gradient of causal_attention", grads);
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor &q = s[0], &k = s[1], &v = s[2], &o = s[3], &lse = s[4], &cu = s[5];
+    const Tensor d_o = as_rows(grads[0].to(q.scalar_type()));
+    Tensor dq = empty_rows(q, is_token_first(q)), dk = empty_rows(k, is_token_first(k)), dv = empty_rows(v, is_token_first(v));
+    lnx_attn_args a = attention_args(q, k, v, o, cu, ctx->saved_data["d"].toDouble());
+    a.d_o = tensor4(d_o), a.d_q = tensor4(dq), a.d_k = tensor4(dk), a.d_v = tensor4(dv), a.lse = fptr(lse);
+    a.workspace_bytes = lnx_attn_bwd_workspace_bytes(&a);
+    const Tensor ws = work_area(q, a.workspace_bytes);
+    a.workspace = ptr(ws);
+    const c10::DeviceGuard guard(q.device());
+    check_status(lnx_attn_bwd(&a, stream_of(q)), "lnx_attn_bwd");
+    return {dq, dk, dv, Tensor(), Tensor()};
+  }
+};
+
+// causal_attention(q, k, v, scale or None, cu): o
+PyObject* py_causal_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  LNX_BEGIN
+  Args in(args, nargs, 5, "causal_attention");
+  const char* op = "causal_attention";
+  const Tensor q = in.tensor(0, "q"), k = in.tensor(1, "k"), v = in.tensor(2, "v"), cu = in.maybe(4, "cu_seqlens");
+  check_attention(op, q, k, v, 4);
+  TORCH_CHECK(!cu.defined() || q.size(0) == 1, "cu_seqlens needs a packed batch with B == 1");
+  check_devices(op, q, {{"cu_seqlens", &cu}});
+  refuse_tangents(op, {&q, &k, &v});
+  const double scale = in.is_none(3) ? 1.0 / std::sqrt((double)q.size(3)) : in.number(3);
+  TORCH_CHECK_VALUE(std::isfinite((float)scale), op, ": scale must be finite, got ", scale);
+  return THPVariable_Wrap(without_lock([&] {
+    const int64_t d = q.size(3), more = (8 - d % 8) % 8;  // zero columns change no product
+    auto wide = [&](const Tensor& t) { return more ? at::constant_pad_nd(t, {0, more}) : t; };
+    const Tensor qw = wide(q), kw = wide(k), vw = wide(v);
+    const Tensor o = wants_grad({&q, &k, &v}) ? AttentionFn::apply(qw, kw, vw, opt(cu), scale) : attention_forward(as_rows(qw), as_rows(kw), as_rows(vw), cu, scale, Tensor());
+    return more ? o.narrow(3, 0, d).contiguous() : o;
+  }));
+  LNX_END
+}
+
+// causal_attention_step(q, k, v, k_cache, v_cache, lengths, scale or None): o
+PyObject* py_causal_attention_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  LNX_BEGIN
+  Args in(args, nargs, 7, "causal_attention_step");
+  const char* op = "causal_attention_step";
+  const Tensor q = in.tensor(0, "q"), k = in.tensor(1, "k"), v = in.tensor(2, "v"), kc = in.tensor(3, "k_cache"), vc = in.tensor(4, "v_cache"), len = in.tensor(5, "lengths");
+  check_attention(op, q, k, v, 3);
+  const int64_t B = q.size(0), H = q.size(1), Hkv = k.size(1), d = q.size(2);
+  TORCH_CHECK(d % 8 == 0, op, ": head dimension ", d, " is not a multiple of 8, which a cache needs");
+  check_devices(op, q, {{"k_cache", &kc}, {"v_cache", &vc}, {"lengths", &len}});
+  for (const auto& [name, t] : {std::make_pair("k_cache", &kc), std::make_pair("v_cache", &vc)}) {
+    TORCH_CHECK(t->scalar_type() == q.scalar_type(), op, ": ", name, " must have q's dtype ", q.scalar_type(), ", got ", t->scalar_type());
+    TORCH_CHECK(t->dim() == 4 && t->size(0) == B && t->size(1) == Hkv && t->size(2) > 0 && t->size(3) == d && t->sizes() == kc.sizes(), op, ": ", name, " must be [", B, ", ", Hkv,
+                ", S, ", d, "], got ", shape_text(*t));
+    bool once = true;
+    for (int64_t i = 0; i < 3; ++i) once = once && (t->size(i) == 1 || t->stride(i) != 0);
+    TORCH_CHECK(vector_rows(*t) && once, op, ": ", name, " is written in place: its rows must be contiguous, 16-byte aligned and each its own memory");
+    TORCH_CHECK(t->size(2) <= INT32_MAX, op, ": ", name, " is too large, got ", shape_text(*t));
+  }
+  TORCH_CHECK(len.scalar_type() == at::kInt && len.dim() == 1 && len.size(0) == B && len.is_contiguous(), op, ": lengths must be a contiguous int32 [", B, "] tensor, got ",
+              shape_text(len), " ", len.scalar_type());
+  TORCH_CHECK(!wants_grad({&q, &k, &v, &kc, &vc}), "cannot differentiate through a step that updates its cache in place");
+  refuse_tangents(op, {&q, &k, &v, &kc, &vc});
+  const double scale = in.is_none(6) ? 1.0 / std::sqrt((double)d) : in.number(6);
+  TORCH_CHECK_VALUE(std::isfinite((float)scale), op, ": scale must be finite, got ", scale);
+  return THPVariable_Wrap(without_lock([&] {
+    const Tensor qr = as_rows(q), kr = as_rows(k), vr = as_rows(v), o = at::empty({B, H, d}, q.options());
+    lnx_attn_step_args a{};
+    a.B = (int32_t)B, a.H = (int32_t)H, a.Hkv = (int32_t)Hkv, a.S = (int32_t)kc.size(2), a.d = (int32_t)d, a.dtype = code_of(q.scalar_type()), a.scale = (float)scale;
+    a.q = tensor4(qr), a.k = tensor4(kr), a.v = tensor4(vr), a.k_cache = tensor4(kc), a.v_cache = tensor4(vc), a.o = ptr(o), a.lengths = static_cast<const int32_t*>(ptr(len));
+    a.workspace_bytes = lnx_attn_step_workspace_bytes(&a);
+    Tensor ws;
+    if (a.workspace_bytes) ws = work_area(q, a.workspace_bytes);
+    a.workspace = ptr(ws);
+    const c10::DeviceGuard guard(q.device());
+    check_status(lnx_attn_step(&a, stream_of(q)), "lnx_attn_step");
+    return o;
+  }));
+  LNX_END
+}
+
 // set_kernel_error(class): the exception a failed C-ABI call raises
 PyObject* py_set_kernel_error(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (nargs != 1 || !PyExceptionClass_Check(args[0])) {
@@ -1357,7 +1499,7 @@ PyObject* py_set_kernel_error(PyObject*, PyObject* const* args, Py_ssize_t nargs
 
 #define LNX_FN(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {LNX_FN(step),     LNX_FN(recurrent), LNX_FN(l2norm), LNX_FN(l2norm_bwd), LNX_FN(chunk), LNX_FN(chunk_segmented),     LNX_FN(conv1d),           LNX_FN(rmsnorm_gated), LNX_FN(gdn_gate),
-                         LNX_FN(kda_gate), LNX_FN(dplr),      LNX_FN(dplr_step), LNX_FN(linrec), LNX_FN(linrec_step), LNX_FN(rmsnorm_residual), LNX_FN(set_kernel_error), {nullptr, nullptr, 0, nullptr}};
+                         LNX_FN(kda_gate), LNX_FN(dplr),      LNX_FN(dplr_step), LNX_FN(linrec), LNX_FN(linrec_step), LNX_FN(rmsnorm_residual), LNX_FN(causal_attention), LNX_FN(causal_attention_step), LNX_FN(set_kernel_error), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_host", "Host path of the linearnexus_amd ops.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
