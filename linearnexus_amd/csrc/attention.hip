@@ -82,14 +82,6 @@ template <int D, int R> struct Tile<bf16_t, D, R> {
     const short8_ v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     return {__builtin_bit_cast(bf16x8, v)};
   }
-  static __device__ __forceinline__ bool finite(const bf16_t* t, int j, int lane) {  // of the granule that instruction j's lane brought
-    typedef unsigned uint4_ __attribute__((ext_vector_type(4)));
-    const uint4_ x = *reinterpret_cast<const uint4_*>(t + (64 * j + lane) * 8);
-    bool ok = true;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) ok = ok && (x[e] & 0x7f80u) != 0x7f80u && (x[e] & 0x7f800000u) != 0x7f800000u;
-    return ok;
-  }
 };
 template <int D, int R> struct Tile<float, D, R> {
   static constexpr int BYTES = R * D * 4, G = D / 4;
@@ -110,13 +102,6 @@ template <int D, int R> struct Tile<float, D, R> {
     for (int e = 0; e < 8; ++e) f.v[e] = t[at(k0 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3), c0 + (lane & 31))];
     return f;
   }
-  static __device__ __forceinline__ bool finite(const float* t, int j, int lane) {
-    const floatx4 x = load4(t + (64 * j + lane) * 4);
-    bool ok = true;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) ok = ok && (__float_as_uint(x[e]) & 0x7f800000u) != 0x7f800000u;
-    return ok;
-  }
 };
 
 // Rows row0 .. row0 + 63 of a [len][d] matrix with row stride `st`, by the workgroup's four waves; rows behind the last are copies of
@@ -132,11 +117,23 @@ template <typename T, int D> __device__ __forceinline__ void fetch_tile(T* tile,
     if (c < d) dma16(base + (int64_t)min(row0 + r, len - 1) * st + c, lds_byte_addr(tile) + 1024 * j);
   }
 }
-template <typename T, int D> __device__ __forceinline__ bool tile_finite(const T* tile, int wave, int lane) {
-  constexpr int N = Tile<T, D>::BYTES / 1024 / 4;
+__device__ __forceinline__ bool is_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
+// Whether the granules that this lane's loads brought hold finite values only; SCRUB: the others become 0.  A wave's granules are
+// rows 16 wave .. 16 wave + 15.
+template <typename T, int D, bool SCRUB> __device__ __forceinline__ bool tile_finite(T* tile, int wave, int lane) {
+  constexpr int N = Tile<T, D>::BYTES / 1024 / 4, VN = Vec16<T>::N;
   bool ok = true;
 #pragma unroll
-  for (int i = 0; i < N; ++i) ok = ok && Tile<T, D>::finite(tile, wave * N + i, lane);
+  for (int i = 0; i < N; ++i) {
+    typename Vec16<T>::V* p = reinterpret_cast<typename Vec16<T>::V*>(tile + (64 * (wave * N + i) + lane) * VN);
+    typename Vec16<T>::V v = *p;
+    bool all = true;
+#pragma unroll
+    for (int e = 0; e < VN; ++e)
+      if (!is_finite(to_f32(v[e]))) all = false, v[e] = from_f32<T>(0.f);
+    if (SCRUB && !all) *p = v;
+    ok = ok && all;
+  }
   return ok;
 }
 __device__ __forceinline__ void clear_lds(char* p, int bytes) {
@@ -149,29 +146,33 @@ __device__ __forceinline__ float half_max(float x) {
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-// acc += (rows of a tile, turned) . B one row at a time, leaving out the (row, column) pairs that are masked: what the products over
-// the rows do when the tile holds values that are not finite, because 0 times those is not 0.  keep(row of the tile): this lane's column takes it.
-template <typename T, int D, typename F> __device__ __forceinline__ void add_rows_singly(floatx16 (&acc)[D / 32], const T* tile, int r0, const Frag8<T> (&b)[2], int lane, F keep) {
+// A product over the rows of a tile takes masked pairs with weight 0, and 0 times a value that is not finite is not 0: such values
+// are scrubbed from the tile, and their part of the product is added here, pair by pair and only where keep(row) lets this lane's
+// column have it.  w: the weights of the 32 rows from row0 on, as an operand; the values are read again from memory.
+template <typename T, int D, typename F>
+__device__ __forceinline__ void add_odd(floatx16 (&acc)[D / 32], const T* base, int64_t st, int row0, int len, int d, const Frag8<T> (&w)[2], int lane, F keep) {
+  const int kg = lane >> 5;
 #pragma unroll 1
-  for (int h = 0; h < 2; ++h)
-#pragma unroll 1
-    for (int e = 0; e < 16; ++e) {
-      const int row = r0 + 16 * h + e, slot = (e & 3) + 4 * (e >> 3), kg = (e >> 2) & 1;
+  for (int j = 0; j < 32 && row0 + j < len; ++j) {
+    const int e = (j & 3) + 4 * (j >> 3);
+    float x = 0.f;
 #pragma unroll
-      for (int m = 0; m < D / 32; ++m) {
-        Frag8<T> a = Tile<T, D>::by_col(tile, r0 + 16 * h, 32 * m, lane);
+    for (int i = 0; i < 16; ++i) x = e == i ? to_f32(w[i >> 3].v[i & 7]) : x;
+    const float other = __shfl_xor(x, 32, LNX_WAVE);
+    x = ((j >> 2) & 1) == kg ? x : other;
+    const bool on = keep(row0 + j);
+    const T* r = base + (int64_t)(row0 + j) * st + 4 * kg;
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (j != slot || (lane >> 5) != kg) a.v[j] = from_f32<T>(0.f);
-        floatx16 t;
+    for (int m = 0; m < D / 32; ++m)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) t[i] = 0.f;
-        mma(t, a, h ? b[1] : b[0]);
-        const bool on = keep(row);
+      for (int q = 0; q < 4; ++q)
+        if (32 * m + 8 * q + 4 * kg < d) {
+          const floatx4 v = load4(r + 32 * m + 8 * q);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[m][i] += on ? t[i] : 0.f;
-      }
-    }
+          for (int i = 0; i < 4; ++i)
+            if (on && !is_finite(v[i])) acc[m][4 * q + i] += x * v[i];
+        }
+  }
 }
 
 // Where a workgroup works: sequence (its first token, its length), block of `size` rows, heads
@@ -297,13 +298,14 @@ template <typename T, int D, int NQ> __global__ __launch_bounds__(256, sizeof(T)
   }
   for (int it = 0; it < ntile; ++it) {
     const int key0 = it * ROWS, buf = it & 1;
+    const int ln = fresh(lane);  // LDS addresses are formed again where they are used: kept over the loop they cost the accumulators' registers
     dma_wait<0>();
     const bool edge = key0 + ROWS > q_wg;  // some pairs of this tile are masked
-    if (edge && !tile_finite<T, D>(vt(buf), wave, lane)) odd[buf] = 1;
+    if (edge && !tile_finite<T, D, true>(vt(buf), wave, ln)) odd[buf] = 1;
     lds_barrier();
     if (it + 1 < ntile) {
-      fetch_tile<T, D>(kt(buf ^ 1), kb, a.ks[2], key0 + ROWS, p.len, a.d, wave, lane);
-      fetch_tile<T, D>(vt(buf ^ 1), vb, a.vs[2], key0 + ROWS, p.len, a.d, wave, lane);
+      fetch_tile<T, D>(kt(buf ^ 1), kb, a.ks[2], key0 + ROWS, p.len, a.d, wave, ln);
+      fetch_tile<T, D>(vt(buf ^ 1), vb, a.vs[2], key0 + ROWS, p.len, a.d, wave, ln);
     }
     if (key0 >= q0 + 32 * NQ) continue;  // behind all of this wave's queries
     floatx16 sc[NQ][2];
@@ -317,7 +319,7 @@ template <typename T, int D, int NQ> __global__ __launch_bounds__(256, sizeof(T)
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int s = 0; s < D / 16; ++s) {
-        const Frag8<T> kf = TL::by_row(kt(buf), 32 * i, 16 * s, lane);
+        const Frag8<T> kf = TL::by_row(kt(buf), 32 * i, 16 * s, ln);
 #pragma unroll
         for (int t = 0; t < NQ; ++t) mma(sc[t][i], kf, qf[t][s]);
       }
@@ -330,7 +332,7 @@ template <typename T, int D, int NQ> __global__ __launch_bounds__(256, sizeof(T)
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            if (key0 + 32 * i + frag_row(e, lane) > q) sc[t][i][e] = -INFINITY;
+            if (key0 + 32 * i + frag_row(e, ln) > q) sc[t][i][e] = -INFINITY;
       }
       float top = sc[t][0][0];
 #pragma unroll
@@ -363,24 +365,21 @@ template <typename T, int D, int NQ> __global__ __launch_bounds__(256, sizeof(T)
 #pragma unroll
       for (int s = 0; s < 4; ++s) from_acc(pf[t][s], sc[t][s >> 1], s & 1);
     }
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        const Frag8<T> vf = TL::by_col(vt(buf), 16 * s, 32 * i, ln);
+#pragma unroll
+        for (int t = 0; t < NQ; ++t) mma(acc[t][i], vf, pf[t][s]);
+      }
     if (edge && odd[buf]) {
 #pragma unroll
-      for (int t = 0; t < NQ; ++t) {
-        const int q = q0 + 32 * t + n;
+      for (int t = 0; t < NQ; ++t)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const Frag8<T> two[2] = {pf[t][2 * i], pf[t][2 * i + 1]};
-          add_rows_singly<T, D>(acc[t], vt(buf), 32 * i, two, lane, [&](int row) { return key0 + row <= q; });
-        }
-      }
-    } else {
-#pragma unroll
-      for (int s = 0; s < 4; ++s)
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-          const Frag8<T> vf = TL::by_col(vt(buf), 16 * s, 32 * i, lane);
-#pragma unroll
-          for (int t = 0; t < NQ; ++t) mma(acc[t][i], vf, pf[t][s]);
+          add_odd<T, D>(acc[t], vb, a.vs[2], key0 + 32 * i, p.len, a.d, two, ln, [&](int row) { return row <= q0 + 32 * t + n; });
         }
     }
   }
@@ -451,40 +450,48 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
     for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
   for (int it = 0; it < ntile; ++it) {
     const int key0 = it * ROWS, buf = it & 1;
+    const int ln = fresh(lane);  // LDS addresses are formed again where they are used: kept over the loop they cost the accumulators' registers
     dma_wait<0>();
     const bool edge = key0 + ROWS > q_wg;
-    if (edge && !tile_finite<T, D>(kt(buf), wave, lane)) odd[buf] = 1;
+    if (edge && !tile_finite<T, D, false>(kt(buf), wave, ln)) odd[buf] = 1;
     lds_barrier();
     if (it + 1 < ntile) {
-      fetch_tile<T, D>(kt(buf ^ 1), kb, a.ks[2], key0 + ROWS, p.len, a.d, wave, lane);
-      fetch_tile<T, D>(vt(buf ^ 1), vb, a.vs[2], key0 + ROWS, p.len, a.d, wave, lane);
+      fetch_tile<T, D>(kt(buf ^ 1), kb, a.ks[2], key0 + ROWS, p.len, a.d, wave, ln);
+      fetch_tile<T, D>(vt(buf ^ 1), vb, a.vs[2], key0 + ROWS, p.len, a.d, wave, ln);
     }
+    const bool scrub = edge && odd[buf];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      if (key0 + 32 * i > q0 + 31) continue;  // behind all of this wave's queries
-      floatx16 sc, dp;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) sc[e] = dp[e] = 0.f;
-#pragma unroll
-      for (int s = 0; s < D / 16; ++s) {
-        mma(sc, TL::by_row(kt(buf), 32 * i, 16 * s, lane), qf[s]);
-        mma(dp, TL::by_row(vt(buf), 32 * i, 16 * s, lane), gf[s]);
-      }
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float pe = __builtin_amdgcn_exp2f(sc[e] * c - lse);
-        sc[e] = key0 + 32 * i + frag_row(e, lane) <= q ? pe * (dp[e] - delta) : 0.f;
-      }
+      const bool mine = key0 + 32 * i <= q0 + 31;  // not behind all of this wave's queries
       Frag8<T> ds[2];
-      from_acc(ds[0], sc, 0);
-      from_acc(ds[1], sc, 1);
-      if (edge && odd[buf]) {
-        add_rows_singly<T, D>(acc, kt(buf), 32 * i, ds, lane, [&](int r) { return key0 + r <= q; });
-      } else {
+      if (mine) {
+        floatx16 sc, dp;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc[e] = dp[e] = 0.f;
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) {
+          mma(sc, TL::by_row(kt(buf), 32 * i, 16 * s, ln), qf[s]);
+          mma(dp, TL::by_row(vt(buf), 32 * i, 16 * s, ln), gf[s]);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float pe = __builtin_amdgcn_exp2f(sc[e] * c - lse);
+          sc[e] = key0 + 32 * i + frag_row(e, ln) <= q ? pe * (dp[e] - delta) : 0.f;
+        }
+        from_acc(ds[0], sc, 0);
+        from_acc(ds[1], sc, 1);
+      }
+      if (scrub) {  // the scores are made of the keys as they are
+        lds_barrier();
+        if (wave >> 1 == i) tile_finite<T, D, true>(kt(buf), wave, ln);
+        lds_barrier();
+      }
+      if (mine) {
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
-          for (int m = 0; m < D / 32; ++m) mma(acc[m], TL::by_col(kt(buf), 32 * i + 16 * s, 32 * m, lane), ds[s]);
+          for (int m = 0; m < D / 32; ++m) mma(acc[m], TL::by_col(kt(buf), 32 * i + 16 * s, 32 * m, ln), ds[s]);
+        if (scrub) add_odd<T, D>(acc, kb, a.ks[2], key0 + 32 * i, p.len, a.d, ds, ln, [&](int row) { return row <= q; });
       }
     }
   }
@@ -503,19 +510,19 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
   if (!p.on) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, kg = lane >> 5;
   const int kw = wave & 1, r0 = 32 * (wave >> 1), key0 = p.blk * ROWS + 32 * kw, key = key0 + n;
-  const int ntile = (p.len + ROWS - 1) / ROWS, per = ntile - p.blk, total = per * a.G;
+  const int total = ((p.len + ROWS - 1) / ROWS - p.blk) * a.G;
   if (a.d < D) clear_lds(lds, 4 * TL::BYTES);
   if (threadIdx.x < 2) odd[threadIdx.x] = 0;
   lds_barrier();
-  auto fetch = [&](int it, int buf) {
-    const int h = p.hkv * a.G + it / per, row0 = (p.blk + it % per) * ROWS;
+  auto fetch = [&](int h, int row0, int buf) {
     fetch_tile<T, D>(qt(buf), at<T>(a.q, a.qs, p.b, h, p.tok), a.qs[2], row0, p.len, a.d, wave, lane);
     fetch_tile<T, D>(gt(buf), at<T>(a.dout, a.gs, p.b, h, p.tok), a.gs[2], row0, p.len, a.d, wave, lane);
     const int64_t stat = ((int64_t)p.b * a.H + h) * a.T + p.tok + min(row0 + lane, p.len - 1);
     if (wave == 0) dma4(a.lse + stat, lds_byte_addr(stats + buf * 128));
     if (wave == 1) dma4(a.delta + stat, lds_byte_addr(stats + buf * 128 + 64));
   };
-  fetch(0, 0);
+  int h = p.hkv * a.G, row0 = p.blk * ROWS;  // the tile being multiplied
+  fetch(h, row0, 0);
   const float c = a.scale * LOG2E;
   const int64_t krow = p.tok + min(key, p.len - 1);
   const T* kr = at<T>(a.k, a.ks, p.b, p.hkv, krow);
@@ -532,49 +539,62 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
 #pragma unroll
     for (int e = 0; e < 16; ++e) dk[i][e] = dv[i][e] = 0.f;
   for (int it = 0; it < total; ++it) {
-    const int buf = it & 1, row0 = (p.blk + it % per) * ROWS;
+    const int buf = it & 1;
+    const int ln = fresh(lane);  // LDS addresses are formed again where they are used: kept over the loop they cost the accumulators' registers
     dma_wait<0>();
-    const bool edge = it % per == 0 || row0 + ROWS > p.len;
-    if (edge && !(tile_finite<T, D>(qt(buf), wave, lane) && tile_finite<T, D>(gt(buf), wave, lane))) odd[buf] = 1;
+    const bool edge = row0 == p.blk * ROWS || row0 + ROWS > p.len;
+    const int next_h = row0 + ROWS >= p.len ? h + 1 : h, next_row0 = next_h == h ? row0 + ROWS : p.blk * ROWS;
+    if (edge && !(tile_finite<T, D, false>(qt(buf), wave, ln) && tile_finite<T, D, false>(gt(buf), wave, ln))) odd[buf] = 1;
     lds_barrier();
-    if (it + 1 < total) fetch(it + 1, buf ^ 1);
-    if (row0 + r0 + 31 < key0 || row0 + r0 >= p.len) continue;  // queries before all of this wave's keys, or none
-    const float* st = stats + buf * 128 + r0;
-    floatx16 sc, dp;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) sc[e] = dp[e] = 0.f;
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s) mma(sc, TL::by_row(qt(buf), r0, 16 * s, lane), kf[s]);
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s) mma(dp, TL::by_row(gt(buf), r0, 16 * s, lane), vf[s]);
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const floatx4 lse = load4(st + 8 * g + 4 * kg), delta = load4(st + 64 + 8 * g + 4 * kg);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int q = row0 + r0 + 8 * g + 4 * kg + e;
-        const bool on = q >= key && q < p.len;
-        const float pe = on ? __builtin_amdgcn_exp2f(sc[4 * g + e] * c - lse[e]) : 0.f;
-        sc[4 * g + e] = pe;
-        dp[4 * g + e] = on ? pe * (dp[4 * g + e] - delta[e]) : 0.f;
-      }
-    }
+    if (it + 1 < total) fetch(next_h, next_row0, buf ^ 1);
+    const bool mine = row0 + r0 + 31 >= key0 && row0 + r0 < p.len, scrub = edge && odd[buf];
     Frag8<T> pf[2], ds[2];
+    if (mine) {  // some of these queries come after some of this wave's keys
+      const float* st = stats + buf * 128 + r0;
+      floatx16 sc, dp;
 #pragma unroll
-    for (int s = 0; s < 2; ++s) from_acc(pf[s], sc, s), from_acc(ds[s], dp, s);
-    if (edge && odd[buf]) {
-      const auto keep = [&](int r) { return row0 + r >= key && row0 + r < p.len; };
-      add_rows_singly<T, D>(dv, gt(buf), r0, pf, lane, keep);
-      add_rows_singly<T, D>(dk, qt(buf), r0, ds, lane, keep);
-    } else {
+      for (int e = 0; e < 16; ++e) sc[e] = dp[e] = 0.f;
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s) mma(sc, TL::by_row(qt(buf), r0, 16 * s, ln), kf[s]);
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s) mma(dp, TL::by_row(gt(buf), r0, 16 * s, ln), vf[s]);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const floatx4 lse = load4(st + 8 * g + 4 * kg), delta = load4(st + 64 + 8 * g + 4 * kg);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int q = row0 + r0 + 8 * g + 4 * kg + e;
+          const bool on = q >= key && q < p.len;
+          const float pe = on ? __builtin_amdgcn_exp2f(sc[4 * g + e] * c - lse[e]) : 0.f;
+          sc[4 * g + e] = pe;
+          dp[4 * g + e] = on ? pe * (dp[4 * g + e] - delta[e]) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s) from_acc(pf[s], sc, s), from_acc(ds[s], dp, s);
+    }
+    if (scrub) {  // the scores are made of the queries and gradients as they are
+      lds_barrier();
+      tile_finite<T, D, true>(qt(buf), wave, ln);
+      tile_finite<T, D, true>(gt(buf), wave, ln);
+      lds_barrier();
+    }
+    if (mine) {
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int m = 0; m < D / 32; ++m) {
-          mma(dv[m], TL::by_col(gt(buf), r0 + 16 * s, 32 * m, lane), pf[s]);
-          mma(dk[m], TL::by_col(qt(buf), r0 + 16 * s, 32 * m, lane), ds[s]);
+          mma(dv[m], TL::by_col(gt(buf), r0 + 16 * s, 32 * m, ln), pf[s]);
+          mma(dk[m], TL::by_col(qt(buf), r0 + 16 * s, 32 * m, ln), ds[s]);
         }
+      if (scrub) {
+        const auto keep = [&](int row) { return row >= key; };
+        add_odd<T, D>(dv, at<T>(a.dout, a.gs, p.b, h, p.tok), a.gs[2], row0 + r0, p.len, a.d, pf, ln, keep);
+        add_odd<T, D>(dk, at<T>(a.q, a.qs, p.b, h, p.tok), a.qs[2], row0 + r0, p.len, a.d, ds, ln, keep);
+      }
     }
+    h = next_h;
+    row0 = next_row0;
   }
   lds_barrier();
   float* sums = reinterpret_cast<float*>(lds) + kw * (2 * D / 32) * 16 * 64;
