@@ -17,6 +17,7 @@ namespace {
 
 constexpr int ROWS = 64;  // rows of a tile
 constexpr float LOG2E = 1.4426950408889634f;
+__device__ __forceinline__ unsigned fresh(unsigned x) { return (unsigned)::fresh((int)x); }
 
 struct Args {
   const void *q, *k, *v, *dout;
@@ -68,38 +69,55 @@ template <> __device__ __forceinline__ void from_global<float>(Frag8<float>& f, 
   }
 }
 
-// A [R][D] tile in LDS, 16-byte granules of a row permuted by the row so that row reads and reads along the rows spread over the banks
+// A [R][D] tile in LDS, 16-byte granules of a row permuted by an exclusive or with the row, so that row reads and reads along the rows
+// spread over the banks.  A lane reads at an address of its own exclusive-or a constant per column block, plus a constant per
+// block of rows that fits the instruction's offset: rows() and cols() give the lane's addresses, by_row and by_col the operands.
+typedef __attribute__((address_space(3))) char lds_char;
+template <typename V> __device__ __forceinline__ V lds_load(unsigned addr) { return *(__attribute__((address_space(3))) const V*)(lds_char*)(uintptr_t)addr; }
+
 template <typename T, int D, int R = ROWS> struct Tile;
 template <int D, int R> struct Tile<bf16_t, D, R> {
   typedef SwzTile<R, D> S;
-  static constexpr int BYTES = R * D * 2;
+  static constexpr int BYTES = R * D * 2, ROWB = D * 2;
   static __device__ __forceinline__ void src(int j, int lane, int& r, int& c) { S::src(j, lane, r, c); }
-  static __device__ __forceinline__ Frag8<bf16_t> by_row(const bf16_t* t, int r0, int k0, int lane) { return {S::load(t, r0 + (lane & 31), k0 + 8 * (lane >> 5))}; }
-  static __device__ __forceinline__ Frag8<bf16_t> by_col(const bf16_t* t, int k0, int c0, int lane) {
+  // rows r = lane & 31 of 32, columns 16 s + 8 kg + 0 .. 7: granule (2 s + kg) ^ x(r)
+  static __device__ __forceinline__ unsigned rows(int lane) { return 2 * S::at(lane & 31, 8 * (lane >> 5)); }
+  static __device__ __forceinline__ Frag8<bf16_t> by_row(unsigned rows, int off, int s) { return {lds_load<bf16x8>((rows ^ (32 * s)) + off)}; }
+  // rows 4 kg + 0 .. 3 and 8 + 4 kg + 0 .. 3 of 16, column 32 m + (lane & 31): two transposing reads of four rows each
+  static __device__ __forceinline__ unsigned cols(int lane) {
+    const int s = lane & 15, grp = lane >> 4;
+    return 2 * S::at(4 * (grp >> 1) + (s >> 2), 16 * (grp & 1) + 4 * (s & 3));
+  }
+  static __device__ __forceinline__ Frag8<bf16_t> by_col(unsigned cols, int off, int m) {
+    typedef short short4_ __attribute__((ext_vector_type(4)));
     typedef short short8_ __attribute__((ext_vector_type(8)));
-    const int grp = lane >> 4;
-    const auto lo = S::tr4(t, k0 + 4 * (grp >> 1), c0 + 16 * (grp & 1), lane), hi = S::tr4(t, k0 + 8 + 4 * (grp >> 1), c0 + 16 * (grp & 1), lane);
+    typedef __attribute__((address_space(3))) short4_ lds_short4;
+    // eight rows further on x differs by 2 in its low bits (128-byte and 256-byte rows alike)
+    const unsigned at = cols ^ (64 * m);
+    const short4_ lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(lds_char*)(uintptr_t)(at + off));
+    const short4_ hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(lds_char*)(uintptr_t)((at ^ 32) + off + 8 * ROWB));
     const short8_ v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     return {__builtin_bit_cast(bf16x8, v)};
   }
 };
 template <int D, int R> struct Tile<float, D, R> {
-  static constexpr int BYTES = R * D * 4, G = D / 4;
+  static constexpr int BYTES = R * D * 4, ROWB = D * 4, G = D / 4;
   static __device__ __forceinline__ int at(int r, int c) { return r * D + ((((c >> 2) ^ (r & 7)) << 2) | (c & 3)); }
   static __device__ __forceinline__ void src(int j, int lane, int& r, int& c) {
     const int p = 64 * j + lane;
     r = p / G;
     c = ((p % G) ^ (r & 7)) << 2;
   }
-  static __device__ __forceinline__ Frag8<float> by_row(const float* t, int r0, int k0, int lane) {
-    const int r = r0 + (lane & 31), c = k0 + 8 * (lane >> 5);
-    const floatx4 a = load4(t + at(r, c)), b = load4(t + at(r, c + 4));
+  static __device__ __forceinline__ unsigned rows(int lane) { return 4 * at(lane & 31, 8 * (lane >> 5)); }
+  static __device__ __forceinline__ Frag8<float> by_row(unsigned rows, int off, int s) {
+    const floatx4 a = lds_load<floatx4>((rows ^ (64 * s)) + off), b = lds_load<floatx4>((rows ^ (64 * s + 16)) + off);
     return {{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}};
   }
-  static __device__ __forceinline__ Frag8<float> by_col(const float* t, int k0, int c0, int lane) {
+  static __device__ __forceinline__ unsigned cols(int lane) { return 4 * at(4 * (lane >> 5), lane & 31); }
+  static __device__ __forceinline__ Frag8<float> by_col(unsigned cols, int off, int m) {
     Frag8<float> f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f.v[e] = t[at(k0 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3), c0 + (lane & 31))];
+    for (int e = 0; e < 8; ++e) f.v[e] = lds_load<float>((cols ^ (16 * (e & 3))) + off + (8 * (e >> 2) + (e & 3)) * ROWB + 128 * m);
     return f;
   }
 };
@@ -138,6 +156,20 @@ template <typename T, int D, bool SCRUB> __device__ __forceinline__ bool tile_fi
 }
 __device__ __forceinline__ void clear_lds(char* p, int bytes) {
   for (int i = threadIdx.x * 16; i < bytes; i += 256 * 16) *reinterpret_cast<floatx4*>(p + i) = floatx4{0.f, 0.f, 0.f, 0.f};
+}
+
+// How a run of N products takes its operands from LDS (COL: through by_col): AHEAD operands are on their way before the first product
+// and each product is followed by the reads of another.  Left to itself the compiler saves the registers and waits for every operand
+// right before its product, 130 cycles for 32 of work.
+template <typename T, bool COL, int N, int AHEAD> __device__ __forceinline__ void read_ahead() {
+  constexpr int READS = sizeof(T) == 2 ? (COL ? 2 : 1) : (COL ? 8 : 2), PRODUCTS = sizeof(T) == 2 ? 1 : 8, DS = 0x100, MFMA = 0x8;
+  __builtin_amdgcn_sched_group_barrier(DS, READS * AHEAD, 0);
+#pragma unroll
+  for (int i = 0; i < N - AHEAD; ++i) {
+    __builtin_amdgcn_sched_group_barrier(MFMA, PRODUCTS, 0);
+    __builtin_amdgcn_sched_group_barrier(DS, READS, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(MFMA, PRODUCTS * AHEAD, 0);
 }
 
 // max over the wave's two halves
@@ -296,16 +328,17 @@ template <typename T, int D, int NQ> __global__ __launch_bounds__(256, sizeof(T)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[t][i][e] = 0.f;
   }
+  const unsigned row_addr = lds_byte_addr(lds) + TL::rows(lane), col_addr = lds_byte_addr(lds) + TL::cols(lane);
   for (int it = 0; it < ntile; ++it) {
     const int key0 = it * ROWS, buf = it & 1;
-    const int ln = fresh(lane);  // LDS addresses are formed again where they are used: kept over the loop they cost the accumulators' registers
+    const unsigned rows = row_addr + 2 * buf * TL::BYTES, cols = col_addr + 2 * buf * TL::BYTES;
     dma_wait<0>();
     const bool edge = key0 + ROWS > q_wg;  // some pairs of this tile are masked
-    if (edge && !tile_finite<T, D, true>(vt(buf), wave, ln)) odd[buf] = 1;
+    if (edge && !tile_finite<T, D, true>(vt(buf), wave, lane)) odd[buf] = 1;
     lds_barrier();
     if (it + 1 < ntile) {
-      fetch_tile<T, D>(kt(buf ^ 1), kb, a.ks[2], key0 + ROWS, p.len, a.d, wave, ln);
-      fetch_tile<T, D>(vt(buf ^ 1), vb, a.vs[2], key0 + ROWS, p.len, a.d, wave, ln);
+      fetch_tile<T, D>(kt(buf ^ 1), kb, a.ks[2], key0 + ROWS, p.len, a.d, wave, lane);
+      fetch_tile<T, D>(vt(buf ^ 1), vb, a.vs[2], key0 + ROWS, p.len, a.d, wave, lane);
     }
     if (key0 >= q0 + 32 * NQ) continue;  // behind all of this wave's queries
     floatx16 sc[NQ][2];
@@ -319,10 +352,11 @@ template <typename T, int D, int NQ> __global__ __launch_bounds__(256, sizeof(T)
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int s = 0; s < D / 16; ++s) {
-        const Frag8<T> kf = TL::by_row(kt(buf), 32 * i, 16 * s, ln);
+        const Frag8<T> kf = TL::by_row(rows, 32 * i * TL::ROWB, s);
 #pragma unroll
         for (int t = 0; t < NQ; ++t) mma(sc[t][i], kf, qf[t][s]);
       }
+    read_ahead<T, false, 2 * (D / 16), 4>();
     Frag8<T> pf[NQ][4];
 #pragma unroll
     for (int t = 0; t < NQ; ++t) {
@@ -332,7 +366,7 @@ template <typename T, int D, int NQ> __global__ __launch_bounds__(256, sizeof(T)
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            if (key0 + 32 * i + frag_row(e, ln) > q) sc[t][i][e] = -INFINITY;
+            if (key0 + 32 * i + frag_row(e, lane) > q) sc[t][i][e] = -INFINITY;
       }
       float top = sc[t][0][0];
 #pragma unroll
@@ -369,17 +403,18 @@ template <typename T, int D, int NQ> __global__ __launch_bounds__(256, sizeof(T)
     for (int s = 0; s < 4; ++s)
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
-        const Frag8<T> vf = TL::by_col(vt(buf), 16 * s, 32 * i, ln);
+        const Frag8<T> vf = TL::by_col(cols, TL::BYTES + 16 * s * TL::ROWB, i);
 #pragma unroll
         for (int t = 0; t < NQ; ++t) mma(acc[t][i], vf, pf[t][s]);
       }
+    read_ahead<T, true, 4 * (D / 32), 4>();
     if (edge && odd[buf]) {
 #pragma unroll
       for (int t = 0; t < NQ; ++t)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const Frag8<T> two[2] = {pf[t][2 * i], pf[t][2 * i + 1]};
-          add_odd<T, D>(acc[t], vb, a.vs[2], key0 + 32 * i, p.len, a.d, two, ln, [&](int row) { return row <= q0 + 32 * t + n; });
+          add_odd<T, D>(acc[t], vb, a.vs[2], key0 + 32 * i, p.len, a.d, two, lane, [&](int row) { return row <= q0 + 32 * t + n; });
         }
     }
   }
@@ -448,16 +483,17 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
   for (int i = 0; i < D / 32; ++i)
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
+  const unsigned row_addr = lds_byte_addr(lds) + TL::rows(lane), col_addr = lds_byte_addr(lds) + TL::cols(lane);
   for (int it = 0; it < ntile; ++it) {
     const int key0 = it * ROWS, buf = it & 1;
-    const int ln = fresh(lane);  // LDS addresses are formed again where they are used: kept over the loop they cost the accumulators' registers
+    const unsigned rows = row_addr + 2 * buf * TL::BYTES, cols = col_addr + 2 * buf * TL::BYTES;
     dma_wait<0>();
     const bool edge = key0 + ROWS > q_wg;
-    if (edge && !tile_finite<T, D, false>(kt(buf), wave, ln)) odd[buf] = 1;
+    if (edge && !tile_finite<T, D, false>(kt(buf), wave, lane)) odd[buf] = 1;
     lds_barrier();
     if (it + 1 < ntile) {
-      fetch_tile<T, D>(kt(buf ^ 1), kb, a.ks[2], key0 + ROWS, p.len, a.d, wave, ln);
-      fetch_tile<T, D>(vt(buf ^ 1), vb, a.vs[2], key0 + ROWS, p.len, a.d, wave, ln);
+      fetch_tile<T, D>(kt(buf ^ 1), kb, a.ks[2], key0 + ROWS, p.len, a.d, wave, lane);
+      fetch_tile<T, D>(vt(buf ^ 1), vb, a.vs[2], key0 + ROWS, p.len, a.d, wave, lane);
     }
     const bool scrub = edge && odd[buf];
 #pragma unroll
@@ -470,28 +506,31 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
         for (int e = 0; e < 16; ++e) sc[e] = dp[e] = 0.f;
 #pragma unroll
         for (int s = 0; s < D / 16; ++s) {
-          mma(sc, TL::by_row(kt(buf), 32 * i, 16 * s, ln), qf[s]);
-          mma(dp, TL::by_row(vt(buf), 32 * i, 16 * s, ln), gf[s]);
+          mma(sc, TL::by_row(rows, 32 * i * TL::ROWB, s), qf[s]);
+          mma(dp, TL::by_row(rows, TL::BYTES + 32 * i * TL::ROWB, s), gf[s]);
         }
+        read_ahead<T, false, 2 * (D / 16), 4>();
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float pe = __builtin_amdgcn_exp2f(sc[e] * c - lse);
-          sc[e] = key0 + 32 * i + frag_row(e, ln) <= q ? pe * (dp[e] - delta) : 0.f;
-        }
+        for (int e = 0; e < 16; ++e) sc[e] = __builtin_amdgcn_exp2f(sc[e] * c - lse) * (dp[e] - delta);
+        if (key0 + 32 * i + 31 > q0)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (key0 + 32 * i + frag_row(e, lane) > q) sc[e] = 0.f;
         from_acc(ds[0], sc, 0);
         from_acc(ds[1], sc, 1);
       }
       if (scrub) {  // the scores are made of the keys as they are
         lds_barrier();
-        if (wave >> 1 == i) tile_finite<T, D, true>(kt(buf), wave, ln);
+        if (wave >> 1 == i) tile_finite<T, D, true>(kt(buf), wave, lane);
         lds_barrier();
       }
       if (mine) {
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
-          for (int m = 0; m < D / 32; ++m) mma(acc[m], TL::by_col(kt(buf), 32 * i + 16 * s, 32 * m, ln), ds[s]);
-        if (scrub) add_odd<T, D>(acc, kb, a.ks[2], key0 + 32 * i, p.len, a.d, ds, ln, [&](int row) { return row <= q; });
+          for (int m = 0; m < D / 32; ++m) mma(acc[m], TL::by_col(cols, (32 * i + 16 * s) * TL::ROWB, m), ds[s]);
+        read_ahead<T, true, 2 * (D / 32), 4>();
+        if (scrub) add_odd<T, D>(acc, kb, a.ks[2], key0 + 32 * i, p.len, a.d, ds, lane, [&](int row) { return row <= q; });
       }
     }
   }
@@ -499,7 +538,7 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
 }
 
 // A workgroup owns 64 keys: two waves of 32 take the first half of a tile's queries, two the second; their sums meet at the end.
-template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dkv_kernel(Args a) {
+template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 && D == 64 ? 2 : 1) void attn_dkv_kernel(Args a) {
   typedef Tile<T, D> TL;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const auto qt = [](int buf) { return reinterpret_cast<T*>(lds + 2 * buf * TL::BYTES); };
@@ -538,13 +577,14 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
   for (int i = 0; i < D / 32; ++i)
 #pragma unroll
     for (int e = 0; e < 16; ++e) dk[i][e] = dv[i][e] = 0.f;
+  const unsigned row_addr = lds_byte_addr(lds) + r0 * TL::ROWB + TL::rows(lane), col_addr = lds_byte_addr(lds) + r0 * TL::ROWB + TL::cols(lane);
   for (int it = 0; it < total; ++it) {
     const int buf = it & 1;
-    const int ln = fresh(lane);  // LDS addresses are formed again where they are used: kept over the loop they cost the accumulators' registers
+    const unsigned rows = fresh(row_addr) + 2 * buf * TL::BYTES, cols = fresh(col_addr) + 2 * buf * TL::BYTES;  // what is formed from them is formed where it is used
     dma_wait<0>();
     const bool edge = row0 == p.blk * ROWS || row0 + ROWS > p.len;
     const int next_h = row0 + ROWS >= p.len ? h + 1 : h, next_row0 = next_h == h ? row0 + ROWS : p.blk * ROWS;
-    if (edge && !(tile_finite<T, D, false>(qt(buf), wave, ln) && tile_finite<T, D, false>(gt(buf), wave, ln))) odd[buf] = 1;
+    if (edge && !(tile_finite<T, D, false>(qt(buf), wave, lane) && tile_finite<T, D, false>(gt(buf), wave, lane))) odd[buf] = 1;
     lds_barrier();
     if (it + 1 < total) fetch(next_h, next_row0, buf ^ 1);
     const bool mine = row0 + r0 + 31 >= key0 && row0 + r0 < p.len, scrub = edge && odd[buf];
@@ -555,28 +595,32 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
 #pragma unroll
       for (int e = 0; e < 16; ++e) sc[e] = dp[e] = 0.f;
 #pragma unroll
-      for (int s = 0; s < D / 16; ++s) mma(sc, TL::by_row(qt(buf), r0, 16 * s, ln), kf[s]);
+      for (int s = 0; s < D / 16; ++s) mma(sc, TL::by_row(rows, 0, s), kf[s]);
 #pragma unroll
-      for (int s = 0; s < D / 16; ++s) mma(dp, TL::by_row(gt(buf), r0, 16 * s, ln), vf[s]);
+      for (int s = 0; s < D / 16; ++s) mma(dp, TL::by_row(rows, TL::BYTES, s), vf[s]);
+      read_ahead<T, false, 2 * (D / 16), 4>();
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const floatx4 lse = load4(st + 8 * g + 4 * kg), delta = load4(st + 64 + 8 * g + 4 * kg);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int q = row0 + r0 + 8 * g + 4 * kg + e;
-          const bool on = q >= key && q < p.len;
-          const float pe = on ? __builtin_amdgcn_exp2f(sc[4 * g + e] * c - lse[e]) : 0.f;
-          sc[4 * g + e] = pe;
-          dp[4 * g + e] = on ? pe * (dp[4 * g + e] - delta[e]) : 0.f;
+          sc[4 * g + e] = __builtin_amdgcn_exp2f(sc[4 * g + e] * c - lse[e]);
+          dp[4 * g + e] = sc[4 * g + e] * (dp[4 * g + e] - delta[e]);
         }
       }
+      if (edge)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int q = row0 + r0 + frag_row(e, lane);
+          if (q < key || q >= p.len) sc[e] = dp[e] = 0.f;
+        }
 #pragma unroll
       for (int s = 0; s < 2; ++s) from_acc(pf[s], sc, s), from_acc(ds[s], dp, s);
     }
     if (scrub) {  // the scores are made of the queries and gradients as they are
       lds_barrier();
-      tile_finite<T, D, true>(qt(buf), wave, ln);
-      tile_finite<T, D, true>(gt(buf), wave, ln);
+      tile_finite<T, D, true>(qt(buf), wave, lane);
+      tile_finite<T, D, true>(gt(buf), wave, lane);
       lds_barrier();
     }
     if (mine) {
@@ -584,13 +628,14 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
       for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int m = 0; m < D / 32; ++m) {
-          mma(dv[m], TL::by_col(gt(buf), r0 + 16 * s, 32 * m, ln), pf[s]);
-          mma(dk[m], TL::by_col(qt(buf), r0 + 16 * s, 32 * m, ln), ds[s]);
+          mma(dv[m], TL::by_col(cols, TL::BYTES + 16 * s * TL::ROWB, m), pf[s]);
+          mma(dk[m], TL::by_col(cols, 16 * s * TL::ROWB, m), ds[s]);
         }
+      read_ahead<T, true, 4 * (D / 32), 4>();
       if (scrub) {
         const auto keep = [&](int row) { return row >= key; };
-        add_odd<T, D>(dv, at<T>(a.dout, a.gs, p.b, h, p.tok), a.gs[2], row0 + r0, p.len, a.d, pf, ln, keep);
-        add_odd<T, D>(dk, at<T>(a.q, a.qs, p.b, h, p.tok), a.qs[2], row0 + r0, p.len, a.d, ds, ln, keep);
+        add_odd<T, D>(dv, at<T>(a.dout, a.gs, p.b, h, p.tok), a.gs[2], row0 + r0, p.len, a.d, pf, lane, keep);
+        add_odd<T, D>(dk, at<T>(a.q, a.qs, p.b, h, p.tok), a.qs[2], row0 + r0, p.len, a.d, ds, lane, keep);
       }
     }
     h = next_h;
@@ -783,6 +828,7 @@ template <typename T, int D> __global__ __launch_bounds__(64 * step_waves<T>(), 
     if (tile + step < ntile) fetch(tile + step, buf ^ 1);
     if (tile + step < ntile - 1) dma_wait<2 * NI>();
     else dma_wait<0>();  // the last tile may be short of rows, and of loads
+    const unsigned rows = lds_byte_addr(kt(buf)) + TL::rows(lane), cols = lds_byte_addr(kt(buf)) + TL::cols(lane);
     if (tile == ntile - 1 && ct == 0) {  // the new token's place
       T* kw = const_cast<T*>(kc) + (int64_t)len * a.kcs[2];
       T* vw = const_cast<T*>(vc) + (int64_t)len * a.vcs[2];
@@ -792,7 +838,7 @@ template <typename T, int D> __global__ __launch_bounds__(64 * step_waves<T>(), 
 #pragma unroll
     for (int e = 0; e < 16; ++e) sc[e] = 0.f;
 #pragma unroll
-    for (int s = 0; s < D / 16; ++s) mma(sc, TL::by_row(kt(buf), 0, 16 * s, lane), qf[s]);
+    for (int s = 0; s < D / 16; ++s) mma(sc, TL::by_row(rows, 0, s), qf[s]);
     float top = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
@@ -818,7 +864,7 @@ template <typename T, int D> __global__ __launch_bounds__(64 * step_waves<T>(), 
       Frag8<T> pf;
       from_acc(pf, sc, s);
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) mma(acc[i], TL::by_col(vt(buf), 16 * s, 32 * i, lane), pf);
+      for (int i = 0; i < D / 32; ++i) mma(acc[i], TL::by_col(cols, TL::BYTES + 16 * s * TL::ROWB, i), pf);
     }
   }
   // the waves' sums, and this workgroup's share of the result
