@@ -122,19 +122,42 @@ template <int D, int R> struct Tile<float, D, R> {
   }
 };
 
-// Rows row0 .. row0 + 63 of a [len][d] matrix with row stride `st`, by the workgroup's four waves; rows behind the last are copies of
-// the last, columns behind d keep the zeros that clear_tiles left.
-template <typename T, int D> __device__ __forceinline__ void fetch_tile(T* tile, const T* base, int64_t st, int row0, int len, int d, int wave, int lane) {
-  typedef Tile<T, D> TL;
-  constexpr int N = TL::BYTES / 1024 / 4;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int j = wave * N + i;
-    int r, c;
-    TL::src(j, lane, r, c);
-    if (c < d) dma16(base + (int64_t)min(row0 + r, len - 1) * st + c, lds_byte_addr(tile) + 1024 * j);
-  }
+// 16 bytes a lane from `base` + off bytes straight to LDS, lane l at dst + 16 l; the base is the wave's, so a tile's loads cost no
+// vector arithmetic
+__device__ __forceinline__ void dma16_at(const void* base, unsigned off, unsigned dst) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(__builtin_amdgcn_readfirstlane(dst)) : "memory", "m0");
 }
+// Brings tiles of [len][d] matrices with one row stride to LDS by the workgroup's four waves: which bytes a lane fetches is formed once.
+template <typename T, int D> struct Mover {
+  typedef Tile<T, D> TL;
+  static constexpr int N = TL::BYTES / 1024 / 4;
+  unsigned off[N];
+  int64_t st;
+  int d, lane, wave;
+  __device__ __forceinline__ Mover(int64_t st_, int d_, int wave_, int lane_) : st(st_), d(d_), lane(lane_), wave(wave_) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      int r, c;
+      TL::src(wave * N + i, lane, r, c);
+      off[i] = (unsigned)((r * (int)st + c) * (int)sizeof(T));
+    }
+  }
+  // rows row0 .. row0 + 63; rows behind the last are copies of the last, columns behind d keep the zeros that clear_lds left
+  __device__ __forceinline__ void fetch(unsigned tile, const T* matrix, int row0, int len) const {
+    if (row0 + ROWS <= len && d == D) {
+      const T* base = matrix + (int64_t)row0 * st;
+#pragma unroll
+      for (int i = 0; i < N; ++i) dma16_at(base, off[i], tile + 1024 * (wave * N + i));
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < N; ++i) {
+        int r, c;
+        TL::src(wave * N + i, lane, r, c);
+        if (c < d) dma16(matrix + (int64_t)min(row0 + r, len - 1) * st + c, tile + 1024 * (wave * N + i));
+      }
+    }
+  }
+};
 __device__ __forceinline__ bool is_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 // Whether the granules that this lane's loads brought hold finite values only; SCRUB: the others become 0.  A wave's granules are
 // rows 16 wave .. 16 wave + 15.
@@ -300,8 +323,10 @@ template <typename T, int D, int NQ> __global__ __launch_bounds__(256, sizeof(T)
   if (a.d < D) clear_lds(lds, 4 * TL::BYTES);
   if (threadIdx.x < 2) odd[threadIdx.x] = 0;
   lds_barrier();
-  fetch_tile<T, D>(kt(0), kb, a.ks[2], 0, p.len, a.d, wave, lane);
-  fetch_tile<T, D>(vt(0), vb, a.vs[2], 0, p.len, a.d, wave, lane);
+  const Mover<T, D> mk(a.ks[2], a.d, wave, lane), mv(a.vs[2], a.d, wave, lane);
+  const unsigned lds0 = lds_byte_addr(lds);
+  mk.fetch(lds0, kb, 0, p.len);
+  mv.fetch(lds0 + TL::BYTES, vb, 0, p.len);
   // queries as B operands; a negative scale turns their sign, so that the largest product has the largest score
   const float c = fmaxf(fabsf(a.scale) * LOG2E, 1e-30f);  // above 0: -inf stays what a masked score is
   Frag8<T> qf[NQ][D / 16];
@@ -328,7 +353,7 @@ template <typename T, int D, int NQ> __global__ __launch_bounds__(256, sizeof(T)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[t][i][e] = 0.f;
   }
-  const unsigned row_addr = lds_byte_addr(lds) + TL::rows(lane), col_addr = lds_byte_addr(lds) + TL::cols(lane);
+  const unsigned row_addr = lds0 + TL::rows(lane), col_addr = lds0 + TL::cols(lane);
   for (int it = 0; it < ntile; ++it) {
     const int key0 = it * ROWS, buf = it & 1;
     const unsigned rows = row_addr + 2 * buf * TL::BYTES, cols = col_addr + 2 * buf * TL::BYTES;
@@ -337,8 +362,8 @@ template <typename T, int D, int NQ> __global__ __launch_bounds__(256, sizeof(T)
     if (edge && !tile_finite<T, D, true>(vt(buf), wave, lane)) odd[buf] = 1;
     lds_barrier();
     if (it + 1 < ntile) {
-      fetch_tile<T, D>(kt(buf ^ 1), kb, a.ks[2], key0 + ROWS, p.len, a.d, wave, lane);
-      fetch_tile<T, D>(vt(buf ^ 1), vb, a.vs[2], key0 + ROWS, p.len, a.d, wave, lane);
+      mk.fetch(lds0 + 2 * (buf ^ 1) * TL::BYTES, kb, key0 + ROWS, p.len);
+      mv.fetch(lds0 + (2 * (buf ^ 1) + 1) * TL::BYTES, vb, key0 + ROWS, p.len);
     }
     if (key0 >= q0 + 32 * NQ) continue;  // behind all of this wave's queries
     floatx16 sc[NQ][2];
@@ -465,8 +490,10 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
   if (a.d < D) clear_lds(lds, 4 * TL::BYTES);
   if (threadIdx.x < 2) odd[threadIdx.x] = 0;
   lds_barrier();
-  fetch_tile<T, D>(kt(0), kb, a.ks[2], 0, p.len, a.d, wave, lane);
-  fetch_tile<T, D>(vt(0), vb, a.vs[2], 0, p.len, a.d, wave, lane);
+  const Mover<T, D> mk(a.ks[2], a.d, wave, lane), mv(a.vs[2], a.d, wave, lane);
+  const unsigned lds0 = lds_byte_addr(lds);
+  mk.fetch(lds0, kb, 0, p.len);
+  mv.fetch(lds0 + TL::BYTES, vb, 0, p.len);
   const float c = a.scale * LOG2E;
   const int64_t row = min(q, p.len - 1), stat = ((int64_t)p.b * a.H + h) * a.T + p.tok + row;
   const float lse = a.lse[stat], delta = a.delta[stat];
@@ -483,7 +510,7 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
   for (int i = 0; i < D / 32; ++i)
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
-  const unsigned row_addr = lds_byte_addr(lds) + TL::rows(lane), col_addr = lds_byte_addr(lds) + TL::cols(lane);
+  const unsigned row_addr = lds0 + TL::rows(lane), col_addr = lds0 + TL::cols(lane);
   for (int it = 0; it < ntile; ++it) {
     const int key0 = it * ROWS, buf = it & 1;
     const unsigned rows = row_addr + 2 * buf * TL::BYTES, cols = col_addr + 2 * buf * TL::BYTES;
@@ -492,8 +519,8 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
     if (edge && !tile_finite<T, D, false>(kt(buf), wave, lane)) odd[buf] = 1;
     lds_barrier();
     if (it + 1 < ntile) {
-      fetch_tile<T, D>(kt(buf ^ 1), kb, a.ks[2], key0 + ROWS, p.len, a.d, wave, lane);
-      fetch_tile<T, D>(vt(buf ^ 1), vb, a.vs[2], key0 + ROWS, p.len, a.d, wave, lane);
+      mk.fetch(lds0 + 2 * (buf ^ 1) * TL::BYTES, kb, key0 + ROWS, p.len);
+      mv.fetch(lds0 + (2 * (buf ^ 1) + 1) * TL::BYTES, vb, key0 + ROWS, p.len);
     }
     const bool scrub = edge && odd[buf];
 #pragma unroll
@@ -553,9 +580,11 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 &&
   if (a.d < D) clear_lds(lds, 4 * TL::BYTES);
   if (threadIdx.x < 2) odd[threadIdx.x] = 0;
   lds_barrier();
+  const Mover<T, D> mq(a.qs[2], a.d, wave, lane), mg(a.gs[2], a.d, wave, lane);
+  const unsigned lds0 = lds_byte_addr(lds);
   auto fetch = [&](int h, int row0, int buf) {
-    fetch_tile<T, D>(qt(buf), at<T>(a.q, a.qs, p.b, h, p.tok), a.qs[2], row0, p.len, a.d, wave, lane);
-    fetch_tile<T, D>(gt(buf), at<T>(a.dout, a.gs, p.b, h, p.tok), a.gs[2], row0, p.len, a.d, wave, lane);
+    mq.fetch(lds0 + 2 * buf * TL::BYTES, at<T>(a.q, a.qs, p.b, h, p.tok), row0, p.len);
+    mg.fetch(lds0 + (2 * buf + 1) * TL::BYTES, at<T>(a.dout, a.gs, p.b, h, p.tok), row0, p.len);
     const int64_t stat = ((int64_t)p.b * a.H + h) * a.T + p.tok + min(row0 + lane, p.len - 1);
     if (wave == 0) dma4(a.lse + stat, lds_byte_addr(stats + buf * 128));
     if (wave == 1) dma4(a.delta + stat, lds_byte_addr(stats + buf * 128 + 64));
@@ -577,7 +606,7 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 &&
   for (int i = 0; i < D / 32; ++i)
 #pragma unroll
     for (int e = 0; e < 16; ++e) dk[i][e] = dv[i][e] = 0.f;
-  const unsigned row_addr = lds_byte_addr(lds) + r0 * TL::ROWB + TL::rows(lane), col_addr = lds_byte_addr(lds) + r0 * TL::ROWB + TL::cols(lane);
+  const unsigned row_addr = lds0 + r0 * TL::ROWB + TL::rows(lane), col_addr = lds0 + r0 * TL::ROWB + TL::cols(lane);
   for (int it = 0; it < total; ++it) {
     const int buf = it & 1;
     const unsigned rows = fresh(row_addr) + 2 * buf * TL::BYTES, cols = fresh(col_addr) + 2 * buf * TL::BYTES;  // what is formed from them is formed where it is used
@@ -667,8 +696,9 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 &&
 
 int64_t blocks_of(const lnx_attn_args* a, int size) { return a->nseq ? (int64_t)a->T / size + a->nseq : ((int64_t)a->T + size - 1) / size; }
 
+// Rows that the kernels move as vectors, 64 of them within the 31 bits of a lane's offset
 bool rows_fit(const lnx_tensor4* t, int64_t size) {
-  return reinterpret_cast<uintptr_t>(t->p) % 16 == 0 && t->stride_b * size % 16 == 0 && t->stride_h * size % 16 == 0 && t->stride_t * size % 16 == 0;
+  return t->stride_t >= 0 && t->stride_t * size <= (int64_t)1 << 24 && reinterpret_cast<uintptr_t>(t->p) % 16 == 0 && t->stride_b * size % 16 == 0 && t->stride_h * size % 16 == 0 && t->stride_t * size % 16 == 0;
 }
 
 int check(const char* what, const lnx_attn_args* a, bool bwd) {
@@ -683,7 +713,7 @@ int check(const char* what, const lnx_attn_args* a, bool bwd) {
   const lnx_tensor4* ts[] = {&a->q, &a->k, &a->v, &a->o, &a->d_o, &a->d_q, &a->d_k, &a->d_v};
   for (int i = 0; i < (bwd ? 8 : 4); ++i) {
     if (!ts[i]->p) return lnx_set_error(LNX_ERR_NULL, "%s: a tensor is missing", what);
-    if (!rows_fit(ts[i], a->dtype == LNX_BF16 ? 2 : 4)) return lnx_set_error(LNX_ERR_SHAPE, "%s: tensors must be 16-byte aligned, rows whole numbers of 16 bytes apart", what);
+    if (!rows_fit(ts[i], a->dtype == LNX_BF16 ? 2 : 4)) return lnx_set_error(LNX_ERR_SHAPE, "%s: tensors must be 16-byte aligned, rows whole numbers of 16 bytes and at most 16 MiB apart", what);
   }
   if (bwd && (!a->lse || !a->workspace || a->workspace_bytes < lnx_attn_bwd_workspace_bytes(a)))
     return lnx_set_error(LNX_ERR_WORKSPACE, "%s: lse and a workspace of %llu bytes are required", what, (unsigned long long)lnx_attn_bwd_workspace_bytes(a));
@@ -958,10 +988,10 @@ int check_step(const lnx_attn_step_args* a) {
   const lnx_tensor4* ts[] = {&a->q, &a->k, &a->v, &a->k_cache, &a->v_cache};
   for (const lnx_tensor4* t : ts) {
     if (!t->p) return lnx_set_error(LNX_ERR_NULL, "%s: a tensor is missing", what);
-    if (!rows_fit(t, a->dtype == LNX_BF16 ? 2 : 4)) return lnx_set_error(LNX_ERR_SHAPE, "%s: tensors must be 16-byte aligned, rows whole numbers of 16 bytes apart", what);
+    if (!rows_fit(t, a->dtype == LNX_BF16 ? 2 : 4)) return lnx_set_error(LNX_ERR_SHAPE, "%s: tensors must be 16-byte aligned, rows whole numbers of 16 bytes and at most 16 MiB apart", what);
   }
   if (!a->o || !a->lengths) return lnx_set_error(LNX_ERR_NULL, "%s: o and lengths are required", what);
-  if (reinterpret_cast<uintptr_t>(a->o) % 16) return lnx_set_error(LNX_ERR_SHAPE, "%s: tensors must be 16-byte aligned, rows whole numbers of 16 bytes apart", what);
+  if (reinterpret_cast<uintptr_t>(a->o) % 16) return lnx_set_error(LNX_ERR_SHAPE, "%s: tensors must be 16-byte aligned, rows whole numbers of 16 bytes and at most 16 MiB apart", what);
   if ((int64_t)a->B * a->H * step_splits(a) > 0x7fffffff) return lnx_set_error(LNX_ERR_SHAPE, "%s: too many rows", what);
   const uint64_t need = lnx_attn_step_workspace_bytes(a);
   if (need && (!a->workspace || a->workspace_bytes < need)) return lnx_set_error(LNX_ERR_WORKSPACE, "%s: needs a workspace of %llu bytes", what, (unsigned long long)need);

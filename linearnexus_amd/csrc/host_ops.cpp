@@ -1349,8 +1349,10 @@ PyObject* py_linrec_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 // causal attention
 // ---------------------------------------------------------------------------------------------------------------
 
-// [B, H, T, d] (or [B, H, d]) tensors as the kernels read and write them: any strides that are whole numbers of 16 bytes
+// [B, H, T, d] (or [B, H, d]) tensors as the kernels read and write them: any strides that are whole numbers of 16 bytes, tokens at most
+// 16 MiB apart
 bool vector_rows(const Tensor& t) {
+  if (t.dim() == 4 && t.stride(2) * t.element_size() > (int64_t)1 << 24) return false;
   if (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 || (t.size(-1) != 1 && t.stride(-1) != 1)) return false;
   for (int64_t i = 0; i + 1 < t.dim(); ++i)
     if (t.stride(i) * t.element_size() % 16) return false;
