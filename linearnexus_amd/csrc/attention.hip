@@ -88,6 +88,7 @@ template <int D, int R> struct Tile<bf16_t, D, R> {
     const int s = lane & 15, grp = lane >> 4;
     return 2 * S::at(4 * (grp >> 1) + (s >> 2), 16 * (grp & 1) + 4 * (s & 3));
   }
+  static __device__ __forceinline__ unsigned col_block(unsigned cols, int m) { return cols ^ (64 * m); }  // by_col's m counts from there
   static __device__ __forceinline__ Frag8<bf16_t> by_col(unsigned cols, int off, int m) {
     typedef short short4_ __attribute__((ext_vector_type(4)));
     typedef short short8_ __attribute__((ext_vector_type(8)));
@@ -114,6 +115,7 @@ template <int D, int R> struct Tile<float, D, R> {
     return {{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}};
   }
   static __device__ __forceinline__ unsigned cols(int lane) { return 4 * at(4 * (lane >> 5), lane & 31); }
+  static __device__ __forceinline__ unsigned col_block(unsigned cols, int m) { return cols + 128 * m; }
   static __device__ __forceinline__ Frag8<float> by_col(unsigned cols, int off, int m) {
     Frag8<float> f;
 #pragma unroll
@@ -204,8 +206,8 @@ __device__ __forceinline__ float half_max(float x) {
 // A product over the rows of a tile takes masked pairs with weight 0, and 0 times a value that is not finite is not 0: such values
 // are scrubbed from the tile, and their part of the product is added here, pair by pair and only where keep(row) lets this lane's
 // column have it.  w: the weights of the 32 rows from row0 on, as an operand; the values are read again from memory.
-template <typename T, int D, typename F>
-__device__ __forceinline__ void add_odd(floatx16 (&acc)[D / 32], const T* base, int64_t st, int row0, int len, int d, const Frag8<T> (&w)[2], int lane, F keep) {
+template <typename T, int M, typename F>
+__device__ __forceinline__ void add_odd(floatx16 (&acc)[M], const T* base, int64_t st, int row0, int len, int d, const Frag8<T> (&w)[2], int lane, F keep) {
   const int kg = lane >> 5;
 #pragma unroll 1
   for (int j = 0; j < 32 && row0 + j < len; ++j) {
@@ -218,7 +220,7 @@ __device__ __forceinline__ void add_odd(floatx16 (&acc)[D / 32], const T* base, 
     const bool on = keep(row0 + j);
     const T* r = base + (int64_t)(row0 + j) * st + 4 * kg;
 #pragma unroll
-    for (int m = 0; m < D / 32; ++m)
+    for (int m = 0; m < M; ++m)
 #pragma unroll
       for (int q = 0; q < 4; ++q)
         if (32 * m + 8 * q + 4 * kg < d) {
@@ -295,10 +297,10 @@ template <typename T> __device__ __forceinline__ T* at(const void* p, const int6
   return const_cast<T*>(static_cast<const T*>(p)) + b * s[0] + h * s[1] + t * s[2];
 }
 
-// One column's D values from accumulators over rows, times f: the lane writes four consecutive elements at a time
-template <typename T, int D> __device__ __forceinline__ void store_column(T* p, const floatx16 (&acc)[D / 32], float f, int d, int lane) {
+// One column's 32 M values from accumulators over rows, the first d of them, times f: the lane writes four consecutive elements at a time
+template <typename T, int M> __device__ __forceinline__ void store_column(T* p, const floatx16 (&acc)[M], float f, int d, int lane) {
 #pragma unroll
-  for (int m = 0; m < D / 32; ++m)
+  for (int m = 0; m < M; ++m)
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const int c = 32 * m + 8 * q + 4 * (lane >> 5);
@@ -439,7 +441,7 @@ template <typename T, int D, int NQ> __global__ __launch_bounds__(256, sizeof(T)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const Frag8<T> two[2] = {pf[t][2 * i], pf[t][2 * i + 1]};
-          add_odd<T, D>(acc[t], vb, a.vs[2], key0 + 32 * i, p.len, a.d, two, lane, [&](int row) { return row <= q0 + 32 * t + n; });
+          add_odd<T, D / 32>(acc[t], vb, a.vs[2], key0 + 32 * i, p.len, a.d, two, lane, [&](int row) { return row <= q0 + 32 * t + n; });
         }
     }
   }
@@ -448,7 +450,7 @@ template <typename T, int D, int NQ> __global__ __launch_bounds__(256, sizeof(T)
     const int q = q0 + 32 * t + n;
     const float sum = xor32_sum(l[t]);
     if (q < p.len) {
-      store_column<T, D>(at<T>(a.o, a.os, p.b, h, p.tok + q), acc[t], 1.f / sum, a.d, lane);
+      store_column<T, D / 32>(at<T>(a.o, a.os, p.b, h, p.tok + q), acc[t], 1.f / sum, a.d, lane);
       if (a.lse && kg == 0) a.lse[((int64_t)p.b * a.H + h) * a.T + p.tok + q] = m[t] * c + __builtin_amdgcn_logf(sum);
     }
   }
@@ -557,40 +559,76 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
 #pragma unroll
           for (int m = 0; m < D / 32; ++m) mma(acc[m], TL::by_col(cols, (32 * i + 16 * s) * TL::ROWB, m), ds[s]);
         read_ahead<T, true, 2 * (D / 32), 4>();
-        if (scrub) add_odd<T, D>(acc, kb, a.ks[2], key0 + 32 * i, p.len, a.d, ds, lane, [&](int row) { return row <= q; });
+        if (scrub) add_odd<T, D / 32>(acc, kb, a.ks[2], key0 + 32 * i, p.len, a.d, ds, lane, [&](int row) { return row <= q; });
       }
     }
   }
-  if (q < p.len) store_column<T, D>(at<T>(a.dq, a.dqs, p.b, h, p.tok + q), acc, a.scale, a.d, lane);
+  if (q < p.len) store_column<T, D / 32>(at<T>(a.dq, a.dqs, p.b, h, p.tok + q), acc, a.scale, a.d, lane);
 }
 
-// A workgroup owns 64 keys: two waves of 32 take the first half of a tile's queries, two the second; their sums meet at the end.
-template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 && D == 64 ? 2 : 1) void attn_dkv_kernel(Args a) {
+// An operand through LDS to another wave of the workgroup
+template <typename T> __device__ __forceinline__ void leave_frag(unsigned at, const Frag8<T>& f, int lane) {
+  typedef __attribute__((address_space(3))) floatx4 lds_float4;
+  const floatx4* v = reinterpret_cast<const floatx4*>(&f);
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) *(lds_float4*)(lds_char*)(uintptr_t)(at + 1024 * i + 16 * lane) = v[i];
+}
+template <typename T> __device__ __forceinline__ void take_frag(unsigned at, Frag8<T>& f, int lane) {
+  floatx4* v = reinterpret_cast<floatx4*>(&f);
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = lds_load<floatx4>(at + 1024 * i + 16 * lane);
+}
+
+// A workgroup owns 64 keys.  Wave (kw, qw) forms the weights of 32 keys and the half qw of a tile's queries, hands them to the wave of
+// the other half, and adds up the half qw of the columns of dk and dv over all queries: accumulators of half the size, so that two
+// workgroups share a CU (both halves in every wave took 416 registers, one workgroup a CU and 1.6 times as long).  The LDS of a
+// workgroup is 80 KB to the byte: the queries' lse and delta go straight to registers, a flag crosses in the hand-over's place.
+template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dkv_kernel(Args a) {
   typedef Tile<T, D> TL;
+  typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
+  constexpr int M = D / 64, FRAG = 1024 * (int)sizeof(T) / 2;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const auto qt = [](int buf) { return reinterpret_cast<T*>(lds + 2 * buf * TL::BYTES); };
   const auto gt = [](int buf) { return reinterpret_cast<T*>(lds + (2 * buf + 1) * TL::BYTES); };
-  float* stats = reinterpret_cast<float*>(lds + 4 * TL::BYTES);  // [buffer][lse, delta][64]
-  int* odd = reinterpret_cast<int*>(stats + 256);
   const Place p = place(a, ROWS, 1, false);
   if (!p.on) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, kg = lane >> 5;
-  const int kw = wave & 1, r0 = 32 * (wave >> 1), key0 = p.blk * ROWS + 32 * kw, key = key0 + n;
+  const int kw = wave & 1, qw = wave >> 1, r0 = 32 * qw, key0 = p.blk * ROWS + 32 * kw, key = key0 + n;
   const int total = ((p.len + ROWS - 1) / ROWS - p.blk) * a.G;
-  if (a.d < D) clear_lds(lds, 4 * TL::BYTES);
-  if (threadIdx.x < 2) odd[threadIdx.x] = 0;
-  lds_barrier();
+  if (a.d < D) {
+    clear_lds(lds, 4 * TL::BYTES);
+    lds_barrier();
+  }
   const Mover<T, D> mq(a.qs[2], a.d, wave, lane), mg(a.gs[2], a.d, wave, lane);
-  const unsigned lds0 = lds_byte_addr(lds);
+  const unsigned lds0 = lds_byte_addr(lds), mine = lds0 + 4 * TL::BYTES + 4 * FRAG * wave, theirs = lds0 + 4 * TL::BYTES + 4 * FRAG * (wave ^ 2);
+  floatx4 lse[4], delta[4];
+  auto fetch_stats = [&](int h, int row0) {
+    const int64_t first = ((int64_t)p.b * a.H + h) * a.T + p.tok;
+    const int row = row0 + r0 + 4 * kg;
+    if (row0 + ROWS <= p.len) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        lse[g] = *reinterpret_cast<const float4u*>(a.lse + first + row + 8 * g);
+        delta[g] = *reinterpret_cast<const float4u*>(a.delta + first + row + 8 * g);
+      }
+    } else {
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int64_t at = first + min(row + 8 * g + e, p.len - 1);
+          lse[g][e] = a.lse[at];
+          delta[g][e] = a.delta[at];
+        }
+    }
+  };
   auto fetch = [&](int h, int row0, int buf) {
     mq.fetch(lds0 + 2 * buf * TL::BYTES, at<T>(a.q, a.qs, p.b, h, p.tok), row0, p.len);
     mg.fetch(lds0 + (2 * buf + 1) * TL::BYTES, at<T>(a.dout, a.gs, p.b, h, p.tok), row0, p.len);
-    const int64_t stat = ((int64_t)p.b * a.H + h) * a.T + p.tok + min(row0 + lane, p.len - 1);
-    if (wave == 0) dma4(a.lse + stat, lds_byte_addr(stats + buf * 128));
-    if (wave == 1) dma4(a.delta + stat, lds_byte_addr(stats + buf * 128 + 64));
   };
   int h = p.hkv * a.G, row0 = p.blk * ROWS;  // the tile being multiplied
   fetch(h, row0, 0);
+  fetch_stats(h, row0);
   const float c = a.scale * LOG2E;
   const int64_t krow = p.tok + min(key, p.len - 1);
   const T* kr = at<T>(a.k, a.ks, p.b, p.hkv, krow);
@@ -601,25 +639,37 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 &&
     from_global<T>(kf[s], kr + 16 * s + 8 * kg, 16 * s + 8 * kg < a.d);
     from_global<T>(vf[s], vr + 16 * s + 8 * kg, 16 * s + 8 * kg < a.d);
   }
-  floatx16 dk[D / 32], dv[D / 32];
+  floatx16 dk[M], dv[M];
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i)
+  for (int i = 0; i < M; ++i)
 #pragma unroll
     for (int e = 0; e < 16; ++e) dk[i][e] = dv[i][e] = 0.f;
-  const unsigned row_addr = lds0 + r0 * TL::ROWB + TL::rows(lane), col_addr = lds0 + r0 * TL::ROWB + TL::cols(lane);
+  const unsigned row_addr = lds0 + r0 * TL::ROWB + TL::rows(lane), col_addr = TL::col_block(lds0 + TL::cols(lane), M * qw);
   for (int it = 0; it < total; ++it) {
     const int buf = it & 1;
-    const unsigned rows = fresh(row_addr) + 2 * buf * TL::BYTES, cols = fresh(col_addr) + 2 * buf * TL::BYTES;  // what is formed from them is formed where it is used
     dma_wait<0>();
+#pragma unroll
+    for (int g = 0; g < 4; ++g) asm volatile("" : "+v"(lse[g]), "+v"(delta[g]));  // have come too: no wait for the next tile at their use
     const bool edge = row0 == p.blk * ROWS || row0 + ROWS > p.len;
     const int next_h = row0 + ROWS >= p.len ? h + 1 : h, next_row0 = next_h == h ? row0 + ROWS : p.blk * ROWS;
-    if (edge && !(tile_finite<T, D, false>(qt(buf), wave, lane) && tile_finite<T, D, false>(gt(buf), wave, lane))) odd[buf] = 1;
     lds_barrier();
+    bool scrub = false;
+    if (edge) {
+      const bool ok = tile_finite<T, D, false>(qt(buf), wave, lane) && tile_finite<T, D, false>(gt(buf), wave, lane);
+      typedef __attribute__((address_space(3))) int lds_int;
+      const int all = __all(ok);
+      if (lane == 0) *(lds_int*)(lds_char*)(uintptr_t)mine = !all;
+      lds_barrier();
+#pragma unroll
+      for (int w = 0; w < 4; ++w) scrub = scrub || lds_load<int>(lds0 + 4 * TL::BYTES + 4 * FRAG * w) != 0;
+      scrub = __builtin_amdgcn_readfirstlane(scrub);
+      lds_barrier();
+    }
     if (it + 1 < total) fetch(next_h, next_row0, buf ^ 1);
-    const bool mine = row0 + r0 + 31 >= key0 && row0 + r0 < p.len, scrub = edge && odd[buf];
+    const unsigned rows = row_addr + 2 * buf * TL::BYTES, cols = col_addr + 2 * buf * TL::BYTES;
+    const auto active = [&](int q) { return row0 + 32 * q + 31 >= key0 && row0 + 32 * q < p.len; };  // some of these queries come after some of the keys
     Frag8<T> pf[2], ds[2];
-    if (mine) {  // some of these queries come after some of this wave's keys
-      const float* st = stats + buf * 128 + r0;
+    if (active(qw)) {
       floatx16 sc, dp;
 #pragma unroll
       for (int e = 0; e < 16; ++e) sc[e] = dp[e] = 0.f;
@@ -629,13 +679,9 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 &&
       for (int s = 0; s < D / 16; ++s) mma(dp, TL::by_row(rows, TL::BYTES, s), vf[s]);
       read_ahead<T, false, 2 * (D / 16), 4>();
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const floatx4 lse = load4(st + 8 * g + 4 * kg), delta = load4(st + 64 + 8 * g + 4 * kg);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          sc[4 * g + e] = __builtin_amdgcn_exp2f(sc[4 * g + e] * c - lse[e]);
-          dp[4 * g + e] = sc[4 * g + e] * (dp[4 * g + e] - delta[e]);
-        }
+      for (int e = 0; e < 16; ++e) {
+        sc[e] = __builtin_amdgcn_exp2f(sc[e] * c - lse[e >> 2][e & 3]);
+        dp[e] = sc[e] * (dp[e] - delta[e >> 2][e & 3]);
       }
       if (edge)
 #pragma unroll
@@ -644,54 +690,52 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 &&
           if (q < key || q >= p.len) sc[e] = dp[e] = 0.f;
         }
 #pragma unroll
-      for (int s = 0; s < 2; ++s) from_acc(pf[s], sc, s), from_acc(ds[s], dp, s);
+      for (int s = 0; s < 2; ++s) {
+        from_acc(pf[s], sc, s);
+        from_acc(ds[s], dp, s);
+        leave_frag<T>(mine + s * FRAG, pf[s], lane);
+        leave_frag<T>(mine + (2 + s) * FRAG, ds[s], lane);
+      }
     }
-    if (scrub) {  // the scores are made of the queries and gradients as they are
-      lds_barrier();
+    if (it + 1 < total) fetch_stats(next_h, next_row0);
+    lds_barrier();
+    if (scrub) {  // the scores were made of the queries and gradients as they are
       tile_finite<T, D, true>(qt(buf), wave, lane);
       tile_finite<T, D, true>(gt(buf), wave, lane);
       lds_barrier();
     }
-    if (mine) {
+    const auto add = [&](int half) {
+      const unsigned from = cols + 32 * half * TL::ROWB;
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
-        for (int m = 0; m < D / 32; ++m) {
-          mma(dv[m], TL::by_col(cols, TL::BYTES + 16 * s * TL::ROWB, m), pf[s]);
-          mma(dk[m], TL::by_col(cols, 16 * s * TL::ROWB, m), ds[s]);
+        for (int m = 0; m < M; ++m) {
+          mma(dv[m], TL::by_col(from, TL::BYTES + 16 * s * TL::ROWB, m), pf[s]);
+          mma(dk[m], TL::by_col(from, 16 * s * TL::ROWB, m), ds[s]);
         }
-      read_ahead<T, true, 4 * (D / 32), 4>();
+      read_ahead<T, true, 4 * M, 4>();
       if (scrub) {
         const auto keep = [&](int row) { return row >= key; };
-        add_odd<T, D>(dv, at<T>(a.dout, a.gs, p.b, h, p.tok), a.gs[2], row0 + r0, p.len, a.d, pf, lane, keep);
-        add_odd<T, D>(dk, at<T>(a.q, a.qs, p.b, h, p.tok), a.qs[2], row0 + r0, p.len, a.d, ds, lane, keep);
+        add_odd<T, M>(dv, at<T>(a.dout, a.gs, p.b, h, p.tok) + 32 * M * qw, a.gs[2], row0 + 32 * half, p.len, a.d - 32 * M * qw, pf, lane, keep);
+        add_odd<T, M>(dk, at<T>(a.q, a.qs, p.b, h, p.tok) + 32 * M * qw, a.qs[2], row0 + 32 * half, p.len, a.d - 32 * M * qw, ds, lane, keep);
       }
+    };
+    if (active(qw)) add(qw);
+    if (active(qw ^ 1)) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        take_frag<T>(theirs + s * FRAG, pf[s], lane);
+        take_frag<T>(theirs + (2 + s) * FRAG, ds[s], lane);
+      }
+      add(qw ^ 1);
     }
     h = next_h;
     row0 = next_row0;
   }
-  lds_barrier();
-  float* sums = reinterpret_cast<float*>(lds) + kw * (2 * D / 32) * 16 * 64;
-  if (wave >= 2) {
-#pragma unroll
-    for (int m = 0; m < D / 32; ++m)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        sums[((2 * m) * 16 + e) * 64 + lane] = dk[m][e];
-        sums[((2 * m + 1) * 16 + e) * 64 + lane] = dv[m][e];
-      }
-  }
-  lds_barrier();
-  if (wave >= 2 || key >= p.len) return;
-#pragma unroll
-  for (int m = 0; m < D / 32; ++m)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      dk[m][e] += sums[((2 * m) * 16 + e) * 64 + lane];
-      dv[m][e] += sums[((2 * m + 1) * 16 + e) * 64 + lane];
-    }
-  store_column<T, D>(at<T>(a.dk, a.dks, p.b, p.hkv, krow), dk, a.scale, a.d, lane);
-  store_column<T, D>(at<T>(a.dv, a.dvs, p.b, p.hkv, krow), dv, 1.f, a.d, lane);
+  if (key >= p.len) return;
+  const int c0 = 32 * M * qw;
+  store_column<T, M>(at<T>(a.dk, a.dks, p.b, p.hkv, krow) + c0, dk, a.scale, a.d - c0, lane);
+  store_column<T, M>(at<T>(a.dv, a.dvs, p.b, p.hkv, krow) + c0, dv, 1.f, a.d - c0, lane);
 }
 
 int64_t blocks_of(const lnx_attn_args* a, int size) { return a->nseq ? (int64_t)a->T / size + a->nseq : ((int64_t)a->T + size - 1) / size; }
@@ -751,7 +795,7 @@ template <typename T, int D> int launch_bwd(const lnx_attn_args* a, hipStream_t 
   lnx_profile_mark("attn_delta", st);
   attn_delta_kernel<T><<<dim3((unsigned)(((int64_t)k.B * k.H * k.T + 15) / 16)), 256, 0, st>>>(k);
   k.nblk = (int)blocks_of(a, ROWS);
-  if (int rc = start(attn_dkv_kernel<T, D>, "attn_dkv", k, (int64_t)k.B * k.Hkv * k.nblk, 4 * Tile<T, D>::BYTES + 1024 + 16, st)) return rc;
+  if (int rc = start(attn_dkv_kernel<T, D>, "attn_dkv", k, (int64_t)k.B * k.Hkv * k.nblk, 4 * Tile<T, D>::BYTES + 8192 * sizeof(T), st)) return rc;
   k.nblk = (int)blocks_of(a, 128);
   return start(attn_dq_kernel<T, D>, "attn_dq", k, (int64_t)k.B * k.H * k.nblk, 4 * Tile<T, D>::BYTES + 16, st);
 }
