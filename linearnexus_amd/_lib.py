@@ -21,7 +21,7 @@ EXPORTS = (
     "lnx_gdn_gate_fwd", "lnx_gdn_gate_bwd", "lnx_gdn_gate_bwd_workspace_bytes", "lnx_kda_gate_fwd", "lnx_kda_gate_bwd", "lnx_kda_gate_bwd_workspace_bytes", "lnx_sigmoid_fwd", "lnx_sigmoid_bwd",
     "lnx_linrec_workspace_bytes", "lnx_linrec_kept_bytes", "lnx_linrec_fwd", "lnx_linrec_bwd", "lnx_linrec_step",
     "lnx_rmsnorm_residual_bwd_workspace_bytes", "lnx_rmsnorm_residual_fwd", "lnx_rmsnorm_residual_bwd",
-    "lnx_attn_bwd_workspace_bytes", "lnx_attn_fwd", "lnx_attn_bwd", "lnx_attn_step_workspace_bytes", "lnx_attn_step",
+    "lnx_attn_fwd_workspace_bytes", "lnx_attn_bwd_workspace_bytes", "lnx_attn_fwd", "lnx_attn_bwd", "lnx_attn_step_workspace_bytes", "lnx_attn_step",
     "lnx_profile_enable", "lnx_profile_read",
 )
 
@@ -210,8 +210,9 @@ def load() -> C.CDLL:
     for name in ("lnx_rmsnorm_residual_fwd", "lnx_rmsnorm_residual_bwd"):
         getattr(lib, name).restype = C.c_int
         getattr(lib, name).argtypes = [C.POINTER(RmsnormResidualArgs), C.c_void_p]
-    lib.lnx_attn_bwd_workspace_bytes.restype = C.c_uint64
-    lib.lnx_attn_bwd_workspace_bytes.argtypes = [C.POINTER(AttnArgs)]
+    for name in ("lnx_attn_fwd_workspace_bytes", "lnx_attn_bwd_workspace_bytes"):
+        getattr(lib, name).restype = C.c_uint64
+        getattr(lib, name).argtypes = [C.POINTER(AttnArgs)]
     for name in ("lnx_attn_fwd", "lnx_attn_bwd"):
         getattr(lib, name).restype = C.c_int
         getattr(lib, name).argtypes = [C.POINTER(AttnArgs), C.c_void_p]

@@ -25,7 +25,8 @@ struct Args {
   float *lse, *delta;  // [B, H, T]; lse in units of log 2
   const int32_t* cu;
   int64_t qs[3], ks[3], vs[3], os[3], gs[3], dqs[3], dks[3], dvs[3];  // strides of batch, head, token in elements
-  int B, H, Hkv, G, T, d, nseq, nblk;
+  float *part, *part_stat;  // shares of workgroups that split a block's rows between them: [parts][rows of the result][d], [parts][rows][2]
+  int B, H, Hkv, G, T, d, nseq, nblk, parts;
   float scale;
 };
 
@@ -234,28 +235,30 @@ __device__ __forceinline__ void add_odd(floatx16 (&acc)[M], const T* base, int64
 
 // Where a workgroup works: sequence (its first token, its length), block of `size` rows, heads
 struct Place {
-  int b, hkv, g, len, blk;
+  int b, hkv, g, part, len, blk;
   int64_t tok;
   bool on;
 };
-// `per_group`: workgroups per (batch, key head, block) -- the query heads of a group, or one.  Heavy blocks first: of causal queries
+// `heads`: query heads of a group that have workgroups of their own -- all or one; each block is split into a.parts.  Heavy blocks first: of causal queries
 // the last ones (`last_first`), of keys the first ones.  Where the groups divide among the eight XCDs, workgroups of one group stay on
 // one, whose L2 then holds the group's keys and values.
-__device__ __forceinline__ Place place(const Args& a, int size, int per_group, bool last_first) {
+__device__ __forceinline__ Place place(const Args& a, int size, int heads, bool last_first) {
   Place p;
   int w = blockIdx.x, group, blk;
-  const int groups = a.B * a.Hkv, per = a.nblk * per_group;
+  const int groups = a.B * a.Hkv, per_group = heads * a.parts, per = a.nblk * per_group;
   if (groups % 8 == 0) {
     const int slot = w >> 3;
     group = (w & 7) + 8 * (slot / per);
     blk = slot % per / per_group;
-    p.g = slot % per_group;
+    w = slot % per_group;
   } else {
     blk = w / (groups * per_group);
     w -= blk * groups * per_group;
     group = w / per_group;
-    p.g = w % per_group;
+    w %= per_group;
   }
+  p.g = w / a.parts;
+  p.part = w % a.parts;
   p.b = group / a.Hkv;
   p.hkv = group % a.Hkv;
   p.tok = 0;
@@ -308,152 +311,171 @@ template <typename T, int M> __device__ __forceinline__ void store_column(T* p, 
     }
 }
 
-// A wave owns 32 NQ queries, the workgroup 128 NQ.
-template <typename T, int D, int NQ> __global__ __launch_bounds__(256, sizeof(T) == 2 && NQ == 1 ? 2 : 1) void attn_fwd_kernel(Args a) {
+// A wave owns 32 queries, the workgroup 128; of a block's key tiles every a.parts-th.
+template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kernel(Args a) {
   typedef Tile<T, D> TL;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const auto kt = [](int buf) { return reinterpret_cast<T*>(lds + 2 * buf * TL::BYTES); };
   const auto vt = [](int buf) { return reinterpret_cast<T*>(lds + (2 * buf + 1) * TL::BYTES); };
   int* odd = reinterpret_cast<int*>(lds + 4 * TL::BYTES);
-  const Place p = place(a, 128 * NQ, a.G, true);
+  const Place p = place(a, 128, a.G, true);
   if (!p.on) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, kg = lane >> 5;
-  const int h = p.hkv * a.G + p.g, q_wg = p.blk * 128 * NQ, q0 = q_wg + wave * 32 * NQ;
+  const int h = p.hkv * a.G + p.g, q_wg = p.blk * 128, q0 = q_wg + wave * 32, q = q0 + n;
   const T* kb = at<T>(a.k, a.ks, p.b, p.hkv, p.tok);
   const T* vb = at<T>(a.v, a.vs, p.b, p.hkv, p.tok);
-  const int q_end = min(q_wg + 128 * NQ, p.len), ntile = (q_end + ROWS - 1) / ROWS;
+  const int q_end = min(q_wg + 128, p.len), ntile = (q_end + ROWS - 1) / ROWS;
   if (a.d < D) clear_lds(lds, 4 * TL::BYTES);
   if (threadIdx.x < 2) odd[threadIdx.x] = 0;
   lds_barrier();
   const Mover<T, D> mk(a.ks[2], a.d, wave, lane), mv(a.vs[2], a.d, wave, lane);
   const unsigned lds0 = lds_byte_addr(lds);
-  mk.fetch(lds0, kb, 0, p.len);
-  mv.fetch(lds0 + TL::BYTES, vb, 0, p.len);
+  if (p.part < ntile) {
+    mk.fetch(lds0, kb, p.part * ROWS, p.len);
+    mv.fetch(lds0 + TL::BYTES, vb, p.part * ROWS, p.len);
+  }
   // queries as B operands; a negative scale turns their sign, so that the largest product has the largest score
   const float c = fmaxf(fabsf(a.scale) * LOG2E, 1e-30f);  // above 0: -inf stays what a masked score is
-  Frag8<T> qf[NQ][D / 16];
+  Frag8<T> qf[D / 16];
+  const T* qr = at<T>(a.q, a.qs, p.b, h, p.tok + min(q, p.len - 1));
 #pragma unroll
-  for (int t = 0; t < NQ; ++t) {
-    const int row = q0 + 32 * t + n;
-    const T* qr = at<T>(a.q, a.qs, p.b, h, p.tok) + (int64_t)min(row, p.len - 1) * a.qs[2];
+  for (int s = 0; s < D / 16; ++s) {
+    from_global<T>(qf[s], qr + 16 * s + 8 * kg, 16 * s + 8 * kg < a.d);
+    if (a.scale < 0.f)
 #pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
-      from_global<T>(qf[t][s], qr + 16 * s + 8 * kg, 16 * s + 8 * kg < a.d);
-      if (a.scale < 0.f)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) qf[t][s].v[e] = -qf[t][s].v[e];
-    }
+      for (int e = 0; e < 8; ++e) qf[s].v[e] = -qf[s].v[e];
   }
-  floatx16 acc[NQ][D / 32];
-  float m[NQ], l[NQ];
+  floatx16 acc[D / 32];
+  float m = -INFINITY, l = 0.f;
 #pragma unroll
-  for (int t = 0; t < NQ; ++t) {
-    m[t] = -INFINITY;
-    l[t] = 0.f;
+  for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[t][i][e] = 0.f;
-  }
+    for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
   const unsigned row_addr = lds0 + TL::rows(lane), col_addr = lds0 + TL::cols(lane);
-  for (int it = 0; it < ntile; ++it) {
-    const int key0 = it * ROWS, buf = it & 1;
+  for (int it = p.part, buf = 0; it < ntile; it += a.parts, buf ^= 1) {
+    const int key0 = it * ROWS, next = key0 + a.parts * ROWS;
     const unsigned rows = row_addr + 2 * buf * TL::BYTES, cols = col_addr + 2 * buf * TL::BYTES;
     dma_wait<0>();
     const bool edge = key0 + ROWS > q_wg;  // some pairs of this tile are masked
     if (edge && !tile_finite<T, D, true>(vt(buf), wave, lane)) odd[buf] = 1;
     lds_barrier();
-    if (it + 1 < ntile) {
-      mk.fetch(lds0 + 2 * (buf ^ 1) * TL::BYTES, kb, key0 + ROWS, p.len);
-      mv.fetch(lds0 + (2 * (buf ^ 1) + 1) * TL::BYTES, vb, key0 + ROWS, p.len);
+    if (it + a.parts < ntile) {
+      mk.fetch(lds0 + 2 * (buf ^ 1) * TL::BYTES, kb, next, p.len);
+      mv.fetch(lds0 + (2 * (buf ^ 1) + 1) * TL::BYTES, vb, next, p.len);
     }
-    if (key0 >= q0 + 32 * NQ) continue;  // behind all of this wave's queries
-    floatx16 sc[NQ][2];
-#pragma unroll
-    for (int t = 0; t < NQ; ++t)
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) sc[t][i][e] = 0.f;
+    if (key0 >= q0 + 32) continue;  // behind all of this wave's queries
+    floatx16 sc[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int s = 0; s < D / 16; ++s) {
-        const Frag8<T> kf = TL::by_row(rows, 32 * i * TL::ROWB, s);
+      for (int e = 0; e < 16; ++e) sc[i][e] = 0.f;
 #pragma unroll
-        for (int t = 0; t < NQ; ++t) mma(sc[t][i], kf, qf[t][s]);
-      }
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s) mma(sc[i], TL::by_row(rows, 32 * i * TL::ROWB, s), qf[s]);
     read_ahead<T, false, 2 * (D / 16), 4>();
-    Frag8<T> pf[NQ][4];
-#pragma unroll
-    for (int t = 0; t < NQ; ++t) {
-      const int q = q0 + 32 * t + n;
-      if (key0 + ROWS - 1 > q0 + 32 * t) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (key0 + 32 * i + frag_row(e, lane) > q) sc[t][i][e] = -INFINITY;
-      }
-      float top = sc[t][0][0];
+    if (key0 + ROWS - 1 > q0) {
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) top = fmaxf(top, sc[t][i][e]);
-      top = half_max(top);
-      // a new reference only where the old one is short by more than 2^8: sums and accumulators stay far inside fp32's range
-      const float far = 8.f / c;
-      if (__any(top > m[t] + far || (m[t] == -INFINITY && top > m[t]))) {
-        const float next = fmaxf(m[t], top);
-        const float f = m[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[t] - next) * c);
-        l[t] *= f;
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) acc[t][i][e] *= f;
-        m[t] = next;
-      }
-      const float ref = m[t] == -INFINITY ? 0.f : m[t] * c;
-      float sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          sc[t][i][e] = __builtin_amdgcn_exp2f(sc[t][i][e] * c - ref);
-          sum += sc[t][i][e];
-        }
-      l[t] += sum;
-#pragma unroll
-      for (int s = 0; s < 4; ++s) from_acc(pf[t][s], sc[t][s >> 1], s & 1);
+        for (int e = 0; e < 16; ++e)
+          if (key0 + 32 * i + frag_row(e, lane) > q) sc[i][e] = -INFINITY;
     }
+    float top = sc[0][0];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) top = fmaxf(top, sc[i][e]);
+    top = half_max(top);
+    // a new reference only where the old one is short by more than 2^8: sums and accumulators stay far inside fp32's range
+    if (__any(top > m + 8.f / c || (m == -INFINITY && top > m))) {
+      const float higher = fmaxf(m, top);
+      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - higher) * c);
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][e] *= f;
+      m = higher;
+    }
+    const float ref = m == -INFINITY ? 0.f : m * c;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        sc[i][e] = __builtin_amdgcn_exp2f(sc[i][e] * c - ref);
+        sum += sc[i][e];
+      }
+    l += sum;
+    Frag8<T> pf[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) from_acc(pf[s], sc[s >> 1], s & 1);
 #pragma unroll
     for (int s = 0; s < 4; ++s)
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        const Frag8<T> vf = TL::by_col(cols, TL::BYTES + 16 * s * TL::ROWB, i);
-#pragma unroll
-        for (int t = 0; t < NQ; ++t) mma(acc[t][i], vf, pf[t][s]);
-      }
+      for (int i = 0; i < D / 32; ++i) mma(acc[i], TL::by_col(cols, TL::BYTES + 16 * s * TL::ROWB, i), pf[s]);
     read_ahead<T, true, 4 * (D / 32), 4>();
-    if (edge && odd[buf]) {
+    if (edge && odd[buf])
 #pragma unroll
-      for (int t = 0; t < NQ; ++t)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const Frag8<T> two[2] = {pf[t][2 * i], pf[t][2 * i + 1]};
-          add_odd<T, D / 32>(acc[t], vb, a.vs[2], key0 + 32 * i, p.len, a.d, two, lane, [&](int row) { return row <= q0 + 32 * t + n; });
-        }
-    }
+      for (int i = 0; i < 2; ++i) {
+        const Frag8<T> two[2] = {pf[2 * i], pf[2 * i + 1]};
+        add_odd<T, D / 32>(acc, vb, a.vs[2], key0 + 32 * i, p.len, a.d, two, lane, [&](int row) { return row <= q; });
+      }
   }
-#pragma unroll
-  for (int t = 0; t < NQ; ++t) {
-    const int q = q0 + 32 * t + n;
-    const float sum = xor32_sum(l[t]);
-    if (q < p.len) {
-      store_column<T, D / 32>(at<T>(a.o, a.os, p.b, h, p.tok + q), acc[t], 1.f / sum, a.d, lane);
-      if (a.lse && kg == 0) a.lse[((int64_t)p.b * a.H + h) * a.T + p.tok + q] = m[t] * c + __builtin_amdgcn_logf(sum);
-    }
+  const float sum = xor32_sum(l);
+  if (q >= p.len) return;
+  const int64_t row = ((int64_t)p.b * a.H + h) * a.T + p.tok + q;
+  if (a.parts == 1) {
+    store_column<T, D / 32>(at<T>(a.o, a.os, p.b, h, p.tok + q), acc, 1.f / sum, a.d, lane);
+    if (a.lse && kg == 0) a.lse[row] = m * c + __builtin_amdgcn_logf(sum);
+  } else {
+    const int64_t at_part = (int64_t)p.part * a.B * a.H * a.T + row;
+    store_column<float, D / 32>(a.part + at_part * a.d, acc, 1.f, a.d, lane);
+    if (kg == 0) a.part_stat[2 * at_part] = m * c, a.part_stat[2 * at_part + 1] = sum;
   }
+}
+
+// The parts of a row's result, sixteen lanes a row
+template <typename T> __global__ __launch_bounds__(256) void attn_join_kernel(Args a) {
+  const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4), all = (int64_t)a.B * a.H * a.T;
+  const int c = 8 * (threadIdx.x & 15);
+  if (row >= all || c >= a.d) return;
+  float top = -INFINITY, sum = 0.f, o[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o[e] = 0.f;
+  for (int s = 0; s < a.parts; ++s) top = fmaxf(top, a.part_stat[2 * (s * all + row)]);
+  for (int s = 0; s < a.parts; ++s) {
+    const float f = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(a.part_stat[2 * (s * all + row)] - top);
+    sum += a.part_stat[2 * (s * all + row) + 1] * f;
+    const float* p = a.part + (s * all + row) * a.d + c;
+    const floatx4 x = load4(p), y = load4(p + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += x[e] * f, o[e + 4] += y[e] * f;
+  }
+  const int64_t t = row % a.T, bh = row / a.T;
+  T* p = at<T>(a.o, a.os, bh / a.H, bh % a.H, t) + c;
+  store4(p, floatx4{o[0] / sum, o[1] / sum, o[2] / sum, o[3] / sum});
+  store4(p + 4, floatx4{o[4] / sum, o[5] / sum, o[6] / sum, o[7] / sum});
+  if (a.lse && c == 0) a.lse[row] = top + __builtin_amdgcn_logf(sum);
+}
+
+// The sum of the parts [parts][stride rows][d] of a [B, heads, T, d] gradient, sixteen lanes a row
+template <typename T> __global__ __launch_bounds__(256) void attn_sum_kernel(const float* part, int parts, int64_t stride, T* out, int64_t sb, int64_t sh, int64_t st, int B,
+                                                                             int heads, int T_, int d) {
+  const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+  const int c = 8 * (threadIdx.x & 15);
+  if (row >= (int64_t)B * heads * T_ || c >= d) return;
+  floatx4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
+  for (int s = 0; s < parts; ++s) {
+    const float* p = part + (s * stride + row) * d + c;
+    x += load4(p);
+    y += load4(p + 4);
+  }
+  const int64_t t = row % T_, bh = row / T_;
+  T* p = out + bh / heads * sb + bh % heads * sh + t * st + c;
+  store4(p, x);
+  store4(p + 4, y);
 }
 
 // delta_i = o_i . do_i, sixteen lanes a row
@@ -494,8 +516,10 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
   lds_barrier();
   const Mover<T, D> mk(a.ks[2], a.d, wave, lane), mv(a.vs[2], a.d, wave, lane);
   const unsigned lds0 = lds_byte_addr(lds);
-  mk.fetch(lds0, kb, 0, p.len);
-  mv.fetch(lds0 + TL::BYTES, vb, 0, p.len);
+  if (p.part < ntile) {
+    mk.fetch(lds0, kb, p.part * ROWS, p.len);
+    mv.fetch(lds0 + TL::BYTES, vb, p.part * ROWS, p.len);
+  }
   const float c = a.scale * LOG2E;
   const int64_t row = min(q, p.len - 1), stat = ((int64_t)p.b * a.H + h) * a.T + p.tok + row;
   const float lse = a.lse[stat], delta = a.delta[stat];
@@ -513,16 +537,16 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
   const unsigned row_addr = lds0 + TL::rows(lane), col_addr = lds0 + TL::cols(lane);
-  for (int it = 0; it < ntile; ++it) {
-    const int key0 = it * ROWS, buf = it & 1;
+  for (int it = p.part, buf = 0; it < ntile; it += a.parts, buf ^= 1) {
+    const int key0 = it * ROWS, next = key0 + a.parts * ROWS;
     const unsigned rows = row_addr + 2 * buf * TL::BYTES, cols = col_addr + 2 * buf * TL::BYTES;
     dma_wait<0>();
     const bool edge = key0 + ROWS > q_wg;
     if (edge && !tile_finite<T, D, false>(kt(buf), wave, lane)) odd[buf] = 1;
     lds_barrier();
-    if (it + 1 < ntile) {
-      mk.fetch(lds0 + 2 * (buf ^ 1) * TL::BYTES, kb, key0 + ROWS, p.len);
-      mv.fetch(lds0 + (2 * (buf ^ 1) + 1) * TL::BYTES, vb, key0 + ROWS, p.len);
+    if (it + a.parts < ntile) {
+      mk.fetch(lds0 + 2 * (buf ^ 1) * TL::BYTES, kb, next, p.len);
+      mv.fetch(lds0 + (2 * (buf ^ 1) + 1) * TL::BYTES, vb, next, p.len);
     }
     const bool scrub = edge && odd[buf];
 #pragma unroll
@@ -563,7 +587,9 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
       }
     }
   }
-  if (q < p.len) store_column<T, D / 32>(at<T>(a.dq, a.dqs, p.b, h, p.tok + q), acc, a.scale, a.d, lane);
+  if (q >= p.len) return;
+  if (a.parts == 1) store_column<T, D / 32>(at<T>(a.dq, a.dqs, p.b, h, p.tok + q), acc, a.scale, a.d, lane);
+  else store_column<float, D / 32>(a.part + ((int64_t)p.part * a.B * a.H * a.T + stat) * a.d, acc, a.scale, a.d, lane);
 }
 
 // An operand through LDS to another wave of the workgroup
@@ -594,7 +620,7 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
   if (!p.on) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, kg = lane >> 5;
   const int kw = wave & 1, qw = wave >> 1, r0 = 32 * qw, key0 = p.blk * ROWS + 32 * kw, key = key0 + n;
-  const int total = ((p.len + ROWS - 1) / ROWS - p.blk) * a.G;
+  const int per = (p.len + ROWS - 1) / ROWS - p.blk, total = per * a.G, last = (p.blk + per) * ROWS;
   if (a.d < D) {
     clear_lds(lds, 4 * TL::BYTES);
     lds_barrier();
@@ -626,9 +652,12 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
     mq.fetch(lds0 + 2 * buf * TL::BYTES, at<T>(a.q, a.qs, p.b, h, p.tok), row0, p.len);
     mg.fetch(lds0 + (2 * buf + 1) * TL::BYTES, at<T>(a.dout, a.gs, p.b, h, p.tok), row0, p.len);
   };
-  int h = p.hkv * a.G, row0 = p.blk * ROWS;  // the tile being multiplied
-  fetch(h, row0, 0);
-  fetch_stats(h, row0);
+  // of the (query head, tile of queries) pairs every a.parts-th: the one being multiplied
+  int h = p.hkv * a.G + p.part / per, row0 = (p.blk + p.part % per) * ROWS;
+  if (p.part < total) {
+    fetch(h, row0, 0);
+    fetch_stats(h, row0);
+  }
   const float c = a.scale * LOG2E;
   const int64_t krow = p.tok + min(key, p.len - 1);
   const T* kr = at<T>(a.k, a.ks, p.b, p.hkv, krow);
@@ -645,13 +674,13 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
 #pragma unroll
     for (int e = 0; e < 16; ++e) dk[i][e] = dv[i][e] = 0.f;
   const unsigned row_addr = lds0 + r0 * TL::ROWB + TL::rows(lane), col_addr = TL::col_block(lds0 + TL::cols(lane), M * qw);
-  for (int it = 0; it < total; ++it) {
-    const int buf = it & 1;
+  for (int it = p.part, buf = 0; it < total; it += a.parts, buf ^= 1) {
     dma_wait<0>();
 #pragma unroll
     for (int g = 0; g < 4; ++g) asm volatile("" : "+v"(lse[g]), "+v"(delta[g]));  // have come too: no wait for the next tile at their use
     const bool edge = row0 == p.blk * ROWS || row0 + ROWS > p.len;
-    const int next_h = row0 + ROWS >= p.len ? h + 1 : h, next_row0 = next_h == h ? row0 + ROWS : p.blk * ROWS;
+    int next_h = h, next_row0 = row0 + a.parts * ROWS;
+    for (; next_row0 >= last; ++next_h) next_row0 -= per * ROWS;
     lds_barrier();
     bool scrub = false;
     if (edge) {
@@ -665,7 +694,7 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
       scrub = __builtin_amdgcn_readfirstlane(scrub);
       lds_barrier();
     }
-    if (it + 1 < total) fetch(next_h, next_row0, buf ^ 1);
+    if (it + a.parts < total) fetch(next_h, next_row0, buf ^ 1);
     const unsigned rows = row_addr + 2 * buf * TL::BYTES, cols = col_addr + 2 * buf * TL::BYTES;
     const auto active = [&](int q) { return row0 + 32 * q + 31 >= key0 && row0 + 32 * q < p.len; };  // some of these queries come after some of the keys
     Frag8<T> pf[2], ds[2];
@@ -697,7 +726,7 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
         leave_frag<T>(mine + (2 + s) * FRAG, ds[s], lane);
       }
     }
-    if (it + 1 < total) fetch_stats(next_h, next_row0);
+    if (it + a.parts < total) fetch_stats(next_h, next_row0);
     lds_barrier();
     if (scrub) {  // the scores were made of the queries and gradients as they are
       tile_finite<T, D, true>(qt(buf), wave, lane);
@@ -734,11 +763,54 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
   }
   if (key >= p.len) return;
   const int c0 = 32 * M * qw;
-  store_column<T, M>(at<T>(a.dk, a.dks, p.b, p.hkv, krow) + c0, dk, a.scale, a.d - c0, lane);
-  store_column<T, M>(at<T>(a.dv, a.dvs, p.b, p.hkv, krow) + c0, dv, 1.f, a.d - c0, lane);
+  if (a.parts == 1) {
+    store_column<T, M>(at<T>(a.dk, a.dks, p.b, p.hkv, krow) + c0, dk, a.scale, a.d - c0, lane);
+    store_column<T, M>(at<T>(a.dv, a.dvs, p.b, p.hkv, krow) + c0, dv, 1.f, a.d - c0, lane);
+  } else {
+    const int64_t rows_all = (int64_t)a.B * a.Hkv * a.T, at_part = 2 * p.part * rows_all + ((int64_t)p.b * a.Hkv + p.hkv) * a.T + krow;
+    store_column<float, M>(a.part + at_part * a.d + c0, dk, a.scale, a.d - c0, lane);
+    store_column<float, M>(a.part + (at_part + rows_all) * a.d + c0, dv, 1.f, a.d - c0, lane);
+  }
 }
 
 int64_t blocks_of(const lnx_attn_args* a, int size) { return a->nseq ? (int64_t)a->T / size + a->nseq : ((int64_t)a->T + size - 1) / size; }
+
+// Into how many parts the rows that a block walks over are split.  In units of one tile's time in a workgroup: the launch takes as long
+// as its work spread over the chip or as its longest workgroup, whichever is more; a split adds to each workgroup the time that
+// its share of the result takes to be written and read in fp32 (`share`), and the joining launch.  Measured at bf16, d = 128: a tile
+// 1.5 us in a workgroup with another on its CU, a share of 64 KB 5 tiles, a launch 4.  `longest`: tiles of the longest block.
+int parts_for(int64_t wgs, int64_t longest, int slots, double share, double launch) {
+  const double work = (double)wgs * (longest + 1) / 2 / slots;
+  int best = 1;
+  double least = 1e300;
+  for (int s = 1; s <= 8 && s <= longest; ++s) {
+    const double extra = s > 1 ? share : 0, spread = work + extra * s * (double)wgs / slots, one = (double)longest / s + extra;
+    const double t = (spread > one ? spread : one) + (s > 1 ? launch : 0);
+    if (t < least * 0.95) least = t, best = s;
+  }
+  return best;
+}
+enum { FWD, DQ, DKV };
+int parts_of(const lnx_attn_args* a, int kernel) {
+  const int64_t len = a->nseq ? (a->T + a->nseq - 1) / a->nseq : a->T, rows = a->nseq ? a->nseq : a->B;  // sequences of the average length
+  const bool bf16 = a->dtype == LNX_BF16;
+  const int slots = bf16 ? 512 : 256;
+  const double share = bf16 ? 5 : 1, launch = bf16 ? 4 : 1.5;
+  const int64_t keys = (len + ROWS - 1) / ROWS;
+  if (kernel == DKV) return parts_for(rows * a->Hkv * keys, keys * (a->H / a->Hkv), slots, share / 2, launch);
+  return parts_for(rows * a->H * ((len + 127) / 128), keys, slots, share, launch);
+}
+// Bytes of the workspaces: shares of the forward kernel; delta and the shares of either gradient kernel
+uint64_t fwd_bytes(const lnx_attn_args* a) {
+  const int s = parts_of(a, FWD);
+  return s > 1 ? (uint64_t)s * a->B * a->H * a->T * (a->d + 2) * sizeof(float) : 0;
+}
+uint64_t delta_bytes(const lnx_attn_args* a) { return ((uint64_t)a->B * a->H * a->T * sizeof(float) + 15) / 16 * 16; }
+uint64_t bwd_bytes(const lnx_attn_args* a) {
+  const int sq = parts_of(a, DQ), sk = parts_of(a, DKV);
+  const uint64_t q = sq > 1 ? (uint64_t)sq * a->B * a->H * a->T * a->d * sizeof(float) : 0, k = sk > 1 ? (uint64_t)sk * 2 * a->B * a->Hkv * a->T * a->d * sizeof(float) : 0;
+  return delta_bytes(a) + (q > k ? q : k);
+}
 
 // Rows that the kernels move as vectors, 64 of them within the 31 bits of a lane's offset
 bool rows_fit(const lnx_tensor4* t, int64_t size) {
@@ -759,9 +831,11 @@ int check(const char* what, const lnx_attn_args* a, bool bwd) {
     if (!ts[i]->p) return lnx_set_error(LNX_ERR_NULL, "%s: a tensor is missing", what);
     if (!rows_fit(ts[i], a->dtype == LNX_BF16 ? 2 : 4)) return lnx_set_error(LNX_ERR_SHAPE, "%s: tensors must be 16-byte aligned, rows whole numbers of 16 bytes and at most 16 MiB apart", what);
   }
-  if (bwd && (!a->lse || !a->workspace || a->workspace_bytes < lnx_attn_bwd_workspace_bytes(a)))
-    return lnx_set_error(LNX_ERR_WORKSPACE, "%s: lse and a workspace of %llu bytes are required", what, (unsigned long long)lnx_attn_bwd_workspace_bytes(a));
-  if ((int64_t)a->B * a->H * blocks_of(a, ROWS) > 0x7fffffff || (int64_t)a->B * a->H * a->T / 16 >= 0x7fffffff)
+  if (bwd && !a->lse) return lnx_set_error(LNX_ERR_NULL, "%s: lse is required", what);
+  const uint64_t need = bwd ? bwd_bytes(a) : fwd_bytes(a);
+  if (need && (!a->workspace || a->workspace_bytes < need || reinterpret_cast<uintptr_t>(a->workspace) % 16))
+    return lnx_set_error(LNX_ERR_WORKSPACE, "%s: needs a 16-byte aligned workspace of %llu bytes", what, (unsigned long long)need);
+  if ((int64_t)a->B * a->H * blocks_of(a, ROWS) * 8 > 0x7fffffff || (int64_t)a->B * a->H * a->T / 16 >= 0x7fffffff)
     return lnx_set_error(LNX_ERR_SHAPE, "%s: too many rows", what);
   return LNX_OK;
 }
@@ -771,7 +845,7 @@ Args kernel_args(const lnx_attn_args* a) {
   auto strides = [](int64_t (&s)[3], const lnx_tensor4& t) { s[0] = t.stride_b, s[1] = t.stride_h, s[2] = t.stride_t; };
   k.q = a->q.p, k.k = a->k.p, k.v = a->v.p, k.dout = a->d_o.p, k.o = a->o.p, k.dq = a->d_q.p, k.dk = a->d_k.p, k.dv = a->d_v.p;
   strides(k.qs, a->q), strides(k.ks, a->k), strides(k.vs, a->v), strides(k.os, a->o), strides(k.gs, a->d_o), strides(k.dqs, a->d_q), strides(k.dks, a->d_k), strides(k.dvs, a->d_v);
-  k.lse = a->lse, k.delta = static_cast<float*>(a->workspace), k.cu = a->cu_seqlens;
+  k.lse = a->lse, k.cu = a->cu_seqlens;
   k.B = a->B, k.H = a->H, k.Hkv = a->Hkv, k.G = a->H / a->Hkv, k.T = a->T, k.d = a->d, k.nseq = a->nseq, k.scale = a->scale;
   return k;
 }
@@ -785,19 +859,39 @@ template <typename K> int start(K kernel, const char* name, const Args& a, int64
 
 template <typename T, int D> int launch_fwd(const lnx_attn_args* a, hipStream_t st) {
   Args k = kernel_args(a);
-  constexpr int NQ = 1;
-  k.nblk = (int)blocks_of(a, 128 * NQ);
-  return start(attn_fwd_kernel<T, D, NQ>, "attn_fwd", k, (int64_t)k.B * k.H * k.nblk, 4 * Tile<T, D>::BYTES + 16, st);
+  k.nblk = (int)blocks_of(a, 128), k.parts = parts_of(a, FWD);
+  const int64_t rows = (int64_t)k.B * k.H * k.T;
+  k.part = static_cast<float*>(a->workspace), k.part_stat = k.part ? k.part + k.parts * rows * k.d : nullptr;
+  if (int rc = start(attn_fwd_kernel<T, D>, "attn_fwd", k, (int64_t)k.B * k.H * k.nblk * k.parts, 4 * Tile<T, D>::BYTES + 16, st)) return rc;
+  if (k.parts > 1) {
+    lnx_profile_mark("attn_join", st);
+    attn_join_kernel<T><<<dim3((unsigned)((rows + 15) / 16)), 256, 0, st>>>(k);
+  }
+  return LNX_OK;
+}
+
+template <typename T> void sum_parts(const Args& k, const float* part, int64_t stride, void* out, const int64_t (&s)[3], int heads, hipStream_t st) {
+  lnx_profile_mark("attn_sum", st);
+  attn_sum_kernel<T><<<dim3((unsigned)(((int64_t)k.B * heads * k.T + 15) / 16)), 256, 0, st>>>(part, k.parts, stride, static_cast<T*>(out), s[0], s[1], s[2], k.B, heads, k.T, k.d);
 }
 
 template <typename T, int D> int launch_bwd(const lnx_attn_args* a, hipStream_t st) {
   Args k = kernel_args(a);
+  k.delta = static_cast<float*>(a->workspace);
+  k.part = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + delta_bytes(a));
   lnx_profile_mark("attn_delta", st);
   attn_delta_kernel<T><<<dim3((unsigned)(((int64_t)k.B * k.H * k.T + 15) / 16)), 256, 0, st>>>(k);
-  k.nblk = (int)blocks_of(a, ROWS);
-  if (int rc = start(attn_dkv_kernel<T, D>, "attn_dkv", k, (int64_t)k.B * k.Hkv * k.nblk, 4 * Tile<T, D>::BYTES + 8192 * sizeof(T), st)) return rc;
-  k.nblk = (int)blocks_of(a, 128);
-  return start(attn_dq_kernel<T, D>, "attn_dq", k, (int64_t)k.B * k.H * k.nblk, 4 * Tile<T, D>::BYTES + 16, st);
+  k.nblk = (int)blocks_of(a, ROWS), k.parts = parts_of(a, DKV);
+  if (int rc = start(attn_dkv_kernel<T, D>, "attn_dkv", k, (int64_t)k.B * k.Hkv * k.nblk * k.parts, 4 * Tile<T, D>::BYTES + 8192 * sizeof(T), st)) return rc;
+  if (k.parts > 1) {
+    const int64_t rows = (int64_t)k.B * k.Hkv * k.T;
+    sum_parts<T>(k, k.part, 2 * rows, k.dk, k.dks, k.Hkv, st);
+    sum_parts<T>(k, k.part + rows * k.d, 2 * rows, k.dv, k.dvs, k.Hkv, st);
+  }
+  k.nblk = (int)blocks_of(a, 128), k.parts = parts_of(a, DQ);
+  if (int rc = start(attn_dq_kernel<T, D>, "attn_dq", k, (int64_t)k.B * k.H * k.nblk * k.parts, 4 * Tile<T, D>::BYTES + 16, st)) return rc;
+  if (k.parts > 1) sum_parts<T>(k, k.part, (int64_t)k.B * k.H * k.T, k.dq, k.dqs, k.H, st);
+  return LNX_OK;
 }
 
 int run(const char* what, const lnx_attn_args* a, bool bwd, hipStream_t st) {
@@ -1083,8 +1177,8 @@ extern "C" int lnx_attn_step(const lnx_attn_step_args* a, void* hip_stream) {
   return e == hipSuccess ? LNX_OK : lnx_set_error(LNX_ERR_LAUNCH, "attn_step: %s", hipGetErrorString(e));
 }
 
-extern "C" uint64_t lnx_attn_bwd_workspace_bytes(const lnx_attn_args* a) {
-  return a && a->B > 0 && a->H > 0 && a->T > 0 ? (uint64_t)a->B * a->H * a->T * sizeof(float) : 0;
-}
+static bool attn_sizes(const lnx_attn_args* a) { return a && a->B > 0 && a->H > 0 && a->Hkv > 0 && a->T > 0 && a->d > 0 && a->nseq >= 0; }
+extern "C" uint64_t lnx_attn_fwd_workspace_bytes(const lnx_attn_args* a) { return attn_sizes(a) ? fwd_bytes(a) : 0; }
+extern "C" uint64_t lnx_attn_bwd_workspace_bytes(const lnx_attn_args* a) { return attn_sizes(a) ? bwd_bytes(a) : 0; }
 extern "C" int lnx_attn_fwd(const lnx_attn_args* a, void* hip_stream) { return run("attn_fwd", a, false, static_cast<hipStream_t>(hip_stream)); }
 extern "C" int lnx_attn_bwd(const lnx_attn_args* a, void* hip_stream) { return run("attn_bwd", a, true, static_cast<hipStream_t>(hip_stream)); }

@@ -1395,6 +1395,10 @@ Tensor attention_forward(const Tensor& q, const Tensor& k, const Tensor& v, cons
   const Tensor o = empty_rows(q, is_token_first(q));
   lnx_attn_args a = attention_args(q, k, v, o, cu, scale);
   a.lse = fptr(lse);
+  a.workspace_bytes = lnx_attn_fwd_workspace_bytes(&a);
+  Tensor ws;
+  if (a.workspace_bytes) ws = work_area(q, a.workspace_bytes);
+  a.workspace = ptr(ws);
   const c10::DeviceGuard guard(q.device());
   check_status(lnx_attn_fwd(&a, stream_of(q)), "lnx_attn_fwd");
   return o;
