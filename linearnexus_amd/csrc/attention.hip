@@ -245,12 +245,13 @@ struct Place {
 __device__ __forceinline__ Place place(const Args& a, int size, int heads, bool last_first) {
   Place p;
   int w = blockIdx.x, group, blk;
-  const int groups = a.B * a.Hkv, per_group = heads * a.parts, per = a.nblk * per_group;
+  const int groups = a.B * a.Hkv, per_group = heads * a.parts;
   if (groups % 8 == 0) {
-    const int slot = w >> 3;
-    group = (w & 7) + 8 * (slot / per);
-    blk = slot % per / per_group;
-    w = slot % per_group;
+    const int slot = w >> 3, here = groups / 8 * per_group;
+    blk = slot / here;
+    w = slot % here;
+    group = (w / per_group) * 8 + (blockIdx.x & 7);
+    w %= per_group;
   } else {
     blk = w / (groups * per_group);
     w -= blk * groups * per_group;
