@@ -1217,8 +1217,8 @@ PyObject* py_dplr_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 // element-wise gated linear recurrence
 // ---------------------------------------------------------------------------------------------------------------
 
-// What the kernels read in place: any strides over rows and tokens, channels next to each other
-Tensor channels_dense(const Tensor& x) { return x.size(-1) == 1 || x.stride(-1) == 1 ? x : x.contiguous(); }
+// What the kernels read in place: any strides over rows and tokens (at most 4 MiB), channels next to each other
+Tensor channels_dense(const Tensor& x) { return (x.size(-1) == 1 || x.stride(-1) == 1) && x.stride(1) * x.element_size() <= 4 << 20 ? x : x.contiguous(); }
 
 struct RecShape {
   int64_t B, T, D, nseq, rows;
@@ -1232,7 +1232,7 @@ RecShape rec_shape(const char* op, const Tensor& x, const Tensor& g, const Tenso
   TORCH_CHECK(g.is_floating_point(), op, ": g must be a floating-point tensor, got ", g.scalar_type());
   check_devices(op, x, {{"g", &g}, {"state", &s0}, {"cu_seqlens", &cu}});
   RecShape s{x.size(0), dims == 3 ? x.size(1) : 1, x.size(-1), 0, x.size(0)};
-  TORCH_CHECK(s.B <= INT32_MAX && s.T <= INT32_MAX && s.D <= INT32_MAX, op, ": x is too large, got ", shape_text(x));
+  TORCH_CHECK(s.B <= INT32_MAX && s.T <= INT32_MAX && s.D <= 1 << 20, op, ": x is too large, got ", shape_text(x));
   if (cu.defined()) {
     TORCH_CHECK(s.B == 1, "cu_seqlens needs a packed batch with B == 1");
     s.rows = s.nseq = cu.numel() - 1;

@@ -1,13 +1,14 @@
 // Element-wise gated linear recurrence over [rows, T, D] tensors, dense or packed, forward, backward and one token:
 //   h_t = e^{g_t} h_{t-1} + x_t,  y_t = h_t                                    (h_0 the initial state, g log-decays)
 //   dh_t = dy_t + e^{g_{t+1}} dh_{t+1},  dx_t = dh_t,  dg_t = e^{g_t} h_{t-1} dh_t,  dh_0 = e^{g_1} dh_1
-// No products to speak of: every pass is bound by the bytes of its tensors.  A workgroup owns 128 bytes of channels of one row and
-// walks its tokens in tiles of 256: a thread holds eight (bf16) or four (fp32) channels of four consecutive tokens as one 16-byte
-// vector each and reduces them to a pair (A, H), the map h -> A h + H; pairs are scanned over the eight token groups of a wave by
-// shuffles; the eight waves' pairs are chained through LDS by one lane per channel, which carries the state from tile to tile.  The
-// loads of the next tile are in flight meanwhile.
-// Everything between loads and stores is fp32.  The backward pass reads x again instead of y, which is rounded: the forward pass
-// leaves the state entering every tile (fp32, 1 / 256 of x's elements), so the states behind dg are the unrounded ones.
+// No products to speak of: every pass is bound by the bytes of its tensors.  A workgroup owns 64 channels of one row and walks its
+// tokens in tiles: a thread holds four channels of R consecutive tokens and reduces them to a pair (A, H), the map h -> A h + H; pairs
+// are scanned over the four token groups of a wave by lane swaps, and the eight waves' pairs are chained through LDS by one lane per
+// channel, which carries the state from tile to tile.  The loads of the next tile are in flight meanwhile.  (Eight channels of four
+// tokens a thread, scanned over eight groups by shuffles, were bound by the scan: 4.1 TB/s at [8, 4096, 2048] bf16, the same with
+// twice the loads in flight.)  Everything between loads and stores is fp32.  The backward pass reads x again instead of y, which is
+// rounded: the forward pass leaves the state entering every tile (fp32, 1 / 256 of bf16's elements, 1 / 128 of fp32's), so the states
+// behind dg are the unrounded ones.
 // Where rows and channels give too few workgroups the tokens are cut into segments: a first launch reduces every segment to its
 // pair, the second one starts each segment from the folded pairs before it.  No atomics: results are the same from run to run.
 #include "lnx_common.h"
@@ -15,48 +16,30 @@
 
 namespace {
 
-constexpr int THREADS = 512, WAVES = 8, TCOLS = 8, TROWS = THREADS / TCOLS;
-constexpr int TILE = 4 * TROWS;  // tokens of a tile of the forward pass
-// Tokens per thread of the backward pass, and so the distance of the states that the forward pass leaves for it: eight channels of
-// four tokens would need 340 registers a lane.
-template <typename T> constexpr int bwd_r() { return sizeof(T) == 2 ? 2 : 4; }
-template <typename T> constexpr int kept_tokens() { return bwd_r<T>() * TROWS; }
+constexpr int THREADS = 512, WAVES = 8, TCOLS = 16, TROWS = THREADS / TCOLS, N = 4, C = TCOLS * N;  // C channels a workgroup
+// Tokens per thread: what the backward pass's registers take
+template <typename T> constexpr int tokens() { return sizeof(T) == 2 ? 8 : 4; }
+template <typename T> constexpr int tile_of() { return tokens<T>() * TROWS; }
 
-// N consecutive elements as they lie in memory
-template <typename E, int N> struct Raw {
-  typedef typename Vec16<E>::V V;
-  static constexpr int VN = Vec16<E>::N, K = N / VN;
-  V v[K];
-  template <bool VEC> __device__ __forceinline__ void load(const E* p, int left) {
-    if (VEC) {
-#pragma unroll
-      for (int k = 0; k < K; ++k) v[k] = *reinterpret_cast<const V*>(p + k * VN);
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i / VN][i % VN] = i < left ? p[i] : from_f32<E>(0.f);
-    }
-  }
-  __device__ __forceinline__ void zero() {
-#pragma unroll
-    for (int k = 0; k < K; ++k) v[k] = vec_zero<E>();
-  }
-  __device__ __forceinline__ float get(int i) const { return to_f32(v[i / VN][i % VN]); }
-};
-
-template <typename E, int N, bool VEC> __device__ __forceinline__ void put(E* p, const float (&f)[N], int left) {
-  typedef typename Vec16<E>::V V;
-  constexpr int VN = Vec16<E>::N;
-#pragma unroll
-  for (int k = 0; k < N / VN; ++k) {
-    V v;
-#pragma unroll
-    for (int e = 0; e < VN; ++e) v[e] = from_f32<E>(f[k * VN + e]);
-    if (VEC) *reinterpret_cast<V*>(p + k * VN) = v;
+// Four consecutive elements as they lie in memory
+template <typename E, bool VEC> struct Raw {
+  typename Vec4<E>::V v;
+  __device__ __forceinline__ void load(const E* p, int left) {
+    if (VEC) v = *reinterpret_cast<const typename Vec4<E>::V*>(p);
     else
 #pragma unroll
-      for (int e = 0; e < VN; ++e)
-        if (k * VN + e < left) p[k * VN + e] = v[e];
+      for (int i = 0; i < N; ++i) v[i] = i < left ? p[i] : from_f32<E>(0.f);
   }
+  __device__ __forceinline__ void zero() { v = typename Vec4<E>::V{}; }
+  __device__ __forceinline__ float get(int i) const { return to_f32(v[i]); }
+};
+
+template <bool VEC, typename E> __device__ __forceinline__ void put(E* p, const float (&f)[N], int left) {
+  if (VEC) store4(p, floatx4{f[0], f[1], f[2], f[3]});
+  else
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < left) p[i] = from_f32<E>(f[i]);
 }
 
 struct Args {
@@ -70,11 +53,11 @@ struct Args {
   bool packed;
 };
 
-// What a workgroup works on: row, its first channel, its tiles
+// What a workgroup works on: row, its channels, its tiles
 struct Place {
   int row, seg, len, ntile, per, tile0, tile1, c0, c, left;  // c0: the workgroup's first channel, c: this thread's
   int64_t tok, slot;  // first token in a packed batch (0 otherwise); first kept state
-  __device__ __forceinline__ Place(const Args& a, int N, int TILE, int KEPT) {
+  __device__ __forceinline__ Place(const Args& a, int tile) {
     const int ct = blockIdx.x % a.ctiles, rs = blockIdx.x / a.ctiles;
     seg = rs % a.segs;
     row = rs / a.segs;
@@ -82,88 +65,93 @@ struct Place {
       const int first = seq_first(a.cu, row, a.T);
       len = seq_end(a.cu, row, a.T) - first;
       tok = first;
-      slot = first / KEPT + row;
+      slot = first / tile + row;
     } else {
       len = a.T;
       tok = 0;
-      slot = (int64_t)row * ((a.T + KEPT - 1) / KEPT);
+      slot = (int64_t)row * ((a.T + tile - 1) / tile);
     }
-    ntile = (len + TILE - 1) / TILE;
+    ntile = (len + tile - 1) / tile;
     per = (ntile + a.segs - 1) / a.segs;
     tile0 = min(seg * per, ntile);
     tile1 = min(tile0 + per, ntile);
-    c0 = ct * TCOLS * N;
+    c0 = ct * C;
     c = c0 + (threadIdx.x & (TCOLS - 1)) * N;
     left = a.D - c;
   }
-  template <typename E> __device__ __forceinline__ const E* at(const void* p, int64_t b, int64_t t, bool packed) const {
-    return static_cast<const E*>(p) + (packed ? tok * t : row * b) + c;
+  // Token `first` of the row: the wave's pointer and the lane's bytes from there, so that addresses are formed in scalar registers
+  template <typename E> __device__ __forceinline__ const char* at(const void* p, int64_t b, int64_t t, int64_t first) const {
+    return static_cast<const char*>(p) + (row * b + (tok + first) * t) * (int64_t)sizeof(E);
   }
+  template <typename E> __device__ __forceinline__ unsigned lane(int64_t t, int token) const { return (unsigned)((token * (int)t + c) * (int)sizeof(E)); }
 };
+template <typename E> __device__ __forceinline__ const E* elems(const char* p, unsigned off) { return reinterpret_cast<const E*>(p + off); }
+template <typename E> __device__ __forceinline__ E* elems(char* p, unsigned off) { return reinterpret_cast<E*>(p + off); }
 
-// Inclusive scan of the maps over the wave's eight token groups (lanes 8 apart), upwards or downwards in time
-template <int N, bool UP> __device__ __forceinline__ void scan_wave(float (&A)[N], float (&H)[N], int lane) {
-#pragma unroll
-  for (int s = 8; s < 64; s <<= 1) {
-    const bool on = UP ? lane >= s : lane < 64 - s;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float Ap = UP ? __shfl_up(A[i], s, LNX_WAVE) : __shfl_down(A[i], s, LNX_WAVE);
-      const float Hp = UP ? __shfl_up(H[i], s, LNX_WAVE) : __shfl_down(H[i], s, LNX_WAVE);
-      if (on) {
-        H[i] += A[i] * Hp;
-        A[i] *= Ap;
-      }
-    }
+// (a, h): a thread's pair.  Afterwards the wave's pair, and in (ea, eh) that of the wave's groups (16 lanes each) before this one,
+// upwards or downwards in time.
+template <bool UP> __device__ __forceinline__ void scan_wave(float& a, float& h, float& ea, float& eh, int lane) {
+  const auto a16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(a), false, false);  // even groups' values, odd groups'
+  const auto h16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(h), __float_as_uint(h), false, false);
+  const float a1 = __uint_as_float(UP ? a16[0] : a16[1]), h1 = __uint_as_float(UP ? h16[0] : h16[1]);  // the first of two groups
+  const float a2 = __uint_as_float(UP ? a16[1] : a16[0]), h2 = __uint_as_float(UP ? h16[1] : h16[0]);
+  const float ap = a1 * a2, hp = a2 * h1 + h2;
+  const bool second = ((lane >> 4) & 1) == (UP ? 1 : 0);
+  ea = second ? a1 : 1.f;
+  eh = second ? h1 : 0.f;
+  const auto a32 = __builtin_amdgcn_permlane32_swap(__float_as_uint(ap), __float_as_uint(ap), false, false);  // the lower half's, the upper half's
+  const auto h32 = __builtin_amdgcn_permlane32_swap(__float_as_uint(hp), __float_as_uint(hp), false, false);
+  const float A1 = __uint_as_float(UP ? a32[0] : a32[1]), H1 = __uint_as_float(UP ? h32[0] : h32[1]);
+  const float A2 = __uint_as_float(UP ? a32[1] : a32[0]), H2 = __uint_as_float(UP ? h32[1] : h32[0]);
+  a = A1 * A2;
+  h = A2 * H1 + H2;
+  if ((lane >> 5) == (UP ? 1 : 0)) {
+    eh += ea * H1;
+    ea *= A1;
   }
 }
 
 // The eight waves' pairs and the states entering the waves, by channel of the workgroup
-template <int N> struct Waves {
-  static constexpr int C = TCOLS * N;
+struct Waves {
   float A[WAVES][C], H[WAVES][C], in[WAVES][C];
-  // this wave's total out of its inclusive scan
-  template <bool UP> __device__ __forceinline__ void leave(const float (&a)[N], const float (&h)[N], int lane, int wave) {
-    if ((lane >> 3) == (UP ? 7 : 0)) {
-      const int c = (lane & (TCOLS - 1)) * N;
-#pragma unroll
-      for (int i = 0; i < N; ++i) A[wave][c + i] = a[i], H[wave][c + i] = h[i];
+  __device__ __forceinline__ void leave(const float (&a)[N], const float (&h)[N], int lane, int wave) {
+    if (lane < TCOLS) {
+      store4(&A[wave][lane * N], floatx4{a[0], a[1], a[2], a[3]});
+      store4(&H[wave][lane * N], floatx4{h[0], h[1], h[2], h[3]});
     }
   }
-  // one lane per channel: the state entering each wave, `carry` from before the tile to behind it; `all` the tile's product
+  // one lane per channel: the state entering each wave, `carry` from before the tile to behind it; `all` the tiles' product
   template <bool UP> __device__ __forceinline__ void chain(int c, float& carry, float& all) {
+    float a[WAVES], h[WAVES];
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) a[w] = A[w][c], h[w] = H[w][c];
 #pragma unroll
     for (int k = 0; k < WAVES; ++k) {
       const int w = UP ? k : WAVES - 1 - k;
       in[w][c] = carry;
-      carry = A[w][c] * carry + H[w][c];
-      all *= A[w][c];
+      carry = a[w] * carry + h[w];
+      all *= a[w];
     }
   }
-  // the state entering this thread's tokens, from its wave's and the neighbouring groups' inclusive pairs
-  template <bool UP> __device__ __forceinline__ void enter(const float (&a)[N], const float (&h)[N], float (&s)[N], int lane, int wave) const {
-    const int c = (lane & (TCOLS - 1)) * N;
+  // the state entering this thread's tokens
+  __device__ __forceinline__ void enter(const float (&ea)[N], const float (&eh)[N], float (&s)[N], int lane, int wave) const {
+    const floatx4 from = load4(&in[wave][(lane & (TCOLS - 1)) * N]);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float Ap = UP ? __shfl_up(a[i], 8, LNX_WAVE) : __shfl_down(a[i], 8, LNX_WAVE);
-      const float Hp = UP ? __shfl_up(h[i], 8, LNX_WAVE) : __shfl_down(h[i], 8, LNX_WAVE);
-      const float from = in[wave][c + i];
-      s[i] = (UP ? lane >= 8 : lane < 56) ? Ap * from + Hp : from;
-    }
+    for (int i = 0; i < N; ++i) s[i] = ea[i] * from[i] + eh[i];
   }
 };
 
 // SUM: only the pair of each segment (but the last, which nothing follows)
 template <typename T, typename G, bool VEC, bool SUM> __global__ __launch_bounds__(THREADS) void linrec_fwd_kernel(Args a) {
-  constexpr int N = Vec16<T>::N, R = TILE / TROWS, KEPT = kept_tokens<T>(), C = TCOLS * N;
-  __shared__ Waves<N> ws;
-  const Place p(a, N, TILE, KEPT);
+  constexpr int R = tokens<T>(), TILE = tile_of<T>();
+  __shared__ Waves ws;
+  const Place p(a, TILE);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tr = threadIdx.x / TCOLS;
   if (SUM && p.tile1 >= p.ntile) return;
   const bool in_c = p.left > 0;
   // the chain's lanes: one channel each
   const int chan = p.c0 + lane;
-  const bool chains = wave == 0 && lane < C, in_chan = chains && chan < a.D;
+  const bool chains = wave == 0, in_chan = chains && chan < a.D;
   const int64_t row_c = (int64_t)p.row * a.D + chan;
   float carry = 0.f, all = 1.f;
   if (!SUM && in_chan) {
@@ -174,26 +162,31 @@ template <typename T, typename G, bool VEC, bool SUM> __global__ __launch_bounds
         carry = q[0] * carry + q[a.D];
       }
   }
-  const T* x = p.at<T>(a.x, a.xb, a.xt, a.packed);
-  const G* g = p.at<G>(a.g, a.gb, a.gt, a.packed);
-  T* y = static_cast<T*>(a.y) + (a.packed ? p.tok : (int64_t)p.row * a.T) * a.D + p.c;
-  Raw<T, N> xr[R];
-  Raw<G, N> gr[R];
-  auto fetch = [&](int tile) {
+  const int64_t first = (int64_t)p.tile0 * TILE, row_b = a.packed ? 0 : 1;  // a packed batch is one row
+  const char* x = p.at<T>(a.x, row_b * a.xb, a.xt, first);
+  const char* g = p.at<G>(a.g, row_b * a.gb, a.gt, first);
+  char* y = const_cast<char*>(p.at<T>(a.y, row_b * a.T * a.D, a.D, first));
+  const unsigned xo = p.lane<T>(a.xt, tr * R), go = p.lane<G>(a.gt, tr * R), yo = p.lane<T>(a.D, tr * R);
+  const int64_t xs = a.xt * (int64_t)sizeof(T), gs = a.gt * (int64_t)sizeof(G), ys = a.D * (int64_t)sizeof(T);
+  Raw<T, VEC> xr[R];
+  Raw<G, VEC> gr[R];
+  // the tile that x and g point at
+  const auto fetch = [&](int tile) {
+    if ((tile + 1) * (int64_t)TILE <= p.len && p.c0 + C <= a.D) {
 #pragma unroll
-    for (int u = 0; u < R; ++u) {
-      const int64_t t = (int64_t)tile * TILE + tr * R + u;
-      xr[u].zero();
-      gr[u].zero();
-      if (t < p.len && in_c) {
-        xr[u].template load<VEC>(x + t * a.xt, p.left);
-        gr[u].template load<VEC>(g + t * a.gt, p.left);
+      for (int u = 0; u < R; ++u) xr[u].load(elems<T>(x + u * xs, xo), N), gr[u].load(elems<G>(g + u * gs, go), N);
+    } else {
+#pragma unroll
+      for (int u = 0; u < R; ++u) {
+        xr[u].zero();
+        gr[u].zero();
+        if ((int64_t)tile * TILE + tr * R + u < p.len && in_c) xr[u].load(elems<T>(x + u * xs, xo), p.left), gr[u].load(elems<G>(g + u * gs, go), p.left);
       }
     }
   };
   if (p.tile0 < p.tile1) fetch(p.tile0);
   for (int tile = p.tile0; tile < p.tile1; ++tile) {
-    float e[R][N], xv[R][N], A[N], H[N];
+    float e[R][N], xv[R][N], A[N], H[N], ea[N], eh[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) A[i] = 1.f, H[i] = 0.f;
 #pragma unroll
@@ -205,29 +198,29 @@ template <typename T, typename G, bool VEC, bool SUM> __global__ __launch_bounds
         H[i] = e[u][i] * H[i] + xv[u][i];
         A[i] *= e[u][i];
       }
+    x += TILE * xs;
+    g += TILE * gs;
     if (tile + 1 < p.tile1) fetch(tile + 1);
-    scan_wave<N, true>(A, H, lane);
-    ws.template leave<true>(A, H, lane, wave);
+#pragma unroll
+    for (int i = 0; i < N; ++i) scan_wave<true>(A[i], H[i], ea[i], eh[i], lane);
+    ws.leave(A, H, lane, wave);
     lds_barrier();
     if (chains) {
-      ws.template chain<true>(lane, carry, all);
-      if (!SUM && a.kept && in_chan) {
-#pragma unroll
-        for (int k = 0; k < TILE / KEPT; ++k)
-          if (tile * (int64_t)TILE + k * KEPT < p.len) a.kept[(p.slot + tile * (TILE / KEPT) + k) * a.D + chan] = ws.in[k * WAVES * KEPT / TILE][lane];
-      }
+      if (!SUM && a.kept && in_chan) a.kept[(p.slot + tile) * a.D + chan] = carry;
+      ws.chain<true>(lane, carry, all);
     }
     lds_barrier();
     if (!SUM) {
       float h[N];
-      ws.template enter<true>(A, H, h, lane, wave);
+      ws.enter(ea, eh, h, lane, wave);
+      const bool whole = (tile + 1) * (int64_t)TILE <= p.len && p.c0 + C <= a.D;
 #pragma unroll
       for (int u = 0; u < R; ++u) {
-        const int64_t t = (int64_t)tile * TILE + tr * R + u;
 #pragma unroll
         for (int i = 0; i < N; ++i) h[i] = e[u][i] * h[i] + xv[u][i];
-        if (t < p.len && in_c) put<T, N, VEC>(y + t * a.D, h, p.left);
+        if (whole || ((int64_t)tile * TILE + tr * R + u < p.len && in_c)) put<VEC>(elems<T>(y + u * ys, yo), h, p.left);
       }
+      y += TILE * ys;
     }
   }
   if (!in_chan) return;
@@ -242,14 +235,14 @@ template <typename T, typename G, bool VEC, bool SUM> __global__ __launch_bounds
 
 // Backwards in time: o is e^{g_{t+1}} dh_{t+1}.  SUM: only the pair of each segment (but the first, which nothing precedes)
 template <typename T, typename G, bool VEC, bool SUM> __global__ __launch_bounds__(THREADS) void linrec_bwd_kernel(Args a) {
-  constexpr int N = Vec16<T>::N, R = bwd_r<T>(), TILE = kept_tokens<T>(), C = TCOLS * N;
-  __shared__ Waves<N> ws, wf;
-  const Place p(a, N, TILE, TILE);
+  constexpr int R = tokens<T>(), TILE = tile_of<T>();
+  __shared__ Waves ws, wf;
+  const Place p(a, TILE);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tr = threadIdx.x / TCOLS;
   if (SUM && (p.seg == 0 || p.tile0 >= p.tile1)) return;
   const bool in_c = p.left > 0;
   const int chan = p.c0 + lane;  // wave 0 chains the gradients, wave 1 the states
-  const bool chains = wave == 0 && lane < C, in_chan = chains && chan < a.D, states = !SUM && wave == 1 && lane < C;
+  const bool chains = wave == 0, in_chan = chains && chan < a.D, states = !SUM && wave == 1;
   const int64_t row_c = (int64_t)p.row * a.D + chan;
   float carry = 0.f, all = 1.f, start = 0.f;
   if (!SUM && in_chan) {
@@ -260,89 +253,113 @@ template <typename T, typename G, bool VEC, bool SUM> __global__ __launch_bounds
         carry = q[0] * carry + q[a.D];
       }
   }
-  const T* x = p.at<T>(a.x, a.xb, a.xt, a.packed);
-  const G* g = p.at<G>(a.g, a.gb, a.gt, a.packed);
-  const T* dy = p.at<T>(a.dy, a.yb, a.yt, a.packed);
-  const int64_t base = (a.packed ? p.tok : (int64_t)p.row * a.T) * a.D + p.c;
-  T* dx = static_cast<T*>(a.dx) + base;
-  G* dg = static_cast<G*>(a.dg) + base;
-  Raw<T, N> xr[R], yr[R];
-  Raw<G, N> gr[R];
-  auto fetch = [&](int tile) {
-    if (states && chan < a.D) start = a.kept[(p.slot + tile) * a.D + chan];
+  const int64_t first = (int64_t)(p.tile1 - 1) * TILE, row_b = a.packed ? 0 : 1;  // of the last tile
+  const char* x = p.at<T>(a.x, row_b * a.xb, a.xt, first);
+  const char* g = p.at<G>(a.g, row_b * a.gb, a.gt, first);
+  const char* dy = p.at<T>(a.dy, row_b * a.yb, a.yt, first);
+  char* dx = const_cast<char*>(p.at<T>(a.dx, row_b * a.T * a.D, a.D, first));
+  char* dg = const_cast<char*>(p.at<G>(a.dg, row_b * a.T * a.D, a.D, first));
+  const unsigned xo = p.lane<T>(a.xt, tr * R), go = p.lane<G>(a.gt, tr * R), yo = p.lane<T>(a.yt, tr * R), dxo = p.lane<T>(a.D, tr * R), dgo = p.lane<G>(a.D, tr * R);
+  const int64_t xs = a.xt * (int64_t)sizeof(T), gs = a.gt * (int64_t)sizeof(G), ys = a.yt * (int64_t)sizeof(T), dxs = a.D * (int64_t)sizeof(T), dgs = a.D * (int64_t)sizeof(G);
+  Raw<T, VEC> xr[R], yr[R];
+  Raw<G, VEC> gr[R];
+  if (!a.dy)
 #pragma unroll
-    for (int u = 0; u < R; ++u) {
-      const int64_t t = (int64_t)tile * TILE + tr * R + u;
-      xr[u].zero();
-      yr[u].zero();
-      gr[u].zero();
-      if (t < p.len && in_c) {
-        if (!SUM) xr[u].template load<VEC>(x + t * a.xt, p.left);
-        if (a.dy) yr[u].template load<VEC>(dy + t * a.yt, p.left);
-        gr[u].template load<VEC>(g + t * a.gt, p.left);
+    for (int u = 0; u < R; ++u) yr[u].zero();
+  const auto fetch = [&](int tile) {
+    if (states && chan < a.D) start = a.kept[(p.slot + tile) * a.D + chan];
+    if ((tile + 1) * (int64_t)TILE <= p.len && p.c0 + C <= a.D) {
+#pragma unroll
+      for (int u = 0; u < R; ++u) {
+        if (!SUM) xr[u].load(elems<T>(x + u * xs, xo), N);
+        gr[u].load(elems<G>(g + u * gs, go), N);
+      }
+      if (a.dy)
+#pragma unroll
+        for (int u = 0; u < R; ++u) yr[u].load(elems<T>(dy + u * ys, yo), N);
+    } else {
+#pragma unroll
+      for (int u = 0; u < R; ++u) {
+        xr[u].zero();
+        yr[u].zero();
+        gr[u].zero();
+        if ((int64_t)tile * TILE + tr * R + u < p.len && in_c) {
+          if (!SUM) xr[u].load(elems<T>(x + u * xs, xo), p.left);
+          if (a.dy) yr[u].load(elems<T>(dy + u * ys, yo), p.left);
+          gr[u].load(elems<G>(g + u * gs, go), p.left);
+        }
       }
     }
   };
   if (p.tile0 < p.tile1) fetch(p.tile1 - 1);
   for (int tile = p.tile1 - 1; tile >= p.tile0; --tile) {
-    float e[R][N], xv[R][N], dyv[R][N], A[N], H[N], Af[N], Hf[N];
+    float e[R][N], A[N], H[N], ea[N], eh[N], Af[N], Hf[N], fa[N], fh[N];
+    Raw<T, VEC> xk[R], yk[R];
 #pragma unroll
     for (int i = 0; i < N; ++i) A[i] = 1.f, H[i] = 0.f, Hf[i] = 0.f;
 #pragma unroll
-    for (int u = R - 1; u >= 0; --u)
+    for (int u = R - 1; u >= 0; --u) {
+      xk[u] = xr[u];
+      yk[u] = yr[u];
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         e[u][i] = __expf(gr[u].get(i));
-        dyv[u][i] = yr[u].get(i);
-        H[i] = e[u][i] * (dyv[u][i] + H[i]);
+        H[i] = e[u][i] * (yk[u].get(i) + H[i]);
         A[i] *= e[u][i];
       }
-    if (!SUM) {
+    }
+    if (!SUM)
 #pragma unroll
       for (int u = 0; u < R; ++u)
 #pragma unroll
-        for (int i = 0; i < N; ++i) xv[u][i] = xr[u].get(i), Hf[i] = e[u][i] * Hf[i] + xv[u][i];
-    }
+        for (int i = 0; i < N; ++i) Hf[i] = e[u][i] * Hf[i] + xk[u].get(i);
     float from = start;
+    x -= TILE * xs;
+    g -= TILE * gs;
+    dy -= TILE * ys;
     if (tile > p.tile0) fetch(tile - 1);
-    if (!SUM) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) Af[i] = A[i];
-      scan_wave<N, true>(Af, Hf, lane);
-      wf.template leave<true>(Af, Hf, lane, wave);
+    for (int i = 0; i < N; ++i) {
+      if (!SUM) {
+        Af[i] = A[i];
+        scan_wave<true>(Af[i], Hf[i], fa[i], fh[i], lane);
+      }
+      scan_wave<false>(A[i], H[i], ea[i], eh[i], lane);
     }
-    scan_wave<N, false>(A, H, lane);
-    ws.template leave<false>(A, H, lane, wave);
+    if (!SUM) wf.leave(Af, Hf, lane, wave);
+    ws.leave(A, H, lane, wave);
     lds_barrier();
-    if (chains) ws.template chain<false>(lane, carry, all);
+    if (chains) ws.chain<false>(lane, carry, all);
     if (states) {
       float none = 1.f;
-      wf.template chain<true>(lane, from, none);
+      wf.chain<true>(lane, from, none);
     }
     lds_barrier();
     if (!SUM) {
       float h[N], o[N], hb[R][N];
-      wf.template enter<true>(Af, Hf, h, lane, wave);
-      ws.template enter<false>(A, H, o, lane, wave);
+      wf.enter(fa, fh, h, lane, wave);
+      ws.enter(ea, eh, o, lane, wave);
+      const bool whole = (tile + 1) * (int64_t)TILE <= p.len && p.c0 + C <= a.D;
 #pragma unroll
       for (int u = 0; u < R; ++u)
 #pragma unroll
-        for (int i = 0; i < N; ++i) hb[u][i] = h[i], h[i] = e[u][i] * h[i] + xv[u][i];
+        for (int i = 0; i < N; ++i) hb[u][i] = h[i], h[i] = e[u][i] * h[i] + xk[u].get(i);
 #pragma unroll
       for (int u = R - 1; u >= 0; --u) {
-        const int64_t t = (int64_t)tile * TILE + tr * R + u;
         float dh[N], dgv[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          dh[i] = dyv[u][i] + o[i];
+          dh[i] = yk[u].get(i) + o[i];
           o[i] = e[u][i] * dh[i];
           dgv[i] = hb[u][i] * o[i];
         }
-        if (t < p.len && in_c) {
-          put<T, N, VEC>(dx + t * a.D, dh, p.left);
-          put<G, N, VEC>(dg + t * a.D, dgv, p.left);
+        if (whole || ((int64_t)tile * TILE + tr * R + u < p.len && in_c)) {
+          put<VEC>(elems<T>(dx + u * dxs, dxo), dh, p.left);
+          put<VEC>(elems<G>(dg + u * dgs, dgo), dgv, p.left);
         }
       }
+      dx -= TILE * dxs;
+      dg -= TILE * dgs;
     }
   }
   if (!in_chan) return;
@@ -356,10 +373,10 @@ template <typename T, typename G, bool VEC, bool SUM> __global__ __launch_bounds
 }
 
 // One token: four elements a thread, or one where the vectors do not fit
-template <typename T, typename G, int N> __global__ __launch_bounds__(256) void linrec_step_kernel(const T* x, const G* g, const float* s, T* y, float* s_out, int64_t n) {
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * N;
+template <typename T, typename G, int W> __global__ __launch_bounds__(256) void linrec_step_kernel(const T* x, const G* g, const float* s, T* y, float* s_out, int64_t n) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * W;
   if (i >= n) return;
-  if (N == 4) {
+  if (W == 4) {
     const floatx4 xv = load4(x + i), gv = load4(g + i), sv = load4(s + i);
     floatx4 h;
 #pragma unroll
@@ -373,16 +390,15 @@ template <typename T, typename G, int N> __global__ __launch_bounds__(256) void 
   }
 }
 
+constexpr int64_t MAX_STRIDE = 4 << 20;
 int rows_of(const lnx_linrec_args* a) { return a->nseq ? a->nseq : a->B; }
-int channel_tiles(const lnx_linrec_args* a) {
-  const int w = TCOLS * (a->dtype == LNX_BF16 ? 8 : 4);
-  return (a->D + w - 1) / w;
-}
+int channel_tiles(const lnx_linrec_args* a) { return (int)(((int64_t)a->D + C - 1) / C); }
+int tile_of(const lnx_linrec_args* a) { return a->dtype == LNX_BF16 ? tile_of<bf16_t>() : tile_of<float>(); }
 
 // Segments of a row's tokens: as many as bring the launch to one workgroup a CU, of four tiles each at least (the first launch
-// reads the inputs once more, so a launch that fills the chip by itself is not cut).
+// reads the inputs once more, so a launch that nearly fills the chip by itself is not cut).
 int segments(const lnx_linrec_args* a) {
-  const int64_t wgs = (int64_t)rows_of(a) * channel_tiles(a), tiles = (a->T + TILE - 1) / TILE;
+  const int64_t wgs = (int64_t)rows_of(a) * channel_tiles(a), tiles = (a->T + (int64_t)tile_of(a) - 1) / tile_of(a);
   int64_t s = wgs >= 160 ? 1 : 256 / (wgs > 0 ? wgs : 1);
   if (s > tiles / 4) s = tiles / 4;
   return s < 1 ? 1 : (int)s;
@@ -399,6 +415,10 @@ int check(const char* what, const lnx_linrec_args* a, bool bwd) {
   if (tokens && (!a->x || !a->g)) return lnx_set_error(LNX_ERR_NULL, "%s: x and g are required", what);
   if (!bwd && ((tokens && !a->y) || (rows && !a->final_state))) return lnx_set_error(LNX_ERR_NULL, "%s: y and final_state are required", what);
   if (bwd && tokens && (!a->d_x || !a->d_g || !a->kept)) return lnx_set_error(LNX_ERR_NULL, "%s: d_x, d_g and kept are required", what);
+  // a lane's bytes within a tile are a 32-bit offset
+  for (int64_t st : {a->x_stride_t * (a->dtype == LNX_BF16 ? 2 : 4), a->g_stride_t * (a->g_dtype == LNX_BF16 ? 2 : 4), (bwd ? a->d_y_stride_t : 0) * (a->dtype == LNX_BF16 ? 2 : 4),
+                     (int64_t)a->D * 4})
+    if (st < 0 || st > MAX_STRIDE) return lnx_set_error(LNX_ERR_SHAPE, "%s: tokens more than %lld bytes apart", what, (long long)MAX_STRIDE);
   if ((int64_t)rows_of(a) * channel_tiles(a) * segments(a) > 0x7fffffff) return lnx_set_error(LNX_ERR_SHAPE, "%s: too many rows", what);
   if (rows && segments(a) > 1) {
     const uint64_t need = lnx_linrec_workspace_bytes(a);
@@ -407,7 +427,7 @@ int check(const char* what, const lnx_linrec_args* a, bool bwd) {
   return LNX_OK;
 }
 
-bool vectors(const void* p, int64_t sb, int64_t st, int64_t size) { return !p || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && sb * size % 16 == 0 && st * size % 16 == 0); }
+bool vectors(const void* p, int64_t sb, int64_t st, int64_t size) { return !p || (reinterpret_cast<uintptr_t>(p) % (4 * size) == 0 && sb % 4 == 0 && st % 4 == 0); }
 
 Args kernel_args(const lnx_linrec_args* a, int segs) {
   Args k{};
@@ -445,12 +465,11 @@ int run(const char* what, const lnx_linrec_args* a, bool bwd, hipStream_t st) {
   if (int rc = check(what, a, bwd)) return rc;
   if (rows_of(a) == 0) return LNX_OK;
   const int64_t xs = a->dtype == LNX_BF16 ? 2 : 4, gs = a->g_dtype == LNX_BF16 ? 2 : 4;
-  // rows as 16-byte vectors: of the inputs with their strides, and of everything that is [.., D] itself
-  bool vec = a->D * xs % 16 == 0 && vectors(a->x, a->x_stride_b, a->x_stride_t, xs) && vectors(a->g, a->g_stride_b, a->g_stride_t, gs) &&
+  // four elements at a time: of the inputs with their strides, and of the outputs, whose rows are D long
+  bool vec = a->D % 4 == 0 && vectors(a->x, a->x_stride_b, a->x_stride_t, xs) && vectors(a->g, a->g_stride_b, a->g_stride_t, gs) &&
              vectors(a->d_y, a->d_y_stride_b, a->d_y_stride_t, xs);
-  for (const void* p : {(const void*)a->initial_state, (const void*)a->y, (const void*)a->final_state, (const void*)a->kept, (const void*)a->workspace,
-                        (const void*)a->d_final_state, (const void*)a->d_x, (const void*)a->d_g, (const void*)a->d_initial_state})
-    vec = vec && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+  for (const void* p : {(const void*)a->y, (const void*)a->d_x}) vec = vec && reinterpret_cast<uintptr_t>(p) % (4 * xs) == 0;
+  vec = vec && reinterpret_cast<uintptr_t>(a->d_g) % (4 * gs) == 0;
   if (a->dtype == LNX_F32) vec ? launch<float, float, true>(a, bwd, st) : launch<float, float, false>(a, bwd, st);
   else if (a->g_dtype == LNX_F32) vec ? launch<bf16_t, float, true>(a, bwd, st) : launch<bf16_t, float, false>(a, bwd, st);
   else vec ? launch<bf16_t, bf16_t, true>(a, bwd, st) : launch<bf16_t, bf16_t, false>(a, bwd, st);
@@ -474,7 +493,7 @@ extern "C" uint64_t lnx_linrec_workspace_bytes(const lnx_linrec_args* a) {
 
 extern "C" uint64_t lnx_linrec_kept_bytes(const lnx_linrec_args* a) {
   if (!a || a->D <= 0 || a->T < 0 || rows_of(a) <= 0) return 0;
-  const int kept = a->dtype == LNX_BF16 ? kept_tokens<bf16_t>() : kept_tokens<float>();
+  const int kept = tile_of(a);
   const uint64_t slots = a->nseq ? (uint64_t)a->T / kept + a->nseq : (uint64_t)a->B * ((a->T + kept - 1) / kept);
   return slots * a->D * sizeof(float);
 }
