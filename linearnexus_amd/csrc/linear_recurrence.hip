@@ -1,13 +1,13 @@
 // Element-wise gated linear recurrence over [rows, T, D] tensors, dense or packed, forward, backward and one token:
 //   h_t = e^{g_t} h_{t-1} + x_t,  y_t = h_t                                    (h_0 the initial state, g log-decays)
 //   dh_t = dy_t + e^{g_{t+1}} dh_{t+1},  dx_t = dh_t,  dg_t = e^{g_t} h_{t-1} dh_t,  dh_0 = e^{g_1} dh_1
-// No products to speak of: every pass is bound by the bytes of its tensors.  A workgroup owns 64 channels of one row and walks its
-// tokens in tiles: a thread holds four channels of R consecutive tokens and reduces them to a pair (A, H), the map h -> A h + H; pairs
-// are scanned over the four token groups of a wave by lane swaps, and the eight waves' pairs are chained through LDS by one lane per
+// No products to speak of: every pass is bound by the bytes of its tensors.  A workgroup owns 128 bytes of channels of one row and walks
+// its tokens in tiles: a thread holds four channels of R consecutive tokens and reduces them to a pair (A, H), the map h -> A h + H;
+// pairs are scanned over the token groups of a wave by lane swaps, and the eight waves' pairs are chained through LDS by one lane per
 // channel, which carries the state from tile to tile.  The loads of the next tile are in flight meanwhile.  (Eight channels of four
 // tokens a thread, scanned over eight groups by shuffles, were bound by the scan: 4.1 TB/s at [8, 4096, 2048] bf16, the same with
 // twice the loads in flight.)  Everything between loads and stores is fp32.  The backward pass reads x again instead of y, which is
-// rounded: the forward pass leaves the state entering every tile (fp32, 1 / 256 of bf16's elements, 1 / 128 of fp32's), so the states
+// rounded: the forward pass leaves the state entering every tile (fp32, 1 / 256 of the elements), so the states
 // behind dg are the unrounded ones.
 // Where rows and channels give too few workgroups the tokens are cut into segments: a first launch reduces every segment to its
 // pair, the second one starts each segment from the folded pairs before it.  No atomics: results are the same from run to run.
@@ -16,10 +16,12 @@
 
 namespace {
 
-constexpr int THREADS = 512, WAVES = 8, TCOLS = 16, TROWS = THREADS / TCOLS, N = 4, C = TCOLS * N;  // C channels a workgroup
-// Tokens per thread: what the backward pass's registers take
-template <typename T> constexpr int tokens() { return sizeof(T) == 2 ? 8 : 4; }
-template <typename T> constexpr int tile_of() { return tokens<T>() * TROWS; }
+constexpr int THREADS = 512, WAVES = 8, N = 4, TILE = 256;  // tokens of a tile
+// By element type: threads side by side in a row, so that a row of a workgroup is 128 bytes; its channels; tokens per thread (what the
+// backward pass's registers take)
+template <typename T> struct Shape {
+  static constexpr int COLS = sizeof(T) == 2 ? 16 : 8, C = COLS * N, R = TILE * COLS / THREADS;
+};
 
 // Four consecutive elements as they lie in memory
 template <typename E, bool VEC> struct Raw {
@@ -54,10 +56,10 @@ struct Args {
 };
 
 // What a workgroup works on: row, its channels, its tiles
-struct Place {
+template <typename T> struct Place {
   int row, seg, len, ntile, per, tile0, tile1, c0, c, left;  // c0: the workgroup's first channel, c: this thread's
   int64_t tok, slot;  // first token in a packed batch (0 otherwise); first kept state
-  __device__ __forceinline__ Place(const Args& a, int tile) {
+  __device__ __forceinline__ Place(const Args& a) {
     const int ct = blockIdx.x % a.ctiles, rs = blockIdx.x / a.ctiles;
     seg = rs % a.segs;
     row = rs / a.segs;
@@ -65,18 +67,18 @@ struct Place {
       const int first = seq_first(a.cu, row, a.T);
       len = seq_end(a.cu, row, a.T) - first;
       tok = first;
-      slot = first / tile + row;
+      slot = first / TILE + row;
     } else {
       len = a.T;
       tok = 0;
-      slot = (int64_t)row * ((a.T + tile - 1) / tile);
+      slot = (int64_t)row * ((a.T + TILE - 1) / TILE);
     }
-    ntile = (len + tile - 1) / tile;
+    ntile = (len + TILE - 1) / TILE;
     per = (ntile + a.segs - 1) / a.segs;
     tile0 = min(seg * per, ntile);
     tile1 = min(tile0 + per, ntile);
-    c0 = ct * C;
-    c = c0 + (threadIdx.x & (TCOLS - 1)) * N;
+    c0 = ct * Shape<T>::C;
+    c = c0 + (threadIdx.x & (Shape<T>::COLS - 1)) * N;
     left = a.D - c;
   }
   // Token `first` of the row: the wave's pointer and the lane's bytes from there, so that addresses are formed in scalar registers
@@ -88,9 +90,9 @@ struct Place {
 template <typename E> __device__ __forceinline__ const E* elems(const char* p, unsigned off) { return reinterpret_cast<const E*>(p + off); }
 template <typename E> __device__ __forceinline__ E* elems(char* p, unsigned off) { return reinterpret_cast<E*>(p + off); }
 
-// (a, h): a thread's pair.  Afterwards the wave's pair, and in (ea, eh) that of the wave's groups (16 lanes each) before this one,
-// upwards or downwards in time.
-template <bool UP> __device__ __forceinline__ void scan_wave(float& a, float& h, float& ea, float& eh, int lane) {
+// (a, h): a thread's pair.  Afterwards the wave's pair, and in (ea, eh) that of the wave's groups (16 lanes each, or 8) before this
+// one, upwards or downwards in time.
+template <bool UP> __device__ __forceinline__ void scan16(float& a, float& h, float& ea, float& eh, int lane) {
   const auto a16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(a), false, false);  // even groups' values, odd groups'
   const auto h16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(h), __float_as_uint(h), false, false);
   const float a1 = __uint_as_float(UP ? a16[0] : a16[1]), h1 = __uint_as_float(UP ? h16[0] : h16[1]);  // the first of two groups
@@ -111,11 +113,27 @@ template <bool UP> __device__ __forceinline__ void scan_wave(float& a, float& h,
   }
 }
 
+template <int COLS, bool UP> __device__ __forceinline__ void scan_wave(float& a, float& h, float& ea, float& eh, int lane) {
+  if (COLS == 16) return scan16<UP>(a, h, ea, eh, lane);
+  const float ao = __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(a), 0x128, 0xF, 0xF, true));  // row_ror:8, the other group of 16 lanes
+  const float ho = __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(h), 0x128, 0xF, 0xF, true));
+  const bool second = ((lane >> 3) & 1) == (UP ? 1 : 0);
+  const float own_a = a, own_h = h;
+  a = own_a * ao;
+  h = second ? own_a * ho + own_h : ao * own_h + ho;
+  scan16<UP>(a, h, ea, eh, lane);
+  if (second) {  // before this group: what came before the two, then the other one
+    eh = ao * eh + ho;
+    ea *= ao;
+  }
+}
+
 // The eight waves' pairs and the states entering the waves, by channel of the workgroup
-struct Waves {
+template <int COLS> struct Waves {
+  static constexpr int C = COLS * N;
   float A[WAVES][C], H[WAVES][C], in[WAVES][C];
   __device__ __forceinline__ void leave(const float (&a)[N], const float (&h)[N], int lane, int wave) {
-    if (lane < TCOLS) {
+    if (lane < COLS) {
       store4(&A[wave][lane * N], floatx4{a[0], a[1], a[2], a[3]});
       store4(&H[wave][lane * N], floatx4{h[0], h[1], h[2], h[3]});
     }
@@ -135,7 +153,7 @@ struct Waves {
   }
   // the state entering this thread's tokens
   __device__ __forceinline__ void enter(const float (&ea)[N], const float (&eh)[N], float (&s)[N], int lane, int wave) const {
-    const floatx4 from = load4(&in[wave][(lane & (TCOLS - 1)) * N]);
+    const floatx4 from = load4(&in[wave][(lane & (COLS - 1)) * N]);
 #pragma unroll
     for (int i = 0; i < N; ++i) s[i] = ea[i] * from[i] + eh[i];
   }
@@ -143,15 +161,15 @@ struct Waves {
 
 // SUM: only the pair of each segment (but the last, which nothing follows)
 template <typename T, typename G, bool VEC, bool SUM> __global__ __launch_bounds__(THREADS) void linrec_fwd_kernel(Args a) {
-  constexpr int R = tokens<T>(), TILE = tile_of<T>();
-  __shared__ Waves ws;
-  const Place p(a, TILE);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tr = threadIdx.x / TCOLS;
+  constexpr int R = Shape<T>::R, COLS = Shape<T>::COLS, C = Shape<T>::C;
+  __shared__ Waves<COLS> ws;
+  const Place<T> p(a);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tr = threadIdx.x / COLS;
   if (SUM && p.tile1 >= p.ntile) return;
   const bool in_c = p.left > 0;
   // the chain's lanes: one channel each
   const int chan = p.c0 + lane;
-  const bool chains = wave == 0, in_chan = chains && chan < a.D;
+  const bool chains = wave == 0 && lane < C, in_chan = chains && chan < a.D;
   const int64_t row_c = (int64_t)p.row * a.D + chan;
   float carry = 0.f, all = 1.f;
   if (!SUM && in_chan) {
@@ -163,10 +181,10 @@ template <typename T, typename G, bool VEC, bool SUM> __global__ __launch_bounds
       }
   }
   const int64_t first = (int64_t)p.tile0 * TILE, row_b = a.packed ? 0 : 1;  // a packed batch is one row
-  const char* x = p.at<T>(a.x, row_b * a.xb, a.xt, first);
-  const char* g = p.at<G>(a.g, row_b * a.gb, a.gt, first);
-  char* y = const_cast<char*>(p.at<T>(a.y, row_b * a.T * a.D, a.D, first));
-  const unsigned xo = p.lane<T>(a.xt, tr * R), go = p.lane<G>(a.gt, tr * R), yo = p.lane<T>(a.D, tr * R);
+  const char* x = p.template at<T>(a.x, row_b * a.xb, a.xt, first);
+  const char* g = p.template at<G>(a.g, row_b * a.gb, a.gt, first);
+  char* y = const_cast<char*>(p.template at<T>(a.y, row_b * a.T * a.D, a.D, first));
+  const unsigned xo = p.template lane<T>(a.xt, tr * R), go = p.template lane<G>(a.gt, tr * R), yo = p.template lane<T>(a.D, tr * R);
   const int64_t xs = a.xt * (int64_t)sizeof(T), gs = a.gt * (int64_t)sizeof(G), ys = a.D * (int64_t)sizeof(T);
   Raw<T, VEC> xr[R];
   Raw<G, VEC> gr[R];
@@ -202,12 +220,12 @@ template <typename T, typename G, bool VEC, bool SUM> __global__ __launch_bounds
     g += TILE * gs;
     if (tile + 1 < p.tile1) fetch(tile + 1);
 #pragma unroll
-    for (int i = 0; i < N; ++i) scan_wave<true>(A[i], H[i], ea[i], eh[i], lane);
+    for (int i = 0; i < N; ++i) scan_wave<COLS, true>(A[i], H[i], ea[i], eh[i], lane);
     ws.leave(A, H, lane, wave);
     lds_barrier();
     if (chains) {
       if (!SUM && a.kept && in_chan) a.kept[(p.slot + tile) * a.D + chan] = carry;
-      ws.chain<true>(lane, carry, all);
+      ws.template chain<true>(lane, carry, all);
     }
     lds_barrier();
     if (!SUM) {
@@ -235,14 +253,14 @@ template <typename T, typename G, bool VEC, bool SUM> __global__ __launch_bounds
 
 // Backwards in time: o is e^{g_{t+1}} dh_{t+1}.  SUM: only the pair of each segment (but the first, which nothing precedes)
 template <typename T, typename G, bool VEC, bool SUM> __global__ __launch_bounds__(THREADS) void linrec_bwd_kernel(Args a) {
-  constexpr int R = tokens<T>(), TILE = tile_of<T>();
-  __shared__ Waves ws, wf;
-  const Place p(a, TILE);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tr = threadIdx.x / TCOLS;
+  constexpr int R = Shape<T>::R, COLS = Shape<T>::COLS, C = Shape<T>::C;
+  __shared__ Waves<COLS> ws, wf;
+  const Place<T> p(a);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tr = threadIdx.x / COLS;
   if (SUM && (p.seg == 0 || p.tile0 >= p.tile1)) return;
   const bool in_c = p.left > 0;
   const int chan = p.c0 + lane;  // wave 0 chains the gradients, wave 1 the states
-  const bool chains = wave == 0, in_chan = chains && chan < a.D, states = !SUM && wave == 1;
+  const bool chains = wave == 0 && lane < C, in_chan = chains && chan < a.D, states = !SUM && wave == 1 && lane < C;
   const int64_t row_c = (int64_t)p.row * a.D + chan;
   float carry = 0.f, all = 1.f, start = 0.f;
   if (!SUM && in_chan) {
@@ -254,12 +272,12 @@ template <typename T, typename G, bool VEC, bool SUM> __global__ __launch_bounds
       }
   }
   const int64_t first = (int64_t)(p.tile1 - 1) * TILE, row_b = a.packed ? 0 : 1;  // of the last tile
-  const char* x = p.at<T>(a.x, row_b * a.xb, a.xt, first);
-  const char* g = p.at<G>(a.g, row_b * a.gb, a.gt, first);
-  const char* dy = p.at<T>(a.dy, row_b * a.yb, a.yt, first);
-  char* dx = const_cast<char*>(p.at<T>(a.dx, row_b * a.T * a.D, a.D, first));
-  char* dg = const_cast<char*>(p.at<G>(a.dg, row_b * a.T * a.D, a.D, first));
-  const unsigned xo = p.lane<T>(a.xt, tr * R), go = p.lane<G>(a.gt, tr * R), yo = p.lane<T>(a.yt, tr * R), dxo = p.lane<T>(a.D, tr * R), dgo = p.lane<G>(a.D, tr * R);
+  const char* x = p.template at<T>(a.x, row_b * a.xb, a.xt, first);
+  const char* g = p.template at<G>(a.g, row_b * a.gb, a.gt, first);
+  const char* dy = p.template at<T>(a.dy, row_b * a.yb, a.yt, first);
+  char* dx = const_cast<char*>(p.template at<T>(a.dx, row_b * a.T * a.D, a.D, first));
+  char* dg = const_cast<char*>(p.template at<G>(a.dg, row_b * a.T * a.D, a.D, first));
+  const unsigned xo = p.template lane<T>(a.xt, tr * R), go = p.template lane<G>(a.gt, tr * R), yo = p.template lane<T>(a.yt, tr * R), dxo = p.template lane<T>(a.D, tr * R), dgo = p.template lane<G>(a.D, tr * R);
   const int64_t xs = a.xt * (int64_t)sizeof(T), gs = a.gt * (int64_t)sizeof(G), ys = a.yt * (int64_t)sizeof(T), dxs = a.D * (int64_t)sizeof(T), dgs = a.D * (int64_t)sizeof(G);
   Raw<T, VEC> xr[R], yr[R];
   Raw<G, VEC> gr[R];
@@ -322,17 +340,17 @@ template <typename T, typename G, bool VEC, bool SUM> __global__ __launch_bounds
     for (int i = 0; i < N; ++i) {
       if (!SUM) {
         Af[i] = A[i];
-        scan_wave<true>(Af[i], Hf[i], fa[i], fh[i], lane);
+        scan_wave<COLS, true>(Af[i], Hf[i], fa[i], fh[i], lane);
       }
-      scan_wave<false>(A[i], H[i], ea[i], eh[i], lane);
+      scan_wave<COLS, false>(A[i], H[i], ea[i], eh[i], lane);
     }
     if (!SUM) wf.leave(Af, Hf, lane, wave);
     ws.leave(A, H, lane, wave);
     lds_barrier();
-    if (chains) ws.chain<false>(lane, carry, all);
+    if (chains) ws.template chain<false>(lane, carry, all);
     if (states) {
       float none = 1.f;
-      wf.chain<true>(lane, from, none);
+      wf.template chain<true>(lane, from, none);
     }
     lds_barrier();
     if (!SUM) {
@@ -392,13 +410,15 @@ template <typename T, typename G, int W> __global__ __launch_bounds__(256) void 
 
 constexpr int64_t MAX_STRIDE = 4 << 20;
 int rows_of(const lnx_linrec_args* a) { return a->nseq ? a->nseq : a->B; }
-int channel_tiles(const lnx_linrec_args* a) { return (int)(((int64_t)a->D + C - 1) / C); }
-int tile_of(const lnx_linrec_args* a) { return a->dtype == LNX_BF16 ? tile_of<bf16_t>() : tile_of<float>(); }
+int channel_tiles(const lnx_linrec_args* a) {
+  const int c = a->dtype == LNX_BF16 ? Shape<bf16_t>::C : Shape<float>::C;
+  return (int)(((int64_t)a->D + c - 1) / c);
+}
 
 // Segments of a row's tokens: as many as bring the launch to one workgroup a CU, of four tiles each at least (the first launch
 // reads the inputs once more, so a launch that nearly fills the chip by itself is not cut).
 int segments(const lnx_linrec_args* a) {
-  const int64_t wgs = (int64_t)rows_of(a) * channel_tiles(a), tiles = (a->T + (int64_t)tile_of(a) - 1) / tile_of(a);
+  const int64_t wgs = (int64_t)rows_of(a) * channel_tiles(a), len = a->nseq ? a->T / a->nseq : a->T, tiles = (len + TILE - 1) / TILE;  // of the average sequence
   int64_t s = wgs >= 160 ? 1 : 256 / (wgs > 0 ? wgs : 1);
   if (s > tiles / 4) s = tiles / 4;
   return s < 1 ? 1 : (int)s;
@@ -493,8 +513,7 @@ extern "C" uint64_t lnx_linrec_workspace_bytes(const lnx_linrec_args* a) {
 
 extern "C" uint64_t lnx_linrec_kept_bytes(const lnx_linrec_args* a) {
   if (!a || a->D <= 0 || a->T < 0 || rows_of(a) <= 0) return 0;
-  const int kept = tile_of(a);
-  const uint64_t slots = a->nseq ? (uint64_t)a->T / kept + a->nseq : (uint64_t)a->B * ((a->T + kept - 1) / kept);
+  const uint64_t slots = a->nseq ? (uint64_t)a->T / TILE + a->nseq : (uint64_t)a->B * (((int64_t)a->T + TILE - 1) / TILE);
   return slots * a->D * sizeof(float);
 }
 
