@@ -370,11 +370,13 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int e = 0; e < 16; ++e) sc[i][e] = 0.f;
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int s = 0; s < D / 16; ++s) mma(sc[i], TL::by_row(rows, 32 * i * TL::ROWB, s), qf[s]);
     read_ahead<T, false, 2 * (D / 16), 4>();
+    __builtin_amdgcn_s_setprio(0);
     if (key0 + ROWS - 1 > q0) {
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -558,12 +560,14 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
         floatx16 sc, dp;
 #pragma unroll
         for (int e = 0; e < 16; ++e) sc[e] = dp[e] = 0.f;
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int s = 0; s < D / 16; ++s) {
           mma(sc, TL::by_row(rows, 32 * i * TL::ROWB, s), qf[s]);
           mma(dp, TL::by_row(rows, TL::BYTES + 32 * i * TL::ROWB, s), gf[s]);
         }
         read_ahead<T, false, 2 * (D / 16), 4>();
+        __builtin_amdgcn_s_setprio(0);
 #pragma unroll
         for (int e = 0; e < 16; ++e) sc[e] = __builtin_amdgcn_exp2f(sc[e] * c - lse) * (dp[e] - delta);
         if (key0 + 32 * i + 31 > q0)
@@ -703,11 +707,13 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
       floatx16 sc, dp;
 #pragma unroll
       for (int e = 0; e < 16; ++e) sc[e] = dp[e] = 0.f;
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int s = 0; s < D / 16; ++s) mma(sc, TL::by_row(rows, 0, s), kf[s]);
 #pragma unroll
       for (int s = 0; s < D / 16; ++s) mma(dp, TL::by_row(rows, TL::BYTES, s), vf[s]);
       read_ahead<T, false, 2 * (D / 16), 4>();
+      __builtin_amdgcn_s_setprio(0);
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         sc[e] = __builtin_amdgcn_exp2f(sc[e] * c - lse[e >> 2][e & 3]);
