@@ -473,7 +473,8 @@ int lnx_rmsnorm_residual_bwd(const lnx_rmsnorm_residual_args* a, void* hip_strea
  * 0 .. i; query head h reads key head h / (H / Hkv).  q, o, d_o, d_q are [B, H, T, d], k, v, d_k, d_v [B, Hkv, T, d] in `dtype`,
  * each with its own strides (in elements, rows contiguous, every stride and pointer a multiple of 16 bytes, tokens at most
  * 16 MiB apart; an input's stride may be 0).  d <= 128 and a multiple of 8.  Packed batches as above.  lse [B, H, T] fp32 is written by the forward call if not
- * NULL and read by the backward call, which also reads o; a workspace (16-byte aligned, may be NULL where its size is 0)
+ * NULL and read by the backward call, which also reads o and o_low, [B, H, T, d] dense in `dtype`: what the rounding of o left (NULL
+ * in both calls: taken as zero, as it is in fp32); a workspace (16-byte aligned, may be NULL where its size is 0)
  * holds nothing between calls.  Where batch and heads give few workgroups the keys (queries) are split between several and their
  * fp32 shares added in order: no atomics, results are the same from run to run.
  */
@@ -487,6 +488,7 @@ typedef struct lnx_attn_args {
   lnx_tensor4 q, k, v, o;
   lnx_tensor4 d_o, d_q, d_k, d_v;  /* backward only */
   float* lse;
+  void* o_low;
   const int32_t* cu_seqlens;
   void* workspace;
   uint64_t workspace_bytes;

@@ -107,7 +107,7 @@ class AttnArgs(C.Structure):
         ("B", C.c_int32), ("H", C.c_int32), ("Hkv", C.c_int32), ("T", C.c_int32), ("d", C.c_int32), ("nseq", C.c_int32), ("dtype", C.c_int32),
         ("scale", C.c_float),
         ("q", Tensor4), ("k", Tensor4), ("v", Tensor4), ("o", Tensor4), ("d_o", Tensor4), ("d_q", Tensor4), ("d_k", Tensor4), ("d_v", Tensor4),
-        ("lse", C.c_void_p), ("cu_seqlens", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
+        ("lse", C.c_void_p), ("o_low", C.c_void_p), ("cu_seqlens", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
     ]
 
 

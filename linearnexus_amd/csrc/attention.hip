@@ -21,7 +21,7 @@ __device__ __forceinline__ unsigned fresh(unsigned x) { return (unsigned)::fresh
 
 struct Args {
   const void *q, *k, *v, *dout;
-  void *o, *dq, *dk, *dv;
+  void *o, *o_low, *dq, *dk, *dv;  // o_low [B, H, T, d]: what o's rounding left
   float *lse, *delta;  // [B, H, T]; lse in units of log 2
   const int32_t* cu;
   int64_t qs[3], ks[3], vs[3], os[3], gs[3], dqs[3], dks[3], dvs[3];  // strides of batch, head, token in elements
@@ -312,6 +312,23 @@ template <typename T, int M> __device__ __forceinline__ void store_column(T* p, 
     }
 }
 
+// What the rounding of such a column left
+template <typename T, int M> __device__ __forceinline__ void store_low(T* p, const floatx16 (&acc)[M], float f, int d, int lane) {
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int c = 32 * m + 8 * q + 4 * (lane >> 5);
+      floatx4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = acc[m][4 * q + e] * f;
+        v[e] = x - to_f32(from_f32<T>(x));
+      }
+      if (c < d) store4(p + c, v);
+    }
+}
+
 // A wave owns 32 queries, the workgroup 128; of a block's key tiles every a.parts-th.
 template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kernel(Args a) {
   typedef Tile<T, D> TL;
@@ -431,6 +448,7 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
   const int64_t row = ((int64_t)p.b * a.H + h) * a.T + p.tok + q;
   if (a.parts == 1) {
     store_column<T, D / 32>(at<T>(a.o, a.os, p.b, h, p.tok + q), acc, 1.f / sum, a.d, lane);
+    if (a.o_low) store_low<T, D / 32>(static_cast<T*>(a.o_low) + row * a.d, acc, 1.f / sum, a.d, lane);
     if (a.lse && kg == 0) a.lse[row] = m * c + __builtin_amdgcn_logf(sum);
   } else {
     const int64_t at_part = (int64_t)p.part * a.B * a.H * a.T + row;
@@ -458,8 +476,17 @@ template <typename T> __global__ __launch_bounds__(256) void attn_join_kernel(Ar
   }
   const int64_t t = row % a.T, bh = row / a.T;
   T* p = at<T>(a.o, a.os, bh / a.H, bh % a.H, t) + c;
-  store4(p, floatx4{o[0] / sum, o[1] / sum, o[2] / sum, o[3] / sum});
-  store4(p + 4, floatx4{o[4] / sum, o[5] / sum, o[6] / sum, o[7] / sum});
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o[e] /= sum;
+  store4(p, floatx4{o[0], o[1], o[2], o[3]});
+  store4(p + 4, floatx4{o[4], o[5], o[6], o[7]});
+  if (a.o_low) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] -= to_f32(from_f32<T>(o[e]));
+    T* low = static_cast<T*>(a.o_low) + row * a.d + c;
+    store4(low, floatx4{o[0], o[1], o[2], o[3]});
+    store4(low + 4, floatx4{o[4], o[5], o[6], o[7]});
+  }
   if (a.lse && c == 0) a.lse[row] = top + __builtin_amdgcn_logf(sum);
 }
 
@@ -481,26 +508,9 @@ template <typename T> __global__ __launch_bounds__(256) void attn_sum_kernel(con
   store4(p + 4, y);
 }
 
-// delta_i = o_i . do_i, sixteen lanes a row
-template <typename T> __global__ __launch_bounds__(256) void attn_delta_kernel(Args a) {
-  const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-  const int li = threadIdx.x & 15;
-  float s = 0.f;
-  if (row < (int64_t)a.B * a.H * a.T) {
-    const int64_t t = row % a.T, bh = row / a.T;
-    const T* o = at<T>(a.o, a.os, bh / a.H, bh % a.H, t) + 8 * li;
-    const T* g = at<T>(a.dout, a.gs, bh / a.H, bh % a.H, t) + 8 * li;
-    Frag8<T> x, y;
-    from_global<T>(x, o, 8 * li < a.d);
-    from_global<T>(y, g, 8 * li < a.d);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) s += to_f32(x.v[e]) * to_f32(y.v[e]);
-  }
-  s = row16_sum(s);
-  if (li == 0 && row < (int64_t)a.B * a.H * a.T) a.delta[row] = s;
-}
-
-// Queries as in the forward pass, their gradients beside them in registers.
+// Queries as in the forward pass, their gradients beside them in registers.  delta is formed here, for the dk / dv kernel too: of o and
+// what its rounding left, because an error of delta goes into every term of a row of dq (rounded o alone: 1.5 times the error that the
+// rounding of dq has, with it 1.4).
 template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(Args a) {
   typedef Tile<T, D> TL;
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -525,15 +535,26 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
   }
   const float c = a.scale * LOG2E;
   const int64_t row = min(q, p.len - 1), stat = ((int64_t)p.b * a.H + h) * a.T + p.tok + row;
-  const float lse = a.lse[stat], delta = a.delta[stat];
+  const float lse = a.lse[stat];
   const T* qr = at<T>(a.q, a.qs, p.b, h, p.tok + row);
   const T* gr = at<T>(a.dout, a.gs, p.b, h, p.tok + row);
+  const T* orow = at<T>(a.o, a.os, p.b, h, p.tok + row);
+  const T* lrow = a.o_low ? static_cast<const T*>(a.o_low) + stat * a.d : nullptr;
   Frag8<T> qf[D / 16], gf[D / 16];
+  float delta = 0.f;
 #pragma unroll
   for (int s = 0; s < D / 16; ++s) {
-    from_global<T>(qf[s], qr + 16 * s + 8 * kg, 16 * s + 8 * kg < a.d);
-    from_global<T>(gf[s], gr + 16 * s + 8 * kg, 16 * s + 8 * kg < a.d);
+    const int at = 16 * s + 8 * kg;
+    from_global<T>(qf[s], qr + at, at < a.d);
+    from_global<T>(gf[s], gr + at, at < a.d);
+    Frag8<T> o, low;
+    from_global<T>(o, orow + at, at < a.d);
+    from_global<T>(low, lrow + at, lrow && at < a.d);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) delta += (to_f32(o.v[e]) + to_f32(low.v[e])) * to_f32(gf[s].v[e]);
   }
+  delta = xor32_sum(delta);
+  if (kg == 0 && q < p.len) a.delta[stat] = delta;  // every part writes the same
   floatx16 acc[D / 32];
 #pragma unroll
   for (int i = 0; i < D / 32; ++i)
@@ -839,6 +860,7 @@ int check(const char* what, const lnx_attn_args* a, bool bwd) {
     if (!rows_fit(ts[i], a->dtype == LNX_BF16 ? 2 : 4)) return lnx_set_error(LNX_ERR_SHAPE, "%s: tensors must be 16-byte aligned, rows whole numbers of 16 bytes and at most 16 MiB apart", what);
   }
   if (bwd && !a->lse) return lnx_set_error(LNX_ERR_NULL, "%s: lse is required", what);
+  if (a->o_low && reinterpret_cast<uintptr_t>(a->o_low) % 16) return lnx_set_error(LNX_ERR_SHAPE, "%s: o_low must be 16-byte aligned", what);
   const uint64_t need = bwd ? bwd_bytes(a) : fwd_bytes(a);
   if (need && (!a->workspace || a->workspace_bytes < need || reinterpret_cast<uintptr_t>(a->workspace) % 16))
     return lnx_set_error(LNX_ERR_WORKSPACE, "%s: needs a 16-byte aligned workspace of %llu bytes", what, (unsigned long long)need);
@@ -852,7 +874,7 @@ Args kernel_args(const lnx_attn_args* a) {
   auto strides = [](int64_t (&s)[3], const lnx_tensor4& t) { s[0] = t.stride_b, s[1] = t.stride_h, s[2] = t.stride_t; };
   k.q = a->q.p, k.k = a->k.p, k.v = a->v.p, k.dout = a->d_o.p, k.o = a->o.p, k.dq = a->d_q.p, k.dk = a->d_k.p, k.dv = a->d_v.p;
   strides(k.qs, a->q), strides(k.ks, a->k), strides(k.vs, a->v), strides(k.os, a->o), strides(k.gs, a->d_o), strides(k.dqs, a->d_q), strides(k.dks, a->d_k), strides(k.dvs, a->d_v);
-  k.lse = a->lse, k.cu = a->cu_seqlens;
+  k.lse = a->lse, k.o_low = a->o_low, k.cu = a->cu_seqlens;
   k.B = a->B, k.H = a->H, k.Hkv = a->Hkv, k.G = a->H / a->Hkv, k.T = a->T, k.d = a->d, k.nseq = a->nseq, k.scale = a->scale;
   return k;
 }
@@ -886,8 +908,9 @@ template <typename T, int D> int launch_bwd(const lnx_attn_args* a, hipStream_t 
   Args k = kernel_args(a);
   k.delta = static_cast<float*>(a->workspace);
   k.part = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + delta_bytes(a));
-  lnx_profile_mark("attn_delta", st);
-  attn_delta_kernel<T><<<dim3((unsigned)(((int64_t)k.B * k.H * k.T + 15) / 16)), 256, 0, st>>>(k);
+  k.nblk = (int)blocks_of(a, 128), k.parts = parts_of(a, DQ);  // first: it leaves delta
+  if (int rc = start(attn_dq_kernel<T, D>, "attn_dq", k, (int64_t)k.B * k.H * k.nblk * k.parts, 4 * Tile<T, D>::BYTES + 16, st)) return rc;
+  if (k.parts > 1) sum_parts<T>(k, k.part, (int64_t)k.B * k.H * k.T, k.dq, k.dqs, k.H, st);
   k.nblk = (int)blocks_of(a, ROWS), k.parts = parts_of(a, DKV);
   if (int rc = start(attn_dkv_kernel<T, D>, "attn_dkv", k, (int64_t)k.B * k.Hkv * k.nblk * k.parts, 4 * Tile<T, D>::BYTES + 8192 * sizeof(T), st)) return rc;
   if (k.parts > 1) {
@@ -895,9 +918,6 @@ template <typename T, int D> int launch_bwd(const lnx_attn_args* a, hipStream_t 
     sum_parts<T>(k, k.part, 2 * rows, k.dk, k.dks, k.Hkv, st);
     sum_parts<T>(k, k.part + rows * k.d, 2 * rows, k.dv, k.dvs, k.Hkv, st);
   }
-  k.nblk = (int)blocks_of(a, 128), k.parts = parts_of(a, DQ);
-  if (int rc = start(attn_dq_kernel<T, D>, "attn_dq", k, (int64_t)k.B * k.H * k.nblk * k.parts, 4 * Tile<T, D>::BYTES + 16, st)) return rc;
-  if (k.parts > 1) sum_parts<T>(k, k.part, (int64_t)k.B * k.H * k.T, k.dq, k.dqs, k.H, st);
   return LNX_OK;
 }
 

@@ -1391,10 +1391,10 @@ lnx_attn_args attention_args(const Tensor& q, const Tensor& k, const Tensor& v, 
 
 Tensor empty_rows(const Tensor& like, bool token_first) { return empty_layout(like.size(0), like.size(1), like.size(2), like.size(3), like.options(), token_first); }
 
-Tensor attention_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu, double scale, const Tensor& lse) {
+Tensor attention_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu, double scale, const Tensor& lse, const Tensor& low) {
   const Tensor o = empty_rows(q, is_token_first(q));
   lnx_attn_args a = attention_args(q, k, v, o, cu, scale);
-  a.lse = fptr(lse);
+  a.lse = fptr(lse), a.o_low = ptr(low);
   a.workspace_bytes = lnx_attn_fwd_workspace_bytes(&a);
   Tensor ws;
   if (a.workspace_bytes) ws = work_area(q, a.workspace_bytes);
@@ -1407,8 +1407,9 @@ Tensor attention_forward(const Tensor& q, const Tensor& k, const Tensor& v, cons
 struct AttentionFn : Function<AttentionFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q0, const Tensor& k0, const Tensor& v0, const OptT& cu, double scale) {
     const Tensor q = as_rows(q0), k = as_rows(k0), v = as_rows(v0), lse = at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
-    const Tensor o = attention_forward(q, k, v, undef(cu), scale, lse);
-    ctx->save_for_backward({q, k, v, o, lse, undef(cu)});
+    const Tensor low = q.scalar_type() == at::kFloat ? Tensor() : at::empty(q.sizes(), q.options());
+    const Tensor o = attention_forward(q, k, v, undef(cu), scale, lse, low);
+    ctx->save_for_backward({q, k, v, o, lse, undef(cu), low});
     ctx->saved_data["d"] = scale;
     return o;
   }
@@ -1419,7 +1420,7 @@ struct AttentionFn : Function<AttentionFn> {
     const Tensor d_o = as_rows(grads[0].to(q.scalar_type()));
     Tensor dq = empty_rows(q, is_token_first(q)), dk = empty_rows(k, is_token_first(k)), dv = empty_rows(v, is_token_first(v));
     lnx_attn_args a = attention_args(q, k, v, o, cu, ctx->saved_data["d"].toDouble());
-    a.d_o = tensor4(d_o), a.d_q = tensor4(dq), a.d_k = tensor4(dk), a.d_v = tensor4(dv), a.lse = fptr(lse);
+    a.d_o = tensor4(d_o), a.d_q = tensor4(dq), a.d_k = tensor4(dk), a.d_v = tensor4(dv), a.lse = fptr(lse), a.o_low = ptr(s[6]);
     a.workspace_bytes = lnx_attn_bwd_workspace_bytes(&a);
     const Tensor ws = work_area(q, a.workspace_bytes);
     a.workspace = ptr(ws);
@@ -1445,7 +1446,7 @@ PyObject* py_causal_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs
     const int64_t d = q.size(3), more = (8 - d % 8) % 8;  // zero columns change no product
     auto wide = [&](const Tensor& t) { return more ? at::constant_pad_nd(t, {0, more}) : t; };
     const Tensor qw = wide(q), kw = wide(k), vw = wide(v);
-    const Tensor o = wants_grad({&q, &k, &v}) ? AttentionFn::apply(qw, kw, vw, opt(cu), scale) : attention_forward(as_rows(qw), as_rows(kw), as_rows(vw), cu, scale, Tensor());
+    const Tensor o = wants_grad({&q, &k, &v}) ? AttentionFn::apply(qw, kw, vw, opt(cu), scale) : attention_forward(as_rows(qw), as_rows(kw), as_rows(vw), cu, scale, Tensor(), Tensor());
     return more ? o.narrow(3, 0, d).contiguous() : o;
   }));
   LNX_END
