@@ -410,6 +410,7 @@ int run(const char* what, const lnx_rmsnorm_residual_args* q, bool bwd, hipStrea
   if (params && (!q->workspace || q->workspace_bytes < lnx_rmsnorm_residual_bwd_workspace_bytes(q->rows, q->d, q->dtype)))
     return lnx_set_error(LNX_ERR_WORKSPACE, "%s: the parameters' gradients need a workspace of %llu bytes", what,
                          (unsigned long long)lnx_rmsnorm_residual_bwd_workspace_bytes(q->rows, q->d, q->dtype));
+  if (q->rows == 0 && !params) return LNX_OK;
   Args a{};
   a.x = q->x, a.r = q->residual, a.gate = q->gate, a.w = q->weight, a.post = q->post_weight, a.scale_v = q->scale_vector;
   a.scale = q->scale, a.eps = q->eps, a.inv_d = 1.f / (float)q->d, a.rows = q->rows, a.d = q->d, a.dpad = (q->d + 3) / 4 * 4;
