@@ -7,20 +7,28 @@
 // channel, which carries the state from tile to tile.  The loads of the next tile are in flight meanwhile.  (Eight channels of four
 // tokens a thread, scanned over eight groups by shuffles, were bound by the scan: 4.1 TB/s at [8, 4096, 2048] bf16, the same with
 // twice the loads in flight.)  Everything between loads and stores is fp32.  The backward pass reads x again instead of y, which is
-// rounded: the forward pass leaves the state entering every tile (fp32, 1 / 256 of the elements), so the states
+// rounded: the forward pass leaves a state every 128 tokens (fp32, 1 / 128 of the elements), so the states
 // behind dg are the unrounded ones.
-// Where rows and channels give too few workgroups the tokens are cut into segments: a first launch reduces every segment to its
-// pair, the second one starts each segment from the folded pairs before it.  No atomics: results are the same from run to run.
+// Where rows and channels give too few workgroups every tile (of 128 tokens) has a workgroup of its own: it publishes its pair, folds
+// those before it and goes on from there, all tensors still read once (a first launch for the pairs of segments and a second one
+// that read everything again took 352 us for [1, 65536, 2048] with fp32 gates, 229 this way).  Workgroups of one row and channel
+// tile take their tiles from a counter, so a tile is waited for only by workgroups that started after its own; it publishes before it
+// waits.  Every 32nd tile publishes the pair of all 32 as soon as it has the others', every 1024th the state behind it, and a tile goes
+// on from the last such state through the pairs of 32 and of one in the order of time: the same sums in the same order whatever the
+// timing, results are the same from run to run.  (With states every 32 tiles each was a wait for the one before: 3.7 us in a row.)
 #include "lnx_common.h"
 #include "mma_tiles.h"
 
 namespace {
 
-constexpr int THREADS = 512, WAVES = 8, N = 4, TILE = 256;  // tokens of a tile
+constexpr int THREADS = 512, N = 4, TILE = 256;  // tokens of a tile
+constexpr int CTHREADS = 256, CTILE = 128, GROUP = 32, ANCHOR = GROUP * 32;  // where every tile has a workgroup; tiles of a common pair, between states
+constexpr int KEPT = 128;  // tokens between the states that the forward pass leaves for the backward pass
 // By element type: threads side by side in a row, so that a row of a workgroup is 128 bytes; its channels; tokens per thread (what the
 // backward pass's registers take)
 template <typename T> struct Shape {
   static constexpr int COLS = sizeof(T) == 2 ? 16 : 8, C = COLS * N, R = TILE * COLS / THREADS;
+  static_assert(R == CTILE * COLS / CTHREADS, "both forms hold as many tokens a thread");
 };
 
 // Four consecutive elements as they lie in memory
@@ -50,34 +58,32 @@ struct Args {
   const float *s0, *ds;
   const int32_t* cu;
   void *y, *dx, *dg;
-  float *sT, *d0, *kept, *pairs;
-  int T, D, ctiles, segs;
+  float *sT, *d0, *kept;
+  uint64_t *pairs, *sums;  // [rows][tiles][D], (A, H) of a tile, [rows][tiles / GROUP][D], of GROUP tiles; all bits set: not there yet
+  uint32_t* anchors;       // [rows][tiles / ANCHOR][D], the state behind ANCHOR, 2 ANCHOR, ... tiles; likewise
+  uint32_t* counters;      // [rows][channel tiles]: tiles taken
+  int T, D, ctiles, tiles;
   bool packed;
 };
 
 // What a workgroup works on: row, its channels, its tiles
 template <typename T> struct Place {
-  int row, seg, len, ntile, per, tile0, tile1, c0, c, left;  // c0: the workgroup's first channel, c: this thread's
+  int row, len, ntile, c0, c, left;  // c0: the workgroup's first channel, c: this thread's
   int64_t tok, slot;  // first token in a packed batch (0 otherwise); first kept state
-  __device__ __forceinline__ Place(const Args& a) {
-    const int ct = blockIdx.x % a.ctiles, rs = blockIdx.x / a.ctiles;
-    seg = rs % a.segs;
-    row = rs / a.segs;
+  __device__ __forceinline__ Place(const Args& a, int group, int tile) {
+    row = group / a.ctiles;
     if (a.packed) {
       const int first = seq_first(a.cu, row, a.T);
       len = seq_end(a.cu, row, a.T) - first;
       tok = first;
-      slot = first / TILE + row;
+      slot = first / KEPT + row;
     } else {
       len = a.T;
       tok = 0;
-      slot = (int64_t)row * ((a.T + TILE - 1) / TILE);
+      slot = (int64_t)row * (((int64_t)a.T + KEPT - 1) / KEPT);
     }
-    ntile = (len + TILE - 1) / TILE;
-    per = (ntile + a.segs - 1) / a.segs;
-    tile0 = min(seg * per, ntile);
-    tile1 = min(tile0 + per, ntile);
-    c0 = ct * Shape<T>::C;
+    ntile = (int)(((int64_t)len + tile - 1) / tile);
+    c0 = group % a.ctiles * Shape<T>::C;
     c = c0 + (threadIdx.x & (Shape<T>::COLS - 1)) * N;
     left = a.D - c;
   }
@@ -128,8 +134,8 @@ template <int COLS, bool UP> __device__ __forceinline__ void scan_wave(float& a,
   }
 }
 
-// The eight waves' pairs and the states entering the waves, by channel of the workgroup
-template <int COLS> struct Waves {
+// The waves' pairs and the states entering the waves, by channel of the workgroup
+template <int COLS, int WAVES> struct Waves {
   static constexpr int C = COLS * N;
   float A[WAVES][C], H[WAVES][C], in[WAVES][C];
   __device__ __forceinline__ void leave(const float (&a)[N], const float (&h)[N], int lane, int wave) {
@@ -138,8 +144,8 @@ template <int COLS> struct Waves {
       store4(&H[wave][lane * N], floatx4{h[0], h[1], h[2], h[3]});
     }
   }
-  // one lane per channel: the state entering each wave, `carry` from before the tile to behind it; `all` the tiles' product
-  template <bool UP> __device__ __forceinline__ void chain(int c, float& carry, float& all) {
+  // one lane per channel: the state entering each wave, `carry` from before the tile to behind it
+  template <bool UP> __device__ __forceinline__ void chain(int c, float& carry) {
     float a[WAVES], h[WAVES];
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) a[w] = A[w][c], h[w] = H[w][c];
@@ -148,7 +154,17 @@ template <int COLS> struct Waves {
       const int w = UP ? k : WAVES - 1 - k;
       in[w][c] = carry;
       carry = a[w] * carry + h[w];
-      all *= a[w];
+    }
+  }
+  // one lane per channel: the tile's pair
+  template <bool UP> __device__ __forceinline__ void total(int c, float& A_, float& H_) const {
+    A_ = 1.f;
+    H_ = 0.f;
+#pragma unroll
+    for (int k = 0; k < WAVES; ++k) {
+      const int w = UP ? k : WAVES - 1 - k;
+      H_ = A[w][c] * H_ + H[w][c];
+      A_ *= A[w][c];
     }
   }
   // the state entering this thread's tokens
@@ -159,235 +175,403 @@ template <int COLS> struct Waves {
   }
 };
 
-// SUM: only the pair of each segment (but the last, which nothing follows)
-template <typename T, typename G, bool VEC, bool SUM> __global__ __launch_bounds__(THREADS) void linrec_fwd_kernel(Args a) {
-  constexpr int R = Shape<T>::R, COLS = Shape<T>::COLS, C = Shape<T>::C;
-  __shared__ Waves<COLS> ws;
-  const Place<T> p(a);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tr = threadIdx.x / COLS;
-  if (SUM && p.tile1 >= p.ntile) return;
-  const bool in_c = p.left > 0;
-  // the chain's lanes: one channel each
-  const int chan = p.c0 + lane;
-  const bool chains = wave == 0 && lane < C, in_chan = chains && chan < a.D;
-  const int64_t row_c = (int64_t)p.row * a.D + chan;
-  float carry = 0.f, all = 1.f;
-  if (!SUM && in_chan) {
-    if (a.s0) carry = a.s0[row_c];
-    if (p.tile0 < p.tile1)
-      for (int s = 0; s < p.seg; ++s) {
-        const float* q = a.pairs + ((int64_t)p.row * a.segs + s) * 2 * a.D + chan;
-        carry = q[0] * carry + q[a.D];
-      }
+// What a thread holds of a tile: the vectors of its R tokens from `x` and `g` on
+template <typename T, typename G, bool VEC> struct Tokens {
+  static constexpr int R = Shape<T>::R;
+  Raw<T, VEC> x[R];
+  Raw<G, VEC> g[R];
+};
+
+// ---- words that other workgroups wait for ----
+constexpr uint32_t EMPTY = 0xffffffffu, QUIET = 0x7fc00000u;
+// (Waits end by themselves, see above; a bound keeps a fault elsewhere from holding the GPU: the result is NaN then.)
+constexpr int MOST_POLLS = 1 << 22;
+__device__ __forceinline__ uint32_t word(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return u == EMPTY ? QUIET : u;
+}
+__device__ __forceinline__ uint64_t peek(const uint64_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ uint32_t peek(const uint32_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ void publish(uint64_t* p, float A, float H) {
+  __hip_atomic_store(p, (uint64_t)word(A) << 32 | word(H), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void publish(uint32_t* p, float x) { __hip_atomic_store(p, word(x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+template <typename W> __device__ __forceinline__ W await(const W* p, W v) {
+  for (int n = 0; (uint32_t)v == EMPTY && n < MOST_POLLS; ++n) {
+    __builtin_amdgcn_s_sleep(1);
+    v = peek(p);
   }
-  const int64_t first = (int64_t)p.tile0 * TILE, row_b = a.packed ? 0 : 1;  // a packed batch is one row
-  const char* x = p.template at<T>(a.x, row_b * a.xb, a.xt, first);
-  const char* g = p.template at<G>(a.g, row_b * a.gb, a.gt, first);
-  char* y = const_cast<char*>(p.template at<T>(a.y, row_b * a.T * a.D, a.D, first));
-  const unsigned xo = p.template lane<T>(a.xt, tr * R), go = p.template lane<G>(a.gt, tr * R), yo = p.template lane<T>(a.D, tr * R);
-  const int64_t xs = a.xt * (int64_t)sizeof(T), gs = a.gt * (int64_t)sizeof(G), ys = a.D * (int64_t)sizeof(T);
-  Raw<T, VEC> xr[R];
-  Raw<G, VEC> gr[R];
-  // the tile that x and g point at
-  const auto fetch = [&](int tile) {
-    if ((tile + 1) * (int64_t)TILE <= p.len && p.c0 + C <= a.D) {
+  return v;
+}
+
+// (A, H) := the n maps of `p` (D apart) behind it: one lane per channel
+__device__ __forceinline__ void fold(float& A, float& H, const uint64_t* p, int n, int D) {
+  for (int i = 0; i < n; i += 8) {
+    uint64_t v[8];
 #pragma unroll
-      for (int u = 0; u < R; ++u) xr[u].load(elems<T>(x + u * xs, xo), N), gr[u].load(elems<G>(g + u * gs, go), N);
+    for (int u = 0; u < 8; ++u) v[u] = i + u < n ? peek(p + (int64_t)(i + u) * D) : (uint64_t)__float_as_uint(1.f) << 32;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      if (i + u < n) v[u] = await(p + (int64_t)(i + u) * D, v[u]);
+      const float a = __uint_as_float((uint32_t)(v[u] >> 32));
+      H = a * H + __uint_as_float((uint32_t)v[u]);
+      A *= a;
+    }
+  }
+}
+// The state before the j-th of ntile tiles (counted from where the recurrence starts), from `begin` before the first; (A, H) is the
+// tile's pair.  Leaves what others wait for before it waits for what comes before the tile's group.  One lane per channel.
+__device__ __forceinline__ float state_before(const Args& a, int row, int j, int ntile, int chan, float begin, float A, float H) {
+  const int base = j / GROUP * GROUP, top = j / ANCHOR * ANCHOR;
+  uint64_t* pairs = a.pairs + (int64_t)row * a.tiles * a.D + chan;
+  uint64_t* sums = a.sums + (int64_t)row * (a.tiles / GROUP) * a.D + chan;
+  if (j + 1 < ntile) publish(pairs + (int64_t)j * a.D, A, H);
+  float Ag = 1.f, Hg = 0.f;
+  fold(Ag, Hg, pairs + (int64_t)base * a.D, j - base, a.D);
+  if (j - base == GROUP - 1 && j + 1 < ntile) publish(sums + (int64_t)(j / GROUP) * a.D, A * Ag, A * Hg + H);
+  float state = begin;
+  if (top) {
+    const uint32_t* p = a.anchors + ((int64_t)row * (a.tiles / ANCHOR) + top / ANCHOR - 1) * a.D + chan;
+    state = __uint_as_float(await(p, peek(p)));
+  }
+  float unused = 1.f;
+  fold(unused, state, sums + (int64_t)(top / GROUP) * a.D, (base - top) / GROUP, a.D);
+  return Ag * state + Hg;
+}
+__device__ __forceinline__ void leave_state(const Args& a, int row, int j, int ntile, int chan, float state) {
+  if ((j + 1) % ANCHOR == 0 && j + 1 < ntile) publish(a.anchors + ((int64_t)row * (a.tiles / ANCHOR) + (j + 1) / ANCHOR - 1) * a.D + chan, state);
+}
+// The tile of this workgroup: the next one of its group
+__device__ __forceinline__ int take_tile(const Args& a, int group) {
+  __shared__ int tile;
+  if (threadIdx.x == 0) tile = (int)__hip_atomic_fetch_add(a.counters + group, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  return __builtin_amdgcn_readfirstlane(tile);
+}
+__global__ __launch_bounds__(256) void linrec_clear_kernel(uint32_t* words, int64_t n, uint32_t* counters, int groups) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (4 * i + 3 < n) *reinterpret_cast<uint4*>(words + 4 * i) = uint4{EMPTY, EMPTY, EMPTY, EMPTY};
+  else
+    for (int64_t k = 4 * i; k < n; ++k) words[k] = EMPTY;
+  if (i < groups) counters[i] = 0;
+}
+
+// The pointers of a forward pass at token `first` of the row, and a lane's bytes from there
+template <typename T, typename G, bool VEC> struct Forward {
+  static constexpr int R = Shape<T>::R, COLS = Shape<T>::COLS, C = Shape<T>::C;
+  const char *x, *g;
+  char* y;
+  unsigned xo, go, yo;
+  int64_t xs, gs, ys;
+  int tr;
+  __device__ __forceinline__ Forward(const Args& a, const Place<T>& p, int64_t first) {
+    const int64_t row_b = a.packed ? 0 : 1;  // a packed batch is one row
+    tr = threadIdx.x / COLS;
+    x = p.template at<T>(a.x, row_b * a.xb, a.xt, first);
+    g = p.template at<G>(a.g, row_b * a.gb, a.gt, first);
+    y = const_cast<char*>(p.template at<T>(a.y, row_b * a.T * a.D, a.D, first));
+    xo = p.template lane<T>(a.xt, tr * R), go = p.template lane<G>(a.gt, tr * R), yo = p.template lane<T>(a.D, tr * R);
+    xs = a.xt * (int64_t)sizeof(T), gs = a.gt * (int64_t)sizeof(G), ys = a.D * (int64_t)sizeof(T);
+  }
+  // `there`: tokens of the row from the tile's first on
+  __device__ __forceinline__ void fetch(Tokens<T, G, VEC>& in, const Place<T>& p, const Args& a, int64_t there, int tile) const {
+    if (there >= tile && p.c0 + C <= a.D) {
+#pragma unroll
+      for (int u = 0; u < R; ++u) in.x[u].load(elems<T>(x + u * xs, xo), N), in.g[u].load(elems<G>(g + u * gs, go), N);
     } else {
 #pragma unroll
       for (int u = 0; u < R; ++u) {
-        xr[u].zero();
-        gr[u].zero();
-        if ((int64_t)tile * TILE + tr * R + u < p.len && in_c) xr[u].load(elems<T>(x + u * xs, xo), p.left), gr[u].load(elems<G>(g + u * gs, go), p.left);
+        in.x[u].zero();
+        in.g[u].zero();
+        if (tr * R + u < there && p.left > 0) in.x[u].load(elems<T>(x + u * xs, xo), p.left), in.g[u].load(elems<G>(g + u * gs, go), p.left);
       }
     }
-  };
-  if (p.tile0 < p.tile1) fetch(p.tile0);
-  for (int tile = p.tile0; tile < p.tile1; ++tile) {
-    float e[R][N], xv[R][N], A[N], H[N], ea[N], eh[N];
+  }
+  __device__ __forceinline__ void finish(const Place<T>& p, const Args& a, int64_t there, int tile, float (&h)[N], const float (&e)[R][N], const float (&xv)[R][N]) const {
+    const bool whole = there >= tile && p.c0 + C <= a.D;
 #pragma unroll
-    for (int i = 0; i < N; ++i) A[i] = 1.f, H[i] = 0.f;
+    for (int u = 0; u < R; ++u) {
 #pragma unroll
-    for (int u = 0; u < R; ++u)
+      for (int i = 0; i < N; ++i) h[i] = e[u][i] * h[i] + xv[u][i];
+      if (whole || (tr * R + u < there && p.left > 0)) put<VEC>(elems<T>(y + u * ys, yo), h, p.left);
+    }
+  }
+};
+// A thread's factors and inputs, and its pair
+template <typename T, typename G, bool VEC>
+__device__ __forceinline__ void reduce_forward(const Tokens<T, G, VEC>& in, float (&e)[Shape<T>::R][N], float (&xv)[Shape<T>::R][N], float (&A)[N], float (&H)[N]) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        e[u][i] = __expf(gr[u].get(i));  // 1 behind the end: the state stands
-        xv[u][i] = xr[u].get(i);
-        H[i] = e[u][i] * H[i] + xv[u][i];
-        A[i] *= e[u][i];
-      }
-    x += TILE * xs;
-    g += TILE * gs;
-    if (tile + 1 < p.tile1) fetch(tile + 1);
+  for (int i = 0; i < N; ++i) A[i] = 1.f, H[i] = 0.f;
+#pragma unroll
+  for (int u = 0; u < Shape<T>::R; ++u)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      e[u][i] = __expf(in.g[u].get(i));  // 1 behind the end: the state stands
+      xv[u][i] = in.x[u].get(i);
+      H[i] = e[u][i] * H[i] + xv[u][i];
+      A[i] *= e[u][i];
+    }
+}
+
+template <typename T, typename G, bool VEC> __global__ __launch_bounds__(THREADS) void linrec_fwd_kernel(Args a) {
+  constexpr int R = Shape<T>::R, COLS = Shape<T>::COLS, C = Shape<T>::C;
+  __shared__ Waves<COLS, 8> ws;
+  const Place<T> p(a, blockIdx.x, TILE);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // the chain's lanes: one channel each
+  const int chan = p.c0 + lane;
+  const bool chains = wave == 0 && lane < C, in_chan = chains && chan < a.D;
+  float carry = in_chan && a.s0 ? a.s0[(int64_t)p.row * a.D + chan] : 0.f;
+  Forward<T, G, VEC> f(a, p, 0);
+  Tokens<T, G, VEC> in;
+  if (p.ntile) f.fetch(in, p, a, p.len, TILE);
+  for (int tile = 0; tile < p.ntile; ++tile) {
+    const int64_t there = p.len - (int64_t)tile * TILE;
+    float e[R][N], xv[R][N], A[N], H[N], ea[N], eh[N], h[N];
+    reduce_forward<T, G, VEC>(in, e, xv, A, H);
+    f.x += TILE * f.xs;
+    f.g += TILE * f.gs;
+    if (tile + 1 < p.ntile) f.fetch(in, p, a, there - TILE, TILE);
 #pragma unroll
     for (int i = 0; i < N; ++i) scan_wave<COLS, true>(A[i], H[i], ea[i], eh[i], lane);
     ws.leave(A, H, lane, wave);
     lds_barrier();
     if (chains) {
-      if (!SUM && a.kept && in_chan) a.kept[(p.slot + tile) * a.D + chan] = carry;
-      ws.template chain<true>(lane, carry, all);
+      ws.template chain<true>(lane, carry);
+      if (a.kept && in_chan) {
+#pragma unroll
+        for (int k = 0; k < TILE / KEPT; ++k)
+          if (k * KEPT < there) a.kept[(p.slot + tile * (TILE / KEPT) + k) * a.D + chan] = ws.in[k * 8 * KEPT / TILE][lane];
+      }
     }
     lds_barrier();
-    if (!SUM) {
-      float h[N];
-      ws.enter(ea, eh, h, lane, wave);
-      const bool whole = (tile + 1) * (int64_t)TILE <= p.len && p.c0 + C <= a.D;
-#pragma unroll
-      for (int u = 0; u < R; ++u) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) h[i] = e[u][i] * h[i] + xv[u][i];
-        if (whole || ((int64_t)tile * TILE + tr * R + u < p.len && in_c)) put<VEC>(elems<T>(y + u * ys, yo), h, p.left);
-      }
-      y += TILE * ys;
-    }
+    ws.enter(ea, eh, h, lane, wave);
+    f.finish(p, a, there, TILE, h, e, xv);
+    f.y += TILE * f.ys;
   }
-  if (!in_chan) return;
-  if (SUM) {
-    float* q = a.pairs + ((int64_t)p.row * a.segs + p.seg) * 2 * a.D + chan;
-    q[0] = all;
-    q[a.D] = carry;
-  } else if (p.ntile ? p.tile0 < p.tile1 && p.tile1 == p.ntile : p.seg == 0) {
-    a.sT[row_c] = carry;
-  }
+  if (in_chan) a.sT[(int64_t)p.row * a.D + chan] = carry;
 }
 
-// Backwards in time: o is e^{g_{t+1}} dh_{t+1}.  SUM: only the pair of each segment (but the first, which nothing precedes)
-template <typename T, typename G, bool VEC, bool SUM> __global__ __launch_bounds__(THREADS) void linrec_bwd_kernel(Args a) {
+template <typename T, typename G, bool VEC> __global__ __launch_bounds__(CTHREADS) void linrec_fwd_chain_kernel(Args a, int groups) {
   constexpr int R = Shape<T>::R, COLS = Shape<T>::COLS, C = Shape<T>::C;
-  __shared__ Waves<COLS> ws, wf;
-  const Place<T> p(a);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tr = threadIdx.x / COLS;
-  if (SUM && (p.seg == 0 || p.tile0 >= p.tile1)) return;
-  const bool in_c = p.left > 0;
-  const int chan = p.c0 + lane;  // wave 0 chains the gradients, wave 1 the states
-  const bool chains = wave == 0 && lane < C, in_chan = chains && chan < a.D, states = !SUM && wave == 1 && lane < C;
+  __shared__ Waves<COLS, 4> ws;
+  const int group = blockIdx.x % groups, j = take_tile(a, group);
+  const Place<T> p(a, group, CTILE);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, chan = p.c0 + lane;
+  const bool in_chan = wave == 0 && lane < C && chan < a.D;
   const int64_t row_c = (int64_t)p.row * a.D + chan;
-  float carry = 0.f, all = 1.f, start = 0.f;
-  if (!SUM && in_chan) {
-    if (a.ds) carry = a.ds[row_c];
-    if (p.tile0 < p.tile1)
-      for (int s = (p.ntile - 1) / p.per; s > p.seg; --s) {
-        const float* q = a.pairs + ((int64_t)p.row * a.segs + s) * 2 * a.D + chan;
-        carry = q[0] * carry + q[a.D];
-      }
+  if (j >= p.ntile) {
+    if (j == 0 && in_chan) a.sT[row_c] = a.s0 ? a.s0[row_c] : 0.f;  // no tokens at all
+    return;
   }
-  const int64_t first = (int64_t)(p.tile1 - 1) * TILE, row_b = a.packed ? 0 : 1;  // of the last tile
-  const char* x = p.template at<T>(a.x, row_b * a.xb, a.xt, first);
-  const char* g = p.template at<G>(a.g, row_b * a.gb, a.gt, first);
-  const char* dy = p.template at<T>(a.dy, row_b * a.yb, a.yt, first);
-  char* dx = const_cast<char*>(p.template at<T>(a.dx, row_b * a.T * a.D, a.D, first));
-  char* dg = const_cast<char*>(p.template at<G>(a.dg, row_b * a.T * a.D, a.D, first));
-  const unsigned xo = p.template lane<T>(a.xt, tr * R), go = p.template lane<G>(a.gt, tr * R), yo = p.template lane<T>(a.yt, tr * R), dxo = p.template lane<T>(a.D, tr * R), dgo = p.template lane<G>(a.D, tr * R);
-  const int64_t xs = a.xt * (int64_t)sizeof(T), gs = a.gt * (int64_t)sizeof(G), ys = a.yt * (int64_t)sizeof(T), dxs = a.D * (int64_t)sizeof(T), dgs = a.D * (int64_t)sizeof(G);
-  Raw<T, VEC> xr[R], yr[R];
-  Raw<G, VEC> gr[R];
-  if (!a.dy)
+  const int64_t first = (int64_t)j * CTILE, there = p.len - first;
+  const Forward<T, G, VEC> f(a, p, first);
+  Tokens<T, G, VEC> in;
+  f.fetch(in, p, a, there, CTILE);
+  float e[R][N], xv[R][N], A[N], H[N], ea[N], eh[N], h[N];
+  reduce_forward<T, G, VEC>(in, e, xv, A, H);
 #pragma unroll
-    for (int u = 0; u < R; ++u) yr[u].zero();
-  const auto fetch = [&](int tile) {
-    if (states && chan < a.D) start = a.kept[(p.slot + tile) * a.D + chan];
-    if ((tile + 1) * (int64_t)TILE <= p.len && p.c0 + C <= a.D) {
+  for (int i = 0; i < N; ++i) scan_wave<COLS, true>(A[i], H[i], ea[i], eh[i], lane);
+  ws.leave(A, H, lane, wave);
+  lds_barrier();
+  if (in_chan) {
+    float At, Ht;
+    ws.template total<true>(lane, At, Ht);
+    float carry = state_before(a, p.row, j, p.ntile, chan, a.s0 ? a.s0[row_c] : 0.f, At, Ht);
+    if (a.kept) a.kept[(p.slot + j) * a.D + chan] = carry;
+    ws.template chain<true>(lane, carry);
+    leave_state(a, p.row, j, p.ntile, chan, carry);
+    if (j + 1 == p.ntile) a.sT[row_c] = carry;
+  }
+  lds_barrier();
+  ws.enter(ea, eh, h, lane, wave);
+  f.finish(p, a, there, CTILE, h, e, xv);
+}
+
+// The pointers of a backward pass
+template <typename T, typename G, bool VEC> struct Backward {
+  static constexpr int R = Shape<T>::R, COLS = Shape<T>::COLS, C = Shape<T>::C;
+  const char *x, *g, *dy;
+  char *dx, *dg;
+  unsigned xo, go, yo, dxo, dgo;
+  int64_t xs, gs, ys, dxs, dgs;
+  int tr;
+  __device__ __forceinline__ Backward(const Args& a, const Place<T>& p, int64_t first) {
+    const int64_t row_b = a.packed ? 0 : 1;
+    tr = threadIdx.x / COLS;
+    x = p.template at<T>(a.x, row_b * a.xb, a.xt, first);
+    g = p.template at<G>(a.g, row_b * a.gb, a.gt, first);
+    dy = p.template at<T>(a.dy, row_b * a.yb, a.yt, first);
+    dx = const_cast<char*>(p.template at<T>(a.dx, row_b * a.T * a.D, a.D, first));
+    dg = const_cast<char*>(p.template at<G>(a.dg, row_b * a.T * a.D, a.D, first));
+    xo = p.template lane<T>(a.xt, tr * R), go = p.template lane<G>(a.gt, tr * R), yo = p.template lane<T>(a.yt, tr * R);
+    dxo = p.template lane<T>(a.D, tr * R), dgo = p.template lane<G>(a.D, tr * R);
+    xs = a.xt * (int64_t)sizeof(T), gs = a.gt * (int64_t)sizeof(G), ys = a.yt * (int64_t)sizeof(T), dxs = a.D * (int64_t)sizeof(T), dgs = a.D * (int64_t)sizeof(G);
+  }
+  __device__ __forceinline__ void fetch(Tokens<T, G, VEC>& in, Raw<T, VEC> (&yr)[R], const Place<T>& p, const Args& a, int64_t there, int tile) const {
+    if (there >= tile && p.c0 + C <= a.D) {
 #pragma unroll
-      for (int u = 0; u < R; ++u) {
-        if (!SUM) xr[u].load(elems<T>(x + u * xs, xo), N);
-        gr[u].load(elems<G>(g + u * gs, go), N);
-      }
-      if (a.dy)
+      for (int u = 0; u < R; ++u) in.x[u].load(elems<T>(x + u * xs, xo), N), in.g[u].load(elems<G>(g + u * gs, go), N);
+      if (a.dy) {
 #pragma unroll
         for (int u = 0; u < R; ++u) yr[u].load(elems<T>(dy + u * ys, yo), N);
+      } else {
+#pragma unroll
+        for (int u = 0; u < R; ++u) yr[u].zero();
+      }
     } else {
 #pragma unroll
       for (int u = 0; u < R; ++u) {
-        xr[u].zero();
+        in.x[u].zero();
+        in.g[u].zero();
         yr[u].zero();
-        gr[u].zero();
-        if ((int64_t)tile * TILE + tr * R + u < p.len && in_c) {
-          if (!SUM) xr[u].load(elems<T>(x + u * xs, xo), p.left);
+        if (tr * R + u < there && p.left > 0) {
+          in.x[u].load(elems<T>(x + u * xs, xo), p.left);
           if (a.dy) yr[u].load(elems<T>(dy + u * ys, yo), p.left);
-          gr[u].load(elems<G>(g + u * gs, go), p.left);
+          in.g[u].load(elems<G>(g + u * gs, go), p.left);
         }
       }
     }
-  };
-  if (p.tile0 < p.tile1) fetch(p.tile1 - 1);
-  for (int tile = p.tile1 - 1; tile >= p.tile0; --tile) {
-    float e[R][N], A[N], H[N], ea[N], eh[N], Af[N], Hf[N], fa[N], fh[N];
-    Raw<T, VEC> xk[R], yk[R];
+  }
+  // h: the state before this thread's tokens, o: e^g dh of the token behind them
+  __device__ __forceinline__ void finish(const Place<T>& p, const Args& a, int64_t there, int tile, float (&h)[N], float (&o)[N], const float (&e)[R][N],
+                                         const Raw<T, VEC> (&xk)[R], const Raw<T, VEC> (&yk)[R]) const {
+    const bool whole = there >= tile && p.c0 + C <= a.D;
+    float hb[R][N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) A[i] = 1.f, H[i] = 0.f, Hf[i] = 0.f;
+    for (int u = 0; u < R; ++u)
+#pragma unroll
+      for (int i = 0; i < N; ++i) hb[u][i] = h[i], h[i] = e[u][i] * h[i] + xk[u].get(i);
 #pragma unroll
     for (int u = R - 1; u >= 0; --u) {
-      xk[u] = xr[u];
-      yk[u] = yr[u];
+      float dh[N], dgv[N];
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        e[u][i] = __expf(gr[u].get(i));
-        H[i] = e[u][i] * (yk[u].get(i) + H[i]);
-        A[i] *= e[u][i];
+        dh[i] = yk[u].get(i) + o[i];
+        o[i] = e[u][i] * dh[i];
+        dgv[i] = hb[u][i] * o[i];
+      }
+      if (whole || (tr * R + u < there && p.left > 0)) {
+        put<VEC>(elems<T>(dx + u * dxs, dxo), dh, p.left);
+        put<VEC>(elems<G>(dg + u * dgs, dgo), dgv, p.left);
       }
     }
-    if (!SUM)
+  }
+};
+// A thread's factors and its two pairs: of the gradients backwards in time (o is e^{g_{t+1}} dh_{t+1}), of the states forwards
+template <typename T, typename G, bool VEC>
+__device__ __forceinline__ void reduce_backward(const Tokens<T, G, VEC>& in, const Raw<T, VEC> (&yr)[Shape<T>::R], float (&e)[Shape<T>::R][N], float (&A)[N], float (&H)[N],
+                                                float (&Af)[N], float (&Hf)[N]) {
+  constexpr int R = Shape<T>::R;
 #pragma unroll
-      for (int u = 0; u < R; ++u)
+  for (int i = 0; i < N; ++i) A[i] = 1.f, H[i] = 0.f, Hf[i] = 0.f;
 #pragma unroll
-        for (int i = 0; i < N; ++i) Hf[i] = e[u][i] * Hf[i] + xk[u].get(i);
-    float from = start;
-    x -= TILE * xs;
-    g -= TILE * gs;
-    dy -= TILE * ys;
-    if (tile > p.tile0) fetch(tile - 1);
+  for (int u = R - 1; u >= 0; --u)
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      if (!SUM) {
-        Af[i] = A[i];
-        scan_wave<COLS, true>(Af[i], Hf[i], fa[i], fh[i], lane);
-      }
+      e[u][i] = __expf(in.g[u].get(i));
+      H[i] = e[u][i] * (yr[u].get(i) + H[i]);
+      A[i] *= e[u][i];
+    }
+#pragma unroll
+  for (int u = 0; u < R; ++u)
+#pragma unroll
+    for (int i = 0; i < N; ++i) Hf[i] = e[u][i] * Hf[i] + in.x[u].get(i);
+#pragma unroll
+  for (int i = 0; i < N; ++i) Af[i] = A[i];
+}
+
+template <typename T, typename G, bool VEC> __global__ __launch_bounds__(THREADS) void linrec_bwd_kernel(Args a) {
+  constexpr int R = Shape<T>::R, COLS = Shape<T>::COLS, C = Shape<T>::C;
+  __shared__ Waves<COLS, 8> ws, wf;
+  const Place<T> p(a, blockIdx.x, TILE);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int chan = p.c0 + lane;  // wave 0 chains the gradients, wave 1 the states
+  const bool mine = lane < C && chan < a.D, grads = wave == 0 && lane < C, states = wave == 1 && lane < C;
+  float carry = grads && mine && a.ds ? a.ds[(int64_t)p.row * a.D + chan] : 0.f, start = 0.f;
+  Backward<T, G, VEC> f(a, p, (int64_t)(p.ntile - 1) * TILE);  // the last tile
+  Tokens<T, G, VEC> in;
+  Raw<T, VEC> yr[R];
+  const auto fetch = [&](int tile) {
+    if (states && mine) start = a.kept[(p.slot + (int64_t)tile * (TILE / KEPT)) * a.D + chan];
+    f.fetch(in, yr, p, a, p.len - (int64_t)tile * TILE, TILE);
+  };
+  if (p.ntile) fetch(p.ntile - 1);
+  for (int tile = p.ntile - 1; tile >= 0; --tile) {
+    float e[R][N], A[N], H[N], ea[N], eh[N], Af[N], Hf[N], fa[N], fh[N], h[N], o[N];
+    reduce_backward<T, G, VEC>(in, yr, e, A, H, Af, Hf);
+    Raw<T, VEC> xk[R], yk[R];
+#pragma unroll
+    for (int u = 0; u < R; ++u) xk[u] = in.x[u], yk[u] = yr[u];
+    float from = start;
+    f.x -= TILE * f.xs;
+    f.g -= TILE * f.gs;
+    f.dy -= TILE * f.ys;
+    if (tile > 0) fetch(tile - 1);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      scan_wave<COLS, true>(Af[i], Hf[i], fa[i], fh[i], lane);
       scan_wave<COLS, false>(A[i], H[i], ea[i], eh[i], lane);
     }
-    if (!SUM) wf.leave(Af, Hf, lane, wave);
+    wf.leave(Af, Hf, lane, wave);
     ws.leave(A, H, lane, wave);
     lds_barrier();
-    if (chains) ws.template chain<false>(lane, carry, all);
-    if (states) {
-      float none = 1.f;
-      wf.template chain<true>(lane, from, none);
-    }
+    if (grads) ws.template chain<false>(lane, carry);
+    if (states) wf.template chain<true>(lane, from);
     lds_barrier();
-    if (!SUM) {
-      float h[N], o[N], hb[R][N];
-      wf.enter(fa, fh, h, lane, wave);
-      ws.enter(ea, eh, o, lane, wave);
-      const bool whole = (tile + 1) * (int64_t)TILE <= p.len && p.c0 + C <= a.D;
-#pragma unroll
-      for (int u = 0; u < R; ++u)
-#pragma unroll
-        for (int i = 0; i < N; ++i) hb[u][i] = h[i], h[i] = e[u][i] * h[i] + xk[u].get(i);
-#pragma unroll
-      for (int u = R - 1; u >= 0; --u) {
-        float dh[N], dgv[N];
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          dh[i] = yk[u].get(i) + o[i];
-          o[i] = e[u][i] * dh[i];
-          dgv[i] = hb[u][i] * o[i];
-        }
-        if (whole || ((int64_t)tile * TILE + tr * R + u < p.len && in_c)) {
-          put<VEC>(elems<T>(dx + u * dxs, dxo), dh, p.left);
-          put<VEC>(elems<G>(dg + u * dgs, dgo), dgv, p.left);
-        }
-      }
-      dx -= TILE * dxs;
-      dg -= TILE * dgs;
-    }
+    wf.enter(fa, fh, h, lane, wave);
+    ws.enter(ea, eh, o, lane, wave);
+    f.finish(p, a, p.len - (int64_t)tile * TILE, TILE, h, o, e, xk, yk);
+    f.dx -= TILE * f.dxs;
+    f.dg -= TILE * f.dgs;
   }
-  if (!in_chan) return;
-  if (SUM) {
-    float* q = a.pairs + ((int64_t)p.row * a.segs + p.seg) * 2 * a.D + chan;
-    q[0] = all;
-    q[a.D] = carry;
-  } else if (a.d0 && p.seg == 0) {
-    a.d0[row_c] = carry;
+  if (grads && mine && a.d0) a.d0[(int64_t)p.row * a.D + chan] = carry;
+}
+
+template <typename T, typename G, bool VEC> __global__ __launch_bounds__(CTHREADS) void linrec_bwd_chain_kernel(Args a, int groups) {
+  constexpr int R = Shape<T>::R, COLS = Shape<T>::COLS, C = Shape<T>::C;
+  __shared__ Waves<COLS, 4> ws, wf;
+  const int group = blockIdx.x % groups, j = take_tile(a, group);
+  const Place<T> p(a, group, CTILE);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, chan = p.c0 + lane;
+  const bool mine = lane < C && chan < a.D, grads = wave == 0 && mine, states = wave == 1 && mine;
+  const int64_t row_c = (int64_t)p.row * a.D + chan;
+  if (j >= p.ntile) {
+    if (j == 0 && grads && a.d0) a.d0[row_c] = a.ds ? a.ds[row_c] : 0.f;
+    return;
   }
+  const int tile = p.ntile - 1 - j;
+  const int64_t first = (int64_t)tile * CTILE, there = p.len - first;
+  const Backward<T, G, VEC> f(a, p, first);
+  Tokens<T, G, VEC> in;
+  Raw<T, VEC> yr[R];
+  f.fetch(in, yr, p, a, there, CTILE);
+  float e[R][N], A[N], H[N], ea[N], eh[N], Af[N], Hf[N], fa[N], fh[N], h[N], o[N];
+  reduce_backward<T, G, VEC>(in, yr, e, A, H, Af, Hf);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    scan_wave<COLS, true>(Af[i], Hf[i], fa[i], fh[i], lane);
+    scan_wave<COLS, false>(A[i], H[i], ea[i], eh[i], lane);
+  }
+  wf.leave(Af, Hf, lane, wave);
+  ws.leave(A, H, lane, wave);
+  lds_barrier();
+  if (grads) {
+    float At, Ht;
+    ws.template total<false>(lane, At, Ht);
+    float carry = state_before(a, p.row, j, p.ntile, chan, a.ds ? a.ds[row_c] : 0.f, At, Ht);
+    ws.template chain<false>(lane, carry);
+    leave_state(a, p.row, j, p.ntile, chan, carry);
+    if (tile == 0 && a.d0) a.d0[row_c] = carry;
+  }
+  if (states) {
+    float from = a.kept[(p.slot + tile) * a.D + chan];
+    wf.template chain<true>(lane, from);
+  }
+  lds_barrier();
+  wf.enter(fa, fh, h, lane, wave);
+  ws.enter(ea, eh, o, lane, wave);
+  f.finish(p, a, there, CTILE, h, o, e, in.x, yr);
 }
 
 // One token: four elements a thread, or one where the vectors do not fit
@@ -415,14 +599,18 @@ int channel_tiles(const lnx_linrec_args* a) {
   return (int)(((int64_t)a->D + c - 1) / c);
 }
 
-// Segments of a row's tokens: as many as bring the launch to one workgroup a CU, of four tiles each at least (the first launch
-// reads the inputs once more, so a launch that nearly fills the chip by itself is not cut).
-int segments(const lnx_linrec_args* a) {
-  const int64_t wgs = (int64_t)rows_of(a) * channel_tiles(a), len = a->nseq ? a->T / a->nseq : a->T, tiles = (len + TILE - 1) / TILE;  // of the average sequence
-  int64_t s = wgs >= 160 ? 1 : 256 / (wgs > 0 ? wgs : 1);
-  if (s > tiles / 4) s = tiles / 4;
-  return s < 1 ? 1 : (int)s;
+int tiles_of(const lnx_linrec_args* a) { return (int)(((int64_t)a->T + CTILE - 1) / CTILE); }
+// Whether every tile has a workgroup of its own: where walking the rows would leave a third of the chip without work.  With 256 rows and
+// channel tiles both forms move bytes at the same rate forwards and the walk is 13 % faster backwards ([8, 4096, 2048] bf16: 99 and
+// 99, 140 and 158 us); with 128 tiles of 1024 tokens the chained form is faster ([4, 1024, 2048]: 16.6 -> 14.7, 23.5 -> 19.4 us and a
+// clearing launch of 3), with 32 twice as fast (14.6 -> 9.0, 21 -> 10.3).
+bool chained(const lnx_linrec_args* a) {
+  const int64_t wgs = (int64_t)rows_of(a) * channel_tiles(a), len = a->nseq ? a->T / a->nseq : a->T;
+  return wgs < 160 && len >= 8 * CTILE && wgs * tiles_of(a) <= 0x7fffffff;
 }
+// Bytes of what the workgroups leave for each other
+int64_t pair_words(const lnx_linrec_args* a) { return 2 * (int64_t)rows_of(a) * (tiles_of(a) + tiles_of(a) / GROUP) * a->D; }
+int64_t all_words(const lnx_linrec_args* a) { return pair_words(a) + ((int64_t)rows_of(a) * (tiles_of(a) / ANCHOR) * a->D + 3) / 4 * 4; }
 
 int check(const char* what, const lnx_linrec_args* a, bool bwd) {
   if (!a) return lnx_set_error(LNX_ERR_NULL, "%s: args is NULL", what);
@@ -439,45 +627,45 @@ int check(const char* what, const lnx_linrec_args* a, bool bwd) {
   for (int64_t st : {a->x_stride_t * (a->dtype == LNX_BF16 ? 2 : 4), a->g_stride_t * (a->g_dtype == LNX_BF16 ? 2 : 4), (bwd ? a->d_y_stride_t : 0) * (a->dtype == LNX_BF16 ? 2 : 4),
                      (int64_t)a->D * 4})
     if (st < 0 || st > MAX_STRIDE) return lnx_set_error(LNX_ERR_SHAPE, "%s: tokens more than %lld bytes apart", what, (long long)MAX_STRIDE);
-  if ((int64_t)rows_of(a) * channel_tiles(a) * segments(a) > 0x7fffffff) return lnx_set_error(LNX_ERR_SHAPE, "%s: too many rows", what);
-  if (rows && segments(a) > 1) {
+  if ((int64_t)rows_of(a) * channel_tiles(a) > 0x7fffffff) return lnx_set_error(LNX_ERR_SHAPE, "%s: too many rows", what);
+  if (rows && chained(a)) {
     const uint64_t need = lnx_linrec_workspace_bytes(a);
-    if (!a->workspace || a->workspace_bytes < need) return lnx_set_error(LNX_ERR_WORKSPACE, "%s: needs a workspace of %llu bytes", what, (unsigned long long)need);
+    if (!a->workspace || a->workspace_bytes < need || reinterpret_cast<uintptr_t>(a->workspace) % 16) return lnx_set_error(LNX_ERR_WORKSPACE, "%s: needs a workspace of %llu bytes", what, (unsigned long long)need);
   }
   return LNX_OK;
 }
 
 bool vectors(const void* p, int64_t sb, int64_t st, int64_t size) { return !p || (reinterpret_cast<uintptr_t>(p) % (4 * size) == 0 && sb % 4 == 0 && st % 4 == 0); }
 
-Args kernel_args(const lnx_linrec_args* a, int segs) {
+Args kernel_args(const lnx_linrec_args* a) {
   Args k{};
   k.x = a->x, k.g = a->g, k.dy = a->d_y;
   k.xb = a->x_stride_b, k.xt = a->x_stride_t, k.gb = a->g_stride_b, k.gt = a->g_stride_t, k.yb = a->d_y_stride_b, k.yt = a->d_y_stride_t;
   k.s0 = a->initial_state, k.ds = a->d_final_state, k.cu = a->cu_seqlens;
   k.y = a->y, k.dx = a->d_x, k.dg = a->d_g, k.sT = a->final_state, k.d0 = a->d_initial_state, k.kept = a->kept;
-  k.pairs = static_cast<float*>(a->workspace);
-  k.T = a->T, k.D = a->D, k.ctiles = channel_tiles(a), k.segs = segs, k.packed = a->nseq != 0;
+  k.T = a->T, k.D = a->D, k.ctiles = channel_tiles(a), k.tiles = tiles_of(a), k.packed = a->nseq != 0;
+  if (chained(a)) {
+    uint32_t* w = static_cast<uint32_t*>(a->workspace);
+    k.pairs = reinterpret_cast<uint64_t*>(w), k.sums = k.pairs + (int64_t)rows_of(a) * k.tiles * k.D, k.anchors = w + pair_words(a), k.counters = w + all_words(a);
+  }
   return k;
 }
 
 template <typename T, typename G, bool VEC> void launch(const lnx_linrec_args* a, bool bwd, hipStream_t st) {
-  const int segs = segments(a);
-  const Args k = kernel_args(a, segs);
-  const dim3 grid((unsigned)((int64_t)rows_of(a) * k.ctiles * segs));
-  if (bwd) {
-    if (segs > 1) {
-      lnx_profile_mark("linrec_bwd_pairs", st);
-      linrec_bwd_kernel<T, G, VEC, true><<<grid, THREADS, 0, st>>>(k);
-    }
-    lnx_profile_mark("linrec_bwd", st);
-    linrec_bwd_kernel<T, G, VEC, false><<<grid, THREADS, 0, st>>>(k);
+  const Args k = kernel_args(a);
+  const int groups = (int)((int64_t)rows_of(a) * k.ctiles);
+  if (chained(a)) {
+    const int64_t words = all_words(a), threads = words / 4 + 1 > groups ? words / 4 + 1 : groups;
+    lnx_profile_mark("linrec_clear", st);
+    linrec_clear_kernel<<<dim3((unsigned)((threads + 255) / 256)), 256, 0, st>>>(static_cast<uint32_t*>(a->workspace), words, k.counters, groups);
+    const dim3 grid((unsigned)((int64_t)groups * k.tiles));
+    lnx_profile_mark(bwd ? "linrec_bwd_chain" : "linrec_fwd_chain", st);
+    if (bwd) linrec_bwd_chain_kernel<T, G, VEC><<<grid, CTHREADS, 0, st>>>(k, groups);
+    else linrec_fwd_chain_kernel<T, G, VEC><<<grid, CTHREADS, 0, st>>>(k, groups);
   } else {
-    if (segs > 1) {
-      lnx_profile_mark("linrec_fwd_pairs", st);
-      linrec_fwd_kernel<T, G, VEC, true><<<grid, THREADS, 0, st>>>(k);
-    }
-    lnx_profile_mark("linrec_fwd", st);
-    linrec_fwd_kernel<T, G, VEC, false><<<grid, THREADS, 0, st>>>(k);
+    lnx_profile_mark(bwd ? "linrec_bwd" : "linrec_fwd", st);
+    if (bwd) linrec_bwd_kernel<T, G, VEC><<<dim3((unsigned)groups), THREADS, 0, st>>>(k);
+    else linrec_fwd_kernel<T, G, VEC><<<dim3((unsigned)groups), THREADS, 0, st>>>(k);
   }
 }
 
@@ -507,13 +695,12 @@ template <typename T, typename G> void launch_step(const void* x, const void* g,
 
 extern "C" uint64_t lnx_linrec_workspace_bytes(const lnx_linrec_args* a) {
   if (!a || a->D <= 0 || a->T < 0 || rows_of(a) <= 0) return 0;
-  const int s = segments(a);
-  return s > 1 ? (uint64_t)rows_of(a) * s * 2 * a->D * sizeof(float) : 0;
+  return chained(a) ? ((uint64_t)all_words(a) + (uint64_t)rows_of(a) * channel_tiles(a)) * sizeof(uint32_t) : 0;
 }
 
 extern "C" uint64_t lnx_linrec_kept_bytes(const lnx_linrec_args* a) {
   if (!a || a->D <= 0 || a->T < 0 || rows_of(a) <= 0) return 0;
-  const uint64_t slots = a->nseq ? (uint64_t)a->T / TILE + a->nseq : (uint64_t)a->B * (((int64_t)a->T + TILE - 1) / TILE);
+  const uint64_t slots = a->nseq ? (uint64_t)a->T / KEPT + a->nseq : (uint64_t)a->B * (((int64_t)a->T + KEPT - 1) / KEPT);
   return slots * a->D * sizeof(float);
 }
 

@@ -68,8 +68,8 @@ def test_recurrence_refusals():
     _refused(lib.lnx_linrec_fwd(a, None), -4, b"workspace")
     a.B = 0
     assert lib.lnx_linrec_fwd(a, None) == 0 and lib.lnx_linrec_workspace_bytes(a) == 0 and lib.lnx_linrec_kept_bytes(a) == 0
-    assert lib.lnx_linrec_kept_bytes(_lib.LinrecArgs(B=3, T=257, D=5)) == 3 * 2 * 5 * 4
-    assert lib.lnx_linrec_kept_bytes(_lib.LinrecArgs(B=1, T=1000, D=5, nseq=7)) == (1000 // 256 + 7) * 5 * 4
+    assert lib.lnx_linrec_kept_bytes(_lib.LinrecArgs(B=3, T=257, D=5)) == 3 * 3 * 5 * 4
+    assert lib.lnx_linrec_kept_bytes(_lib.LinrecArgs(B=1, T=1000, D=5, nseq=7)) == (1000 // 128 + 7) * 5 * 4
     assert lib.lnx_linrec_step(None, None, None, None, None, 0, 0, 0, None) == 0
     _refused(lib.lnx_linrec_step(None, None, None, None, None, 4, 0, 0, None), -1, b"required")
     _refused(lib.lnx_linrec_step(None, None, None, None, None, -1, 0, 0, None), -2, b"n=-1")

@@ -107,6 +107,40 @@ def test_forward_and_gradients(B, T, D, types):
     _check(*_inputs(B, T, D, *types, rows=B), state=(T % 2 == 1))
 
 
+def test_one_long_row():
+    """More than 1024 tiles of 128 tokens of few channels: pairs of one tile, of 32 and published states all take part."""
+    _check(*_inputs(1, 135_000, 3, "bf16", "f32", rows=1))
+
+
+def test_chained_tiles_repeat_bit_for_bit():
+    x, g, s0, dy, ds = _inputs(1, 20_000, 64, "bf16", "bf16", rows=1)
+    leaves = [t.detach().requires_grad_() for t in (x, g, s0)]
+
+    def both():
+        y, sT = la.gated_linear_recurrence(*leaves)
+        return (y, sT, *torch.autograd.grad([y, sT], leaves, [dy, ds]))
+
+    first = both()
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(first, both()))
+
+
+def test_two_streams_at_once():
+    """Calls that overlap on two streams have workspaces of their own."""
+    sets = [_inputs(1, 9000, 256, "bf16", "f32", rows=1, seed=s)[:3] for s in (1, 2)]
+    want = [la.gated_linear_recurrence(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(la.gated_linear_recurrence(*sets[i]))
+    torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        assert all(torch.equal(w[0], y) and torch.equal(w[1], s) for y, s in g)
+
+
 @pytest.mark.parametrize("types", [("bf16", "f32"), ("f32", "f32")], ids="-".join)
 @pytest.mark.parametrize("lens", [[1], [1, 1, 1], [0, 5, 0, 0, 300, 1, 0], [128, 256, 127, 129], [2500, 3, 1024]], ids=str)
 def test_packed(lens, types):
