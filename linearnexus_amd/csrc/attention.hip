@@ -131,8 +131,8 @@ __device__ __forceinline__ void dma16_at(const void* base, unsigned off, unsigne
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(__builtin_amdgcn_readfirstlane(dst)) : "memory", "m0");
 }
 // Brings tiles of [len][d] matrices with one row stride to LDS by the workgroup's four waves: which bytes a lane fetches is formed once.
-template <typename T, int D> struct Mover {
-  typedef Tile<T, D> TL;
+template <typename T, int D, int R = ROWS> struct Mover {
+  typedef Tile<T, D, R> TL;
   static constexpr int N = TL::BYTES / 1024 / 4;
   unsigned off[N];
   int64_t st;
@@ -147,7 +147,7 @@ template <typename T, int D> struct Mover {
   }
   // rows row0 .. row0 + 63; rows behind the last are copies of the last, columns behind d keep the zeros that clear_lds left
   __device__ __forceinline__ void fetch(unsigned tile, const T* matrix, int row0, int len) const {
-    if (row0 + ROWS <= len && d == D) {
+    if (row0 + R <= len && d == D) {
       const T* base = matrix + (int64_t)row0 * st;
 #pragma unroll
       for (int i = 0; i < N; ++i) dma16_at(base, off[i], tile + 1024 * (wave * N + i));
@@ -164,8 +164,8 @@ template <typename T, int D> struct Mover {
 __device__ __forceinline__ bool is_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 // Whether the granules that this lane's loads brought hold finite values only; SCRUB: the others become 0.  A wave's granules are
 // rows 16 wave .. 16 wave + 15.
-template <typename T, int D, bool SCRUB> __device__ __forceinline__ bool tile_finite(T* tile, int wave, int lane) {
-  constexpr int N = Tile<T, D>::BYTES / 1024 / 4, VN = Vec16<T>::N;
+template <typename T, int D, bool SCRUB, int R = ROWS> __device__ __forceinline__ bool tile_finite(T* tile, int wave, int lane) {
+  constexpr int N = Tile<T, D, R>::BYTES / 1024 / 4, VN = Vec16<T>::N;
   bool ok = true;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -329,9 +329,14 @@ template <typename T, int M> __device__ __forceinline__ void store_low(T* p, con
     }
 }
 
+// Keys of a tile of the forward pass: with 32 three workgroups share a CU (registers, LDS) and less of the diagonal is wasted: eight packed
+// prompts of 8192 tokens 175 us with 64, 160 with 32; B2 H16/4 T4096 154 and 156.
+template <typename T, int D> constexpr int fwd_rows() { return sizeof(T) == 2 && D == 128 ? 32 : 64; }
+
 // A wave owns 32 queries, the workgroup 128; of a block's key tiles every a.parts-th.
-template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kernel(Args a) {
-  typedef Tile<T, D> TL;
+template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 3 : 1) void attn_fwd_kernel(Args a) {
+  constexpr int KT = fwd_rows<T, D>(), KH = KT / 32;
+  typedef Tile<T, D, KT> TL;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const auto kt = [](int buf) { return reinterpret_cast<T*>(lds + 2 * buf * TL::BYTES); };
   const auto vt = [](int buf) { return reinterpret_cast<T*>(lds + (2 * buf + 1) * TL::BYTES); };
@@ -342,15 +347,15 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
   const int h = p.hkv * a.G + p.g, q_wg = p.blk * 128, q0 = q_wg + wave * 32, q = q0 + n;
   const T* kb = at<T>(a.k, a.ks, p.b, p.hkv, p.tok);
   const T* vb = at<T>(a.v, a.vs, p.b, p.hkv, p.tok);
-  const int q_end = min(q_wg + 128, p.len), ntile = (q_end + ROWS - 1) / ROWS;
+  const int q_end = min(q_wg + 128, p.len), ntile = (q_end + KT - 1) / KT;
   if (a.d < D) clear_lds(lds, 4 * TL::BYTES);
   if (threadIdx.x < 2) odd[threadIdx.x] = 0;
   lds_barrier();
-  const Mover<T, D> mk(a.ks[2], a.d, wave, lane), mv(a.vs[2], a.d, wave, lane);
+  const Mover<T, D, KT> mk(a.ks[2], a.d, wave, lane), mv(a.vs[2], a.d, wave, lane);
   const unsigned lds0 = lds_byte_addr(lds);
   if (p.part < ntile) {
-    mk.fetch(lds0, kb, p.part * ROWS, p.len);
-    mv.fetch(lds0 + TL::BYTES, vb, p.part * ROWS, p.len);
+    mk.fetch(lds0, kb, p.part * KT, p.len);
+    mv.fetch(lds0 + TL::BYTES, vb, p.part * KT, p.len);
   }
   // queries as B operands; a negative scale turns their sign, so that the largest product has the largest score
   const float c = fmaxf(fabsf(a.scale) * LOG2E, 1e-30f);  // above 0: -inf stays what a masked score is
@@ -371,39 +376,39 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
     for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
   const unsigned row_addr = lds0 + TL::rows(lane), col_addr = lds0 + TL::cols(lane);
   for (int it = p.part, buf = 0; it < ntile; it += a.parts, buf ^= 1) {
-    const int key0 = it * ROWS, next = key0 + a.parts * ROWS;
+    const int key0 = it * KT, next = key0 + a.parts * KT;
     const unsigned rows = row_addr + 2 * buf * TL::BYTES, cols = col_addr + 2 * buf * TL::BYTES;
     dma_wait<0>();
-    const bool edge = key0 + ROWS > q_wg;  // some pairs of this tile are masked
-    if (edge && !tile_finite<T, D, true>(vt(buf), wave, lane)) odd[buf] = 1;
+    const bool edge = key0 + KT > q_wg;  // some pairs of this tile are masked
+    if (edge && !tile_finite<T, D, true, KT>(vt(buf), wave, lane)) odd[buf] = 1;
     lds_barrier();
     if (it + a.parts < ntile) {
       mk.fetch(lds0 + 2 * (buf ^ 1) * TL::BYTES, kb, next, p.len);
       mv.fetch(lds0 + (2 * (buf ^ 1) + 1) * TL::BYTES, vb, next, p.len);
     }
     if (key0 >= q0 + 32) continue;  // behind all of this wave's queries
-    floatx16 sc[2];
+    floatx16 sc[KH];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < KH; ++i)
 #pragma unroll
       for (int e = 0; e < 16; ++e) sc[i][e] = 0.f;
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < KH; ++i)
 #pragma unroll
       for (int s = 0; s < D / 16; ++s) mma(sc[i], TL::by_row(rows, 32 * i * TL::ROWB, s), qf[s]);
-    read_ahead<T, false, 2 * (D / 16), 4>();
+    read_ahead<T, false, KH * (D / 16), 4>();
     __builtin_amdgcn_s_setprio(0);
-    if (key0 + ROWS - 1 > q0) {
+    if (key0 + KT - 1 > q0) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < KH; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           if (key0 + 32 * i + frag_row(e, lane) > q) sc[i][e] = -INFINITY;
     }
     float top = sc[0][0];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < KH; ++i)
 #pragma unroll
       for (int e = 0; e < 16; ++e) top = fmaxf(top, sc[i][e]);
     top = half_max(top);
@@ -421,24 +426,24 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
     const float ref = m == -INFINITY ? 0.f : m * c;
     float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < KH; ++i)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         sc[i][e] = __builtin_amdgcn_exp2f(sc[i][e] * c - ref);
         sum += sc[i][e];
       }
     l += sum;
-    Frag8<T> pf[4];
+    Frag8<T> pf[2 * KH];
 #pragma unroll
-    for (int s = 0; s < 4; ++s) from_acc(pf[s], sc[s >> 1], s & 1);
+    for (int s = 0; s < 2 * KH; ++s) from_acc(pf[s], sc[s >> 1], s & 1);
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
+    for (int s = 0; s < 2 * KH; ++s)
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) mma(acc[i], TL::by_col(cols, TL::BYTES + 16 * s * TL::ROWB, i), pf[s]);
-    read_ahead<T, true, 4 * (D / 32), 4>();
+    read_ahead<T, true, 2 * KH * (D / 32), 4>();
     if (edge && odd[buf])
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < KH; ++i) {
         const Frag8<T> two[2] = {pf[2 * i], pf[2 * i + 1]};
         add_odd<T, D / 32>(acc, vb, a.vs[2], key0 + 32 * i, p.len, a.d, two, lane, [&](int row) { return row <= q; });
       }
@@ -818,24 +823,23 @@ int parts_for(int64_t wgs, int64_t longest, int slots, double share, double laun
   }
   return best;
 }
-enum { FWD, DQ, DKV };
+enum { QUERIES, DKV };  // the forward and the dq kernel, whose blocks are queries; the dk / dv kernel
 int parts_of(const lnx_attn_args* a, int kernel) {
   const int64_t len = a->nseq ? (a->T + a->nseq - 1) / a->nseq : a->T, rows = a->nseq ? a->nseq : a->B;  // sequences of the average length
   const bool bf16 = a->dtype == LNX_BF16;
-  const int slots = bf16 ? 512 : 256;
   const double share = bf16 ? 5 : 1, launch = bf16 ? 4 : 1.5;
-  const int64_t keys = (len + ROWS - 1) / ROWS;
-  if (kernel == DKV) return parts_for(rows * a->Hkv * keys, keys * (a->H / a->Hkv), slots, share / 2, launch);
-  return parts_for(rows * a->H * ((len + 127) / 128), keys, slots, share, launch);
+  const int64_t keys = (len + ROWS - 1) / ROWS, queries = (len + 127) / 128;
+  if (kernel == DKV) return parts_for(rows * a->Hkv * keys, keys * (a->H / a->Hkv), bf16 ? 512 : 256, share / 2, launch);
+  return parts_for(rows * a->H * queries, keys, bf16 ? 512 : 256, share, launch);
 }
 // Bytes of the workspaces: shares of the forward kernel; delta and the shares of either gradient kernel
 uint64_t fwd_bytes(const lnx_attn_args* a) {
-  const int s = parts_of(a, FWD);
+  const int s = parts_of(a, QUERIES);
   return s > 1 ? (uint64_t)s * a->B * a->H * a->T * (a->d + 2) * sizeof(float) : 0;
 }
 uint64_t delta_bytes(const lnx_attn_args* a) { return ((uint64_t)a->B * a->H * a->T * sizeof(float) + 15) / 16 * 16; }
 uint64_t bwd_bytes(const lnx_attn_args* a) {
-  const int sq = parts_of(a, DQ), sk = parts_of(a, DKV);
+  const int sq = parts_of(a, QUERIES), sk = parts_of(a, DKV);
   const uint64_t q = sq > 1 ? (uint64_t)sq * a->B * a->H * a->T * a->d * sizeof(float) : 0, k = sk > 1 ? (uint64_t)sk * 2 * a->B * a->Hkv * a->T * a->d * sizeof(float) : 0;
   return delta_bytes(a) + (q > k ? q : k);
 }
@@ -888,10 +892,10 @@ template <typename K> int start(K kernel, const char* name, const Args& a, int64
 
 template <typename T, int D> int launch_fwd(const lnx_attn_args* a, hipStream_t st) {
   Args k = kernel_args(a);
-  k.nblk = (int)blocks_of(a, 128), k.parts = parts_of(a, FWD);
+  k.nblk = (int)blocks_of(a, 128), k.parts = parts_of(a, QUERIES);
   const int64_t rows = (int64_t)k.B * k.H * k.T;
   k.part = static_cast<float*>(a->workspace), k.part_stat = k.part ? k.part + k.parts * rows * k.d : nullptr;
-  if (int rc = start(attn_fwd_kernel<T, D>, "attn_fwd", k, (int64_t)k.B * k.H * k.nblk * k.parts, 4 * Tile<T, D>::BYTES + 16, st)) return rc;
+  if (int rc = start(attn_fwd_kernel<T, D>, "attn_fwd", k, (int64_t)k.B * k.H * k.nblk * k.parts, 4 * Tile<T, D, fwd_rows<T, D>()>::BYTES + 16, st)) return rc;
   if (k.parts > 1) {
     lnx_profile_mark("attn_join", st);
     attn_join_kernel<T><<<dim3((unsigned)((rows + 15) / 16)), 256, 0, st>>>(k);
@@ -908,7 +912,7 @@ template <typename T, int D> int launch_bwd(const lnx_attn_args* a, hipStream_t 
   Args k = kernel_args(a);
   k.delta = static_cast<float*>(a->workspace);
   k.part = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + delta_bytes(a));
-  k.nblk = (int)blocks_of(a, 128), k.parts = parts_of(a, DQ);  // first: it leaves delta
+  k.nblk = (int)blocks_of(a, 128), k.parts = parts_of(a, QUERIES);  // first: it leaves delta
   if (int rc = start(attn_dq_kernel<T, D>, "attn_dq", k, (int64_t)k.B * k.H * k.nblk * k.parts, 4 * Tile<T, D>::BYTES + 16, st)) return rc;
   if (k.parts > 1) sum_parts<T>(k, k.part, (int64_t)k.B * k.H * k.T, k.dq, k.dqs, k.H, st);
   k.nblk = (int)blocks_of(a, ROWS), k.parts = parts_of(a, DKV);
