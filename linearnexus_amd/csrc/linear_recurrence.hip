@@ -59,10 +59,10 @@ struct Args {
   const int32_t* cu;
   void *y, *dx, *dg;
   float *sT, *d0, *kept;
-  uint64_t *pairs, *sums;  // [rows][tiles][D], (A, H) of a tile, [rows][tiles / GROUP][D], of GROUP tiles; all bits set: not there yet
-  uint32_t* anchors;       // [rows][tiles / ANCHOR][D], the state behind ANCHOR, 2 ANCHOR, ... tiles; likewise
+  uint64_t *pairs, *sums;  // [slots of CTILE tokens][D], (A, H) of a tile, [slots of GROUP tiles][D], of GROUP tiles; all bits set: not there yet
+  uint32_t* anchors;       // [slots of ANCHOR tiles][D], the state behind ANCHOR, 2 ANCHOR, ... tiles of a row; likewise
   uint32_t* counters;      // [rows][channel tiles]: tiles taken
-  int T, D, ctiles, tiles;
+  int T, D, ctiles;
   bool packed;
 };
 
@@ -70,20 +70,23 @@ struct Args {
 template <typename T> struct Place {
   int row, len, ntile, c0, c, left;  // c0: the workgroup's first channel, c: this thread's
   int64_t tok, slot;  // first token in a packed batch (0 otherwise); first kept state
-  __device__ __forceinline__ Place(const Args& a, int group, int tile) {
-    row = group / a.ctiles;
+  // The first slot of the row where each holds `size` tokens
+  __device__ __forceinline__ int64_t slot_of(const Args& a, int size) const {
+    return a.packed ? packed_slot((int)tok, row, size) : (int64_t)row * (((int64_t)a.T + size - 1) / size);
+  }
+  __device__ __forceinline__ Place(const Args& a, int row_, int ct, int tile) {
+    row = row_;
     if (a.packed) {
       const int first = seq_first(a.cu, row, a.T);
       len = seq_end(a.cu, row, a.T) - first;
       tok = first;
-      slot = first / KEPT + row;
     } else {
       len = a.T;
       tok = 0;
-      slot = (int64_t)row * (((int64_t)a.T + KEPT - 1) / KEPT);
     }
+    slot = slot_of(a, KEPT);
     ntile = (int)(((int64_t)len + tile - 1) / tile);
-    c0 = group % a.ctiles * Shape<T>::C;
+    c0 = ct * Shape<T>::C;
     c = c0 + (threadIdx.x & (Shape<T>::COLS - 1)) * N;
     left = a.D - c;
   }
@@ -221,27 +224,32 @@ __device__ __forceinline__ void fold(float& A, float& H, const uint64_t* p, int 
 }
 // The state before the j-th of ntile tiles (counted from where the recurrence starts), from `begin` before the first; (A, H) is the
 // tile's pair.  Leaves what others wait for before it waits for what comes before the tile's group.  One lane per channel.
-__device__ __forceinline__ float state_before(const Args& a, int row, int j, int ntile, int chan, float begin, float A, float H) {
-  const int base = j / GROUP * GROUP, top = j / ANCHOR * ANCHOR;
-  uint64_t* pairs = a.pairs + (int64_t)row * a.tiles * a.D + chan;
-  uint64_t* sums = a.sums + (int64_t)row * (a.tiles / GROUP) * a.D + chan;
+template <typename P> __device__ __forceinline__ float state_before(const Args& a, const P& p, int j, int chan, float begin, float A, float H) {
+  const int base = j / GROUP * GROUP, top = j / ANCHOR * ANCHOR, ntile = p.ntile;
+  uint64_t* pairs = a.pairs + p.slot_of(a, CTILE) * a.D + chan;
+  uint64_t* sums = a.sums + p.slot_of(a, CTILE * GROUP) * a.D + chan;
   if (j + 1 < ntile) publish(pairs + (int64_t)j * a.D, A, H);
   float Ag = 1.f, Hg = 0.f;
   fold(Ag, Hg, pairs + (int64_t)base * a.D, j - base, a.D);
   if (j - base == GROUP - 1 && j + 1 < ntile) publish(sums + (int64_t)(j / GROUP) * a.D, A * Ag, A * Hg + H);
   float state = begin;
   if (top) {
-    const uint32_t* p = a.anchors + ((int64_t)row * (a.tiles / ANCHOR) + top / ANCHOR - 1) * a.D + chan;
-    state = __uint_as_float(await(p, peek(p)));
+    const uint32_t* at = a.anchors + (p.slot_of(a, CTILE * ANCHOR) + top / ANCHOR - 1) * a.D + chan;
+    state = __uint_as_float(await(at, peek(at)));
   }
   float unused = 1.f;
   fold(unused, state, sums + (int64_t)(top / GROUP) * a.D, (base - top) / GROUP, a.D);
   return Ag * state + Hg;
 }
-__device__ __forceinline__ void leave_state(const Args& a, int row, int j, int ntile, int chan, float state) {
-  if ((j + 1) % ANCHOR == 0 && j + 1 < ntile) publish(a.anchors + ((int64_t)row * (a.tiles / ANCHOR) + (j + 1) / ANCHOR - 1) * a.D + chan, state);
+template <typename P> __device__ __forceinline__ void leave_state(const Args& a, const P& p, int j, int chan, float state) {
+  if ((j + 1) % ANCHOR == 0 && j + 1 < p.ntile) publish(a.anchors + (p.slot_of(a, CTILE * ANCHOR) + (j + 1) / ANCHOR - 1) * a.D + chan, state);
 }
-// The tile of this workgroup: the next one of its group
+// The row of this workgroup; its channel tile is blockIdx % ctiles
+__device__ __forceinline__ int chain_row(const Args& a, int rows) {
+  const int unit = blockIdx.x / a.ctiles;
+  return a.packed ? packed_owner(a.cu, rows, a.T, CTILE, unit) : unit % rows;
+}
+// The tile of this workgroup: the next one of its row and channels
 __device__ __forceinline__ int take_tile(const Args& a, int group) {
   __shared__ int tile;
   if (threadIdx.x == 0) tile = (int)__hip_atomic_fetch_add(a.counters + group, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -316,7 +324,7 @@ __device__ __forceinline__ void reduce_forward(const Tokens<T, G, VEC>& in, floa
 template <typename T, typename G, bool VEC> __global__ __launch_bounds__(THREADS) void linrec_fwd_kernel(Args a) {
   constexpr int R = Shape<T>::R, COLS = Shape<T>::COLS, C = Shape<T>::C;
   __shared__ Waves<COLS, 8> ws;
-  const Place<T> p(a, blockIdx.x, TILE);
+  const Place<T> p(a, blockIdx.x / a.ctiles, blockIdx.x % a.ctiles, TILE);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   // the chain's lanes: one channel each
   const int chan = p.c0 + lane;
@@ -352,11 +360,11 @@ template <typename T, typename G, bool VEC> __global__ __launch_bounds__(THREADS
   if (in_chan) a.sT[(int64_t)p.row * a.D + chan] = carry;
 }
 
-template <typename T, typename G, bool VEC> __global__ __launch_bounds__(CTHREADS) void linrec_fwd_chain_kernel(Args a, int groups) {
+template <typename T, typename G, bool VEC> __global__ __launch_bounds__(CTHREADS) void linrec_fwd_chain_kernel(Args a, int rows) {
   constexpr int R = Shape<T>::R, COLS = Shape<T>::COLS, C = Shape<T>::C;
   __shared__ Waves<COLS, 4> ws;
-  const int group = blockIdx.x % groups, j = take_tile(a, group);
-  const Place<T> p(a, group, CTILE);
+  const int row = chain_row(a, rows), ct = blockIdx.x % a.ctiles, j = take_tile(a, row * a.ctiles + ct);
+  const Place<T> p(a, row, ct, CTILE);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, chan = p.c0 + lane;
   const bool in_chan = wave == 0 && lane < C && chan < a.D;
   const int64_t row_c = (int64_t)p.row * a.D + chan;
@@ -377,10 +385,10 @@ template <typename T, typename G, bool VEC> __global__ __launch_bounds__(CTHREAD
   if (in_chan) {
     float At, Ht;
     ws.template total<true>(lane, At, Ht);
-    float carry = state_before(a, p.row, j, p.ntile, chan, a.s0 ? a.s0[row_c] : 0.f, At, Ht);
+    float carry = state_before(a, p, j, chan, a.s0 ? a.s0[row_c] : 0.f, At, Ht);
     if (a.kept) a.kept[(p.slot + j) * a.D + chan] = carry;
     ws.template chain<true>(lane, carry);
-    leave_state(a, p.row, j, p.ntile, chan, carry);
+    leave_state(a, p, j, chan, carry);
     if (j + 1 == p.ntile) a.sT[row_c] = carry;
   }
   lds_barrier();
@@ -484,7 +492,7 @@ __device__ __forceinline__ void reduce_backward(const Tokens<T, G, VEC>& in, con
 template <typename T, typename G, bool VEC> __global__ __launch_bounds__(THREADS) void linrec_bwd_kernel(Args a) {
   constexpr int R = Shape<T>::R, COLS = Shape<T>::COLS, C = Shape<T>::C;
   __shared__ Waves<COLS, 8> ws, wf;
-  const Place<T> p(a, blockIdx.x, TILE);
+  const Place<T> p(a, blockIdx.x / a.ctiles, blockIdx.x % a.ctiles, TILE);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int chan = p.c0 + lane;  // wave 0 chains the gradients, wave 1 the states
   const bool mine = lane < C && chan < a.D, grads = wave == 0 && lane < C, states = wave == 1 && lane < C;
@@ -528,11 +536,11 @@ template <typename T, typename G, bool VEC> __global__ __launch_bounds__(THREADS
   if (grads && mine && a.d0) a.d0[(int64_t)p.row * a.D + chan] = carry;
 }
 
-template <typename T, typename G, bool VEC> __global__ __launch_bounds__(CTHREADS) void linrec_bwd_chain_kernel(Args a, int groups) {
+template <typename T, typename G, bool VEC> __global__ __launch_bounds__(CTHREADS) void linrec_bwd_chain_kernel(Args a, int rows) {
   constexpr int R = Shape<T>::R, COLS = Shape<T>::COLS, C = Shape<T>::C;
   __shared__ Waves<COLS, 4> ws, wf;
-  const int group = blockIdx.x % groups, j = take_tile(a, group);
-  const Place<T> p(a, group, CTILE);
+  const int row = chain_row(a, rows), ct = blockIdx.x % a.ctiles, j = take_tile(a, row * a.ctiles + ct);
+  const Place<T> p(a, row, ct, CTILE);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, chan = p.c0 + lane;
   const bool mine = lane < C && chan < a.D, grads = wave == 0 && mine, states = wave == 1 && mine;
   const int64_t row_c = (int64_t)p.row * a.D + chan;
@@ -559,9 +567,9 @@ template <typename T, typename G, bool VEC> __global__ __launch_bounds__(CTHREAD
   if (grads) {
     float At, Ht;
     ws.template total<false>(lane, At, Ht);
-    float carry = state_before(a, p.row, j, p.ntile, chan, a.ds ? a.ds[row_c] : 0.f, At, Ht);
+    float carry = state_before(a, p, j, chan, a.ds ? a.ds[row_c] : 0.f, At, Ht);
     ws.template chain<false>(lane, carry);
-    leave_state(a, p.row, j, p.ntile, chan, carry);
+    leave_state(a, p, j, chan, carry);
     if (tile == 0 && a.d0) a.d0[row_c] = carry;
   }
   if (states) {
@@ -592,25 +600,29 @@ template <typename T, typename G, int W> __global__ __launch_bounds__(256) void 
   }
 }
 
-constexpr int64_t MAX_STRIDE = 4 << 20;
+constexpr int64_t MAX_STRIDE = 4 << 20, MAX_GRID = 0xffffffff;  // threads of a launch
 int rows_of(const lnx_linrec_args* a) { return a->nseq ? a->nseq : a->B; }
 int channel_tiles(const lnx_linrec_args* a) {
   const int c = a->dtype == LNX_BF16 ? Shape<bf16_t>::C : Shape<float>::C;
   return (int)(((int64_t)a->D + c - 1) / c);
 }
 
-int tiles_of(const lnx_linrec_args* a) { return (int)(((int64_t)a->T + CTILE - 1) / CTILE); }
+// Slots of `size` tokens in all rows
+int64_t slots_of(const lnx_linrec_args* a, int64_t size) { return a->nseq ? a->T / size + a->nseq : a->B * ((a->T + size - 1) / size); }
 // Whether every tile has a workgroup of its own: where walking the rows would leave a third of the chip without work.  With 256 rows and
 // channel tiles both forms move bytes at the same rate forwards and the walk is 13 % faster backwards ([8, 4096, 2048] bf16: 99 and
 // 99, 140 and 158 us); with 128 tiles of 1024 tokens the chained form is faster ([4, 1024, 2048]: 16.6 -> 14.7, 23.5 -> 19.4 us and a
 // clearing launch of 3), with 32 twice as fast (14.6 -> 9.0, 21 -> 10.3).
+// Packed rows are as long as the table on the device says, so every tile has a workgroup there from 1024 tokens on: of [1, 65536, 2048]
+// in 8 even rows the walk is 16 % faster (173 and 271 against 207 and 313 us), with all tokens in one of them four times as slow (811
+// and 1258 against 206 and 312); of 512 rows the walk takes 342 and 583 us, the chained form 188 and 307.
 bool chained(const lnx_linrec_args* a) {
-  const int64_t wgs = (int64_t)rows_of(a) * channel_tiles(a), len = a->nseq ? a->T / a->nseq : a->T;
-  return wgs < 160 && len >= 8 * CTILE && wgs * tiles_of(a) <= 0x7fffffff;
+  const int64_t wgs = (int64_t)rows_of(a) * channel_tiles(a);
+  return a->T >= 8 * CTILE && (a->nseq || wgs < 160) && slots_of(a, CTILE) * channel_tiles(a) <= MAX_GRID / CTHREADS;
 }
 // Bytes of what the workgroups leave for each other
-int64_t pair_words(const lnx_linrec_args* a) { return 2 * (int64_t)rows_of(a) * (tiles_of(a) + tiles_of(a) / GROUP) * a->D; }
-int64_t all_words(const lnx_linrec_args* a) { return pair_words(a) + ((int64_t)rows_of(a) * (tiles_of(a) / ANCHOR) * a->D + 3) / 4 * 4; }
+int64_t pair_words(const lnx_linrec_args* a) { return 2 * (slots_of(a, CTILE) + slots_of(a, CTILE * GROUP)) * a->D; }
+int64_t all_words(const lnx_linrec_args* a) { return pair_words(a) + (slots_of(a, CTILE * ANCHOR) * a->D + 3) / 4 * 4; }
 
 int check(const char* what, const lnx_linrec_args* a, bool bwd) {
   if (!a) return lnx_set_error(LNX_ERR_NULL, "%s: args is NULL", what);
@@ -627,7 +639,7 @@ int check(const char* what, const lnx_linrec_args* a, bool bwd) {
   for (int64_t st : {a->x_stride_t * (a->dtype == LNX_BF16 ? 2 : 4), a->g_stride_t * (a->g_dtype == LNX_BF16 ? 2 : 4), (bwd ? a->d_y_stride_t : 0) * (a->dtype == LNX_BF16 ? 2 : 4),
                      (int64_t)a->D * 4})
     if (st < 0 || st > MAX_STRIDE) return lnx_set_error(LNX_ERR_SHAPE, "%s: tokens more than %lld bytes apart", what, (long long)MAX_STRIDE);
-  if ((int64_t)rows_of(a) * channel_tiles(a) > 0x7fffffff) return lnx_set_error(LNX_ERR_SHAPE, "%s: too many rows", what);
+  if ((int64_t)rows_of(a) * channel_tiles(a) > MAX_GRID / THREADS) return lnx_set_error(LNX_ERR_SHAPE, "%s: too many rows", what);
   if (rows && chained(a)) {
     const uint64_t need = lnx_linrec_workspace_bytes(a);
     if (!a->workspace || a->workspace_bytes < need || reinterpret_cast<uintptr_t>(a->workspace) % 16) return lnx_set_error(LNX_ERR_WORKSPACE, "%s: needs a workspace of %llu bytes", what, (unsigned long long)need);
@@ -643,10 +655,10 @@ Args kernel_args(const lnx_linrec_args* a) {
   k.xb = a->x_stride_b, k.xt = a->x_stride_t, k.gb = a->g_stride_b, k.gt = a->g_stride_t, k.yb = a->d_y_stride_b, k.yt = a->d_y_stride_t;
   k.s0 = a->initial_state, k.ds = a->d_final_state, k.cu = a->cu_seqlens;
   k.y = a->y, k.dx = a->d_x, k.dg = a->d_g, k.sT = a->final_state, k.d0 = a->d_initial_state, k.kept = a->kept;
-  k.T = a->T, k.D = a->D, k.ctiles = channel_tiles(a), k.tiles = tiles_of(a), k.packed = a->nseq != 0;
+  k.T = a->T, k.D = a->D, k.ctiles = channel_tiles(a), k.packed = a->nseq != 0;
   if (chained(a)) {
     uint32_t* w = static_cast<uint32_t*>(a->workspace);
-    k.pairs = reinterpret_cast<uint64_t*>(w), k.sums = k.pairs + (int64_t)rows_of(a) * k.tiles * k.D, k.anchors = w + pair_words(a), k.counters = w + all_words(a);
+    k.pairs = reinterpret_cast<uint64_t*>(w), k.sums = k.pairs + slots_of(a, CTILE) * k.D, k.anchors = w + pair_words(a), k.counters = w + all_words(a);
   }
   return k;
 }
@@ -658,10 +670,10 @@ template <typename T, typename G, bool VEC> void launch(const lnx_linrec_args* a
     const int64_t words = all_words(a), threads = words / 4 + 1 > groups ? words / 4 + 1 : groups;
     lnx_profile_mark("linrec_clear", st);
     linrec_clear_kernel<<<dim3((unsigned)((threads + 255) / 256)), 256, 0, st>>>(static_cast<uint32_t*>(a->workspace), words, k.counters, groups);
-    const dim3 grid((unsigned)((int64_t)groups * k.tiles));
+    const dim3 grid((unsigned)(slots_of(a, CTILE) * k.ctiles));
     lnx_profile_mark(bwd ? "linrec_bwd_chain" : "linrec_fwd_chain", st);
-    if (bwd) linrec_bwd_chain_kernel<T, G, VEC><<<grid, CTHREADS, 0, st>>>(k, groups);
-    else linrec_fwd_chain_kernel<T, G, VEC><<<grid, CTHREADS, 0, st>>>(k, groups);
+    if (bwd) linrec_bwd_chain_kernel<T, G, VEC><<<grid, CTHREADS, 0, st>>>(k, rows_of(a));
+    else linrec_fwd_chain_kernel<T, G, VEC><<<grid, CTHREADS, 0, st>>>(k, rows_of(a));
   } else {
     lnx_profile_mark(bwd ? "linrec_bwd" : "linrec_fwd", st);
     if (bwd) linrec_bwd_kernel<T, G, VEC><<<dim3((unsigned)groups), THREADS, 0, st>>>(k);
@@ -717,6 +729,7 @@ extern "C" int lnx_linrec_step(const void* x, const void* g, const float* state,
   hipStream_t st = static_cast<hipStream_t>(hip_stream);
   bool vec = n % 4 == 0;
   for (const void* p : {x, g, (const void*)state, (const void*)y, (const void*)new_state}) vec = vec && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+  if ((vec ? n / 4 : n) > MAX_GRID - 256) return lnx_set_error(LNX_ERR_SHAPE, "linrec_step: n=%lld is too large for one launch", (long long)n);
   lnx_profile_mark("linrec_step", st);
   if (dtype == LNX_F32) launch_step<float, float>(x, g, state, y, new_state, n, vec, st);
   else if (g_dtype == LNX_F32) launch_step<bf16_t, float>(x, g, state, y, new_state, n, vec, st);
