@@ -16,6 +16,7 @@
 namespace {
 
 constexpr int ROWS = 64;  // rows of a tile
+constexpr int64_t MAX_GRID = 0xffffffff / 256;  // workgroups of a launch
 constexpr float LOG2E = 1.4426950408889634f;
 __device__ __forceinline__ unsigned fresh(unsigned x) { return (unsigned)::fresh((int)x); }
 
@@ -269,32 +270,13 @@ __device__ __forceinline__ Place place(const Args& a, int size, int heads, bool 
     p.blk = last_first ? a.nblk - 1 - blk : blk;
     return p;
   }
-  // packed: the sequence that holds block `blk` of all sequences' blocks, one lane per sequence
-  const int lane = threadIdx.x & 63;
-  p.on = false;
-  for (int s0 = 0, before = 0; s0 < a.nseq; s0 += 64) {
-    const int s = s0 + lane;
-    const int first = s < a.nseq ? seq_first(a.cu, s, a.T) : 0, len = s < a.nseq ? seq_end(a.cu, s, a.T) - first : 0;
-    const int n = (len + size - 1) / size;
-    int upto = n;
-#pragma unroll
-    for (int k = 1; k < 64; k <<= 1) {
-      const int o = __shfl_up(upto, k, LNX_WAVE);
-      if (lane >= k) upto += o;
-    }
-    const uint64_t hit = __ballot(blk < before + upto);
-    if (hit) {
-      const int l = __builtin_ctzll(hit);
-      const int nb = __builtin_amdgcn_readlane(n, l), end = before + __builtin_amdgcn_readlane(upto, l);
-      p.tok = __builtin_amdgcn_readlane(first, l);
-      p.len = __builtin_amdgcn_readlane(len, l);
-      p.blk = blk - (end - nb);
-      if (last_first) p.blk = nb - 1 - p.blk;
-      p.on = true;
-      break;
-    }
-    before += __builtin_amdgcn_readlane(upto, 63);
-  }
+  const int seq = packed_owner(a.cu, a.nseq, a.T, size, blk);
+  p.tok = seq_first(a.cu, seq, a.T);
+  p.len = seq_end(a.cu, seq, a.T) - (int)p.tok;
+  const int n = (int)(((unsigned)p.len + size - 1) / size);
+  p.blk = (int)(blk - packed_slot((int)p.tok, seq, size));
+  p.on = p.blk >= 0 && p.blk < n;
+  if (last_first) p.blk = n - 1 - p.blk;
   return p;
 }
 template <typename T> __device__ __forceinline__ T* at(const void* p, const int64_t (&s)[3], int64_t b, int64_t h, int64_t t) {
@@ -868,7 +850,7 @@ int check(const char* what, const lnx_attn_args* a, bool bwd) {
   const uint64_t need = bwd ? bwd_bytes(a) : fwd_bytes(a);
   if (need && (!a->workspace || a->workspace_bytes < need || reinterpret_cast<uintptr_t>(a->workspace) % 16))
     return lnx_set_error(LNX_ERR_WORKSPACE, "%s: needs a 16-byte aligned workspace of %llu bytes", what, (unsigned long long)need);
-  if ((int64_t)a->B * a->H * blocks_of(a, ROWS) * 8 > 0x7fffffff || (int64_t)a->B * a->H * a->T / 16 >= 0x7fffffff)
+  if ((int64_t)a->B * a->H * blocks_of(a, ROWS) > MAX_GRID)  // nothing is split into parts where there are that many
     return lnx_set_error(LNX_ERR_SHAPE, "%s: too many rows", what);
   return LNX_OK;
 }
@@ -1113,37 +1095,66 @@ template <typename T, int D> __global__ __launch_bounds__(64 * step_waves<T>(), 
   }
 }
 
-// One wave per head joins its splits
-template <typename T, int D> __global__ __launch_bounds__(64) void attn_step_join_kernel(const float* part, T* o, int splits, int d) {
+// One workgroup per head joins its splits (1024 at most): the factors once, then every wave adds up shares of its own, eight loads in flight
+constexpr int MOST_SPLITS = 1024;
+template <typename T, int D> __global__ __launch_bounds__(1024) void attn_step_join_kernel(const float* part, T* o, int splits, int d) {
+  constexpr int M = D / 64;
+  __shared__ float factor[MOST_SPLITS], red[16][M][64];
   const int64_t row = blockIdx.x;
-  const int lane = threadIdx.x;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
   const float* p = part + row * splits * (D + 4);
-  float top = -INFINITY;
-  for (int s = 0; s < splits; ++s) top = fmaxf(top, p[s * (D + 4) + D]);
-  float sum = 0.f, t[D / 64];
+  float top = -INFINITY, sum = 0.f, t[M];
+  for (int s = lane; s < splits; s += 64) top = fmaxf(top, p[s * (D + 4) + D]);  // every wave on its own: one barrier less
 #pragma unroll
-  for (int i = 0; i < D / 64; ++i) t[i] = 0.f;
-  for (int s = 0; s < splits; ++s) {
-    const float* q = p + s * (D + 4);
-    const float f = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(q[D] - top);
-    sum += q[D + 1] * f;
-#pragma unroll
-    for (int i = 0; i < D / 64; ++i) t[i] += q[64 * i + lane] * f;
+  for (int k = 1; k < 64; k <<= 1) top = fmaxf(top, __shfl_xor(top, k, LNX_WAVE));
+  for (int s = lane; s < splits; s += 64) {
+    const float f = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(p[s * (D + 4) + D] - top);
+    if (wave == 0) factor[s] = f;
+    sum += p[s * (D + 4) + D + 1] * f;
   }
 #pragma unroll
-  for (int i = 0; i < D / 64; ++i)
+  for (int k = 1; k < 64; k <<= 1) sum += __shfl_xor(sum, k, LNX_WAVE);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < M; ++i) t[i] = 0.f;
+  for (int s0 = wave; s0 < splits; s0 += 8 * waves) {
+    float v[8][M];
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+#pragma unroll
+      for (int i = 0; i < M; ++i) v[u][i] = s0 + u * waves < splits ? p[(s0 + u * waves) * (D + 4) + 64 * i + lane] : 0.f;
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (s0 + u * waves < splits)
+#pragma unroll
+        for (int i = 0; i < M; ++i) t[i] += v[u][i] * factor[s0 + u * waves];
+  }
+  if (waves > 1) {
+#pragma unroll
+    for (int i = 0; i < M; ++i) red[wave][i][lane] = t[i];
+    __syncthreads();
+    if (wave > 0) return;
+    for (int w = 1; w < waves; ++w)
+#pragma unroll
+      for (int i = 0; i < M; ++i) t[i] += red[w][i][lane];
+  }
+#pragma unroll
+  for (int i = 0; i < M; ++i)
     if (64 * i + lane < d) o[row * d + 64 * i + lane] = from_f32<T>(t[i] / sum);
 }
 
 // Splits of a cache: workgroups for four to a CU, but two tiles a wave at least of a cache that is full
 int step_splits(const lnx_attn_step_args* a) {
   const int waves = a->dtype == LNX_BF16 ? step_waves<bf16_t>() : step_waves<float>();
-  const int64_t wgs = (int64_t)a->B * a->Hkv * ((a->H / a->Hkv + 31) / 32), tiles = (a->S + SROWS - 1) / SROWS;
-  int64_t s = (1024 + wgs - 1) / wgs;
+  const int64_t wgs = (int64_t)a->B * a->Hkv * ((a->H / a->Hkv + 31) / 32), tiles = ((int64_t)a->S + SROWS - 1) / SROWS;
+  int64_t s = (MOST_SPLITS + wgs - 1) / wgs;
   const int64_t most = (tiles + 2 * waves - 1) / (2 * waves);
   if (s > most) s = most;
   return (int)(s < 1 ? 1 : s);
 }
+
+// Threads of the joining workgroups: a wave for four shares
+int join_threads(int splits) { return 64 * (splits <= 4 ? 1 : splits >= 64 ? 16 : (splits + 3) / 4); }
 
 int check_step(const lnx_attn_step_args* a) {
   const char* what = "attn_step";
@@ -1161,9 +1172,10 @@ int check_step(const lnx_attn_step_args* a) {
   }
   if (!a->o || !a->lengths) return lnx_set_error(LNX_ERR_NULL, "%s: o and lengths are required", what);
   if (reinterpret_cast<uintptr_t>(a->o) % 16) return lnx_set_error(LNX_ERR_SHAPE, "%s: tensors must be 16-byte aligned, rows whole numbers of 16 bytes and at most 16 MiB apart", what);
-  if ((int64_t)a->B * a->H * step_splits(a) > 0x7fffffff) return lnx_set_error(LNX_ERR_SHAPE, "%s: too many rows", what);
+  if ((int64_t)a->B * a->H > MAX_GRID || (int64_t)a->B * a->Hkv * ((a->H / a->Hkv + 31) / 32) * step_splits(a) > MAX_GRID) return lnx_set_error(LNX_ERR_SHAPE, "%s: too many rows", what);
   const uint64_t need = lnx_attn_step_workspace_bytes(a);
-  if (need && (!a->workspace || a->workspace_bytes < need)) return lnx_set_error(LNX_ERR_WORKSPACE, "%s: needs a workspace of %llu bytes", what, (unsigned long long)need);
+  if (need && (!a->workspace || a->workspace_bytes < need || reinterpret_cast<uintptr_t>(a->workspace) % 16))
+    return lnx_set_error(LNX_ERR_WORKSPACE, "%s: needs a 16-byte aligned workspace of %llu bytes", what, (unsigned long long)need);
   return LNX_OK;
 }
 
@@ -1183,7 +1195,7 @@ template <typename T, int D> int launch_step(const lnx_attn_step_args* a, hipStr
   hipLaunchKernelGGL(kernel, dim3((unsigned)((int64_t)k.B * k.Hkv * k.ctiles * k.splits)), dim3(64 * W), bytes, st, k);
   if (k.splits > 1) {
     lnx_profile_mark("attn_step_join", st);
-    attn_step_join_kernel<T, D><<<dim3((unsigned)((int64_t)k.B * k.H)), 64, 0, st>>>(k.part, static_cast<T*>(a->o), k.splits, k.d);
+    attn_step_join_kernel<T, D><<<dim3((unsigned)((int64_t)k.B * k.H)), join_threads(k.splits), 0, st>>>(k.part, static_cast<T*>(a->o), k.splits, k.d);
   }
   return LNX_OK;
 }

@@ -14,6 +14,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 #include <optional>
@@ -1358,6 +1359,17 @@ bool vector_rows(const Tensor& t) {
     if (t.stride(i) * t.element_size() % 16) return false;
   return true;
 }
+// Whether no two rows share memory: each dimension steps over the whole extent of those with smaller strides
+bool disjoint_rows(const Tensor& t) {
+  int64_t extent = t.size(-1), order[3] = {0, 1, 2};
+  std::sort(order, order + 3, [&](int64_t a, int64_t b) { return t.stride(a) < t.stride(b); });
+  for (int64_t i : order) {
+    if (t.size(i) <= 1) continue;
+    if (t.stride(i) < extent) return false;
+    extent += (t.size(i) - 1) * t.stride(i);
+  }
+  return true;
+}
 Tensor as_rows(const Tensor& t) {
   if (vector_rows(t)) return t;
   const Tensor c = t.contiguous();
@@ -1466,11 +1478,10 @@ PyObject* py_causal_attention_step(PyObject*, PyObject* const* args, Py_ssize_t 
     TORCH_CHECK(t->scalar_type() == q.scalar_type(), op, ": ", name, " must have q's dtype ", q.scalar_type(), ", got ", t->scalar_type());
     TORCH_CHECK(t->dim() == 4 && t->size(0) == B && t->size(1) == Hkv && t->size(2) > 0 && t->size(3) == d && t->sizes() == kc.sizes(), op, ": ", name, " must be [", B, ", ", Hkv,
                 ", S, ", d, "], got ", shape_text(*t));
-    bool once = true;
-    for (int64_t i = 0; i < 3; ++i) once = once && (t->size(i) == 1 || t->stride(i) != 0);
-    TORCH_CHECK(vector_rows(*t) && once, op, ": ", name, " is written in place: its rows must be contiguous, 16-byte aligned and each its own memory");
+    TORCH_CHECK(vector_rows(*t) && disjoint_rows(*t), op, ": ", name, " is written in place: its rows must be contiguous, 16-byte aligned and each its own memory");
     TORCH_CHECK(t->size(2) <= INT32_MAX, op, ": ", name, " is too large, got ", shape_text(*t));
   }
+  TORCH_CHECK(B == 0 || kc.data_ptr() != vc.data_ptr(), op, ": k_cache and v_cache are the same memory");
   TORCH_CHECK(len.scalar_type() == at::kInt && len.dim() == 1 && len.size(0) == B && len.is_contiguous(), op, ": lengths must be a contiguous int32 [", B, "] tensor, got ",
               shape_text(len), " ", len.scalar_type());
   TORCH_CHECK(!wants_grad({&q, &k, &v, &kc, &vc}), "cannot differentiate through a step that updates its cache in place");

@@ -123,6 +123,24 @@ def test_many_short_sequences():
     _check(*_inputs(1, 2, 1, 450, 64, "bf16"), cu=cu)
 
 
+def test_more_sequences_than_a_wave_looks_at():
+    lens = [0, 3, 1, 0, 70, 2, 0, 1] * 60 + [200]
+    _check(*_inputs(1, 2, 1, sum(lens), 16, "bf16"), cu=np.concatenate([[0], np.cumsum(lens)]).tolist())
+    cu = np.concatenate([[0], np.cumsum([1, 0, 1] * 1700)]).tolist()  # every query has one key
+    q, k, v, do = _inputs(1, 2, 2, cu[-1], 16, "f32")
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = la.causal_attention(*leaves, cu_seqlens=cu)
+    dq, dk, dv = torch.autograd.grad(o, leaves, do)
+    # the bounds above with T = 1 and P = 1: the weight is exp(S - lse), whose argument is rounded, not 1 itself
+    nq, nk, nv, nd = (_np(t) for t in (q, k, v, do))
+    mag = 0.25 * (nq.abs() * nk.abs()).sum(-1, True)
+    EP = 2 * ((16 + 8) * UP * mag + 4 * U * (0.25 * (nq * nk).sum(-1, True)).abs()) + 17 * UP
+    _within(o, nv, (EP + 17 * UP) * nv.abs(), "o")
+    _within(dv, nd, (EP + 17 * UP) * nd.abs(), "dv")
+    # do . v - delta is the same sum twice: 2 (d + 8) 2^-23 abs(do) . abs(v) (< 40), times scale = 1/4 and abs(k), abs(q) (< 8)
+    assert float(dq.abs().max()) < 4.6e-4 and float(dk.abs().max()) < 4.6e-4
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_strides_and_broadcast_heads(dtype):
     q, k, v, do = _inputs(2, 4, 4, 90, 64, dtype)
@@ -276,6 +294,22 @@ def test_step(B, H, Hkv, S, d, lens, dtype):
         kc[b, :, n:] = float("nan")
         vc[b, :, n:] = float("nan")
     _check_step(q, k, v, kc, vc, lens)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("H,S,d,n", [(8, 70_000, 128, 69_999), (3, 70_000, 64, 2), (40, 20_000, 40, 17_003)])
+def test_step_in_many_shares(H, S, d, n, dtype):
+    """One key head and a long cache: hundreds of workgroups share the sequence, or find nothing of it."""
+    _check_step(*_step_inputs(1, H, 1, S, d, dtype), [n])
+
+
+def test_step_refuses_caches_that_share_memory():
+    q, k, v, kc, vc = _step_inputs(2, 4, 2, 20, 64, "bf16")
+    lengths = torch.zeros(2, dtype=torch.int32, device=DEV)
+    for a, b in ((kc, kc), (kc.as_strided(kc.shape, (0, 64 * 20, 64, 1)), vc), (kc, vc.as_strided(vc.shape, (64 * 40, 64 * 20, 8, 1))),
+                 (kc, vc.as_strided(vc.shape, (64 * 20, 64 * 20, 64, 1)))):
+        with pytest.raises(RuntimeError, match="memory"):
+            la.causal_attention_step(q, k, v, a, b, lengths)
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
