@@ -114,7 +114,7 @@ template <typename T, typename S, int TPR, int K, bool VEC> __global__ __launch_
   constexpr int VN = Vec16<T>::N, RPB = block_of(TPR) / TPR;
   __shared__ float red[2][16];
   const int li = threadIdx.x % TPR;
-  const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+  const int64_t row = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * RPB + threadIdx.x / TPR;
   if (row >= a.rows) return;  // whole waves: rows of one wave have no barrier
   const int64_t base = row * a.d;
   const T* x = static_cast<const T*>(a.x) + base;
@@ -377,7 +377,8 @@ int bwd_blocks(int64_t rows, const Plan& p) {
 }
 
 template <typename T, typename S, int TPR, int K> void launch(const Args& a, bool vec, bool bwd, int blocks, hipStream_t st) {
-  const dim3 g((unsigned)blocks), b(block_of(TPR));
+  const int wide = blocks < 1 << 22 ? blocks : 1 << 22;  // a launch takes 2^32 threads in one direction
+  const dim3 g((unsigned)wide, (unsigned)((blocks + wide - 1) / wide)), b(block_of(TPR));
   if (bwd) {
     if (vec) rmsnorm_residual_bwd_kernel<T, S, TPR, K, true><<<g, b, 0, st>>>(a);
     else rmsnorm_residual_bwd_kernel<T, S, TPR, K, false><<<g, b, 0, st>>>(a);
@@ -407,8 +408,8 @@ int run(const char* what, const lnx_rmsnorm_residual_args* q, bool bwd, hipStrea
   if (!bwd && q->rows > 0 && (!q->out || (q->z && !q->weight))) return lnx_set_error(LNX_ERR_NULL, "%s: out (and weight for z) is required", what);
   if (bwd && q->rows > 0 && (!q->d_x || (q->gate && !q->d_gate) || (q->d_z && !q->weight)))
     return lnx_set_error(LNX_ERR_NULL, "%s: d_x (d_gate with a gate, weight with d_z) is required", what);
-  if (params && (!q->workspace || q->workspace_bytes < lnx_rmsnorm_residual_bwd_workspace_bytes(q->rows, q->d, q->dtype)))
-    return lnx_set_error(LNX_ERR_WORKSPACE, "%s: the parameters' gradients need a workspace of %llu bytes", what,
+  if (params && (!q->workspace || reinterpret_cast<uintptr_t>(q->workspace) % 16 || q->workspace_bytes < lnx_rmsnorm_residual_bwd_workspace_bytes(q->rows, q->d, q->dtype)))
+    return lnx_set_error(LNX_ERR_WORKSPACE, "%s: the parameters' gradients need a 16-byte aligned workspace of %llu bytes", what,
                          (unsigned long long)lnx_rmsnorm_residual_bwd_workspace_bytes(q->rows, q->d, q->dtype));
   if (q->rows == 0 && !params) return LNX_OK;
   Args a{};

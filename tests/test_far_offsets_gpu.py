@@ -71,3 +71,31 @@ def test_a_result_of_more_than_2_31_elements():
     x[0, 7] = 1
     y, s = la.gated_linear_recurrence(x, g)
     assert bool((s == 1).all()) and bool((y[0, -3:] == 1).all()) and not bool(y[0, :7].any())
+    del x, g, y, s
+    x = torch.zeros(1, T, D, dtype=torch.bfloat16, device=DEV)
+    x[0, 7] = 1
+    x.requires_grad_()
+    g = torch.zeros(1, T, 1, dtype=torch.bfloat16, device=DEV).expand(1, T, D).requires_grad_()
+    y = la.gated_linear_recurrence(x, g)[0]
+    dy = torch.zeros_like(x)
+    dy[0, -2] = 1
+    dx, dg = torch.autograd.grad(y, (x, g), dy)
+    assert bool((dx[0, :-1] == 1).all()) and not bool(dx[0, -1].any())
+    assert bool((dg[0, 8:-1] == 1).all()) and not bool(dg[0, :8].any()) and not bool(dg[0, -1].any())
+
+
+def test_attention_of_more_than_2_31_elements():
+    H, d, lens = 17, 128, [128] * 8190 + [200]
+    cu = torch.tensor([0] + lens).cumsum(0).tolist()
+    T = cu[-1]
+    q, do = (torch.randn(1, H, T, d, device=DEV, dtype=torch.bfloat16) for _ in range(2))
+    k, v = (torch.randn(1, 1, T, d, device=DEV, dtype=torch.bfloat16) for _ in range(2))
+    assert q.numel() > 2 ** 31
+    outs = []
+    for lo in (0, cu[-2]):
+        leaves = [t[:, :, lo:].detach().requires_grad_() for t in (q, k, v)]
+        o = la.causal_attention(*leaves, cu_seqlens=cu if lo == 0 else None)
+        outs.append([t[:, :, -200:] for t in (o, *torch.autograd.grad(o, leaves, do[:, :, lo:]))])
+    # the same sums, of the lone sequence perhaps split between workgroups: both round operands and results to 2^-8 of themselves
+    for a, b in zip(*outs):
+        assert float((a.float() - b.float()).norm() / b.float().norm()) < 2 ** -6

@@ -169,6 +169,29 @@ def test_attention_step_refusals():
     assert lib.lnx_attn_step(step(B=0), None) == 0 and lib.lnx_attn_step_workspace_bytes(step(B=0)) == 0
 
 
+def test_more_than_a_launch_takes_is_refused():
+    lib = _lib.load()
+    a = _lib.LinrecArgs(B=1 << 24, T=1, D=64, x_stride_t=64, g_stride_t=64)
+    a.x = a.g = a.y = a.final_state = _ptr()
+    _refused(lib.lnx_linrec_fwd(a, None), -2, b"too many rows")
+    p = _ptr()
+    _refused(lib.lnx_linrec_step(p, p, p, p, p, (1 << 32) + 1, 0, 0, None), -2, b"too large")
+    _refused(lib.lnx_linrec_step(p, p, p, p, p, 1 << 36, 0, 0, None), -2, b"too large")
+    _refused(lib.lnx_attn_fwd(_attn(B=1 << 22, T=1), None), -2, b"too many rows")
+    s = _lib.AttnStepArgs(B=1 << 26, H=4, Hkv=4, S=8, d=64, dtype=_lib.LNX_BF16, scale=1.0)
+    for n in ("q", "k", "v", "k_cache", "v_cache"):
+        setattr(s, n, _lib.Tensor4(_ptr(), 4 * 64, 64, 64))
+    s.o = s.lengths = _ptr()
+    _refused(lib.lnx_attn_step(s, None), -2, b"too many rows")
+    a = _attn()
+    a.lse, a.workspace, a.workspace_bytes = _ptr(), _ptr(4), 1 << 20
+    _refused(lib.lnx_attn_bwd(a, None), -4, b"aligned")
+    n = _lib.RmsnormResidualArgs(rows=2, d=8)
+    n.x = n.d_x = n.d_weight = _ptr()
+    n.workspace, n.workspace_bytes = _ptr(4), 1 << 20
+    _refused(lib.lnx_rmsnorm_residual_bwd(n, None), -4, b"aligned")
+
+
 def test_tensors_off_the_gpu_are_refused():
     x, v = torch.zeros(1, 4, 8), torch.ones(8)
     h = torch.zeros(1, 2, 4, 8)

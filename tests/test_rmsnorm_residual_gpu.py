@@ -245,6 +245,19 @@ def test_repeats_bit_for_bit_and_replays():
         assert all(torch.equal(a, b) for a, b in zip(out, both()))
 
 
+def test_more_rows_than_one_direction_of_a_launch():
+    rows = 2 ** 26 + 5  # of 64 threads: more than 2^32
+    x = torch.zeros(rows, 8, dtype=torch.bfloat16, device=DEV)
+    x[-7:] = torch.randn(7, 8, generator=torch.Generator().manual_seed(5)).to(DEV, torch.bfloat16)
+    w = torch.ones(8, device=DEV)
+    leaves = [t.detach().requires_grad_() for t in (x, x[-7:])]
+    whole, few = (la.rmsnorm_residual(t, None, w) for t in leaves)
+    assert all(torch.equal(a[-7:], b) and not bool(a[:-7].any()) for a, b in zip(whole, few))
+    dz = torch.ones_like(whole[0])
+    dx, ds = torch.autograd.grad(whole[0], leaves[0], dz)[0], torch.autograd.grad(few[0], leaves[1], dz[-7:])[0]
+    assert torch.equal(dx[-7:], ds)
+
+
 def test_empty():
     w = torch.ones(32, device=DEV, requires_grad=True)
     x = torch.zeros(0, 32, device=DEV, requires_grad=True)
