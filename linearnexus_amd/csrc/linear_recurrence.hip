@@ -613,12 +613,14 @@ int64_t slots_of(const lnx_linrec_args* a, int64_t size) { return a->nseq ? a->T
 // channel tiles both forms move bytes at the same rate forwards and the walk is 13 % faster backwards ([8, 4096, 2048] bf16: 99 and
 // 99, 140 and 158 us); with 128 tiles of 1024 tokens the chained form is faster ([4, 1024, 2048]: 16.6 -> 14.7, 23.5 -> 19.4 us and a
 // clearing launch of 3), with 32 twice as fast (14.6 -> 9.0, 21 -> 10.3).
-// Packed rows are as long as the table on the device says, so every tile has a workgroup there from 1024 tokens on: of [1, 65536, 2048]
+// Packed rows are as long as the table on the device says, so every tile has a workgroup there from 8192 tokens on: of [1, 65536, 2048]
 // in 8 even rows the walk is 16 % faster (173 and 271 against 207 and 313 us), with all tokens in one of them four times as slow (811
 // and 1258 against 206 and 312); of 512 rows the walk takes 342 and 583 us, the chained form 188 and 307.
+// Of fewer than 8192 tokens no row is that long, and a clearing launch is what it would cost ([1, 5003, 1000] fp32 in 7 rows: 20.5 and
+// 29.9 us walked, 21.2 and 29.8 chained, 6.6 to clear).
 bool chained(const lnx_linrec_args* a) {
   const int64_t wgs = (int64_t)rows_of(a) * channel_tiles(a);
-  return a->T >= 8 * CTILE && (a->nseq || wgs < 160) && slots_of(a, CTILE) * channel_tiles(a) <= MAX_GRID / CTHREADS;
+  return a->T >= 8 * CTILE && (wgs < 160 || (a->nseq && a->T >= 64 * CTILE)) && slots_of(a, CTILE) * channel_tiles(a) <= MAX_GRID / CTHREADS;
 }
 // Bytes of what the workgroups leave for each other
 int64_t pair_words(const lnx_linrec_args* a) { return 2 * (slots_of(a, CTILE) + slots_of(a, CTILE * GROUP)) * a->D; }

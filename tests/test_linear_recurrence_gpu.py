@@ -148,11 +148,13 @@ def test_packed(lens, types):
     _check(*_inputs(1, cu[-1], 48, *types, rows=len(lens)), cu=cu)
 
 
-@pytest.mark.parametrize("kind", ["uneven", "short", "long"])
+@pytest.mark.parametrize("kind", ["uneven", "short", "long", "uneven more", "short more"])
 def test_packed_rows_of_every_kind(kind):
     """More rows than a wave looks at in one go, with empty ones; one row of more than 1024 tiles behind short ones."""
     r = np.random.default_rng(3)
-    lens = {"uneven": (r.integers(0, 5, 700) * (r.random(700) < 0.5)).tolist() + [2000, 0, 129, 0], "short": [1, 0, 2] * 1500, "long": [5, 0, 132_000, 0, 900]}[kind]
+    lens = {"uneven": (r.integers(0, 5, 700) * (r.random(700) < 0.5)).tolist() + [2000, 0, 129, 0], "short": [1, 0, 2] * 1500, "long": [5, 0, 132_000, 0, 900]}
+    lens |= {"uneven more": lens["uneven"] + [7000, 1, 0, 300], "short more": lens["short"] * 2}
+    lens = lens[kind]
     cu = np.concatenate([[0], np.cumsum(lens)]).tolist()
     _check(*_inputs(1, cu[-1], 3 if kind == "long" else 70, "bf16", "f32", rows=len(lens)), cu=cu)
 
