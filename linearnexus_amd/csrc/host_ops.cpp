@@ -94,6 +94,21 @@ std::string shape_text(const Tensor& t) {
   return s + (t.dim() == 1 ? ",)" : ")");
 }
 
+// A pass that is captured while an eager graph of one of its leaves is alive: the engine then takes that graph's stream for the leaf's
+// gradient, waits across streams, and the broken capture ends the process.  Refused before anything is launched.
+void refuse_live_graph(const char* op, std::initializer_list<const Tensor*> ts) {
+  bool any = false;
+  for (const Tensor* t : ts) any = any || (t->defined() && t->requires_grad());
+  if (!any || !capturing(**ts.begin())) return;
+  const c10::Stream now = c10::hip::getCurrentHIPStream((*ts.begin())->get_device()).unwrap();
+  for (const Tensor* t : ts) {
+    if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto stream = node ? node->stream() : std::nullopt;
+    TORCH_CHECK(!stream || *stream == now, op, ": a graph of this leaf from another stream is alive while this pass is captured; let go of its outputs first, or run it on the capturing stream");
+  }
+}
+
 // Tensors of one call lie on one GPU; a tensor that is absent is not asked.
 void check_devices(const char* op, const Tensor& first, std::initializer_list<std::pair<const char*, const Tensor*>> rest) {
   for (const auto& [name, t] : rest)
@@ -898,6 +913,7 @@ PyObject* py_rmsnorm_residual(PyObject*, PyObject* const* args, Py_ssize_t nargs
   refuse_tangents(op, {&x, &residual, &weight, &post, &gate, &scale_v});
   const auto r = without_lock([&]() -> std::pair<Tensor, Tensor> {
     if (wants_grad({&x, &residual, &weight, &post, &gate, &scale_v})) {
+      refuse_live_graph(op, {&x, &residual, &weight, &post, &gate, &scale_v});
       const variable_list r = AroundFn::apply(x, opt(residual), opt(weight), opt(post), opt(gate), opt(scale_v), scale, eps);
       return {r.size() > 1 ? r[1] : Tensor(), r[0]};
     }
@@ -1302,6 +1318,7 @@ struct RecFn : Function<RecFn> {
 
 std::pair<Tensor, Tensor> rec_scan(const RecShape& s, const Tensor& x, const Tensor& g, const Tensor& s0, const Tensor& cu) {
   if (wants_grad({&x, &g, &s0})) {
+    refuse_live_graph("gated_linear_recurrence", {&x, &g, &s0});
     const variable_list r = RecFn::apply(x, g, opt(s0), opt(cu), s);
     return {r[0], r[1]};
   }
@@ -1456,6 +1473,7 @@ PyObject* py_causal_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs
   TORCH_CHECK_VALUE(std::isfinite((float)scale), op, ": scale must be finite, got ", scale);
   return THPVariable_Wrap(without_lock([&] {
     const int64_t d = q.size(3), more = (8 - d % 8) % 8;  // zero columns change no product
+    if (wants_grad({&q, &k, &v})) refuse_live_graph(op, {&q, &k, &v});
     auto wide = [&](const Tensor& t) { return more ? at::constant_pad_nd(t, {0, more}) : t; };
     const Tensor qw = wide(q), kw = wide(k), vw = wide(v);
     const Tensor o = wants_grad({&q, &k, &v}) ? AttentionFn::apply(qw, kw, vw, opt(cu), scale) : attention_forward(as_rows(qw), as_rows(kw), as_rows(vw), cu, scale, Tensor(), Tensor());
