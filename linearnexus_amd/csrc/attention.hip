@@ -7,8 +7,11 @@
 // the products over the head dimension and through transposing reads for the products over the rows.  A score fragment holds one
 // column per lane and half, so maxima and sums are within the lane and one exchange of the wave's halves.
 // Tiles of 64 rows come in through loads that go straight to LDS, the next tile behind the one being multiplied, one barrier a tile.
-// bf16 takes v_mfma_f32_32x32x16_bf16 (probabilities and score gradients are rounded to bf16 as operands: 2^-9 of each term, what the
-// outputs are rounded to), fp32 takes v_mfma_f32_32x32x2_f32 throughout.  Sums, maxima and accumulators are fp32.
+// bf16 takes v_mfma_f32_32x32x16_bf16 (probabilities and score gradients are rounded to bf16 as operands: at most 2^-8 of each term, what
+// the outputs are rounded to), fp32 takes v_mfma_f32_32x32x2_f32 throughout.  Sums, maxima and accumulators are fp32.
+// Bound by the matrix cores and the exponentials beside them: at B2 H16/4 T4096 d128 bf16 the forward kernel takes 147-164 us (840-930
+// TFLOP/s of the causal half; matrix cores busy 41 %, vector instructions 41 % of the time), dq 194-217 (950-1060), dk / dv 311-343
+// (800-880) and the two sums of its parts 7 each, where a large library product reaches 1200.
 // No atomics: dk and dv are summed over the group's query heads by the workgroup that owns the keys, dq by a kernel of its own.
 #include "lnx_common.h"
 #include "mma_tiles.h"
@@ -312,7 +315,7 @@ template <typename T, int M> __device__ __forceinline__ void store_low(T* p, con
 }
 
 // Keys of a tile of the forward pass: with 32 three workgroups share a CU (registers, LDS) and less of the diagonal is wasted: eight packed
-// prompts of 8192 tokens 175 us with 64, 160 with 32; B2 H16/4 T4096 154 and 156.
+// prompts of 8192 tokens together 175 us with 64, 160 with 32; B2 H16/4 T4096 154 and 156.
 template <typename T, int D> constexpr int fwd_rows() { return sizeof(T) == 2 && D == 128 ? 32 : 64; }
 
 // A wave owns 32 queries, the workgroup 128; of a block's key tiles every a.parts-th.
@@ -620,8 +623,10 @@ template <typename T> __device__ __forceinline__ void take_frag(unsigned at, Fra
 
 // A workgroup owns 64 keys.  Wave (kw, qw) forms the weights of 32 keys and the half qw of a tile's queries, hands them to the wave of
 // the other half, and adds up the half qw of the columns of dk and dv over all queries: accumulators of half the size, so that two
-// workgroups share a CU (both halves in every wave took 416 registers, one workgroup a CU and 1.6 times as long).  The LDS of a
-// workgroup is 80 KB to the byte: the queries' lse and delta go straight to registers, a flag crosses in the hand-over's place.
+// workgroups share a CU.  (With both halves in every wave it took 416 registers and one workgroup a CU; as long, 456 and 469 us at B2 H16/4
+// T4096 d128, while the first keys' workgroups, which walk over all queries, were what the launch waited for.  Their queries split into
+// parts need the second workgroup: 317 us.)  The LDS of a workgroup is 80 KB to the byte: the queries' lse and delta go straight to
+// registers, a flag crosses in the hand-over's place.
 template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dkv_kernel(Args a) {
   typedef Tile<T, D> TL;
   typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
@@ -944,7 +949,8 @@ template <typename T> constexpr int step_waves() { return sizeof(T) == 2 ? 4 : 2
 // The queries that share a key head are the 32 columns, every wave walks over tiles of 32 cached tokens of its own: no barrier until
 // the waves' sums meet.  Bound by the bytes of the cache (the matrix products take a sixteenth of the time): the next tile is in
 // flight while one is multiplied.  The new token's key and value come from the call and are written to the cache by the wave whose
-// tile holds the place; what lies behind it is never read.
+// tile holds the place; what lies behind it is never read.  32 sequences of 6300 places on average, 8 key heads of 128: 152-161 us for 825
+// MB, 5.2-5.4 TB/s, and 5 us to join the shares.
 template <typename T, int D> __global__ __launch_bounds__(64 * step_waves<T>(), 1) void attn_step_kernel(StepArgs a) {
   constexpr int W = step_waves<T>();
   typedef Tile<T, D, SROWS> TL;

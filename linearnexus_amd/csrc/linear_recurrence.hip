@@ -1,7 +1,8 @@
 // Element-wise gated linear recurrence over [rows, T, D] tensors, dense or packed, forward, backward and one token:
 //   h_t = e^{g_t} h_{t-1} + x_t,  y_t = h_t                                    (h_0 the initial state, g log-decays)
 //   dh_t = dy_t + e^{g_{t+1}} dh_{t+1},  dx_t = dh_t,  dg_t = e^{g_t} h_{t-1} dh_t,  dh_0 = e^{g_1} dh_1
-// No products to speak of: every pass is bound by the bytes of its tensors.  A workgroup owns 128 bytes of channels of one row and walks
+// No products to speak of: every pass is bound by the bytes of its tensors ([8, 4096, 2048] bf16: forward 90-97 us for 403 MB, 4.2-4.5
+// TB/s, backward 131-135 for 671 MB, 5.0-5.1 TB/s; a copy reaches 4.97).  A workgroup owns 128 bytes of channels of one row and walks
 // its tokens in tiles: a thread holds four channels of R consecutive tokens and reduces them to a pair (A, H), the map h -> A h + H;
 // pairs are scanned over the token groups of a wave by lane swaps, and the eight waves' pairs are chained through LDS by one lane per
 // channel, which carries the state from tile to tile.  The loads of the next tile are in flight meanwhile.  (Eight channels of four
