@@ -798,13 +798,15 @@ int64_t blocks_of(const lnx_attn_args* a, int size) { return a->nseq ? (int64_t)
 // Into how many parts the rows that a block walks over are split.  In units of one tile's time in a workgroup: the launch takes as long
 // as its work spread over the chip or as its longest workgroup, whichever is more; a split adds to each workgroup the time that
 // its share of the result takes to be written and read in fp32 (`share`), and the joining launch.  Measured at bf16, d = 128: a tile
-// 1.5 us in a workgroup with another on its CU, a share of 64 KB 5 tiles, a launch 4.  `longest`: tiles of the longest block.
-int parts_for(int64_t wgs, int64_t longest, int slots, double share, double launch) {
+// 1.5 us in a workgroup with another on its CU, a share of 64 KB 5 tiles, a launch 4.  `longest`: tiles of the longest block; `most`: of
+// the queries' kernels eight parts (sixteen gave nothing at any shape), of the keys', whose blocks are as long as the group's queries, sixteen
+// (B1 H8/2 T1000 d128 fp32: eight 93 us, twelve 72).
+int parts_for(int64_t wgs, int64_t longest, int slots, int most, double share, double launch) {
   const double work = (double)wgs * (longest + 1) / 2 / slots;
   int best = 1;
   double least = 1e300;
-  for (int s = 1; s <= 8 && s <= longest; ++s) {
-    const double extra = s > 1 ? share : 0, spread = work + extra * s * (double)wgs / slots, one = (double)longest / s + extra;
+  for (int s = 1; s <= most && s <= longest; ++s) {
+    const double extra = s > 1 ? share : 0, spread = work + extra * s * (double)wgs / slots, one = (double)((longest + s - 1) / s) + extra;
     const double t = (spread > one ? spread : one) + (s > 1 ? launch : 0);
     if (t < least * 0.95) least = t, best = s;
   }
@@ -816,8 +818,9 @@ int parts_of(const lnx_attn_args* a, int kernel) {
   const bool bf16 = a->dtype == LNX_BF16;
   const double share = bf16 ? 5 : 1, launch = bf16 ? 4 : 1.5;
   const int64_t keys = (len + ROWS - 1) / ROWS, queries = (len + 127) / 128;
-  if (kernel == DKV) return parts_for(rows * a->Hkv * keys, keys * (a->H / a->Hkv), bf16 ? 512 : 256, share / 2, launch);
-  return parts_for(rows * a->H * queries, keys, bf16 ? 512 : 256, share, launch);
+  // workgroups that the chip holds at a time: two a CU, one where fp32 tiles take most of its LDS
+  if (kernel == DKV) return parts_for(rows * a->Hkv * keys, keys * (a->H / a->Hkv), bf16 ? 512 : 256, 16, share / 2, launch);
+  return parts_for(rows * a->H * queries, keys, bf16 || a->d <= 64 ? 512 : 256, 8, share, launch);
 }
 // Bytes of the workspaces: shares of the forward kernel; delta and the shares of either gradient kernel
 uint64_t fwd_bytes(const lnx_attn_args* a) {
