@@ -166,6 +166,12 @@ template <typename T, int D, int R = ROWS> struct Mover {
   }
 };
 __device__ __forceinline__ bool is_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
+// What the rounding of that operand left, as a second operand
+__device__ __forceinline__ void rest_of(Frag8<bf16_t>& f, const floatx16& c, int h, const Frag8<bf16_t>& rounded) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f.v[e] = from_f32<bf16_t>(is_finite(to_f32(rounded.v[e])) ? c[8 * h + e] - to_f32(rounded.v[e]) : 0.f);
+}
+__device__ __forceinline__ void rest_of(Frag8<float>&, const floatx16&, int, const Frag8<float>&) {}
 // Whether the granules that this lane's loads brought hold finite values only; SCRUB: the others become 0.  A wave's granules are
 // rows 16 wave .. 16 wave + 15.
 template <typename T, int D, bool SCRUB, int R = ROWS> __device__ __forceinline__ bool tile_finite(T* tile, int wave, int lane) {
@@ -319,7 +325,10 @@ template <typename T, int M> __device__ __forceinline__ void store_low(T* p, con
 template <typename T, int D> constexpr int fwd_rows() { return sizeof(T) == 2 && D == 128 ? 32 : 64; }
 
 // A wave owns 32 queries, the workgroup 128; of a block's key tiles every a.parts-th.
-template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 3 : 1) void attn_fwd_kernel(Args a) {
+// TWO (all three kernels): weights and score gradients enter the products in two bf16 parts.  For sequences of one tile on average: a
+// gradient there is a sum of a few terms, whose roundings (2^-8 each) do not average out: of three tokens dq and dk were 1.8 times as
+// far off as their own rounding leaves them, of 64 and more 1.4 times.
+template <typename T, int D, bool TWO> __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : TWO ? 2 : 3) void attn_fwd_kernel(Args a) {
   constexpr int KT = fwd_rows<T, D>(), KH = KT / 32;
   typedef Tile<T, D, KT> TL;
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -426,6 +435,14 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) mma(acc[i], TL::by_col(cols, TL::BYTES + 16 * s * TL::ROWB, i), pf[s]);
     read_ahead<T, true, 2 * KH * (D / 32), 4>();
+    if constexpr (TWO)
+#pragma unroll
+      for (int s = 0; s < 2 * KH; ++s) {
+        Frag8<T> rest;
+        rest_of(rest, sc[s >> 1], s & 1, pf[s]);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) mma(acc[i], TL::by_col(cols, TL::BYTES + 16 * s * TL::ROWB, i), rest);
+      }
     if (edge && odd[buf])
 #pragma unroll
       for (int i = 0; i < KH; ++i) {
@@ -501,7 +518,7 @@ template <typename T> __global__ __launch_bounds__(256) void attn_sum_kernel(con
 // Queries as in the forward pass, their gradients beside them in registers.  delta is formed here, for the dk / dv kernel too: of o and
 // what its rounding left, because an error of delta goes into every term of a row of dq (rounded o alone: 1.5 times the error that the
 // rounding of dq has, with it 1.4).
-template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(Args a) {
+template <typename T, int D, bool TWO> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(Args a) {
   typedef Tile<T, D> TL;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const auto kt = [](int buf) { return reinterpret_cast<T*>(lds + 2 * buf * TL::BYTES); };
@@ -566,7 +583,7 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const bool mine = key0 + 32 * i <= q0 + 31;  // not behind all of this wave's queries
-      Frag8<T> ds[2];
+      Frag8<T> ds[2], rest[2];
       if (mine) {
         floatx16 sc, dp;
 #pragma unroll
@@ -587,6 +604,7 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
             if (key0 + 32 * i + frag_row(e, lane) > q) sc[e] = 0.f;
         from_acc(ds[0], sc, 0);
         from_acc(ds[1], sc, 1);
+        if constexpr (TWO) rest_of(rest[0], sc, 0, ds[0]), rest_of(rest[1], sc, 1, ds[1]);
       }
       if (scrub) {  // the scores are made of the keys as they are
         lds_barrier();
@@ -599,6 +617,11 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
 #pragma unroll
           for (int m = 0; m < D / 32; ++m) mma(acc[m], TL::by_col(cols, (32 * i + 16 * s) * TL::ROWB, m), ds[s]);
         read_ahead<T, true, 2 * (D / 32), 4>();
+        if constexpr (TWO)
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int m = 0; m < D / 32; ++m) mma(acc[m], TL::by_col(cols, (32 * i + 16 * s) * TL::ROWB, m), rest[s]);
         if (scrub) add_odd<T, D / 32>(acc, kb, a.ks[2], key0 + 32 * i, p.len, a.d, ds, lane, [&](int row) { return row <= q; });
       }
     }
@@ -621,16 +644,18 @@ template <typename T> __device__ __forceinline__ void take_frag(unsigned at, Fra
   for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = lds_load<floatx4>(at + 1024 * i + 16 * lane);
 }
 
+template <typename T, bool TWO> constexpr int hand_over() { return (TWO ? 16384 : 8192) * (int)sizeof(T); }  // bytes of a workgroup
+
 // A workgroup owns 64 keys.  Wave (kw, qw) forms the weights of 32 keys and the half qw of a tile's queries, hands them to the wave of
 // the other half, and adds up the half qw of the columns of dk and dv over all queries: accumulators of half the size, so that two
 // workgroups share a CU.  (With both halves in every wave it took 416 registers and one workgroup a CU; as long, 456 and 469 us at B2 H16/4
 // T4096 d128, while the first keys' workgroups, which walk over all queries, were what the launch waited for.  Their queries split into
 // parts need the second workgroup: 317 us.)  The LDS of a workgroup is 80 KB to the byte: the queries' lse and delta go straight to
 // registers, a flag crosses in the hand-over's place.
-template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dkv_kernel(Args a) {
+template <typename T, int D, bool TWO> __global__ __launch_bounds__(256, sizeof(T) == 2 && !TWO ? 2 : 1) void attn_dkv_kernel(Args a) {
   typedef Tile<T, D> TL;
   typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
-  constexpr int M = D / 64, FRAG = 1024 * (int)sizeof(T) / 2;
+  constexpr int M = D / 64, FRAG = 1024 * (int)sizeof(T) / 2, HAND = hand_over<T, TWO>() / 4;  // bytes that a wave hands over
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const auto qt = [](int buf) { return reinterpret_cast<T*>(lds + 2 * buf * TL::BYTES); };
   const auto gt = [](int buf) { return reinterpret_cast<T*>(lds + (2 * buf + 1) * TL::BYTES); };
@@ -644,7 +669,7 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
     lds_barrier();
   }
   const Mover<T, D> mq(a.qs[2], a.d, wave, lane), mg(a.gs[2], a.d, wave, lane);
-  const unsigned lds0 = lds_byte_addr(lds), mine = lds0 + 4 * TL::BYTES + 4 * FRAG * wave, theirs = lds0 + 4 * TL::BYTES + 4 * FRAG * (wave ^ 2);
+  const unsigned lds0 = lds_byte_addr(lds), mine = lds0 + 4 * TL::BYTES + HAND * wave, theirs = lds0 + 4 * TL::BYTES + HAND * (wave ^ 2);
   floatx4 lse[4], delta[4];
   auto fetch_stats = [&](int h, int row0) {
     const int64_t first = ((int64_t)p.b * a.H + h) * a.T + p.tok;
@@ -708,14 +733,14 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
       if (lane == 0) *(lds_int*)(lds_char*)(uintptr_t)mine = !all;
       lds_barrier();
 #pragma unroll
-      for (int w = 0; w < 4; ++w) scrub = scrub || lds_load<int>(lds0 + 4 * TL::BYTES + 4 * FRAG * w) != 0;
+      for (int w = 0; w < 4; ++w) scrub = scrub || lds_load<int>(lds0 + 4 * TL::BYTES + HAND * w) != 0;
       scrub = __builtin_amdgcn_readfirstlane(scrub);
       lds_barrier();
     }
     if (it + a.parts < total) fetch(next_h, next_row0, buf ^ 1);
     const unsigned rows = row_addr + 2 * buf * TL::BYTES, cols = col_addr + 2 * buf * TL::BYTES;
     const auto active = [&](int q) { return row0 + 32 * q + 31 >= key0 && row0 + 32 * q < p.len; };  // some of these queries come after some of the keys
-    Frag8<T> pf[2], ds[2];
+    Frag8<T> pf[2], ds[2], pr[2], dr[2];
     if (active(qw)) {
       floatx16 sc, dp;
 #pragma unroll
@@ -744,6 +769,12 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
         from_acc(ds[s], dp, s);
         leave_frag<T>(mine + s * FRAG, pf[s], lane);
         leave_frag<T>(mine + (2 + s) * FRAG, ds[s], lane);
+        if constexpr (TWO) {
+          rest_of(pr[s], sc, s, pf[s]);
+          rest_of(dr[s], dp, s, ds[s]);
+          leave_frag<T>(mine + (4 + s) * FRAG, pr[s], lane);
+          leave_frag<T>(mine + (6 + s) * FRAG, dr[s], lane);
+        }
       }
     }
     if (it + a.parts < total) fetch_stats(next_h, next_row0);
@@ -763,6 +794,14 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
           mma(dk[m], TL::by_col(from, 16 * s * TL::ROWB, m), ds[s]);
         }
       read_ahead<T, true, 4 * M, 4>();
+      if constexpr (TWO)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int m = 0; m < M; ++m) {
+            mma(dv[m], TL::by_col(from, TL::BYTES + 16 * s * TL::ROWB, m), pr[s]);
+            mma(dk[m], TL::by_col(from, 16 * s * TL::ROWB, m), dr[s]);
+          }
       if (scrub) {
         const auto keep = [&](int row) { return row >= key; };
         add_odd<T, M>(dv, at<T>(a.dout, a.gs, p.b, h, p.tok) + 32 * M * qw, a.gs[2], row0 + 32 * half, p.len, a.d - 32 * M * qw, pf, lane, keep);
@@ -775,6 +814,10 @@ template <typename T, int D> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 
       for (int s = 0; s < 2; ++s) {
         take_frag<T>(theirs + s * FRAG, pf[s], lane);
         take_frag<T>(theirs + (2 + s) * FRAG, ds[s], lane);
+        if constexpr (TWO) {
+          take_frag<T>(theirs + (4 + s) * FRAG, pr[s], lane);
+          take_frag<T>(theirs + (6 + s) * FRAG, dr[s], lane);
+        }
       }
       add(qw ^ 1);
     }
@@ -812,9 +855,10 @@ int parts_for(int64_t wgs, int64_t longest, int slots, int most, double share, d
   }
   return best;
 }
+int64_t average_length(const lnx_attn_args* a) { return a->nseq ? ((int64_t)a->T + a->nseq - 1) / a->nseq : a->T; }
 enum { QUERIES, DKV };  // the forward and the dq kernel, whose blocks are queries; the dk / dv kernel
 int parts_of(const lnx_attn_args* a, int kernel) {
-  const int64_t len = a->nseq ? (a->T + a->nseq - 1) / a->nseq : a->T, rows = a->nseq ? a->nseq : a->B;  // sequences of the average length
+  const int64_t len = average_length(a), rows = a->nseq ? a->nseq : a->B;  // sequences of the average length
   const bool bf16 = a->dtype == LNX_BF16;
   const double share = bf16 ? 5 : 1, launch = bf16 ? 4 : 1.5;
   const int64_t keys = (len + ROWS - 1) / ROWS, queries = (len + 127) / 128;
@@ -880,12 +924,12 @@ template <typename K> int start(K kernel, const char* name, const Args& a, int64
   return LNX_OK;
 }
 
-template <typename T, int D> int launch_fwd(const lnx_attn_args* a, hipStream_t st) {
+template <typename T, int D, bool TWO> int launch_fwd(const lnx_attn_args* a, hipStream_t st) {
   Args k = kernel_args(a);
   k.nblk = (int)blocks_of(a, 128), k.parts = parts_of(a, QUERIES);
   const int64_t rows = (int64_t)k.B * k.H * k.T;
   k.part = static_cast<float*>(a->workspace), k.part_stat = k.part ? k.part + k.parts * rows * k.d : nullptr;
-  if (int rc = start(attn_fwd_kernel<T, D>, "attn_fwd", k, (int64_t)k.B * k.H * k.nblk * k.parts, 4 * Tile<T, D, fwd_rows<T, D>()>::BYTES + 16, st)) return rc;
+  if (int rc = start(attn_fwd_kernel<T, D, TWO>, "attn_fwd", k, (int64_t)k.B * k.H * k.nblk * k.parts, 4 * Tile<T, D, fwd_rows<T, D>()>::BYTES + 16, st)) return rc;
   if (k.parts > 1) {
     lnx_profile_mark("attn_join", st);
     attn_join_kernel<T><<<dim3((unsigned)((rows + 15) / 16)), 256, 0, st>>>(k);
@@ -898,15 +942,15 @@ template <typename T> void sum_parts(const Args& k, const float* part, int64_t s
   attn_sum_kernel<T><<<dim3((unsigned)(((int64_t)k.B * heads * k.T + 15) / 16)), 256, 0, st>>>(part, k.parts, stride, static_cast<T*>(out), s[0], s[1], s[2], k.B, heads, k.T, k.d);
 }
 
-template <typename T, int D> int launch_bwd(const lnx_attn_args* a, hipStream_t st) {
+template <typename T, int D, bool TWO> int launch_bwd(const lnx_attn_args* a, hipStream_t st) {
   Args k = kernel_args(a);
   k.delta = static_cast<float*>(a->workspace);
   k.part = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + delta_bytes(a));
   k.nblk = (int)blocks_of(a, 128), k.parts = parts_of(a, QUERIES);  // first: it leaves delta
-  if (int rc = start(attn_dq_kernel<T, D>, "attn_dq", k, (int64_t)k.B * k.H * k.nblk * k.parts, 4 * Tile<T, D>::BYTES + 16, st)) return rc;
+  if (int rc = start(attn_dq_kernel<T, D, TWO>, "attn_dq", k, (int64_t)k.B * k.H * k.nblk * k.parts, 4 * Tile<T, D>::BYTES + 16, st)) return rc;
   if (k.parts > 1) sum_parts<T>(k, k.part, (int64_t)k.B * k.H * k.T, k.dq, k.dqs, k.H, st);
   k.nblk = (int)blocks_of(a, ROWS), k.parts = parts_of(a, DKV);
-  if (int rc = start(attn_dkv_kernel<T, D>, "attn_dkv", k, (int64_t)k.B * k.Hkv * k.nblk * k.parts, 4 * Tile<T, D>::BYTES + 8192 * sizeof(T), st)) return rc;
+  if (int rc = start(attn_dkv_kernel<T, D, TWO>, "attn_dkv", k, (int64_t)k.B * k.Hkv * k.nblk * k.parts, 4 * Tile<T, D>::BYTES + hand_over<T, TWO>(), st)) return rc;
   if (k.parts > 1) {
     const int64_t rows = (int64_t)k.B * k.Hkv * k.T;
     sum_parts<T>(k, k.part, 2 * rows, k.dk, k.dks, k.Hkv, st);
@@ -915,16 +959,17 @@ template <typename T, int D> int launch_bwd(const lnx_attn_args* a, hipStream_t 
   return LNX_OK;
 }
 
+template <typename T, int D, bool TWO> int launch(const lnx_attn_args* a, bool bwd, hipStream_t st) { return bwd ? launch_bwd<T, D, TWO>(a, st) : launch_fwd<T, D, TWO>(a, st); }
+
 int run(const char* what, const lnx_attn_args* a, bool bwd, hipStream_t st) {
   if (int rc = check(what, a, bwd)) return rc;
   if (a->B == 0 || a->T == 0) return LNX_OK;
   int rc;
   if (a->dtype == LNX_BF16) {
-    if (a->d <= 64) rc = bwd ? launch_bwd<bf16_t, 64>(a, st) : launch_fwd<bf16_t, 64>(a, st);
-    else rc = bwd ? launch_bwd<bf16_t, 128>(a, st) : launch_fwd<bf16_t, 128>(a, st);
+    if (average_length(a) <= ROWS) rc = a->d <= 64 ? launch<bf16_t, 64, true>(a, bwd, st) : launch<bf16_t, 128, true>(a, bwd, st);
+    else rc = a->d <= 64 ? launch<bf16_t, 64, false>(a, bwd, st) : launch<bf16_t, 128, false>(a, bwd, st);
   } else {
-    if (a->d <= 64) rc = bwd ? launch_bwd<float, 64>(a, st) : launch_fwd<float, 64>(a, st);
-    else rc = bwd ? launch_bwd<float, 128>(a, st) : launch_fwd<float, 128>(a, st);
+    rc = a->d <= 64 ? launch<float, 64, false>(a, bwd, st) : launch<float, 128, false>(a, bwd, st);
   }
   if (rc) return rc;
   lnx_profile_mark(nullptr, st);

@@ -72,7 +72,7 @@ def _inputs(B, H, Hkv, T, d, dtype, token_first=False, seed=0):
     return n(H, 1.5), n(Hkv), n(Hkv), n(H)
 
 
-def _check(q, k, v, do, scale=None, cu=None):
+def _check(q, k, v, do, scale=None, cu=None, r=None):
     B, H, T, d = q.shape
     G = H // k.shape[1]
     leaves = [t.detach().requires_grad_() for t in (q, k, v)]
@@ -82,7 +82,8 @@ def _check(q, k, v, do, scale=None, cu=None):
         assert torch.equal(la.causal_attention(q, k, v, scale, cu_seqlens=cu), o)
     dq, dk, dv = torch.autograd.grad(o, leaves, do)
     s = d ** -0.5 if scale is None else scale
-    r = 2.0 ** -8 if q.dtype == torch.bfloat16 else 0.0
+    if r is None:
+        r = 2.0 ** -8 if q.dtype == torch.bfloat16 else 0.0
     spans = [(0, T)] if cu is None else list(zip(cu[:-1], cu[1:]))
     nq, nk, nv, nd = (_np(t) for t in (q, k, v, do))
     for b in range(B):
@@ -121,6 +122,14 @@ def test_packed(lens, H, Hkv, d, dtype):
 def test_many_short_sequences():
     cu = list(range(0, 3 * 150 + 1, 3))  # more than a wave of sequences
     _check(*_inputs(1, 2, 1, 450, 64, "bf16"), cu=cu)
+
+
+@pytest.mark.parametrize("lens,H,Hkv,d", [([1], 2, 1, 64), ([2], 8, 4, 64), ([3], 8, 4, 64), ([7], 2, 2, 128), ([64], 2, 1, 128), ([3, 1, 90, 0, 5], 4, 2, 80)], ids=str)
+def test_short_sequences_are_as_exact_as_their_rounding(lens, H, Hkv, d):
+    """With one tile of keys on average operands go in in two bfloat16 parts: each rounding of 2^-8 is one of 2^-16.  o and what its rounding
+    left are bfloat16 each, so delta's is 2^-16, too."""
+    cu = np.concatenate([[0], np.cumsum(lens)]).tolist()
+    _check(*_inputs(1, H, Hkv, cu[-1], d, "bf16"), cu=cu, r=2.0 ** -16)
 
 
 def test_more_sequences_than_a_wave_looks_at():
