@@ -31,11 +31,17 @@ struct Args {
   float scale, eps, inv_d;
 };
 
-// VN elements of a row as fp32; `left` of them exist
-template <typename E, int VN, bool VEC> __device__ __forceinline__ void load_row(const E* p, int left, float* f) {
-  if constexpr (!VEC) {
+// The VN elements of a row that a thread holds: consecutive ones as 16-byte vectors (ES = 1), or, where widths or pointers do not allow
+// that, ES = threads of the row apart, one at a time, so that a wave's loads are still whole lines (consecutive ones a lane touched every line
+// VN times: 6435 rows of 4475, bf16 with an fp32 stream and a gate, forward 247 us, this way 128;
+// 8751 rows of 3834 in fp32, backward 332 and 224).
+template <int TPR, int VN, int ES> __device__ __forceinline__ int first_column(int k, int li) { return ES == 1 ? (k * TPR + li) * VN : k * TPR * VN + li; }
+
+// VN elements of a row as fp32; those less than `left` from the first exist
+template <typename E, int VN, int ES> __device__ __forceinline__ void load_row(const E* p, int left, float* f) {
+  if constexpr (ES > 1) {
 #pragma unroll
-    for (int e = 0; e < VN; ++e) f[e] = e < left ? to_f32(p[e]) : 0.f;
+    for (int e = 0; e < VN; ++e) f[e] = e * ES < left ? to_f32(p[e * ES]) : 0.f;
   } else if constexpr (VN == Vec16<E>::N) {
     const typename Vec16<E>::V v = *reinterpret_cast<const typename Vec16<E>::V*>(p);
 #pragma unroll
@@ -47,11 +53,11 @@ template <typename E, int VN, bool VEC> __device__ __forceinline__ void load_row
   }
 }
 
-template <typename E, int VN, bool VEC> __device__ __forceinline__ void store_row(E* p, int left, const float* f) {
-  if constexpr (!VEC) {
+template <typename E, int VN, int ES> __device__ __forceinline__ void store_row(E* p, int left, const float* f) {
+  if constexpr (ES > 1) {
 #pragma unroll
     for (int e = 0; e < VN; ++e)
-      if (e < left) p[e] = from_f32<E>(f[e]);
+      if (e * ES < left) p[e * ES] = from_f32<E>(f[e]);
   } else if constexpr (VN == Vec16<E>::N) {
     typename Vec16<E>::V v;
 #pragma unroll
@@ -64,19 +70,19 @@ template <typename E, int VN, bool VEC> __device__ __forceinline__ void store_ro
 }
 
 // The same as it lies in memory, for a row that is fetched ahead of its use
-template <typename E, int VN, bool VEC> struct RawRow {
+template <typename E, int VN, int ES> struct RawRow {
   static constexpr int N = Vec16<E>::N;
   typename Vec16<E>::V v[VN / N];
   __device__ __forceinline__ void load(const E* p, int left) {
 #pragma unroll
     for (int k = 0; k < VN / N; ++k) {
       v[k] = vec_zero<E>();
-      if constexpr (VEC) {
+      if constexpr (ES == 1) {
         if (left > 0) v[k] = *reinterpret_cast<const typename Vec16<E>::V*>(p + k * N);
       } else {
 #pragma unroll
         for (int e = 0; e < N; ++e)
-          if (k * N + e < left) v[k][e] = p[k * N + e];
+          if ((k * N + e) * ES < left) v[k][e] = p[(k * N + e) * ES];
       }
     }
   }
@@ -113,7 +119,7 @@ template <int TPR> __device__ __forceinline__ void row_sum2(float& x, float& y, 
 constexpr int block_of(int tpr) { return tpr < 256 ? 256 : tpr; }
 
 template <typename T, typename S, int TPR, int K, bool VEC> __global__ __launch_bounds__(block_of(TPR)) void rmsnorm_residual_fwd_kernel(Args a) {
-  constexpr int VN = Vec16<T>::N, RPB = block_of(TPR) / TPR;
+  constexpr int VN = Vec16<T>::N, RPB = block_of(TPR) / TPR, ES = VEC ? 1 : TPR;
   __shared__ float red[2][16];
   const int li = threadIdx.x % TPR;
   const int64_t row = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * RPB + threadIdx.x / TPR;
@@ -125,13 +131,13 @@ template <typename T, typename S, int TPR, int K, bool VEC> __global__ __launch_
   float xv[K][VN], rv[K][VN], gv[K][VN], ss = 0.f;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int c = (k * TPR + li) * VN, left = a.d - c;
+    const int c = first_column<TPR, VN, ES>(k, li), left = a.d - c;
 #pragma unroll
     for (int e = 0; e < VN; ++e) xv[k][e] = rv[k][e] = gv[k][e] = 0.f;
     if (left > 0) {
-      load_row<T, VN, VEC>(x + c, left, xv[k]);
-      if (r) load_row<S, VN, VEC>(r + c, left, rv[k]);
-      if (gate) load_row<T, VN, VEC>(gate + c, left, gv[k]);
+      load_row<T, VN, ES>(x + c, left, xv[k]);
+      if (r) load_row<S, VN, ES>(r + c, left, rv[k]);
+      if (gate) load_row<T, VN, ES>(gate + c, left, gv[k]);
     }
   }
   float rho = 1.f;
@@ -145,13 +151,13 @@ template <typename T, typename S, int TPR, int K, bool VEC> __global__ __launch_
   ss = 0.f;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int c = (k * TPR + li) * VN, left = a.d - c;
+    const int c = first_column<TPR, VN, ES>(k, li), left = a.d - c;
     if (left > 0) {
       float pv[VN], sv[VN];
 #pragma unroll
       for (int e = 0; e < VN; ++e) pv[e] = 1.f, sv[e] = a.scale;
-      if (a.post) load_row<float, VN, VEC>(a.post + c, left, pv);
-      if (a.scale_v) load_row<float, VN, VEC>(a.scale_v + c, left, sv);
+      if (a.post) load_row<float, VN, ES>(a.post + c, left, pv);
+      if (a.scale_v) load_row<float, VN, ES>(a.scale_v + c, left, sv);
 #pragma unroll
       for (int e = 0; e < VN; ++e) {
         float u = xv[k][e] * rho * (pv[e] * sv[e]);
@@ -159,53 +165,53 @@ template <typename T, typename S, int TPR, int K, bool VEC> __global__ __launch_
         rv[k][e] += u;
         ss += rv[k][e] * rv[k][e];
       }
-      if (a.out) store_row<S, VN, VEC>(static_cast<S*>(a.out) + base + c, left, rv[k]);
+      if (a.out) store_row<S, VN, ES>(static_cast<S*>(a.out) + base + c, left, rv[k]);
     }
   }
   if (!a.z) return;
   const float rho2 = rsqrtf(row_sum<TPR>(ss, red[1]) * a.inv_d + a.eps);
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int c = (k * TPR + li) * VN, left = a.d - c;
+    const int c = first_column<TPR, VN, ES>(k, li), left = a.d - c;
     if (left > 0) {
       float wv[VN], zv[VN];
-      load_row<float, VN, VEC>(a.w + c, left, wv);
+      load_row<float, VN, ES>(a.w + c, left, wv);
 #pragma unroll
       for (int e = 0; e < VN; ++e) zv[e] = rv[k][e] * rho2 * wv[e];
-      store_row<T, VN, VEC>(static_cast<T*>(a.z) + base + c, left, zv);
+      store_row<T, VN, ES>(static_cast<T*>(a.z) + base + c, left, zv);
     }
   }
 }
 
 // Rows blockIdx, blockIdx + gridDim, ...; the next row is on its way while one is worked on.
 template <typename T, typename S, int TPR, int K, bool VEC> __global__ __launch_bounds__(block_of(TPR)) void rmsnorm_residual_bwd_kernel(Args a) {
-  constexpr int VN = Vec16<T>::N, RPB = block_of(TPR) / TPR, C = TPR * K * VN;
+  constexpr int VN = Vec16<T>::N, RPB = block_of(TPR) / TPR, C = TPR * K * VN, ES = VEC ? 1 : TPR;
   __shared__ float red[2][3][32];
   const int li = threadIdx.x % TPR, sub = threadIdx.x / TPR;
   float wv[K][VN], cp[K][VN], dw[K][VN], db[K][VN];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int c = (k * TPR + li) * VN, left = a.d - c;
+    const int c = first_column<TPR, VN, ES>(k, li), left = a.d - c;
 #pragma unroll
     for (int e = 0; e < VN; ++e) wv[k][e] = dw[k][e] = db[k][e] = 0.f, cp[k][e] = a.scale;
     if (left > 0) {
       float t[VN];
-      if (a.w) load_row<float, VN, VEC>(a.w + c, left, wv[k]);
-      if (a.scale_v) load_row<float, VN, VEC>(a.scale_v + c, left, cp[k]);
+      if (a.w) load_row<float, VN, ES>(a.w + c, left, wv[k]);
+      if (a.scale_v) load_row<float, VN, ES>(a.scale_v + c, left, cp[k]);
       if (a.post) {
-        load_row<float, VN, VEC>(a.post + c, left, t);
+        load_row<float, VN, ES>(a.post + c, left, t);
 #pragma unroll
         for (int e = 0; e < VN; ++e) cp[k][e] *= t[e];
       }
     }
   }
-  RawRow<T, VN, VEC> xr[K], gr[K], zr[K];
-  RawRow<S, VN, VEC> rr[K], orr[K];
+  RawRow<T, VN, ES> xr[K], gr[K], zr[K];
+  RawRow<S, VN, ES> rr[K], orr[K];
   auto fetch = [&](int64_t row) {
     const int64_t base = row * a.d;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int c = (k * TPR + li) * VN, left = row < a.rows ? a.d - c : 0;
+      const int c = first_column<TPR, VN, ES>(k, li), left = row < a.rows ? a.d - c : 0;
       const int64_t at = base + c;
       xr[k].load(static_cast<const T*>(a.x) + at, left);
       if (a.r) rr[k].load(static_cast<const S*>(a.r) + at, left);
@@ -263,8 +269,8 @@ template <typename T, typename S, int TPR, int K, bool VEC> __global__ __launch_
     dot = 0.f;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int c = (k * TPR + li) * VN, left = a.d - c;
-      if (a.dr && left > 0) store_row<S, VN, VEC>(static_cast<S*>(a.dr) + base + c, left, ov[k]);
+      const int c = first_column<TPR, VN, ES>(k, li), left = a.d - c;
+      if (a.dr && left > 0) store_row<S, VN, ES>(static_cast<S*>(a.dr) + base + c, left, ov[k]);
       float dg[VN];
 #pragma unroll
       for (int e = 0; e < VN; ++e) {
@@ -274,16 +280,16 @@ template <typename T, typename S, int TPR, int K, bool VEC> __global__ __launch_
         dg[e] = ov[k][e] * xn * (1.f - sg[k][e]);
         dot += ov[k][e] * xv[k][e];
       }
-      if (a.dgate && left > 0) store_row<T, VN, VEC>(static_cast<T*>(a.dgate) + base + c, left, dg);
+      if (a.dgate && left > 0) store_row<T, VN, ES>(static_cast<T*>(a.dgate) + base + c, left, dg);
     }
     float m = 0.f;
     if (a.post) m = row_sum<TPR>(dot, red[turn][2]) * a.inv_d * rho * rho;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int c = (k * TPR + li) * VN, left = a.d - c;
+      const int c = first_column<TPR, VN, ES>(k, li), left = a.d - c;
 #pragma unroll
       for (int e = 0; e < VN; ++e) ov[k][e] = rho * (ov[k][e] - xv[k][e] * m);
-      if (left > 0) store_row<T, VN, VEC>(static_cast<T*>(a.dx) + base + c, left, ov[k]);
+      if (left > 0) store_row<T, VN, ES>(static_cast<T*>(a.dx) + base + c, left, ov[k]);
     }
   }
   if (!a.dw) return;
@@ -315,9 +321,13 @@ template <typename T, typename S, int TPR, int K, bool VEC> __global__ __launch_
 #pragma unroll
   for (int k = 0; k < K; ++k)
 #pragma unroll
-    for (int e = 0; e < VN; e += 4) {
-      const int c = (k * TPR + li) * VN + e;
-      if (c < a.dpad) {
+    for (int e = 0; e < VN; e += VEC ? 4 : 1) {
+      const int c = first_column<TPR, VN, ES>(k, li) + e * ES;
+      if (c >= a.dpad) continue;
+      if constexpr (!VEC) {
+        part[c] = dw[k][e];
+        part[a.dpad + c] = db[k][e];
+      } else {
         store4(part + c, floatx4{dw[k][e], dw[k][e + 1], dw[k][e + 2], dw[k][e + 3]});
         store4(part + a.dpad + c, floatx4{db[k][e], db[k][e + 1], db[k][e + 2], db[k][e + 3]});
       }
