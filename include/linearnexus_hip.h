@@ -438,7 +438,8 @@ int lnx_linrec_step(const void* x, const void* g, const float* state, void* y, f
  * scale_vector [d] takes the place of `scale`.  x, gate, z and their gradients in `dtype`, residual, out and theirs in
  * `r_dtype` (LNX_F32 or `dtype`), weights and their gradients fp32.  z is the norm of the unrounded sum.  The backward call
  * reads the forward call's inputs; d_z and d_out may be NULL (zeros), d_residual, d_weight, d_post_weight and d_scale (the
- * vector's) may be NULL (not wanted); the last three are summed without atomics through the workspace.
+ * vector's) may be NULL (not wanted); the last three are summed without atomics through the workspace
+ * (16-byte aligned, like the workspaces below).
  */
 typedef struct lnx_rmsnorm_residual_args {
   int64_t rows;
@@ -503,6 +504,7 @@ int lnx_attn_bwd(const lnx_attn_args* a, void* hip_stream);
  * k_cache, v_cache [B, Hkv, S, d], and its queries attend to places 0 .. lengths[b].  q [B, H, d], k, v [B, Hkv, d] (stride_t
  * unused), caches with their own strides, o [B, H, d] dense; lengths [B] int32 on the device, left as it is.  Places behind the
  * token are not read.  A length outside 0 .. S - 1 writes nothing and gives NaN.  The workspace holds nothing between calls.
+ * Caches whose rows share memory are the caller's error: several workgroups write and read them at a time.
  */
 typedef struct lnx_attn_step_args {
   int32_t B, H, Hkv, S, d, dtype;
