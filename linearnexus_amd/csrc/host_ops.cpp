@@ -94,18 +94,19 @@ std::string shape_text(const Tensor& t) {
   return s + (t.dim() == 1 ? ",)" : ")");
 }
 
-// A pass that is captured while an eager graph of one of its leaves is alive: the engine then takes that graph's stream for the leaf's
-// gradient, waits across streams, and the broken capture ends the process.  Refused before anything is launched.
+// A pass that is captured while a graph of one of its leaves from the default stream is alive: the engine then takes that stream for the
+// leaf's gradient, which cannot join a capture, and the broken capture ends the process.  Refused before anything is launched.  (Another
+// stream forks from the capture and joins it again: warm-up passes on a side stream whose outputs are still held are fine.)
 void refuse_live_graph(const char* op, std::initializer_list<const Tensor*> ts) {
   bool any = false;
   for (const Tensor* t : ts) any = any || (t->defined() && t->requires_grad());
   if (!any || !capturing(**ts.begin())) return;
-  const c10::Stream now = c10::hip::getCurrentHIPStream((*ts.begin())->get_device()).unwrap();
+  const c10::StreamId eager = c10::hip::getDefaultHIPStream((*ts.begin())->get_device()).id();  // ids: the engine's streams carry another device type
   for (const Tensor* t : ts) {
     if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
     const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
     const auto stream = node ? node->stream() : std::nullopt;
-    TORCH_CHECK(!stream || *stream == now, op, ": a graph of this leaf from another stream is alive while this pass is captured; let go of its outputs first, or run it on the capturing stream");
+    TORCH_CHECK(!stream || stream->id() != eager, op, ": a graph of this leaf from the default stream is alive while this pass is captured; let go of its outputs first, or run it on another stream");
   }
 }
 

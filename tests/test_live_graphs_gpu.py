@@ -1,4 +1,4 @@
-"""A pass that is captured while an eager graph of the same leaves is alive is refused before anything is launched."""
+"""A pass that is captured while a graph of the same leaves from the default stream is alive is refused before anything is launched."""
 import pytest
 import torch
 
@@ -45,3 +45,23 @@ def test_refused_while_the_leaf_has_another_graph(name):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and bool(torch.isfinite(grad).all())
+
+
+@pytest.mark.parametrize("name", list(CALLS))
+def test_warm_up_on_a_side_stream_may_be_alive(name):
+    FIXED.update(g=-torch.ones(1, 40, 64, device=DEV), w=torch.ones(64, device=DEV))
+    leaf = torch.randn(*((1, 40, 64) if name == "recurrence" else (1, 1, 40, 64)), device=DEV, requires_grad=True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        alive = CALLS[name](leaf)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = CALLS[name](leaf)
+    for _ in range(3):
+        with torch.no_grad():
+            out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, alive)
