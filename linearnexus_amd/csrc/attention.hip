@@ -997,7 +997,9 @@ template <typename T> constexpr int step_waves() { return sizeof(T) == 2 ? 4 : 2
 // The queries that share a key head are the 32 columns, every wave walks over tiles of 32 cached tokens of its own: no barrier until
 // the waves' sums meet.  Bound by the bytes of the cache (the matrix products take a sixteenth of the time): the next tile is in
 // flight while one is multiplied.  The new token's key and value come from the call and are written to the cache by the wave whose
-// tile holds the place; what lies behind it is never read.  32 sequences of 6300 places on average, 8 key heads of 128: 152-161 us for 825
+// tile holds the place; what lies behind it is never read.  bf16 weights enter the product in two parts, so that a weight is off by 2^-16
+// and not by 2^-8: the products wait for the cache anyway (32 full caches of 8192 places, replayed: 195 us in one part, 197.6 in two;
+// caches that lie in L2, 8 of 4096 places of 64: 21.6 and 22.6).  32 sequences of 6300 places on average, 8 key heads of 128: 152-161 us for 825
 // MB, 5.2-5.4 TB/s, and 5 us to join the shares.
 template <typename T, int D> __global__ __launch_bounds__(64 * step_waves<T>(), 1) void attn_step_kernel(StepArgs a) {
   constexpr int W = step_waves<T>();
@@ -1096,10 +1098,15 @@ template <typename T, int D> __global__ __launch_bounds__(64 * step_waves<T>(), 
       for (int e = 0; e < 16; ++e) acc[i][e] *= f;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      Frag8<T> pf;
+      Frag8<T> pf, rest;
       from_acc(pf, sc, s);
+      rest_of(rest, sc, s, pf);
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) mma(acc[i], TL::by_col(cols, TL::BYTES + 16 * s * TL::ROWB, i), pf);
+      for (int i = 0; i < D / 32; ++i) {
+        const Frag8<T> v = TL::by_col(cols, TL::BYTES + 16 * s * TL::ROWB, i);
+        mma(acc[i], v, pf);
+        if constexpr (sizeof(T) == 2) mma(acc[i], v, rest);
+      }
     }
   }
   // the waves' sums, and this workgroup's share of the result
