@@ -473,7 +473,7 @@ int lnx_rmsnorm_residual_bwd(const lnx_rmsnorm_residual_args* a, void* hip_strea
  * Causal softmax attention over whole prompts with grouped heads, and its gradient: query i of a sequence attends to its keys
  * 0 .. i; query head h reads key head h / (H / Hkv).  q, o, d_o, d_q are [B, H, T, d], k, v, d_k, d_v [B, Hkv, T, d] in `dtype`,
  * each with its own strides (in elements, rows contiguous, every stride and pointer a multiple of 16 bytes, tokens at most
- * 16 MiB apart; an input's stride may be 0).  d <= 128 and a multiple of 8.  Packed batches as above.  lse [B, H, T] fp32 is written by the forward call if not
+ * 16 MiB apart; an input's stride may be 0, that of a dimension of one element anything).  d <= 128 and a multiple of 8.  Packed batches as above.  lse [B, H, T] fp32 is written by the forward call if not
  * NULL and read by the backward call, which also reads o and o_low, [B, H, T, d] dense in `dtype`: what the rounding of o left (NULL
  * in both calls: taken as zero, as it is in fp32); a workspace (16-byte aligned, may be NULL where its size is 0)
  * holds nothing between calls.  Where batch and heads give few workgroups the keys (queries) are split between several and their

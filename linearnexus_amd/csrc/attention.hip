@@ -878,10 +878,14 @@ uint64_t bwd_bytes(const lnx_attn_args* a) {
   return delta_bytes(a) + (q > k ? q : k);
 }
 
-// Rows that the kernels move as vectors, 64 of them within the 31 bits of a lane's offset
-bool rows_fit(const lnx_tensor4* t, int64_t size) {
-  return t->stride_t >= 0 && t->stride_t * size <= (int64_t)1 << 24 && reinterpret_cast<uintptr_t>(t->p) % 16 == 0 && t->stride_b * size % 16 == 0 && t->stride_h * size % 16 == 0 && t->stride_t * size % 16 == 0;
+// Rows that the kernels move as vectors, 64 of them within the 31 bits of a lane's offset.  The stride of a dimension of one element is
+// never stepped over, whatever it is.
+bool rows_fit(const lnx_tensor4* t, int64_t size, int B, int heads, int tokens) {
+  const auto fits = [&](int extent, int64_t stride) { return extent <= 1 || stride * size % 16 == 0; };
+  return (tokens <= 1 || (t->stride_t >= 0 && t->stride_t * size <= (int64_t)1 << 24)) && reinterpret_cast<uintptr_t>(t->p) % 16 == 0 && fits(B, t->stride_b) && fits(heads, t->stride_h) &&
+         fits(tokens, t->stride_t);
 }
+int64_t stride_over(int extent, int64_t stride) { return extent > 1 ? stride : 0; }
 
 int check(const char* what, const lnx_attn_args* a, bool bwd) {
   if (!a) return lnx_set_error(LNX_ERR_NULL, "%s: args is NULL", what);
@@ -893,9 +897,10 @@ int check(const char* what, const lnx_attn_args* a, bool bwd) {
   if (a->B == 0 || a->T == 0) return LNX_OK;
   if (!(a->scale == a->scale) || a->scale - a->scale != 0.f) return lnx_set_error(LNX_ERR_SHAPE, "%s: scale must be finite", what);
   const lnx_tensor4* ts[] = {&a->q, &a->k, &a->v, &a->o, &a->d_o, &a->d_q, &a->d_k, &a->d_v};
+  const int heads[] = {a->H, a->Hkv, a->Hkv, a->H, a->H, a->H, a->Hkv, a->Hkv};
   for (int i = 0; i < (bwd ? 8 : 4); ++i) {
     if (!ts[i]->p) return lnx_set_error(LNX_ERR_NULL, "%s: a tensor is missing", what);
-    if (!rows_fit(ts[i], a->dtype == LNX_BF16 ? 2 : 4)) return lnx_set_error(LNX_ERR_SHAPE, "%s: tensors must be 16-byte aligned, rows whole numbers of 16 bytes and at most 16 MiB apart", what);
+    if (!rows_fit(ts[i], a->dtype == LNX_BF16 ? 2 : 4, a->B, heads[i], a->T)) return lnx_set_error(LNX_ERR_SHAPE, "%s: tensors must be 16-byte aligned, rows whole numbers of 16 bytes and at most 16 MiB apart", what);
   }
   if (bwd && !a->lse) return lnx_set_error(LNX_ERR_NULL, "%s: lse is required", what);
   if (a->o_low && reinterpret_cast<uintptr_t>(a->o_low) % 16) return lnx_set_error(LNX_ERR_SHAPE, "%s: o_low must be 16-byte aligned", what);
@@ -909,9 +914,12 @@ int check(const char* what, const lnx_attn_args* a, bool bwd) {
 
 Args kernel_args(const lnx_attn_args* a) {
   Args k{};
-  auto strides = [](int64_t (&s)[3], const lnx_tensor4& t) { s[0] = t.stride_b, s[1] = t.stride_h, s[2] = t.stride_t; };
+  auto strides = [a](int64_t (&s)[3], const lnx_tensor4& t, int heads) {
+    s[0] = stride_over(a->B, t.stride_b), s[1] = stride_over(heads, t.stride_h), s[2] = stride_over(a->T, t.stride_t);
+  };
   k.q = a->q.p, k.k = a->k.p, k.v = a->v.p, k.dout = a->d_o.p, k.o = a->o.p, k.dq = a->d_q.p, k.dk = a->d_k.p, k.dv = a->d_v.p;
-  strides(k.qs, a->q), strides(k.ks, a->k), strides(k.vs, a->v), strides(k.os, a->o), strides(k.gs, a->d_o), strides(k.dqs, a->d_q), strides(k.dks, a->d_k), strides(k.dvs, a->d_v);
+  strides(k.qs, a->q, a->H), strides(k.ks, a->k, a->Hkv), strides(k.vs, a->v, a->Hkv), strides(k.os, a->o, a->H);
+  strides(k.gs, a->d_o, a->H), strides(k.dqs, a->d_q, a->H), strides(k.dks, a->d_k, a->Hkv), strides(k.dvs, a->d_v, a->Hkv);
   k.lse = a->lse, k.o_low = a->o_low, k.cu = a->cu_seqlens;
   k.B = a->B, k.H = a->H, k.Hkv = a->Hkv, k.G = a->H / a->Hkv, k.T = a->T, k.d = a->d, k.nseq = a->nseq, k.scale = a->scale;
   return k;
@@ -1227,9 +1235,9 @@ int check_step(const lnx_attn_step_args* a) {
   if (a->B == 0) return LNX_OK;
   if (!(a->scale == a->scale) || a->scale - a->scale != 0.f) return lnx_set_error(LNX_ERR_SHAPE, "%s: scale must be finite", what);
   const lnx_tensor4* ts[] = {&a->q, &a->k, &a->v, &a->k_cache, &a->v_cache};
-  for (const lnx_tensor4* t : ts) {
-    if (!t->p) return lnx_set_error(LNX_ERR_NULL, "%s: a tensor is missing", what);
-    if (!rows_fit(t, a->dtype == LNX_BF16 ? 2 : 4)) return lnx_set_error(LNX_ERR_SHAPE, "%s: tensors must be 16-byte aligned, rows whole numbers of 16 bytes and at most 16 MiB apart", what);
+  for (int i = 0; i < 5; ++i) {
+    if (!ts[i]->p) return lnx_set_error(LNX_ERR_NULL, "%s: a tensor is missing", what);
+    if (!rows_fit(ts[i], a->dtype == LNX_BF16 ? 2 : 4, a->B, i == 0 ? a->H : a->Hkv, i < 3 ? 1 : a->S)) return lnx_set_error(LNX_ERR_SHAPE, "%s: tensors must be 16-byte aligned, rows whole numbers of 16 bytes and at most 16 MiB apart", what);
   }
   if (!a->o || !a->lengths) return lnx_set_error(LNX_ERR_NULL, "%s: o and lengths are required", what);
   if (reinterpret_cast<uintptr_t>(a->o) % 16) return lnx_set_error(LNX_ERR_SHAPE, "%s: tensors must be 16-byte aligned, rows whole numbers of 16 bytes and at most 16 MiB apart", what);
@@ -1244,9 +1252,9 @@ template <typename T, int D> int launch_step(const lnx_attn_step_args* a, hipStr
   constexpr int W = step_waves<T>();
   StepArgs k{};
   k.q = a->q.p, k.k = a->k.p, k.v = a->v.p, k.kc = a->k_cache.p, k.vc = a->v_cache.p, k.o = a->o, k.len = a->lengths, k.part = static_cast<float*>(a->workspace);
-  k.qs[0] = a->q.stride_b, k.qs[1] = a->q.stride_h, k.ks[0] = a->k.stride_b, k.ks[1] = a->k.stride_h, k.vs[0] = a->v.stride_b, k.vs[1] = a->v.stride_h;
-  k.kcs[0] = a->k_cache.stride_b, k.kcs[1] = a->k_cache.stride_h, k.kcs[2] = a->k_cache.stride_t;
-  k.vcs[0] = a->v_cache.stride_b, k.vcs[1] = a->v_cache.stride_h, k.vcs[2] = a->v_cache.stride_t;
+  auto strides = [a](int64_t* s, const lnx_tensor4& t, int heads) { s[0] = stride_over(a->B, t.stride_b), s[1] = stride_over(heads, t.stride_h); };
+  strides(k.qs, a->q, a->H), strides(k.ks, a->k, a->Hkv), strides(k.vs, a->v, a->Hkv), strides(k.kcs, a->k_cache, a->Hkv), strides(k.vcs, a->v_cache, a->Hkv);
+  k.kcs[2] = stride_over(a->S, a->k_cache.stride_t), k.vcs[2] = stride_over(a->S, a->v_cache.stride_t);
   k.B = a->B, k.H = a->H, k.Hkv = a->Hkv, k.G = a->H / a->Hkv, k.S = a->S, k.d = a->d, k.scale = a->scale;
   k.splits = step_splits(a), k.ctiles = (k.G + 31) / 32;
   const size_t tiles = W * 4 * Tile<T, D, SROWS>::BYTES, sums = W * ((D / 32) * 16 * 64 + 64) * sizeof(float), bytes = tiles > sums ? tiles : sums;

@@ -1369,12 +1369,12 @@ PyObject* py_linrec_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 // ---------------------------------------------------------------------------------------------------------------
 
 // [B, H, T, d] (or [B, H, d]) tensors as the kernels read and write them: any strides that are whole numbers of 16 bytes, tokens at most
-// 16 MiB apart
+// 16 MiB apart.  The stride of a dimension of one element says nothing (and contiguous() leaves it as it is).
 bool vector_rows(const Tensor& t) {
-  if (t.dim() == 4 && t.stride(2) * t.element_size() > (int64_t)1 << 24) return false;
+  if (t.dim() == 4 && t.size(2) > 1 && t.stride(2) * t.element_size() > (int64_t)1 << 24) return false;
   if (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 || (t.size(-1) != 1 && t.stride(-1) != 1)) return false;
   for (int64_t i = 0; i + 1 < t.dim(); ++i)
-    if (t.stride(i) * t.element_size() % 16) return false;
+    if (t.size(i) > 1 && t.stride(i) * t.element_size() % 16) return false;
   return true;
 }
 // Whether no two rows share memory: each dimension steps over the whole extent of those with smaller strides

@@ -26,3 +26,43 @@ def test_step_is_as_exact_as_its_rounding(B, H, Hkv, S, d, lens):
             P = torch.softmax(S_, 0)
             EP = P * (ES + 2 * ES.max() + (n + 32) * UP)
             _within(o[b, h], P @ val, (EP + (r + (n + 32) * UP) * P) @ val.abs(), f"o {b} {h}")
+
+
+# -- dimensions of one element, whose strides say nothing ----------------------------------------------------------
+
+def _slices(B, T, H, Hkv, d, dtype, more):
+    """q, k, v as a fused projection leaves them, its rows `more` columns longer than what the heads take."""
+    width = (H + 2 * Hkv) * d + more
+    g = torch.Generator().manual_seed(3)
+    p = torch.randn(B, T, width, generator=g).to(DEV, torch.bfloat16 if dtype == "bf16" else torch.float32)
+    cut = lambda first, h: p.as_strided((B, T, h, d), (T * width, width, d, 1), first)
+    return cut(0, H), cut(H * d, Hkv), cut((H + Hkv) * d, Hkv)
+
+
+@pytest.mark.parametrize("dtype,more", [("bf16", 4), ("f32", 2)])
+@pytest.mark.parametrize("B,T,H,Hkv", [(1, 1, 4, 1), (1, 1, 2, 2), (3, 1, 4, 1), (1, 5, 4, 1), (1, 5, 1, 1)])
+def test_prompt_strides_of_single_elements(B, T, H, Hkv, dtype, more):
+    q, k, v = (t.transpose(1, 2) for t in _slices(B, T, H, Hkv, 64, dtype, more))
+    do = _slices(B, T, H, Hkv, 64, dtype, more)[0].transpose(1, 2)
+    _check(q, k, v, do)
+
+
+@pytest.mark.parametrize("dtype,more", [("bf16", 4), ("f32", 2)])
+@pytest.mark.parametrize("B,H,Hkv", [(1, 8, 1), (1, 4, 2), (2, 4, 1)])
+def test_step_strides_of_single_elements(B, H, Hkv, dtype, more):
+    q, k, v = (t[:, 0] for t in _slices(B, 1, H, Hkv, 64, dtype, more))
+    _, _, _, kc, vc = _step_inputs(B, H, Hkv, 50, 64, dtype)
+    _check_step(q, k, v, kc, vc, [49 - b for b in range(B)])
+
+
+@pytest.mark.parametrize("dtype,more", [("bf16", 4), ("f32", 2)])
+@pytest.mark.parametrize("Hkv,S", [(1, 40), (2, 1), (1, 1)])
+def test_step_cache_strides_of_single_elements(Hkv, S, dtype, more):
+    """Caches of one sequence (and one key head, one place) inside a buffer whose rows the strides of those dimensions do not fit."""
+    q, k, v, kc, vc = _step_inputs(1, 4, Hkv, S, 64, dtype)
+
+    def odd(t):
+        strides = [64 * Hkv * S + more, 64 * S + (more if Hkv == 1 else 0), 64 + (more if S == 1 else 0), 1]
+        return torch.empty(t.numel() + 64, device=DEV, dtype=t.dtype).as_strided(t.shape, strides).copy_(t)
+
+    _check_step(q, k, v, odd(kc), odd(vc), [S - 1])

@@ -1,0 +1,43 @@
+"""Strides of dimensions of one element at the C boundary, without a GPU.  Every call below is
+refused for another reason behind the strides' check, so that nothing is launched."""
+from linearnexus_amd import _lib
+from test_layer_ops_cpu import _attn, _ptr, _refused
+
+ODD = 644  # elements of two bytes: no whole number of 16 bytes
+
+
+def test_attention_strides_of_single_elements():
+    lib = _lib.load()
+    long = _attn(H=1, Hkv=1, T=65536)  # needs a workspace, and has none
+    for n in ("q", "k", "v", "o"):
+        setattr(long, n, _lib.Tensor4(_ptr(), ODD, ODD, 64))
+    _refused(lib.lnx_attn_fwd(long, None), -4, b"workspace")
+    long.k.stride_t = ODD
+    _refused(lib.lnx_attn_fwd(long, None), -2, b"aligned")
+    one = _attn(B=2, H=2, Hkv=2, T=1)
+    one.lse = _ptr()
+    for n in ("q", "k", "v", "o", "d_o", "d_q", "d_k", "d_v"):
+        setattr(one, n, _lib.Tensor4(_ptr(), 128, 64, (1 << 40) + 1))
+    _refused(lib.lnx_attn_bwd(one, None), -4, b"workspace")
+    one.d_k.stride_t = -1
+    _refused(lib.lnx_attn_bwd(one, None), -4, b"workspace")
+    one.d_v.stride_h = 65
+    _refused(lib.lnx_attn_bwd(one, None), -2, b"aligned")
+
+
+def test_attention_step_strides_of_single_elements():
+    lib = _lib.load()
+
+    def step(**kw):
+        a = _lib.AttnStepArgs(**{**dict(B=1, H=4, Hkv=1, S=4096, d=64, dtype=_lib.LNX_BF16, scale=1.0), **kw})
+        a.q, a.k, a.v = _lib.Tensor4(_ptr(), ODD, 64, 3), _lib.Tensor4(_ptr(), ODD, ODD, 3), _lib.Tensor4(_ptr(), ODD, ODD, 3)
+        a.k_cache, a.v_cache = _lib.Tensor4(_ptr(), ODD, ODD, 64), _lib.Tensor4(_ptr(), ODD, ODD, 64)
+        a.o = a.lengths = _ptr()
+        return a
+
+    _refused(lib.lnx_attn_step(step(), None), -4, b"workspace")
+    _refused(lib.lnx_attn_step(step(B=2), None), -2, b"aligned")
+    _refused(lib.lnx_attn_step(step(H=4, Hkv=2), None), -2, b"aligned")
+    a = step()
+    a.k_cache.stride_t = 65
+    _refused(lib.lnx_attn_step(a, None), -2, b"aligned")
