@@ -400,7 +400,7 @@ int lnx_sigmoid_bwd(const float* y, const float* dy, float* dx, int64_t n, void*
  *   h_t = e^{g_t} h_{t-1} + x_t,  y_t = h_t;   dh_t = dy_t + e^{g_{t+1}} dh_{t+1},  dx = dh,  dg_t = e^{g_t} h_{t-1} dh_t
  * x, y, d_y, d_x in `dtype`, g and d_g in `g_dtype` (LNX_F32 or `dtype`; log-decays, <= 0, -inf drops what came before);
  * states [B, D] ([nseq, D] packed) fp32.  x, g and d_y have a stride per row and per token in elements (last dimension
- * contiguous, tokens at most 4 MiB apart); everything else is dense.  The forward call leaves in `kept` what the backward call reads (NULL: no backward
+ * contiguous, tokens at most 4 MiB apart where there are two); everything else is dense.  The forward call leaves in `kept` what the backward call reads (NULL: no backward
  * pass will follow); `workspace` holds nothing between calls and may be NULL where its size is 0.  initial_state, d_y,
  * d_final_state (zeros) and d_initial_state may be NULL.  lnx_linrec_step is one token on n = B D contiguous elements;
  * new_state may be state.

@@ -1235,8 +1235,11 @@ PyObject* py_dplr_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 // element-wise gated linear recurrence
 // ---------------------------------------------------------------------------------------------------------------
 
-// What the kernels read in place: any strides over rows and tokens (at most 4 MiB), channels next to each other
-Tensor channels_dense(const Tensor& x) { return (x.size(-1) == 1 || x.stride(-1) == 1) && x.stride(1) * x.element_size() <= 4 << 20 ? x : x.contiguous(); }
+// What the kernels read in place: any strides over rows and tokens (at most 4 MiB; that of a single token says nothing), channels next to
+// each other
+Tensor channels_dense(const Tensor& x) {
+  return (x.size(-1) == 1 || x.stride(-1) == 1) && (x.size(1) == 1 || x.stride(1) * x.element_size() <= 4 << 20) ? x : x.contiguous();
+}
 
 struct RecShape {
   int64_t B, T, D, nseq, rows;

@@ -627,6 +627,8 @@ bool chained(const lnx_linrec_args* a) {
 int64_t pair_words(const lnx_linrec_args* a) { return 2 * (slots_of(a, CTILE) + slots_of(a, CTILE * GROUP)) * a->D; }
 int64_t all_words(const lnx_linrec_args* a) { return pair_words(a) + (slots_of(a, CTILE * ANCHOR) * a->D + 3) / 4 * 4; }
 
+int64_t token_stride(const lnx_linrec_args* a, int64_t stride) { return a->T > 1 ? stride : a->D; }
+
 int check(const char* what, const lnx_linrec_args* a, bool bwd) {
   if (!a) return lnx_set_error(LNX_ERR_NULL, "%s: args is NULL", what);
   if (a->B < 0 || a->T < 0 || a->D <= 0 || a->nseq < 0 || (a->nseq && a->B != 1))
@@ -638,9 +640,9 @@ int check(const char* what, const lnx_linrec_args* a, bool bwd) {
   if (tokens && (!a->x || !a->g)) return lnx_set_error(LNX_ERR_NULL, "%s: x and g are required", what);
   if (!bwd && ((tokens && !a->y) || (rows && !a->final_state))) return lnx_set_error(LNX_ERR_NULL, "%s: y and final_state are required", what);
   if (bwd && tokens && (!a->d_x || !a->d_g || !a->kept)) return lnx_set_error(LNX_ERR_NULL, "%s: d_x, d_g and kept are required", what);
-  // a lane's bytes within a tile are a 32-bit offset
-  for (int64_t st : {a->x_stride_t * (a->dtype == LNX_BF16 ? 2 : 4), a->g_stride_t * (a->g_dtype == LNX_BF16 ? 2 : 4), (bwd ? a->d_y_stride_t : 0) * (a->dtype == LNX_BF16 ? 2 : 4),
-                     (int64_t)a->D * 4})
+  // a lane's bytes within a tile are a 32-bit offset; the stride of a single token is never stepped over
+  for (int64_t st : {token_stride(a, a->x_stride_t) * (a->dtype == LNX_BF16 ? 2 : 4), token_stride(a, a->g_stride_t) * (a->g_dtype == LNX_BF16 ? 2 : 4),
+                     (bwd ? token_stride(a, a->d_y_stride_t) : 0) * (a->dtype == LNX_BF16 ? 2 : 4), (int64_t)a->D * 4})
     if (st < 0 || st > MAX_STRIDE) return lnx_set_error(LNX_ERR_SHAPE, "%s: tokens more than %lld bytes apart", what, (long long)MAX_STRIDE);
   if ((int64_t)rows_of(a) * channel_tiles(a) > MAX_GRID / THREADS) return lnx_set_error(LNX_ERR_SHAPE, "%s: too many rows", what);
   if (rows && chained(a)) {
@@ -655,7 +657,8 @@ bool vectors(const void* p, int64_t sb, int64_t st, int64_t size) { return !p ||
 Args kernel_args(const lnx_linrec_args* a) {
   Args k{};
   k.x = a->x, k.g = a->g, k.dy = a->d_y;
-  k.xb = a->x_stride_b, k.xt = a->x_stride_t, k.gb = a->g_stride_b, k.gt = a->g_stride_t, k.yb = a->d_y_stride_b, k.yt = a->d_y_stride_t;
+  k.xb = a->x_stride_b, k.gb = a->g_stride_b, k.yb = a->d_y_stride_b;
+  k.xt = token_stride(a, a->x_stride_t), k.gt = token_stride(a, a->g_stride_t), k.yt = token_stride(a, a->d_y_stride_t);
   k.s0 = a->initial_state, k.ds = a->d_final_state, k.cu = a->cu_seqlens;
   k.y = a->y, k.dx = a->d_x, k.dg = a->d_g, k.sT = a->final_state, k.d0 = a->d_initial_state, k.kept = a->kept;
   k.T = a->T, k.D = a->D, k.ctiles = channel_tiles(a), k.packed = a->nseq != 0;
@@ -689,8 +692,8 @@ int run(const char* what, const lnx_linrec_args* a, bool bwd, hipStream_t st) {
   if (rows_of(a) == 0) return LNX_OK;
   const int64_t xs = a->dtype == LNX_BF16 ? 2 : 4, gs = a->g_dtype == LNX_BF16 ? 2 : 4;
   // four elements at a time: of the inputs with their strides, and of the outputs, whose rows are D long
-  bool vec = a->D % 4 == 0 && vectors(a->x, a->x_stride_b, a->x_stride_t, xs) && vectors(a->g, a->g_stride_b, a->g_stride_t, gs) &&
-             vectors(a->d_y, a->d_y_stride_b, a->d_y_stride_t, xs);
+  bool vec = a->D % 4 == 0 && vectors(a->x, a->x_stride_b, token_stride(a, a->x_stride_t), xs) && vectors(a->g, a->g_stride_b, token_stride(a, a->g_stride_t), gs) &&
+             vectors(a->d_y, a->d_y_stride_b, token_stride(a, a->d_y_stride_t), xs);
   for (const void* p : {(const void*)a->y, (const void*)a->d_x}) vec = vec && reinterpret_cast<uintptr_t>(p) % (4 * xs) == 0;
   vec = vec && reinterpret_cast<uintptr_t>(a->d_g) % (4 * gs) == 0;
   if (a->dtype == LNX_F32) vec ? launch<float, float, true>(a, bwd, st) : launch<float, float, false>(a, bwd, st);

@@ -41,3 +41,14 @@ def test_attention_step_strides_of_single_elements():
     a = step()
     a.k_cache.stride_t = 65
     _refused(lib.lnx_attn_step(a, None), -2, b"aligned")
+
+
+def test_recurrence_stride_of_a_single_token():
+    lib = _lib.load()
+    a = _lib.LinrecArgs(B=1 << 24, T=1, D=64, x_stride_t=1 << 40, g_stride_t=-1, d_y_stride_t=1 << 40)
+    a.x = a.g = a.y = a.final_state = a.d_x = a.d_g = a.kept = _ptr()
+    for fn in (lib.lnx_linrec_fwd, lib.lnx_linrec_bwd):
+        _refused(fn(a, None), -2, b"too many rows")
+    a.T = 2
+    for fn in (lib.lnx_linrec_fwd, lib.lnx_linrec_bwd):
+        _refused(fn(a, None), -2, b"apart")
