@@ -166,12 +166,13 @@ template <typename T, int D, int R = ROWS> struct Mover {
   }
 };
 __device__ __forceinline__ bool is_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
-// What the rounding of that operand left, as a second operand
-__device__ __forceinline__ void rest_of(Frag8<bf16_t>& f, const floatx16& c, int h, const Frag8<bf16_t>& rounded) {
+// What the rounding of that operand left, as a second operand.  WEIGHTS: the values are at most 2^8 or NaN (of a score gradient that is
+// infinite, or becomes so, nothing is left).
+template <bool WEIGHTS> __device__ __forceinline__ void rest_of(Frag8<bf16_t>& f, const floatx16& c, int h, const Frag8<bf16_t>& rounded) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) f.v[e] = from_f32<bf16_t>(is_finite(to_f32(rounded.v[e])) ? c[8 * h + e] - to_f32(rounded.v[e]) : 0.f);
+  for (int e = 0; e < 8; ++e) f.v[e] = from_f32<bf16_t>(WEIGHTS || is_finite(to_f32(rounded.v[e])) ? c[8 * h + e] - to_f32(rounded.v[e]) : 0.f);
 }
-__device__ __forceinline__ void rest_of(Frag8<float>&, const floatx16&, int, const Frag8<float>&) {}
+template <bool WEIGHTS> __device__ __forceinline__ void rest_of(Frag8<float>&, const floatx16&, int, const Frag8<float>&) {}
 // Whether the granules that this lane's loads brought hold finite values only; SCRUB: the others become 0.  A wave's granules are
 // rows 16 wave .. 16 wave + 15.
 template <typename T, int D, bool SCRUB, int R = ROWS> __device__ __forceinline__ bool tile_finite(T* tile, int wave, int lane) {
@@ -196,9 +197,9 @@ __device__ __forceinline__ void clear_lds(char* p, int bytes) {
 
 // How a run of N products takes its operands from LDS (COL: through by_col): AHEAD operands are on their way before the first product
 // and each product is followed by the reads of another.  Left to itself the compiler saves the registers and waits for every operand
-// right before its product, 130 cycles for 32 of work.
-template <typename T, bool COL, int N, int AHEAD> __device__ __forceinline__ void read_ahead() {
-  constexpr int READS = sizeof(T) == 2 ? (COL ? 2 : 1) : (COL ? 8 : 2), PRODUCTS = sizeof(T) == 2 ? 1 : 8, DS = 0x100, MFMA = 0x8;
+// right before its product, 130 cycles for 32 of work.  EACH: products that take the same operand.
+template <typename T, bool COL, int N, int AHEAD, int EACH = 1> __device__ __forceinline__ void read_ahead() {
+  constexpr int READS = sizeof(T) == 2 ? (COL ? 2 : 1) : (COL ? 8 : 2), PRODUCTS = EACH * (sizeof(T) == 2 ? 1 : 8), DS = 0x100, MFMA = 0x8;
   __builtin_amdgcn_sched_group_barrier(DS, READS * AHEAD, 0);
 #pragma unroll
   for (int i = 0; i < N - AHEAD; ++i) {
@@ -324,19 +325,22 @@ template <typename T, int M> __device__ __forceinline__ void store_low(T* p, con
 // prompts of 8192 tokens together 175 us with 64, 160 with 32; B2 H16/4 T4096 154 and 156.
 template <typename T, int D> constexpr int fwd_rows() { return sizeof(T) == 2 && D == 128 ? 32 : 64; }
 
-// A wave owns 32 queries, the workgroup 128; of a block's key tiles every a.parts-th.
-// TWO (all three kernels): weights and score gradients enter the products in two bf16 parts.  For sequences of one tile on average: a
+// TWO (all three kernels): weights and score gradients enter the products in two bf16 parts.  For sequences of up to SHORT tokens: a
 // gradient there is a sum of a few terms, whose roundings (2^-8 each) do not average out: of three tokens dq and dk were 1.8 times as
-// far off as their own rounding leaves them, of 64 and more 1.4 times.
-template <typename T, int D, bool TWO> __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : TWO ? 2 : 3) void attn_fwd_kernel(Args a) {
+// far off as their own rounding leaves them, of 64 and more 1.4 times.  Every workgroup goes by its own sequence, so that a document's
+// operands do not depend on what it is packed with; kernels that may meet both kinds hold both forms (MIXED: packed batches; forward of
+// eight prompts of 8192 tokens together 175 us with one form, 177-183 with both).  128 tokens are one block of queries.  By the average
+// length a document of 8000 tokens among 150 of one, H16/4 d128, took 422 us forward and 2035 backward, this way 305 and 1405; 2048 of
+// 128, H8/2 d128, in one part 760 and 1955, in two 759 and 2247.
+constexpr int SHORT = 128;
+
+// A wave owns 32 queries, the workgroup 128; of a block's key tiles every a.parts-th.
+template <typename T, int D, bool TWO> __device__ __forceinline__ void fwd_block(const Args& a, const Place& p, char* lds) {
   constexpr int KT = fwd_rows<T, D>(), KH = KT / 32;
   typedef Tile<T, D, KT> TL;
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-  const auto kt = [](int buf) { return reinterpret_cast<T*>(lds + 2 * buf * TL::BYTES); };
-  const auto vt = [](int buf) { return reinterpret_cast<T*>(lds + (2 * buf + 1) * TL::BYTES); };
+  const auto kt = [=](int buf) { return reinterpret_cast<T*>(lds + 2 * buf * TL::BYTES); };
+  const auto vt = [=](int buf) { return reinterpret_cast<T*>(lds + (2 * buf + 1) * TL::BYTES); };
   int* odd = reinterpret_cast<int*>(lds + 4 * TL::BYTES);
-  const Place p = place(a, 128, a.G, true);
-  if (!p.on) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, kg = lane >> 5;
   const int h = p.hkv * a.G + p.g, q_wg = p.blk * 128, q0 = q_wg + wave * 32, q = q0 + n;
   const T* kb = at<T>(a.k, a.ks, p.b, p.hkv, p.tok);
@@ -427,22 +431,21 @@ template <typename T, int D, bool TWO> __global__ __launch_bounds__(256, sizeof(
         sum += sc[i][e];
       }
     l += sum;
-    Frag8<T> pf[2 * KH];
+    Frag8<T> pf[2 * KH], rest[2 * KH];
 #pragma unroll
-    for (int s = 0; s < 2 * KH; ++s) from_acc(pf[s], sc[s >> 1], s & 1);
+    for (int s = 0; s < 2 * KH; ++s) {
+      from_acc(pf[s], sc[s >> 1], s & 1);
+      if constexpr (TWO) rest_of<true>(rest[s], sc[s >> 1], s & 1, pf[s]);
+    }
 #pragma unroll
     for (int s = 0; s < 2 * KH; ++s)
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) mma(acc[i], TL::by_col(cols, TL::BYTES + 16 * s * TL::ROWB, i), pf[s]);
-    read_ahead<T, true, 2 * KH * (D / 32), 4>();
-    if constexpr (TWO)
-#pragma unroll
-      for (int s = 0; s < 2 * KH; ++s) {
-        Frag8<T> rest;
-        rest_of(rest, sc[s >> 1], s & 1, pf[s]);
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) mma(acc[i], TL::by_col(cols, TL::BYTES + 16 * s * TL::ROWB, i), rest);
+      for (int i = 0; i < D / 32; ++i) {
+        const Frag8<T> v = TL::by_col(cols, TL::BYTES + 16 * s * TL::ROWB, i);
+        mma(acc[i], v, pf[s]);
+        if constexpr (TWO) mma(acc[i], v, rest[s]);
       }
+    read_ahead<T, true, 2 * KH * (D / 32), TWO ? 1 : 4, TWO ? 2 : 1>();  // (four ahead of two products each spill: 1134 us for those 2048, 759)
     if (edge && odd[buf])
 #pragma unroll
       for (int i = 0; i < KH; ++i) {
@@ -462,6 +465,14 @@ template <typename T, int D, bool TWO> __global__ __launch_bounds__(256, sizeof(
     store_column<float, D / 32>(a.part + at_part * a.d, acc, 1.f, a.d, lane);
     if (kg == 0) a.part_stat[2 * at_part] = m * c, a.part_stat[2 * at_part + 1] = sum;
   }
+}
+
+template <typename T, int D, bool MIXED> __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 3) void attn_fwd_kernel(Args a) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const Place p = place(a, 128, a.G, true);
+  if (!p.on) return;
+  if (MIXED && __builtin_amdgcn_readfirstlane(p.len) <= SHORT) fwd_block<T, D, MIXED>(a, p, lds);
+  else fwd_block<T, D, false>(a, p, lds);
 }
 
 // The parts of a row's result, sixteen lanes a row
@@ -518,14 +529,10 @@ template <typename T> __global__ __launch_bounds__(256) void attn_sum_kernel(con
 // Queries as in the forward pass, their gradients beside them in registers.  delta is formed here, for the dk / dv kernel too: of o and
 // what its rounding left, because an error of delta goes into every term of a row of dq (rounded o alone: 1.5 times the error that the
 // rounding of dq has, with it 1.4).
-template <typename T, int D, bool TWO> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(Args a) {
+template <typename T, int D, bool TWO> __device__ __forceinline__ void dq_block(const Args& a, const Place& p, char* lds) {
   typedef Tile<T, D> TL;
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-  const auto kt = [](int buf) { return reinterpret_cast<T*>(lds + 2 * buf * TL::BYTES); };
-  const auto vt = [](int buf) { return reinterpret_cast<T*>(lds + (2 * buf + 1) * TL::BYTES); };
+  const auto kt = [=](int buf) { return reinterpret_cast<T*>(lds + 2 * buf * TL::BYTES); };
   int* odd = reinterpret_cast<int*>(lds + 4 * TL::BYTES);
-  const Place p = place(a, 128, a.G, true);
-  if (!p.on) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, kg = lane >> 5;
   const int h = p.hkv * a.G + p.g, q_wg = p.blk * 128, q0 = q_wg + wave * 32, q = q0 + n;
   const T* kb = at<T>(a.k, a.ks, p.b, p.hkv, p.tok);
@@ -604,7 +611,7 @@ template <typename T, int D, bool TWO> __global__ __launch_bounds__(256, sizeof(
             if (key0 + 32 * i + frag_row(e, lane) > q) sc[e] = 0.f;
         from_acc(ds[0], sc, 0);
         from_acc(ds[1], sc, 1);
-        if constexpr (TWO) rest_of(rest[0], sc, 0, ds[0]), rest_of(rest[1], sc, 1, ds[1]);
+        if constexpr (TWO) rest_of<false>(rest[0], sc, 0, ds[0]), rest_of<false>(rest[1], sc, 1, ds[1]);
       }
       if (scrub) {  // the scores are made of the keys as they are
         lds_barrier();
@@ -615,13 +622,12 @@ template <typename T, int D, bool TWO> __global__ __launch_bounds__(256, sizeof(
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
-          for (int m = 0; m < D / 32; ++m) mma(acc[m], TL::by_col(cols, (32 * i + 16 * s) * TL::ROWB, m), ds[s]);
-        read_ahead<T, true, 2 * (D / 32), 4>();
-        if constexpr (TWO)
-#pragma unroll
-          for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int m = 0; m < D / 32; ++m) mma(acc[m], TL::by_col(cols, (32 * i + 16 * s) * TL::ROWB, m), rest[s]);
+          for (int m = 0; m < D / 32; ++m) {
+            const Frag8<T> k = TL::by_col(cols, (32 * i + 16 * s) * TL::ROWB, m);
+            mma(acc[m], k, ds[s]);
+            if constexpr (TWO) mma(acc[m], k, rest[s]);
+          }
+        read_ahead<T, true, 2 * (D / 32), 4, TWO ? 2 : 1>();
         if (scrub) add_odd<T, D / 32>(acc, kb, a.ks[2], key0 + 32 * i, p.len, a.d, ds, lane, [&](int row) { return row <= q; });
       }
     }
@@ -629,6 +635,14 @@ template <typename T, int D, bool TWO> __global__ __launch_bounds__(256, sizeof(
   if (q >= p.len) return;
   if (a.parts == 1) store_column<T, D / 32>(at<T>(a.dq, a.dqs, p.b, h, p.tok + q), acc, a.scale, a.d, lane);
   else store_column<float, D / 32>(a.part + ((int64_t)p.part * a.B * a.H * a.T + stat) * a.d, acc, a.scale, a.d, lane);
+}
+
+template <typename T, int D, bool MIXED> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(Args a) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const Place p = place(a, 128, a.G, true);
+  if (!p.on) return;
+  if (MIXED && __builtin_amdgcn_readfirstlane(p.len) <= SHORT) dq_block<T, D, MIXED>(a, p, lds);
+  else dq_block<T, D, false>(a, p, lds);
 }
 
 // An operand through LDS to another wave of the workgroup
@@ -644,23 +658,23 @@ template <typename T> __device__ __forceinline__ void take_frag(unsigned at, Fra
   for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = lds_load<floatx4>(at + 1024 * i + 16 * lane);
 }
 
-template <typename T, bool TWO> constexpr int hand_over() { return (TWO ? 16384 : 8192) * (int)sizeof(T); }  // bytes of a workgroup
+template <typename T> constexpr int hand_over() { return 8192 * (int)sizeof(T); }  // bytes of a workgroup
 
 // A workgroup owns 64 keys.  Wave (kw, qw) forms the weights of 32 keys and the half qw of a tile's queries, hands them to the wave of
 // the other half, and adds up the half qw of the columns of dk and dv over all queries: accumulators of half the size, so that two
 // workgroups share a CU.  (With both halves in every wave it took 416 registers and one workgroup a CU; as long, 456 and 469 us at B2 H16/4
 // T4096 d128, while the first keys' workgroups, which walk over all queries, were what the launch waited for.  Their queries split into
 // parts need the second workgroup: 317 us.)  The LDS of a workgroup is 80 KB to the byte: the queries' lse and delta go straight to
-// registers, a flag crosses in the hand-over's place.
-template <typename T, int D, bool TWO> __global__ __launch_bounds__(256, sizeof(T) == 2 && !TWO ? 2 : 1) void attn_dkv_kernel(Args a) {
+// registers, a flag crosses in the hand-over's place.  In two parts twice as much is handed over, in the place of the second buffer of
+// tiles, and the next tile is fetched when the waves have done with the one before: a short sequence has one or two for each query head.
+template <typename T, int D, bool TWO> __device__ __forceinline__ void dkv_block(const Args& a, const Place& p, char* lds) {
   typedef Tile<T, D> TL;
   typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
-  constexpr int M = D / 64, FRAG = 1024 * (int)sizeof(T) / 2, HAND = hand_over<T, TWO>() / 4;  // bytes that a wave hands over
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-  const auto qt = [](int buf) { return reinterpret_cast<T*>(lds + 2 * buf * TL::BYTES); };
-  const auto gt = [](int buf) { return reinterpret_cast<T*>(lds + (2 * buf + 1) * TL::BYTES); };
-  const Place p = place(a, ROWS, 1, false);
-  if (!p.on) return;
+  constexpr int M = D / 64, FRAG = 1024 * (int)sizeof(T) / 2, HAND = hand_over<T>() / 4 * (TWO ? 2 : 1);  // bytes that a wave hands over
+  constexpr int BUFS = TWO ? 1 : 2;
+  static_assert(2 * BUFS * TL::BYTES + 4 * HAND <= 4 * TL::BYTES + hand_over<T>(), "both forms have the same LDS");
+  const auto qt = [=](int buf) { return reinterpret_cast<T*>(lds + 2 * buf * TL::BYTES); };
+  const auto gt = [=](int buf) { return reinterpret_cast<T*>(lds + (2 * buf + 1) * TL::BYTES); };
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, kg = lane >> 5;
   const int kw = wave & 1, qw = wave >> 1, r0 = 32 * qw, key0 = p.blk * ROWS + 32 * kw, key = key0 + n;
   const int per = (p.len + ROWS - 1) / ROWS - p.blk, total = per * a.G, last = (p.blk + per) * ROWS;
@@ -669,7 +683,7 @@ template <typename T, int D, bool TWO> __global__ __launch_bounds__(256, sizeof(
     lds_barrier();
   }
   const Mover<T, D> mq(a.qs[2], a.d, wave, lane), mg(a.gs[2], a.d, wave, lane);
-  const unsigned lds0 = lds_byte_addr(lds), mine = lds0 + 4 * TL::BYTES + HAND * wave, theirs = lds0 + 4 * TL::BYTES + HAND * (wave ^ 2);
+  const unsigned lds0 = lds_byte_addr(lds), hand = lds0 + 2 * BUFS * TL::BYTES, mine = hand + HAND * wave, theirs = hand + HAND * (wave ^ 2);
   floatx4 lse[4], delta[4];
   auto fetch_stats = [&](int h, int row0) {
     const int64_t first = ((int64_t)p.b * a.H + h) * a.T + p.tok;
@@ -717,7 +731,7 @@ template <typename T, int D, bool TWO> __global__ __launch_bounds__(256, sizeof(
 #pragma unroll
     for (int e = 0; e < 16; ++e) dk[i][e] = dv[i][e] = 0.f;
   const unsigned row_addr = lds0 + r0 * TL::ROWB + TL::rows(lane), col_addr = TL::col_block(lds0 + TL::cols(lane), M * qw);
-  for (int it = p.part, buf = 0; it < total; it += a.parts, buf ^= 1) {
+  for (int it = p.part, buf = 0; it < total; it += a.parts, buf ^= BUFS - 1) {
     dma_wait<0>();
 #pragma unroll
     for (int g = 0; g < 4; ++g) asm volatile("" : "+v"(lse[g]), "+v"(delta[g]));  // have come too: no wait for the next tile at their use
@@ -733,14 +747,14 @@ template <typename T, int D, bool TWO> __global__ __launch_bounds__(256, sizeof(
       if (lane == 0) *(lds_int*)(lds_char*)(uintptr_t)mine = !all;
       lds_barrier();
 #pragma unroll
-      for (int w = 0; w < 4; ++w) scrub = scrub || lds_load<int>(lds0 + 4 * TL::BYTES + HAND * w) != 0;
+      for (int w = 0; w < 4; ++w) scrub = scrub || lds_load<int>(hand + HAND * w) != 0;
       scrub = __builtin_amdgcn_readfirstlane(scrub);
       lds_barrier();
     }
-    if (it + a.parts < total) fetch(next_h, next_row0, buf ^ 1);
+    if (!TWO && it + a.parts < total) fetch(next_h, next_row0, buf ^ 1);
     const unsigned rows = row_addr + 2 * buf * TL::BYTES, cols = col_addr + 2 * buf * TL::BYTES;
     const auto active = [&](int q) { return row0 + 32 * q + 31 >= key0 && row0 + 32 * q < p.len; };  // some of these queries come after some of the keys
-    Frag8<T> pf[2], ds[2], pr[2], dr[2];
+    Frag8<T> pf[2], ds[2];
     if (active(qw)) {
       floatx16 sc, dp;
 #pragma unroll
@@ -770,10 +784,11 @@ template <typename T, int D, bool TWO> __global__ __launch_bounds__(256, sizeof(
         leave_frag<T>(mine + s * FRAG, pf[s], lane);
         leave_frag<T>(mine + (2 + s) * FRAG, ds[s], lane);
         if constexpr (TWO) {
-          rest_of(pr[s], sc, s, pf[s]);
-          rest_of(dr[s], dp, s, ds[s]);
-          leave_frag<T>(mine + (4 + s) * FRAG, pr[s], lane);
-          leave_frag<T>(mine + (6 + s) * FRAG, dr[s], lane);
+          Frag8<T> rest;
+          rest_of<true>(rest, sc, s, pf[s]);
+          leave_frag<T>(mine + (4 + s) * FRAG, rest, lane);
+          rest_of<false>(rest, dp, s, ds[s]);
+          leave_frag<T>(mine + (6 + s) * FRAG, rest, lane);
         }
       }
     }
@@ -784,42 +799,45 @@ template <typename T, int D, bool TWO> __global__ __launch_bounds__(256, sizeof(
       tile_finite<T, D, true>(gt(buf), wave, lane);
       lds_barrier();
     }
-    const auto add = [&](int half) {
+    const auto add = [&](int half, unsigned area) {
       const unsigned from = cols + 32 * half * TL::ROWB;
+      Frag8<T> pr[2], dr[2];
+      if constexpr (TWO)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          take_frag<T>(area + (4 + s) * FRAG, pr[s], lane);
+          take_frag<T>(area + (6 + s) * FRAG, dr[s], lane);
+        }
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int m = 0; m < M; ++m) {
-          mma(dv[m], TL::by_col(from, TL::BYTES + 16 * s * TL::ROWB, m), pf[s]);
-          mma(dk[m], TL::by_col(from, 16 * s * TL::ROWB, m), ds[s]);
+          const Frag8<T> g = TL::by_col(from, TL::BYTES + 16 * s * TL::ROWB, m);
+          mma(dv[m], g, pf[s]);
+          if constexpr (TWO) mma(dv[m], g, pr[s]);
+          const Frag8<T> q = TL::by_col(from, 16 * s * TL::ROWB, m);
+          mma(dk[m], q, ds[s]);
+          if constexpr (TWO) mma(dk[m], q, dr[s]);
         }
-      read_ahead<T, true, 4 * M, 4>();
-      if constexpr (TWO)
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-          for (int m = 0; m < M; ++m) {
-            mma(dv[m], TL::by_col(from, TL::BYTES + 16 * s * TL::ROWB, m), pr[s]);
-            mma(dk[m], TL::by_col(from, 16 * s * TL::ROWB, m), dr[s]);
-          }
+      read_ahead<T, true, 4 * M, 4, TWO ? 2 : 1>();
       if (scrub) {
         const auto keep = [&](int row) { return row >= key; };
         add_odd<T, M>(dv, at<T>(a.dout, a.gs, p.b, h, p.tok) + 32 * M * qw, a.gs[2], row0 + 32 * half, p.len, a.d - 32 * M * qw, pf, lane, keep);
         add_odd<T, M>(dk, at<T>(a.q, a.qs, p.b, h, p.tok) + 32 * M * qw, a.qs[2], row0 + 32 * half, p.len, a.d - 32 * M * qw, ds, lane, keep);
       }
     };
-    if (active(qw)) add(qw);
+    if (active(qw)) add(qw, mine);
     if (active(qw ^ 1)) {
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         take_frag<T>(theirs + s * FRAG, pf[s], lane);
         take_frag<T>(theirs + (2 + s) * FRAG, ds[s], lane);
-        if constexpr (TWO) {
-          take_frag<T>(theirs + (4 + s) * FRAG, pr[s], lane);
-          take_frag<T>(theirs + (6 + s) * FRAG, dr[s], lane);
-        }
       }
-      add(qw ^ 1);
+      add(qw ^ 1, theirs);
+    }
+    if (TWO && it + a.parts < total) {
+      lds_barrier();
+      fetch(next_h, next_row0, 0);
     }
     h = next_h;
     row0 = next_row0;
@@ -834,6 +852,14 @@ template <typename T, int D, bool TWO> __global__ __launch_bounds__(256, sizeof(
     store_column<float, M>(a.part + at_part * a.d + c0, dk, a.scale, a.d - c0, lane);
     store_column<float, M>(a.part + (at_part + rows_all) * a.d + c0, dv, 1.f, a.d - c0, lane);
   }
+}
+
+template <typename T, int D, bool MIXED> __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dkv_kernel(Args a) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const Place p = place(a, ROWS, 1, false);
+  if (!p.on) return;
+  if (MIXED && __builtin_amdgcn_readfirstlane(p.len) <= SHORT) dkv_block<T, D, MIXED>(a, p, lds);
+  else dkv_block<T, D, false>(a, p, lds);
 }
 
 int64_t blocks_of(const lnx_attn_args* a, int size) { return a->nseq ? (int64_t)a->T / size + a->nseq : ((int64_t)a->T + size - 1) / size; }
@@ -932,12 +958,12 @@ template <typename K> int start(K kernel, const char* name, const Args& a, int64
   return LNX_OK;
 }
 
-template <typename T, int D, bool TWO> int launch_fwd(const lnx_attn_args* a, hipStream_t st) {
+template <typename T, int D, bool MIXED> int launch_fwd(const lnx_attn_args* a, hipStream_t st) {
   Args k = kernel_args(a);
   k.nblk = (int)blocks_of(a, 128), k.parts = parts_of(a, QUERIES);
   const int64_t rows = (int64_t)k.B * k.H * k.T;
   k.part = static_cast<float*>(a->workspace), k.part_stat = k.part ? k.part + k.parts * rows * k.d : nullptr;
-  if (int rc = start(attn_fwd_kernel<T, D, TWO>, "attn_fwd", k, (int64_t)k.B * k.H * k.nblk * k.parts, 4 * Tile<T, D, fwd_rows<T, D>()>::BYTES + 16, st)) return rc;
+  if (int rc = start(attn_fwd_kernel<T, D, MIXED>, "attn_fwd", k, (int64_t)k.B * k.H * k.nblk * k.parts, 4 * Tile<T, D, fwd_rows<T, D>()>::BYTES + 16, st)) return rc;
   if (k.parts > 1) {
     lnx_profile_mark("attn_join", st);
     attn_join_kernel<T><<<dim3((unsigned)((rows + 15) / 16)), 256, 0, st>>>(k);
@@ -950,15 +976,15 @@ template <typename T> void sum_parts(const Args& k, const float* part, int64_t s
   attn_sum_kernel<T><<<dim3((unsigned)(((int64_t)k.B * heads * k.T + 15) / 16)), 256, 0, st>>>(part, k.parts, stride, static_cast<T*>(out), s[0], s[1], s[2], k.B, heads, k.T, k.d);
 }
 
-template <typename T, int D, bool TWO> int launch_bwd(const lnx_attn_args* a, hipStream_t st) {
+template <typename T, int D, bool MIXED> int launch_bwd(const lnx_attn_args* a, hipStream_t st) {
   Args k = kernel_args(a);
   k.delta = static_cast<float*>(a->workspace);
   k.part = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + delta_bytes(a));
   k.nblk = (int)blocks_of(a, 128), k.parts = parts_of(a, QUERIES);  // first: it leaves delta
-  if (int rc = start(attn_dq_kernel<T, D, TWO>, "attn_dq", k, (int64_t)k.B * k.H * k.nblk * k.parts, 4 * Tile<T, D>::BYTES + 16, st)) return rc;
+  if (int rc = start(attn_dq_kernel<T, D, MIXED>, "attn_dq", k, (int64_t)k.B * k.H * k.nblk * k.parts, 4 * Tile<T, D>::BYTES + 16, st)) return rc;
   if (k.parts > 1) sum_parts<T>(k, k.part, (int64_t)k.B * k.H * k.T, k.dq, k.dqs, k.H, st);
   k.nblk = (int)blocks_of(a, ROWS), k.parts = parts_of(a, DKV);
-  if (int rc = start(attn_dkv_kernel<T, D, TWO>, "attn_dkv", k, (int64_t)k.B * k.Hkv * k.nblk * k.parts, 4 * Tile<T, D>::BYTES + hand_over<T, TWO>(), st)) return rc;
+  if (int rc = start(attn_dkv_kernel<T, D, MIXED>, "attn_dkv", k, (int64_t)k.B * k.Hkv * k.nblk * k.parts, 4 * Tile<T, D>::BYTES + hand_over<T>(), st)) return rc;
   if (k.parts > 1) {
     const int64_t rows = (int64_t)k.B * k.Hkv * k.T;
     sum_parts<T>(k, k.part, 2 * rows, k.dk, k.dks, k.Hkv, st);
@@ -967,14 +993,14 @@ template <typename T, int D, bool TWO> int launch_bwd(const lnx_attn_args* a, hi
   return LNX_OK;
 }
 
-template <typename T, int D, bool TWO> int launch(const lnx_attn_args* a, bool bwd, hipStream_t st) { return bwd ? launch_bwd<T, D, TWO>(a, st) : launch_fwd<T, D, TWO>(a, st); }
+template <typename T, int D, bool MIXED> int launch(const lnx_attn_args* a, bool bwd, hipStream_t st) { return bwd ? launch_bwd<T, D, MIXED>(a, st) : launch_fwd<T, D, MIXED>(a, st); }
 
 int run(const char* what, const lnx_attn_args* a, bool bwd, hipStream_t st) {
   if (int rc = check(what, a, bwd)) return rc;
   if (a->B == 0 || a->T == 0) return LNX_OK;
   int rc;
   if (a->dtype == LNX_BF16) {
-    if (average_length(a) <= ROWS) rc = a->d <= 64 ? launch<bf16_t, 64, true>(a, bwd, st) : launch<bf16_t, 128, true>(a, bwd, st);
+    if (a->nseq || a->T <= SHORT) rc = a->d <= 64 ? launch<bf16_t, 64, true>(a, bwd, st) : launch<bf16_t, 128, true>(a, bwd, st);
     else rc = a->d <= 64 ? launch<bf16_t, 64, false>(a, bwd, st) : launch<bf16_t, 128, false>(a, bwd, st);
   } else {
     rc = a->d <= 64 ? launch<float, 64, false>(a, bwd, st) : launch<float, 128, false>(a, bwd, st);
@@ -1108,7 +1134,7 @@ template <typename T, int D> __global__ __launch_bounds__(64 * step_waves<T>(), 
     for (int s = 0; s < 2; ++s) {
       Frag8<T> pf, rest;
       from_acc(pf, sc, s);
-      rest_of(rest, sc, s, pf);
+      rest_of<true>(rest, sc, s, pf);
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
         const Frag8<T> v = TL::by_col(cols, TL::BYTES + 16 * s * TL::ROWB, i);

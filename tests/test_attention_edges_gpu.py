@@ -66,3 +66,30 @@ def test_step_cache_strides_of_single_elements(Hkv, S, dtype, more):
         return torch.empty(t.numel() + 64, device=DEV, dtype=t.dtype).as_strided(t.shape, strides).copy_(t)
 
     _check_step(q, k, v, odd(kc), odd(vc), [S - 1])
+
+
+# -- packed batches of short and long documents ---------------------------------------------------------------------
+
+@pytest.mark.parametrize("lens,H,Hkv,d", [([3, 300], 4, 2, 64), ([1, 2, 500], 8, 4, 64), ([2, 700, 5], 2, 1, 128), ([7, 0, 400, 1, 128], 4, 2, 80)], ids=str)
+def test_short_documents_beside_long_ones_are_as_exact_as_their_rounding(lens, H, Hkv, d):
+    """A document's operands go in in two parts by its own length, whatever it is packed with."""
+    cu = np.concatenate([[0], np.cumsum(lens)]).tolist()
+    q, k, v, do = _inputs(1, H, Hkv, cu[-1], d, "bf16")
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = la.causal_attention(*leaves, cu_seqlens=cu)
+    dq, dk, dv = torch.autograd.grad(o, leaves, do)
+    G = H // Hkv
+    nq, nk, nv, nd = (_np(t[0]) for t in (q, k, v, do))
+    for lo, hi in zip(cu[:-1], cu[1:]):
+        if not 0 < hi - lo <= 128:
+            continue
+        for kv in range(Hkv):
+            sums = {"dk": (0, 0), "dv": (0, 0)}
+            for h in range(kv * G, (kv + 1) * G):
+                ref = _reference(nq[h, lo:hi], nk[kv, lo:hi], nv[kv, lo:hi], nd[h, lo:hi], d ** -0.5, 2.0 ** -16)
+                _within(o[0, h, lo:hi], *ref["o"], f"o {lo}")
+                _within(dq[0, h, lo:hi], *ref["dq"], f"dq {lo}")
+                sums = {n: (sums[n][0] + ref[n][0], sums[n][1] + ref[n][1] + G * UP * ref[n][0].abs()) for n in sums}
+            _within(dk[0, kv, lo:hi], *sums["dk"], f"dk {lo}")
+            _within(dv[0, kv, lo:hi], *sums["dv"], f"dv {lo}")
+    _check(q, k, v, do, cu=cu)
