@@ -436,7 +436,8 @@ int lnx_linrec_step(const void* x, const void* g, const float* state, void* y, f
  *   u = RMSNorm(x) post_weight sigmoid(gate)    out = residual + scale u    z = RMSNorm(out) weight
  * post_weight NULL: x itself in place of its norm; gate NULL: no gate; residual NULL: out = scale u; z NULL: no second norm;
  * scale_vector [d] takes the place of `scale`.  x, gate, z and their gradients in `dtype`, residual, out and theirs in
- * `r_dtype` (LNX_F32 or `dtype`), weights and their gradients fp32.  z is the norm of the unrounded sum.  The backward call
+ * `r_dtype` (LNX_F32 or `dtype`), weights and their gradients fp32; with gate_f32 the gate and its gradient are fp32 beside any
+ * `dtype`.  z is the norm of the unrounded sum.  The backward call
  * reads the forward call's inputs; d_z and d_out may be NULL (zeros), d_residual, d_weight, d_post_weight and d_scale (the
  * vector's) may be NULL (not wanted); the last three are summed without atomics through the workspace
  * (16-byte aligned, like the workspaces below).
@@ -445,7 +446,7 @@ typedef struct lnx_rmsnorm_residual_args {
   int64_t rows;
   int32_t d, dtype, r_dtype;
   float scale, eps;
-  int32_t reserved;
+  int32_t gate_f32;
   const void* x;
   const void* residual;
   const void* gate;

@@ -86,7 +86,7 @@ class RmsnormResidualArgs(C.Structure):
 
     _fields_ = [
         ("rows", C.c_int64), ("d", C.c_int32), ("dtype", C.c_int32), ("r_dtype", C.c_int32), ("scale", C.c_float), ("eps", C.c_float),
-        ("reserved", C.c_int32),
+        ("gate_f32", C.c_int32),
         ("x", C.c_void_p), ("residual", C.c_void_p), ("gate", C.c_void_p), ("weight", C.c_void_p), ("post_weight", C.c_void_p),
         ("scale_vector", C.c_void_p), ("z", C.c_void_p), ("out", C.c_void_p), ("d_z", C.c_void_p), ("d_out", C.c_void_p), ("d_x", C.c_void_p),
         ("d_residual", C.c_void_p), ("d_gate", C.c_void_p), ("d_weight", C.c_void_p), ("d_post_weight", C.c_void_p), ("d_scale", C.c_void_p),

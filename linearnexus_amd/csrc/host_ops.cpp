@@ -68,6 +68,9 @@ at::ScalarType type_of(int64_t code) { return code == LNX_BF16 ? at::kBFloat16 :
 
 Tensor f32(const Tensor& t) { return t.defined() ? t.to(at::kFloat).contiguous() : t; }
 
+// A gate in x's type, or in float32 beside it
+Tensor gate_type(const Tensor& g, at::ScalarType x) { return g.scalar_type() == x ? g : g.to(at::kFloat); }
+
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : ts)
@@ -835,7 +838,7 @@ lnx_rmsnorm_residual_args around_args(const Around& n) {
   const int64_t d = n.x.size(-1);
   a.rows = n.x.numel() / d, a.d = (int32_t)d;
   a.dtype = code_of(n.x.scalar_type()), a.r_dtype = n.residual.defined() ? code_of(n.residual.scalar_type()) : a.dtype;
-  a.scale = (float)n.scale, a.eps = (float)n.eps;
+  a.scale = (float)n.scale, a.eps = (float)n.eps, a.gate_f32 = n.gate.defined() && n.gate.scalar_type() == at::kFloat;
   a.x = ptr(n.x), a.residual = ptr(n.residual), a.gate = ptr(n.gate), a.weight = fptr(n.weight), a.post_weight = fptr(n.post), a.scale_vector = fptr(n.scale_v);
   return a;
 }
@@ -853,9 +856,8 @@ struct AroundFn : Function<AroundFn> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x0, const OptT& residual0, const OptT& weight0, const OptT& post0, const OptT& gate0, const OptT& scale0,
                                double scale, double eps) {
     auto dense = [&](const OptT& t, at::ScalarType type) { return t.has_value() ? t->to(type).contiguous() : Tensor(); };
-    const auto dt = x0.scalar_type();
-    const Around n{x0.contiguous(), residual0.has_value() ? residual0->contiguous() : Tensor(), dense(gate0, dt), dense(weight0, at::kFloat), dense(post0, at::kFloat),
-                   dense(scale0, at::kFloat), scale, eps};
+    const Around n{x0.contiguous(), residual0.has_value() ? residual0->contiguous() : Tensor(), gate0.has_value() ? gate_type(*gate0, x0.scalar_type()).contiguous() : Tensor(),
+                   dense(weight0, at::kFloat), dense(post0, at::kFloat), dense(scale0, at::kFloat), scale, eps};
     auto [z, out] = around_forward(n);
     ctx->save_for_backward({n.x, n.residual, n.gate, n.weight, n.post, n.scale_v});
     auto kind = [](const OptT& t) { return (int64_t)(t.has_value() ? t->scalar_type() : at::kFloat); };
@@ -918,7 +920,7 @@ PyObject* py_rmsnorm_residual(PyObject*, PyObject* const* args, Py_ssize_t nargs
       const variable_list r = AroundFn::apply(x, opt(residual), opt(weight), opt(post), opt(gate), opt(scale_v), scale, eps);
       return {r.size() > 1 ? r[1] : Tensor(), r[0]};
     }
-    return around_forward({x.contiguous(), residual.defined() ? residual.contiguous() : residual, gate.defined() ? gate.to(x.scalar_type()).contiguous() : gate, f32(weight),
+    return around_forward({x.contiguous(), residual.defined() ? residual.contiguous() : residual, gate.defined() ? gate_type(gate, x.scalar_type()).contiguous() : gate, f32(weight),
                            f32(post), f32(scale_v), scale, eps});
   });
   return pack(r.first, r.second);
@@ -1262,8 +1264,6 @@ RecShape rec_shape(const char* op, const Tensor& x, const Tensor& g, const Tenso
               ") tensor, got ", s0.defined() ? shape_text(s0) : "");
   return s;
 }
-
-Tensor gate_type(const Tensor& g, at::ScalarType x) { return g.scalar_type() == x ? g : g.to(at::kFloat); }
 
 lnx_linrec_args rec_args(const RecShape& s, const Tensor& x, const Tensor& g, const Tensor& s0, const Tensor& cu) {
   lnx_linrec_args a{};

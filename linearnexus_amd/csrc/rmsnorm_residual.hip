@@ -118,7 +118,7 @@ template <int TPR> __device__ __forceinline__ void row_sum2(float& x, float& y, 
 
 constexpr int block_of(int tpr) { return tpr < 256 ? 256 : tpr; }
 
-template <typename T, typename S, int TPR, int K, bool VEC> __global__ __launch_bounds__(block_of(TPR)) void rmsnorm_residual_fwd_kernel(Args a) {
+template <typename T, typename S, typename G, int TPR, int K, bool VEC> __global__ __launch_bounds__(block_of(TPR)) void rmsnorm_residual_fwd_kernel(Args a) {
   constexpr int VN = Vec16<T>::N, RPB = block_of(TPR) / TPR, ES = VEC ? 1 : TPR;
   __shared__ float red[2][16];
   const int li = threadIdx.x % TPR;
@@ -126,7 +126,7 @@ template <typename T, typename S, int TPR, int K, bool VEC> __global__ __launch_
   if (row >= a.rows) return;  // whole waves: rows of one wave have no barrier
   const int64_t base = row * a.d;
   const T* x = static_cast<const T*>(a.x) + base;
-  const T* gate = a.gate ? static_cast<const T*>(a.gate) + base : nullptr;
+  const G* gate = a.gate ? static_cast<const G*>(a.gate) + base : nullptr;
   const S* r = a.r ? static_cast<const S*>(a.r) + base : nullptr;
   float xv[K][VN], rv[K][VN], gv[K][VN], ss = 0.f;
 #pragma unroll
@@ -137,7 +137,7 @@ template <typename T, typename S, int TPR, int K, bool VEC> __global__ __launch_
     if (left > 0) {
       load_row<T, VN, ES>(x + c, left, xv[k]);
       if (r) load_row<S, VN, ES>(r + c, left, rv[k]);
-      if (gate) load_row<T, VN, ES>(gate + c, left, gv[k]);
+      if (gate) load_row<G, VN, ES>(gate + c, left, gv[k]);
     }
   }
   float rho = 1.f;
@@ -184,7 +184,7 @@ template <typename T, typename S, int TPR, int K, bool VEC> __global__ __launch_
 }
 
 // Rows blockIdx, blockIdx + gridDim, ...; the next row is on its way while one is worked on.
-template <typename T, typename S, int TPR, int K, bool VEC> __global__ __launch_bounds__(block_of(TPR)) void rmsnorm_residual_bwd_kernel(Args a) {
+template <typename T, typename S, typename G, int TPR, int K, bool VEC> __global__ __launch_bounds__(block_of(TPR)) void rmsnorm_residual_bwd_kernel(Args a) {
   constexpr int VN = Vec16<T>::N, RPB = block_of(TPR) / TPR, C = TPR * K * VN, ES = VEC ? 1 : TPR;
   __shared__ float red[2][3][32];
   const int li = threadIdx.x % TPR, sub = threadIdx.x / TPR;
@@ -205,7 +205,8 @@ template <typename T, typename S, int TPR, int K, bool VEC> __global__ __launch_
       }
     }
   }
-  RawRow<T, VN, ES> xr[K], gr[K], zr[K];
+  RawRow<T, VN, ES> xr[K], zr[K];
+  RawRow<G, VN, ES> gr[K];
   RawRow<S, VN, ES> rr[K], orr[K];
   auto fetch = [&](int64_t row) {
     const int64_t base = row * a.d;
@@ -216,7 +217,7 @@ template <typename T, typename S, int TPR, int K, bool VEC> __global__ __launch_
       xr[k].load(static_cast<const T*>(a.x) + at, left);
       if (a.r) rr[k].load(static_cast<const S*>(a.r) + at, left);
       else rr[k].zero();
-      if (a.gate) gr[k].load(static_cast<const T*>(a.gate) + at, left);
+      if (a.gate) gr[k].load(static_cast<const G*>(a.gate) + at, left);
       else gr[k].zero();
       if (a.dz) zr[k].load(static_cast<const T*>(a.dz) + at, left);
       else zr[k].zero();
@@ -280,7 +281,7 @@ template <typename T, typename S, int TPR, int K, bool VEC> __global__ __launch_
         dg[e] = ov[k][e] * xn * (1.f - sg[k][e]);
         dot += ov[k][e] * xv[k][e];
       }
-      if (a.dgate && left > 0) store_row<T, VN, ES>(static_cast<T*>(a.dgate) + base + c, left, dg);
+      if (a.dgate && left > 0) store_row<G, VN, ES>(static_cast<G*>(a.dgate) + base + c, left, dg);
     }
     float m = 0.f;
     if (a.post) m = row_sum<TPR>(dot, red[turn][2]) * a.inv_d * rho * rho;
@@ -388,25 +389,25 @@ int bwd_blocks(int64_t rows, const Plan& p) {
   return (int)(all < 768 ? all : 768);
 }
 
-template <typename T, typename S, int TPR, int K> void launch(const Args& a, bool vec, bool bwd, int blocks, hipStream_t st) {
+template <typename T, typename S, typename G, int TPR, int K> void launch(const Args& a, bool vec, bool bwd, int blocks, hipStream_t st) {
   const int wide = blocks < 1 << 22 ? blocks : 1 << 22;  // a launch takes 2^32 threads in one direction
   const dim3 g((unsigned)wide, (unsigned)((blocks + wide - 1) / wide)), b(block_of(TPR));
   if (bwd) {
-    if (vec) rmsnorm_residual_bwd_kernel<T, S, TPR, K, true><<<g, b, 0, st>>>(a);
-    else rmsnorm_residual_bwd_kernel<T, S, TPR, K, false><<<g, b, 0, st>>>(a);
+    if (vec) rmsnorm_residual_bwd_kernel<T, S, G, TPR, K, true><<<g, b, 0, st>>>(a);
+    else rmsnorm_residual_bwd_kernel<T, S, G, TPR, K, false><<<g, b, 0, st>>>(a);
   } else {
-    if (vec) rmsnorm_residual_fwd_kernel<T, S, TPR, K, true><<<g, b, 0, st>>>(a);
-    else rmsnorm_residual_fwd_kernel<T, S, TPR, K, false><<<g, b, 0, st>>>(a);
+    if (vec) rmsnorm_residual_fwd_kernel<T, S, G, TPR, K, true><<<g, b, 0, st>>>(a);
+    else rmsnorm_residual_fwd_kernel<T, S, G, TPR, K, false><<<g, b, 0, st>>>(a);
   }
 }
 
-template <typename T, typename S> void pick(const Args& a, const Plan& p, bool vec, bool bwd, int blocks, hipStream_t st) {
-  if (p.tpr == 64 && p.k == 1) launch<T, S, 64, 1>(a, vec, bwd, blocks, st);
-  else if (p.tpr == 64) launch<T, S, 64, 2>(a, vec, bwd, blocks, st);
-  else if (p.tpr == 256 && p.k == 1) launch<T, S, 256, 1>(a, vec, bwd, blocks, st);
-  else if (p.tpr == 256) launch<T, S, 256, 2>(a, vec, bwd, blocks, st);
-  else if (p.k == 2) launch<T, S, 512, 2>(a, vec, bwd, blocks, st);
-  else if constexpr (sizeof(T) == 4) launch<T, S, 512, 4>(a, vec, bwd, blocks, st);
+template <typename T, typename S, typename G> void pick(const Args& a, const Plan& p, bool vec, bool bwd, int blocks, hipStream_t st) {
+  if (p.tpr == 64 && p.k == 1) launch<T, S, G, 64, 1>(a, vec, bwd, blocks, st);
+  else if (p.tpr == 64) launch<T, S, G, 64, 2>(a, vec, bwd, blocks, st);
+  else if (p.tpr == 256 && p.k == 1) launch<T, S, G, 256, 1>(a, vec, bwd, blocks, st);
+  else if (p.tpr == 256) launch<T, S, G, 256, 2>(a, vec, bwd, blocks, st);
+  else if (p.k == 2) launch<T, S, G, 512, 2>(a, vec, bwd, blocks, st);
+  else if constexpr (sizeof(T) == 4) launch<T, S, G, 512, 4>(a, vec, bwd, blocks, st);
 }
 
 int run(const char* what, const lnx_rmsnorm_residual_args* q, bool bwd, hipStream_t st) {
@@ -441,9 +442,10 @@ int run(const char* what, const lnx_rmsnorm_residual_args* q, bool bwd, hipStrea
     blocks = bwd ? bwd_blocks(q->rows, p) : (int)((q->rows + rpb - 1) / rpb);
     if (params) a.dw = static_cast<float*>(q->workspace);
     lnx_profile_mark(what, st);
-    if (q->dtype == LNX_F32) pick<float, float>(a, p, vec, bwd, blocks, st);
-    else if (q->r_dtype == LNX_F32) pick<bf16_t, float>(a, p, vec, bwd, blocks, st);
-    else pick<bf16_t, bf16_t>(a, p, vec, bwd, blocks, st);
+    const bool wide = q->gate && q->gate_f32;  // a gate of its own type beside bf16
+    if (q->dtype == LNX_F32) pick<float, float, float>(a, p, vec, bwd, blocks, st);
+    else if (q->r_dtype == LNX_F32) wide ? pick<bf16_t, float, float>(a, p, vec, bwd, blocks, st) : pick<bf16_t, float, bf16_t>(a, p, vec, bwd, blocks, st);
+    else wide ? pick<bf16_t, bf16_t, float>(a, p, vec, bwd, blocks, st) : pick<bf16_t, bf16_t, bf16_t>(a, p, vec, bwd, blocks, st);
   }
   if (params) {
     lnx_profile_mark("rmsnorm_residual_sums", st);

@@ -32,6 +32,6 @@ def rmsnorm_residual(x: Tensor, residual: Optional[Tensor], weight: Optional[Ten
 
     Norms are over the last dimension (at most 8192 wide).  ``post_weight=None``: x itself takes the place of its norm; ``gate=None``: no
     gate; ``residual=None``: ``r = scale * u`` (the first block); ``weight=None``: z is None (behind the last block).  ``scale`` is a number
-    or a ``[d]`` tensor.  ``x, gate [..., d]`` and z are float32 or bfloat16, the residual and r float32 or x's dtype; z is the norm of
-    the sum before it is rounded to r's dtype.  Differentiable with respect to every tensor."""
+    or a ``[d]`` tensor.  ``x [..., d]`` and z are float32 or bfloat16, the residual and r float32 or x's dtype, the gate likewise (one of
+    another type is taken in float32); z is the norm of the sum before it is rounded to r's dtype.  Differentiable with respect to every tensor."""
     return _lib.host().rmsnorm_residual(x, residual, weight, post_weight, gate, scale, eps)

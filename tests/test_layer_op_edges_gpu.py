@@ -1,8 +1,9 @@
-"""The gated linear recurrence at its edges."""
+"""The gated linear recurrence and the residual norm at their edges."""
 import pytest
 import torch
 
 import linearnexus_amd as la
+from test_rmsnorm_residual_gpu import _np as _npy, _reference as _norm_reference, _within as _norm_within
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -29,3 +30,38 @@ def test_one_token_of_a_sequence_first_batch(dtype):
     for got, ref, mag, last in ((y[:, 0], e * s0 + xd, (e * s0).abs() + xd.abs(), eps), (state, e * s0 + xd, (e * s0).abs() + xd.abs(), 0),
                                 (dg[:, 0], e * s0 * dyd, (e * s0 * dyd).abs(), 0), (ds, e * dyd, (e * dyd).abs(), 0)):
         assert bool(((got.double() - ref).abs() <= 2.0 ** -21 * mag + last * (ref.abs() + 2.0 ** -21 * mag) + 1e-36).all())
+
+
+# -- residual norm: a gate in float32 beside bfloat16 ------------------------------------------------------------------
+
+@pytest.mark.parametrize("r_dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,d", [(5, 33), (7, 64), (3, 512), (9, 1000), (4, 1024), (6, 2048), (3, 3001), (2, 4096), (2, 8192), (1500, 264)])
+def test_gate_keeps_its_type(rows, d, r_dtype):
+    """Neither the gate nor its gradient is rounded to x's type: both are what the formula gives, in float32."""
+    g = torch.Generator().manual_seed(rows + d)
+    n = lambda *s, t=torch.float32, std=1.0: (torch.randn(*s, generator=g) * std).to(DEV, t)
+    x, r, gate, w, post = n(rows, d, t=torch.bfloat16), n(rows, d, t=DT[r_dtype], std=2.0), n(rows, d, std=2.0), 1 + n(d, std=0.3), 1 + n(d, std=0.3)
+    dz, do = n(rows, d, t=torch.bfloat16), n(rows, d, t=DT[r_dtype])
+    leaves = [t.detach().requires_grad_() for t in (x, r, w, post, gate)]
+    z, out = la.rmsnorm_residual(leaves[0], leaves[1], leaves[2], leaves[3], leaves[4], 0.7)
+    grads = torch.autograd.grad([z, out], leaves, [dz, do])
+    ref = _norm_reference(_npy(x), _npy(r), _npy(w), _npy(post), _npy(gate), 0.7, _npy(dz), _npy(do))
+    _norm_within(z, ref["z"], "z")
+    _norm_within(out, ref["r"], "r")
+    for got, name in zip(grads, ("dx", "dr", "dw", "dpost", "dgate")):
+        _norm_within(got, ref[name], name)
+    with torch.no_grad():
+        z2, out2 = la.rmsnorm_residual(x, r, w, post, gate, 0.7)
+    assert torch.equal(z2, z) and torch.equal(out2, out) and grads[4].dtype == torch.float32
+
+
+def test_gates_of_other_types():
+    """A float16 gate is exact in float32, a float64 one is rounded to it."""
+    g = torch.Generator().manual_seed(1)
+    x, gate = torch.randn(6, 128, generator=g).to(DEV, torch.bfloat16), torch.randn(6, 128, generator=g).to(DEV)
+    for t in (torch.float16, torch.float64):
+        other = gate.to(t).requires_grad_()
+        _, out = la.rmsnorm_residual(x, None, None, None, other)
+        _, want = la.rmsnorm_residual(x, None, None, None, other.detach().float())
+        assert torch.equal(out, want)
+        assert torch.autograd.grad(out, other, torch.ones_like(out))[0].dtype == t
