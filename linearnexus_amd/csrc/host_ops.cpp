@@ -1424,8 +1424,12 @@ lnx_attn_args attention_args(const Tensor& q, const Tensor& k, const Tensor& v, 
 
 Tensor empty_rows(const Tensor& like, bool token_first) { return empty_layout(like.size(0), like.size(1), like.size(2), like.size(3), like.options(), token_first); }
 
+// Whether a token's heads lie closer together than a head's tokens: q in [B, T, H, d] memory, or a slice of a wider projection
+bool tokens_outside(const Tensor& q) { return q.size(1) > 1 && q.size(2) > 1 && q.stride(1) > 0 && q.stride(1) < q.stride(2); }
+
+// o lies in memory as q does: [B, T, H, d] or [B, H, T, d]
 Tensor attention_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu, double scale, const Tensor& lse, const Tensor& low) {
-  const Tensor o = empty_rows(q, is_token_first(q));
+  const Tensor o = empty_rows(q, tokens_outside(q));
   lnx_attn_args a = attention_args(q, k, v, o, cu, scale);
   a.lse = fptr(lse), a.o_low = ptr(low);
   a.workspace_bytes = lnx_attn_fwd_workspace_bytes(&a);
@@ -1478,10 +1482,15 @@ PyObject* py_causal_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs
   return THPVariable_Wrap(without_lock([&] {
     const int64_t d = q.size(3), more = (8 - d % 8) % 8;  // zero columns change no product
     if (wants_grad({&q, &k, &v})) refuse_live_graph(op, {&q, &k, &v});
-    auto wide = [&](const Tensor& t) { return more ? at::constant_pad_nd(t, {0, more}) : t; };
+    const bool outside = tokens_outside(q);
+    auto wide = [&](const Tensor& t) {  // in t's memory order, which a padded copy of a view would lose
+      if (!more) return t;
+      return tokens_outside(t) ? at::constant_pad_nd(t.transpose(1, 2), {0, more}).transpose(1, 2) : at::constant_pad_nd(t, {0, more});
+    };
     const Tensor qw = wide(q), kw = wide(k), vw = wide(v);
     const Tensor o = wants_grad({&q, &k, &v}) ? AttentionFn::apply(qw, kw, vw, opt(cu), scale) : attention_forward(as_rows(qw), as_rows(kw), as_rows(vw), cu, scale, Tensor(), Tensor());
-    return more ? o.narrow(3, 0, d).contiguous() : o;
+    if (!more) return o;
+    return outside ? o.transpose(1, 2).narrow(3, 0, d).contiguous().transpose(1, 2) : o.narrow(3, 0, d).contiguous();
   }));
   LNX_END
 }

@@ -93,3 +93,21 @@ def test_short_documents_beside_long_ones_are_as_exact_as_their_rounding(lens, H
             _within(dk[0, kv, lo:hi], *sums["dk"], f"dk {lo}")
             _within(dv[0, kv, lo:hi], *sums["dv"], f"dv {lo}")
     _check(q, k, v, do, cu=cu)
+
+
+# -- memory order ---------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("d", [20, 33, 64, 80])
+@pytest.mark.parametrize("how", ["head first", "token first", "slice of a projection"])
+def test_results_lie_as_the_queries_do(how, d):
+    B, T, H = 2, 9, 4
+    q, k, v, do = _inputs(B, H, 2, T, d, "bf16", token_first=how != "head first")
+    if how == "slice of a projection":
+        q = torch.cat([q.transpose(1, 2).flatten(2), torch.zeros(B, T, 48, device=DEV, dtype=q.dtype)], 2)[..., : H * d].unflatten(2, (H, d)).transpose(1, 2)
+    with torch.no_grad():
+        o = la.causal_attention(q, k, v)
+    leaf = q.detach().requires_grad_()
+    graded = la.causal_attention(leaf, k, v)
+    for t in (o, graded):
+        assert (t if how == "head first" else t.transpose(1, 2)).is_contiguous() and torch.equal(t, o)
+    _check(q, k, v, do)
