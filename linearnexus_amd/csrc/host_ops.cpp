@@ -9,6 +9,7 @@
 #include <torch/extension.h>
 
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <c10/core/DeviceGuard.h>
@@ -21,6 +22,7 @@
 #include <stdexcept>
 #include <string>
 #include <tuple>
+#include <unordered_set>
 #include <vector>
 
 #include "../../include/linearnexus_hip.h"
@@ -109,7 +111,36 @@ void refuse_live_graph(const char* op, std::initializer_list<const Tensor*> ts) 
     if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
     const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
     const auto stream = node ? node->stream() : std::nullopt;
-    TORCH_CHECK(!stream || stream->id() != eager, op, ": a graph of this leaf from the default stream is alive while this pass is captured; let go of its outputs first, or run it on another stream");
+    TORCH_CHECK(!stream || stream->id() != eager, op, ": a graph of this leaf from the default stream is alive while this pass is captured; let go of its outputs first, run it on another stream, or "
+                "capture under torch.no_grad() where no gradient is wanted");
+  }
+}
+
+// The same for what lies behind other operations, asked when the captured backward pass of an op begins: nothing that this pass will run
+// behind it may belong to the default stream -- no leaf that a live graph holds, no operation that ran before the capture.
+void refuse_live_graph_behind(const char* op, const Tensor& like) {
+  if (!capturing(like)) return;
+  const auto self = torch::autograd::get_current_node();
+  if (!self) return;
+  const c10::StreamId eager = c10::hip::getDefaultHIPStream(like.get_device()).id();
+  const auto* runs = torch::autograd::get_current_graph_task_exec_info();  // empty: everything
+  std::vector<torch::autograd::Node*> todo{self.get()};
+  std::unordered_set<torch::autograd::Node*> seen{self.get()};
+  while (!todo.empty()) {
+    torch::autograd::Node* node = todo.back();
+    todo.pop_back();
+    for (const torch::autograd::Edge& e : node->next_edges()) {
+      torch::autograd::Node* next = e.function.get();
+      if (!next || !seen.insert(next).second) continue;
+      if (runs && !runs->empty()) {
+        const auto it = runs->find(next);
+        if (it == runs->end() || !it->second.should_execute()) continue;
+      }
+      const auto stream = next->stream();
+      TORCH_CHECK(!stream || stream->id() != eager, op, ": a graph from the default stream is alive behind this pass (", next->name(),
+                  ") while it is captured; let go of its outputs first, or run it on another stream");
+      todo.push_back(next);
+    }
   }
 }
 
@@ -871,6 +902,7 @@ struct AroundFn : Function<AroundFn> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     refuse_tangents("the gradient of rmsnorm_residual", grads);
     const variable_list s = ctx->get_saved_variables();
+    refuse_live_graph_behind("the gradient of rmsnorm_residual", s[0]);
     const std::vector<int64_t> m = ctx->saved_data["i"].toIntVector();
     const std::vector<double> sc = ctx->saved_data["d"].toDoubleVector();
     const Around n{s[0], s[1], s[2], s[3], s[4], s[5], sc[0], sc[1]};
@@ -1302,6 +1334,7 @@ struct RecFn : Function<RecFn> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     refuse_tangents("the gradient of gated_linear_recurrence", grads);
     const variable_list sv = ctx->get_saved_variables();
+    refuse_live_graph_behind("the gradient of gated_linear_recurrence", sv[0]);
     const std::vector<int64_t> m = ctx->saved_data["i"].toIntVector();
     const Tensor &x = sv[0], &g = sv[1], &cu = sv[2], &kept = sv[3];
     const RecShape s{m[0], m[1], m[2], m[3], m[4]};
@@ -1453,6 +1486,7 @@ struct AttentionFn : Function<AttentionFn> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     refuse_tangents("the gradient of causal_attention", grads);
     const variable_list s = ctx->get_saved_variables();
+    refuse_live_graph_behind("the gradient of causal_attention", s[0]);
     const Tensor &q = s[0], &k = s[1], &v = s[2], &o = s[3], &lse = s[4], &cu = s[5];
     const Tensor d_o = as_rows(grads[0].to(q.scalar_type()));
     Tensor dq = empty_rows(q, is_token_first(q)), dk = empty_rows(k, is_token_first(k)), dv = empty_rows(v, is_token_first(v));

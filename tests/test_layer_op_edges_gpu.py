@@ -1,4 +1,4 @@
-"""The gated linear recurrence and the residual norm at their edges."""
+"""The gated linear recurrence and the residual norm at their edges; captured passes of both and of attention."""
 import pytest
 import torch
 
@@ -65,3 +65,52 @@ def test_gates_of_other_types():
         _, want = la.rmsnorm_residual(x, None, None, None, other.detach().float())
         assert torch.equal(out, want)
         assert torch.autograd.grad(out, other, torch.ones_like(out))[0].dtype == t
+
+
+# -- captured passes ----------------------------------------------------------------------------------------------------
+
+CALLS = {
+    "recurrence": lambda x, c: la.gated_linear_recurrence(x, c)[0],
+    "norm": lambda x, c: la.rmsnorm_residual(x, None, c)[0],
+    "attention": lambda x, c: la.causal_attention(x, x, x),
+}
+
+
+def _leaf_and_constant(name):
+    if name == "attention":
+        return torch.randn(1, 1, 40, 64, device=DEV, requires_grad=True), None
+    return torch.randn(1, 40, 64, device=DEV, requires_grad=True), -torch.ones(1, 40, 64, device=DEV) if name == "recurrence" else torch.ones(64, device=DEV)
+
+
+@pytest.mark.parametrize("name", list(CALLS))
+def test_a_leaf_behind_another_operation_is_seen(name):
+    """The leaf's gradient would be added on the default stream, which cannot join the capture: the captured backward pass is refused."""
+    leaf, c = _leaf_and_constant(name)
+    free = torch.randn_like(leaf, requires_grad=True)
+    alive = leaf * 2.0
+    keep = torch.zeros(8, device=DEV)
+    ones = torch.ones_like(leaf)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        keep.add_(1)
+        out = CALLS[name](leaf * 3.0 + free, c)
+        with pytest.raises(RuntimeError, match="alive"):
+            torch.autograd.grad(out, leaf, ones, retain_graph=True)
+        with pytest.raises(RuntimeError, match="alive"):
+            out.backward(ones, retain_graph=True)
+        grad, = torch.autograd.grad(out, free, ones)  # does not touch the other leaf
+    assert leaf.grad is None
+    want, = torch.autograd.grad(CALLS[name]((leaf * 3.0).detach() + free, c), free, ones)
+    for i in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert bool((keep == i + 1).all()) and torch.equal(grad, want)
+    del alive, out
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grad, = torch.autograd.grad(CALLS[name](leaf * 3.0 + free.detach(), c), leaf, ones)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(grad, 3.0 * want)
