@@ -144,6 +144,12 @@ void refuse_live_graph_behind(const char* op, const Tensor& like) {
   }
 }
 
+// A tensor that a kernel has written in place counts as written: a graph that saved it refuses to go backwards, as after torch's own
+// in-place operations.  (Tensors of inference mode have no version.)
+void written(const Tensor& t) {
+  if (!t.is_inference()) torch::autograd::impl::bump_version(t);
+}
+
 // Tensors of one call lie on one GPU; a tensor that is absent is not asked.
 void check_devices(const char* op, const Tensor& first, std::initializer_list<std::pair<const char*, const Tensor*>> rest) {
   for (const auto& [name, t] : rest)
@@ -1394,6 +1400,7 @@ PyObject* py_linrec_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     const c10::DeviceGuard guard(x.device());
     check_status(lnx_linrec_step(ptr(xc), ptr(gc), fptr(si), ptr(y), fptr(so), xc.numel(), code_of(xc.scalar_type()), code_of(gc.scalar_type()), stream_of(xc)),
                  "lnx_linrec_step");
+    if (inplace) written(state);
     return {y, so};
   });
   return pack(r.first, r.second);
@@ -1564,6 +1571,8 @@ PyObject* py_causal_attention_step(PyObject*, PyObject* const* args, Py_ssize_t 
     a.workspace = ptr(ws);
     const c10::DeviceGuard guard(q.device());
     check_status(lnx_attn_step(&a, stream_of(q)), "lnx_attn_step");
+    written(kc);
+    written(vc);
     return o;
   }));
   LNX_END

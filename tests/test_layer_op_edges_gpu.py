@@ -1,4 +1,4 @@
-"""The gated linear recurrence and the residual norm at their edges; captured passes of both and of attention."""
+"""The gated linear recurrence and the residual norm at their edges; captured passes and in-place steps of both and of attention."""
 import pytest
 import torch
 
@@ -114,3 +114,43 @@ def test_a_leaf_behind_another_operation_is_seen(name):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(grad, 3.0 * want)
+
+
+# -- steps in place count as writes -------------------------------------------------------------------------------------
+
+def _attention_step(kc, vc):
+    q, k, v = (torch.randn(2, h, 64, device=DEV) for h in (4, 2, 2))
+    la.causal_attention_step(q, k, v, kc, vc, torch.zeros(2, dtype=torch.int32, device=DEV))
+
+
+@pytest.mark.parametrize("which", ["state", "k_cache", "v_cache"])
+def test_what_a_step_overwrites_is_no_longer_what_was_saved(which):
+    if which == "state":
+        buf = torch.randn(3, 64, device=DEV)
+        write = lambda: la.gated_linear_recurrence_step(torch.randn(3, 64, device=DEV), -torch.ones(3, 64, device=DEV), buf, inplace=True)
+    else:
+        buf, other = torch.randn(2, 2, 5, 64, device=DEV), torch.randn(2, 2, 5, 64, device=DEV)
+        write = lambda: _attention_step(*((buf, other) if which == "k_cache" else (other, buf)))
+    w = torch.ones_like(buf, requires_grad=True)
+    saved = (w * buf[:]).sum()  # a view of it is saved
+    before = buf._version
+    write()
+    assert buf._version == before + 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        saved.backward()
+    again = (w * buf).sum()
+    again.backward()
+    assert torch.equal(w.grad, buf)
+
+
+def test_steps_in_inference_mode():
+    with torch.inference_mode():
+        state = torch.randn(3, 64, device=DEV)
+        caches = [torch.randn(2, 2, 5, 64, device=DEV) for _ in "kv"]
+        for _ in range(2):
+            la.gated_linear_recurrence_step(state, -torch.ones_like(state), state, inplace=True)
+            _attention_step(*caches)
+    with torch.no_grad():  # tensors of inference mode have no version to count
+        la.gated_linear_recurrence_step(torch.ones(3, 64, device=DEV), -torch.ones(3, 64, device=DEV), state, inplace=True)
+        _attention_step(*caches)
+    assert bool(torch.isfinite(state).all())
