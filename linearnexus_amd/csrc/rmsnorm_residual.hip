@@ -289,7 +289,7 @@ template <typename T, typename S, typename G, int TPR, int K, bool VEC> __global
     for (int k = 0; k < K; ++k) {
       const int c = first_column<TPR, VN, ES>(k, li), left = a.d - c;
 #pragma unroll
-      for (int e = 0; e < VN; ++e) ov[k][e] = rho * (ov[k][e] - xv[k][e] * m);
+      for (int e = 0; e < VN; ++e) ov[k][e] = a.post ? rho * (ov[k][e] - xv[k][e] * m) : ov[k][e];  // (an infinite x times m = 0 is no 0)
       if (left > 0) store_row<T, VN, ES>(static_cast<T*>(a.dx) + base + c, left, ov[k]);
     }
   }

@@ -67,6 +67,19 @@ def test_gates_of_other_types():
         assert torch.autograd.grad(out, other, torch.ones_like(out))[0].dtype == t
 
 
+# -- residual norm: without a norm behind the block an infinite x is like any other -------------------------------------
+
+@pytest.mark.parametrize("d", [64, 65, 1000])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_infinite_x_without_a_norm_has_a_finite_gradient(dtype, d):
+    x, r, do = torch.ones(3, d, device=DEV, dtype=DT[dtype]), torch.zeros(3, d, device=DEV), torch.full((3, d), 2.0, device=DEV)
+    x[1, 5], x[2, 7] = float("inf"), float("nan")
+    leaf = x.requires_grad_()
+    z, out = la.rmsnorm_residual(leaf, r, torch.ones(d, device=DEV), None, None, 0.5)
+    assert torch.isinf(out[1, 5]) and torch.isnan(out[2, 7])
+    assert torch.equal(torch.autograd.grad(out, leaf, do)[0], torch.ones_like(x))
+
+
 # -- captured passes ----------------------------------------------------------------------------------------------------
 
 CALLS = {
