@@ -15,6 +15,7 @@
 // No atomics: dk and dv are summed over the group's query heads by the workgroup that owns the keys, dq by a kernel of its own.
 #include "lnx_common.h"
 #include "mma_tiles.h"
+#include "packed_slots.h"
 
 namespace {
 

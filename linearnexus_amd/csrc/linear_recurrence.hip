@@ -19,6 +19,7 @@
 // timing, results are the same from run to run.  (With states every 32 tiles each was a wait for the one before: 3.7 us in a row.)
 #include "lnx_common.h"
 #include "mma_tiles.h"
+#include "packed_slots.h"
 
 namespace {
 

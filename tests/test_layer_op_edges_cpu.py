@@ -1,5 +1,9 @@
-"""Strides of dimensions of one element at the C boundary, without a GPU.  Every call below is
+"""Strides of dimensions of one element at the C boundary, and the records of the kernels' traffic, without a GPU.  Every call below is
 refused for another reason behind the strides' check, so that nothing is launched."""
+import json
+import os
+
+from conftest import ROOT
 from linearnexus_amd import _lib
 from test_layer_ops_cpu import _attn, _ptr, _refused
 
@@ -52,3 +56,15 @@ def test_recurrence_stride_of_a_single_token():
     a.T = 2
     for fn in (lib.lnx_linrec_fwd, lib.lnx_linrec_bwd):
         _refused(fn(a, None), -2, b"apart")
+
+
+def test_recorded_traffic_is_of_the_sources():
+    """profiles/traffic.json is quoted only while the sources hash to what was measured.  Who changes one of them measures its kernels again or
+    drops the entry; what only other kernels use belongs into a header of its own."""
+    import bench
+
+    with open(os.path.join(ROOT, "profiles", "traffic.json")) as f:
+        entries = json.load(f)["measurements"]
+    assert entries
+    for e in entries:
+        assert bench.sources_sha256(e["sources"]) == e["sources_sha256"], (e["commit"], e["sources"])
