@@ -6,12 +6,16 @@
 // the dk / dv kernel -- whose vectors stay in registers as B operands, and the rows that it walks over lie in LDS, read by rows for
 // the products over the head dimension and through transposing reads for the products over the rows.  A score fragment holds one
 // column per lane and half, so maxima and sums are within the lane and one exchange of the wave's halves.
-// Tiles of 64 rows come in through loads that go straight to LDS, the next tile behind the one being multiplied, one barrier a tile.
+// Tiles of 64 rows (32 in the bf16 forward kernel at d > 64) come in through loads that go straight to LDS, the next tile behind the one being
+// multiplied, one barrier a tile.
 // bf16 takes v_mfma_f32_32x32x16_bf16 (probabilities and score gradients are rounded to bf16 as operands: at most 2^-8 of each term, what
-// the outputs are rounded to), fp32 takes v_mfma_f32_32x32x2_f32 throughout.  Sums, maxima and accumulators are fp32.
+// the outputs are rounded to; all in all 0.0024 of the norm for a training step and 0.0021 for a prompt, where the rounding of the results alone
+// is 0.0017 and 0.0016; in two parts, a third of the products more, it is that alone: see SHORT), fp32 takes v_mfma_f32_32x32x2_f32
+// throughout.  Sums, maxima and accumulators are fp32.
 // Bound by the matrix cores and the exponentials beside them: at B2 H16/4 T4096 d128 bf16 the forward kernel takes 147-164 us (840-930
-// TFLOP/s of the causal half; matrix cores busy 41 %, vector instructions 41 % of the time), dq 194-217 (950-1060), dk / dv 311-343
-// (800-880) and the two sums of its parts 7 each, where a large library product reaches 1200.
+// TFLOP/s of the causal half), dq 194-217, dk / dv 311-343 and the two sums of its parts 7 each, together 600-650 TFLOP/s of the 10 d operations a
+// pair that the gradient needs (scores and do . v are formed in both kernels, 14 d in all), where a large library product reaches 1200.  Matrix cores
+// are busy 44, 45 and 36 % of the time, vector instructions 50, 33 and 26 %.
 // No atomics: dk and dv are summed over the group's query heads by the workgroup that owns the keys, dq by a kernel of its own.
 #include "lnx_common.h"
 #include "mma_tiles.h"
@@ -40,7 +44,6 @@ template <typename T> struct Frag8;
 template <> struct Frag8<bf16_t> {
   bf16x8 v;
   __device__ __forceinline__ void zero() { v = vec_zero<bf16_t>(); }
-  __device__ __forceinline__ bf16_t get(int j) const { return v[j]; }
 };
 template <> struct Frag8<float> {
   float v[8];
@@ -150,7 +153,7 @@ template <typename T, int D, int R = ROWS> struct Mover {
       off[i] = (unsigned)((r * (int)st + c) * (int)sizeof(T));
     }
   }
-  // rows row0 .. row0 + 63; rows behind the last are copies of the last, columns behind d keep the zeros that clear_lds left
+  // rows row0 .. row0 + R - 1; rows behind the last are copies of the last, columns behind d keep the zeros that clear_lds left
   __device__ __forceinline__ void fetch(unsigned tile, const T* matrix, int row0, int len) const {
     if (row0 + R <= len && d == D) {
       const T* base = matrix + (int64_t)row0 * st;
@@ -175,7 +178,7 @@ template <bool WEIGHTS> __device__ __forceinline__ void rest_of(Frag8<bf16_t>& f
 }
 template <bool WEIGHTS> __device__ __forceinline__ void rest_of(Frag8<float>&, const floatx16&, int, const Frag8<float>&) {}
 // Whether the granules that this lane's loads brought hold finite values only; SCRUB: the others become 0.  A wave's granules are
-// rows 16 wave .. 16 wave + 15.
+// the rows of its quarter of the tile.
 template <typename T, int D, bool SCRUB, int R = ROWS> __device__ __forceinline__ bool tile_finite(T* tile, int wave, int lane) {
   constexpr int N = Tile<T, D, R>::BYTES / 1024 / 4, VN = Vec16<T>::N;
   bool ok = true;
@@ -330,7 +333,7 @@ template <typename T, int D> constexpr int fwd_rows() { return sizeof(T) == 2 &&
 // gradient there is a sum of a few terms, whose roundings (2^-8 each) do not average out: of three tokens dq and dk were 1.8 times as
 // far off as their own rounding leaves them, of 64 and more 1.4 times.  Every workgroup goes by its own sequence, so that a document's
 // operands do not depend on what it is packed with; kernels that may meet both kinds hold both forms (MIXED: packed batches; forward of
-// eight prompts of 8192 tokens together 175 us with one form, 177-183 with both).  128 tokens are one block of queries.  By the average
+// eight prompts of 8192 tokens together 161 us with one form, 163 with both, backward 623 and 636).  128 tokens are one block of queries.  By the average
 // length a document of 8000 tokens among 150 of one, H16/4 d128, took 422 us forward and 2035 backward, this way 305 and 1405; 2048 of
 // 128, H8/2 d128, in one part 760 and 1955, in two 759 and 2247.
 constexpr int SHORT = 128;
@@ -889,7 +892,8 @@ int parts_of(const lnx_attn_args* a, int kernel) {
   const bool bf16 = a->dtype == LNX_BF16;
   const double share = bf16 ? 5 : 1, launch = bf16 ? 4 : 1.5;
   const int64_t keys = (len + ROWS - 1) / ROWS, queries = (len + 127) / 128;
-  // workgroups that the chip holds at a time: two a CU, one where fp32 tiles take most of its LDS
+  // workgroups that the chip holds at a time, about: two a CU, one where fp32 tiles take most of its LDS.  (The bf16 forward kernel at d > 64
+  // holds three, and shares its split with the dq kernel; the model was fitted to times as it is.)
   if (kernel == DKV) return parts_for(rows * a->Hkv * keys, keys * (a->H / a->Hkv), bf16 ? 512 : 256, 16, share / 2, launch);
   return parts_for(rows * a->H * queries, keys, bf16 || a->d <= 64 ? 512 : 256, 8, share, launch);
 }
@@ -1034,8 +1038,8 @@ template <typename T> constexpr int step_waves() { return sizeof(T) == 2 ? 4 : 2
 // flight while one is multiplied.  The new token's key and value come from the call and are written to the cache by the wave whose
 // tile holds the place; what lies behind it is never read.  bf16 weights enter the product in two parts, so that a weight is off by 2^-16
 // and not by 2^-8: the products wait for the cache anyway (32 full caches of 8192 places, replayed: 195 us in one part, 197.6 in two;
-// caches that lie in L2, 8 of 4096 places of 64: 21.6 and 22.6).  32 sequences of 6300 places on average, 8 key heads of 128: 152-161 us for 825
-// MB, 5.2-5.4 TB/s, and 5 us to join the shares.
+// caches that lie in L2, 8 of 4096 places of 64: 21.6 and 22.6).  32 sequences of 6300 places on average, 8 key heads of 128: 155-163 us for 825
+// MB, 5.1-5.3 TB/s, and 5 us to join the shares.
 template <typename T, int D> __global__ __launch_bounds__(64 * step_waves<T>(), 1) void attn_step_kernel(StepArgs a) {
   constexpr int W = step_waves<T>();
   typedef Tile<T, D, SROWS> TL;

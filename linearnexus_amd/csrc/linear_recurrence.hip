@@ -619,7 +619,7 @@ int64_t slots_of(const lnx_linrec_args* a, int64_t size) { return a->nseq ? a->T
 // in 8 even rows the walk is 16 % faster (173 and 271 against 207 and 313 us), with all tokens in one of them four times as slow (811
 // and 1258 against 206 and 312); of 512 rows the walk takes 342 and 583 us, the chained form 188 and 307.
 // Of fewer than 8192 tokens no row is that long, and a clearing launch is what it would cost ([1, 5003, 1000] fp32 in 7 rows: 20.5 and
-// 29.9 us walked, 21.2 and 29.8 chained, 6.6 to clear).
+// 29.9 us walked, 21.2 and 29.8 chained, 6.6 to clear; so what bounds that batch is not its longest row).
 bool chained(const lnx_linrec_args* a) {
   const int64_t wgs = (int64_t)rows_of(a) * channel_tiles(a);
   return a->T >= 8 * CTILE && (wgs < 160 || (a->nseq && a->T >= 64 * CTILE)) && slots_of(a, CTILE) * channel_tiles(a) <= MAX_GRID / CTHREADS;

@@ -10,7 +10,8 @@
 // no rounding of the stream enters the sums over the rows, which are fp32 outputs.  Those sums stay in registers over all rows of a
 // workgroup and leave as one partial row each; a second launch adds them (no atomics, the same from run to run).
 // 32768 rows of 2048, bf16 with an fp32 stream and all options: forward 160-170 us for 940 MB (5.5-5.9 TB/s), backward 281-289 for 1.48 GB
-// (5.1-5.3 TB/s) and 8 for the sums; a copy reaches 4.97.
+// (5.1-5.3 TB/s) and 8 for the sums; a copy reaches 4.97.  16384 rows of 2048 in fp32: 126 and 207 us (5.3 and 5.2 TB/s).  Of 4097 to 8192 fp32
+// columns the backward pass spills some 40 registers: 4096 rows of 8192 take 294 us, 8192 of 4096 208.
 #include "lnx_common.h"
 #include "mma_tiles.h"
 #include "reduce_rows.h"
