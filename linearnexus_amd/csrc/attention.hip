@@ -10,7 +10,7 @@
 // multiplied, one barrier a tile.
 // bf16 takes v_mfma_f32_32x32x16_bf16 (probabilities and score gradients are rounded to bf16 as operands: at most 2^-8 of each term, what
 // the outputs are rounded to; all in all 0.0024 of the norm for a training step and 0.0021 for a prompt, where the rounding of the results alone
-// is 0.0017 and 0.0016; in two parts, a third of the products more, it is that alone: see SHORT), fp32 takes v_mfma_f32_32x32x2_f32
+// is 0.0017 and 0.0016; in two parts, with up to half of the products more, it is that alone: see SHORT), fp32 takes v_mfma_f32_32x32x2_f32
 // throughout.  Sums, maxima and accumulators are fp32.
 // Bound by the matrix cores and the exponentials beside them: at B2 H16/4 T4096 d128 bf16 the forward kernel takes 147-164 us (840-930
 // TFLOP/s of the causal half), dq 194-217, dk / dv 311-343 and the two sums of its parts 7 each, together 600-650 TFLOP/s of the 10 d operations a

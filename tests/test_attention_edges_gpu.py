@@ -95,6 +95,63 @@ def test_short_documents_beside_long_ones_are_as_exact_as_their_rounding(lens, H
     _check(q, k, v, do, cu=cu)
 
 
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("d", [64, 80, 128])
+@pytest.mark.parametrize("lens", [[100], [100, 300, 3, 128]], ids=str)
+def test_values_behind_the_mask_of_short_documents(lens, d, bad):
+    """Keys and values behind a row's queries, and queries and gradients before a key, are not in its results, in either form of the kernels."""
+    cu = np.concatenate([[0], np.cumsum(lens)]).tolist()
+    q, k, v, do = _inputs(1, 4, 2, cu[-1], d, "bf16")
+    cut = 57  # of the first document
+    keep = do.clone()
+    keep[:, :, cut:100] = 0
+
+    def run(q, k, v, do):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        o = la.causal_attention(*leaves, cu_seqlens=cu)
+        return (o.detach(), *torch.autograd.grad(o, leaves, do))
+
+    clean = run(q, k, v, keep)
+    k2, v2 = k.clone(), v.clone()
+    k2[:, :, cut:100] = bad
+    v2[:, :, cut:100] = bad
+    dirty = run(q, k2, v2, keep)
+    rest = torch.tensor([i for i in range(cu[-1]) if not cut <= i < 100], device=DEV)
+    for a, b in zip(dirty[:2], clean[:2]):
+        assert torch.equal(a[:, :, rest], b[:, :, rest])
+    assert not bool(torch.isfinite(dirty[0][:, :, cut:100]).any())
+    q2, do2 = q.clone(), do.clone()
+    q2[:, :, :20] = bad
+    do2[:, :, :20] = bad
+    full, dirty = run(q, k, v, do), run(q2, k, v, do2)
+    for a, b in zip(dirty[2:], full[2:]):
+        assert torch.equal(a[:, :, 20:], b[:, :, 20:])
+
+
+def test_packed_documents_of_both_kinds_in_a_replayed_graph():
+    q, k, v, do = _inputs(1, 4, 2, 640, 128, "bf16", token_first=True)
+    leaves = [t.detach().clone().requires_grad_() for t in (q, k, v)]
+    cu = torch.tensor([0, 3, 303, 303, 400, 640], dtype=torch.int32, device=DEV)
+
+    def both():
+        o = la.causal_attention(*leaves, cu_seqlens=cu)
+        return (o, *torch.autograd.grad(o, leaves, do))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = both()
+    for table in ([0, 3, 303, 303, 400, 640], [0, 1, 2, 3, 4, 640], [0, 128, 256, 384, 512, 640], [0, 129, 258, 387, 516, 640]):
+        cu.copy_(torch.tensor(table, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, both()))
+
+
 # -- memory order ---------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("d", [20, 33, 64, 80])
