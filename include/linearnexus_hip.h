@@ -471,6 +471,31 @@ int lnx_rmsnorm_residual_fwd(const lnx_rmsnorm_residual_args* a, void* hip_strea
 int lnx_rmsnorm_residual_bwd(const lnx_rmsnorm_residual_args* a, void* hip_stream);
 
 /*
+ * Layer norm over rows of d columns (d <= 8192): y = (x - mean) / sqrt(var + eps) weight + bias, var the mean of the squared differences.
+ * weight and bias (and their gradients) are fp32 [heads, d]: row r takes set r % heads, one set for all rows with heads = 1; either
+ * may be NULL (ones, zeros).  x, y, d_y, d_x dense in `dtype`.  The backward call reads x, weight and d_y; d_weight and d_bias may be NULL (not
+ * wanted) and are summed without atomics through the workspace (16-byte aligned).
+ */
+typedef struct lnx_layer_norm_args {
+  int64_t rows;             /* a multiple of heads */
+  int32_t heads, d, dtype;
+  float eps;
+  const void* x;
+  const float* weight;
+  const float* bias;
+  void* y;
+  const void* d_y;          /* backward only, from here */
+  void* d_x;
+  float* d_weight;
+  float* d_bias;
+  void* workspace;
+  uint64_t workspace_bytes;
+} lnx_layer_norm_args;
+uint64_t lnx_layer_norm_bwd_workspace_bytes(int64_t rows, int32_t heads, int32_t d, int32_t dtype);
+int lnx_layer_norm_fwd(const lnx_layer_norm_args* a, void* hip_stream);
+int lnx_layer_norm_bwd(const lnx_layer_norm_args* a, void* hip_stream);
+
+/*
  * Causal softmax attention over whole prompts with grouped heads, and its gradient: query i of a sequence attends to its keys
  * 0 .. i; query head h reads key head h / (H / Hkv).  q, o, d_o, d_q are [B, H, T, d], k, v, d_k, d_v [B, Hkv, T, d] in `dtype`,
  * each with its own strides (in elements, rows contiguous, every stride and pointer a multiple of 16 bytes, tokens at most

@@ -21,6 +21,7 @@ EXPORTS = (
     "lnx_gdn_gate_fwd", "lnx_gdn_gate_bwd", "lnx_gdn_gate_bwd_workspace_bytes", "lnx_kda_gate_fwd", "lnx_kda_gate_bwd", "lnx_kda_gate_bwd_workspace_bytes", "lnx_sigmoid_fwd", "lnx_sigmoid_bwd",
     "lnx_linrec_workspace_bytes", "lnx_linrec_kept_bytes", "lnx_linrec_fwd", "lnx_linrec_bwd", "lnx_linrec_step",
     "lnx_rmsnorm_residual_bwd_workspace_bytes", "lnx_rmsnorm_residual_fwd", "lnx_rmsnorm_residual_bwd",
+    "lnx_layer_norm_bwd_workspace_bytes", "lnx_layer_norm_fwd", "lnx_layer_norm_bwd",
     "lnx_attn_fwd_workspace_bytes", "lnx_attn_bwd_workspace_bytes", "lnx_attn_fwd", "lnx_attn_bwd", "lnx_attn_step_workspace_bytes", "lnx_attn_step",
     "lnx_profile_enable", "lnx_profile_read",
 )
@@ -91,6 +92,16 @@ class RmsnormResidualArgs(C.Structure):
         ("scale_vector", C.c_void_p), ("z", C.c_void_p), ("out", C.c_void_p), ("d_z", C.c_void_p), ("d_out", C.c_void_p), ("d_x", C.c_void_p),
         ("d_residual", C.c_void_p), ("d_gate", C.c_void_p), ("d_weight", C.c_void_p), ("d_post_weight", C.c_void_p), ("d_scale", C.c_void_p),
         ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
+    ]
+
+
+class LayerNormArgs(C.Structure):
+    """Mirror of ``struct lnx_layer_norm_args``."""
+
+    _fields_ = [
+        ("rows", C.c_int64), ("heads", C.c_int32), ("d", C.c_int32), ("dtype", C.c_int32), ("eps", C.c_float),
+        ("x", C.c_void_p), ("weight", C.c_void_p), ("bias", C.c_void_p), ("y", C.c_void_p), ("d_y", C.c_void_p), ("d_x", C.c_void_p),
+        ("d_weight", C.c_void_p), ("d_bias", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
     ]
 
 
@@ -210,6 +221,11 @@ def load() -> C.CDLL:
     for name in ("lnx_rmsnorm_residual_fwd", "lnx_rmsnorm_residual_bwd"):
         getattr(lib, name).restype = C.c_int
         getattr(lib, name).argtypes = [C.POINTER(RmsnormResidualArgs), C.c_void_p]
+    lib.lnx_layer_norm_bwd_workspace_bytes.restype = C.c_uint64
+    lib.lnx_layer_norm_bwd_workspace_bytes.argtypes = [C.c_int64, C.c_int32, C.c_int32, C.c_int32]
+    for name in ("lnx_layer_norm_fwd", "lnx_layer_norm_bwd"):
+        getattr(lib, name).restype = C.c_int
+        getattr(lib, name).argtypes = [C.POINTER(LayerNormArgs), C.c_void_p]
     for name in ("lnx_attn_fwd_workspace_bytes", "lnx_attn_bwd_workspace_bytes"):
         getattr(lib, name).restype = C.c_uint64
         getattr(lib, name).argtypes = [C.POINTER(AttnArgs)]

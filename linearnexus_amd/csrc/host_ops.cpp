@@ -966,6 +966,98 @@ PyObject* py_rmsnorm_residual(PyObject*, PyObject* const* args, Py_ssize_t nargs
 }
 
 // ---------------------------------------------------------------------------------------------------------------
+// layer norm
+// ---------------------------------------------------------------------------------------------------------------
+
+// x dense, weight and bias dense fp32: [d] or [heads, d]
+lnx_layer_norm_args layer_norm_args(const Tensor& x, const Tensor& w, const Tensor& b, int64_t heads, double eps) {
+  lnx_layer_norm_args a{};
+  const int64_t d = x.size(-1);
+  a.rows = x.numel() / d, a.heads = (int32_t)heads, a.d = (int32_t)d, a.dtype = code_of(x.scalar_type()), a.eps = (float)eps;
+  a.x = ptr(x), a.weight = fptr(w), a.bias = fptr(b);
+  return a;
+}
+
+Tensor layer_norm_forward(const Tensor& x, const Tensor& w, const Tensor& b, int64_t heads, double eps) {
+  const Tensor y = at::empty_like(x);
+  lnx_layer_norm_args a = layer_norm_args(x, w, b, heads, eps);
+  a.y = ptr(y);
+  const c10::DeviceGuard guard(x.device());
+  check_status(lnx_layer_norm_fwd(&a, stream_of(x)), "lnx_layer_norm_fwd");
+  return y;
+}
+
+struct LayerNormFn : Function<LayerNormFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x0, const OptT& weight, const OptT& bias, int64_t heads, double eps) {
+    const Tensor x = x0.contiguous(), w = f32(undef(weight)), b = f32(undef(bias));
+    const Tensor y = layer_norm_forward(x, w, b, heads, eps);
+    ctx->save_for_backward({x, w});
+    auto kind = [](const OptT& t) { return (int64_t)(t.has_value() ? t->scalar_type() : at::kFloat); };
+    auto wants = [](const OptT& t) { return (int64_t)(t.has_value() && t->requires_grad()); };
+    ctx->saved_data["i"] = std::vector<int64_t>{heads, kind(weight), kind(bias), wants(weight), wants(bias), bias.has_value() ? bias->dim() : 0};
+    ctx->saved_data["d"] = eps;
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_tangents("the gradient of layer_norm", grads);
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor &x = s[0], &w = s[1];
+    refuse_live_graph_behind("the gradient of layer_norm", x);
+    const std::vector<int64_t> m = ctx->saved_data["i"].toIntVector();
+    const Tensor dy = grads[0].to(x.scalar_type()).contiguous();
+    lnx_layer_norm_args a = layer_norm_args(x, w, Tensor(), m[0], ctx->saved_data["d"].toDouble());
+    Tensor dx = at::empty_like(x), dw, db, ws;
+    if (m[3]) dw = at::empty_like(w);
+    if (m[4]) db = m[5] == 2 ? at::empty({m[0], a.d}, x.options().dtype(at::kFloat)) : at::empty({a.d}, x.options().dtype(at::kFloat));
+    if (m[3] || m[4]) {
+      a.workspace_bytes = lnx_layer_norm_bwd_workspace_bytes(a.rows, a.heads, a.d, a.dtype);
+      ws = work_area(x, a.workspace_bytes);
+      a.workspace = ptr(ws);
+    }
+    a.d_y = ptr(dy), a.d_x = ptr(dx), a.d_weight = fptr(dw), a.d_bias = fptr(db);
+    const c10::DeviceGuard guard(x.device());
+    check_status(lnx_layer_norm_bwd(&a, stream_of(x)), "lnx_layer_norm_bwd");
+    auto to = [](const Tensor& t, int64_t type) { return t.defined() ? t.to((at::ScalarType)type) : t; };
+    return {dx, to(dw, m[1]), to(db, m[2]), Tensor(), Tensor()};
+  }
+};
+
+// layer_norm(x, weight, bias, eps)
+PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  LNX_BEGIN
+  Args in(args, nargs, 4, "layer_norm");
+  const char* op = "layer_norm";
+  const Tensor x = in.tensor(0, "x"), weight = in.maybe(1, "weight"), bias = in.maybe(2, "bias");
+  const double eps = in.number(3);
+  TORCH_CHECK(x.is_cuda(), op, ": x is on ", x.device().str(), "; the op runs on the GPU only");
+  TORCH_CHECK(known_dtype(x.scalar_type()), "unsupported dtype ", x.scalar_type(), ": use float32 or bfloat16");
+  TORCH_CHECK(x.dim() > 0 && x.size(-1) > 0, op, ": x must have rows, got ", shape_text(x));
+  const int64_t d = x.size(-1);
+  int64_t heads = 0;  // 0: nothing has said so yet
+  for (const auto& [name, t] : {std::make_pair("weight", &weight), std::make_pair("bias", &bias)}) {
+    if (!t->defined()) continue;
+    const bool one = t->dim() == 1 && t->size(0) == d, many = t->dim() == 2 && x.dim() >= 2 && t->size(0) == x.size(-2) && t->size(0) > 0 && t->size(1) == d;
+    TORCH_CHECK(one || many, op, ": ", name, " must be [", d, "], or [heads, ", d, "] for x [..., heads, ", d, "], got ", shape_text(*t), " for x ", shape_text(x));
+    TORCH_CHECK(t->is_floating_point(), op, ": ", name, " must be a floating-point tensor, got ", t->scalar_type());
+    const int64_t h = one ? 1 : t->size(0);
+    TORCH_CHECK(heads == 0 || (weight.dim() == bias.dim()), op, ": weight ", shape_text(weight), " and bias ", shape_text(*t), " must have one shape");
+    heads = h;
+  }
+  heads = std::max<int64_t>(heads, 1);
+  TORCH_CHECK(std::isfinite((float)eps) && eps >= 0, op, ": eps must be finite and not negative, got ", eps);
+  check_devices(op, x, {{"weight", &weight}, {"bias", &bias}});
+  refuse_tangents(op, {&x, &weight, &bias});
+  return THPVariable_Wrap(without_lock([&] {
+    if (wants_grad({&x, &weight, &bias})) {
+      refuse_live_graph(op, {&x, &weight, &bias});
+      return LayerNormFn::apply(x, opt(weight), opt(bias), heads, eps);
+    }
+    return layer_norm_forward(x.contiguous(), f32(weight), f32(bias), heads, eps);
+  }));
+  LNX_END
+}
+
+// ---------------------------------------------------------------------------------------------------------------
 // gate activations
 // ---------------------------------------------------------------------------------------------------------------
 
@@ -1591,7 +1683,7 @@ PyObject* py_set_kernel_error(PyObject*, PyObject* const* args, Py_ssize_t nargs
 
 #define LNX_FN(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {LNX_FN(step),     LNX_FN(recurrent), LNX_FN(l2norm), LNX_FN(l2norm_bwd), LNX_FN(chunk), LNX_FN(chunk_segmented),     LNX_FN(conv1d),           LNX_FN(rmsnorm_gated), LNX_FN(gdn_gate),
-                         LNX_FN(kda_gate), LNX_FN(dplr),      LNX_FN(dplr_step), LNX_FN(linrec), LNX_FN(linrec_step), LNX_FN(rmsnorm_residual), LNX_FN(causal_attention), LNX_FN(causal_attention_step), LNX_FN(set_kernel_error), {nullptr, nullptr, 0, nullptr}};
+                         LNX_FN(kda_gate), LNX_FN(dplr),      LNX_FN(dplr_step), LNX_FN(linrec), LNX_FN(linrec_step), LNX_FN(rmsnorm_residual), LNX_FN(layer_norm), LNX_FN(causal_attention), LNX_FN(causal_attention_step), LNX_FN(set_kernel_error), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_host", "Host path of the linearnexus_amd ops.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -8,6 +8,9 @@ the HIP backward kernel.
 behind a block with its gate and residual scale, the addition to the residual stream and the norm before the next block (the
 reference's blocks add and norm separately, modules/common.py:27, kda.py:831-995), one pass forward and one backward.
 
+``layer_norm(x, weight, bias, eps)`` is the norm with a mean, for blocks and heads that take one (the reference's ``LayerNorm``, modules/common.py): weights
+for the last dimension, or a set for each head.
+
 There is no other code path: the ops raise if the library is missing.
 """
 from __future__ import annotations
@@ -35,3 +38,12 @@ def rmsnorm_residual(x: Tensor, residual: Optional[Tensor], weight: Optional[Ten
     or a ``[d]`` tensor.  ``x [..., d]`` and z are float32 or bfloat16, the residual and r float32 or x's dtype, the gate likewise (one of
     another type is taken in float32); z is the norm of the sum before it is rounded to r's dtype.  Differentiable with respect to every tensor."""
     return _lib.host().rmsnorm_residual(x, residual, weight, post_weight, gate, scale, eps)
+
+
+def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5) -> Tensor:
+    """``(x - mean) * rsqrt(var + eps) * weight + bias`` over the last dimension (at most 8192 wide), ``var`` the mean of the squared differences.
+
+    ``x [..., d]`` and the result are float32 or bfloat16; sums are float32.  ``weight`` and ``bias`` are ``[d]``, or ``[heads, d]`` for
+    ``x [..., heads, d]``: every head is a row of its own with its own weights (the norm behind a linear-attention mixer).  ``None``: ones, zeros.
+    Differentiable with respect to all three."""
+    return _lib.host().layer_norm(x, weight, bias, eps)
