@@ -546,6 +546,29 @@ uint64_t lnx_attn_step_workspace_bytes(const lnx_attn_step_args* a);
 int lnx_attn_step(const lnx_attn_step_args* a, void* hip_stream);
 
 /*
+ * The same against a cache in pages: k_cache, v_cache [pages, Hkv, page, d] (stride_b: of a page, stride_t: of a place in it), the places
+ * page j .. of sequence b in page page_table[b][j / page].  page_table [B, table_width] int32 on the device, rows table_stride
+ * apart; a sequence has room for table_width * page places (fewer than 2^31).  Entries behind the new token's page are not read; an entry in use that
+ * is no page gives NaN (and nothing is written where the new token's is none).  Sequences may share the pages of what they have in common, but
+ * not the place that a call writes.
+ */
+typedef struct lnx_attn_step_paged_args {
+  int32_t B, H, Hkv, d, dtype;
+  int32_t page, pages, table_width;
+  float scale;
+  int32_t reserved;
+  lnx_tensor4 q, k, v, k_cache, v_cache;
+  void* o;
+  const int32_t* lengths;
+  const int32_t* page_table;
+  int64_t table_stride;
+  void* workspace;
+  uint64_t workspace_bytes;
+} lnx_attn_step_paged_args;
+uint64_t lnx_attn_step_paged_workspace_bytes(const lnx_attn_step_paged_args* a);
+int lnx_attn_step_paged(const lnx_attn_step_paged_args* a, void* hip_stream);
+
+/*
  * Optional per-kernel timing for benchmarks (no counterpart in the reference; its micro-benchmark
  * times whole jitted ops, bench_kda_kernels.py:216-249).  While enabled (process-wide),
  * every entry point records HIP events around each kernel it launches, on the caller's stream.

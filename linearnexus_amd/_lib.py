@@ -22,7 +22,7 @@ EXPORTS = (
     "lnx_linrec_workspace_bytes", "lnx_linrec_kept_bytes", "lnx_linrec_fwd", "lnx_linrec_bwd", "lnx_linrec_step",
     "lnx_rmsnorm_residual_bwd_workspace_bytes", "lnx_rmsnorm_residual_fwd", "lnx_rmsnorm_residual_bwd",
     "lnx_layer_norm_bwd_workspace_bytes", "lnx_layer_norm_fwd", "lnx_layer_norm_bwd",
-    "lnx_attn_fwd_workspace_bytes", "lnx_attn_bwd_workspace_bytes", "lnx_attn_fwd", "lnx_attn_bwd", "lnx_attn_step_workspace_bytes", "lnx_attn_step",
+    "lnx_attn_fwd_workspace_bytes", "lnx_attn_bwd_workspace_bytes", "lnx_attn_fwd", "lnx_attn_bwd", "lnx_attn_step_workspace_bytes", "lnx_attn_step", "lnx_attn_step_paged_workspace_bytes", "lnx_attn_step_paged",
     "lnx_profile_enable", "lnx_profile_read",
 )
 
@@ -133,6 +133,18 @@ class AttnStepArgs(C.Structure):
     ]
 
 
+class AttnStepPagedArgs(C.Structure):
+    """Mirror of ``struct lnx_attn_step_paged_args``."""
+
+    _fields_ = [
+        ("B", C.c_int32), ("H", C.c_int32), ("Hkv", C.c_int32), ("d", C.c_int32), ("dtype", C.c_int32),
+        ("page", C.c_int32), ("pages", C.c_int32), ("table_width", C.c_int32), ("scale", C.c_float), ("reserved", C.c_int32),
+        ("q", Tensor4), ("k", Tensor4), ("v", Tensor4), ("k_cache", Tensor4), ("v_cache", Tensor4),
+        ("o", C.c_void_p), ("lengths", C.c_void_p), ("page_table", C.c_void_p), ("table_stride", C.c_int64),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
+    ]
+
+
 _lib = None
 
 
@@ -236,6 +248,10 @@ def load() -> C.CDLL:
     lib.lnx_attn_step_workspace_bytes.argtypes = [C.POINTER(AttnStepArgs)]
     lib.lnx_attn_step.restype = C.c_int
     lib.lnx_attn_step.argtypes = [C.POINTER(AttnStepArgs), C.c_void_p]
+    lib.lnx_attn_step_paged_workspace_bytes.restype = C.c_uint64
+    lib.lnx_attn_step_paged_workspace_bytes.argtypes = [C.POINTER(AttnStepPagedArgs)]
+    lib.lnx_attn_step_paged.restype = C.c_int
+    lib.lnx_attn_step_paged.argtypes = [C.POINTER(AttnStepPagedArgs), C.c_void_p]
     lib.lnx_profile_enable.restype = C.c_int
     lib.lnx_profile_enable.argtypes = [C.c_int]
     lib.lnx_profile_read.restype = C.c_int

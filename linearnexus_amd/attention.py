@@ -6,7 +6,8 @@ Hkv (query head h reads key head ``h // (H // Hkv)``), float32 or bfloat16, d at
 order: ``[B,T,H,d]`` tensors are passed as ``x.transpose(1, 2)`` views and nothing is copied.  Packed batches pass B = 1 and
 ``cu_seqlens``, like the chunked ops; no query sees another sequence.  Differentiable with respect to q, k and v.
 ``causal_attention_step(q, k, v, k_cache, v_cache, lengths, scale=None)`` is one decode token: its key and value are written into the
-caches at ``lengths`` and its queries attend to everything up to it.  There is no other code path: the ops raise if the library is
+caches at ``lengths`` and its queries attend to everything up to it.  ``causal_attention_step_paged(q, k, v, k_pages, v_pages, page_table,
+lengths, scale=None)`` is the same over a cache whose places lie in pages of one pool.  There is no other code path: the ops raise if the library is
 missing.
 """
 from __future__ import annotations
@@ -34,3 +35,12 @@ def causal_attention_step(q: Tensor, k: Tensor, v: Tensor, k_cache: Tensor, v_ca
     are written in place), ``lengths [B]`` int32 on the GPU: tokens each sequence already holds.  Returns ``o [B,H,d]``.  The caller
     advances ``lengths``.  Places behind the token are not read; a length outside ``0 .. S - 1`` writes nothing and gives NaN."""
     return _lib.host().causal_attention_step(q, k, v, k_cache, v_cache, lengths, scale)
+
+
+def causal_attention_step_paged(q: Tensor, k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, lengths: Tensor,
+                                scale: Optional[float] = None) -> Tensor:
+    """One token per sequence over paged caches: ``k_pages, v_pages [pages, Hkv, page, d]`` (any page size; d a multiple of 8; strided views such as
+    transposed ``[pages, page, Hkv, d]`` are fine, they are written in place), ``page_table [B, n]`` int32 on the GPU: place ``j`` of a
+    sequence lies in page ``page_table[b, j // page]``.  Otherwise as ``causal_attention_step``; entries behind the new token's page are not read, and an
+    entry in use that names no page gives NaN.  Sequences may share pages, but not the place that a call writes."""
+    return _lib.host().causal_attention_step_paged(q, k, v, k_pages, v_pages, page_table, lengths, scale)

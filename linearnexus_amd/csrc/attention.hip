@@ -1026,7 +1026,9 @@ struct StepArgs {
   const int32_t* len;
   int64_t qs[2], ks[2], vs[2], kcs[3], vcs[3];  // strides of batch, head (and place) in elements; o is dense
   float* part;  // [B H][splits][D + 2]: sums relative to a maximum, the maximum, the sum of weights
-  int B, H, Hkv, G, S, d, splits, ctiles;
+  const int32_t* table;  // paged: page of every `page` places of a sequence; kcs and vcs are then the strides of page, head and place
+  int64_t table_stride;
+  int B, H, Hkv, G, S, d, splits, ctiles, page, pages;
   float scale;
 };
 
@@ -1040,7 +1042,11 @@ template <typename T> constexpr int step_waves() { return sizeof(T) == 2 ? 4 : 2
 // and not by 2^-8: the products wait for the cache anyway (32 full caches of 8192 places, replayed: 195 us in one part, 197.6 in two;
 // caches that lie in L2, 8 of 4096 places of 64: 21.6 and 22.6).  32 sequences of 6300 places on average, 8 key heads of 128: 155-163 us for 825
 // MB, 5.1-5.3 TB/s, and 5 us to join the shares.
-template <typename T, int D> __global__ __launch_bounds__(64 * step_waves<T>(), 1) void attn_step_kernel(StepArgs a) {
+//
+// PAGED: places lie in pages that a table names.  A wave brings the pages' numbers of a tile's 32 rows to LDS with one load of four bytes a lane, two
+// tiles ahead: ordered like every other load, so that nothing waits for the table but the first tile.  A page may end anywhere in a tile.  A
+// number outside the pool is not followed: its sequence's result is NaN.
+template <typename T, int D, bool PAGED> __global__ __launch_bounds__(64 * step_waves<T>(), 1) void attn_step_kernel(StepArgs a) {
   constexpr int W = step_waves<T>();
   typedef Tile<T, D, SROWS> TL;
   constexpr int NI = TL::BYTES / 1024;
@@ -1055,8 +1061,8 @@ template <typename T, int D> __global__ __launch_bounds__(64 * step_waves<T>(), 
   const int len = a.len[b];
   const bool good = len >= 0 && len < a.S;
   const int ntile = good ? len / SROWS + 1 : 0;
-  const T* kc = static_cast<const T*>(a.kc) + b * a.kcs[0] + hkv * a.kcs[1];
-  const T* vc = static_cast<const T*>(a.vc) + b * a.vcs[0] + hkv * a.vcs[1];
+  const T* kc = static_cast<const T*>(a.kc) + (PAGED ? 0 : b * a.kcs[0]) + hkv * a.kcs[1];
+  const T* vc = static_cast<const T*>(a.vc) + (PAGED ? 0 : b * a.vcs[0]) + hkv * a.vcs[1];
   const T* kn = static_cast<const T*>(a.k) + b * a.ks[0] + hkv * a.ks[1];
   const T* vn = static_cast<const T*>(a.v) + b * a.vs[0] + hkv * a.vs[1];
   char* mine = lds + wave * 4 * TL::BYTES;
@@ -1067,23 +1073,61 @@ template <typename T, int D> __global__ __launch_bounds__(64 * step_waves<T>(), 
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   };
   if (a.d < D) clear(mine, 4 * TL::BYTES);
+  // PAGED: page numbers of the rows of two tiles; whether one of them was none
+  int* ids = reinterpret_cast<int*>(lds + W * 4 * TL::BYTES) + wave * 128;
+  const int32_t* table = PAGED ? a.table + b * a.table_stride : nullptr;
+  bool lost = false;
+  // where row r of a tile whose first row is place `rem` of its page lies: in which page from there on, at which place of it
+  const auto turn = [&](int rem, int r, int& place) {
+    const int x = rem + r, q = a.page >= SROWS ? x >= a.page : (int)(((float)x + 0.5f) * __builtin_amdgcn_rcpf((float)a.page));  // x < 63 there: 1/62 from every integer
+    place = x - q * a.page;
+    return q;
+  };
+  const auto look = [&](int tile, int buf) {  // the pages of a tile's rows; behind the new token its own
+    if constexpr (PAGED) {
+      int place;
+      const int first = tile * SROWS, r = min(lane & 31, len - first);
+      const int q = turn(first % a.page, r, place);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the reads of the numbers that lay here
+      dma4(table + first / a.page + q, lds_byte_addr(ids + 64 * buf));
+    }
+  };
   const auto fetch = [&](int tile, int buf) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the reads of the tile that lay here
     if (tile == ntile - 1) clear(vt(buf), TL::BYTES);  // rows behind the new token: no value at all
+    const int rem = PAGED ? tile * SROWS % a.page : 0;
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
       int r, c;
       TL::src(j, lane, r, c);
-      r += tile * SROWS;
+      int64_t ko, vo;
+      if constexpr (PAGED) {
+        int place, id = ids[64 * buf + r];
+        turn(rem, r, place);
+        lost = lost || id < 0 || id >= a.pages;
+        id = id < 0 || id >= a.pages ? 0 : id;
+        ko = id * a.kcs[0] + place * a.kcs[2], vo = id * a.vcs[0] + place * a.vcs[2];
+        r += tile * SROWS;
+      } else {
+        r += tile * SROWS;
+        ko = (int64_t)r * a.kcs[2], vo = (int64_t)r * a.vcs[2];
+      }
       if (c < a.d && r <= len) {
-        dma16(r < len ? kc + (int64_t)r * a.kcs[2] + c : kn + c, lds_byte_addr(kt(buf)) + 1024 * j);
-        dma16(r < len ? vc + (int64_t)r * a.vcs[2] + c : vn + c, lds_byte_addr(vt(buf)) + 1024 * j);
+        dma16(r < len ? kc + ko + c : kn + c, lds_byte_addr(kt(buf)) + 1024 * j);
+        dma16(r < len ? vc + vo + c : vn + c, lds_byte_addr(vt(buf)) + 1024 * j);
       }
     }
   };
   const int step = a.splits * W;
   int tile = split * W + wave;
-  if (tile < ntile) fetch(tile, 0);
+  if (tile < ntile) {
+    if constexpr (PAGED) {
+      look(tile, 0);
+      if (tile + step < ntile) look(tile + step, 1);
+      dma_wait<0>();
+    }
+    fetch(tile, 0);
+  }
   const float c = fmaxf(fabsf(a.scale) * LOG2E, 1e-30f);
   const T* qr = static_cast<const T*>(a.q) + b * a.qs[0] + (int64_t)(n < cols ? h : hkv * a.G) * a.qs[1];
   Frag8<T> qf[D / 16];
@@ -1101,14 +1145,23 @@ template <typename T, int D> __global__ __launch_bounds__(64 * step_waves<T>(), 
     for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
   float m = -INFINITY, l = 0.f;
   for (int buf = 0; tile < ntile; tile += step, buf ^= 1) {
+    if (tile + 2 * step < ntile) look(tile + 2 * step, buf);
     if (tile + step < ntile) fetch(tile + step, buf ^ 1);
     if (tile + step < ntile - 1) dma_wait<2 * NI>();
     else dma_wait<0>();  // the last tile may be short of rows, and of loads
     const unsigned rows = lds_byte_addr(kt(buf)) + TL::rows(lane), cols = lds_byte_addr(kt(buf)) + TL::cols(lane);
     if (tile == ntile - 1 && ct == 0) {  // the new token's place
-      T* kw = const_cast<T*>(kc) + (int64_t)len * a.kcs[2];
-      T* vw = const_cast<T*>(vc) + (int64_t)len * a.vcs[2];
-      for (int i = lane; i < a.d; i += 64) kw[i] = kn[i], vw[i] = vn[i];
+      int64_t ko = (int64_t)len * a.kcs[2], vo = (int64_t)len * a.vcs[2];
+      bool there = true;
+      if constexpr (PAGED) {
+        const int id = table[len / a.page], place = len % a.page;
+        there = id >= 0 && id < a.pages;
+        ko = id * a.kcs[0] + place * a.kcs[2], vo = id * a.vcs[0] + place * a.vcs[2];
+      }
+      T* kw = const_cast<T*>(kc) + ko;
+      T* vw = const_cast<T*>(vc) + vo;
+      if (there)
+        for (int i = lane; i < a.d; i += 64) kw[i] = kn[i], vw[i] = vn[i];
     }
     floatx16 sc;
 #pragma unroll
@@ -1157,6 +1210,7 @@ template <typename T, int D> __global__ __launch_bounds__(64 * step_waves<T>(), 
 #pragma unroll
     for (int e = 0; e < 16; ++e) sums[((wave * (D / 32) + i) * 16 + e) * 64 + lane] = acc[i][e];
   l = xor32_sum(l);
+  if (PAGED && __any(lost)) l = NAN;
   if (kg == 0) stat[wave * 64 + n] = m, stat[wave * 64 + 32 + n] = l;
   __syncthreads();
   float top = stat[n], sum = 0.f, f[W];
@@ -1244,80 +1298,107 @@ template <typename T, int D> __global__ __launch_bounds__(1024) void attn_step_j
 }
 
 // Splits of a cache: workgroups for four to a CU, but two tiles a wave at least of a cache that is full
-int step_splits(const lnx_attn_step_args* a) {
-  const int waves = a->dtype == LNX_BF16 ? step_waves<bf16_t>() : step_waves<float>();
-  const int64_t wgs = (int64_t)a->B * a->Hkv * ((a->H / a->Hkv + 31) / 32), tiles = ((int64_t)a->S + SROWS - 1) / SROWS;
+int step_splits(int B, int H, int Hkv, int64_t S, int dtype) {
+  const int waves = dtype == LNX_BF16 ? step_waves<bf16_t>() : step_waves<float>();
+  const int64_t wgs = (int64_t)B * Hkv * ((H / Hkv + 31) / 32), tiles = (S + SROWS - 1) / SROWS;
   int64_t s = (MOST_SPLITS + wgs - 1) / wgs;
   const int64_t most = (tiles + 2 * waves - 1) / (2 * waves);
   if (s > most) s = most;
   return (int)(s < 1 ? 1 : s);
 }
+uint64_t step_bytes(int B, int H, int Hkv, int64_t S, int d, int dtype) {
+  if (B <= 0 || H <= 0 || Hkv <= 0 || S <= 0) return 0;
+  const int s = step_splits(B, H, Hkv, S, dtype);
+  return s > 1 ? (uint64_t)B * H * s * ((d <= 64 ? 64 : 128) + 4) * sizeof(float) : 0;
+}
 
 // Threads of the joining workgroups: a wave for four shares
 int join_threads(int splits) { return 64 * (splits <= 4 ? 1 : splits >= 64 ? 16 : (splits + 3) / 4); }
 
-int check_step(const lnx_attn_step_args* a) {
-  const char* what = "attn_step";
-  if (!a) return lnx_set_error(LNX_ERR_NULL, "%s: args is NULL", what);
-  if (a->B < 0 || a->H <= 0 || a->Hkv <= 0 || a->H % a->Hkv || a->S <= 0 || a->d <= 0 || a->d > 128 || a->d % 8)
-    return lnx_set_error(LNX_ERR_SHAPE, "%s: unsupported dimensions B=%d H=%d Hkv=%d S=%d d=%d (d a multiple of 8, at most 128; H a multiple of Hkv)", what, a->B, a->H, a->Hkv,
-                         a->S, a->d);
+// What both kinds of cache have in common: `outer` rows of the caches' first dimension, `places` next to each other, S places a sequence
+template <typename A> int check_step(const char* what, const A* a, int outer, int places, int64_t S) {
   if (a->dtype != LNX_F32 && a->dtype != LNX_BF16) return lnx_set_error(LNX_ERR_DTYPE, "%s: dtype %d", what, a->dtype);
   if (a->B == 0) return LNX_OK;
   if (!(a->scale == a->scale) || a->scale - a->scale != 0.f) return lnx_set_error(LNX_ERR_SHAPE, "%s: scale must be finite", what);
   const lnx_tensor4* ts[] = {&a->q, &a->k, &a->v, &a->k_cache, &a->v_cache};
   for (int i = 0; i < 5; ++i) {
     if (!ts[i]->p) return lnx_set_error(LNX_ERR_NULL, "%s: a tensor is missing", what);
-    if (!rows_fit(ts[i], a->dtype == LNX_BF16 ? 2 : 4, a->B, i == 0 ? a->H : a->Hkv, i < 3 ? 1 : a->S)) return lnx_set_error(LNX_ERR_SHAPE, "%s: tensors must be 16-byte aligned, rows whole numbers of 16 bytes and at most 16 MiB apart", what);
+    if (!rows_fit(ts[i], a->dtype == LNX_BF16 ? 2 : 4, i < 3 ? a->B : outer, i == 0 ? a->H : a->Hkv, i < 3 ? 1 : places)) return lnx_set_error(LNX_ERR_SHAPE, "%s: tensors must be 16-byte aligned, rows whole numbers of 16 bytes and at most 16 MiB apart", what);
   }
   if (!a->o || !a->lengths) return lnx_set_error(LNX_ERR_NULL, "%s: o and lengths are required", what);
   if (reinterpret_cast<uintptr_t>(a->o) % 16) return lnx_set_error(LNX_ERR_SHAPE, "%s: tensors must be 16-byte aligned, rows whole numbers of 16 bytes and at most 16 MiB apart", what);
-  if ((int64_t)a->B * a->H > MAX_GRID || (int64_t)a->B * a->Hkv * ((a->H / a->Hkv + 31) / 32) * step_splits(a) > MAX_GRID) return lnx_set_error(LNX_ERR_SHAPE, "%s: too many rows", what);
-  const uint64_t need = lnx_attn_step_workspace_bytes(a);
+  if ((int64_t)a->B * a->H > MAX_GRID || (int64_t)a->B * a->Hkv * ((a->H / a->Hkv + 31) / 32) * step_splits(a->B, a->H, a->Hkv, S, a->dtype) > MAX_GRID) return lnx_set_error(LNX_ERR_SHAPE, "%s: too many rows", what);
+  const uint64_t need = step_bytes(a->B, a->H, a->Hkv, S, a->d, a->dtype);
   if (need && (!a->workspace || a->workspace_bytes < need || reinterpret_cast<uintptr_t>(a->workspace) % 16))
     return lnx_set_error(LNX_ERR_WORKSPACE, "%s: needs a 16-byte aligned workspace of %llu bytes", what, (unsigned long long)need);
   return LNX_OK;
 }
 
-template <typename T, int D> int launch_step(const lnx_attn_step_args* a, hipStream_t st) {
-  constexpr int W = step_waves<T>();
+template <typename A> StepArgs step_args(const A* a, int outer, int places, int64_t S) {
   StepArgs k{};
   k.q = a->q.p, k.k = a->k.p, k.v = a->v.p, k.kc = a->k_cache.p, k.vc = a->v_cache.p, k.o = a->o, k.len = a->lengths, k.part = static_cast<float*>(a->workspace);
-  auto strides = [a](int64_t* s, const lnx_tensor4& t, int heads) { s[0] = stride_over(a->B, t.stride_b), s[1] = stride_over(heads, t.stride_h); };
-  strides(k.qs, a->q, a->H), strides(k.ks, a->k, a->Hkv), strides(k.vs, a->v, a->Hkv), strides(k.kcs, a->k_cache, a->Hkv), strides(k.vcs, a->v_cache, a->Hkv);
-  k.kcs[2] = stride_over(a->S, a->k_cache.stride_t), k.vcs[2] = stride_over(a->S, a->v_cache.stride_t);
-  k.B = a->B, k.H = a->H, k.Hkv = a->Hkv, k.G = a->H / a->Hkv, k.S = a->S, k.d = a->d, k.scale = a->scale;
-  k.splits = step_splits(a), k.ctiles = (k.G + 31) / 32;
-  const size_t tiles = W * 4 * Tile<T, D, SROWS>::BYTES, sums = W * ((D / 32) * 16 * 64 + 64) * sizeof(float), bytes = tiles > sums ? tiles : sums;
-  const auto kernel = attn_step_kernel<T, D>;
+  auto strides = [](int64_t* s, const lnx_tensor4& t, int rows, int heads) { s[0] = stride_over(rows, t.stride_b), s[1] = stride_over(heads, t.stride_h); };
+  strides(k.qs, a->q, a->B, a->H), strides(k.ks, a->k, a->B, a->Hkv), strides(k.vs, a->v, a->B, a->Hkv), strides(k.kcs, a->k_cache, outer, a->Hkv), strides(k.vcs, a->v_cache, outer, a->Hkv);
+  k.kcs[2] = stride_over(places, a->k_cache.stride_t), k.vcs[2] = stride_over(places, a->v_cache.stride_t);
+  k.B = a->B, k.H = a->H, k.Hkv = a->Hkv, k.G = a->H / a->Hkv, k.S = (int)S, k.d = a->d, k.scale = a->scale;
+  k.splits = step_splits(a->B, a->H, a->Hkv, S, a->dtype), k.ctiles = (k.G + 31) / 32;
+  return k;
+}
+
+template <typename T, int D, bool PAGED> int launch_step(const StepArgs& k, hipStream_t st) {
+  constexpr int W = step_waves<T>();
+  const size_t tiles = W * 4 * Tile<T, D, SROWS>::BYTES + (PAGED ? W * 512 : 0), sums = W * ((D / 32) * 16 * 64 + 64) * sizeof(float), bytes = tiles > sums ? tiles : sums;
+  const auto kernel = attn_step_kernel<T, D, PAGED>;
   if (int rc = lnx_lds_limit(reinterpret_cast<const void*>(kernel), bytes)) return rc;
-  lnx_profile_mark("attn_step", st);
+  lnx_profile_mark(PAGED ? "attn_step_paged" : "attn_step", st);
   hipLaunchKernelGGL(kernel, dim3((unsigned)((int64_t)k.B * k.Hkv * k.ctiles * k.splits)), dim3(64 * W), bytes, st, k);
   if (k.splits > 1) {
     lnx_profile_mark("attn_step_join", st);
-    attn_step_join_kernel<T, D><<<dim3((unsigned)((int64_t)k.B * k.H)), join_threads(k.splits), 0, st>>>(k.part, static_cast<T*>(a->o), k.splits, k.d);
+    attn_step_join_kernel<T, D><<<dim3((unsigned)((int64_t)k.B * k.H)), join_threads(k.splits), 0, st>>>(k.part, static_cast<T*>(k.o), k.splits, k.d);
   }
   return LNX_OK;
 }
 
-}  // namespace
-
-extern "C" uint64_t lnx_attn_step_workspace_bytes(const lnx_attn_step_args* a) {
-  if (!a || a->B <= 0 || a->H <= 0 || a->Hkv <= 0 || a->S <= 0) return 0;
-  const int s = step_splits(a);
-  return s > 1 ? (uint64_t)a->B * a->H * s * ((a->d <= 64 ? 64 : 128) + 4) * sizeof(float) : 0;
-}
-extern "C" int lnx_attn_step(const lnx_attn_step_args* a, void* hip_stream) {
-  if (int rc = check_step(a)) return rc;
-  if (a->B == 0) return LNX_OK;
-  hipStream_t st = static_cast<hipStream_t>(hip_stream);
+template <bool PAGED> int run_step(const char* what, const StepArgs& k, int dtype, hipStream_t st) {
   int rc;
-  if (a->dtype == LNX_BF16) rc = a->d <= 64 ? launch_step<bf16_t, 64>(a, st) : launch_step<bf16_t, 128>(a, st);
-  else rc = a->d <= 64 ? launch_step<float, 64>(a, st) : launch_step<float, 128>(a, st);
+  if (dtype == LNX_BF16) rc = k.d <= 64 ? launch_step<bf16_t, 64, PAGED>(k, st) : launch_step<bf16_t, 128, PAGED>(k, st);
+  else rc = k.d <= 64 ? launch_step<float, 64, PAGED>(k, st) : launch_step<float, 128, PAGED>(k, st);
   if (rc) return rc;
   lnx_profile_mark(nullptr, st);
   const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? LNX_OK : lnx_set_error(LNX_ERR_LAUNCH, "attn_step: %s", hipGetErrorString(e));
+  return e == hipSuccess ? LNX_OK : lnx_set_error(LNX_ERR_LAUNCH, "%s: %s", what, hipGetErrorString(e));
+}
+
+}  // namespace
+
+extern "C" uint64_t lnx_attn_step_workspace_bytes(const lnx_attn_step_args* a) { return a ? step_bytes(a->B, a->H, a->Hkv, a->S, a->d, a->dtype) : 0; }
+extern "C" int lnx_attn_step(const lnx_attn_step_args* a, void* hip_stream) {
+  const char* what = "attn_step";
+  if (!a) return lnx_set_error(LNX_ERR_NULL, "%s: args is NULL", what);
+  if (a->B < 0 || a->H <= 0 || a->Hkv <= 0 || a->H % a->Hkv || a->S <= 0 || a->d <= 0 || a->d > 128 || a->d % 8)
+    return lnx_set_error(LNX_ERR_SHAPE, "%s: unsupported dimensions B=%d H=%d Hkv=%d S=%d d=%d (d a multiple of 8, at most 128; H a multiple of Hkv)", what, a->B, a->H, a->Hkv,
+                         a->S, a->d);
+  if (int rc = check_step(what, a, a->B, a->S, a->S)) return rc;
+  if (a->B == 0) return LNX_OK;
+  return run_step<false>(what, step_args(a, a->B, a->S, a->S), a->dtype, static_cast<hipStream_t>(hip_stream));
+}
+
+static int64_t paged_places(const lnx_attn_step_paged_args* a) { return (int64_t)a->table_width * a->page; }
+extern "C" uint64_t lnx_attn_step_paged_workspace_bytes(const lnx_attn_step_paged_args* a) {
+  return a && a->table_width > 0 && a->page > 0 && paged_places(a) <= INT32_MAX ? step_bytes(a->B, a->H, a->Hkv, paged_places(a), a->d, a->dtype) : 0;
+}
+extern "C" int lnx_attn_step_paged(const lnx_attn_step_paged_args* a, void* hip_stream) {
+  const char* what = "attn_step_paged";
+  if (!a) return lnx_set_error(LNX_ERR_NULL, "%s: args is NULL", what);
+  if (a->B < 0 || a->H <= 0 || a->Hkv <= 0 || a->H % a->Hkv || a->page <= 0 || a->pages <= 0 || a->table_width <= 0 || paged_places(a) > INT32_MAX || a->d <= 0 || a->d > 128 || a->d % 8)
+    return lnx_set_error(LNX_ERR_SHAPE, "%s: unsupported dimensions B=%d H=%d Hkv=%d pages=%d page=%d table_width=%d d=%d (d a multiple of 8, at most 128; H a multiple of Hkv; fewer "
+                         "than 2^31 places a sequence)", what, a->B, a->H, a->Hkv, a->pages, a->page, a->table_width, a->d);
+  if (int rc = check_step(what, a, a->pages, a->page, paged_places(a))) return rc;
+  if (a->B == 0) return LNX_OK;
+  if (!a->page_table) return lnx_set_error(LNX_ERR_NULL, "%s: the page table is required", what);
+  StepArgs k = step_args(a, a->pages, a->page, paged_places(a));
+  k.table = a->page_table, k.table_stride = stride_over(a->B, a->table_stride), k.page = a->page, k.pages = a->pages;
+  return run_step<true>(what, k, a->dtype, static_cast<hipStream_t>(hip_stream));
 }
 
 static bool attn_sizes(const lnx_attn_args* a) { return a && a->B > 0 && a->H > 0 && a->Hkv > 0 && a->T > 0 && a->d > 0 && a->nseq >= 0; }

@@ -1670,6 +1670,54 @@ PyObject* py_causal_attention_step(PyObject*, PyObject* const* args, Py_ssize_t 
   LNX_END
 }
 
+// causal_attention_step_paged(q, k, v, k_pages, v_pages, page_table, lengths, scale or None): o
+PyObject* py_causal_attention_step_paged(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  LNX_BEGIN
+  Args in(args, nargs, 8, "causal_attention_step_paged");
+  const char* op = "causal_attention_step_paged";
+  const Tensor q = in.tensor(0, "q"), k = in.tensor(1, "k"), v = in.tensor(2, "v"), kp = in.tensor(3, "k_pages"), vp = in.tensor(4, "v_pages"), table = in.tensor(5, "page_table"),
+               len = in.tensor(6, "lengths");
+  check_attention(op, q, k, v, 3);
+  const int64_t B = q.size(0), H = q.size(1), Hkv = k.size(1), d = q.size(2);
+  TORCH_CHECK(d % 8 == 0, op, ": head dimension ", d, " is not a multiple of 8, which a cache needs");
+  check_devices(op, q, {{"k_pages", &kp}, {"v_pages", &vp}, {"page_table", &table}, {"lengths", &len}});
+  for (const auto& [name, t] : {std::make_pair("k_pages", &kp), std::make_pair("v_pages", &vp)}) {
+    TORCH_CHECK(t->scalar_type() == q.scalar_type(), op, ": ", name, " must have q's dtype ", q.scalar_type(), ", got ", t->scalar_type());
+    TORCH_CHECK(t->dim() == 4 && t->size(0) > 0 && t->size(1) == Hkv && t->size(2) > 0 && t->size(3) == d && t->sizes() == kp.sizes(), op, ": ", name, " must be [pages, ", Hkv,
+                ", page, ", d, "], got ", shape_text(*t));
+    TORCH_CHECK(vector_rows(*t) && disjoint_rows(*t), op, ": ", name, " is written in place: its rows must be contiguous, 16-byte aligned and each its own memory");
+    TORCH_CHECK(t->size(0) <= INT32_MAX && t->size(2) <= INT32_MAX, op, ": ", name, " is too large, got ", shape_text(*t));
+  }
+  TORCH_CHECK(B == 0 || kp.data_ptr() != vp.data_ptr(), op, ": k_pages and v_pages are the same memory");
+  TORCH_CHECK(len.scalar_type() == at::kInt && len.dim() == 1 && len.size(0) == B && len.is_contiguous(), op, ": lengths must be a contiguous int32 [", B, "] tensor, got ",
+              shape_text(len), " ", len.scalar_type());
+  TORCH_CHECK(table.scalar_type() == at::kInt && table.dim() == 2 && table.size(0) == B && table.size(1) > 0 && (table.size(1) == 1 || table.stride(1) == 1), op,
+              ": page_table must be an int32 [", B, ", pages of a sequence] tensor with contiguous rows, got ", shape_text(table), " ", table.scalar_type());
+  TORCH_CHECK(table.size(1) <= INT32_MAX / kp.size(2), op, ": a sequence of ", table.size(1), " pages of ", kp.size(2), " places is too long");
+  TORCH_CHECK(!wants_grad({&q, &k, &v, &kp, &vp}), "cannot differentiate through a step that updates its cache in place");
+  refuse_tangents(op, {&q, &k, &v, &kp, &vp});
+  const double scale = in.is_none(7) ? 1.0 / std::sqrt((double)d) : in.number(7);
+  TORCH_CHECK_VALUE(std::isfinite((float)scale), op, ": scale must be finite, got ", scale);
+  return THPVariable_Wrap(without_lock([&] {
+    const Tensor qr = as_rows(q), kr = as_rows(k), vr = as_rows(v), o = at::empty({B, H, d}, q.options());
+    lnx_attn_step_paged_args a{};
+    a.B = (int32_t)B, a.H = (int32_t)H, a.Hkv = (int32_t)Hkv, a.d = (int32_t)d, a.dtype = code_of(q.scalar_type()), a.scale = (float)scale;
+    a.page = (int32_t)kp.size(2), a.pages = (int32_t)kp.size(0), a.table_width = (int32_t)table.size(1), a.table_stride = table.stride(0);
+    a.q = tensor4(qr), a.k = tensor4(kr), a.v = tensor4(vr), a.k_cache = tensor4(kp), a.v_cache = tensor4(vp), a.o = ptr(o);
+    a.lengths = static_cast<const int32_t*>(ptr(len)), a.page_table = static_cast<const int32_t*>(ptr(table));
+    a.workspace_bytes = lnx_attn_step_paged_workspace_bytes(&a);
+    Tensor ws;
+    if (a.workspace_bytes) ws = work_area(q, a.workspace_bytes);
+    a.workspace = ptr(ws);
+    const c10::DeviceGuard guard(q.device());
+    check_status(lnx_attn_step_paged(&a, stream_of(q)), "lnx_attn_step_paged");
+    written(kp);
+    written(vp);
+    return o;
+  }));
+  LNX_END
+}
+
 // set_kernel_error(class): the exception a failed C-ABI call raises
 PyObject* py_set_kernel_error(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (nargs != 1 || !PyExceptionClass_Check(args[0])) {
@@ -1683,7 +1731,7 @@ PyObject* py_set_kernel_error(PyObject*, PyObject* const* args, Py_ssize_t nargs
 
 #define LNX_FN(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {LNX_FN(step),     LNX_FN(recurrent), LNX_FN(l2norm), LNX_FN(l2norm_bwd), LNX_FN(chunk), LNX_FN(chunk_segmented),     LNX_FN(conv1d),           LNX_FN(rmsnorm_gated), LNX_FN(gdn_gate),
-                         LNX_FN(kda_gate), LNX_FN(dplr),      LNX_FN(dplr_step), LNX_FN(linrec), LNX_FN(linrec_step), LNX_FN(rmsnorm_residual), LNX_FN(layer_norm), LNX_FN(causal_attention), LNX_FN(causal_attention_step), LNX_FN(set_kernel_error), {nullptr, nullptr, 0, nullptr}};
+                         LNX_FN(kda_gate), LNX_FN(dplr),      LNX_FN(dplr_step), LNX_FN(linrec), LNX_FN(linrec_step), LNX_FN(rmsnorm_residual), LNX_FN(layer_norm), LNX_FN(causal_attention), LNX_FN(causal_attention_step), LNX_FN(causal_attention_step_paged), LNX_FN(set_kernel_error), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_host", "Host path of the linearnexus_amd ops.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
