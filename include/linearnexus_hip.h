@@ -569,6 +569,60 @@ uint64_t lnx_attn_step_paged_workspace_bytes(const lnx_attn_step_paged_args* a);
 int lnx_attn_step_paged(const lnx_attn_step_paged_args* a, void* hip_stream);
 
 /*
+ * Linear attention with a decay for each head, and its gradient:
+ *   S_t = e^{g_t} S_{t-1} + k_t^T v_t,  o_t = scale q_t S_t
+ * q, k, d_q, d_k are [B, H, T, dk], v, o, d_o, d_v [B, H, T, dv] in `dtype`, each with its own strides like the tensors of causal
+ * attention above; dk, dv <= 256.  Rows are whole numbers of 16 bytes: columns behind dk and dv up to the next multiple of 8 (bf16) or 4 (fp32)
+ * exist and hold zeros in the inputs.  g [B, H, T] fp32 with its own strides (any; 0 for a constant), <= 0, -inf drops what came before the token;
+ * d_g is dense [B, H, T], or [H], the sums over rows and tokens, with g_per_head.  States [B, H, dk, dv] ([nseq, H, dk, dv] packed) dense fp32;
+ * initial_state, d_final_state (zeros) and d_initial_state may be NULL.  The forward call leaves in `kept` what the backward call reads (NULL:
+ * no backward pass will follow; lnx_decay_kept_bytes may be 0); the backward call reads the forward call's inputs, `kept`, and final_state where d_final_state
+ * is given.  The workspace (16-byte aligned, may be NULL where its size is 0; the forward size depends on whether kept is set) holds nothing between
+ * calls.  No atomics.
+ */
+typedef struct lnx_decay_args {
+  int32_t B, H, T, dk, dv, nseq, dtype, g_per_head;
+  float scale;
+  int32_t reserved;
+  lnx_tensor4 q, k, v, o;
+  lnx_tensor4 d_o, d_q, d_k, d_v;  /* backward only */
+  const float* g;
+  int64_t g_stride_b, g_stride_h, g_stride_t;
+  const int32_t* cu_seqlens;
+  const float* initial_state;
+  float* final_state;
+  float* kept;
+  void* workspace;
+  uint64_t workspace_bytes;
+  const float* d_final_state;      /* backward only, from here */
+  float* d_g;
+  float* d_initial_state;
+} lnx_decay_args;
+uint64_t lnx_decay_kept_bytes(const lnx_decay_args* a);
+uint64_t lnx_decay_fwd_workspace_bytes(const lnx_decay_args* a);
+uint64_t lnx_decay_bwd_workspace_bytes(const lnx_decay_args* a);
+int lnx_decay_fwd(const lnx_decay_args* a, void* hip_stream);
+int lnx_decay_bwd(const lnx_decay_args* a, void* hip_stream);
+
+/*
+ * One token of it: q, k [B, H, dk] (dk <= 256), v, o [B, H, dv] dense in `dtype`, g [B, H] fp32 with its own strides, states [B, H, dk, dv] dense
+ * fp32; new_state may be state.
+ */
+typedef struct lnx_decay_step_args {
+  int32_t B, H, dk, dv, dtype;
+  float scale;
+  const void* q;
+  const void* k;
+  const void* v;
+  const float* g;
+  int64_t g_stride_b, g_stride_h;
+  const float* state;
+  void* o;
+  float* new_state;
+} lnx_decay_step_args;
+int lnx_decay_step(const lnx_decay_step_args* a, void* hip_stream);
+
+/*
  * Optional per-kernel timing for benchmarks (no counterpart in the reference; its micro-benchmark
  * times whole jitted ops, bench_kda_kernels.py:216-249).  While enabled (process-wide),
  * every entry point records HIP events around each kernel it launches, on the caller's stream.

@@ -1,6 +1,7 @@
 """MI355X-native delta-rule scan (DeltaNet / Gated DeltaNet / KDA) behind the reference's op names."""
 from .attention import causal_attention, causal_attention_step, causal_attention_step_paged
 from .backend import KernelBackend, select_kernel_backend
+from .decay_attention import decay_linear_attention, decay_linear_attention_step
 from .conv import depthwise_conv1d_causal
 from .gate import gated_deltanet_gate, kda_gate
 from .norm import layer_norm, rmsnorm_gated, rmsnorm_residual
@@ -32,4 +33,5 @@ __all__ = [
     "dplr_delta_rule_recurrent", "dplr_delta_rule_step", "rmsnorm_gated", "kda_gate", "gated_deltanet_gate",
     "gated_linear_recurrence", "gated_linear_recurrence_step", "rmsnorm_residual", "layer_norm",
     "causal_attention", "causal_attention_step", "causal_attention_step_paged",
+    "decay_linear_attention", "decay_linear_attention_step",
 ]

@@ -23,6 +23,7 @@ EXPORTS = (
     "lnx_rmsnorm_residual_bwd_workspace_bytes", "lnx_rmsnorm_residual_fwd", "lnx_rmsnorm_residual_bwd",
     "lnx_layer_norm_bwd_workspace_bytes", "lnx_layer_norm_fwd", "lnx_layer_norm_bwd",
     "lnx_attn_fwd_workspace_bytes", "lnx_attn_bwd_workspace_bytes", "lnx_attn_fwd", "lnx_attn_bwd", "lnx_attn_step_workspace_bytes", "lnx_attn_step", "lnx_attn_step_paged_workspace_bytes", "lnx_attn_step_paged",
+    "lnx_decay_kept_bytes", "lnx_decay_fwd_workspace_bytes", "lnx_decay_bwd_workspace_bytes", "lnx_decay_fwd", "lnx_decay_bwd", "lnx_decay_step",
     "lnx_profile_enable", "lnx_profile_read",
 )
 
@@ -145,6 +146,29 @@ class AttnStepPagedArgs(C.Structure):
     ]
 
 
+class DecayArgs(C.Structure):
+    """Mirror of ``struct lnx_decay_args``."""
+
+    _fields_ = [
+        ("B", C.c_int32), ("H", C.c_int32), ("T", C.c_int32), ("dk", C.c_int32), ("dv", C.c_int32), ("nseq", C.c_int32), ("dtype", C.c_int32),
+        ("g_per_head", C.c_int32), ("scale", C.c_float), ("reserved", C.c_int32),
+        ("q", Tensor4), ("k", Tensor4), ("v", Tensor4), ("o", Tensor4), ("d_o", Tensor4), ("d_q", Tensor4), ("d_k", Tensor4), ("d_v", Tensor4),
+        ("g", C.c_void_p), ("g_stride_b", C.c_int64), ("g_stride_h", C.c_int64), ("g_stride_t", C.c_int64), ("cu_seqlens", C.c_void_p),
+        ("initial_state", C.c_void_p), ("final_state", C.c_void_p), ("kept", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
+        ("d_final_state", C.c_void_p), ("d_g", C.c_void_p), ("d_initial_state", C.c_void_p),
+    ]
+
+
+class DecayStepArgs(C.Structure):
+    """Mirror of ``struct lnx_decay_step_args``."""
+
+    _fields_ = [
+        ("B", C.c_int32), ("H", C.c_int32), ("dk", C.c_int32), ("dv", C.c_int32), ("dtype", C.c_int32), ("scale", C.c_float),
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("g", C.c_void_p), ("g_stride_b", C.c_int64), ("g_stride_h", C.c_int64),
+        ("state", C.c_void_p), ("o", C.c_void_p), ("new_state", C.c_void_p),
+    ]
+
+
 _lib = None
 
 
@@ -252,6 +276,14 @@ def load() -> C.CDLL:
     lib.lnx_attn_step_paged_workspace_bytes.argtypes = [C.POINTER(AttnStepPagedArgs)]
     lib.lnx_attn_step_paged.restype = C.c_int
     lib.lnx_attn_step_paged.argtypes = [C.POINTER(AttnStepPagedArgs), C.c_void_p]
+    for name in ("lnx_decay_kept_bytes", "lnx_decay_fwd_workspace_bytes", "lnx_decay_bwd_workspace_bytes"):
+        getattr(lib, name).restype = C.c_uint64
+        getattr(lib, name).argtypes = [C.POINTER(DecayArgs)]
+    for name in ("lnx_decay_fwd", "lnx_decay_bwd"):
+        getattr(lib, name).restype = C.c_int
+        getattr(lib, name).argtypes = [C.POINTER(DecayArgs), C.c_void_p]
+    lib.lnx_decay_step.restype = C.c_int
+    lib.lnx_decay_step.argtypes = [C.POINTER(DecayStepArgs), C.c_void_p]
     lib.lnx_profile_enable.restype = C.c_int
     lib.lnx_profile_enable.argtypes = [C.c_int]
     lib.lnx_profile_read.restype = C.c_int

@@ -133,11 +133,6 @@ template <int D, int R> struct Tile<float, D, R> {
   }
 };
 
-// 16 bytes a lane from `base` + off bytes straight to LDS, lane l at dst + 16 l; the base is the wave's, so a tile's loads cost no
-// vector arithmetic
-__device__ __forceinline__ void dma16_at(const void* base, unsigned off, unsigned dst) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(__builtin_amdgcn_readfirstlane(dst)) : "memory", "m0");
-}
 // Brings tiles of [len][d] matrices with one row stride to LDS by the workgroup's four waves: which bytes a lane fetches is formed once.
 template <typename T, int D, int R = ROWS> struct Mover {
   typedef Tile<T, D, R> TL;

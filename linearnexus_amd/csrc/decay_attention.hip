@@ -1,0 +1,948 @@
+// Linear attention with a decay for each head, forward, backward and one token:
+//   S_t = e^{g_t} S_{t-1} + k_t^T v_t     o_t = scale q_t S_t
+//   dS_t = scale q_t^T do_t + e^{g_{t+1}} dS_{t+1}     dq_t = scale do_t S_t^T     dk_t = v_t dS_t^T     dv_t = k_t dS_t     dg_t = e^{g_t} <dS_t, S_{t-1}>
+// All four results are one walk over chunks of C tokens, forwards or backwards (G: sums of g within the chunk):
+//   out_i = sum_{j <= i} (x_i . y_j) e^{G_i - G_j} z_j + e^{G_i} x_i S       S <- e^{G_C} S + sum_j e^{G_C - G_j} y_j^T z_j
+// with (x, y, z) = (q, k, v) for o, (do, v, k) for dq and, mirrored in time, (v, do, q) for dk and (k, q, do) for dv.  A workgroup walks 64
+// columns of z: each of its four waves keeps 16 columns of the state in registers, in the layout of a product's result, which is the layout
+// of the next product's operand (tile pairs of 16 x 16), so the state never leaves them.  A chunk's pairs are formed once per workgroup
+// and handed over through LDS.
+// Rounding (bf16): pairs, the state as an operand and the z_j with their factors enter the products in two bf16 parts (2^-16 of each term), so results
+// are off by their own rounding alone, and dg, a running difference of x . out and y . out over a whole sequence, keeps its digits.
+// Exponents are differences of sums over a chunk: the sums are held as a multiple of 1/64 and a rest, so that a difference is exact to a unit
+// however far the sums have run (a decay of e^-100 beside one of 1).
+#include "lnx_common.h"
+#include "mma_tiles.h"
+#include "packed_slots.h"
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int SLAB = 64;                        // columns of z of a workgroup: 16 a wave
+constexpr int64_t MAX_GRID = 0xffffffff / 256;  // workgroups of a launch
+typedef __attribute__((address_space(3))) char lds_char;
+
+// Products of 16 x 16 tiles: K contraction slots an operand, which the results of TP tiles fill.  Slot (a, r) of lane group g = lane / 16 is
+// index 16 a + 4 g + r of the K: element r of that group in result tile a.
+template <typename T> struct Form;
+template <> struct Form<bf16_t> {
+  static constexpr int C = 64, K = 32, TP = 2, PARTS = 2;
+  typedef bf16x8 Frag;
+  static __device__ __forceinline__ void mma(floatx4& c, const Frag& a, const Frag& b) { c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ void put(Frag& f, int a, int r, float x) { f[4 * a + r] = (bf16_t)x; }
+  static __device__ __forceinline__ float get(const Frag& f, int a, int r) { return (float)f[4 * a + r]; }
+};
+template <> struct Form<float> {
+  static constexpr int C = 32, K = 16, TP = 1, PARTS = 1;
+  typedef floatx4 Frag;
+  static __device__ __forceinline__ void mma(floatx4& c, const Frag& a, const Frag& b) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], b[r], c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ void put(Frag& f, int, int r, float x) { f[r] = x; }
+  static __device__ __forceinline__ float get(const Frag& f, int, int r) { return f[r]; }
+};
+__device__ __forceinline__ bool is_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
+
+// Result tiles as an operand, and what its rounding left (of an infinite value nothing)
+__device__ __forceinline__ void split(const floatx4 (&v)[2], bf16x8& hi, bf16x8& lo) {
+  hi = Mma16::from_acc(v[0], v[1]);
+  floatx4 d[2];
+#pragma unroll
+  for (int a = 0; a < 2; ++a)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float h = (float)hi[4 * a + r];
+      d[a][r] = is_finite(h) ? v[a][r] - h : 0.f;
+    }
+  lo = Mma16::from_acc(d[0], d[1]);
+}
+__device__ __forceinline__ void split(const floatx4 (&v)[1], floatx4& hi, floatx4&) { hi = v[0]; }
+
+// A [C][W] tile in LDS as loads that go straight there leave it: 16-byte granules of a row permuted by an exclusive or with x(row), chosen so that
+// row operands (16 consecutive rows, one granule) and column operands (the transposing reads of two lane groups: 8 consecutive rows, 2 granules;
+// fp32: rows 4 g + r for one r, 4 granules) touch every bank once.  x depends on row % 16 only.
+template <typename V> __device__ __forceinline__ V lds_load(unsigned addr) { return *(__attribute__((address_space(3))) const V*)(lds_char*)(uintptr_t)addr; }
+template <typename T, int W> struct Cells;
+template <int W> struct Cells<bf16_t, W> {
+  static constexpr int ROWB = 2 * W, G = W / 8;
+  static __device__ __forceinline__ int x(int r) { return G == 8 ? (r & 6) | ((r >> 3) & 1) : ((r & 3) << 2) | ((r >> 1) & 2) | ((r >> 3) & 1); }
+  static __device__ __forceinline__ void src(int p, int& r, int& c) {  // row and first column of granule p of the tile's memory
+    r = p / G;
+    c = ((p % G) ^ x(r)) << 3;
+  }
+  static __device__ __forceinline__ unsigned rows(int lane) {
+    const int r = lane & 15, g = lane >> 4;
+    return r * ROWB + (((g >> 1) ^ x(r)) << 4) + 8 * (g & 1);
+  }
+  // columns K s + slots of the row that `rows` points at; `off`: whole groups of 16 rows, tiles
+  static __device__ __forceinline__ bf16x8 by_row(unsigned rows, int off, int s) {
+    typedef float float2_ __attribute__((ext_vector_type(2)));
+    typedef const volatile __attribute__((address_space(3))) float2_ lds_float2;  // (kept apart: one ds_read2_b64 takes longer than two ds_read_b64)
+    const float2_ lo = *(lds_float2*)(lds_char*)(uintptr_t)((rows ^ (64 * s)) + off), hi = *(lds_float2*)(lds_char*)(uintptr_t)((rows ^ (64 * s + 32)) + off);
+    return Mma16::join(__builtin_bit_cast(bf16x4, lo), __builtin_bit_cast(bf16x4, hi));
+  }
+  static __device__ __forceinline__ unsigned cols(int lane) {
+    const int s = lane & 15, r = 4 * (lane >> 4) + (s >> 2);
+    return r * ROWB + ((((s >> 1) & 1) ^ x(r)) << 4) + 8 * (s & 1);
+  }
+  // rows k0 + slots of column 16 i + (lane & 15)
+  static __device__ __forceinline__ bf16x8 by_col(unsigned cols, int k0, int i) {
+    typedef short short4_ __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) short4_ lds_short4;
+    const unsigned at = (cols ^ (32 * i)) + k0 * ROWB;
+    return Mma16::join(__builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(lds_char*)(uintptr_t)at)),
+                       __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(lds_char*)(uintptr_t)(at + 16 * ROWB))));
+  }
+};
+template <int W> struct Cells<float, W> {
+  static constexpr int ROWB = 4 * W, G = W / 4;
+  static __device__ __forceinline__ int x(int r) { return (r & 12) | (r & 3); }
+  static __device__ __forceinline__ void src(int p, int& r, int& c) {
+    r = p / G;
+    c = ((p % G) ^ x(r)) << 2;
+  }
+  static __device__ __forceinline__ unsigned rows(int lane) {
+    const int r = lane & 15;
+    return r * ROWB + (((lane >> 4) ^ x(r)) << 4);
+  }
+  static __device__ __forceinline__ floatx4 by_row(unsigned rows, int off, int s) { return lds_load<floatx4>((rows ^ (64 * s)) + off); }
+  static __device__ __forceinline__ unsigned cols(int lane) {
+    const int l = lane & 15, g = lane >> 4;
+    return 4 * g * ROWB + (((l >> 2) ^ (4 * g)) << 4) + 4 * (l & 3);
+  }
+  static __device__ __forceinline__ floatx4 by_col(unsigned cols, int k0, int i) {
+    floatx4 f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) f[r] = lds_load<float>((cols ^ (16 * r) ^ (64 * i)) + (k0 + r) * ROWB);
+    return f;
+  }
+};
+
+// Sum over the lanes up to this one
+template <int CTRL, int ROWS> __device__ __forceinline__ float from_lane(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, ROWS, 0xF, false));
+}
+__device__ __forceinline__ float running_sum(float x) {
+  x += from_lane<0x111, 0xF>(x);  // row_shr:1, 2, 4, 8
+  x += from_lane<0x112, 0xF>(x);
+  x += from_lane<0x114, 0xF>(x);
+  x += from_lane<0x118, 0xF>(x);
+  x += from_lane<0x142, 0xA>(x);  // row_bcast:15 into rows 1 and 3
+  x += from_lane<0x143, 0xC>(x);  // row_bcast:31 into rows 2 and 3
+  return x;
+}
+__device__ __forceinline__ float lane_value(float x, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane)); }
+
+// 2^(difference of two sums), each a multiple of 1/64 and a rest
+__device__ __forceinline__ float between(float h1, float l1, float h0, float l0) {
+#pragma clang fp reassociate(off)
+  const float h = h1 - h0, l = l1 - l0;
+  return __builtin_amdgcn_exp2f(h + l);
+}
+
+struct Side {
+  void* p;
+  int64_t sb, sh, st;  // strides of batch, head and token in elements
+};
+// One walk.  The state is [width of y][width of z]; in memory always [dk][dv], `turned` says that y runs along dv.
+struct Role {
+  Side x, y, z, w, out;  // w: what the results are multiplied with for dg
+  int kw, vw;            // widths of x and y, of z and out
+  int sk, sn;            // the state's, which the tensors may exceed by columns of zeros
+  int rev, turned, slabs;
+  float row_scale, col_scale;  // of a state's part of the results; of what a token adds to the state
+  const float* init;
+  float* fin;
+  float* dots;  // [inter, pairs][slab][B H][T]
+};
+struct Walk {
+  Role role[3];
+  const float* g;
+  int64_t gb, gh, gt;
+  const int32_t* cu;
+  float* whole;      // local walks: every segment's factor e^{sum g}, [slot][H]
+  int B, H, T, nseq, dv;
+  int seg, nseg;     // tokens of a segment; segments of a dense row
+  int by_slot;       // init is per segment, not per row
+  int units, per;    // (slot, head) pairs; workgroups of each
+  int64_t dots_step; // from one slab's dots to the next
+  float scale;
+};
+
+// Where a segment lies: its row (batch row or sequence), first token, length; whether it is its row's first or last
+struct Spot {
+  int b, row, len;
+  int64_t tok;
+  bool on, first, last;
+};
+__device__ __forceinline__ Spot spot(const Walk& a, int slot) {
+  Spot s;
+  if (!a.nseq) {
+    s.b = s.row = slot / a.nseg;
+    const int i = slot % a.nseg;
+    s.tok = (int64_t)i * a.seg;
+    s.len = min(a.seg, a.T - (int)s.tok);
+    s.on = true, s.first = i == 0, s.last = i == a.nseg - 1;
+    return s;
+  }
+  s.b = 0;
+  s.row = packed_owner(a.cu, a.nseq, a.T, a.seg, slot);
+  const int from = seq_first(a.cu, s.row, a.T), len = seq_end(a.cu, s.row, a.T) - from;
+  const int n = max(1, (int)(((unsigned)len + a.seg - 1) / a.seg)), i = (int)(slot - packed_slot(from, s.row, a.seg));
+  s.tok = from + (int64_t)i * a.seg;
+  s.len = min(a.seg, len - i * a.seg);
+  s.on = i >= 0 && i < n, s.first = i == 0, s.last = i == n - 1;
+  return s;
+}
+
+// Brings [C][W] tiles to LDS by the workgroup's four waves; which bytes a lane fetches is formed once.
+template <typename T, int W> struct Mover {
+  typedef Cells<T, W> CL;
+  static constexpr int C = Form<T>::C, N = C * CL::ROWB / 1024 / 4;
+  unsigned off[N];
+  __device__ __forceinline__ Mover(int64_t st, int wave, int lane) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      int r, c;
+      CL::src(64 * (wave * N + i) + lane, r, c);
+      off[i] = (unsigned)((r * (int)st + c) * (int)sizeof(T));
+    }
+  }
+  // rows t0 .. t0 + C - 1; rows behind the last of `valid` are copies of it, columns behind `width` keep the zeros that lie there
+  __device__ __forceinline__ void fetch(unsigned tile, const T* matrix, int64_t st, int64_t t0, int valid, int width, int wave, int lane) const {
+    const T* base = matrix + t0 * st;
+    if (valid == C && width >= W) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) dma16_at(base, off[i], tile + 1024 * (wave * N + i));
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < N; ++i) {
+        int r, c;
+        CL::src(64 * (wave * N + i) + lane, r, c);
+        if (c < width) dma16(base + (int64_t)min(r, valid - 1) * st + c, tile + 1024 * (wave * N + i));
+      }
+    }
+  }
+};
+
+template <typename T> __device__ __forceinline__ const T* head_of(const Side& s, const Spot& p, int h) {
+  return static_cast<const T*>(s.p) + p.b * s.sb + h * s.sh + p.tok * s.st;
+}
+
+template <typename T, int KW, int BUFS, bool OUT> struct Room {
+  static constexpr int C = Form<T>::C, NI = C / 16, NJ = C / Form<T>::K;
+  static constexpr int XB = C * KW * sizeof(T), ZB = C * SLAB * sizeof(T), BUF = (OUT ? 2 : 1) * XB + ZB;
+  static constexpr int PAIRS = BUFS * BUF, GATES = PAIRS + (OUT ? NI * NJ * Form<T>::PARTS * 1024 : 0), RAW = GATES + 4 * 1024, DOTS = RAW + BUFS * 256;
+  static constexpr int BYTES = DOTS + (OUT ? 4 * 2 * C * 4 : 0);
+};
+
+// OUT: false for the local walks of segments, which leave what a segment adds to the state and nothing else.
+template <typename T, int KW, int BUFS, bool OUT> __global__ __launch_bounds__(256) void decay_walk_kernel(Walk a) {
+  typedef Form<T> F;
+  typedef typename F::Frag Frag;
+  typedef Cells<T, KW> XC;
+  typedef Cells<T, SLAB> ZC;
+  typedef Room<T, KW, BUFS, OUT> R;
+  constexpr int C = F::C, NI = R::NI, NJ = R::NJ, NS = KW / F::K, NT = KW / 16, WPI = 4 / NI;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g4 = 4 * (lane >> 4);
+  // workgroups of one (slot, head) follow each other on one XCD, whose L2 then holds what they share
+  int w = blockIdx.x, unit, item;
+  if (a.units % 8 == 0) {
+    unit = (w >> 3) / a.per * 8 + (w & 7);
+    item = (w >> 3) % a.per;
+  } else {
+    unit = w / a.per;
+    item = w % a.per;
+  }
+  int which = 0;
+  while (item >= a.role[which].slabs) item -= a.role[which++].slabs;
+  const Role& ro = a.role[which];
+  const int slot = unit / a.H, h = unit % a.H;
+  const Spot p = spot(a, slot);
+  if (!p.on) return;
+  const bool rev = ro.rev;
+  if (!OUT && (rev ? p.first : p.last)) return;  // nothing walks on from there
+  const int col0 = item * SLAB, vw = min(SLAB, ro.vw - col0), n0 = col0 + 16 * wave;
+  const int nchunk = (p.len + C - 1) / C;
+  const T* xp = OUT ? head_of<T>(ro.x, p, h) : nullptr;
+  const T* yp = head_of<T>(ro.y, p, h);
+  const T* zp = head_of<T>(ro.z, p, h) + col0;
+  const float* gp = a.g + p.b * a.gb + h * a.gh + p.tok * a.gt;
+  const unsigned lds0 = lds_byte_addr(lds);
+  const auto xt = [&](int buf) { return lds0 + buf * R::BUF + R::XB + R::ZB; };
+  const auto yt = [&](int buf) { return lds0 + buf * R::BUF; };
+  const auto zt = [&](int buf) { return lds0 + buf * R::BUF + R::XB; };
+  float* gates = reinterpret_cast<float*>(lds + R::GATES) + 256 * wave;  // of this wave: sums' multiples, rests, row factors, column factors
+  const float* raw = reinterpret_cast<const float*>(lds + R::RAW);
+  if (ro.kw < KW || vw < SLAB) {
+    for (int i = threadIdx.x * 16; i < R::PAIRS; i += 256 * 16) *reinterpret_cast<floatx4*>(lds + i) = floatx4{0.f, 0.f, 0.f, 0.f};
+    lds_barrier();
+  }
+  const Mover<T, KW> mx(OUT ? ro.x.st : 0, wave, lane), my(ro.y.st, wave, lane);
+  const Mover<T, SLAB> mz(ro.z.st, wave, lane);
+  const auto fetch = [&](int chunk, int buf) {
+    const int t0 = chunk * C, valid = min(C, p.len - t0);
+    if constexpr (OUT) mx.fetch(xt(buf), xp, ro.x.st, t0, valid, ro.kw, wave, lane);
+    my.fetch(yt(buf), yp, ro.y.st, t0, valid, ro.kw, wave, lane);
+    mz.fetch(zt(buf), zp, ro.z.st, t0, valid, vw, wave, lane);
+    if (wave == 0) dma4(gp + (int64_t)(t0 + min(lane, valid - 1)) * a.gt, lds0 + R::RAW + 256 * buf);
+  };
+  // the state: tile i holds rows 16 i + 4 g + r of column n0 + l16
+  floatx4 st[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) st[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+  const int n = n0 + l16, step_k = ro.turned ? 1 : a.dv, step_n = ro.turned ? a.dv : 1;
+  const int64_t state_size = (int64_t)ro.sk * ro.sn;
+  if (OUT && ro.init) {
+    const float* s = ro.init + ((int64_t)(a.by_slot ? slot : p.row) * a.H + h) * state_size + (int64_t)n * step_n;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (16 * i + g4 + r < ro.sk && n < ro.sn) st[i][r] = s[(int64_t)(16 * i + g4 + r) * step_k];
+  }
+  float* red = reinterpret_cast<float*>(lds + R::DOTS);  // [wave][inter, pairs][C]
+  const bool dots = OUT && ro.dots;
+  const auto leave_dots = [&](int chunk) {
+    const int t0 = chunk * C, i = threadIdx.x % C, kind = threadIdx.x / C;
+    if (kind < 2 && t0 + i < p.len) {
+      const float* q = red + kind * C + i;
+      ro.dots[(int64_t)(kind * ro.slabs + item) * a.dots_step + (int64_t)(p.b * a.H + h) * a.T + p.tok + t0 + i] = (q[0] + q[2 * C]) + (q[4 * C] + q[6 * C]);
+    }
+  };
+  float whole_h = 0.f, whole_l = 0.f;
+  int done = -1;  // the chunk before
+  bool counted = false;
+  if (nchunk > 0) fetch(rev ? nchunk - 1 : 0, 0);
+  for (int it = 0; it < nchunk; ++it) {
+    const int chunk = rev ? nchunk - 1 - it : it, t0 = chunk * C, valid = min(C, p.len - t0), buf = BUFS == 2 ? it & 1 : 0;
+    if (counted) dma_wait<NI>();  // all but the results of the chunk before
+    else dma_wait<0>();
+    lds_barrier();
+    floatx4 wv[NI];
+    if (dots) {
+      if (it > 0) leave_dots(done);
+      const T* wp = head_of<T>(ro.w, p, h) + (int64_t)t0 * ro.w.st + n0 + g4;
+#pragma unroll
+      for (int t = 0; t < NI; ++t) {
+        wv[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+        if (16 * t + l16 < valid && n0 + g4 < ro.vw) wv[t] = load4(wp + (int64_t)(16 * t + l16) * ro.w.st);
+      }
+    }
+    if (BUFS == 2 && it + 1 < nchunk) fetch(rev ? chunk - 1 : chunk + 1, buf ^ 1);
+    // ---- the chunk's decays: lane = token
+    float gv = lane < valid ? raw[64 * buf + lane] * LOG2E : 0.f;
+    gv = gv < -200.f ? -200.f : gv;  // e^-138 is nothing
+    const float gm = rintf(gv * 64.f) * (1.f / 64.f), H = running_sum(gm), L = running_sum(gv - gm), HT = lane_value(H, 63), LT = lane_value(L, 63);
+    const float head = between(H, L, 0.f, 0.f), tail = between(HT, LT, H, L), total = between(HT, LT, 0.f, 0.f);
+    gates[lane] = H;
+    gates[64 + lane] = L;
+    gates[128 + lane] = (rev ? tail : head) * ro.row_scale;
+    gates[192 + lane] = lane < valid ? (rev ? head : tail) * ro.col_scale : 0.f;
+    if (!OUT) whole_h += HT, whole_l += LT;
+    const unsigned xr = xt(buf) + XC::rows(lane), yr = yt(buf) + XC::rows(lane), yc = yt(buf) + XC::cols(lane), zc = zt(buf) + ZC::cols(lane);
+    char* pairs = lds + R::PAIRS;
+    const auto needed = [&](int i, int j) { return rev ? F::K * j + F::K > 16 * i : F::K * j <= 16 * i + 15; };  // pairs of row tile i with columns of block j
+    floatx4 acc[NI];
+    if constexpr (OUT) {
+      // ---- pairs of one row tile a wave: rows of the result are j, its column is i
+      const int it16 = wave / WPI, i = 16 * it16 + l16;
+      floatx4 sc[NJ][F::TP];
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int t = 0; t < F::TP; ++t) sc[j][t] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        const Frag xf = XC::by_row(xr, it16 * 16 * XC::ROWB, s);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+          if (j % WPI == wave % WPI && needed(it16, j)) {
+#pragma unroll
+            for (int t = 0; t < F::TP; ++t) F::mma(sc[j][t], XC::by_row(yr, (F::K * j + 16 * t) * XC::ROWB, s), xf);
+          }
+      }
+      const float hi_ = gates[i], li_ = gates[64 + i];
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+        if (j % WPI == wave % WPI && needed(it16, j)) {
+#pragma unroll
+          for (int t = 0; t < F::TP; ++t) {
+            const int j0 = F::K * j + 16 * t + g4;
+            const floatx4 hj = load4(gates + j0), lj = load4(gates + 64 + j0);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const bool on = rev ? j0 + r >= i && j0 + r < valid : j0 + r <= i;
+              const float f = (rev ? between(hj[r], lj[r], hi_, li_) : between(hi_, li_, hj[r], lj[r])) * a.scale;
+              sc[j][t][r] = on ? sc[j][t][r] * f : 0.f;
+            }
+          }
+          Frag hi, lo;
+          split(sc[j], hi, lo);
+          char* q = pairs + (it16 * NJ + j) * F::PARTS * 1024 + 16 * lane;
+          *reinterpret_cast<Frag*>(q) = hi;
+          if (F::PARTS == 2) *reinterpret_cast<Frag*>(q + 1024) = lo;
+        }
+      // ---- what the state gives: rows of the result are columns of z, its column is i
+#pragma unroll
+      for (int t = 0; t < NI; ++t) acc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        Frag hi, lo;
+        floatx4 v[F::TP];
+#pragma unroll
+        for (int t = 0; t < F::TP; ++t) v[t] = st[F::TP * s + t];
+        split(v, hi, lo);
+#pragma unroll
+        for (int t = 0; t < NI; ++t) {
+          const Frag xf = XC::by_row(xr, 16 * t * XC::ROWB, s);
+          F::mma(acc[t], hi, xf);
+          if (F::PARTS == 2) F::mma(acc[t], lo, xf);
+        }
+      }
+    }
+    // ---- z by columns, as it is and with each token's factor
+    Frag zf[NJ], zh[NJ], zl[NJ];
+    bool odd = false;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      zf[j] = ZC::by_col(zc, F::K * j, wave);
+      floatx4 v[F::TP];
+#pragma unroll
+      for (int t = 0; t < F::TP; ++t) {
+        const floatx4 f = load4(gates + 192 + F::K * j + 16 * t + g4);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float z = F::get(zf[j], t, r);
+          const bool fine = is_finite(z);
+          odd = odd || !fine;
+          v[t][r] = fine || F::K * j + 16 * t + g4 + r < valid ? z * f[r] : 0.f;
+          if (!fine) F::put(zf[j], t, r, 0.f);
+        }
+      }
+      split(v, zh[j], zl[j]);
+    }
+    odd = __any(odd);
+    // ---- the state behind the chunk
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      st[i] *= total;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const Frag yf = XC::by_col(yc, F::K * j, i);
+        F::mma(st[i], yf, zh[j]);
+        if (F::PARTS == 2) F::mma(st[i], yf, zl[j]);
+      }
+    }
+    if (OUT || BUFS == 1) lds_barrier();  // the pairs are there, and nothing reads the tiles any more
+    if (BUFS == 1 && it + 1 < nchunk) fetch(rev ? chunk - 1 : chunk + 1, 0);
+    if constexpr (OUT) {
+      float inter[NI];
+#pragma unroll
+      for (int t = 0; t < NI; ++t) {
+        acc[t] *= gates[128 + 16 * t + l16];
+        if (dots) inter[t] = acc[t][0] * wv[t][0] + acc[t][1] * wv[t][1] + acc[t][2] * wv[t][2] + acc[t][3] * wv[t][3];
+      }
+      floatx4 in[NI];
+#pragma unroll
+      for (int t = 0; t < NI; ++t) {
+        in[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+          if (needed(t, j)) {
+            const char* q = pairs + (t * NJ + j) * F::PARTS * 1024 + 16 * lane;
+            F::mma(in[t], zf[j], *reinterpret_cast<const Frag*>(q));
+            if (F::PARTS == 2) F::mma(in[t], zf[j], *reinterpret_cast<const Frag*>(q + 1024));
+          }
+      }
+      if (odd) {  // values that are not finite were taken out of the product, where a masked pair would be 0 times one: added pair by pair
+#pragma unroll 1
+        for (int j = 0; j < valid; ++j) {
+          const bool here = n0 + g4 < ro.vw;
+          const floatx4 z = here ? load4(zp + (int64_t)(t0 + j) * ro.z.st + 16 * wave + g4) : floatx4{0.f, 0.f, 0.f, 0.f};
+          const int k = j % F::K, e = k % 4, tile = k / 16, from = (k % 16) / 4;  // its slot and the lane group that holds it
+#pragma unroll
+          for (int t = 0; t < NI; ++t) {
+            const int i = 16 * t + l16;
+            if (rev ? j < i : j > i) continue;
+            const T* q = reinterpret_cast<const T*>(pairs + (t * NJ + j / F::K) * F::PARTS * 1024 + 16 * (16 * from + l16)) + 4 * tile + e;
+            const float x = to_f32(q[0]) + (F::PARTS == 2 ? to_f32(q[1024 / sizeof(T)]) : 0.f);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (!is_finite(z[r])) in[t][r] += x * z[r];
+          }
+        }
+      }
+      T* op = const_cast<T*>(head_of<T>(ro.out, p, h)) + (int64_t)t0 * ro.out.st + n0 + g4;
+#pragma unroll
+      for (int t = 0; t < NI; ++t) {
+        if (dots) {
+          float x = inter[t], y = in[t][0] * wv[t][0] + in[t][1] * wv[t][1] + in[t][2] * wv[t][2] + in[t][3] * wv[t][3];
+          x = xor32_sum(xor16_sum(x));
+          y = xor32_sum(xor16_sum(y));
+          if (g4 == 0) red[(2 * wave) * C + 16 * t + l16] = x, red[(2 * wave + 1) * C + 16 * t + l16] = y;
+        }
+        if (16 * t + l16 < valid && n0 + g4 < ro.vw) store4(op + (int64_t)(16 * t + l16) * ro.out.st, acc[t] + in[t]);
+      }
+      counted = valid == C && n0 + 16 <= ro.vw;
+    }
+    done = chunk;
+  }
+  if (dots && nchunk > 0) {
+    lds_barrier();
+    leave_dots(done);
+  }
+  if (ro.fin && (!OUT || (rev ? p.first : p.last))) {
+    float* s = ro.fin + ((int64_t)(OUT ? p.row : slot) * a.H + h) * state_size + (int64_t)n * step_n;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (16 * i + g4 + r < ro.sk && n < ro.sn) s[(int64_t)(16 * i + g4 + r) * step_k] = st[i][r];
+  }
+  if (!OUT && item == 0 && threadIdx.x == 0) a.whole[(int64_t)slot * a.H + h] = between(whole_h, whole_l, 0.f, 0.f);
+}
+
+// States before every segment (behind it, backwards) from what each adds: in place, four elements a thread, a row's segments one after the other.
+struct Join {
+  float* states;
+  const float *whole, *init;
+  const int32_t* cu;
+  int H, T, nseq, seg, nseg, rev;
+  int64_t size;
+};
+__global__ __launch_bounds__(256) void decay_join_kernel(Join a) {
+  const int row = blockIdx.x / a.H, h = blockIdx.x % a.H;
+  int64_t slot = (int64_t)row * a.nseg;
+  int n = a.nseg;
+  if (a.nseq) {
+    const int from = seq_first(a.cu, row, a.T), len = seq_end(a.cu, row, a.T) - from;
+    n = max(1, (int)(((unsigned)len + a.seg - 1) / a.seg));
+    slot = packed_slot(from, row, a.seg);
+  }
+  const int64_t e0 = ((int64_t)blockIdx.y * 256 + threadIdx.x) * 4;
+  const int many = (int)min((int64_t)4, a.size - e0);
+  float s[4], add[4], next[4];
+  const auto at = [&](int i) { return a.states + ((slot + (a.rev ? n - 1 - i : i)) * a.H + h) * a.size + e0; };
+  const auto get = [&](float (&x)[4], const float* q) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = q && e < many ? q[e] : 0.f;
+  };
+  get(s, a.init ? a.init + ((int64_t)row * a.H + h) * a.size + e0 : nullptr);
+  get(add, n > 1 ? at(0) : nullptr);
+  for (int i = 0; i < n; ++i) {
+    get(next, i + 2 < n ? at(i + 1) : nullptr);
+    const float f = i + 1 < n ? a.whole[(slot + (a.rev ? n - 1 - i : i)) * a.H + h] : 0.f;
+    float* q = at(i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (e < many) q[e] = s[e];
+      s[e] = f * s[e] + add[e];
+      add[e] = next[e];
+    }
+  }
+}
+
+// dg from the walks' dots.  In a chunk with W = <dS, S> behind it:
+//   dg_t = sum_{s >= t} (x_s + u_s) + sum_{r < t} y_r + Z     Z = W - sum y     W before the chunk = Z + sum x
+// x: what a token's outputs took from the state before the chunk, y: what its key hands to the state behind it, u: its pairs as a query less those as
+// a key.  A strong decay makes x, y and Z small, and they are summed apart from the pairs, which cancel over a chunk.
+struct GateGrad {
+  const float *dots_q, *dots_k;  // [inter, pairs][slab][B H][T]
+  const float *fin, *d_fin;
+  const int32_t* cu;
+  float *dg, *part;  // part: sums over a row, [row][H]
+  int B, H, T, nseq, slabs;
+  int64_t step, size;
+};
+template <int C> __global__ __launch_bounds__(1024) void decay_gate_grad_kernel(GateGrad a) {
+  constexpr int NC = 1024 / C;
+  __shared__ float chunk[2][NC], red[16];
+  const int row = blockIdx.x / a.H, h = blockIdx.x % a.H, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, in = lane % C, mine = threadIdx.x / C;
+  int from = 0, len = a.T;
+  if (a.nseq) from = seq_first(a.cu, row, a.T), len = seq_end(a.cu, row, a.T) - from;
+  const int64_t base = (int64_t)((a.nseq ? 0 : row) * a.H + h) * a.T + from;
+  const auto block_sum = [&](float x) {
+    x = wave_sum(x);
+    __syncthreads();
+    if (lane == 0) red[wave] = x;
+    __syncthreads();
+    float s = 0.f;
+    for (int i = 0; i < 16; ++i) s += red[i];
+    return s;
+  };
+  float W = 0.f;
+  if (a.d_fin) {
+    const int64_t at = ((int64_t)row * a.H + h) * a.size;
+    for (int64_t i = threadIdx.x; i < a.size; i += 1024) W += a.fin[at + i] * a.d_fin[at + i];
+    W = block_sum(W);
+  }
+  const auto get = [&](int t, float& x, float& y, float& u) {
+    x = y = u = 0.f;
+    if (t < 0 || t >= len) return;
+    for (int s = 0; s < a.slabs; ++s) {
+      x += a.dots_q[s * a.step + base + t];
+      y += a.dots_k[s * a.step + base + t];
+      u += a.dots_q[(a.slabs + s) * a.step + base + t] - a.dots_k[(a.slabs + s) * a.step + base + t];
+    }
+  };
+  float sum = 0.f, x, y, u, nx, ny, nu;
+  int t = (len - 1) / 1024 * 1024 + threadIdx.x;
+  get(t, x, y, u);
+  for (int turn = 0; t > -1024 + (int)threadIdx.x; t -= 1024, turn ^= 1) {
+    get(t - 1024, nx, ny, nu);
+    float sx = x, su = u, py = y;
+#pragma unroll
+    for (int o = 1; o < C; o <<= 1) {
+      const float bx = __shfl_down(sx, o, LNX_WAVE), bu = __shfl_down(su, o, LNX_WAVE), by = __shfl_up(py, o, LNX_WAVE);
+      if (in + o < C) sx += bx, su += bu;
+      if (in >= o) py += by;
+    }
+    const float X = __shfl(sx, lane - in, LNX_WAVE), Y = __shfl(py, lane - in + C - 1, LNX_WAVE);
+    if (in == 0) chunk[turn][mine] = X - Y;
+    __syncthreads();
+    float behind = W;
+    for (int i = NC - 1; i >= 0; --i) {
+      if (i == mine) behind = W;
+      W += chunk[turn][i];
+    }
+    const float d = sx + su + (py - y) + (behind - Y);
+    if (t < len) {
+      if (a.dg) a.dg[base + t] = d;
+      sum += d;
+    }
+    x = nx, y = ny, u = nu;
+  }
+  if (a.part) {
+    sum = block_sum(sum);
+    if (threadIdx.x == 0) a.part[(int64_t)row * a.H + h] = sum;
+  }
+}
+// dg[h] = sum of the rows' sums
+__global__ __launch_bounds__(256) void decay_gate_sum_kernel(const float* part, int64_t rows, int H, float* dg) {
+  __shared__ float red[4];
+  float s = 0.f;
+  for (int64_t r = threadIdx.x; r < rows; r += 256) s += part[r * H + blockIdx.x];
+  s = wave_sum(s);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) dg[blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+// One token: a workgroup per (row, head, 128 columns).  Bound by the state, read and written once.
+struct Step {
+  const void *q, *k, *v;
+  const float *g, *s0;
+  void* o;
+  float* s1;
+  int64_t gb, gh;
+  int H, dk, dv, slabs;
+  float scale;
+};
+constexpr int STEP_COLS = 128, STEP_MAX_DK = 256;
+template <typename T, int VN> __global__ __launch_bounds__(256) void decay_step_kernel(Step a) {
+  constexpr int LPR = STEP_COLS / VN, GROUPS = 256 / LPR, U = 8;  // lanes of a row, rows at a time
+  __shared__ float qk[2][STEP_MAX_DK], red[GROUPS][STEP_COLS];
+  const int slab = blockIdx.x % a.slabs, bh = blockIdx.x / a.slabs, h = bh % a.H, li = threadIdx.x % LPR, grp = threadIdx.x / LPR, c = slab * STEP_COLS + li * VN;
+  const float f = __expf(a.g[bh / a.H * a.gb + h * a.gh]);
+  for (int i = threadIdx.x; i < a.dk; i += 256) {
+    qk[0][i] = to_f32(static_cast<const T*>(a.q)[(int64_t)bh * a.dk + i]) * a.scale;
+    qk[1][i] = to_f32(static_cast<const T*>(a.k)[(int64_t)bh * a.dk + i]);
+  }
+  float v[VN], o[VN];
+#pragma unroll
+  for (int e = 0; e < VN; ++e) {
+    v[e] = c + e < a.dv ? to_f32(static_cast<const T*>(a.v)[(int64_t)bh * a.dv + c + e]) : 0.f;
+    o[e] = 0.f;
+  }
+  __syncthreads();
+  const int64_t base = (int64_t)bh * a.dk * a.dv + c;
+  for (int i0 = grp; i0 < a.dk; i0 += GROUPS * U) {
+    float s[U][VN];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * GROUPS;
+      const float* p = a.s0 + base + (int64_t)i * a.dv;
+      if constexpr (VN == 4) {
+        floatx4 x = {0.f, 0.f, 0.f, 0.f};
+        if (i < a.dk && c < a.dv) x = load4(p);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[u][e] = x[e];
+      } else {
+        s[u][0] = i < a.dk && c < a.dv ? p[0] : 0.f;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * GROUPS;
+      if (i >= a.dk || c >= a.dv) continue;
+      const float qi = qk[0][i], ki = qk[1][i];
+#pragma unroll
+      for (int e = 0; e < VN; ++e) {
+        s[u][e] = f * s[u][e] + ki * v[e];
+        o[e] += qi * s[u][e];
+      }
+      float* p = a.s1 + base + (int64_t)i * a.dv;
+      if constexpr (VN == 4) store4(p, floatx4{s[u][0], s[u][1], s[u][2], s[u][3]});
+      else p[0] = s[u][0];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < VN; ++e) red[grp][li * VN + e] = o[e];
+  __syncthreads();
+  const int col = slab * STEP_COLS + threadIdx.x;
+  if (threadIdx.x < STEP_COLS && col < a.dv) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) s += red[i][threadIdx.x];
+    static_cast<T*>(a.o)[(int64_t)bh * a.dv + col] = from_f32<T>(s);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------------------------------------------
+
+int up(int x, int to) { return (x + to - 1) / to * to; }
+int64_t ceil_div(int64_t x, int64_t y) { return (x + y - 1) / y; }
+constexpr int MAX_D = 256, SHORTEST = 512;
+
+// Tokens of a segment, a multiple of 64, or 0: rows are walked whole.  Segments read keys and values (queries and gradients) once more, so they
+// are for few rows: 512 workgroups at least, of 512 tokens and more.  The rows of a packed batch are taken for one: their lengths are not
+// known here, and sequences of one segment are walked once whatever its size.
+int segment(const lnx_decay_args* a) {
+  const int64_t walks = (a->nseq ? 1 : (int64_t)a->B) * a->H * ceil_div(a->dv, SLAB);
+  if (walks >= 192) return 0;
+  int64_t s = up((int)ceil_div(a->T, ceil_div(512, walks)), 64);
+  if (s < SHORTEST) s = SHORTEST;
+  return s >= a->T ? 0 : (int)s;
+}
+struct Layout {
+  int seg, nseg;
+  int64_t slots, states, factors, dots, part, rows;  // bytes: states of all segments, their factors, the walks' dots, rows' sums
+};
+Layout layout(const lnx_decay_args* a) {
+  Layout l{};
+  const int s = segment(a);
+  l.rows = a->nseq ? a->nseq : a->B;
+  l.seg = s ? s : 0x7fffffc0;
+  l.nseg = s ? (int)ceil_div(a->T, s) : 1;
+  l.slots = a->nseq ? a->T / l.seg + a->nseq : (int64_t)a->B * l.nseg;
+  if (s) l.states = l.slots * a->H * a->dk * a->dv * 4, l.factors = ceil_div(l.slots * a->H * 4, 16) * 16;
+  l.dots = ceil_div(4 * ceil_div(a->dk, SLAB) * a->B * a->H * (int64_t)a->T * 4, 16) * 16;
+  l.part = l.rows * a->H * 4;
+  return l;
+}
+
+bool aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+int check(const char* what, const lnx_decay_args* a, bool bwd) {
+  if (!a) return lnx_set_error(LNX_ERR_NULL, "%s: args is NULL", what);
+  if (a->B < 0 || a->H <= 0 || a->T < 0 || a->T > 0x7fffff00 || a->dk <= 0 || a->dk > MAX_D || a->dv <= 0 || a->dv > MAX_D || a->nseq < 0 || (a->nseq && a->B != 1))
+    return lnx_set_error(LNX_ERR_SHAPE, "%s: unsupported dimensions B=%d H=%d T=%d dk=%d dv=%d nseq=%d (heads of at most %d; packed batches have B = 1)", what, a->B, a->H, a->T,
+                         a->dk, a->dv, a->nseq, MAX_D);
+  if (a->dtype != LNX_F32 && a->dtype != LNX_BF16) return lnx_set_error(LNX_ERR_DTYPE, "%s: dtype %d", what, a->dtype);
+  if (!(a->scale == a->scale) || a->scale - a->scale != 0.f) return lnx_set_error(LNX_ERR_SHAPE, "%s: scale must be finite", what);
+  if (a->nseq && !a->cu_seqlens) return lnx_set_error(LNX_ERR_NULL, "%s: nseq without cu_seqlens", what);
+  if (a->B == 0) return LNX_OK;
+  const Layout l = layout(a);
+  if (l.slots * a->H * (2 * ceil_div(a->dk, SLAB) + ceil_div(a->dv, SLAB)) > MAX_GRID || l.rows * a->H > MAX_GRID) return lnx_set_error(LNX_ERR_SHAPE, "%s: too many rows", what);
+  if (!bwd && !a->final_state) return lnx_set_error(LNX_ERR_NULL, "%s: final_state is required", what);
+  if (bwd && a->d_final_state && !a->final_state) return lnx_set_error(LNX_ERR_NULL, "%s: d_final_state needs final_state", what);
+  if (bwd && !a->d_g) return lnx_set_error(LNX_ERR_NULL, "%s: d_g is required", what);
+  const lnx_tensor4* ts[] = {&a->q, &a->k, &a->v, &a->o, &a->d_o, &a->d_q, &a->d_k, &a->d_v};
+  const int64_t size = a->dtype == LNX_BF16 ? 2 : 4;
+  const auto fits = [&](int extent, int64_t stride) { return extent <= 1 || stride * size % 16 == 0; };
+  for (int i = 0; i < 8; ++i) {
+    if (bwd ? i == 3 : i > 3) continue;
+    const lnx_tensor4& t = *ts[i];
+    if (a->T && !t.p) return lnx_set_error(LNX_ERR_NULL, "%s: a tensor is missing", what);
+    if (!aligned(t.p, 16) || !fits(a->B, t.stride_b) || !fits(a->H, t.stride_h) || !fits(a->T, t.stride_t) || (a->T > 1 && (t.stride_t < 0 || t.stride_t * size > 1 << 24)))
+      return lnx_set_error(LNX_ERR_SHAPE, "%s: tensors must be 16-byte aligned, rows whole numbers of 16 bytes and at most 16 MiB apart", what);
+  }
+  if (a->T && !a->g) return lnx_set_error(LNX_ERR_NULL, "%s: g is required", what);
+  if (bwd && l.states && !a->kept) return lnx_set_error(LNX_ERR_NULL, "%s: needs what the forward call kept", what);
+  const uint64_t need = bwd ? lnx_decay_bwd_workspace_bytes(a) : lnx_decay_fwd_workspace_bytes(a);
+  if (need && (!a->workspace || a->workspace_bytes < need || !aligned(a->workspace, 16)))
+    return lnx_set_error(LNX_ERR_WORKSPACE, "%s: needs a 16-byte aligned workspace of %llu bytes", what, (unsigned long long)need);
+  return LNX_OK;
+}
+
+Side side(const lnx_decay_args* a, const lnx_tensor4& t) {
+  return {t.p, a->B > 1 ? t.stride_b : 0, a->H > 1 ? t.stride_h : 0, a->T > 1 ? t.stride_t : 0};
+}
+int width(const lnx_decay_args* a, int d) { return up(d, a->dtype == LNX_BF16 ? 8 : 4); }
+
+// dims: of y in the state and of z
+Role role(const lnx_decay_args* a, const lnx_tensor4& x, const lnx_tensor4& y, const lnx_tensor4& z, const lnx_tensor4& out, int sk, int sn, bool rev, bool turned) {
+  Role r{};
+  r.x = side(a, x), r.y = side(a, y), r.z = side(a, z), r.out = side(a, out);
+  r.sk = sk, r.sn = sn, r.kw = width(a, sk), r.vw = width(a, sn);
+  r.rev = rev, r.turned = turned, r.slabs = (int)ceil_div(sn, SLAB);
+  r.row_scale = rev ? 1.f : a->scale, r.col_scale = rev ? a->scale : 1.f;
+  return r;
+}
+Walk walk(const lnx_decay_args* a, const Layout& l) {
+  Walk k{};
+  k.g = a->g, k.gb = a->B > 1 ? a->g_stride_b : 0, k.gh = a->H > 1 ? a->g_stride_h : 0, k.gt = a->T > 1 ? a->g_stride_t : 0;
+  k.cu = a->cu_seqlens;
+  k.B = a->B, k.H = a->H, k.T = a->T, k.nseq = a->nseq, k.dv = a->dv, k.seg = l.seg, k.nseg = l.nseg, k.by_slot = l.states != 0;
+  k.units = (int)(l.slots * a->H), k.scale = a->scale;
+  k.dots_step = (int64_t)a->B * a->H * a->T;
+  return k;
+}
+
+template <typename T, int KW, int BUFS, bool OUT> int start(const Walk& k, const char* name, hipStream_t st) {
+  const auto kernel = decay_walk_kernel<T, KW, BUFS, OUT>;
+  constexpr int bytes = Room<T, KW, BUFS, OUT>::BYTES;
+  if (int rc = lnx_lds_limit(reinterpret_cast<const void*>(kernel), bytes)) return rc;
+  lnx_profile_mark(name, st);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)((int64_t)k.units * k.per)), dim3(256), bytes, st, k);
+  return LNX_OK;
+}
+// kw: the widest of the launch's keys
+template <typename T, bool OUT> int start(Walk& k, int roles, const char* name, hipStream_t st) {
+  k.per = 0;
+  int kw = 0;
+  for (int i = 0; i < roles; ++i) k.per += k.role[i].slabs, kw = kw < k.role[i].kw ? k.role[i].kw : kw;
+  // two buffers where a CU has one workgroup
+  if (OUT && roles == 1 && !k.role[0].dots && (int64_t)k.units * k.per <= 256) {
+    if (kw <= 64) return start<T, 64, 2, OUT>(k, name, st);
+    if (kw <= 128) return start<T, 128, 2, OUT>(k, name, st);
+  }
+  if (kw <= 64) return start<T, 64, 1, OUT>(k, name, st);
+  if (kw <= 128) return start<T, 128, 1, OUT>(k, name, st);
+  return start<T, 256, 1, OUT>(k, name, st);
+}
+
+void join(const lnx_decay_args* a, const Layout& l, float* states, const float* whole, const float* init, bool rev, hipStream_t st) {
+  Join j{states, whole, init, a->cu_seqlens, a->H, a->T, a->nseq, l.seg, l.nseg, rev, (int64_t)a->dk * a->dv};
+  lnx_profile_mark("decay_join", st);
+  decay_join_kernel<<<dim3((unsigned)(l.rows * a->H), (unsigned)ceil_div(j.size, 1024)), 256, 0, st>>>(j);
+}
+
+template <typename T> int forward(const lnx_decay_args* a, hipStream_t st) {
+  const Layout l = layout(a);
+  Walk k = walk(a, l);
+  Role r = role(a, a->q, a->k, a->v, a->o, a->dk, a->dv, false, false);
+  r.init = a->initial_state;
+  if (l.states) {
+    char* ws = static_cast<char*>(a->workspace);
+    float* states = a->kept ? a->kept : reinterpret_cast<float*>(ws + l.factors);
+    k.whole = reinterpret_cast<float*>(ws);
+    k.role[0] = r;
+    k.role[0].fin = states;
+    if (int rc = start<T, false>(k, 1, "decay_local", st)) return rc;
+    join(a, l, states, k.whole, a->initial_state, false, st);
+    r.init = states;
+  }
+  r.fin = a->final_state;
+  k.role[0] = r;
+  return start<T, true>(k, 1, "decay_fwd", st);
+}
+
+template <typename T> int backward(const lnx_decay_args* a, hipStream_t st) {
+  const Layout l = layout(a);
+  Walk k = walk(a, l);
+  char* ws = static_cast<char*>(a->workspace);
+  Role q = role(a, a->d_o, a->v, a->k, a->d_q, a->dv, a->dk, false, true), kk = role(a, a->v, a->d_o, a->q, a->d_k, a->dv, a->dk, true, true),
+       v = role(a, a->k, a->q, a->d_o, a->d_v, a->dk, a->dv, true, false);
+  q.w = side(a, a->q), kk.w = side(a, a->k);
+  q.dots = reinterpret_cast<float*>(ws), kk.dots = q.dots + 2 * q.slabs * k.dots_step;
+  q.init = l.states ? a->kept : a->initial_state;
+  kk.init = v.init = a->d_final_state;
+  if (l.states) {
+    float* states = reinterpret_cast<float*>(ws + ceil_div(l.dots + l.part, 16) * 16 + l.factors);
+    k.whole = reinterpret_cast<float*>(ws + ceil_div(l.dots + l.part, 16) * 16);
+    k.role[0] = v;
+    k.role[0].fin = states;
+    if (int rc = start<T, false>(k, 1, "decay_local", st)) return rc;
+    join(a, l, states, k.whole, a->d_final_state, true, st);
+    kk.init = v.init = states;
+  }
+  v.fin = a->d_initial_state;
+  const int wide = a->dk > a->dv ? a->dk : a->dv, narrow = a->dk + a->dv - wide;
+  const auto step = [](int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; };
+  k.role[0] = q, k.role[1] = kk, k.role[2] = v;
+  if (step(wide) == step(narrow)) {
+    if (int rc = start<T, true>(k, 3, "decay_bwd", st)) return rc;
+  } else {
+    if (int rc = start<T, true>(k, 2, "decay_bwd_qk", st)) return rc;
+    k.role[0] = v;
+    if (int rc = start<T, true>(k, 1, "decay_bwd_v", st)) return rc;
+  }
+  GateGrad d{};
+  d.dots_q = q.dots, d.dots_k = kk.dots, d.fin = a->final_state, d.d_fin = a->d_final_state, d.cu = a->cu_seqlens;
+  if (a->g_per_head) d.part = reinterpret_cast<float*>(ws + l.dots);
+  else d.dg = a->d_g;
+  d.B = a->B, d.H = a->H, d.T = a->T, d.nseq = a->nseq, d.slabs = q.slabs, d.step = k.dots_step, d.size = (int64_t)a->dk * a->dv;
+  lnx_profile_mark("decay_gate_grad", st);
+  decay_gate_grad_kernel<Form<T>::C><<<dim3((unsigned)(l.rows * a->H)), 1024, 0, st>>>(d);
+  if (a->g_per_head) {
+    lnx_profile_mark("decay_gate_sum", st);
+    decay_gate_sum_kernel<<<dim3((unsigned)a->H), 256, 0, st>>>(d.part, l.rows, a->H, a->d_g);
+  }
+  return LNX_OK;
+}
+
+int finish(const char* what, int rc, hipStream_t st) {
+  if (rc) return rc;
+  lnx_profile_mark(nullptr, st);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? LNX_OK : lnx_set_error(LNX_ERR_LAUNCH, "%s: %s", what, hipGetErrorString(e));
+}
+
+bool sizes(const lnx_decay_args* a) {
+  return a && a->B > 0 && a->H > 0 && a->T >= 0 && a->T <= 0x7fffff00 && a->dk > 0 && a->dk <= MAX_D && a->dv > 0 && a->dv <= MAX_D && a->nseq >= 0;
+}
+
+}  // namespace
+
+extern "C" uint64_t lnx_decay_kept_bytes(const lnx_decay_args* a) { return sizes(a) ? layout(a).states : 0; }
+extern "C" uint64_t lnx_decay_fwd_workspace_bytes(const lnx_decay_args* a) {
+  if (!sizes(a)) return 0;
+  const Layout l = layout(a);
+  return l.states ? l.factors + (a->kept ? 0 : l.states) : 0;
+}
+extern "C" uint64_t lnx_decay_bwd_workspace_bytes(const lnx_decay_args* a) {
+  if (!sizes(a)) return 0;
+  const Layout l = layout(a);
+  return ceil_div(l.dots + l.part, 16) * 16 + l.factors + l.states;
+}
+extern "C" int lnx_decay_fwd(const lnx_decay_args* a, void* hip_stream) {
+  if (int rc = check("decay_fwd", a, false)) return rc;
+  if (a->B == 0) return LNX_OK;
+  hipStream_t st = static_cast<hipStream_t>(hip_stream);
+  return finish("decay_fwd", a->dtype == LNX_BF16 ? forward<bf16_t>(a, st) : forward<float>(a, st), st);
+}
+extern "C" int lnx_decay_bwd(const lnx_decay_args* a, void* hip_stream) {
+  if (int rc = check("decay_bwd", a, true)) return rc;
+  if (a->B == 0) return LNX_OK;
+  hipStream_t st = static_cast<hipStream_t>(hip_stream);
+  return finish("decay_bwd", a->dtype == LNX_BF16 ? backward<bf16_t>(a, st) : backward<float>(a, st), st);
+}
+extern "C" int lnx_decay_step(const lnx_decay_step_args* a, void* hip_stream) {
+  const char* what = "decay_step";
+  if (!a) return lnx_set_error(LNX_ERR_NULL, "%s: args is NULL", what);
+  if (a->B < 0 || a->H <= 0 || a->dk <= 0 || a->dk > STEP_MAX_DK || a->dv <= 0)
+    return lnx_set_error(LNX_ERR_SHAPE, "%s: unsupported dimensions B=%d H=%d dk=%d dv=%d (dk at most %d)", what, a->B, a->H, a->dk, a->dv, STEP_MAX_DK);
+  if (a->dtype != LNX_F32 && a->dtype != LNX_BF16) return lnx_set_error(LNX_ERR_DTYPE, "%s: dtype %d", what, a->dtype);
+  if (a->B == 0) return LNX_OK;
+  if (!a->q || !a->k || !a->v || !a->g || !a->state || !a->o || !a->new_state) return lnx_set_error(LNX_ERR_NULL, "%s: a tensor is missing", what);
+  Step k{a->q, a->k, a->v, a->g, a->state, a->o, a->new_state, a->B > 1 ? a->g_stride_b : 0, a->H > 1 ? a->g_stride_h : 0, a->H, a->dk, a->dv, (int)ceil_div(a->dv, STEP_COLS), a->scale};
+  const int64_t grid = (int64_t)a->B * a->H * k.slabs;
+  if (grid > MAX_GRID) return lnx_set_error(LNX_ERR_SHAPE, "%s: too many rows", what);
+  const bool vec = a->dv % 4 == 0 && aligned(a->state, 16) && aligned(a->new_state, 16);
+  hipStream_t st = static_cast<hipStream_t>(hip_stream);
+  lnx_profile_mark(what, st);
+  if (a->dtype == LNX_BF16) {
+    if (vec) decay_step_kernel<bf16_t, 4><<<dim3((unsigned)grid), 256, 0, st>>>(k);
+    else decay_step_kernel<bf16_t, 1><<<dim3((unsigned)grid), 256, 0, st>>>(k);
+  } else {
+    if (vec) decay_step_kernel<float, 4><<<dim3((unsigned)grid), 256, 0, st>>>(k);
+    else decay_step_kernel<float, 1><<<dim3((unsigned)grid), 256, 0, st>>>(k);
+  }
+  return finish(what, LNX_OK, st);
+}

@@ -1718,6 +1718,174 @@ PyObject* py_causal_attention_step_paged(PyObject*, PyObject* const* args, Py_ss
   LNX_END
 }
 
+// ---------------------------------------------------------------------------------------------------------------
+// linear attention with a decay for each head
+// ---------------------------------------------------------------------------------------------------------------
+
+struct DecayShape {
+  int64_t B, H, T, dk, dv, nseq, rows;
+  bool per_head;
+  double scale;
+};
+
+DecayShape decay_shape(const char* op, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& s0, const Tensor& cu, int64_t dims) {
+  const char* names = "qkv";
+  const Tensor* ts[3] = {&q, &k, &v};
+  for (int i = 0; i < 3; ++i) TORCH_CHECK(ts[i]->is_cuda(), op, ": ", names[i], " is on ", ts[i]->device().str(), "; the op runs on the GPU only");
+  check_inputs(q, k, v);
+  TORCH_CHECK(q.dim() == dims && q.size(1) > 0 && q.size(-1) > 0 && v.size(-1) > 0, op, ": expected q, k ", dims == 4 ? "[B, H, T, dk] and v [B, H, T, dv]" : "[B, H, dk] and v [B, H, dv]",
+              ", got q ", shape_text(q), " v ", shape_text(v));
+  DecayShape s{q.size(0), q.size(1), dims == 4 ? q.size(2) : 1, q.size(-1), v.size(-1), 0, q.size(0), false, 0.0};
+  TORCH_CHECK(s.dk <= 256 && (dims == 3 || s.dv <= 256), op, ": heads of ", s.dk, " and ", s.dv, " are not supported (at most 256)");
+  TORCH_CHECK(s.B <= INT32_MAX && s.H <= INT32_MAX && s.T <= INT32_MAX - 256 && s.dv <= INT32_MAX, op, ": q is too large, got ", shape_text(q));
+  TORCH_CHECK(g.is_floating_point(), op, ": g must be a floating-point tensor, got ", g.scalar_type());
+  s.per_head = g.dim() == 1;
+  TORCH_CHECK(s.per_head ? g.size(0) == s.H : g.sizes() == q.sizes().slice(0, dims - 1), op, ": g must be ", dims == 4 ? "[B, H, T]" : "[B, H]", " or [H], got ", shape_text(g), " for q ",
+              shape_text(q));
+  check_devices(op, q, {{"k", &k}, {"v", &v}, {"g", &g}, {"state", &s0}, {"cu_seqlens", &cu}});
+  if (cu.defined()) {
+    TORCH_CHECK(s.B == 1, "cu_seqlens needs a packed batch with B == 1");
+    s.rows = s.nseq = cu.numel() - 1;
+  }
+  TORCH_CHECK(!s0.defined() || (s0.sizes() == at::IntArrayRef({s.rows, s.H, s.dk, s.dv}) && s0.is_floating_point()), op, ": the state must be a floating-point (", s.rows, ", ", s.H,
+              ", ", s.dk, ", ", s.dv, ") tensor, got ", s0.defined() ? shape_text(s0) : "");
+  return s;
+}
+
+// Rows as the kernels read them, widened by zero columns to whole vectors, in t's memory order
+Tensor decay_rows(const Tensor& t) {
+  const int64_t d = t.size(-1), more = (8 - d % 8) % 8;
+  if (!more) return as_rows(t);
+  return tokens_outside(t) ? at::constant_pad_nd(t.transpose(1, 2), {0, more}).transpose(1, 2) : at::constant_pad_nd(t, {0, more});
+}
+Tensor decay_cut(const Tensor& t, int64_t d) { return t.size(-1) == d ? t : t.narrow(-1, 0, d); }
+
+lnx_decay_args decay_args(const DecayShape& s, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& cu, const Tensor& s0) {
+  lnx_decay_args a{};
+  a.B = (int32_t)s.B, a.H = (int32_t)s.H, a.T = (int32_t)s.T, a.dk = (int32_t)s.dk, a.dv = (int32_t)s.dv, a.nseq = (int32_t)s.nseq;
+  a.dtype = code_of(q.scalar_type()), a.g_per_head = s.per_head, a.scale = (float)s.scale;
+  a.q = tensor4(q), a.k = tensor4(k), a.v = tensor4(v), a.g = fptr(g), a.cu_seqlens = static_cast<const int32_t*>(ptr(cu)), a.initial_state = fptr(s0);
+  if (s.per_head) a.g_stride_h = g.stride(0);
+  else a.g_stride_b = g.stride(0), a.g_stride_h = g.stride(1), a.g_stride_t = g.stride(2);
+  return a;
+}
+
+// q, k, v as rows, g and the state fp32; o in q's memory order with columns up to the next multiple of 8
+std::pair<Tensor, Tensor> decay_forward(const DecayShape& s, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& s0, const Tensor& cu, Tensor* kept) {
+  lnx_decay_args a = decay_args(s, q, k, v, g, cu, s0);
+  const auto fo = q.options().dtype(at::kFloat);
+  const Tensor o = empty_layout(s.B, s.H, s.T, v.size(3), q.options(), tokens_outside(q)), sT = at::empty({s.rows, s.H, s.dk, s.dv}, fo);
+  if (kept) {
+    *kept = at::empty({(int64_t)(lnx_decay_kept_bytes(&a) / sizeof(float))}, fo);
+    if (kept->numel()) a.kept = fptr(*kept);
+  }
+  a.o = tensor4(o), a.final_state = fptr(sT);
+  a.workspace_bytes = lnx_decay_fwd_workspace_bytes(&a);
+  Tensor ws;
+  if (a.workspace_bytes) ws = work_area(q, a.workspace_bytes);
+  a.workspace = ptr(ws);
+  const c10::DeviceGuard guard(q.device());
+  check_status(lnx_decay_fwd(&a, stream_of(q)), "lnx_decay_fwd");
+  return {o, sT};
+}
+
+struct DecayFn : Function<DecayFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q0, const Tensor& k0, const Tensor& v0, const Tensor& g0, const OptT& s0, const OptT& cu, const DecayShape& s) {
+    const Tensor q = decay_rows(q0), k = decay_rows(k0), v = decay_rows(v0), g = g0.to(at::kFloat), si = f32(undef(s0));
+    Tensor kept;
+    auto [o, sT] = decay_forward(s, q, k, v, g, si, undef(cu), &kept);
+    ctx->save_for_backward({q, k, v, g, si, undef(cu), kept, sT});
+    ctx->saved_data["i"] = std::vector<int64_t>{s.B, s.H, s.T, s.dk, s.dv, s.nseq, s.rows, s.per_head, (int64_t)g0.scalar_type(), s0.has_value() && s0->requires_grad(),
+                                                (int64_t)(s0.has_value() ? s0->scalar_type() : at::kFloat)};
+    ctx->saved_data["d"] = s.scale;
+    ctx->set_materialize_grads(false);
+    return {decay_cut(o, s.dv), sT};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_tangents("the gradient of decay_linear_attention", grads);
+    const variable_list sv = ctx->get_saved_variables();
+    refuse_live_graph_behind("the gradient of decay_linear_attention", sv[0]);
+    const std::vector<int64_t> m = ctx->saved_data["i"].toIntVector();
+    const Tensor &q = sv[0], &k = sv[1], &v = sv[2], &g = sv[3], &kept = sv[6];
+    const DecayShape s{m[0], m[1], m[2], m[3], m[4], m[5], m[6], m[7] != 0, ctx->saved_data["d"].toDouble()};
+    lnx_decay_args a = decay_args(s, q, k, v, g, sv[5], sv[4]);
+    const Tensor d_o = grads[0].defined() ? decay_rows(grads[0].to(q.scalar_type())) : at::zeros_like(v), ds = f32(grads[1]);
+    auto like = [](const Tensor& t) { return empty_layout(t.size(0), t.size(1), t.size(2), t.size(3), t.options(), tokens_outside(t)); };
+    const auto fo = q.options().dtype(at::kFloat);
+    const Tensor dq = like(q), dk = like(k), dv = like(v), dg = s.per_head ? at::empty({s.H}, fo) : at::empty({s.B, s.H, s.T}, fo);
+    Tensor d0;
+    if (m[9]) d0 = at::empty({s.rows, s.H, s.dk, s.dv}, fo);
+    a.d_o = tensor4(d_o), a.d_q = tensor4(dq), a.d_k = tensor4(dk), a.d_v = tensor4(dv), a.d_g = fptr(dg), a.d_final_state = fptr(ds), a.d_initial_state = fptr(d0);
+    a.final_state = fptr(sv[7]);
+    if (kept.numel()) a.kept = fptr(kept);
+    a.workspace_bytes = lnx_decay_bwd_workspace_bytes(&a);
+    const Tensor ws = work_area(q, a.workspace_bytes);
+    a.workspace = ptr(ws);
+    const c10::DeviceGuard guard(q.device());
+    check_status(lnx_decay_bwd(&a, stream_of(q)), "lnx_decay_bwd");
+    return {decay_cut(dq, s.dk), decay_cut(dk, s.dk), decay_cut(dv, s.dv), dg.to((at::ScalarType)m[8]), d0.defined() ? d0.to((at::ScalarType)m[10]) : d0, Tensor(), Tensor()};
+  }
+};
+
+std::pair<Tensor, Tensor> decay_scan(const DecayShape& s, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& s0, const Tensor& cu) {
+  if (wants_grad({&q, &k, &v, &g, &s0})) {
+    refuse_live_graph("decay_linear_attention", {&q, &k, &v, &g, &s0});
+    const variable_list r = DecayFn::apply(q, k, v, g, opt(s0), opt(cu), s);
+    return {r[0], r[1]};
+  }
+  const auto r = decay_forward(s, decay_rows(q), decay_rows(k), decay_rows(v), g.to(at::kFloat), f32(s0), cu, nullptr);
+  return {decay_cut(r.first, s.dv), r.second};
+}
+
+// decay_attention(q, k, v, g, scale or None, initial_state, cu): (o, final state)
+PyObject* py_decay_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  LNX_BEGIN
+  Args in(args, nargs, 7, "decay_attention");
+  const char* op = "decay_linear_attention";
+  const Tensor q = in.tensor(0, "q"), k = in.tensor(1, "k"), v = in.tensor(2, "v"), g = in.tensor(3, "g"), s0 = in.maybe(5, "initial_state"), cu = in.maybe(6, "cu_seqlens");
+  DecayShape s = decay_shape(op, q, k, v, g, s0, cu, 4);
+  refuse_tangents(op, {&q, &k, &v, &g, &s0});
+  s.scale = in.is_none(4) ? 1.0 / std::sqrt((double)s.dk) : in.number(4);
+  TORCH_CHECK_VALUE(std::isfinite((float)s.scale), op, ": scale must be finite, got ", s.scale);
+  const auto r = without_lock([&] { return decay_scan(s, q, k, v, g, s0, cu); });
+  return pack(r.first, r.second);
+  LNX_END
+}
+
+// decay_attention_step(q, k, v, g, state, scale or None, inplace): (o, state)
+PyObject* py_decay_attention_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  LNX_BEGIN
+  Args in(args, nargs, 7, "decay_attention_step");
+  const char* op = "decay_linear_attention_step";
+  const Tensor q = in.tensor(0, "q"), k = in.tensor(1, "k"), v = in.tensor(2, "v"), g = in.tensor(3, "g"), state = in.tensor(4, "state");
+  const bool inplace = in.flag(6);
+  DecayShape s = decay_shape(op, q, k, v, g, state, Tensor(), 3);
+  refuse_tangents(op, {&q, &k, &v, &g, &state});
+  s.scale = in.is_none(5) ? 1.0 / std::sqrt((double)s.dk) : in.number(5);
+  TORCH_CHECK_VALUE(std::isfinite((float)s.scale), op, ": scale must be finite, got ", s.scale);
+  const bool grad = wants_grad({&q, &k, &v, &g, &state});
+  TORCH_CHECK(!grad || !inplace, "cannot differentiate through a step that updates its state in place");
+  TORCH_CHECK(!grad || s.dv <= 256, op, ": the gradient takes heads of at most 256, got ", s.dv);
+  TORCH_CHECK(!inplace || (state.scalar_type() == at::kFloat && state.is_contiguous()), "inplace=True needs a contiguous float32 state");
+  const auto r = without_lock([&]() -> std::pair<Tensor, Tensor> {
+    if (grad) {
+      const auto r = decay_scan(s, q.unsqueeze(2), k.unsqueeze(2), v.unsqueeze(2), s.per_head ? g : g.unsqueeze(2), state, Tensor());
+      return {r.first.squeeze(2), r.second};
+    }
+    const Tensor qc = q.contiguous(), kc = k.contiguous(), vc = v.contiguous(), gf = g.to(at::kFloat), si = f32(state), so = inplace ? state : at::empty_like(si), o = at::empty_like(vc);
+    lnx_decay_step_args a{};
+    a.B = (int32_t)s.B, a.H = (int32_t)s.H, a.dk = (int32_t)s.dk, a.dv = (int32_t)s.dv, a.dtype = code_of(q.scalar_type()), a.scale = (float)s.scale;
+    a.q = ptr(qc), a.k = ptr(kc), a.v = ptr(vc), a.g = fptr(gf), a.g_stride_b = s.per_head ? 0 : gf.stride(0), a.g_stride_h = s.per_head ? gf.stride(0) : gf.stride(1);
+    a.state = fptr(si), a.o = ptr(o), a.new_state = fptr(so);
+    const c10::DeviceGuard guard(q.device());
+    check_status(lnx_decay_step(&a, stream_of(q)), "lnx_decay_step");
+    if (inplace) written(state);
+    return {o, so};
+  });
+  return pack(r.first, r.second);
+  LNX_END
+}
+
 // set_kernel_error(class): the exception a failed C-ABI call raises
 PyObject* py_set_kernel_error(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (nargs != 1 || !PyExceptionClass_Check(args[0])) {
@@ -1731,7 +1899,7 @@ PyObject* py_set_kernel_error(PyObject*, PyObject* const* args, Py_ssize_t nargs
 
 #define LNX_FN(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {LNX_FN(step),     LNX_FN(recurrent), LNX_FN(l2norm), LNX_FN(l2norm_bwd), LNX_FN(chunk), LNX_FN(chunk_segmented),     LNX_FN(conv1d),           LNX_FN(rmsnorm_gated), LNX_FN(gdn_gate),
-                         LNX_FN(kda_gate), LNX_FN(dplr),      LNX_FN(dplr_step), LNX_FN(linrec), LNX_FN(linrec_step), LNX_FN(rmsnorm_residual), LNX_FN(layer_norm), LNX_FN(causal_attention), LNX_FN(causal_attention_step), LNX_FN(causal_attention_step_paged), LNX_FN(set_kernel_error), {nullptr, nullptr, 0, nullptr}};
+                         LNX_FN(kda_gate), LNX_FN(dplr),      LNX_FN(dplr_step), LNX_FN(linrec), LNX_FN(linrec_step), LNX_FN(rmsnorm_residual), LNX_FN(layer_norm), LNX_FN(causal_attention), LNX_FN(causal_attention_step), LNX_FN(causal_attention_step_paged), LNX_FN(decay_attention), LNX_FN(decay_attention_step), LNX_FN(set_kernel_error), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_host", "Host path of the linearnexus_amd ops.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
