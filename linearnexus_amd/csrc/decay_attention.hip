@@ -11,6 +11,8 @@
 // are off by their own rounding alone, and dg, a running difference of x . out and y . out over a whole sequence, keeps its digits.
 // Exponents are differences of sums over a chunk: the sums are held as a multiple of 1/64 and a rest, so that a difference is exact to a unit
 // however far the sums have run (a decay of e^-100 beside one of 1).
+#include <type_traits>
+
 #include "lnx_common.h"
 #include "mma_tiles.h"
 #include "packed_slots.h"
@@ -26,14 +28,14 @@ typedef __attribute__((address_space(3))) char lds_char;
 // index 16 a + 4 g + r of the K: element r of that group in result tile a.
 template <typename T> struct Form;
 template <> struct Form<bf16_t> {
-  static constexpr int C = 64, K = 32, TP = 2, PARTS = 2;
+  static constexpr int K = 32, TP = 2, PARTS = 2;
   typedef bf16x8 Frag;
   static __device__ __forceinline__ void mma(floatx4& c, const Frag& a, const Frag& b) { c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
   static __device__ __forceinline__ void put(Frag& f, int a, int r, float x) { f[4 * a + r] = (bf16_t)x; }
   static __device__ __forceinline__ float get(const Frag& f, int a, int r) { return (float)f[4 * a + r]; }
 };
 template <> struct Form<float> {
-  static constexpr int C = 32, K = 16, TP = 1, PARTS = 1;
+  static constexpr int K = 16, TP = 1, PARTS = 1;
   typedef floatx4 Frag;
   static __device__ __forceinline__ void mma(floatx4& c, const Frag& a, const Frag& b) {
 #pragma unroll
@@ -42,10 +44,12 @@ template <> struct Form<float> {
   static __device__ __forceinline__ void put(Frag& f, int, int r, float x) { f[r] = x; }
   static __device__ __forceinline__ float get(const Frag& f, int, int r) { return f[r]; }
 };
+// Tokens of a chunk: three of them lie in LDS at a time
+template <typename T, int KW> constexpr int chunk_of() { return (sizeof(T) == 2 ? 64 : 32) / (KW > 128 ? 2 : 1); }
 __device__ __forceinline__ bool is_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
-// Result tiles as an operand, and what its rounding left (of an infinite value nothing)
-__device__ __forceinline__ void split(const floatx4 (&v)[2], bf16x8& hi, bf16x8& lo) {
+// Result tiles as an operand, and what its rounding left; GUARD: of an infinite value nothing (otherwise NaN, for the caller to notice)
+template <bool GUARD> __device__ __forceinline__ void split(const floatx4 (&v)[2], bf16x8& hi, bf16x8& lo) {
   hi = Mma16::from_acc(v[0], v[1]);
   floatx4 d[2];
 #pragma unroll
@@ -53,11 +57,11 @@ __device__ __forceinline__ void split(const floatx4 (&v)[2], bf16x8& hi, bf16x8&
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const float h = (float)hi[4 * a + r];
-      d[a][r] = is_finite(h) ? v[a][r] - h : 0.f;
+      d[a][r] = !GUARD || is_finite(h) ? v[a][r] - h : 0.f;
     }
   lo = Mma16::from_acc(d[0], d[1]);
 }
-__device__ __forceinline__ void split(const floatx4 (&v)[1], floatx4& hi, floatx4&) { hi = v[0]; }
+template <bool GUARD> __device__ __forceinline__ void split(const floatx4 (&v)[1], floatx4& hi, floatx4&) { hi = v[0]; }
 
 // A [C][W] tile in LDS as loads that go straight there leave it: 16-byte granules of a row permuted by an exclusive or with x(row), chosen so that
 // row operands (16 consecutive rows, one granule) and column operands (the transposing reads of two lane groups: 8 consecutive rows, 2 granules;
@@ -196,10 +200,10 @@ __device__ __forceinline__ Spot spot(const Walk& a, int slot) {
   return s;
 }
 
-// Brings [C][W] tiles to LDS by the workgroup's four waves; which bytes a lane fetches is formed once.
-template <typename T, int W> struct Mover {
+// Brings [C][W] tiles to LDS by four waves; which bytes a lane fetches is formed once.
+template <typename T, int W, int C> struct Mover {
   typedef Cells<T, W> CL;
-  static constexpr int C = Form<T>::C, N = C * CL::ROWB / 1024 / 4;
+  static constexpr int N = C * CL::ROWB / 1024 / 4;
   unsigned off[N];
   __device__ __forceinline__ Mover(int64_t st, int wave, int lane) {
 #pragma unroll
@@ -230,25 +234,32 @@ template <typename T> __device__ __forceinline__ const T* head_of(const Side& s,
   return static_cast<const T*>(s.p) + p.b * s.sb + h * s.sh + p.tok * s.st;
 }
 
-template <typename T, int KW, int BUFS, bool OUT> struct Room {
-  static constexpr int C = Form<T>::C, NI = C / 16, NJ = C / Form<T>::K;
-  static constexpr int XB = C * KW * sizeof(T), ZB = C * SLAB * sizeof(T), BUF = (OUT ? 2 : 1) * XB + ZB;
-  static constexpr int PAIRS = BUFS * BUF, GATES = PAIRS + (OUT ? NI * NJ * Form<T>::PARTS * 1024 : 0), RAW = GATES + 4 * 1024, DOTS = RAW + BUFS * 256;
-  static constexpr int BYTES = DOTS + (OUT ? 4 * 2 * C * 4 : 0);
+// LDS of a walk.  OUT: false for the local walks of segments, which leave what a segment adds to the state and nothing else.
+template <typename T, int KW, bool OUT> struct Room {
+  static constexpr int C = chunk_of<T, KW>(), NI = C / 16, NJ = C / Form<T>::K;
+  static constexpr int SLOTS = NI == 4 && NJ == 2 ? 6 : NI * NJ;  // of 16 x K blocks of pairs; of the wide ones two are always empty
+  static constexpr int XB = C * KW * sizeof(T), ZB = C * SLAB * sizeof(T), BUF = (OUT ? 2 : 1) * XB + ZB, PAIRB = OUT ? SLOTS * Form<T>::PARTS * 1024 : 0;
+  static constexpr int PAIRS = 3 * BUF, FACTORS = PAIRS + 2 * PAIRB, SUMS = FACTORS + 2 * 1024, RAW = SUMS + 4 * 512, DOTS = RAW + 3 * 256;
+  static constexpr int BYTES = DOTS + (OUT ? 2 * 4 * 2 * C * 4 : 0);
+  static __device__ __forceinline__ int slot(int i, int j, bool rev) { return SLOTS != 6 ? i * NJ + j : rev ? (i < 2 ? 2 * i + j : i + 2) : (i < 2 ? i : 2 * i - 2 + j); }
+  // whether row tile i has pairs with block j
+  static __device__ __forceinline__ bool needed(int i, int j, bool rev) { return rev ? Form<T>::K * (j + 1) > 16 * i : Form<T>::K * j <= 16 * i + 15; }
 };
 
-// OUT: false for the local walks of segments, which leave what a segment adds to the state and nothing else.
-template <typename T, int KW, int BUFS, bool OUT> __global__ __launch_bounds__(256) void decay_walk_kernel(Walk a) {
+// A walk's eight waves.  Four hold the state, 16 columns each, and turn chunk c into results; the other four bring chunk c + 2 to LDS and form the
+// decays and the pairs of chunk c + 1, one tile of 16 rows each.  One barrier a chunk.
+template <typename T, int KW, bool OUT> __global__ __launch_bounds__(512) void decay_walk_kernel(Walk a) {
   typedef Form<T> F;
   typedef typename F::Frag Frag;
   typedef Cells<T, KW> XC;
   typedef Cells<T, SLAB> ZC;
-  typedef Room<T, KW, BUFS, OUT> R;
-  constexpr int C = F::C, NI = R::NI, NJ = R::NJ, NS = KW / F::K, NT = KW / 16, WPI = 4 / NI;
+  typedef Room<T, KW, OUT> R;
+  constexpr int C = R::C, NI = R::NI, NJ = R::NJ, NS = KW / F::K, NT = KW / 16;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g4 = 4 * (lane >> 4);
+  const int lane = threadIdx.x & 63, wave8 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = wave8 & 3, l16 = lane & 15, g4 = 4 * (lane >> 4);
   // workgroups of one (slot, head) follow each other on one XCD, whose L2 then holds what they share
-  int w = blockIdx.x, unit, item;
+  const int w = blockIdx.x;
+  int unit, item;
   if (a.units % 8 == 0) {
     unit = (w >> 3) / a.per * 8 + (w & 7);
     item = (w >> 3) % a.per;
@@ -266,30 +277,112 @@ template <typename T, int KW, int BUFS, bool OUT> __global__ __launch_bounds__(2
   if (!OUT && (rev ? p.first : p.last)) return;  // nothing walks on from there
   const int col0 = item * SLAB, vw = min(SLAB, ro.vw - col0), n0 = col0 + 16 * wave;
   const int nchunk = (p.len + C - 1) / C;
-  const T* xp = OUT ? head_of<T>(ro.x, p, h) : nullptr;
-  const T* yp = head_of<T>(ro.y, p, h);
-  const T* zp = head_of<T>(ro.z, p, h) + col0;
-  const float* gp = a.g + p.b * a.gb + h * a.gh + p.tok * a.gt;
+  const auto chunk_at = [&](int it) { return rev ? nchunk - 1 - it : it; };
   const unsigned lds0 = lds_byte_addr(lds);
-  const auto xt = [&](int buf) { return lds0 + buf * R::BUF + R::XB + R::ZB; };
-  const auto yt = [&](int buf) { return lds0 + buf * R::BUF; };
-  const auto zt = [&](int buf) { return lds0 + buf * R::BUF + R::XB; };
-  float* gates = reinterpret_cast<float*>(lds + R::GATES) + 256 * wave;  // of this wave: sums' multiples, rests, row factors, column factors
-  const float* raw = reinterpret_cast<const float*>(lds + R::RAW);
+  const auto yt = [&](int it) { return lds0 + it % 3 * R::BUF; };
+  const auto zt = [&](int it) { return lds0 + it % 3 * R::BUF + R::XB; };
+  const auto xt = [&](int it) { return lds0 + it % 3 * R::BUF + R::XB + R::ZB; };
+  float* factors = reinterpret_cast<float*>(lds + R::FACTORS);  // [it & 1]: of rows [64], of columns [64], of the state
+  float* red = reinterpret_cast<float*>(lds + R::DOTS);         // [it & 1][wave][inter, pairs][C]
+  const bool dots = OUT && ro.dots;
   if (ro.kw < KW || vw < SLAB) {
-    for (int i = threadIdx.x * 16; i < R::PAIRS; i += 256 * 16) *reinterpret_cast<floatx4*>(lds + i) = floatx4{0.f, 0.f, 0.f, 0.f};
+    for (int i = threadIdx.x * 16; i < R::PAIRS; i += 512 * 16) *reinterpret_cast<floatx4*>(lds + i) = floatx4{0.f, 0.f, 0.f, 0.f};
     lds_barrier();
   }
-  const Mover<T, KW> mx(OUT ? ro.x.st : 0, wave, lane), my(ro.y.st, wave, lane);
-  const Mover<T, SLAB> mz(ro.z.st, wave, lane);
-  const auto fetch = [&](int chunk, int buf) {
-    const int t0 = chunk * C, valid = min(C, p.len - t0);
-    if constexpr (OUT) mx.fetch(xt(buf), xp, ro.x.st, t0, valid, ro.kw, wave, lane);
-    my.fetch(yt(buf), yp, ro.y.st, t0, valid, ro.kw, wave, lane);
-    mz.fetch(zt(buf), zp, ro.z.st, t0, valid, vw, wave, lane);
-    if (wave == 0) dma4(gp + (int64_t)(t0 + min(lane, valid - 1)) * a.gt, lds0 + R::RAW + 256 * buf);
-  };
-  // the state: tile i holds rows 16 i + 4 g + r of column n0 + l16
+  if (wave8 >= 4) {
+    // ---------------------------------------------------------------------------------------------------- tiles, decays, pairs
+    const T* xp = OUT ? head_of<T>(ro.x, p, h) : nullptr;
+    const T* yp = head_of<T>(ro.y, p, h);
+    const T* zp = head_of<T>(ro.z, p, h) + col0;
+    const float* gp = a.g + p.b * a.gb + h * a.gh + p.tok * a.gt;
+    const Mover<T, KW, C> mx(OUT ? ro.x.st : 0, wave, lane), my(ro.y.st, wave, lane);
+    const Mover<T, SLAB, C> mz(ro.z.st, wave, lane);
+    const auto fetch = [&](int it) {
+      const int t0 = chunk_at(it) * C, valid = min(C, p.len - t0);
+      if constexpr (OUT) mx.fetch(xt(it), xp, ro.x.st, t0, valid, ro.kw, wave, lane);
+      my.fetch(yt(it), yp, ro.y.st, t0, valid, ro.kw, wave, lane);
+      mz.fetch(zt(it), zp, ro.z.st, t0, valid, vw, wave, lane);
+      if (wave == 0) dma4(gp + (int64_t)(t0 + min(lane, valid - 1)) * a.gt, lds0 + R::RAW + 256 * (it % 3));
+    };
+    const auto leave_dots = [&](int it) {
+      const int t0 = chunk_at(it) * C, tid = threadIdx.x - 256, i = tid % C, kind = tid / C;
+      if (kind < 2 && t0 + i < p.len) {
+        const float* q = red + (it & 1) * 8 * C + kind * C + i;
+        ro.dots[(int64_t)(kind * ro.slabs + item) * a.dots_step + (int64_t)(p.b * a.H + h) * a.T + p.tok + t0 + i] = (q[0] + q[2 * C]) + (q[4 * C] + q[6 * C]);
+      }
+    };
+    constexpr int WPI = NI >= 4 ? 1 : 4 / NI;  // waves of a row tile: they share its blocks
+    const int mine = wave / WPI, i = 16 * mine + l16;
+    float* sums = reinterpret_cast<float*>(lds + R::SUMS) + 128 * wave;  // of this wave: multiples, rests
+    const float* raw = reinterpret_cast<const float*>(lds + R::RAW);
+    float whole_h = 0.f, whole_l = 0.f;
+    if (nchunk > 0) fetch(0);
+    dma_wait<0>();
+    lds_barrier();
+    for (int it = 0; it <= nchunk; ++it) {  // chunk `it` is prepared while it - 1 is walked
+      if (it + 1 < nchunk) fetch(it + 1);
+      if (dots && it >= 2) leave_dots(it - 2);
+      if (it < nchunk) {
+        const int t0 = chunk_at(it) * C, valid = min(C, p.len - t0);
+        // ---- the chunk's decays: lane = token
+        float gv = lane < valid ? raw[64 * (it % 3) + lane] * LOG2E : 0.f;
+        gv = gv < -200.f ? -200.f : gv;  // e^-138 is nothing
+        const float gm = rintf(gv * 64.f) * (1.f / 64.f), H = running_sum(gm), L = running_sum(gv - gm), HT = lane_value(H, 63), LT = lane_value(L, 63);
+        sums[lane] = H;
+        sums[64 + lane] = L;
+        if (wave == 0) {
+          const float head = between(H, L, 0.f, 0.f), tail = between(HT, LT, H, L);
+          float* f = factors + 256 * (it & 1);
+          f[lane] = (rev ? tail : head) * ro.row_scale;
+          f[64 + lane] = lane < valid ? (rev ? head : tail) * ro.col_scale : 0.f;
+          f[128 + lane] = between(HT, LT, 0.f, 0.f);
+          if (!OUT) whole_h += HT, whole_l += LT;
+        }
+        if constexpr (OUT) {
+          // ---- pairs of one row tile: rows of the result are j, its column is i
+          const unsigned xr = xt(it) + XC::rows(lane) + mine * 16 * XC::ROWB, yr = yt(it) + XC::rows(lane);
+          char* pairs = lds + R::PAIRS + (it & 1) * R::PAIRB;
+          const float hi_ = sums[i], li_ = sums[64 + i];
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) {
+            if (j % WPI != wave % WPI || !R::needed(mine, j, rev)) continue;
+            floatx4 sc[F::TP];
+#pragma unroll
+            for (int t = 0; t < F::TP; ++t) sc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+              const Frag xf = XC::by_row(xr, 0, s);
+#pragma unroll
+              for (int t = 0; t < F::TP; ++t) F::mma(sc[t], XC::by_row(yr, (F::K * j + 16 * t) * XC::ROWB, s), xf);
+            }
+#pragma unroll
+            for (int t = 0; t < F::TP; ++t) {
+              const int j0 = F::K * j + 16 * t + g4;
+              const floatx4 hj = load4(sums + j0), lj = load4(sums + 64 + j0);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const bool on = rev ? j0 + r >= i && j0 + r < valid : j0 + r <= i;
+                const float f = (rev ? between(hj[r], lj[r], hi_, li_) : between(hi_, li_, hj[r], lj[r])) * a.scale;
+                sc[t][r] = on ? sc[t][r] * f : 0.f;
+              }
+            }
+            Frag hi, lo;
+            split<true>(sc, hi, lo);
+            char* q = pairs + R::slot(mine, j, rev) * F::PARTS * 1024 + 16 * lane;
+            *reinterpret_cast<Frag*>(q) = hi;
+            if (F::PARTS == 2) *reinterpret_cast<Frag*>(q + 1024) = lo;
+          }
+        }
+      }
+      dma_wait<0>();
+      lds_barrier();
+    }
+    if (dots && nchunk > 0) leave_dots(nchunk - 1);
+    if (!OUT && item == 0 && threadIdx.x == 256) a.whole[(int64_t)slot * a.H + h] = between(whole_h, whole_l, 0.f, 0.f);
+    return;
+  }
+  // -------------------------------------------------------------------------------------------------------- state and results
+  // tile i of the state holds rows 16 i + 4 g + r of column n0 + l16
   floatx4 st[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) st[i] = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -303,171 +396,121 @@ template <typename T, int KW, int BUFS, bool OUT> __global__ __launch_bounds__(2
       for (int r = 0; r < 4; ++r)
         if (16 * i + g4 + r < ro.sk && n < ro.sn) st[i][r] = s[(int64_t)(16 * i + g4 + r) * step_k];
   }
-  float* red = reinterpret_cast<float*>(lds + R::DOTS);  // [wave][inter, pairs][C]
-  const bool dots = OUT && ro.dots;
-  const auto leave_dots = [&](int chunk) {
-    const int t0 = chunk * C, i = threadIdx.x % C, kind = threadIdx.x / C;
-    if (kind < 2 && t0 + i < p.len) {
-      const float* q = red + kind * C + i;
-      ro.dots[(int64_t)(kind * ro.slabs + item) * a.dots_step + (int64_t)(p.b * a.H + h) * a.T + p.tok + t0 + i] = (q[0] + q[2 * C]) + (q[4 * C] + q[6 * C]);
+  const bool here = n0 + g4 < ro.vw;  // this lane's four columns of a result exist
+  T* op = OUT ? const_cast<T*>(head_of<T>(ro.out, p, h)) + n0 + g4 : nullptr;
+  const T* wp = dots ? head_of<T>(ro.w, p, h) + n0 + g4 : nullptr;
+  const auto partners = [&](floatx4 (&wv)[NI], int it) {
+    const int t0 = chunk_at(it) * C;
+#pragma unroll
+    for (int t = 0; t < NI; ++t) {
+      wv[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+      if (t0 + 16 * t + l16 < p.len && here) wv[t] = load4(wp + (int64_t)(t0 + 16 * t + l16) * ro.w.st);
     }
   };
-  float whole_h = 0.f, whole_l = 0.f;
-  int done = -1;  // the chunk before
-  bool counted = false;
-  if (nchunk > 0) fetch(rev ? nchunk - 1 : 0, 0);
+  lds_barrier();  // the first chunk's tiles
+  lds_barrier();  // its pairs
   for (int it = 0; it < nchunk; ++it) {
-    const int chunk = rev ? nchunk - 1 - it : it, t0 = chunk * C, valid = min(C, p.len - t0), buf = BUFS == 2 ? it & 1 : 0;
-    if (counted) dma_wait<NI>();  // all but the results of the chunk before
-    else dma_wait<0>();
-    lds_barrier();
+    const int t0 = chunk_at(it) * C, valid = min(C, p.len - t0);
     floatx4 wv[NI];
-    if (dots) {
-      if (it > 0) leave_dots(done);
-      const T* wp = head_of<T>(ro.w, p, h) + (int64_t)t0 * ro.w.st + n0 + g4;
-#pragma unroll
-      for (int t = 0; t < NI; ++t) {
-        wv[t] = floatx4{0.f, 0.f, 0.f, 0.f};
-        if (16 * t + l16 < valid && n0 + g4 < ro.vw) wv[t] = load4(wp + (int64_t)(16 * t + l16) * ro.w.st);
-      }
-    }
-    if (BUFS == 2 && it + 1 < nchunk) fetch(rev ? chunk - 1 : chunk + 1, buf ^ 1);
-    // ---- the chunk's decays: lane = token
-    float gv = lane < valid ? raw[64 * buf + lane] * LOG2E : 0.f;
-    gv = gv < -200.f ? -200.f : gv;  // e^-138 is nothing
-    const float gm = rintf(gv * 64.f) * (1.f / 64.f), H = running_sum(gm), L = running_sum(gv - gm), HT = lane_value(H, 63), LT = lane_value(L, 63);
-    const float head = between(H, L, 0.f, 0.f), tail = between(HT, LT, H, L), total = between(HT, LT, 0.f, 0.f);
-    gates[lane] = H;
-    gates[64 + lane] = L;
-    gates[128 + lane] = (rev ? tail : head) * ro.row_scale;
-    gates[192 + lane] = lane < valid ? (rev ? head : tail) * ro.col_scale : 0.f;
-    if (!OUT) whole_h += HT, whole_l += LT;
-    const unsigned xr = xt(buf) + XC::rows(lane), yr = yt(buf) + XC::rows(lane), yc = yt(buf) + XC::cols(lane), zc = zt(buf) + ZC::cols(lane);
-    char* pairs = lds + R::PAIRS;
-    const auto needed = [&](int i, int j) { return rev ? F::K * j + F::K > 16 * i : F::K * j <= 16 * i + 15; };  // pairs of row tile i with columns of block j
-    floatx4 acc[NI];
-    if constexpr (OUT) {
-      // ---- pairs of one row tile a wave: rows of the result are j, its column is i
-      const int it16 = wave / WPI, i = 16 * it16 + l16;
-      floatx4 sc[NJ][F::TP];
-#pragma unroll
-      for (int j = 0; j < NJ; ++j)
-#pragma unroll
-        for (int t = 0; t < F::TP; ++t) sc[j][t] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        const Frag xf = XC::by_row(xr, it16 * 16 * XC::ROWB, s);
-#pragma unroll
-        for (int j = 0; j < NJ; ++j)
-          if (j % WPI == wave % WPI && needed(it16, j)) {
-#pragma unroll
-            for (int t = 0; t < F::TP; ++t) F::mma(sc[j][t], XC::by_row(yr, (F::K * j + 16 * t) * XC::ROWB, s), xf);
-          }
-      }
-      const float hi_ = gates[i], li_ = gates[64 + i];
-#pragma unroll
-      for (int j = 0; j < NJ; ++j)
-        if (j % WPI == wave % WPI && needed(it16, j)) {
-#pragma unroll
-          for (int t = 0; t < F::TP; ++t) {
-            const int j0 = F::K * j + 16 * t + g4;
-            const floatx4 hj = load4(gates + j0), lj = load4(gates + 64 + j0);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const bool on = rev ? j0 + r >= i && j0 + r < valid : j0 + r <= i;
-              const float f = (rev ? between(hj[r], lj[r], hi_, li_) : between(hi_, li_, hj[r], lj[r])) * a.scale;
-              sc[j][t][r] = on ? sc[j][t][r] * f : 0.f;
-            }
-          }
-          Frag hi, lo;
-          split(sc[j], hi, lo);
-          char* q = pairs + (it16 * NJ + j) * F::PARTS * 1024 + 16 * lane;
-          *reinterpret_cast<Frag*>(q) = hi;
-          if (F::PARTS == 2) *reinterpret_cast<Frag*>(q + 1024) = lo;
-        }
-      // ---- what the state gives: rows of the result are columns of z, its column is i
-#pragma unroll
-      for (int t = 0; t < NI; ++t) acc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        Frag hi, lo;
-        floatx4 v[F::TP];
-#pragma unroll
-        for (int t = 0; t < F::TP; ++t) v[t] = st[F::TP * s + t];
-        split(v, hi, lo);
-#pragma unroll
-        for (int t = 0; t < NI; ++t) {
-          const Frag xf = XC::by_row(xr, 16 * t * XC::ROWB, s);
-          F::mma(acc[t], hi, xf);
-          if (F::PARTS == 2) F::mma(acc[t], lo, xf);
-        }
-      }
-    }
+    if (dots) partners(wv, it);
+    const float* f = factors + 256 * (it & 1);
+    const unsigned xr = xt(it) + XC::rows(lane), yc = yt(it) + XC::cols(lane), zc = zt(it) + ZC::cols(lane);
+    const char* pairs = lds + R::PAIRS + (it & 1) * R::PAIRB + 16 * lane;
     // ---- z by columns, as it is and with each token's factor
     Frag zf[NJ], zh[NJ], zl[NJ];
     bool odd = false;
 #pragma unroll
+    for (int j = 0; j < NJ; ++j) zf[j] = ZC::by_col(zc, F::K * j, wave);
+    floatx4 acc[NI];
+    if constexpr (OUT) {
+      // ---- what the state gives: rows of the result are columns of z, its column is i
+      const auto from_state = [&](auto guard) {
+#pragma unroll
+        for (int t = 0; t < NI; ++t) acc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+          Frag hi, lo, xf[NI];
+          floatx4 v[F::TP];
+#pragma unroll
+          for (int t = 0; t < NI; ++t) xf[t] = XC::by_row(xr, 16 * t * XC::ROWB, s);
+#pragma unroll
+          for (int t = 0; t < F::TP; ++t) v[t] = st[F::TP * s + t];
+          split<decltype(guard)::value>(v, hi, lo);
+#pragma unroll
+          for (int t = 0; t < NI; ++t) F::mma(acc[t], hi, xf[t]);
+          if (F::PARTS == 2)
+#pragma unroll
+            for (int t = 0; t < NI; ++t) F::mma(acc[t], lo, xf[t]);
+        }
+      };
+      from_state(std::false_type{});
+      if (F::PARTS == 2) {
+        float any = 0.f;
+#pragma unroll
+        for (int t = 0; t < NI; ++t) any += (acc[t][0] + acc[t][1]) + (acc[t][2] + acc[t][3]);
+        if (__any(!is_finite(any))) from_state(std::true_type{});  // an infinite state: what its rounding left is not a number
+      }
+    }
+#pragma unroll
     for (int j = 0; j < NJ; ++j) {
-      zf[j] = ZC::by_col(zc, F::K * j, wave);
       floatx4 v[F::TP];
 #pragma unroll
       for (int t = 0; t < F::TP; ++t) {
-        const floatx4 f = load4(gates + 192 + F::K * j + 16 * t + g4);
+        const floatx4 c = load4(f + 64 + F::K * j + 16 * t + g4);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const float z = F::get(zf[j], t, r);
-          const bool fine = is_finite(z);
-          odd = odd || !fine;
-          v[t][r] = fine || F::K * j + 16 * t + g4 + r < valid ? z * f[r] : 0.f;
-          if (!fine) F::put(zf[j], t, r, 0.f);
+          odd = odd || !is_finite(z);
+          v[t][r] = z * c[r];
         }
       }
-      split(v, zh[j], zl[j]);
+      split<false>(v, zh[j], zl[j]);
     }
     odd = __any(odd);
-    // ---- the state behind the chunk
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      st[i] *= total;
+    if (odd) {
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
-        const Frag yf = XC::by_col(yc, F::K * j, i);
-        F::mma(st[i], yf, zh[j]);
-        if (F::PARTS == 2) F::mma(st[i], yf, zl[j]);
+        floatx4 v[F::TP];
+#pragma unroll
+        for (int t = 0; t < F::TP; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int row = F::K * j + 16 * t + g4 + r;
+            const float z = F::get(zf[j], t, r);
+            v[t][r] = row < valid ? z * f[64 + row] : 0.f;
+            if (!is_finite(z)) F::put(zf[j], t, r, 0.f);
+          }
+        split<true>(v, zh[j], zl[j]);
       }
     }
-    if (OUT || BUFS == 1) lds_barrier();  // the pairs are there, and nothing reads the tiles any more
-    if (BUFS == 1 && it + 1 < nchunk) fetch(rev ? chunk - 1 : chunk + 1, 0);
     if constexpr (OUT) {
       float inter[NI];
 #pragma unroll
       for (int t = 0; t < NI; ++t) {
-        acc[t] *= gates[128 + 16 * t + l16];
+        acc[t] *= f[16 * t + l16];
         if (dots) inter[t] = acc[t][0] * wv[t][0] + acc[t][1] * wv[t][1] + acc[t][2] * wv[t][2] + acc[t][3] * wv[t][3];
       }
       floatx4 in[NI];
 #pragma unroll
-      for (int t = 0; t < NI; ++t) {
-        in[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+      for (int t = 0; t < NI; ++t) in[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int part = 0; part < F::PARTS; ++part)
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
-          if (needed(t, j)) {
-            const char* q = pairs + (t * NJ + j) * F::PARTS * 1024 + 16 * lane;
-            F::mma(in[t], zf[j], *reinterpret_cast<const Frag*>(q));
-            if (F::PARTS == 2) F::mma(in[t], zf[j], *reinterpret_cast<const Frag*>(q + 1024));
-          }
-      }
+#pragma unroll
+          for (int t = 0; t < NI; ++t)
+            if (R::needed(t, j, rev)) F::mma(in[t], zf[j], *reinterpret_cast<const Frag*>(pairs + (R::slot(t, j, rev) * F::PARTS + part) * 1024));
       if (odd) {  // values that are not finite were taken out of the product, where a masked pair would be 0 times one: added pair by pair
+        const T* zp = head_of<T>(ro.z, p, h) + n0 + g4;
 #pragma unroll 1
         for (int j = 0; j < valid; ++j) {
-          const bool here = n0 + g4 < ro.vw;
-          const floatx4 z = here ? load4(zp + (int64_t)(t0 + j) * ro.z.st + 16 * wave + g4) : floatx4{0.f, 0.f, 0.f, 0.f};
+          const floatx4 z = here ? load4(zp + (int64_t)(t0 + j) * ro.z.st) : floatx4{0.f, 0.f, 0.f, 0.f};
           const int k = j % F::K, e = k % 4, tile = k / 16, from = (k % 16) / 4;  // its slot and the lane group that holds it
 #pragma unroll
           for (int t = 0; t < NI; ++t) {
             const int i = 16 * t + l16;
             if (rev ? j < i : j > i) continue;
-            const T* q = reinterpret_cast<const T*>(pairs + (t * NJ + j / F::K) * F::PARTS * 1024 + 16 * (16 * from + l16)) + 4 * tile + e;
+            const T* q = reinterpret_cast<const T*>(lds + R::PAIRS + (it & 1) * R::PAIRB + R::slot(t, j / F::K, rev) * F::PARTS * 1024 + 16 * (16 * from + l16)) + 4 * tile + e;
             const float x = to_f32(q[0]) + (F::PARTS == 2 ? to_f32(q[1024 / sizeof(T)]) : 0.f);
 #pragma unroll
             for (int r = 0; r < 4; ++r)
@@ -475,24 +518,31 @@ template <typename T, int KW, int BUFS, bool OUT> __global__ __launch_bounds__(2
           }
         }
       }
-      T* op = const_cast<T*>(head_of<T>(ro.out, p, h)) + (int64_t)t0 * ro.out.st + n0 + g4;
 #pragma unroll
       for (int t = 0; t < NI; ++t) {
         if (dots) {
           float x = inter[t], y = in[t][0] * wv[t][0] + in[t][1] * wv[t][1] + in[t][2] * wv[t][2] + in[t][3] * wv[t][3];
           x = xor32_sum(xor16_sum(x));
           y = xor32_sum(xor16_sum(y));
-          if (g4 == 0) red[(2 * wave) * C + 16 * t + l16] = x, red[(2 * wave + 1) * C + 16 * t + l16] = y;
+          float* q = red + (it & 1) * 8 * C + 2 * wave * C + 16 * t + l16;
+          if (g4 == 0) q[0] = x, q[C] = y;
         }
-        if (16 * t + l16 < valid && n0 + g4 < ro.vw) store4(op + (int64_t)(16 * t + l16) * ro.out.st, acc[t] + in[t]);
+        if (16 * t + l16 < valid && here) store4(op + (int64_t)(t0 + 16 * t + l16) * ro.out.st, acc[t] + in[t]);
       }
-      counted = valid == C && n0 + 16 <= ro.vw;
     }
-    done = chunk;
-  }
-  if (dots && nchunk > 0) {
+    // ---- the state behind the chunk
+    const float total = f[128];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) st[i] *= total;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const Frag yf = XC::by_col(yc, F::K * j, i);
+        F::mma(st[i], yf, zh[j]);
+        if (F::PARTS == 2) F::mma(st[i], yf, zl[j]);
+      }
     lds_barrier();
-    leave_dots(done);
   }
   if (ro.fin && (!OUT || (rev ? p.first : p.last))) {
     float* s = ro.fin + ((int64_t)(OUT ? p.row : slot) * a.H + h) * state_size + (int64_t)n * step_n;
@@ -502,7 +552,6 @@ template <typename T, int KW, int BUFS, bool OUT> __global__ __launch_bounds__(2
       for (int r = 0; r < 4; ++r)
         if (16 * i + g4 + r < ro.sk && n < ro.sn) s[(int64_t)(16 * i + g4 + r) * step_k] = st[i][r];
   }
-  if (!OUT && item == 0 && threadIdx.x == 0) a.whole[(int64_t)slot * a.H + h] = between(whole_h, whole_l, 0.f, 0.f);
 }
 
 // States before every segment (behind it, backwards) from what each adds: in place, four elements a thread, a row's segments one after the other.
@@ -710,12 +759,12 @@ int64_t ceil_div(int64_t x, int64_t y) { return (x + y - 1) / y; }
 constexpr int MAX_D = 256, SHORTEST = 512;
 
 // Tokens of a segment, a multiple of 64, or 0: rows are walked whole.  Segments read keys and values (queries and gradients) once more, so they
-// are for few rows: 512 workgroups at least, of 512 tokens and more.  The rows of a packed batch are taken for one: their lengths are not
-// known here, and sequences of one segment are walked once whatever its size.
+// are for rows and heads that leave most CUs without a workgroup: as many as give every CU one, of 512 tokens and more.  The rows of a packed
+// batch are taken for one: their lengths are not known here, and sequences of one segment are walked once whatever its size.
 int segment(const lnx_decay_args* a) {
   const int64_t walks = (a->nseq ? 1 : (int64_t)a->B) * a->H * ceil_div(a->dv, SLAB);
-  if (walks >= 192) return 0;
-  int64_t s = up((int)ceil_div(a->T, ceil_div(512, walks)), 64);
+  if (walks > 128) return 0;
+  int64_t s = up((int)ceil_div(a->T, 256 / walks), 64);
   if (s < SHORTEST) s = SHORTEST;
   return s >= a->T ? 0 : (int)s;
 }
@@ -794,27 +843,22 @@ Walk walk(const lnx_decay_args* a, const Layout& l) {
   return k;
 }
 
-template <typename T, int KW, int BUFS, bool OUT> int start(const Walk& k, const char* name, hipStream_t st) {
-  const auto kernel = decay_walk_kernel<T, KW, BUFS, OUT>;
-  constexpr int bytes = Room<T, KW, BUFS, OUT>::BYTES;
+template <typename T, int KW, bool OUT> int start(const Walk& k, const char* name, hipStream_t st) {
+  const auto kernel = decay_walk_kernel<T, KW, OUT>;
+  constexpr int bytes = Room<T, KW, OUT>::BYTES;
+  static_assert(bytes <= 160 * 1024, "LDS of a CU");
   if (int rc = lnx_lds_limit(reinterpret_cast<const void*>(kernel), bytes)) return rc;
   lnx_profile_mark(name, st);
-  hipLaunchKernelGGL(kernel, dim3((unsigned)((int64_t)k.units * k.per)), dim3(256), bytes, st, k);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)((int64_t)k.units * k.per)), dim3(512), bytes, st, k);
   return LNX_OK;
 }
-// kw: the widest of the launch's keys
 template <typename T, bool OUT> int start(Walk& k, int roles, const char* name, hipStream_t st) {
   k.per = 0;
-  int kw = 0;
+  int kw = 0;  // the widest of the launch's keys
   for (int i = 0; i < roles; ++i) k.per += k.role[i].slabs, kw = kw < k.role[i].kw ? k.role[i].kw : kw;
-  // two buffers where a CU has one workgroup
-  if (OUT && roles == 1 && !k.role[0].dots && (int64_t)k.units * k.per <= 256) {
-    if (kw <= 64) return start<T, 64, 2, OUT>(k, name, st);
-    if (kw <= 128) return start<T, 128, 2, OUT>(k, name, st);
-  }
-  if (kw <= 64) return start<T, 64, 1, OUT>(k, name, st);
-  if (kw <= 128) return start<T, 128, 1, OUT>(k, name, st);
-  return start<T, 256, 1, OUT>(k, name, st);
+  if (kw <= 64) return start<T, 64, OUT>(k, name, st);
+  if (kw <= 128) return start<T, 128, OUT>(k, name, st);
+  return start<T, 256, OUT>(k, name, st);
 }
 
 void join(const lnx_decay_args* a, const Layout& l, float* states, const float* whole, const float* init, bool rev, hipStream_t st) {
@@ -879,7 +923,9 @@ template <typename T> int backward(const lnx_decay_args* a, hipStream_t st) {
   else d.dg = a->d_g;
   d.B = a->B, d.H = a->H, d.T = a->T, d.nseq = a->nseq, d.slabs = q.slabs, d.step = k.dots_step, d.size = (int64_t)a->dk * a->dv;
   lnx_profile_mark("decay_gate_grad", st);
-  decay_gate_grad_kernel<Form<T>::C><<<dim3((unsigned)(l.rows * a->H)), 1024, 0, st>>>(d);
+  const dim3 rows((unsigned)(l.rows * a->H));
+  if (q.kw <= 128) decay_gate_grad_kernel<chunk_of<T, 128>()><<<rows, 1024, 0, st>>>(d);
+  else decay_gate_grad_kernel<chunk_of<T, 256>()><<<rows, 1024, 0, st>>>(d);
   if (a->g_per_head) {
     lnx_profile_mark("decay_gate_sum", st);
     decay_gate_sum_kernel<<<dim3((unsigned)a->H), 256, 0, st>>>(d.part, l.rows, a->H, a->d_g);
