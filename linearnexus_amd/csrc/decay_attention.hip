@@ -138,12 +138,13 @@ __device__ __forceinline__ float running_sum(float x) {
 }
 __device__ __forceinline__ float lane_value(float x, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane)); }
 
-// 2^(difference of two sums), each a multiple of 1/64 and a rest
-__device__ __forceinline__ float between(float h1, float l1, float h0, float l0) {
-#pragma clang fp reassociate(off)
-  const float h = h1 - h0, l = l1 - l0;
-  return __builtin_amdgcn_exp2f(h + l);
+// A value as it is, which the compiler may not regroup or fuse with what takes it
+__device__ __forceinline__ float rounded(float x) {
+  asm("" : "+v"(x));
+  return x;
 }
+// 2^(difference of two sums), each a multiple of 1/64 and a rest
+__device__ __forceinline__ float between(float h1, float l1, float h0, float l0) { return __builtin_amdgcn_exp2f(rounded(h1 - h0) + (l1 - l0)); }
 
 struct Side {
   void* p;
@@ -246,17 +247,348 @@ template <typename T, int KW, bool OUT> struct Room {
   static __device__ __forceinline__ bool needed(int i, int j, bool rev) { return rev ? Form<T>::K * (j + 1) > 16 * i : Form<T>::K * j <= 16 * i + 15; }
 };
 
-// A walk's eight waves.  Four hold the state, 16 columns each, and turn chunk c into results; the other four bring chunk c + 2 to LDS and form the
-// decays and the pairs of chunk c + 1, one tile of 16 rows each.  One barrier a chunk.
-template <typename T, int KW, bool OUT> __global__ __launch_bounds__(512) void decay_walk_kernel(Walk a) {
+// What a workgroup works on
+struct Task {
+  Spot p;
+  int slot, h, item, nchunk, col0, vw;  // vw: columns of its slab that exist
+};
+template <bool REV> __device__ __forceinline__ int chunk_at(const Task& k, int it) { return REV ? k.nchunk - 1 - it : it; }
+
+// Scheduling of a stretch of MFMAS matrix instructions: READS reads of LDS first, then VALUS vector instructions behind each of them.  Left to itself
+// the compiler puts what can run beside a matrix instruction (16 cycles) before or behind the whole run.
+template <typename T, int READS, int MFMAS, int VALUS> __device__ __forceinline__ void interleave() {
+  if constexpr (sizeof(T) == 2) {
+    if constexpr (READS > 0) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+#pragma unroll
+    for (int i = 0; i < MFMAS; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x2, VALUS, 0);
+    }
+  }
+}
+
+// Four of a walk's eight waves: they bring chunk c + 1 to LDS and form the decays and the pairs of chunk c, one tile of 16 rows each, while
+// the others walk chunk c - 1.  One barrier a chunk.
+template <typename T, int KW, bool OUT, bool REV> __device__ __forceinline__ void walk_pairs(const Walk& a, const Role& ro, const Task& k, char* lds) {
+  typedef Form<T> F;
+  typedef typename F::Frag Frag;
+  typedef Cells<T, KW> XC;
+  typedef Room<T, KW, OUT> R;
+  constexpr int C = R::C, NI = R::NI, NJ = R::NJ, NS = KW / F::K;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) - 4, l16 = lane & 15, g4 = 4 * (lane >> 4);
+  const Spot& p = k.p;
+  const unsigned lds0 = lds_byte_addr(lds);
+  const T* xp = OUT ? head_of<T>(ro.x, p, k.h) : nullptr;
+  const T* yp = head_of<T>(ro.y, p, k.h);
+  const T* zp = head_of<T>(ro.z, p, k.h) + k.col0;
+  const float* gp = a.g + p.b * a.gb + k.h * a.gh + p.tok * a.gt;
+  const Mover<T, KW, C> mx(OUT ? ro.x.st : 0, wave, lane), my(ro.y.st, wave, lane);
+  const Mover<T, SLAB, C> mz(ro.z.st, wave, lane);
+  const auto fetch = [&](int it, int buf) {
+    const int t0 = chunk_at<REV>(k, it) * C, valid = min(C, p.len - t0);
+    const unsigned tiles = lds0 + buf * R::BUF;
+    my.fetch(tiles, yp, ro.y.st, t0, valid, ro.kw, wave, lane);
+    if constexpr (OUT) mx.fetch(tiles + R::XB + R::ZB, xp, ro.x.st, t0, valid, ro.kw, wave, lane);
+    mz.fetch(tiles + R::XB, zp, ro.z.st, t0, valid, k.vw, wave, lane);
+    if (wave == 0) dma4(gp + (int64_t)(t0 + min(lane, valid - 1)) * a.gt, lds0 + R::RAW + 256 * buf);
+  };
+  const float* red = reinterpret_cast<const float*>(lds + R::DOTS);
+  const bool dots = OUT && ro.dots;
+  const auto leave_dots = [&](int it) {
+    const int t0 = chunk_at<REV>(k, it) * C, tid = threadIdx.x - 256, i = tid % C, kind = tid / C;
+    if (kind < 2 && t0 + i < p.len) {
+      const float* q = red + (it & 1) * 8 * C + kind * C + i;
+      ro.dots[(int64_t)(kind * ro.slabs + k.item) * a.dots_step + (int64_t)(p.b * a.H + k.h) * a.T + p.tok + t0 + i] = (q[0] + q[2 * C]) + (q[4 * C] + q[6 * C]);
+    }
+  };
+  constexpr int WPI = NI >= 4 ? 1 : 4 / NI;  // waves of a row tile: they share its blocks
+  const int mine = wave / WPI, i = 16 * mine + l16;
+  float* sums = reinterpret_cast<float*>(lds + R::SUMS) + 128 * wave;  // of this wave: multiples, rests
+  const float* raw = reinterpret_cast<const float*>(lds + R::RAW);
+  float whole_h = 0.f, whole_l = 0.f;
+  if (k.nchunk > 0) fetch(0, 0);
+  dma_wait<0>();
+  lds_barrier();
+  for (int it = 0, buf = 0; it <= k.nchunk; ++it) {
+    const int next = buf == 2 ? 0 : buf + 1;
+    if (it + 1 < k.nchunk) fetch(it + 1, next);
+    if (dots && it >= 2) leave_dots(it - 2);
+    if (it < k.nchunk) {
+      const int t0 = chunk_at<REV>(k, it) * C, valid = min(C, p.len - t0);
+      // ---- the chunk's decays: lane = token
+      float gv = lane < valid ? raw[64 * buf + lane] * LOG2E : 0.f;
+      gv = gv < -200.f ? -200.f : gv;  // e^-138 is nothing
+      const float gm = rounded(rintf(gv * 64.f) * (1.f / 64.f)), H = running_sum(gm), L = running_sum(gv - gm), HT = lane_value(H, 63), LT = lane_value(L, 63);
+      sums[lane] = H;
+      sums[64 + lane] = L;
+      if (wave == 0) {
+        const float head = between(H, L, 0.f, 0.f), tail = between(HT, LT, H, L);
+        float* f = reinterpret_cast<float*>(lds + R::FACTORS) + 256 * (it & 1);
+        f[lane] = (REV ? tail : head) * ro.row_scale;
+        f[64 + lane] = lane < valid ? (REV ? head : tail) * ro.col_scale : 0.f;
+        f[128 + lane] = between(HT, LT, 0.f, 0.f);
+        if (!OUT) whole_h += HT, whole_l += LT;
+      }
+      if constexpr (OUT) {
+        // ---- pairs of one row tile: rows of the result are j, its column is i
+        const unsigned xr = lds0 + buf * R::BUF + R::XB + R::ZB + XC::rows(lane) + mine * 16 * XC::ROWB, yr = lds0 + buf * R::BUF + XC::rows(lane);
+        char* pairs = lds + R::PAIRS + (it & 1) * R::PAIRB + 16 * lane;
+        const float hi_ = sums[i], li_ = sums[64 + i];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          if (j % WPI != wave % WPI || !R::needed(mine, j, REV)) continue;
+          floatx4 sc[F::TP];
+          Frag xf[NS], yf[NS][F::TP];
+#pragma unroll
+          for (int s = 0; s < NS; ++s) {
+            xf[s] = XC::by_row(xr, 0, s);
+#pragma unroll
+            for (int t = 0; t < F::TP; ++t) yf[s][t] = XC::by_row(yr, (F::K * j + 16 * t) * XC::ROWB, s);
+          }
+#pragma unroll
+          for (int t = 0; t < F::TP; ++t) sc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int t = 0; t < F::TP; ++t) F::mma(sc[t], yf[s][t], xf[s]);
+#pragma unroll
+          for (int t = 0; t < F::TP; ++t) {
+            const int j0 = F::K * j + 16 * t + g4;
+            const floatx4 hj = load4(sums + j0), lj = load4(sums + 64 + j0);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const bool on = REV ? j0 + r >= i && j0 + r < valid : j0 + r <= i;
+              const float f = REV ? between(hj[r], lj[r], hi_, li_) : between(hi_, li_, hj[r], lj[r]);
+              sc[t][r] = rounded(on ? sc[t][r] * f : 0.f);
+            }
+          }
+          Frag hi, lo;
+          split<true>(sc, hi, lo);
+          char* q = pairs + R::slot(mine, j, REV) * F::PARTS * 1024;
+          *reinterpret_cast<Frag*>(q) = hi;
+          if (F::PARTS == 2) *reinterpret_cast<Frag*>(q + 1024) = lo;
+        }
+      }
+    }
+    dma_wait<0>();
+    lds_barrier();
+    buf = next;
+  }
+  if (dots && k.nchunk > 0) leave_dots(k.nchunk - 1);
+  if (!OUT && k.item == 0 && threadIdx.x == 256) a.whole[(int64_t)k.slot * a.H + k.h] = between(whole_h, whole_l, 0.f, 0.f);
+}
+
+// The other four: 16 columns of the state and of the results each.
+template <typename T, int KW, bool OUT, bool REV, bool DOTS> __device__ __forceinline__ void walk_state(const Walk& a, const Role& ro, const Task& k, char* lds) {
   typedef Form<T> F;
   typedef typename F::Frag Frag;
   typedef Cells<T, KW> XC;
   typedef Cells<T, SLAB> ZC;
   typedef Room<T, KW, OUT> R;
-  constexpr int C = R::C, NI = R::NI, NJ = R::NJ, NS = KW / F::K, NT = KW / 16;
+  constexpr int C = R::C, NI = R::NI, NJ = R::NJ, NS = KW / F::K, NT = KW / 16, TP = F::TP, PARTS = F::PARTS;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g4 = 4 * (lane >> 4), n0 = k.col0 + 16 * wave;
+  const Spot& p = k.p;
+  const unsigned lds0 = lds_byte_addr(lds);
+  // tile i of the state holds rows 16 i + 4 g + r of column n0 + l16
+  floatx4 st[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) st[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+  const int n = n0 + l16, step_k = ro.turned ? 1 : a.dv, step_n = ro.turned ? a.dv : 1;
+  const int64_t state_size = (int64_t)ro.sk * ro.sn;
+  if (OUT && ro.init) {
+    const float* s = ro.init + ((int64_t)(a.by_slot ? k.slot : p.row) * a.H + k.h) * state_size + (int64_t)n * step_n;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (16 * i + g4 + r < ro.sk && n < ro.sn) st[i][r] = s[(int64_t)(16 * i + g4 + r) * step_k];
+  }
+  const bool here = n0 + g4 < ro.vw;  // this lane's four columns of a result exist
+  T* op = OUT ? const_cast<T*>(head_of<T>(ro.out, p, k.h)) + n0 + g4 : nullptr;
+  const T* wp = DOTS ? head_of<T>(ro.w, p, k.h) + n0 + g4 : nullptr;
+  const unsigned xa = lds0 + R::XB + R::ZB + XC::rows(lane), ya = lds0 + XC::cols(lane), za = (lds0 + R::XB + ZC::cols(lane)) ^ (sizeof(T) == 2 ? 32 * wave : 64 * wave);
+  lds_barrier();  // the first chunk's tiles
+  lds_barrier();  // its pairs
+  for (int it = 0, at = 0; it < k.nchunk; ++it) {
+    const int t0 = chunk_at<REV>(k, it) * C, valid = min(C, p.len - t0);
+    floatx4 wv[NI];
+    if constexpr (DOTS) {
+#pragma unroll
+      for (int t = 0; t < NI; ++t) {
+        wv[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+        if (16 * t + l16 < valid && here) wv[t] = load4(wp + (int64_t)(t0 + 16 * t + l16) * ro.w.st);
+      }
+    }
+    const float* f = reinterpret_cast<const float*>(lds + R::FACTORS) + 256 * (it & 1);
+    const unsigned xr = xa + at, yc = ya + at, zc = za + at;
+    const char* pairs = lds + R::PAIRS + (it & 1) * R::PAIRB + 16 * lane;
+    const float total = f[128];
+    Frag zf[NJ], zh[NJ], zl[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) zf[j] = ZC::by_col(zc, F::K * j, 0);
+    // z with each token's factor, as an operand
+    const auto scaled = [&](auto guard, bool& odd) {
+      constexpr bool G = decltype(guard)::value;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        floatx4 v[TP];
+#pragma unroll
+        for (int t = 0; t < TP; ++t) {
+          const floatx4 c = load4(f + 64 + F::K * j + 16 * t + g4);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float z = F::get(zf[j], t, r);
+            v[t][r] = rounded(!G || F::K * j + 16 * t + g4 + r < valid ? z * c[r] : 0.f);
+            if (G && !is_finite(z)) F::put(zf[j], t, r, 0.f), odd = true;
+          }
+        }
+        split<G>(v, zh[j], zl[j]);
+      }
+    };
+    floatx4 acc[NI], in[NI];
+    Frag x[2][NI], hi[2], lo[2];
+    const auto read_x = [&](int s) {
+#pragma unroll
+      for (int t = 0; t < NI; ++t) x[s & 1][t] = XC::by_row(xr, 16 * t * XC::ROWB, s);
+    };
+    const auto split_state = [&](auto guard, int s) {
+      floatx4 v[TP];
+#pragma unroll
+      for (int t = 0; t < TP; ++t) v[t] = st[TP * s + t];
+      split<decltype(guard)::value>(v, hi[s & 1], lo[s & 1]);
+    };
+    const auto from_state = [&](int s) {
+#pragma unroll
+      for (int t = 0; t < NI; ++t) F::mma(acc[t], hi[s & 1], x[s & 1][t]);
+      if (PARTS == 2)
+#pragma unroll
+        for (int t = 0; t < NI; ++t) F::mma(acc[t], lo[s & 1], x[s & 1][t]);
+    };
+    if constexpr (OUT) {
+      // ---- what the state gives: rows of the result are columns of z, its column is i
+#pragma unroll
+      for (int t = 0; t < NI; ++t) acc[t] = in[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+      read_x(0);
+      split_state(std::false_type{}, 0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        if (s + 1 < NS) read_x(s + 1);
+        if (s + 1 < NS) split_state(std::false_type{}, s + 1);
+        from_state(s);
+        interleave<T, 2 * NI, PARTS * NI, 3>();
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      // ---- what the chunk's pairs give
+#pragma unroll
+      for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int t = 0; t < NI; ++t)
+            if (R::needed(t, j, REV)) F::mma(in[t], zf[j], *reinterpret_cast<const Frag*>(pairs + (R::slot(t, j, REV) * PARTS + part) * 1024));
+    }
+    bool odd = false;
+    scaled(std::false_type{}, odd);
+    if constexpr (OUT) interleave<T, 8, R::SLOTS * PARTS, 8>();
+    // Anything that is not finite shows in one of these sums: what the rounding of an infinite value left is not a number
+    {
+      float any = 0.f;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int t = 0; t < TP; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) any += F::get(PARTS == 2 ? zl[j] : zf[j], t, r);
+      if constexpr (OUT && PARTS == 2)
+#pragma unroll
+        for (int t = 0; t < NI; ++t) any += (acc[t][0] + acc[t][1]) + (acc[t][2] + acc[t][3]);
+      odd = __any(!is_finite(any));
+    }
+    if (odd) {
+      odd = false;
+      scaled(std::true_type{}, odd);
+      odd = __any(odd);
+      if constexpr (OUT) {
+#pragma unroll
+        for (int t = 0; t < NI; ++t) acc[t] = in[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+          read_x(s);
+          split_state(std::true_type{}, s);
+          from_state(s);
+        }
+        // values that are not finite are taken out of the product, where a masked pair would be 0 times one, and added pair by pair
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+          for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int t = 0; t < NI; ++t)
+              if (R::needed(t, j, REV)) F::mma(in[t], zf[j], *reinterpret_cast<const Frag*>(pairs + (R::slot(t, j, REV) * PARTS + part) * 1024));
+        if (odd) {
+          const T* zp = head_of<T>(ro.z, p, k.h) + n0 + g4;
+#pragma unroll 1
+          for (int j = 0; j < valid; ++j) {
+            const floatx4 z = here ? load4(zp + (int64_t)(t0 + j) * ro.z.st) : floatx4{0.f, 0.f, 0.f, 0.f};
+            const int e = j % 4, tile = j % F::K / 16, from = j % 16 / 4;  // its slot and the lane group that holds it
+#pragma unroll
+            for (int t = 0; t < NI; ++t) {
+              const int i = 16 * t + l16;
+              if (REV ? j < i : j > i) continue;
+              const T* q = reinterpret_cast<const T*>(pairs + R::slot(t, j / F::K, REV) * PARTS * 1024 + 16 * (16 * from + l16 - lane)) + 4 * tile + e;
+              const float w = to_f32(q[0]) + (PARTS == 2 ? to_f32(q[1024 / sizeof(T)]) : 0.f);
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (!is_finite(z[r])) in[t][r] += w * z[r];
+            }
+          }
+        }
+      }
+    }
+    // ---- the state behind the chunk, and beside its products the results
+#pragma unroll
+    for (int i = 0; i < NT; ++i) st[i] *= total;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const Frag yf = XC::by_col(yc, F::K * j, i);
+        F::mma(st[i], yf, zh[j]);
+        if (PARTS == 2) F::mma(st[i], yf, zl[j]);
+      }
+    if constexpr (OUT) {
+#pragma unroll
+      for (int t = 0; t < NI; ++t) {
+        acc[t] *= f[16 * t + l16];
+        in[t] *= a.scale;
+        if constexpr (DOTS) {
+          float xd = acc[t][0] * wv[t][0] + acc[t][1] * wv[t][1] + acc[t][2] * wv[t][2] + acc[t][3] * wv[t][3];
+          float yd = in[t][0] * wv[t][0] + in[t][1] * wv[t][1] + in[t][2] * wv[t][2] + in[t][3] * wv[t][3];
+          xd = xor32_sum(xor16_sum(xd));
+          yd = xor32_sum(xor16_sum(yd));
+          float* q = reinterpret_cast<float*>(lds + R::DOTS) + (it & 1) * 8 * C + 2 * wave * C + 16 * t + l16;  // [it & 1][wave][inter, pairs][C]
+          if (g4 == 0) q[0] = xd, q[C] = yd;
+        }
+        if (16 * t + l16 < valid && here) store4(op + (int64_t)(t0 + 16 * t + l16) * ro.out.st, acc[t] + in[t]);
+      }
+    }
+    lds_barrier();
+    at = at == 2 * R::BUF ? 0 : at + R::BUF;
+  }
+  if (ro.fin && (!OUT || (REV ? p.first : p.last))) {
+    float* s = ro.fin + ((int64_t)(OUT ? p.row : k.slot) * a.H + k.h) * state_size + (int64_t)n * step_n;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (16 * i + g4 + r < ro.sk && n < ro.sn) s[(int64_t)(16 * i + g4 + r) * step_k] = st[i][r];
+  }
+}
+
+template <typename T, int KW, bool OUT> __global__ __launch_bounds__(512) void decay_walk_kernel(Walk a) {
+  typedef Room<T, KW, OUT> R;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
-  const int lane = threadIdx.x & 63, wave8 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = wave8 & 3, l16 = lane & 15, g4 = 4 * (lane >> 4);
   // workgroups of one (slot, head) follow each other on one XCD, whose L2 then holds what they share
   const int w = blockIdx.x;
   int unit, item;
@@ -270,287 +602,25 @@ template <typename T, int KW, bool OUT> __global__ __launch_bounds__(512) void d
   int which = 0;
   while (item >= a.role[which].slabs) item -= a.role[which++].slabs;
   const Role& ro = a.role[which];
-  const int slot = unit / a.H, h = unit % a.H;
-  const Spot p = spot(a, slot);
-  if (!p.on) return;
-  const bool rev = ro.rev;
-  if (!OUT && (rev ? p.first : p.last)) return;  // nothing walks on from there
-  const int col0 = item * SLAB, vw = min(SLAB, ro.vw - col0), n0 = col0 + 16 * wave;
-  const int nchunk = (p.len + C - 1) / C;
-  const auto chunk_at = [&](int it) { return rev ? nchunk - 1 - it : it; };
-  const unsigned lds0 = lds_byte_addr(lds);
-  const auto yt = [&](int it) { return lds0 + it % 3 * R::BUF; };
-  const auto zt = [&](int it) { return lds0 + it % 3 * R::BUF + R::XB; };
-  const auto xt = [&](int it) { return lds0 + it % 3 * R::BUF + R::XB + R::ZB; };
-  float* factors = reinterpret_cast<float*>(lds + R::FACTORS);  // [it & 1]: of rows [64], of columns [64], of the state
-  float* red = reinterpret_cast<float*>(lds + R::DOTS);         // [it & 1][wave][inter, pairs][C]
-  const bool dots = OUT && ro.dots;
-  if (ro.kw < KW || vw < SLAB) {
+  Task k;
+  k.slot = unit / a.H, k.h = unit % a.H, k.item = item;
+  k.p = spot(a, k.slot);
+  if (!k.p.on) return;
+  if (!OUT && (ro.rev ? k.p.first : k.p.last)) return;  // nothing walks on from there
+  k.nchunk = (k.p.len + R::C - 1) / R::C, k.col0 = item * SLAB, k.vw = min(SLAB, ro.vw - k.col0);
+  if (ro.kw < KW || k.vw < SLAB) {
     for (int i = threadIdx.x * 16; i < R::PAIRS; i += 512 * 16) *reinterpret_cast<floatx4*>(lds + i) = floatx4{0.f, 0.f, 0.f, 0.f};
     lds_barrier();
   }
-  if (wave8 >= 4) {
-    // ---------------------------------------------------------------------------------------------------- tiles, decays, pairs
-    const T* xp = OUT ? head_of<T>(ro.x, p, h) : nullptr;
-    const T* yp = head_of<T>(ro.y, p, h);
-    const T* zp = head_of<T>(ro.z, p, h) + col0;
-    const float* gp = a.g + p.b * a.gb + h * a.gh + p.tok * a.gt;
-    const Mover<T, KW, C> mx(OUT ? ro.x.st : 0, wave, lane), my(ro.y.st, wave, lane);
-    const Mover<T, SLAB, C> mz(ro.z.st, wave, lane);
-    const auto fetch = [&](int it) {
-      const int t0 = chunk_at(it) * C, valid = min(C, p.len - t0);
-      if constexpr (OUT) mx.fetch(xt(it), xp, ro.x.st, t0, valid, ro.kw, wave, lane);
-      my.fetch(yt(it), yp, ro.y.st, t0, valid, ro.kw, wave, lane);
-      mz.fetch(zt(it), zp, ro.z.st, t0, valid, vw, wave, lane);
-      if (wave == 0) dma4(gp + (int64_t)(t0 + min(lane, valid - 1)) * a.gt, lds0 + R::RAW + 256 * (it % 3));
-    };
-    const auto leave_dots = [&](int it) {
-      const int t0 = chunk_at(it) * C, tid = threadIdx.x - 256, i = tid % C, kind = tid / C;
-      if (kind < 2 && t0 + i < p.len) {
-        const float* q = red + (it & 1) * 8 * C + kind * C + i;
-        ro.dots[(int64_t)(kind * ro.slabs + item) * a.dots_step + (int64_t)(p.b * a.H + h) * a.T + p.tok + t0 + i] = (q[0] + q[2 * C]) + (q[4 * C] + q[6 * C]);
-      }
-    };
-    constexpr int WPI = NI >= 4 ? 1 : 4 / NI;  // waves of a row tile: they share its blocks
-    const int mine = wave / WPI, i = 16 * mine + l16;
-    float* sums = reinterpret_cast<float*>(lds + R::SUMS) + 128 * wave;  // of this wave: multiples, rests
-    const float* raw = reinterpret_cast<const float*>(lds + R::RAW);
-    float whole_h = 0.f, whole_l = 0.f;
-    if (nchunk > 0) fetch(0);
-    dma_wait<0>();
-    lds_barrier();
-    for (int it = 0; it <= nchunk; ++it) {  // chunk `it` is prepared while it - 1 is walked
-      if (it + 1 < nchunk) fetch(it + 1);
-      if (dots && it >= 2) leave_dots(it - 2);
-      if (it < nchunk) {
-        const int t0 = chunk_at(it) * C, valid = min(C, p.len - t0);
-        // ---- the chunk's decays: lane = token
-        float gv = lane < valid ? raw[64 * (it % 3) + lane] * LOG2E : 0.f;
-        gv = gv < -200.f ? -200.f : gv;  // e^-138 is nothing
-        const float gm = rintf(gv * 64.f) * (1.f / 64.f), H = running_sum(gm), L = running_sum(gv - gm), HT = lane_value(H, 63), LT = lane_value(L, 63);
-        sums[lane] = H;
-        sums[64 + lane] = L;
-        if (wave == 0) {
-          const float head = between(H, L, 0.f, 0.f), tail = between(HT, LT, H, L);
-          float* f = factors + 256 * (it & 1);
-          f[lane] = (rev ? tail : head) * ro.row_scale;
-          f[64 + lane] = lane < valid ? (rev ? head : tail) * ro.col_scale : 0.f;
-          f[128 + lane] = between(HT, LT, 0.f, 0.f);
-          if (!OUT) whole_h += HT, whole_l += LT;
-        }
-        if constexpr (OUT) {
-          // ---- pairs of one row tile: rows of the result are j, its column is i
-          const unsigned xr = xt(it) + XC::rows(lane) + mine * 16 * XC::ROWB, yr = yt(it) + XC::rows(lane);
-          char* pairs = lds + R::PAIRS + (it & 1) * R::PAIRB;
-          const float hi_ = sums[i], li_ = sums[64 + i];
-#pragma unroll
-          for (int j = 0; j < NJ; ++j) {
-            if (j % WPI != wave % WPI || !R::needed(mine, j, rev)) continue;
-            floatx4 sc[F::TP];
-#pragma unroll
-            for (int t = 0; t < F::TP; ++t) sc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int s = 0; s < NS; ++s) {
-              const Frag xf = XC::by_row(xr, 0, s);
-#pragma unroll
-              for (int t = 0; t < F::TP; ++t) F::mma(sc[t], XC::by_row(yr, (F::K * j + 16 * t) * XC::ROWB, s), xf);
-            }
-#pragma unroll
-            for (int t = 0; t < F::TP; ++t) {
-              const int j0 = F::K * j + 16 * t + g4;
-              const floatx4 hj = load4(sums + j0), lj = load4(sums + 64 + j0);
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const bool on = rev ? j0 + r >= i && j0 + r < valid : j0 + r <= i;
-                const float f = (rev ? between(hj[r], lj[r], hi_, li_) : between(hi_, li_, hj[r], lj[r])) * a.scale;
-                sc[t][r] = on ? sc[t][r] * f : 0.f;
-              }
-            }
-            Frag hi, lo;
-            split<true>(sc, hi, lo);
-            char* q = pairs + R::slot(mine, j, rev) * F::PARTS * 1024 + 16 * lane;
-            *reinterpret_cast<Frag*>(q) = hi;
-            if (F::PARTS == 2) *reinterpret_cast<Frag*>(q + 1024) = lo;
-          }
-        }
-      }
-      dma_wait<0>();
-      lds_barrier();
-    }
-    if (dots && nchunk > 0) leave_dots(nchunk - 1);
-    if (!OUT && item == 0 && threadIdx.x == 256) a.whole[(int64_t)slot * a.H + h] = between(whole_h, whole_l, 0.f, 0.f);
-    return;
-  }
-  // -------------------------------------------------------------------------------------------------------- state and results
-  // tile i of the state holds rows 16 i + 4 g + r of column n0 + l16
-  floatx4 st[NT];
-#pragma unroll
-  for (int i = 0; i < NT; ++i) st[i] = floatx4{0.f, 0.f, 0.f, 0.f};
-  const int n = n0 + l16, step_k = ro.turned ? 1 : a.dv, step_n = ro.turned ? a.dv : 1;
-  const int64_t state_size = (int64_t)ro.sk * ro.sn;
-  if (OUT && ro.init) {
-    const float* s = ro.init + ((int64_t)(a.by_slot ? slot : p.row) * a.H + h) * state_size + (int64_t)n * step_n;
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (16 * i + g4 + r < ro.sk && n < ro.sn) st[i][r] = s[(int64_t)(16 * i + g4 + r) * step_k];
-  }
-  const bool here = n0 + g4 < ro.vw;  // this lane's four columns of a result exist
-  T* op = OUT ? const_cast<T*>(head_of<T>(ro.out, p, h)) + n0 + g4 : nullptr;
-  const T* wp = dots ? head_of<T>(ro.w, p, h) + n0 + g4 : nullptr;
-  const auto partners = [&](floatx4 (&wv)[NI], int it) {
-    const int t0 = chunk_at(it) * C;
-#pragma unroll
-    for (int t = 0; t < NI; ++t) {
-      wv[t] = floatx4{0.f, 0.f, 0.f, 0.f};
-      if (t0 + 16 * t + l16 < p.len && here) wv[t] = load4(wp + (int64_t)(t0 + 16 * t + l16) * ro.w.st);
-    }
-  };
-  lds_barrier();  // the first chunk's tiles
-  lds_barrier();  // its pairs
-  for (int it = 0; it < nchunk; ++it) {
-    const int t0 = chunk_at(it) * C, valid = min(C, p.len - t0);
-    floatx4 wv[NI];
-    if (dots) partners(wv, it);
-    const float* f = factors + 256 * (it & 1);
-    const unsigned xr = xt(it) + XC::rows(lane), yc = yt(it) + XC::cols(lane), zc = zt(it) + ZC::cols(lane);
-    const char* pairs = lds + R::PAIRS + (it & 1) * R::PAIRB + 16 * lane;
-    // ---- z by columns, as it is and with each token's factor
-    Frag zf[NJ], zh[NJ], zl[NJ];
-    bool odd = false;
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) zf[j] = ZC::by_col(zc, F::K * j, wave);
-    floatx4 acc[NI];
-    if constexpr (OUT) {
-      // ---- what the state gives: rows of the result are columns of z, its column is i
-      const auto from_state = [&](auto guard) {
-#pragma unroll
-        for (int t = 0; t < NI; ++t) acc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < NS; ++s) {
-          Frag hi, lo, xf[NI];
-          floatx4 v[F::TP];
-#pragma unroll
-          for (int t = 0; t < NI; ++t) xf[t] = XC::by_row(xr, 16 * t * XC::ROWB, s);
-#pragma unroll
-          for (int t = 0; t < F::TP; ++t) v[t] = st[F::TP * s + t];
-          split<decltype(guard)::value>(v, hi, lo);
-#pragma unroll
-          for (int t = 0; t < NI; ++t) F::mma(acc[t], hi, xf[t]);
-          if (F::PARTS == 2)
-#pragma unroll
-            for (int t = 0; t < NI; ++t) F::mma(acc[t], lo, xf[t]);
-        }
-      };
-      from_state(std::false_type{});
-      if (F::PARTS == 2) {
-        float any = 0.f;
-#pragma unroll
-        for (int t = 0; t < NI; ++t) any += (acc[t][0] + acc[t][1]) + (acc[t][2] + acc[t][3]);
-        if (__any(!is_finite(any))) from_state(std::true_type{});  // an infinite state: what its rounding left is not a number
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      floatx4 v[F::TP];
-#pragma unroll
-      for (int t = 0; t < F::TP; ++t) {
-        const floatx4 c = load4(f + 64 + F::K * j + 16 * t + g4);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float z = F::get(zf[j], t, r);
-          odd = odd || !is_finite(z);
-          v[t][r] = z * c[r];
-        }
-      }
-      split<false>(v, zh[j], zl[j]);
-    }
-    odd = __any(odd);
-    if (odd) {
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        floatx4 v[F::TP];
-#pragma unroll
-        for (int t = 0; t < F::TP; ++t)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int row = F::K * j + 16 * t + g4 + r;
-            const float z = F::get(zf[j], t, r);
-            v[t][r] = row < valid ? z * f[64 + row] : 0.f;
-            if (!is_finite(z)) F::put(zf[j], t, r, 0.f);
-          }
-        split<true>(v, zh[j], zl[j]);
-      }
-    }
-    if constexpr (OUT) {
-      float inter[NI];
-#pragma unroll
-      for (int t = 0; t < NI; ++t) {
-        acc[t] *= f[16 * t + l16];
-        if (dots) inter[t] = acc[t][0] * wv[t][0] + acc[t][1] * wv[t][1] + acc[t][2] * wv[t][2] + acc[t][3] * wv[t][3];
-      }
-      floatx4 in[NI];
-#pragma unroll
-      for (int t = 0; t < NI; ++t) in[t] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int part = 0; part < F::PARTS; ++part)
-#pragma unroll
-        for (int j = 0; j < NJ; ++j)
-#pragma unroll
-          for (int t = 0; t < NI; ++t)
-            if (R::needed(t, j, rev)) F::mma(in[t], zf[j], *reinterpret_cast<const Frag*>(pairs + (R::slot(t, j, rev) * F::PARTS + part) * 1024));
-      if (odd) {  // values that are not finite were taken out of the product, where a masked pair would be 0 times one: added pair by pair
-        const T* zp = head_of<T>(ro.z, p, h) + n0 + g4;
-#pragma unroll 1
-        for (int j = 0; j < valid; ++j) {
-          const floatx4 z = here ? load4(zp + (int64_t)(t0 + j) * ro.z.st) : floatx4{0.f, 0.f, 0.f, 0.f};
-          const int k = j % F::K, e = k % 4, tile = k / 16, from = (k % 16) / 4;  // its slot and the lane group that holds it
-#pragma unroll
-          for (int t = 0; t < NI; ++t) {
-            const int i = 16 * t + l16;
-            if (rev ? j < i : j > i) continue;
-            const T* q = reinterpret_cast<const T*>(lds + R::PAIRS + (it & 1) * R::PAIRB + R::slot(t, j / F::K, rev) * F::PARTS * 1024 + 16 * (16 * from + l16)) + 4 * tile + e;
-            const float x = to_f32(q[0]) + (F::PARTS == 2 ? to_f32(q[1024 / sizeof(T)]) : 0.f);
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (!is_finite(z[r])) in[t][r] += x * z[r];
-          }
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < NI; ++t) {
-        if (dots) {
-          float x = inter[t], y = in[t][0] * wv[t][0] + in[t][1] * wv[t][1] + in[t][2] * wv[t][2] + in[t][3] * wv[t][3];
-          x = xor32_sum(xor16_sum(x));
-          y = xor32_sum(xor16_sum(y));
-          float* q = red + (it & 1) * 8 * C + 2 * wave * C + 16 * t + l16;
-          if (g4 == 0) q[0] = x, q[C] = y;
-        }
-        if (16 * t + l16 < valid && here) store4(op + (int64_t)(t0 + 16 * t + l16) * ro.out.st, acc[t] + in[t]);
-      }
-    }
-    // ---- the state behind the chunk
-    const float total = f[128];
-#pragma unroll
-    for (int i = 0; i < NT; ++i) st[i] *= total;
-#pragma unroll
-    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        const Frag yf = XC::by_col(yc, F::K * j, i);
-        F::mma(st[i], yf, zh[j]);
-        if (F::PARTS == 2) F::mma(st[i], yf, zl[j]);
-      }
-    lds_barrier();
-  }
-  if (ro.fin && (!OUT || (rev ? p.first : p.last))) {
-    float* s = ro.fin + ((int64_t)(OUT ? p.row : slot) * a.H + h) * state_size + (int64_t)n * step_n;
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (16 * i + g4 + r < ro.sk && n < ro.sn) s[(int64_t)(16 * i + g4 + r) * step_k] = st[i][r];
+  if (threadIdx.x >= 256) {
+    if (ro.rev) walk_pairs<T, KW, OUT, true>(a, ro, k, lds);
+    else walk_pairs<T, KW, OUT, false>(a, ro, k, lds);
+  } else if (OUT && ro.dots) {
+    if (ro.rev) walk_state<T, KW, OUT, true, OUT>(a, ro, k, lds);
+    else walk_state<T, KW, OUT, false, OUT>(a, ro, k, lds);
+  } else {
+    if (ro.rev) walk_state<T, KW, OUT, true, false>(a, ro, k, lds);
+    else walk_state<T, KW, OUT, false, false>(a, ro, k, lds);
   }
 }
 
