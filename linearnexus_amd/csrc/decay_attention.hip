@@ -407,16 +407,20 @@ template <typename T, int KW, bool OUT, bool REV, bool DOTS> __device__ __forcei
   T* op = OUT ? const_cast<T*>(head_of<T>(ro.out, p, k.h)) + n0 + g4 : nullptr;
   const T* wp = DOTS ? head_of<T>(ro.w, p, k.h) + n0 + g4 : nullptr;
   const unsigned xa = lds0 + R::XB + R::ZB + XC::rows(lane), ya = lds0 + XC::cols(lane), za = (lds0 + R::XB + ZC::cols(lane)) ^ (sizeof(T) == 2 ? 32 * wave : 64 * wave);
+  // the state is there before the loop begins: a wait for it inside would, from the second turn on, be one for the results' stores
+#pragma unroll
+  for (int i = 0; i < NT; ++i) asm volatile("" : "+v"(st[i]));
   lds_barrier();  // the first chunk's tiles
   lds_barrier();  // its pairs
   for (int it = 0, at = 0; it < k.nchunk; ++it) {
     const int t0 = chunk_at<REV>(k, it) * C, valid = min(C, p.len - t0);
-    floatx4 wv[NI];
+    typename Vec4<T>::V wr[NI];  // as they lie in memory: converted only where they are used, behind the products
     if constexpr (DOTS) {
 #pragma unroll
       for (int t = 0; t < NI; ++t) {
-        wv[t] = floatx4{0.f, 0.f, 0.f, 0.f};
-        if (16 * t + l16 < valid && here) wv[t] = load4(wp + (int64_t)(t0 + 16 * t + l16) * ro.w.st);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) wr[t][r] = (T)0.f;
+        if (16 * t + l16 < valid && here) wr[t] = *reinterpret_cast<const typename Vec4<T>::V*>(wp + (int64_t)(t0 + 16 * t + l16) * ro.w.st);
       }
     }
     const float* f = reinterpret_cast<const float*>(lds + R::FACTORS) + 256 * (it & 1);
@@ -563,8 +567,9 @@ template <typename T, int KW, bool OUT, bool REV, bool DOTS> __device__ __forcei
         acc[t] *= f[16 * t + l16];
         in[t] *= a.scale;
         if constexpr (DOTS) {
-          float xd = acc[t][0] * wv[t][0] + acc[t][1] * wv[t][1] + acc[t][2] * wv[t][2] + acc[t][3] * wv[t][3];
-          float yd = in[t][0] * wv[t][0] + in[t][1] * wv[t][1] + in[t][2] * wv[t][2] + in[t][3] * wv[t][3];
+          float xd = 0.f, yd = 0.f;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) xd += acc[t][r] * to_f32(wr[t][r]), yd += in[t][r] * to_f32(wr[t][r]);
           xd = xor32_sum(xor16_sum(xd));
           yd = xor32_sum(xor16_sum(yd));
           float* q = reinterpret_cast<float*>(lds + R::DOTS) + (it & 1) * 8 * C + 2 * wave * C + 16 * t + l16;  // [it & 1][wave][inter, pairs][C]
