@@ -48,20 +48,28 @@ template <> struct Form<float> {
 template <typename T, int KW> constexpr int chunk_of() { return (sizeof(T) == 2 ? 64 : 32) / (KW > 128 ? 2 : 1); }
 __device__ __forceinline__ bool is_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
-// Result tiles as an operand, and what its rounding left; GUARD: of an infinite value nothing (otherwise NaN, for the caller to notice)
-template <bool GUARD> __device__ __forceinline__ void split(const floatx4 (&v)[2], bf16x8& hi, bf16x8& lo) {
+// Result tiles as an operand, and what its rounding left.  Of an infinite value that would not be a number: it becomes some finite one, which
+// changes no sum that the infinite one is in (and of values from 2^107 on the rest is cut).
+__device__ __forceinline__ void split(const floatx4 (&v)[2], bf16x8& hi, bf16x8& lo) {
   hi = Mma16::from_acc(v[0], v[1]);
   floatx4 d[2];
 #pragma unroll
   for (int a = 0; a < 2; ++a)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const float h = (float)hi[4 * a + r];
-      d[a][r] = !GUARD || is_finite(h) ? v[a][r] - h : 0.f;
-    }
+    for (int r = 0; r < 4; ++r) d[a][r] = __builtin_amdgcn_fmed3f(v[a][r] - (float)hi[4 * a + r], -1e30f, 1e30f);
   lo = Mma16::from_acc(d[0], d[1]);
 }
-template <bool GUARD> __device__ __forceinline__ void split(const floatx4 (&v)[1], floatx4& hi, floatx4&) { hi = v[0]; }
+__device__ __forceinline__ void split(const floatx4 (&v)[1], floatx4& hi, floatx4&) { hi = v[0]; }
+// Whether all of an operand's values are finite: their exponents, two of bf16 at a time
+__device__ __forceinline__ bool all_finite(const bf16x8& f) {
+  typedef unsigned uint4_ __attribute__((ext_vector_type(4)));
+  const uint4_ u = __builtin_bit_cast(uint4_, f);
+  unsigned any = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) any |= (u[i] & 0x7f807f80u) + 0x00800080u;
+  return !(any & 0x80008000u);
+}
+__device__ __forceinline__ bool all_finite(const floatx4& f) { return is_finite(f[0]) && is_finite(f[1]) && is_finite(f[2]) && is_finite(f[3]); }
 
 // A [C][W] tile in LDS as loads that go straight there leave it: 16-byte granules of a row permuted by an exclusive or with x(row), chosen so that
 // row operands (16 consecutive rows, one granule) and column operands (the transposing reads of two lane groups: 8 consecutive rows, 2 granules;
@@ -363,7 +371,7 @@ template <typename T, int KW, bool OUT, bool REV> __device__ __forceinline__ voi
             }
           }
           Frag hi, lo;
-          split<true>(sc, hi, lo);
+          split(sc, hi, lo);
           char* q = pairs + R::slot(mine, j, REV) * F::PARTS * 1024;
           *reinterpret_cast<Frag*>(q) = hi;
           if (F::PARTS == 2) *reinterpret_cast<Frag*>(q + 1024) = lo;
@@ -426,145 +434,160 @@ template <typename T, int KW, bool OUT, bool REV, bool DOTS> __device__ __forcei
     const float* f = reinterpret_cast<const float*>(lds + R::FACTORS) + 256 * (it & 1);
     const unsigned xr = xa + at, yc = ya + at, zc = za + at;
     const char* pairs = lds + R::PAIRS + (it & 1) * R::PAIRB + 16 * lane;
-    const float total = f[128];
-    Frag zf[NJ], zh[NJ], zl[NJ];
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) zf[j] = ZC::by_col(zc, F::K * j, 0);
-    // z with each token's factor, as an operand
-    const auto scaled = [&](auto guard, bool& odd) {
-      constexpr bool G = decltype(guard)::value;
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        floatx4 v[TP];
-#pragma unroll
-        for (int t = 0; t < TP; ++t) {
-          const floatx4 c = load4(f + 64 + F::K * j + 16 * t + g4);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float z = F::get(zf[j], t, r);
-            v[t][r] = rounded(!G || F::K * j + 16 * t + g4 + r < valid ? z * c[r] : 0.f);
-            if (G && !is_finite(z)) F::put(zf[j], t, r, 0.f), odd = true;
-          }
-        }
-        split<G>(v, zh[j], zl[j]);
-      }
-    };
-    floatx4 acc[NI], in[NI];
-    Frag x[2][NI], hi[2], lo[2];
+    // What LDS holds is read well ahead of its use: two steps of x, all pairs, four tiles of y
+    Frag zf[NJ], zh[NJ], zl[NJ], x[3][NI], hi[2], lo[2], pf[R::SLOTS > 0 ? R::SLOTS : 1][PARTS], yf[4][NJ];
+    floatx4 acc[NI], in[NI], cf[NJ][TP];
     const auto read_x = [&](int s) {
 #pragma unroll
-      for (int t = 0; t < NI; ++t) x[s & 1][t] = XC::by_row(xr, 16 * t * XC::ROWB, s);
+      for (int t = 0; t < NI; ++t) x[s % 3][t] = XC::by_row(xr, 16 * t * XC::ROWB, s);
     };
-    const auto split_state = [&](auto guard, int s) {
+    const auto read_pairs = [&](int half) {
+#pragma unroll
+      for (int t = 0; t < NI; ++t)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+          if (R::needed(t, j, REV) && (half < 0 || (t < (NI + 1) / 2) == (half == 0)))
+#pragma unroll
+            for (int part = 0; part < PARTS; ++part) pf[R::slot(t, j, REV)][part] = *reinterpret_cast<const Frag*>(pairs + (R::slot(t, j, REV) * PARTS + part) * 1024);
+    };
+    const auto read_y = [&](int i) {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) yf[i & 3][j] = XC::by_col(yc, F::K * j, i);
+    };
+    const auto split_state = [&](int s) {
       floatx4 v[TP];
 #pragma unroll
       for (int t = 0; t < TP; ++t) v[t] = st[TP * s + t];
-      split<decltype(guard)::value>(v, hi[s & 1], lo[s & 1]);
+      split(v, hi[s & 1], lo[s & 1]);
     };
-    const auto from_state = [&](int s) {
+    const auto from_state = [&](int s) {  // rows of the result are columns of z, its column is i
 #pragma unroll
-      for (int t = 0; t < NI; ++t) F::mma(acc[t], hi[s & 1], x[s & 1][t]);
+      for (int t = 0; t < NI; ++t) F::mma(acc[t], hi[s & 1], x[s % 3][t]);
       if (PARTS == 2)
 #pragma unroll
-        for (int t = 0; t < NI; ++t) F::mma(acc[t], lo[s & 1], x[s & 1][t]);
+        for (int t = 0; t < NI; ++t) F::mma(acc[t], lo[s & 1], x[s % 3][t]);
     };
-    if constexpr (OUT) {
-      // ---- what the state gives: rows of the result are columns of z, its column is i
-#pragma unroll
-      for (int t = 0; t < NI; ++t) acc[t] = in[t] = floatx4{0.f, 0.f, 0.f, 0.f};
-      read_x(0);
-      split_state(std::false_type{}, 0);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        if (s + 1 < NS) read_x(s + 1);
-        if (s + 1 < NS) split_state(std::false_type{}, s + 1);
-        from_state(s);
-        interleave<T, 2 * NI, PARTS * NI, 3>();
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      // ---- what the chunk's pairs give
+    const auto from_pairs = [&] {
 #pragma unroll
       for (int part = 0; part < PARTS; ++part)
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
           for (int t = 0; t < NI; ++t)
-            if (R::needed(t, j, REV)) F::mma(in[t], zf[j], *reinterpret_cast<const Frag*>(pairs + (R::slot(t, j, REV) * PARTS + part) * 1024));
-    }
-    bool odd = false;
-    scaled(std::false_type{}, odd);
-    if constexpr (OUT) interleave<T, 8, R::SLOTS * PARTS, 8>();
-    // Anything that is not finite shows in one of these sums: what the rounding of an infinite value left is not a number
-    {
-      float any = 0.f;
+            if (R::needed(t, j, REV)) F::mma(in[t], zf[j], pf[R::slot(t, j, REV)][part]);
+    };
+    // z with each token's factor, as an operand
+    const auto scaled = [&](auto guard) {
 #pragma unroll
-      for (int j = 0; j < NJ; ++j)
+      for (int j = 0; j < NJ; ++j) {
+        floatx4 v[TP];
 #pragma unroll
         for (int t = 0; t < TP; ++t)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) any += F::get(PARTS == 2 ? zl[j] : zf[j], t, r);
-      if constexpr (OUT && PARTS == 2)
-#pragma unroll
-        for (int t = 0; t < NI; ++t) any += (acc[t][0] + acc[t][1]) + (acc[t][2] + acc[t][3]);
-      odd = __any(!is_finite(any));
+          for (int r = 0; r < 4; ++r) {
+            const bool there = !decltype(guard)::value || F::K * j + 16 * t + g4 + r < valid;  // (0 times what is not finite)
+            v[t][r] = rounded(there ? F::get(zf[j], t, r) * cf[j][t][r] : 0.f);
+          }
+        split(v, zh[j], zl[j]);
+      }
+    };
+    if constexpr (OUT) {
+      read_x(0);
+      if (NS > 1) read_x(1);
     }
-    if (odd) {
-      odd = false;
-      scaled(std::true_type{}, odd);
-      odd = __any(odd);
+    const float total = f[128];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      zf[j] = ZC::by_col(zc, F::K * j, 0);
+#pragma unroll
+      for (int t = 0; t < TP; ++t) cf[j][t] = load4(f + 64 + F::K * j + 16 * t + g4);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (OUT) {
+      // ---- what the state gives
+#pragma unroll
+      for (int t = 0; t < NI; ++t) acc[t] = in[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+      split_state(0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        if (s + 2 < NS) read_x(s + 2);
+        else read_pairs(NS == 1 ? -1 : s + 2 - NS);
+        __builtin_amdgcn_sched_barrier(0);
+        if (s + 1 < NS) split_state(s + 1);
+        from_state(s);
+        interleave<T, 0, PARTS * NI, 3>();
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4 && i < NT; ++i) read_y(i);
+    __builtin_amdgcn_sched_barrier(0);
+    // ---- what the chunk's pairs give
+    if constexpr (OUT) from_pairs();
+    scaled(std::false_type{});
+    if constexpr (OUT) interleave<T, 0, R::SLOTS * PARTS, 9>();
+    bool fine = true;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) fine = fine && all_finite(zf[j]);
+    if (__any(!fine)) {
+      scaled(std::true_type{});
       if constexpr (OUT) {
+        // A masked pair would be 0 times such a value: they are taken out of the product and added pair by pair
 #pragma unroll
-        for (int t = 0; t < NI; ++t) acc[t] = in[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < NJ; ++j)
 #pragma unroll
-        for (int s = 0; s < NS; ++s) {
-          read_x(s);
-          split_state(std::true_type{}, s);
-          from_state(s);
-        }
-        // values that are not finite are taken out of the product, where a masked pair would be 0 times one, and added pair by pair
+          for (int t = 0; t < TP; ++t)
 #pragma unroll
-        for (int part = 0; part < PARTS; ++part)
+            for (int r = 0; r < 4; ++r)
+              if (!is_finite(F::get(zf[j], t, r))) F::put(zf[j], t, r, 0.f);
 #pragma unroll
-          for (int j = 0; j < NJ; ++j)
+        for (int t = 0; t < NI; ++t) {
+          in[t] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int t = 0; t < NI; ++t)
+          for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
               if (R::needed(t, j, REV)) F::mma(in[t], zf[j], *reinterpret_cast<const Frag*>(pairs + (R::slot(t, j, REV) * PARTS + part) * 1024));
-        if (odd) {
-          const T* zp = head_of<T>(ro.z, p, k.h) + n0 + g4;
+        }
+        const T* zp = head_of<T>(ro.z, p, k.h) + n0 + g4;
 #pragma unroll 1
-          for (int j = 0; j < valid; ++j) {
-            const floatx4 z = here ? load4(zp + (int64_t)(t0 + j) * ro.z.st) : floatx4{0.f, 0.f, 0.f, 0.f};
-            const int e = j % 4, tile = j % F::K / 16, from = j % 16 / 4;  // its slot and the lane group that holds it
+        for (int j = 0; j < valid; ++j) {
+          const floatx4 z = here ? load4(zp + (int64_t)(t0 + j) * ro.z.st) : floatx4{0.f, 0.f, 0.f, 0.f};
+          const int e = j % 4, tile = j % F::K / 16, from = j % 16 / 4;  // its slot and the lane group that holds it
 #pragma unroll
-            for (int t = 0; t < NI; ++t) {
-              const int i = 16 * t + l16;
-              if (REV ? j < i : j > i) continue;
-              const T* q = reinterpret_cast<const T*>(pairs + R::slot(t, j / F::K, REV) * PARTS * 1024 + 16 * (16 * from + l16 - lane)) + 4 * tile + e;
-              const float w = to_f32(q[0]) + (PARTS == 2 ? to_f32(q[1024 / sizeof(T)]) : 0.f);
+          for (int t = 0; t < NI; ++t) {
+            const int i = 16 * t + l16;
+            if (REV ? j < i : j > i) continue;
+            const T* q = reinterpret_cast<const T*>(pairs + R::slot(t, j / F::K, REV) * PARTS * 1024 + 16 * (16 * from + l16 - lane)) + 4 * tile + e;
+            const float w = to_f32(q[0]) + (PARTS == 2 ? to_f32(q[1024 / sizeof(T)]) : 0.f);
 #pragma unroll
-              for (int r = 0; r < 4; ++r)
-                if (!is_finite(z[r])) in[t][r] += w * z[r];
-            }
+            for (int r = 0; r < 4; ++r)
+              if (!is_finite(z[r])) in[t][r] += w * z[r];
           }
         }
       }
     }
     // ---- the state behind the chunk, and beside its products the results
+    float rf[NI];
+    if constexpr (OUT)
+#pragma unroll
+      for (int t = 0; t < NI; ++t) rf[t] = f[16 * t + l16];
 #pragma unroll
     for (int i = 0; i < NT; ++i) st[i] *= total;
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
+    for (int i = 0; i < NT; ++i) {
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const Frag yf = XC::by_col(yc, F::K * j, i);
-        F::mma(st[i], yf, zh[j]);
-        if (PARTS == 2) F::mma(st[i], yf, zl[j]);
-      }
+      for (int j = 0; j < NJ; ++j) F::mma(st[i], yf[i & 3][j], zh[j]);
+      if (PARTS == 2)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) F::mma(st[i], yf[i & 3][j], zl[j]);
+      if (i + 4 < NT) read_y(i + 4);
+    }
     if constexpr (OUT) {
 #pragma unroll
       for (int t = 0; t < NI; ++t) {
-        acc[t] *= f[16 * t + l16];
+        acc[t] *= rf[t];
         in[t] *= a.scale;
         if constexpr (DOTS) {
           float xd = 0.f, yd = 0.f;
