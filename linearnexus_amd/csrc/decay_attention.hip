@@ -48,18 +48,25 @@ template <> struct Form<float> {
 template <typename T, int KW> constexpr int chunk_of() { return (sizeof(T) == 2 ? 64 : 32) / (KW > 128 ? 2 : 1); }
 __device__ __forceinline__ bool is_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
-// Result tiles as an operand, and what its rounding left.  Of an infinite value that would not be a number: it becomes some finite one, which
-// changes no sum that the infinite one is in (and of values from 2^107 on the rest is cut).
+// Result tiles as an operand, and what its rounding left.  Of an infinite value that is not a number: as an integer it lies above 2^100, where rests
+// are cut (two at a time), so that it adds nothing to a sum that the infinite value is in.
+__device__ __forceinline__ bf16x4 rest_of(floatx4 v, bf16x4 h) {
+  typedef unsigned uint2_ __attribute__((ext_vector_type(2)));
+  uint2_ u = __builtin_bit_cast(uint2_, h);
+  asm("" : "+v"(u[0]), "+v"(u[1]));  // (not the value itself: -ffast-math takes a conversion and its inverse for nothing)
+  h = __builtin_bit_cast(bf16x4, u);
+  const floatx4 d = {v[0] - (float)h[0], v[1] - (float)h[1], v[2] - (float)h[2], v[3] - (float)h[3]};
+  u = __builtin_bit_cast(uint2_, pack_bf16x4(d));
+  typedef short short4_ __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(bf16x4, __builtin_elementwise_min(__builtin_bit_cast(short4_, u), short4_{0x7180, 0x7180, 0x7180, 0x7180}));
+}
 __device__ __forceinline__ void split(const floatx4 (&v)[2], bf16x8& hi, bf16x8& lo) {
-  hi = Mma16::from_acc(v[0], v[1]);
-  floatx4 d[2];
-#pragma unroll
-  for (int a = 0; a < 2; ++a)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) d[a][r] = __builtin_amdgcn_fmed3f(v[a][r] - (float)hi[4 * a + r], -1e30f, 1e30f);
-  lo = Mma16::from_acc(d[0], d[1]);
+  const bf16x4 h[2] = {pack_bf16x4(v[0]), pack_bf16x4(v[1])};
+  hi = Mma16::join(h[0], h[1]);
+  lo = Mma16::join(rest_of(v[0], h[0]), rest_of(v[1], h[1]));
 }
 __device__ __forceinline__ void split(const floatx4 (&v)[1], floatx4& hi, floatx4&) { hi = v[0]; }
+
 // Whether all of an operand's values are finite: their exponents, two of bf16 at a time
 __device__ __forceinline__ bool all_finite(const bf16x8& f) {
   typedef unsigned uint4_ __attribute__((ext_vector_type(4)));
@@ -130,6 +137,16 @@ template <int W> struct Cells<float, W> {
     return f;
   }
 };
+
+// Of two values the sums over pairs of rows of 16 lanes (over the halves): even rows (the lower half) get the first's, odd ones the second's
+__device__ __forceinline__ float rows_join16(float a, float b) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float rows_join32(float a, float b) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
 
 // Sum over the lanes up to this one
 template <int CTRL, int ROWS> __device__ __forceinline__ float from_lane(float x) {
@@ -222,19 +239,15 @@ template <typename T, int W, int C> struct Mover {
       off[i] = (unsigned)((r * (int)st + c) * (int)sizeof(T));
     }
   }
-  // rows t0 .. t0 + C - 1; rows behind the last of `valid` are copies of it, columns behind `width` keep the zeros that lie there
-  __device__ __forceinline__ void fetch(unsigned tile, const T* matrix, int64_t st, int64_t t0, int valid, int width, int wave, int lane) const {
-    const T* base = matrix + t0 * st;
-    if (valid == C && width >= W) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) dma16_at(base, off[i], tile + 1024 * (wave * N + i));
-    } else {
+  // Rows from `base` on, all of them there: load i of this wave's
+  __device__ __forceinline__ void one(int i, unsigned tile, const T* base, int wave) const { dma16_at(base, off[i], tile + 1024 * (wave * N + i)); }
+  // Rows behind the last of `valid` are copies of it, columns behind `width` keep the zeros that lie there
+  __device__ __forceinline__ void edge(unsigned tile, const T* base, int64_t st, int valid, int width, int wave, int lane) const {
 #pragma unroll 1
-      for (int i = 0; i < N; ++i) {
-        int r, c;
-        CL::src(64 * (wave * N + i) + lane, r, c);
-        if (c < width) dma16(base + (int64_t)min(r, valid - 1) * st + c, tile + 1024 * (wave * N + i));
-      }
+    for (int i = 0; i < N; ++i) {
+      int r, c;
+      CL::src(64 * (wave * N + i) + lane, r, c);
+      if (c < width) dma16(base + (int64_t)min(r, valid - 1) * st + c, tile + 1024 * (wave * N + i));
     }
   }
 };
@@ -253,6 +266,14 @@ template <typename T, int KW, bool OUT> struct Room {
   static __device__ __forceinline__ int slot(int i, int j, bool rev) { return SLOTS != 6 ? i * NJ + j : rev ? (i < 2 ? 2 * i + j : i + 2) : (i < 2 ? i : 2 * i - 2 + j); }
   // whether row tile i has pairs with block j
   static __device__ __forceinline__ bool needed(int i, int j, bool rev) { return rev ? Form<T>::K * (j + 1) > 16 * i : Form<T>::K * j <= 16 * i + 15; }
+  // The 16 x 16 tiles of pairs, ten of a chunk of 64, in four nearly equal shares: tile u of wave w; those above the diagonal hold zeros
+  static constexpr int UNITS = NI == 4 ? 3 : 1;
+  static __device__ __forceinline__ int units(int w) { return NI == 4 ? (w < 2 ? 2 : 3) : w < NI * (NI + 1) / 2; }
+  static __device__ __forceinline__ void unit(int w, int u, bool rev, int& i, int& j) {
+    if (NI == 4) i = w == 0 ? 3 * u : w, j = w == 0 ? 0 : w == 3 ? u + 1 : u;
+    else i = w > 0, j = w == 2;
+    if (rev) i = NI - 1 - i, j = NI - 1 - j;
+  }
 };
 
 // What a workgroup works on
@@ -282,7 +303,7 @@ template <typename T, int KW, bool OUT, bool REV> __device__ __forceinline__ voi
   typedef typename F::Frag Frag;
   typedef Cells<T, KW> XC;
   typedef Room<T, KW, OUT> R;
-  constexpr int C = R::C, NI = R::NI, NJ = R::NJ, NS = KW / F::K;
+  constexpr int C = R::C, NS = KW / F::K;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) - 4, l16 = lane & 15, g4 = 4 * (lane >> 4);
   const Spot& p = k.p;
   const unsigned lds0 = lds_byte_addr(lds);
@@ -292,13 +313,34 @@ template <typename T, int KW, bool OUT, bool REV> __device__ __forceinline__ voi
   const float* gp = a.g + p.b * a.gb + k.h * a.gh + p.tok * a.gt;
   const Mover<T, KW, C> mx(OUT ? ro.x.st : 0, wave, lane), my(ro.y.st, wave, lane);
   const Mover<T, SLAB, C> mz(ro.z.st, wave, lane);
-  const auto fetch = [&](int it, int buf) {
-    const int t0 = chunk_at<REV>(k, it) * C, valid = min(C, p.len - t0);
-    const unsigned tiles = lds0 + buf * R::BUF;
-    my.fetch(tiles, yp, ro.y.st, t0, valid, ro.kw, wave, lane);
-    if constexpr (OUT) mx.fetch(tiles + R::XB + R::ZB, xp, ro.x.st, t0, valid, ro.kw, wave, lane);
-    mz.fetch(tiles + R::XB, zp, ro.z.st, t0, valid, k.vw, wave, lane);
-    if (wave == 0) dma4(gp + (int64_t)(t0 + min(lane, valid - 1)) * a.gt, lds0 + R::RAW + 256 * buf);
+  // A chunk's loads, ten of a wave at KW = 128: a CU takes 64 bytes a cycle, so they are handed out between the steps of the work; `part` of PARTS_OF
+  constexpr int NX = OUT ? decltype(mx)::N : 0, NY = decltype(my)::N, NZ = decltype(mz)::N, PARTS_OF = 4;
+  int next_t0 = 0, next_valid = 0;
+  unsigned next_tiles = 0;
+  const auto aim = [&](int it, int buf) {
+    next_t0 = chunk_at<REV>(k, it) * C;
+    next_valid = it < k.nchunk ? min(C, p.len - next_t0) : 0;
+    next_tiles = lds0 + buf * R::BUF;
+    if (next_valid > 0 && wave == 0) dma4(gp + (int64_t)(next_t0 + min(lane, next_valid - 1)) * a.gt, lds0 + R::RAW + 256 * buf);
+  };
+  const auto fetch = [&](int part) {
+    if (next_valid <= 0) return;
+    const T* yb = yp + (int64_t)next_t0 * ro.y.st;
+    const T* zb = zp + (int64_t)next_t0 * ro.z.st;
+    const T* xb = OUT ? xp + (int64_t)next_t0 * ro.x.st : nullptr;
+    if (next_valid == C && ro.kw >= KW && k.vw == SLAB) {
+#pragma unroll
+      for (int i = 0; i < NY + NX + NZ; ++i) {
+        if (i * PARTS_OF / (NY + NX + NZ) != part) continue;
+        if (i < NY) my.one(i, next_tiles, yb, wave);
+        else if (i < NY + NX) mx.one(OUT ? i - NY : 0, next_tiles + R::XB + R::ZB, xb, wave);
+        else mz.one(i - NY - NX, next_tiles + R::XB, zb, wave);
+      }
+    } else if (part == 0) {
+      my.edge(next_tiles, yb, ro.y.st, next_valid, ro.kw, wave, lane);
+      if constexpr (OUT) mx.edge(next_tiles + R::XB + R::ZB, xb, ro.x.st, next_valid, ro.kw, wave, lane);
+      mz.edge(next_tiles + R::XB, zb, ro.z.st, next_valid, k.vw, wave, lane);
+    }
   };
   const float* red = reinterpret_cast<const float*>(lds + R::DOTS);
   const bool dots = OUT && ro.dots;
@@ -309,20 +351,25 @@ template <typename T, int KW, bool OUT, bool REV> __device__ __forceinline__ voi
       ro.dots[(int64_t)(kind * ro.slabs + k.item) * a.dots_step + (int64_t)(p.b * a.H + k.h) * a.T + p.tok + t0 + i] = (q[0] + q[2 * C]) + (q[4 * C] + q[6 * C]);
     }
   };
-  constexpr int WPI = NI >= 4 ? 1 : 4 / NI;  // waves of a row tile: they share its blocks
-  const int mine = wave / WPI, i = 16 * mine + l16;
   float* sums = reinterpret_cast<float*>(lds + R::SUMS) + 128 * wave;  // of this wave: multiples, rests
   const float* raw = reinterpret_cast<const float*>(lds + R::RAW);
   float whole_h = 0.f, whole_l = 0.f;
-  if (k.nchunk > 0) fetch(0, 0);
+  if constexpr (OUT)
+    for (int i = (threadIdx.x - 256) * 16; i < 2 * R::PAIRB; i += 256 * 16) *reinterpret_cast<floatx4*>(lds + R::PAIRS + i) = floatx4{0.f, 0.f, 0.f, 0.f};
+  aim(0, 0);
+#pragma unroll
+  for (int i = 0; i < PARTS_OF; ++i) fetch(i);
   dma_wait<0>();
   lds_barrier();
   for (int it = 0, buf = 0; it <= k.nchunk; ++it) {
     const int next = buf == 2 ? 0 : buf + 1;
-    if (it + 1 < k.nchunk) fetch(it + 1, next);
+    aim(it + 1, next);
+#pragma unroll
+    for (int i = 0; i < PARTS_OF; ++i) fetch(i);
     if (dots && it >= 2) leave_dots(it - 2);
     if (it < k.nchunk) {
       const int t0 = chunk_at<REV>(k, it) * C, valid = min(C, p.len - t0);
+      const unsigned xr = lds0 + buf * R::BUF + R::XB + R::ZB + XC::rows(lane), yr = lds0 + buf * R::BUF + XC::rows(lane);
       // ---- the chunk's decays: lane = token
       float gv = lane < valid ? raw[64 * buf + lane] * LOG2E : 0.f;
       gv = gv < -200.f ? -200.f : gv;  // e^-138 is nothing
@@ -338,43 +385,51 @@ template <typename T, int KW, bool OUT, bool REV> __device__ __forceinline__ voi
         if (!OUT) whole_h += HT, whole_l += LT;
       }
       if constexpr (OUT) {
-        // ---- pairs of one row tile: rows of the result are j, its column is i
-        const unsigned xr = lds0 + buf * R::BUF + R::XB + R::ZB + XC::rows(lane) + mine * 16 * XC::ROWB, yr = lds0 + buf * R::BUF + XC::rows(lane);
+        // ---- pairs: rows of a result are j, its column is i
         char* pairs = lds + R::PAIRS + (it & 1) * R::PAIRB + 16 * lane;
-        const float hi_ = sums[i], li_ = sums[64 + i];
+        const int units = R::units(wave);
+        floatx4 sc[R::UNITS];
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          if (j % WPI != wave % WPI || !R::needed(mine, j, REV)) continue;
-          floatx4 sc[F::TP];
-          Frag xf[NS], yf[NS][F::TP];
+        for (int u = 0; u < R::UNITS; ++u) sc[u] = floatx4{0.f, 0.f, 0.f, 0.f};
+        if (units > 0) {
+          // a wave's tiles are of one row tile, but the first of wave 0, whose third does not exist
+          int i0, i1, j[3];
+          R::unit(wave, 0, REV, i0, j[0]);
+          R::unit(wave, units > 2 ? 2 : 0, REV, i1, j[2]);  // (a product more where there are two)
+          R::unit(wave, units > 1 ? 1 : 0, REV, i1, j[1]);
 #pragma unroll
           for (int s = 0; s < NS; ++s) {
-            xf[s] = XC::by_row(xr, 0, s);
-#pragma unroll
-            for (int t = 0; t < F::TP; ++t) yf[s][t] = XC::by_row(yr, (F::K * j + 16 * t) * XC::ROWB, s);
+            const Frag x0 = XC::by_row(xr, i0 * 16 * XC::ROWB, s);
+            F::mma(sc[0], XC::by_row(yr, j[0] * 16 * XC::ROWB, s), x0);
+            if constexpr (R::UNITS > 1) {
+              const Frag x1 = XC::by_row(xr, i1 * 16 * XC::ROWB, s);
+              F::mma(sc[1], XC::by_row(yr, j[1] * 16 * XC::ROWB, s), x1);
+              F::mma(sc[2], XC::by_row(yr, j[2] * 16 * XC::ROWB, s), x1);
+            }
           }
 #pragma unroll
-          for (int t = 0; t < F::TP; ++t) sc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int s = 0; s < NS; ++s)
-#pragma unroll
-            for (int t = 0; t < F::TP; ++t) F::mma(sc[t], yf[s][t], xf[s]);
-#pragma unroll
-          for (int t = 0; t < F::TP; ++t) {
-            const int j0 = F::K * j + 16 * t + g4;
+          for (int u = 0; u < R::UNITS; ++u) {
+            if (u >= units) continue;
+            int it16, jt;
+            R::unit(wave, u, REV, it16, jt);
+            const int i = 16 * it16 + l16, j0 = 16 * jt + g4;
+            const float hi_ = sums[i], li_ = sums[64 + i];
             const floatx4 hj = load4(sums + j0), lj = load4(sums + 64 + j0);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               const bool on = REV ? j0 + r >= i && j0 + r < valid : j0 + r <= i;
               const float f = REV ? between(hj[r], lj[r], hi_, li_) : between(hi_, li_, hj[r], lj[r]);
-              sc[t][r] = rounded(on ? sc[t][r] * f : 0.f);
+              sc[u][r] = rounded(on ? sc[u][r] * f : 0.f);
+            }
+            char* q = pairs + R::slot(it16, jt / F::TP, REV) * F::PARTS * 1024;
+            if constexpr (F::PARTS == 2) {
+              const bf16x4 h = pack_bf16x4(sc[u]);
+              *reinterpret_cast<bf16x4*>(q + 8 * (jt % 2)) = h;
+              *reinterpret_cast<bf16x4*>(q + 8 * (jt % 2) + 1024) = rest_of(sc[u], h);
+            } else {
+              *reinterpret_cast<floatx4*>(q) = sc[u];
             }
           }
-          Frag hi, lo;
-          split(sc, hi, lo);
-          char* q = pairs + R::slot(mine, j, REV) * F::PARTS * 1024;
-          *reinterpret_cast<Frag*>(q) = hi;
-          if (F::PARTS == 2) *reinterpret_cast<Frag*>(q + 1024) = lo;
         }
       }
     }
@@ -411,8 +466,11 @@ template <typename T, int KW, bool OUT, bool REV, bool DOTS> __device__ __forcei
       for (int r = 0; r < 4; ++r)
         if (16 * i + g4 + r < ro.sk && n < ro.sn) st[i][r] = s[(int64_t)(16 * i + g4 + r) * step_k];
   }
-  const bool here = n0 + g4 < ro.vw;  // this lane's four columns of a result exist
-  T* op = OUT ? const_cast<T*>(head_of<T>(ro.out, p, k.h)) + n0 + g4 : nullptr;
+  const bool here = n0 + g4 < ro.vw, full = n0 + 16 <= ro.vw;  // this lane's four columns of a result exist; the wave's
+  T* op = OUT ? const_cast<T*>(head_of<T>(ro.out, p, k.h)) + n0 : nullptr;
+  unsigned row_off[NI];  // tokens are at most 16 MiB apart
+#pragma unroll
+  for (int t = 0; t < NI; ++t) row_off[t] = (unsigned)((16 * t + l16) * (int)(OUT ? ro.out.st : 0) + g4);
   const T* wp = DOTS ? head_of<T>(ro.w, p, k.h) + n0 + g4 : nullptr;
   const unsigned xa = lds0 + R::XB + R::ZB + XC::rows(lane), ya = lds0 + XC::cols(lane), za = (lds0 + R::XB + ZC::cols(lane)) ^ (sizeof(T) == 2 ? 32 * wave : 64 * wave);
   // the state is there before the loop begins: a wait for it inside would, from the second turn on, be one for the results' stores
@@ -503,12 +561,15 @@ template <typename T, int KW, bool OUT, bool REV, bool DOTS> __device__ __forcei
       for (int t = 0; t < TP; ++t) cf[j][t] = load4(f + 64 + F::K * j + 16 * t + g4);
     }
     __builtin_amdgcn_sched_barrier(0);
+    bool fine = true;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) fine = fine && all_finite(zf[j]);
+    const bool odd = __any(!fine);
     if constexpr (OUT) {
       // ---- what the state gives
 #pragma unroll
       for (int t = 0; t < NI; ++t) acc[t] = in[t] = floatx4{0.f, 0.f, 0.f, 0.f};
       split_state(0);
-      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
         if (s + 2 < NS) read_x(s + 2);
@@ -527,10 +588,7 @@ template <typename T, int KW, bool OUT, bool REV, bool DOTS> __device__ __forcei
     if constexpr (OUT) from_pairs();
     scaled(std::false_type{});
     if constexpr (OUT) interleave<T, 0, R::SLOTS * PARTS, 9>();
-    bool fine = true;
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) fine = fine && all_finite(zf[j]);
-    if (__any(!fine)) {
+    if (__builtin_expect(odd, 0)) {
       scaled(std::true_type{});
       if constexpr (OUT) {
         // A masked pair would be 0 times such a value: they are taken out of the product and added pair by pair
@@ -585,20 +643,44 @@ template <typename T, int KW, bool OUT, bool REV, bool DOTS> __device__ __forcei
       if (i + 4 < NT) read_y(i + 4);
     }
     if constexpr (OUT) {
+      float d[2 * NI];  // what w makes of them: by the state, by the pairs
+      T* ob = op + (int64_t)t0 * ro.out.st;
 #pragma unroll
       for (int t = 0; t < NI; ++t) {
         acc[t] *= rf[t];
-        in[t] *= a.scale;
         if constexpr (DOTS) {
-          float xd = 0.f, yd = 0.f;
+          d[t] = d[NI + t] = 0.f;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) xd += acc[t][r] * to_f32(wr[t][r]), yd += in[t][r] * to_f32(wr[t][r]);
-          xd = xor32_sum(xor16_sum(xd));
-          yd = xor32_sum(xor16_sum(yd));
-          float* q = reinterpret_cast<float*>(lds + R::DOTS) + (it & 1) * 8 * C + 2 * wave * C + 16 * t + l16;  // [it & 1][wave][inter, pairs][C]
-          if (g4 == 0) q[0] = xd, q[C] = yd;
+          for (int r = 0; r < 4; ++r) d[t] += acc[t][r] * to_f32(wr[t][r]), d[NI + t] += in[t][r] * to_f32(wr[t][r]);
         }
-        if (16 * t + l16 < valid && here) store4(op + (int64_t)(t0 + 16 * t + l16) * ro.out.st, acc[t] + in[t]);
+        acc[t] += in[t] * a.scale;
+      }
+      if (valid == C && full) {
+#pragma unroll
+        for (int t = 0; t < NI; ++t) store4(ob + row_off[t], acc[t]);
+      } else {
+#pragma unroll
+        for (int t = 0; t < NI; ++t)
+          if (16 * t + l16 < valid && here) store4(ob + row_off[t], acc[t]);
+      }
+      if constexpr (DOTS) {
+        // over the lanes of a token: an exchange of two sums leaves one, whose rows of 16 lanes are the first's and the second's in turn
+        float* q = reinterpret_cast<float*>(lds + R::DOTS) + (it & 1) * 8 * C + 2 * wave * C;  // [it & 1][wave][inter, pairs][C]
+        const int row = lane >> 4;
+        if constexpr (NI == 4) {
+          float e[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) e[i] = rows_join16(d[2 * i], d[2 * i + 1]);  // row r: of d[2 i + r % 2], half r / 2
+          const float s0 = rows_join32(e[0], e[1]), s1 = rows_join32(e[2], e[3]);  // row r: of d[2 (r / 2) + r % 2] and four further on
+          q[16 * row + l16] = s0;
+          q[C + 16 * row + l16] = s1 * a.scale;
+        } else {
+#pragma unroll
+          for (int t = 0; t < NI; ++t) {
+            const float s0 = xor32_sum(rows_join16(d[t], d[NI + t]));  // even rows: by the state, odd ones: by the pairs
+            if (row < 2) q[row * C + 16 * t + l16] = row ? s0 * a.scale : s0;
+          }
+        }
       }
     }
     lds_barrier();
