@@ -307,76 +307,96 @@ template <typename T, int KW, bool OUT, bool REV> __device__ __forceinline__ voi
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) - 4, l16 = lane & 15, g4 = 4 * (lane >> 4);
   const Spot& p = k.p;
   const unsigned lds0 = lds_byte_addr(lds);
-  const T* xp = OUT ? head_of<T>(ro.x, p, k.h) : nullptr;
-  const T* yp = head_of<T>(ro.y, p, k.h);
-  const T* zp = head_of<T>(ro.z, p, k.h) + k.col0;
-  const float* gp = a.g + p.b * a.gb + k.h * a.gh + p.tok * a.gt;
+  // Where the next chunk lies: what a lane fetches is at a fixed offset from these
+  const int64_t dir = REV ? -C : C;
+  const int first = chunk_at<REV>(k, 0) * C;
+  const T* xp = OUT ? head_of<T>(ro.x, p, k.h) + first * ro.x.st : nullptr;
+  const T* yp = head_of<T>(ro.y, p, k.h) + first * ro.y.st;
+  const T* zp = head_of<T>(ro.z, p, k.h) + k.col0 + first * ro.z.st;
+  const int64_t x_step = OUT ? dir * ro.x.st : 0, y_step = dir * ro.y.st, z_step = dir * ro.z.st, g_step = dir * a.gt;
+  const float* gp = a.g + p.b * a.gb + k.h * a.gh + (p.tok + first + min(lane, C - 1)) * a.gt;
   const Mover<T, KW, C> mx(OUT ? ro.x.st : 0, wave, lane), my(ro.y.st, wave, lane);
   const Mover<T, SLAB, C> mz(ro.z.st, wave, lane);
-  // A chunk's loads, ten of a wave at KW = 128: a CU takes 64 bytes a cycle, so they are handed out between the steps of the work; `part` of PARTS_OF
-  constexpr int NX = OUT ? decltype(mx)::N : 0, NY = decltype(my)::N, NZ = decltype(mz)::N, PARTS_OF = 4;
-  int next_t0 = 0, next_valid = 0;
-  unsigned next_tiles = 0;
-  const auto aim = [&](int it, int buf) {
-    next_t0 = chunk_at<REV>(k, it) * C;
-    next_valid = it < k.nchunk ? min(C, p.len - next_t0) : 0;
-    next_tiles = lds0 + buf * R::BUF;
-    if (next_valid > 0 && wave == 0) dma4(gp + (int64_t)(next_t0 + min(lane, next_valid - 1)) * a.gt, lds0 + R::RAW + 256 * buf);
-  };
-  const auto fetch = [&](int part) {
-    if (next_valid <= 0) return;
-    const T* yb = yp + (int64_t)next_t0 * ro.y.st;
-    const T* zb = zp + (int64_t)next_t0 * ro.z.st;
-    const T* xb = OUT ? xp + (int64_t)next_t0 * ro.x.st : nullptr;
-    if (next_valid == C && ro.kw >= KW && k.vw == SLAB) {
+  const bool wide = ro.kw >= KW && k.vw == SLAB;
+  int t_next = first;  // the next chunk's first token
+  // A chunk's loads, ten of a wave at KW = 128, all at once: a CU takes 64 bytes a cycle, for which these waves wait (of 40 KB 640 cycles), but
+  // handed out between the steps of their work the last ones came too late for the next chunk (forward at B8 H16 T4096 d128 157 us -> 178 - 210)
+  constexpr int NX = OUT ? decltype(mx)::N : 0, NY = decltype(my)::N, NZ = decltype(mz)::N;
+  const auto fetch = [&](int buf) {
+    const int valid = min(C, p.len - t_next);
+    const unsigned tiles = lds0 + buf * R::BUF;
+    if (valid == C && wide) {
 #pragma unroll
       for (int i = 0; i < NY + NX + NZ; ++i) {
-        if (i * PARTS_OF / (NY + NX + NZ) != part) continue;
-        if (i < NY) my.one(i, next_tiles, yb, wave);
-        else if (i < NY + NX) mx.one(OUT ? i - NY : 0, next_tiles + R::XB + R::ZB, xb, wave);
-        else mz.one(i - NY - NX, next_tiles + R::XB, zb, wave);
+        if (i < NY) my.one(i, tiles, yp, wave);
+        else if (i < NY + NX) mx.one(OUT ? i - NY : 0, tiles + R::XB + R::ZB, xp, wave);
+        else mz.one(i - NY - NX, tiles + R::XB, zp, wave);
       }
-    } else if (part == 0) {
-      my.edge(next_tiles, yb, ro.y.st, next_valid, ro.kw, wave, lane);
-      if constexpr (OUT) mx.edge(next_tiles + R::XB + R::ZB, xb, ro.x.st, next_valid, ro.kw, wave, lane);
-      mz.edge(next_tiles + R::XB, zb, ro.z.st, next_valid, k.vw, wave, lane);
+      if (wave == 0) dma4(gp, lds0 + R::RAW + 256 * buf);
+    } else {
+      my.edge(tiles, yp, ro.y.st, valid, ro.kw, wave, lane);
+      if constexpr (OUT) mx.edge(tiles + R::XB + R::ZB, xp, ro.x.st, valid, ro.kw, wave, lane);
+      mz.edge(tiles + R::XB, zp, ro.z.st, valid, k.vw, wave, lane);
+      if (wave == 0) dma4(gp - max(0, min(lane, C - 1) - (valid - 1)) * a.gt, lds0 + R::RAW + 256 * buf);
     }
+    yp += y_step, xp += x_step, zp += z_step, gp += g_step, t_next += (int)dir;
   };
+  // the dots of the chunk before the one that is walked: thread = (kind, token)
   const float* red = reinterpret_cast<const float*>(lds + R::DOTS);
   const bool dots = OUT && ro.dots;
+  const int dot_i = (threadIdx.x - 256) % C, dot_kind = (threadIdx.x - 256) / C;
+  int dot_t = first + dot_i;
+  float* dot_p = dots && dot_kind < 2 ? ro.dots + (int64_t)(dot_kind * ro.slabs + k.item) * a.dots_step + (int64_t)(p.b * a.H + k.h) * a.T + p.tok + dot_t : nullptr;
   const auto leave_dots = [&](int it) {
-    const int t0 = chunk_at<REV>(k, it) * C, tid = threadIdx.x - 256, i = tid % C, kind = tid / C;
-    if (kind < 2 && t0 + i < p.len) {
-      const float* q = red + (it & 1) * 8 * C + kind * C + i;
-      ro.dots[(int64_t)(kind * ro.slabs + k.item) * a.dots_step + (int64_t)(p.b * a.H + k.h) * a.T + p.tok + t0 + i] = (q[0] + q[2 * C]) + (q[4 * C] + q[6 * C]);
+    if (dot_p && dot_t < p.len) {
+      const float* q = red + (it & 1) * 8 * C + dot_kind * C + dot_i;
+      *dot_p = (q[0] + q[2 * C]) + (q[4 * C] + q[6 * C]);
     }
+    dot_p += dot_p ? dir : 0;
+    dot_t += (int)dir;
   };
   float* sums = reinterpret_cast<float*>(lds + R::SUMS) + 128 * wave;  // of this wave: multiples, rests
   const float* raw = reinterpret_cast<const float*>(lds + R::RAW);
   float whole_h = 0.f, whole_l = 0.f;
   if constexpr (OUT)
     for (int i = (threadIdx.x - 256) * 16; i < 2 * R::PAIRB; i += 256 * 16) *reinterpret_cast<floatx4*>(lds + R::PAIRS + i) = floatx4{0.f, 0.f, 0.f, 0.f};
-  aim(0, 0);
-#pragma unroll
-  for (int i = 0; i < PARTS_OF; ++i) fetch(i);
+  if (k.nchunk > 0) fetch(0);
   dma_wait<0>();
   lds_barrier();
-  for (int it = 0, buf = 0; it <= k.nchunk; ++it) {
-    const int next = buf == 2 ? 0 : buf + 1;
-    aim(it + 1, next);
+  // this wave's tiles of pairs: they are of one row tile, but the first of wave 0, whose third does not exist (a product more for it)
+  const int units = R::units(wave);
+  int ui[3], uj[3];
 #pragma unroll
-    for (int i = 0; i < PARTS_OF; ++i) fetch(i);
-    if (dots && it >= 2) leave_dots(it - 2);
-    if (it < k.nchunk) {
-      const int t0 = chunk_at<REV>(k, it) * C, valid = min(C, p.len - t0);
+  for (int u = 0; u < 3; ++u) R::unit(wave, u < units ? u : 0, REV, ui[u], uj[u]);
+  if (units == 2) ui[2] = ui[1];
+  for (int it = 0, buf = 0, t0 = first; it <= k.nchunk; ++it) {
+    const int next = buf == 2 ? 0 : buf + 1;
+    const bool on = it < k.nchunk;
+    // the next chunk on its way, then the operands of this one's pairs
+    if (it + 1 < k.nchunk) fetch(next);
+    Frag x[2][NS], y[R::UNITS][NS];
+    if (OUT && on && units > 0) {
       const unsigned xr = lds0 + buf * R::BUF + R::XB + R::ZB + XC::rows(lane), yr = lds0 + buf * R::BUF + XC::rows(lane);
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        x[0][s] = XC::by_row(xr, ui[0] * 16 * XC::ROWB, s);
+        y[0][s] = XC::by_row(yr, uj[0] * 16 * XC::ROWB, s);
+        if constexpr (R::UNITS > 1) {
+          x[1][s] = XC::by_row(xr, ui[1] * 16 * XC::ROWB, s);
+          y[1][s] = XC::by_row(yr, uj[1] * 16 * XC::ROWB, s);
+          y[2][s] = XC::by_row(yr, uj[2] * 16 * XC::ROWB, s);
+        }
+      }
+    }
+    const int valid = min(C, p.len - t0);
+    if (on) {
       // ---- the chunk's decays: lane = token
       float gv = lane < valid ? raw[64 * buf + lane] * LOG2E : 0.f;
       gv = gv < -200.f ? -200.f : gv;  // e^-138 is nothing
       const float gm = rounded(rintf(gv * 64.f) * (1.f / 64.f)), H = running_sum(gm), L = running_sum(gv - gm), HT = lane_value(H, 63), LT = lane_value(L, 63);
       sums[lane] = H;
       sums[64 + lane] = L;
-      if (wave == 0) {
+      if (wave == 3) {
         const float head = between(H, L, 0.f, 0.f), tail = between(HT, LT, H, L);
         float* f = reinterpret_cast<float*>(lds + R::FACTORS) + 256 * (it & 1);
         f[lane] = (REV ? tail : head) * ro.row_scale;
@@ -384,51 +404,40 @@ template <typename T, int KW, bool OUT, bool REV> __device__ __forceinline__ voi
         f[128 + lane] = between(HT, LT, 0.f, 0.f);
         if (!OUT) whole_h += HT, whole_l += LT;
       }
-      if constexpr (OUT) {
+    }
+    if (dots && it >= 2) leave_dots(it - 2);
+    if constexpr (OUT) {
+      if (on && units > 0) {
         // ---- pairs: rows of a result are j, its column is i
         char* pairs = lds + R::PAIRS + (it & 1) * R::PAIRB + 16 * lane;
-        const int units = R::units(wave);
         floatx4 sc[R::UNITS];
 #pragma unroll
         for (int u = 0; u < R::UNITS; ++u) sc[u] = floatx4{0.f, 0.f, 0.f, 0.f};
-        if (units > 0) {
-          // a wave's tiles are of one row tile, but the first of wave 0, whose third does not exist
-          int i0, i1, j[3];
-          R::unit(wave, 0, REV, i0, j[0]);
-          R::unit(wave, units > 2 ? 2 : 0, REV, i1, j[2]);  // (a product more where there are two)
-          R::unit(wave, units > 1 ? 1 : 0, REV, i1, j[1]);
 #pragma unroll
-          for (int s = 0; s < NS; ++s) {
-            const Frag x0 = XC::by_row(xr, i0 * 16 * XC::ROWB, s);
-            F::mma(sc[0], XC::by_row(yr, j[0] * 16 * XC::ROWB, s), x0);
-            if constexpr (R::UNITS > 1) {
-              const Frag x1 = XC::by_row(xr, i1 * 16 * XC::ROWB, s);
-              F::mma(sc[1], XC::by_row(yr, j[1] * 16 * XC::ROWB, s), x1);
-              F::mma(sc[2], XC::by_row(yr, j[2] * 16 * XC::ROWB, s), x1);
-            }
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+          for (int u = 0; u < R::UNITS; ++u) F::mma(sc[u], y[u][s], x[u > 0][s]);
+#pragma unroll
+        for (int u = 0; u < R::UNITS; ++u) {
+          if (u >= units) continue;
+          const int i = 16 * ui[u] + l16, j0 = 16 * uj[u] + g4;
+          const float hi_ = sums[i], li_ = sums[64 + i];
+          const floatx4 hj = load4(sums + j0), lj = load4(sums + 64 + j0);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sc[u][r] *= REV ? between(hj[r], lj[r], hi_, li_) : between(hi_, li_, hj[r], lj[r]);
+          if (ui[u] == uj[u] || valid < C) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sc[u][r] = (REV ? j0 + r >= i && j0 + r < valid : j0 + r <= i) ? sc[u][r] : 0.f;
           }
 #pragma unroll
-          for (int u = 0; u < R::UNITS; ++u) {
-            if (u >= units) continue;
-            int it16, jt;
-            R::unit(wave, u, REV, it16, jt);
-            const int i = 16 * it16 + l16, j0 = 16 * jt + g4;
-            const float hi_ = sums[i], li_ = sums[64 + i];
-            const floatx4 hj = load4(sums + j0), lj = load4(sums + 64 + j0);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const bool on = REV ? j0 + r >= i && j0 + r < valid : j0 + r <= i;
-              const float f = REV ? between(hj[r], lj[r], hi_, li_) : between(hi_, li_, hj[r], lj[r]);
-              sc[u][r] = rounded(on ? sc[u][r] * f : 0.f);
-            }
-            char* q = pairs + R::slot(it16, jt / F::TP, REV) * F::PARTS * 1024;
-            if constexpr (F::PARTS == 2) {
-              const bf16x4 h = pack_bf16x4(sc[u]);
-              *reinterpret_cast<bf16x4*>(q + 8 * (jt % 2)) = h;
-              *reinterpret_cast<bf16x4*>(q + 8 * (jt % 2) + 1024) = rest_of(sc[u], h);
-            } else {
-              *reinterpret_cast<floatx4*>(q) = sc[u];
-            }
+          for (int r = 0; r < 4; ++r) sc[u][r] = rounded(sc[u][r]);
+          char* q = pairs + R::slot(ui[u], uj[u] / F::TP, REV) * F::PARTS * 1024;
+          if constexpr (F::PARTS == 2) {
+            const bf16x4 h = pack_bf16x4(sc[u]);
+            *reinterpret_cast<bf16x4*>(q + 8 * (uj[u] % 2)) = h;
+            *reinterpret_cast<bf16x4*>(q + 8 * (uj[u] % 2) + 1024) = rest_of(sc[u], h);
+          } else {
+            *reinterpret_cast<floatx4*>(q) = sc[u];
           }
         }
       }
@@ -436,9 +445,10 @@ template <typename T, int KW, bool OUT, bool REV> __device__ __forceinline__ voi
     dma_wait<0>();
     lds_barrier();
     buf = next;
+    t0 += (int)dir;
   }
   if (dots && k.nchunk > 0) leave_dots(k.nchunk - 1);
-  if (!OUT && k.item == 0 && threadIdx.x == 256) a.whole[(int64_t)k.slot * a.H + k.h] = between(whole_h, whole_l, 0.f, 0.f);
+  if (!OUT && k.item == 0 && threadIdx.x == 448) a.whole[(int64_t)k.slot * a.H + k.h] = between(whole_h, whole_l, 0.f, 0.f);
 }
 
 // The other four: 16 columns of the state and of the results each.
@@ -471,24 +481,39 @@ template <typename T, int KW, bool OUT, bool REV, bool DOTS> __device__ __forcei
   unsigned row_off[NI];  // tokens are at most 16 MiB apart
 #pragma unroll
   for (int t = 0; t < NI; ++t) row_off[t] = (unsigned)((16 * t + l16) * (int)(OUT ? ro.out.st : 0) + g4);
-  const T* wp = DOTS ? head_of<T>(ro.w, p, k.h) + n0 + g4 : nullptr;
+  const T* wp = DOTS ? head_of<T>(ro.w, p, k.h) + n0 : nullptr;
+  unsigned w_off[NI];
+#pragma unroll
+  for (int t = 0; t < NI; ++t) w_off[t] = (unsigned)((16 * t + l16) * (int)(DOTS ? ro.w.st : 0) + g4);
   const unsigned xa = lds0 + R::XB + R::ZB + XC::rows(lane), ya = lds0 + XC::cols(lane), za = (lds0 + R::XB + ZC::cols(lane)) ^ (sizeof(T) == 2 ? 32 * wave : 64 * wave);
   // the state is there before the loop begins: a wait for it inside would, from the second turn on, be one for the results' stores
 #pragma unroll
   for (int i = 0; i < NT; ++i) asm volatile("" : "+v"(st[i]));
   lds_barrier();  // the first chunk's tiles
   lds_barrier();  // its pairs
-  for (int it = 0, at = 0; it < k.nchunk; ++it) {
-    const int t0 = chunk_at<REV>(k, it) * C, valid = min(C, p.len - t0);
-    typename Vec4<T>::V wr[NI];  // as they lie in memory: converted only where they are used, behind the products
-    if constexpr (DOTS) {
+  const int dir = REV ? -C : C;
+  int t0 = chunk_at<REV>(k, 0) * C;
+  T* ob = op + t0 * (OUT ? ro.out.st : 0);
+  const T* wb = wp + t0 * (DOTS ? ro.w.st : 0);
+  const int64_t out_step = dir * (OUT ? ro.out.st : 0), w_step = dir * (DOTS ? ro.w.st : 0);
+  typename Vec4<T>::V wr[NI];  // a chunk's partners, fetched when those of the chunk before have been used
+  const auto partners = [&](int t0) {
+    const bool whole = t0 + C <= p.len && full;
 #pragma unroll
-      for (int t = 0; t < NI; ++t) {
+    for (int t = 0; t < NI; ++t) {
+      if (whole) {
+        wr[t] = *reinterpret_cast<const typename Vec4<T>::V*>(wb + w_off[t]);
+      } else {
 #pragma unroll
         for (int r = 0; r < 4; ++r) wr[t][r] = (T)0.f;
-        if (16 * t + l16 < valid && here) wr[t] = *reinterpret_cast<const typename Vec4<T>::V*>(wp + (int64_t)(t0 + 16 * t + l16) * ro.w.st);
+        if (t0 + 16 * t + l16 < p.len && here) wr[t] = *reinterpret_cast<const typename Vec4<T>::V*>(wb + w_off[t]);
       }
     }
+    wb += w_step;
+  };
+  if (DOTS && k.nchunk > 0) partners(t0);
+  for (int it = 0, at = 0; it < k.nchunk; ++it) {
+    const int valid = min(C, p.len - t0);
     const float* f = reinterpret_cast<const float*>(lds + R::FACTORS) + 256 * (it & 1);
     const unsigned xr = xa + at, yc = ya + at, zc = za + at;
     const char* pairs = lds + R::PAIRS + (it & 1) * R::PAIRB + 16 * lane;
@@ -644,7 +669,6 @@ template <typename T, int KW, bool OUT, bool REV, bool DOTS> __device__ __forcei
     }
     if constexpr (OUT) {
       float d[2 * NI];  // what w makes of them: by the state, by the pairs
-      T* ob = op + (int64_t)t0 * ro.out.st;
 #pragma unroll
       for (int t = 0; t < NI; ++t) {
         acc[t] *= rf[t];
@@ -683,6 +707,9 @@ template <typename T, int KW, bool OUT, bool REV, bool DOTS> __device__ __forcei
         }
       }
     }
+    ob += out_step;
+    t0 += dir;
+    if (DOTS && it + 1 < k.nchunk) partners(t0);
     lds_barrier();
     at = at == 2 * R::BUF ? 0 : at + R::BUF;
   }
