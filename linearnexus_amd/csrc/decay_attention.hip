@@ -261,7 +261,8 @@ template <typename T, int KW, bool OUT> struct Room {
   static constexpr int C = chunk_of<T, KW>(), NI = C / 16, NJ = C / Form<T>::K;
   static constexpr int SLOTS = NI == 4 && NJ == 2 ? 6 : NI * NJ;  // of 16 x K blocks of pairs; of the wide ones two are always empty
   static constexpr int XB = C * KW * sizeof(T), ZB = C * SLAB * sizeof(T), BUF = (OUT ? 2 : 1) * XB + ZB, PAIRB = OUT ? SLOTS * Form<T>::PARTS * 1024 : 0;
-  static constexpr int PAIRS = 3 * BUF, FACTORS = PAIRS + 2 * PAIRB, SUMS = FACTORS + 2 * 1024, RAW = SUMS + 4 * 512, DOTS = RAW + 3 * 256;
+  static constexpr int RING = 3, AHEAD = RING - 2;  // chunks in LDS; how far ahead of the pairs' chunk they are fetched
+  static constexpr int PAIRS = RING * BUF, FACTORS = PAIRS + 2 * PAIRB, SUMS = FACTORS + 2 * 1024, RAW = SUMS + 4 * 512, DOTS = RAW + RING * 256;
   static constexpr int BYTES = DOTS + (OUT ? 2 * 4 * 2 * C * 4 : 0);
   static __device__ __forceinline__ int slot(int i, int j, bool rev) { return SLOTS != 6 ? i * NJ + j : rev ? (i < 2 ? 2 * i + j : i + 2) : (i < 2 ? i : 2 * i - 2 + j); }
   // whether row tile i has pairs with block j
@@ -355,36 +356,47 @@ template <typename T, int KW, bool OUT, bool REV> __device__ __forceinline__ voi
     dot_p += dot_p ? dir : 0;
     dot_t += (int)dir;
   };
+  __builtin_amdgcn_s_setprio(1);  // they have the longer way to the barrier: forward at B8 H16 T4096 d128 166 us -> 154
   float* sums = reinterpret_cast<float*>(lds + R::SUMS) + 128 * wave;  // of this wave: multiples, rests
   const float* raw = reinterpret_cast<const float*>(lds + R::RAW);
   float whole_h = 0.f, whole_l = 0.f;
   if constexpr (OUT)
     for (int i = (threadIdx.x - 256) * 16; i < 2 * R::PAIRB; i += 256 * 16) *reinterpret_cast<floatx4*>(lds + R::PAIRS + i) = floatx4{0.f, 0.f, 0.f, 0.f};
-  if (k.nchunk > 0) fetch(0);
-  dma_wait<0>();
+  // until chunk `it` is there: all but the loads of those behind it, which are whole ones if they are to be counted
+  const auto arrived = [&](int it) {
+    constexpr int N = (R::AHEAD - 1) * (NY + NX + NZ);
+    if (R::AHEAD > 1 && wide && it + R::AHEAD < k.nchunk) {
+      if (wave == 0) dma_wait<N + R::AHEAD - 1>();
+      else dma_wait<N>();
+    } else {
+      dma_wait<0>();
+    }
+  };
+  for (int i = 0; i < R::AHEAD && i < k.nchunk; ++i) fetch(i);
+  arrived(0);
   lds_barrier();
-  // this wave's tiles of pairs: they are of one row tile, but the first of wave 0, whose third does not exist (a product more for it)
+  // this wave's tiles of pairs: they are of one row tile, but the second of wave 0
   const int units = R::units(wave);
   int ui[3], uj[3];
 #pragma unroll
   for (int u = 0; u < 3; ++u) R::unit(wave, u < units ? u : 0, REV, ui[u], uj[u]);
-  if (units == 2) ui[2] = ui[1];
   for (int it = 0, buf = 0, t0 = first; it <= k.nchunk; ++it) {
-    const int next = buf == 2 ? 0 : buf + 1;
+    const int next = buf == R::RING - 1 ? 0 : buf + 1;
     const bool on = it < k.nchunk;
     // the next chunk on its way, then the operands of this one's pairs
-    if (it + 1 < k.nchunk) fetch(next);
-    Frag x[2][NS], y[R::UNITS][NS];
+    if (it + R::AHEAD < k.nchunk) fetch(buf + R::AHEAD < R::RING ? buf + R::AHEAD : buf + R::AHEAD - R::RING);
+    Frag x[NS], x3[R::UNITS > 1 ? NS : 1], y[R::UNITS][NS];
     if (OUT && on && units > 0) {
       const unsigned xr = lds0 + buf * R::BUF + R::XB + R::ZB + XC::rows(lane), yr = lds0 + buf * R::BUF + XC::rows(lane);
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
-        x[0][s] = XC::by_row(xr, ui[0] * 16 * XC::ROWB, s);
-        y[0][s] = XC::by_row(yr, uj[0] * 16 * XC::ROWB, s);
+        x[s] = XC::by_row(xr, ui[0] * 16 * XC::ROWB, s);
+#pragma unroll
+        for (int u = 0; u < R::UNITS; ++u)
+          if (u < 2) y[u][s] = XC::by_row(yr, uj[u] * 16 * XC::ROWB, s);
         if constexpr (R::UNITS > 1) {
-          x[1][s] = XC::by_row(xr, ui[1] * 16 * XC::ROWB, s);
-          y[1][s] = XC::by_row(yr, uj[1] * 16 * XC::ROWB, s);
-          y[2][s] = XC::by_row(yr, uj[2] * 16 * XC::ROWB, s);
+          if (wave == 0) x3[s] = XC::by_row(xr, ui[1] * 16 * XC::ROWB, s);
+          else if (units > 2) y[R::UNITS - 1][s] = XC::by_row(yr, uj[2] * 16 * XC::ROWB, s);
         }
       }
     }
@@ -414,9 +426,17 @@ template <typename T, int KW, bool OUT, bool REV> __device__ __forceinline__ voi
 #pragma unroll
         for (int u = 0; u < R::UNITS; ++u) sc[u] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int s = 0; s < NS; ++s)
-#pragma unroll
-          for (int u = 0; u < R::UNITS; ++u) F::mma(sc[u], y[u][s], x[u > 0][s]);
+        for (int s = 0; s < NS; ++s) {
+          F::mma(sc[0], y[0][s], x[s]);
+          if constexpr (R::UNITS > 1) {
+            if (wave == 0) {
+              F::mma(sc[1], y[1][s], x3[s]);
+            } else {
+              F::mma(sc[1], y[1][s], x[s]);
+              if (units > 2) F::mma(sc[2], y[2][s], x[s]);
+            }
+          }
+        }
 #pragma unroll
         for (int u = 0; u < R::UNITS; ++u) {
           if (u >= units) continue;
@@ -442,7 +462,7 @@ template <typename T, int KW, bool OUT, bool REV> __device__ __forceinline__ voi
         }
       }
     }
-    dma_wait<0>();
+    arrived(it + 1);
     lds_barrier();
     buf = next;
     t0 += (int)dir;
@@ -481,10 +501,8 @@ template <typename T, int KW, bool OUT, bool REV, bool DOTS> __device__ __forcei
   unsigned row_off[NI];  // tokens are at most 16 MiB apart
 #pragma unroll
   for (int t = 0; t < NI; ++t) row_off[t] = (unsigned)((16 * t + l16) * (int)(OUT ? ro.out.st : 0) + g4);
-  const T* wp = DOTS ? head_of<T>(ro.w, p, k.h) + n0 : nullptr;
-  unsigned w_off[NI];
-#pragma unroll
-  for (int t = 0; t < NI; ++t) w_off[t] = (unsigned)((16 * t + l16) * (int)(DOTS ? ro.w.st : 0) + g4);
+  const T* wp = DOTS ? head_of<T>(ro.w, p, k.h) : nullptr;
+  const int w_col = min(n0 + g4, ro.vw - 4);
   const unsigned xa = lds0 + R::XB + R::ZB + XC::rows(lane), ya = lds0 + XC::cols(lane), za = (lds0 + R::XB + ZC::cols(lane)) ^ (sizeof(T) == 2 ? 32 * wave : 64 * wave);
   // the state is there before the loop begins: a wait for it inside would, from the second turn on, be one for the results' stores
 #pragma unroll
@@ -497,18 +515,10 @@ template <typename T, int KW, bool OUT, bool REV, bool DOTS> __device__ __forcei
   const T* wb = wp + t0 * (DOTS ? ro.w.st : 0);
   const int64_t out_step = dir * (OUT ? ro.out.st : 0), w_step = dir * (DOTS ? ro.w.st : 0);
   typename Vec4<T>::V wr[NI];  // a chunk's partners, fetched when those of the chunk before have been used
-  const auto partners = [&](int t0) {
-    const bool whole = t0 + C <= p.len && full;
+  const auto partners = [&](int t0) {  // of tokens and columns that do not exist the last ones': what they give is dropped, or 0
+    const int last = min(C, p.len - t0) - 1;
 #pragma unroll
-    for (int t = 0; t < NI; ++t) {
-      if (whole) {
-        wr[t] = *reinterpret_cast<const typename Vec4<T>::V*>(wb + w_off[t]);
-      } else {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) wr[t][r] = (T)0.f;
-        if (t0 + 16 * t + l16 < p.len && here) wr[t] = *reinterpret_cast<const typename Vec4<T>::V*>(wb + w_off[t]);
-      }
-    }
+    for (int t = 0; t < NI; ++t) wr[t] = *reinterpret_cast<const typename Vec4<T>::V*>(wb + min(16 * t + l16, last) * (int)(DOTS ? ro.w.st : 0) + w_col);
     wb += w_step;
   };
   if (DOTS && k.nchunk > 0) partners(t0);
@@ -679,6 +689,10 @@ template <typename T, int KW, bool OUT, bool REV, bool DOTS> __device__ __forcei
         }
         acc[t] += in[t] * a.scale;
       }
+      // (the partners are used up before the stores go out: a wait for them behind would be one for the stores)
+      if constexpr (DOTS)
+#pragma unroll
+        for (int t = 0; t < 2 * NI; ++t) asm volatile("" : "+v"(d[t]));
       if (valid == C && full) {
 #pragma unroll
         for (int t = 0; t < NI; ++t) store4(ob + row_off[t], acc[t]);
@@ -711,7 +725,7 @@ template <typename T, int KW, bool OUT, bool REV, bool DOTS> __device__ __forcei
     t0 += dir;
     if (DOTS && it + 1 < k.nchunk) partners(t0);
     lds_barrier();
-    at = at == 2 * R::BUF ? 0 : at + R::BUF;
+    at = at == (R::RING - 1) * R::BUF ? 0 : at + R::BUF;
   }
   if (ro.fin && (!OUT || (REV ? p.first : p.last))) {
     float* s = ro.fin + ((int64_t)(OUT ? p.row : k.slot) * a.H + k.h) * state_size + (int64_t)n * step_n;
@@ -966,12 +980,13 @@ int64_t ceil_div(int64_t x, int64_t y) { return (x + y - 1) / y; }
 constexpr int MAX_D = 256, SHORTEST = 512;
 
 // Tokens of a segment, a multiple of 64, or 0: rows are walked whole.  Segments read keys and values (queries and gradients) once more, so they
-// are for rows and heads that leave most CUs without a workgroup: as many as give every CU one, of 512 tokens and more.  The rows of a packed
-// batch are taken for one: their lengths are not known here, and sequences of one segment are walked once whatever its size.
+// are for rows and heads that leave most CUs without a workgroup: as many as give every CU two (of which a CU takes two at a time on the local
+// walks, one on the others), of 512 tokens and more.  The rows of a packed batch are taken for one: their lengths are not known here, and sequences
+// of one segment are walked once whatever its size.
 int segment(const lnx_decay_args* a) {
   const int64_t walks = (a->nseq ? 1 : (int64_t)a->B) * a->H * ceil_div(a->dv, SLAB);
   if (walks > 128) return 0;
-  int64_t s = up((int)ceil_div(a->T, 256 / walks), 64);
+  int64_t s = up((int)ceil_div(a->T, 512 / walks), 64);
   if (s < SHORTEST) s = SHORTEST;
   return s >= a->T ? 0 : (int)s;
 }
