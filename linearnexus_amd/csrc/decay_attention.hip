@@ -51,19 +51,21 @@ __device__ __forceinline__ bool is_finite(float x) { return (__float_as_uint(x) 
 // Result tiles as an operand, and what its rounding left.  Of an infinite value that is not a number: as an integer it lies above 2^100, where rests
 // are cut (two at a time), so that it adds nothing to a sum that the infinite value is in.
 __device__ __forceinline__ bf16x4 rest_of(floatx4 v, bf16x4 h) {
-  typedef unsigned uint2_ __attribute__((ext_vector_type(2)));
-  uint2_ u = __builtin_bit_cast(uint2_, h);
-  asm("" : "+v"(u[0]), "+v"(u[1]));  // (not the value itself: -ffast-math takes a conversion and its inverse for nothing)
-  h = __builtin_bit_cast(bf16x4, u);
-  const floatx4 d = {v[0] - (float)h[0], v[1] - (float)h[1], v[2] - (float)h[2], v[3] - (float)h[3]};
-  u = __builtin_bit_cast(uint2_, pack_bf16x4(d));
   typedef short short4_ __attribute__((ext_vector_type(4)));
-  return __builtin_bit_cast(bf16x4, __builtin_elementwise_min(__builtin_bit_cast(short4_, u), short4_{0x7180, 0x7180, 0x7180, 0x7180}));
+  const floatx4 d = {v[0] - (float)h[0], v[1] - (float)h[1], v[2] - (float)h[2], v[3] - (float)h[3]};
+  return __builtin_bit_cast(bf16x4, __builtin_elementwise_min(__builtin_bit_cast(short4_, pack_bf16x4(d)), short4_{0x7180, 0x7180, 0x7180, 0x7180}));
+}
+// Rounded to bf16, and opaque: -ffast-math takes a conversion and its inverse for nothing, and the rest with them
+__device__ __forceinline__ bf16x4 to_bf16(floatx4 v) {
+  typedef unsigned uint2_ __attribute__((ext_vector_type(2)));
+  uint2_ u = __builtin_bit_cast(uint2_, pack_bf16x4(v));
+  asm("" : "+v"(u));
+  return __builtin_bit_cast(bf16x4, u);
 }
 __device__ __forceinline__ void split(const floatx4 (&v)[2], bf16x8& hi, bf16x8& lo) {
-  const bf16x4 h[2] = {pack_bf16x4(v[0]), pack_bf16x4(v[1])};
-  hi = Mma16::join(h[0], h[1]);
-  lo = Mma16::join(rest_of(v[0], h[0]), rest_of(v[1], h[1]));
+  const bf16x4 h0 = to_bf16(v[0]), h1 = to_bf16(v[1]);
+  hi = Mma16::join(h0, h1);
+  lo = Mma16::join(rest_of(v[0], h0), rest_of(v[1], h1));
 }
 __device__ __forceinline__ void split(const floatx4 (&v)[1], floatx4& hi, floatx4&) { hi = v[0]; }
 
@@ -261,19 +263,21 @@ template <typename T, int KW, bool OUT> struct Room {
   static constexpr int C = chunk_of<T, KW>(), NI = C / 16, NJ = C / Form<T>::K;
   static constexpr int SLOTS = NI == 4 && NJ == 2 ? 6 : NI * NJ;  // of 16 x K blocks of pairs; of the wide ones two are always empty
   static constexpr int XB = C * KW * sizeof(T), ZB = C * SLAB * sizeof(T), BUF = (OUT ? 2 : 1) * XB + ZB, PAIRB = OUT ? SLOTS * Form<T>::PARTS * 1024 : 0;
-  static constexpr int RING = 3, AHEAD = RING - 2;  // chunks in LDS; how far ahead of the pairs' chunk they are fetched
+  static constexpr int RING = OUT ? 3 : 6, AHEAD = RING - 2;  // chunks in LDS; how far ahead of the pairs' chunk they are fetched
   static constexpr int PAIRS = RING * BUF, FACTORS = PAIRS + 2 * PAIRB, SUMS = FACTORS + 2 * 1024, RAW = SUMS + 4 * 512, DOTS = RAW + RING * 256;
   static constexpr int BYTES = DOTS + (OUT ? 2 * 4 * 2 * C * 4 : 0);
-  static __device__ __forceinline__ int slot(int i, int j, bool rev) { return SLOTS != 6 ? i * NJ + j : rev ? (i < 2 ? 2 * i + j : i + 2) : (i < 2 ? i : 2 * i - 2 + j); }
+  static constexpr int slot(int i, int j, bool rev) { return SLOTS != 6 ? i * NJ + j : rev ? (i < 2 ? 2 * i + j : i + 2) : (i < 2 ? i : 2 * i - 2 + j); }
   // whether row tile i has pairs with block j
-  static __device__ __forceinline__ bool needed(int i, int j, bool rev) { return rev ? Form<T>::K * (j + 1) > 16 * i : Form<T>::K * j <= 16 * i + 15; }
+  static constexpr bool needed(int i, int j, bool rev) { return rev ? Form<T>::K * (j + 1) > 16 * i : Form<T>::K * j <= 16 * i + 15; }
   // The 16 x 16 tiles of pairs, ten of a chunk of 64, in four nearly equal shares: tile u of wave w; those above the diagonal hold zeros
-  static constexpr int UNITS = NI == 4 ? 3 : 1;
-  static __device__ __forceinline__ int units(int w) { return NI == 4 ? (w < 2 ? 2 : 3) : w < NI * (NI + 1) / 2; }
-  static __device__ __forceinline__ void unit(int w, int u, bool rev, int& i, int& j) {
-    if (NI == 4) i = w == 0 ? 3 * u : w, j = w == 0 ? 0 : w == 3 ? u + 1 : u;
-    else i = w > 0, j = w == 2;
-    if (rev) i = NI - 1 - i, j = NI - 1 - j;
+  static constexpr int units(int w) { return NI == 4 ? (w < 2 ? 2 : 3) : w < NI * (NI + 1) / 2; }
+  static constexpr int unit_row(int w, int u, bool rev) {
+    const int i = NI == 4 ? (w == 0 ? 3 * u : w) : w > 0;
+    return rev ? NI - 1 - i : i;
+  }
+  static constexpr int unit_col(int w, int u, bool rev) {
+    const int j = NI == 4 ? (w == 0 ? 0 : w == 3 ? u + 1 : u) : w == 2;
+    return rev ? NI - 1 - j : j;
   }
 };
 
@@ -299,13 +303,14 @@ template <typename T, int READS, int MFMAS, int VALUS> __device__ __forceinline_
 
 // Four of a walk's eight waves: they bring chunk c + 1 to LDS and form the decays and the pairs of chunk c, one tile of 16 rows each, while
 // the others walk chunk c - 1.  One barrier a chunk.
-template <typename T, int KW, bool OUT, bool REV> __device__ __forceinline__ void walk_pairs(const Walk& a, const Role& ro, const Task& k, char* lds) {
+template <typename T, int KW, bool OUT, bool REV, int W> __device__ __forceinline__ void walk_pairs(const Walk& a, const Role& ro, const Task& k, char* lds) {
   typedef Form<T> F;
   typedef typename F::Frag Frag;
   typedef Cells<T, KW> XC;
   typedef Room<T, KW, OUT> R;
   constexpr int C = R::C, NS = KW / F::K;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) - 4, l16 = lane & 15, g4 = 4 * (lane >> 4);
+  constexpr int wave = W, UNITS = R::units(W);
+  const int lane = threadIdx.x & 63, l16 = lane & 15, g4 = 4 * (lane >> 4);
   const Spot& p = k.p;
   const unsigned lds0 = lds_byte_addr(lds);
   // Where the next chunk lies: what a lane fetches is at a fixed offset from these
@@ -375,28 +380,21 @@ template <typename T, int KW, bool OUT, bool REV> __device__ __forceinline__ voi
   for (int i = 0; i < R::AHEAD && i < k.nchunk; ++i) fetch(i);
   arrived(0);
   lds_barrier();
-  // this wave's tiles of pairs: they are of one row tile, but the second of wave 0
-  const int units = R::units(wave);
-  int ui[3], uj[3];
-#pragma unroll
-  for (int u = 0; u < 3; ++u) R::unit(wave, u < units ? u : 0, REV, ui[u], uj[u]);
   for (int it = 0, buf = 0, t0 = first; it <= k.nchunk; ++it) {
     const int next = buf == R::RING - 1 ? 0 : buf + 1;
     const bool on = it < k.nchunk;
     // the next chunk on its way, then the operands of this one's pairs
     if (it + R::AHEAD < k.nchunk) fetch(buf + R::AHEAD < R::RING ? buf + R::AHEAD : buf + R::AHEAD - R::RING);
-    Frag x[NS], x3[R::UNITS > 1 ? NS : 1], y[R::UNITS][NS];
-    if (OUT && on && units > 0) {
+    constexpr bool TWO_ROWS = UNITS > 1 && R::unit_row(W, 0, REV) != R::unit_row(W, UNITS > 1, REV);  // (wave 0's)
+    Frag x[1 + TWO_ROWS][NS], y[UNITS > 0 ? UNITS : 1][NS];
+    if (OUT && UNITS > 0 && on) {
       const unsigned xr = lds0 + buf * R::BUF + R::XB + R::ZB + XC::rows(lane), yr = lds0 + buf * R::BUF + XC::rows(lane);
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
-        x[s] = XC::by_row(xr, ui[0] * 16 * XC::ROWB, s);
 #pragma unroll
-        for (int u = 0; u < R::UNITS; ++u)
-          if (u < 2) y[u][s] = XC::by_row(yr, uj[u] * 16 * XC::ROWB, s);
-        if constexpr (R::UNITS > 1) {
-          if (wave == 0) x3[s] = XC::by_row(xr, ui[1] * 16 * XC::ROWB, s);
-          else if (units > 2) y[R::UNITS - 1][s] = XC::by_row(yr, uj[2] * 16 * XC::ROWB, s);
+        for (int u = 0; u < UNITS; ++u) {
+          if (u <= TWO_ROWS) x[u][s] = XC::by_row(xr, R::unit_row(W, u, REV) * 16 * XC::ROWB, s);
+          y[u][s] = XC::by_row(yr, R::unit_col(W, u, REV) * 16 * XC::ROWB, s);
         }
       }
     }
@@ -419,43 +417,34 @@ template <typename T, int KW, bool OUT, bool REV> __device__ __forceinline__ voi
     }
     if (dots && it >= 2) leave_dots(it - 2);
     if constexpr (OUT) {
-      if (on && units > 0) {
+      if (UNITS > 0 && on) {
         // ---- pairs: rows of a result are j, its column is i
         char* pairs = lds + R::PAIRS + (it & 1) * R::PAIRB + 16 * lane;
-        floatx4 sc[R::UNITS];
+        floatx4 sc[UNITS > 0 ? UNITS : 1];
 #pragma unroll
-        for (int u = 0; u < R::UNITS; ++u) sc[u] = floatx4{0.f, 0.f, 0.f, 0.f};
+        for (int u = 0; u < UNITS; ++u) sc[u] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int s = 0; s < NS; ++s) {
-          F::mma(sc[0], y[0][s], x[s]);
-          if constexpr (R::UNITS > 1) {
-            if (wave == 0) {
-              F::mma(sc[1], y[1][s], x3[s]);
-            } else {
-              F::mma(sc[1], y[1][s], x[s]);
-              if (units > 2) F::mma(sc[2], y[2][s], x[s]);
-            }
-          }
-        }
+        for (int s = 0; s < NS; ++s)
 #pragma unroll
-        for (int u = 0; u < R::UNITS; ++u) {
-          if (u >= units) continue;
-          const int i = 16 * ui[u] + l16, j0 = 16 * uj[u] + g4;
+          for (int u = 0; u < UNITS; ++u) F::mma(sc[u], y[u][s], x[u < 1 + TWO_ROWS ? u : TWO_ROWS][s]);
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) {
+          const int it16 = R::unit_row(W, u, REV), jt = R::unit_col(W, u, REV), i = 16 * it16 + l16, j0 = 16 * jt + g4;
           const float hi_ = sums[i], li_ = sums[64 + i];
           const floatx4 hj = load4(sums + j0), lj = load4(sums + 64 + j0);
 #pragma unroll
           for (int r = 0; r < 4; ++r) sc[u][r] *= REV ? between(hj[r], lj[r], hi_, li_) : between(hi_, li_, hj[r], lj[r]);
-          if (ui[u] == uj[u] || valid < C) {
+          if (it16 == jt || (REV && valid < C)) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) sc[u][r] = (REV ? j0 + r >= i && j0 + r < valid : j0 + r <= i) ? sc[u][r] : 0.f;
           }
 #pragma unroll
           for (int r = 0; r < 4; ++r) sc[u][r] = rounded(sc[u][r]);
-          char* q = pairs + R::slot(ui[u], uj[u] / F::TP, REV) * F::PARTS * 1024;
+          char* q = pairs + R::slot(it16, jt / F::TP, REV) * F::PARTS * 1024;
           if constexpr (F::PARTS == 2) {
-            const bf16x4 h = pack_bf16x4(sc[u]);
-            *reinterpret_cast<bf16x4*>(q + 8 * (uj[u] % 2)) = h;
-            *reinterpret_cast<bf16x4*>(q + 8 * (uj[u] % 2) + 1024) = rest_of(sc[u], h);
+            const bf16x4 h = to_bf16(sc[u]);
+            *reinterpret_cast<bf16x4*>(q + 8 * (jt % 2)) = h;
+            *reinterpret_cast<bf16x4*>(q + 8 * (jt % 2) + 1024) = rest_of(sc[u], h);
           } else {
             *reinterpret_cast<floatx4*>(q) = sc[u];
           }
@@ -469,6 +458,13 @@ template <typename T, int KW, bool OUT, bool REV> __device__ __forceinline__ voi
   }
   if (dots && k.nchunk > 0) leave_dots(k.nchunk - 1);
   if (!OUT && k.item == 0 && threadIdx.x == 448) a.whole[(int64_t)k.slot * a.H + k.h] = between(whole_h, whole_l, 0.f, 0.f);
+}
+
+template <typename T, int KW, bool OUT, bool REV> __device__ __forceinline__ void pair_wave(int wave, const Walk& a, const Role& ro, const Task& k, char* lds) {
+  if (wave == 0) walk_pairs<T, KW, OUT, REV, 0>(a, ro, k, lds);
+  else if (wave == 1) walk_pairs<T, KW, OUT, REV, 1>(a, ro, k, lds);
+  else if (wave == 2) walk_pairs<T, KW, OUT, REV, 2>(a, ro, k, lds);
+  else walk_pairs<T, KW, OUT, REV, 3>(a, ro, k, lds);
 }
 
 // The other four: 16 columns of the state and of the results each.
@@ -764,8 +760,9 @@ template <typename T, int KW, bool OUT> __global__ __launch_bounds__(512) void d
     lds_barrier();
   }
   if (threadIdx.x >= 256) {
-    if (ro.rev) walk_pairs<T, KW, OUT, true>(a, ro, k, lds);
-    else walk_pairs<T, KW, OUT, false>(a, ro, k, lds);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) - 4;
+    if (ro.rev) pair_wave<T, KW, OUT, true>(wave, a, ro, k, lds);
+    else pair_wave<T, KW, OUT, false>(wave, a, ro, k, lds);
   } else if (OUT && ro.dots) {
     if (ro.rev) walk_state<T, KW, OUT, true, OUT>(a, ro, k, lds);
     else walk_state<T, KW, OUT, false, OUT>(a, ro, k, lds);
@@ -980,13 +977,13 @@ int64_t ceil_div(int64_t x, int64_t y) { return (x + y - 1) / y; }
 constexpr int MAX_D = 256, SHORTEST = 512;
 
 // Tokens of a segment, a multiple of 64, or 0: rows are walked whole.  Segments read keys and values (queries and gradients) once more, so they
-// are for rows and heads that leave most CUs without a workgroup: as many as give every CU two (of which a CU takes two at a time on the local
-// walks, one on the others), of 512 tokens and more.  The rows of a packed batch are taken for one: their lengths are not known here, and sequences
+// are for rows and heads that leave most CUs without a workgroup: as many as give every CU one, of 512 tokens and more (H16 T65000 d128:
+// 290 us and 125 on the local walks; with two a CU 310 and 138).  The rows of a packed batch are taken for one: their lengths are not known here, and sequences
 // of one segment are walked once whatever its size.
 int segment(const lnx_decay_args* a) {
   const int64_t walks = (a->nseq ? 1 : (int64_t)a->B) * a->H * ceil_div(a->dv, SLAB);
   if (walks > 128) return 0;
-  int64_t s = up((int)ceil_div(a->T, 512 / walks), 64);
+  int64_t s = up((int)ceil_div(a->T, 256 / walks), 64);
   if (s < SHORTEST) s = SHORTEST;
   return s >= a->T ? 0 : (int)s;
 }
