@@ -974,18 +974,19 @@ template <typename T, int VN> __global__ __launch_bounds__(256) void decay_step_
 
 int up(int x, int to) { return (x + to - 1) / to * to; }
 int64_t ceil_div(int64_t x, int64_t y) { return (x + y - 1) / y; }
-constexpr int MAX_D = 256, SHORTEST = 512;
+constexpr int MAX_D = 256;
 
 // Tokens of a segment, a multiple of 64, or 0: rows are walked whole.  Segments read keys and values (queries and gradients) once more, so they
-// are for rows and heads that leave most CUs without a workgroup: as many as give every CU one, of 512 tokens and more (H16 T65000 d128:
-// 290 us and 125 on the local walks; with two a CU 310 and 138).  The rows of a packed batch are taken for one: their lengths are not known here, and sequences
-// of one segment are walked once whatever its size.
+// are for rows and heads that leave CUs without a workgroup: as many as give every CU one (H16 T65000 d128: 290 us and 125 on the local walks; with
+// two a CU 310 and 138), of four chunks and more, for rows of more than eight (us of forward alone and with backward, chunks of 64, eight and
+// more -> four: H8 T1000 d128 35, 79 -> 27, 62; H16 T700 34, 77 -> 25, 68; of two 25, 70 and 23, 74; H16 T500 d64 whole 15, 37, in two 20, 45).
+// The rows of a packed batch are taken for one: their lengths are not known here, and sequences of one segment are walked once whatever its size.
 int segment(const lnx_decay_args* a) {
   const int64_t walks = (a->nseq ? 1 : (int64_t)a->B) * a->H * ceil_div(a->dv, SLAB);
-  if (walks > 128) return 0;
-  int64_t s = up((int)ceil_div(a->T, 256 / walks), 64);
-  if (s < SHORTEST) s = SHORTEST;
-  return s >= a->T ? 0 : (int)s;
+  const int shortest = a->dtype == LNX_BF16 ? 256 : 128;
+  if (walks > 128 || a->T <= 2 * shortest) return 0;
+  const int s = up((int)ceil_div(a->T, 256 / walks), 64);
+  return s < shortest ? shortest : s >= a->T ? 0 : s;
 }
 struct Layout {
   int seg, nseg;
