@@ -21,7 +21,8 @@ namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int SLAB = 64;                        // columns of z of a workgroup: 16 a wave
-constexpr int64_t MAX_GRID = 0xffffffff / 256;  // workgroups of a launch
+constexpr int64_t MAX_GRID = 0xffffffff;        // threads of a launch
+constexpr int WALK_THREADS = 512, JOIN_THREADS = 256, GATE_THREADS = 1024, STEP_THREADS = 256;
 typedef __attribute__((address_space(3))) char lds_char;
 
 // Products of 16 x 16 tiles: K contraction slots an operand, which the results of TP tiles fill.  Slot (a, r) of lane group g = lane / 16 is
@@ -733,7 +734,7 @@ template <typename T, int KW, bool OUT, bool REV, bool DOTS> __device__ __forcei
   }
 }
 
-template <typename T, int KW, bool OUT> __global__ __launch_bounds__(512) void decay_walk_kernel(Walk a) {
+template <typename T, int KW, bool OUT> __global__ __launch_bounds__(WALK_THREADS) void decay_walk_kernel(Walk a) {
   typedef Room<T, KW, OUT> R;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   // workgroups of one (slot, head) follow each other on one XCD, whose L2 then holds what they share
@@ -756,7 +757,7 @@ template <typename T, int KW, bool OUT> __global__ __launch_bounds__(512) void d
   if (!OUT && (ro.rev ? k.p.first : k.p.last)) return;  // nothing walks on from there
   k.nchunk = (k.p.len + R::C - 1) / R::C, k.col0 = item * SLAB, k.vw = min(SLAB, ro.vw - k.col0);
   if (ro.kw < KW || k.vw < SLAB) {
-    for (int i = threadIdx.x * 16; i < R::PAIRS; i += 512 * 16) *reinterpret_cast<floatx4*>(lds + i) = floatx4{0.f, 0.f, 0.f, 0.f};
+    for (int i = threadIdx.x * 16; i < R::PAIRS; i += WALK_THREADS * 16) *reinterpret_cast<floatx4*>(lds + i) = floatx4{0.f, 0.f, 0.f, 0.f};
     lds_barrier();
   }
   if (threadIdx.x >= 256) {
@@ -780,7 +781,7 @@ struct Join {
   int H, T, nseq, seg, nseg, rev;
   int64_t size;
 };
-__global__ __launch_bounds__(256) void decay_join_kernel(Join a) {
+__global__ __launch_bounds__(JOIN_THREADS) void decay_join_kernel(Join a) {
   const int row = blockIdx.x / a.H, h = blockIdx.x % a.H;
   int64_t slot = (int64_t)row * a.nseg;
   int n = a.nseg;
@@ -789,7 +790,7 @@ __global__ __launch_bounds__(256) void decay_join_kernel(Join a) {
     n = max(1, (int)(((unsigned)len + a.seg - 1) / a.seg));
     slot = packed_slot(from, row, a.seg);
   }
-  const int64_t e0 = ((int64_t)blockIdx.y * 256 + threadIdx.x) * 4;
+  const int64_t e0 = ((int64_t)blockIdx.y * JOIN_THREADS + threadIdx.x) * 4;
   const int many = (int)min((int64_t)4, a.size - e0);
   float s[4], add[4], next[4];
   const auto at = [&](int i) { return a.states + ((slot + (a.rev ? n - 1 - i : i)) * a.H + h) * a.size + e0; };
@@ -824,8 +825,8 @@ struct GateGrad {
   int B, H, T, nseq, slabs;
   int64_t step, size;
 };
-template <int C> __global__ __launch_bounds__(1024) void decay_gate_grad_kernel(GateGrad a) {
-  constexpr int NC = 1024 / C;
+template <int C> __global__ __launch_bounds__(GATE_THREADS) void decay_gate_grad_kernel(GateGrad a) {
+  constexpr int NC = GATE_THREADS / C;
   __shared__ float chunk[2][NC], red[16];
   const int row = blockIdx.x / a.H, h = blockIdx.x % a.H, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, in = lane % C, mine = threadIdx.x / C;
   int from = 0, len = a.T;
@@ -843,7 +844,7 @@ template <int C> __global__ __launch_bounds__(1024) void decay_gate_grad_kernel(
   float W = 0.f;
   if (a.d_fin) {
     const int64_t at = ((int64_t)row * a.H + h) * a.size;
-    for (int64_t i = threadIdx.x; i < a.size; i += 1024) W += a.fin[at + i] * a.d_fin[at + i];
+    for (int64_t i = threadIdx.x; i < a.size; i += GATE_THREADS) W += a.fin[at + i] * a.d_fin[at + i];
     W = block_sum(W);
   }
   const auto get = [&](int t, float& x, float& y, float& u) {
@@ -856,10 +857,10 @@ template <int C> __global__ __launch_bounds__(1024) void decay_gate_grad_kernel(
     }
   };
   float sum = 0.f, x, y, u, nx, ny, nu;
-  int t = (len - 1) / 1024 * 1024 + threadIdx.x;
+  int t = (len - 1) / GATE_THREADS * GATE_THREADS + threadIdx.x;
   get(t, x, y, u);
-  for (int turn = 0; t > -1024 + (int)threadIdx.x; t -= 1024, turn ^= 1) {
-    get(t - 1024, nx, ny, nu);
+  for (int turn = 0; t > -GATE_THREADS + (int)threadIdx.x; t -= GATE_THREADS, turn ^= 1) {
+    get(t - GATE_THREADS, nx, ny, nu);
     float sx = x, su = u, py = y;
 #pragma unroll
     for (int o = 1; o < C; o <<= 1) {
@@ -909,12 +910,12 @@ struct Step {
   float scale;
 };
 constexpr int STEP_COLS = 128, STEP_MAX_DK = 256;
-template <typename T, int VN> __global__ __launch_bounds__(256) void decay_step_kernel(Step a) {
-  constexpr int LPR = STEP_COLS / VN, GROUPS = 256 / LPR, U = 8;  // lanes of a row, rows at a time
+template <typename T, int VN> __global__ __launch_bounds__(STEP_THREADS) void decay_step_kernel(Step a) {
+  constexpr int LPR = STEP_COLS / VN, GROUPS = STEP_THREADS / LPR, U = 8;  // lanes of a row, rows at a time
   __shared__ float qk[2][STEP_MAX_DK], red[GROUPS][STEP_COLS];
   const int slab = blockIdx.x % a.slabs, bh = blockIdx.x / a.slabs, h = bh % a.H, li = threadIdx.x % LPR, grp = threadIdx.x / LPR, c = slab * STEP_COLS + li * VN;
   const float f = __expf(a.g[bh / a.H * a.gb + h * a.gh]);
-  for (int i = threadIdx.x; i < a.dk; i += 256) {
+  for (int i = threadIdx.x; i < a.dk; i += STEP_THREADS) {
     qk[0][i] = to_f32(static_cast<const T*>(a.q)[(int64_t)bh * a.dk + i]) * a.scale;
     qk[1][i] = to_f32(static_cast<const T*>(a.k)[(int64_t)bh * a.dk + i]);
   }
@@ -1017,7 +1018,8 @@ int check(const char* what, const lnx_decay_args* a, bool bwd) {
   if (a->nseq && !a->cu_seqlens) return lnx_set_error(LNX_ERR_NULL, "%s: nseq without cu_seqlens", what);
   if (a->B == 0) return LNX_OK;
   const Layout l = layout(a);
-  if (l.slots * a->H * (2 * ceil_div(a->dk, SLAB) + ceil_div(a->dv, SLAB)) > MAX_GRID || l.rows * a->H > MAX_GRID) return lnx_set_error(LNX_ERR_SHAPE, "%s: too many rows", what);
+  const int64_t walks = l.slots * a->H * (bwd ? 2 * ceil_div(a->dk, SLAB) + ceil_div(a->dv, SLAB) : ceil_div(a->dv, SLAB));
+  if (walks > MAX_GRID / WALK_THREADS || l.rows * a->H > MAX_GRID / (bwd ? GATE_THREADS : JOIN_THREADS)) return lnx_set_error(LNX_ERR_SHAPE, "%s: too many rows", what);
   if (!bwd && !a->final_state) return lnx_set_error(LNX_ERR_NULL, "%s: final_state is required", what);
   if (bwd && a->d_final_state && !a->final_state) return lnx_set_error(LNX_ERR_NULL, "%s: d_final_state needs final_state", what);
   if (bwd && !a->d_g) return lnx_set_error(LNX_ERR_NULL, "%s: d_g is required", what);
@@ -1069,7 +1071,7 @@ template <typename T, int KW, bool OUT> int start(const Walk& k, const char* nam
   static_assert(bytes <= 160 * 1024, "LDS of a CU");
   if (int rc = lnx_lds_limit(reinterpret_cast<const void*>(kernel), bytes)) return rc;
   lnx_profile_mark(name, st);
-  hipLaunchKernelGGL(kernel, dim3((unsigned)((int64_t)k.units * k.per)), dim3(512), bytes, st, k);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)((int64_t)k.units * k.per)), dim3(WALK_THREADS), bytes, st, k);
   return LNX_OK;
 }
 template <typename T, bool OUT> int start(Walk& k, int roles, const char* name, hipStream_t st) {
@@ -1084,7 +1086,7 @@ template <typename T, bool OUT> int start(Walk& k, int roles, const char* name, 
 void join(const lnx_decay_args* a, const Layout& l, float* states, const float* whole, const float* init, bool rev, hipStream_t st) {
   Join j{states, whole, init, a->cu_seqlens, a->H, a->T, a->nseq, l.seg, l.nseg, rev, (int64_t)a->dk * a->dv};
   lnx_profile_mark("decay_join", st);
-  decay_join_kernel<<<dim3((unsigned)(l.rows * a->H), (unsigned)ceil_div(j.size, 1024)), 256, 0, st>>>(j);
+  decay_join_kernel<<<dim3((unsigned)(l.rows * a->H), (unsigned)ceil_div(j.size, 4 * JOIN_THREADS)), JOIN_THREADS, 0, st>>>(j);
 }
 
 template <typename T> int forward(const lnx_decay_args* a, hipStream_t st) {
@@ -1144,8 +1146,8 @@ template <typename T> int backward(const lnx_decay_args* a, hipStream_t st) {
   d.B = a->B, d.H = a->H, d.T = a->T, d.nseq = a->nseq, d.slabs = q.slabs, d.step = k.dots_step, d.size = (int64_t)a->dk * a->dv;
   lnx_profile_mark("decay_gate_grad", st);
   const dim3 rows((unsigned)(l.rows * a->H));
-  if (q.kw <= 128) decay_gate_grad_kernel<chunk_of<T, 128>()><<<rows, 1024, 0, st>>>(d);
-  else decay_gate_grad_kernel<chunk_of<T, 256>()><<<rows, 1024, 0, st>>>(d);
+  if (q.kw <= 128) decay_gate_grad_kernel<chunk_of<T, 128>()><<<rows, GATE_THREADS, 0, st>>>(d);
+  else decay_gate_grad_kernel<chunk_of<T, 256>()><<<rows, GATE_THREADS, 0, st>>>(d);
   if (a->g_per_head) {
     lnx_profile_mark("decay_gate_sum", st);
     decay_gate_sum_kernel<<<dim3((unsigned)a->H), 256, 0, st>>>(d.part, l.rows, a->H, a->d_g);
@@ -1195,20 +1197,21 @@ extern "C" int lnx_decay_step(const lnx_decay_step_args* a, void* hip_stream) {
   if (a->B < 0 || a->H <= 0 || a->dk <= 0 || a->dk > STEP_MAX_DK || a->dv <= 0)
     return lnx_set_error(LNX_ERR_SHAPE, "%s: unsupported dimensions B=%d H=%d dk=%d dv=%d (dk at most %d)", what, a->B, a->H, a->dk, a->dv, STEP_MAX_DK);
   if (a->dtype != LNX_F32 && a->dtype != LNX_BF16) return lnx_set_error(LNX_ERR_DTYPE, "%s: dtype %d", what, a->dtype);
+  if (!(a->scale == a->scale) || a->scale - a->scale != 0.f) return lnx_set_error(LNX_ERR_SHAPE, "%s: scale must be finite", what);
   if (a->B == 0) return LNX_OK;
   if (!a->q || !a->k || !a->v || !a->g || !a->state || !a->o || !a->new_state) return lnx_set_error(LNX_ERR_NULL, "%s: a tensor is missing", what);
   Step k{a->q, a->k, a->v, a->g, a->state, a->o, a->new_state, a->B > 1 ? a->g_stride_b : 0, a->H > 1 ? a->g_stride_h : 0, a->H, a->dk, a->dv, (int)ceil_div(a->dv, STEP_COLS), a->scale};
   const int64_t grid = (int64_t)a->B * a->H * k.slabs;
-  if (grid > MAX_GRID) return lnx_set_error(LNX_ERR_SHAPE, "%s: too many rows", what);
+  if (grid > MAX_GRID / STEP_THREADS) return lnx_set_error(LNX_ERR_SHAPE, "%s: too many rows", what);
   const bool vec = a->dv % 4 == 0 && aligned(a->state, 16) && aligned(a->new_state, 16);
   hipStream_t st = static_cast<hipStream_t>(hip_stream);
   lnx_profile_mark(what, st);
   if (a->dtype == LNX_BF16) {
-    if (vec) decay_step_kernel<bf16_t, 4><<<dim3((unsigned)grid), 256, 0, st>>>(k);
-    else decay_step_kernel<bf16_t, 1><<<dim3((unsigned)grid), 256, 0, st>>>(k);
+    if (vec) decay_step_kernel<bf16_t, 4><<<dim3((unsigned)grid), STEP_THREADS, 0, st>>>(k);
+    else decay_step_kernel<bf16_t, 1><<<dim3((unsigned)grid), STEP_THREADS, 0, st>>>(k);
   } else {
-    if (vec) decay_step_kernel<float, 4><<<dim3((unsigned)grid), 256, 0, st>>>(k);
-    else decay_step_kernel<float, 1><<<dim3((unsigned)grid), 256, 0, st>>>(k);
+    if (vec) decay_step_kernel<float, 4><<<dim3((unsigned)grid), STEP_THREADS, 0, st>>>(k);
+    else decay_step_kernel<float, 1><<<dim3((unsigned)grid), STEP_THREADS, 0, st>>>(k);
   }
   return finish(what, LNX_OK, st);
 }

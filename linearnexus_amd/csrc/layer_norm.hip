@@ -247,7 +247,7 @@ Plan plan(int d, int dtype) {
   if (v <= 1024) return {512, 2};
   return {512, 4};  // fp32 only: eight vectors of bf16 a thread would not fit the backward pass's registers
 }
-constexpr int MAX_D = 8192, MAX_HEADS = 1 << 16;
+constexpr int MAX_D = 8192, MAX_HEADS = 1 << 16, MAX_WEIGHTS = 1 << 26;  // the last: the sums' launch takes 16 threads a column
 
 // Workgroups of the backward pass per head: three a CU in all, each with one partial row of the parameters' gradients
 int64_t bwd_per_head(int64_t outer, int64_t n, const Plan& p) {
@@ -292,9 +292,9 @@ template <typename T> void pick(const Args& a, const Plan& p, bool vec, bool bwd
 
 int run(const char* what, const lnx_layer_norm_args* q, bool bwd, hipStream_t st) {
   if (!q) return lnx_set_error(LNX_ERR_NULL, "%s: args is NULL", what);
-  if (q->rows < 0 || q->rows > 0x7fffffff || q->d <= 0 || q->d > MAX_D || q->heads <= 0 || q->heads > MAX_HEADS || q->rows % q->heads)
-    return lnx_set_error(LNX_ERR_SHAPE, "%s: rows=%lld heads=%d d=%d (at most %d columns, %d heads; rows a multiple of heads)", what, (long long)q->rows, q->heads, q->d, MAX_D,
-                         MAX_HEADS);
+  if (q->rows < 0 || q->rows > 0x7fffffff || q->d <= 0 || q->d > MAX_D || q->heads <= 0 || q->heads > MAX_HEADS || (int64_t)q->heads * q->d > MAX_WEIGHTS || q->rows % q->heads)
+    return lnx_set_error(LNX_ERR_SHAPE, "%s: rows=%lld heads=%d d=%d (at most %d columns, %d heads, %d weights; rows a multiple of heads)", what, (long long)q->rows, q->heads,
+                         q->d, MAX_D, MAX_HEADS, MAX_WEIGHTS);
   if (q->dtype != LNX_F32 && q->dtype != LNX_BF16) return lnx_set_error(LNX_ERR_DTYPE, "%s: dtype %d", what, q->dtype);
   if (q->rows > 0 && (!q->x || (bwd ? !q->d_y || !q->d_x : !q->y))) return lnx_set_error(LNX_ERR_NULL, "%s: %s required", what, bwd ? "x, d_y and d_x are" : "x and y are");
   const bool params = bwd && (q->d_weight || q->d_bias);
