@@ -7,8 +7,8 @@
 // columns of z: each of its four waves keeps 16 columns of the state in registers, in the layout of a product's result, which is the layout
 // of the next product's operand (tile pairs of 16 x 16), so the state never leaves them.  A chunk's pairs are formed once per workgroup
 // and handed over through LDS.
-// Rounding (bf16): pairs, the state as an operand and the z_j with their factors enter the products in two bf16 parts (2^-16 of each term), so results
-// are off by their own rounding alone, and dg, a running difference of x . out and y . out over a whole sequence, keeps its digits.
+// Rounding (bf16): pairs, the state as an operand and the z_j with their factors enter the products in two bf16 parts or three, so results are off
+// by their own rounding alone, states like fp32's, and dg, a running difference of x . out and y . out over a whole sequence, keeps its digits.
 // Exponents are differences of sums over a chunk: the sums are held as a multiple of 1/64 and a rest, so that a difference is exact to a unit
 // however far the sums have run (a decay of e^-100 beside one of 1).
 #include <type_traits>
@@ -29,14 +29,14 @@ typedef __attribute__((address_space(3))) char lds_char;
 // index 16 a + 4 g + r of the K: element r of that group in result tile a.
 template <typename T> struct Form;
 template <> struct Form<bf16_t> {
-  static constexpr int K = 32, TP = 2, PARTS = 2;
+  static constexpr int K = 32, TP = 2;
   typedef bf16x8 Frag;
   static __device__ __forceinline__ void mma(floatx4& c, const Frag& a, const Frag& b) { c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
   static __device__ __forceinline__ void put(Frag& f, int a, int r, float x) { f[4 * a + r] = (bf16_t)x; }
   static __device__ __forceinline__ float get(const Frag& f, int a, int r) { return (float)f[4 * a + r]; }
 };
 template <> struct Form<float> {
-  static constexpr int K = 16, TP = 1, PARTS = 1;
+  static constexpr int K = 16, TP = 1;
   typedef floatx4 Frag;
   static __device__ __forceinline__ void mma(floatx4& c, const Frag& a, const Frag& b) {
 #pragma unroll
@@ -49,11 +49,11 @@ template <> struct Form<float> {
 template <typename T, int KW> constexpr int chunk_of() { return (sizeof(T) == 2 ? 64 : 32) / (KW > 128 ? 2 : 1); }
 __device__ __forceinline__ bool is_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
-// Result tiles as an operand, and what its rounding left.  Of an infinite value that is not a number: as an integer it lies above 2^100, where rests
-// are cut (two at a time), so that it adds nothing to a sum that the infinite value is in.
-__device__ __forceinline__ bf16x4 rest_of(floatx4 v, bf16x4 h) {
+// Result tiles as an operand in P parts: each is rounded to bf16 and the next holds what that left.  Of an infinite value that is not a number: as
+// an integer it lies above 2^100, where rests are cut (two at a time), so that it adds nothing to a sum that the infinite value is in.
+__device__ __forceinline__ floatx4 minus(floatx4 v, bf16x4 h) { return floatx4{v[0] - (float)h[0], v[1] - (float)h[1], v[2] - (float)h[2], v[3] - (float)h[3]}; }
+__device__ __forceinline__ bf16x4 rest(floatx4 d) {
   typedef short short4_ __attribute__((ext_vector_type(4)));
-  const floatx4 d = {v[0] - (float)h[0], v[1] - (float)h[1], v[2] - (float)h[2], v[3] - (float)h[3]};
   return __builtin_bit_cast(bf16x4, __builtin_elementwise_min(__builtin_bit_cast(short4_, pack_bf16x4(d)), short4_{0x7180, 0x7180, 0x7180, 0x7180}));
 }
 // Rounded to bf16, and opaque: -ffast-math takes a conversion and its inverse for nothing, and the rest with them
@@ -63,12 +63,22 @@ __device__ __forceinline__ bf16x4 to_bf16(floatx4 v) {
   asm("" : "+v"(u));
   return __builtin_bit_cast(bf16x4, u);
 }
-__device__ __forceinline__ void split(const floatx4 (&v)[2], bf16x8& hi, bf16x8& lo) {
-  const bf16x4 h0 = to_bf16(v[0]), h1 = to_bf16(v[1]);
-  hi = Mma16::join(h0, h1);
-  lo = Mma16::join(rest_of(v[0], h0), rest_of(v[1], h1));
+template <int P> __device__ __forceinline__ void parts_of(floatx4 v, bf16x4 (&part)[P]) {
+  part[0] = to_bf16(v);
+#pragma unroll
+  for (int i = 1; i < P; ++i) {
+    v = minus(v, part[i - 1]);
+    part[i] = rest(v);
+  }
 }
-__device__ __forceinline__ void split(const floatx4 (&v)[1], floatx4& hi, floatx4&) { hi = v[0]; }
+template <int P> __device__ __forceinline__ void split(const floatx4 (&v)[2], bf16x8 (&part)[P]) {
+  bf16x4 a[P], b[P];
+  parts_of(v[0], a);
+  parts_of(v[1], b);
+#pragma unroll
+  for (int i = 0; i < P; ++i) part[i] = Mma16::join(a[i], b[i]);
+}
+__device__ __forceinline__ void split(const floatx4 (&v)[1], floatx4 (&part)[1]) { part[0] = v[0]; }
 
 // Whether all of an operand's values are finite: their exponents, two of bf16 at a time
 __device__ __forceinline__ bool all_finite(const bf16x8& f) {
@@ -259,18 +269,38 @@ template <typename T> __device__ __forceinline__ const T* head_of(const Side& s,
   return static_cast<const T*>(s.p) + p.b * s.sb + h * s.sh + p.tok * s.st;
 }
 
+// bf16 parts of an operand that is not one of the inputs.  What a token adds to the state: three, exact as fp32 is.  The state as an operand: three
+// where dg is taken from the results, two where they are rounded to bf16.  Pairs: two.  (Errors against 64 bits at H8 T4096 d128, everything
+// in two parts -> thus: states 2.4e-6 -> 2.2e-7, dg 8.8e-6 -> 1.0e-6; pairs in three too: dg 1.0e-6.  B8 H16 T4096, us: forward 151 -> 165,
+// backward 530 -> 620, 650 with the pairs.)
+template <typename T> constexpr int parts_of_z() { return sizeof(T) == 2 ? 3 : 1; }
+template <typename T> constexpr int parts_of_state(bool dots) { return sizeof(T) == 2 ? (dots ? 3 : 2) : 1; }
+template <typename T> constexpr int parts_of_pairs() { return sizeof(T) == 2 ? 2 : 1; }
+
 // LDS of a walk.  OUT: false for the local walks of segments, which leave what a segment adds to the state and nothing else.
 template <typename T, int KW, bool OUT> struct Room {
   static constexpr int C = chunk_of<T, KW>(), NI = C / 16, NJ = C / Form<T>::K;
-  static constexpr int SLOTS = NI == 4 && NJ == 2 ? 6 : NI * NJ;  // of 16 x K blocks of pairs; of the wide ones two are always empty
-  static constexpr int XB = C * KW * sizeof(T), ZB = C * SLAB * sizeof(T), BUF = (OUT ? 2 : 1) * XB + ZB, PAIRB = OUT ? SLOTS * Form<T>::PARTS * 1024 : 0;
+  // Pairs lie in LDS as operands, in blocks of 16 rows x K: those that have any, of bf16 in half a block where only one of its two tiles has
+  static constexpr bool needed(int i, int j, bool rev) { return rev ? Form<T>::K * (j + 1) > 16 * i : Form<T>::K * j <= 16 * i + 15; }
+  static constexpr bool half(int i, int j, bool rev) { return Form<T>::TP == 2 && (rev ? 2 * j < i : 2 * j + 1 > i); }
+  static constexpr int P = parts_of_pairs<T>();
+  static constexpr int block(int i, int j, bool rev) {  // where block (i, j) begins
+    int at = 0;
+    for (int b = 0; b < i * NJ + j; ++b)
+      if (needed(b / NJ, b % NJ, rev)) at += P * (half(b / NJ, b % NJ, rev) ? 512 : 1024);
+    return at;
+  }
+  static constexpr int slot(int i, int j, bool rev) {  // its number
+    int n = 0;
+    for (int b = 0; b < i * NJ + j; ++b) n += needed(b / NJ, b % NJ, rev);
+    return n;
+  }
+  static constexpr int SLOTS = slot(NI, 0, false);
+  static constexpr int XB = C * KW * sizeof(T), ZB = C * SLAB * sizeof(T), BUF = (OUT ? 2 : 1) * XB + ZB, PAIRB = OUT ? block(NI, 0, false) : 0;
   static constexpr int RING = OUT ? 3 : 6, AHEAD = RING - 2;  // chunks in LDS; how far ahead of the pairs' chunk they are fetched
   static constexpr int PAIRS = RING * BUF, FACTORS = PAIRS + 2 * PAIRB, SUMS = FACTORS + 2 * 1024, RAW = SUMS + 4 * 512, DOTS = RAW + RING * 256;
   static constexpr int BYTES = DOTS + (OUT ? 2 * 4 * 2 * C * 4 : 0);
-  static constexpr int slot(int i, int j, bool rev) { return SLOTS != 6 ? i * NJ + j : rev ? (i < 2 ? 2 * i + j : i + 2) : (i < 2 ? i : 2 * i - 2 + j); }
-  // whether row tile i has pairs with block j
-  static constexpr bool needed(int i, int j, bool rev) { return rev ? Form<T>::K * (j + 1) > 16 * i : Form<T>::K * j <= 16 * i + 15; }
-  // The 16 x 16 tiles of pairs, ten of a chunk of 64, in four nearly equal shares: tile u of wave w; those above the diagonal hold zeros
+  // The 16 x 16 tiles of pairs, ten of a chunk of 64, in four nearly equal shares: tile u of wave w
   static constexpr int units(int w) { return NI == 4 ? (w < 2 ? 2 : 3) : w < NI * (NI + 1) / 2; }
   static constexpr int unit_row(int w, int u, bool rev) {
     const int i = NI == 4 ? (w == 0 ? 3 * u : w) : w > 0;
@@ -366,8 +396,6 @@ template <typename T, int KW, bool OUT, bool REV, int W> __device__ __forceinlin
   float* sums = reinterpret_cast<float*>(lds + R::SUMS) + 128 * wave;  // of this wave: multiples, rests
   const float* raw = reinterpret_cast<const float*>(lds + R::RAW);
   float whole_h = 0.f, whole_l = 0.f;
-  if constexpr (OUT)
-    for (int i = (threadIdx.x - 256) * 16; i < 2 * R::PAIRB; i += 256 * 16) *reinterpret_cast<floatx4*>(lds + R::PAIRS + i) = floatx4{0.f, 0.f, 0.f, 0.f};
   // until chunk `it` is there: all but the loads of those behind it, which are whole ones if they are to be counted
   const auto arrived = [&](int it) {
     constexpr int N = (R::AHEAD - 1) * (NY + NX + NZ);
@@ -420,7 +448,7 @@ template <typename T, int KW, bool OUT, bool REV, int W> __device__ __forceinlin
     if constexpr (OUT) {
       if (UNITS > 0 && on) {
         // ---- pairs: rows of a result are j, its column is i
-        char* pairs = lds + R::PAIRS + (it & 1) * R::PAIRB + 16 * lane;
+        char* pairs = lds + R::PAIRS + (it & 1) * R::PAIRB;
         floatx4 sc[UNITS > 0 ? UNITS : 1];
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) sc[u] = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -441,11 +469,13 @@ template <typename T, int KW, bool OUT, bool REV, int W> __device__ __forceinlin
           }
 #pragma unroll
           for (int r = 0; r < 4; ++r) sc[u][r] = rounded(sc[u][r]);
-          char* q = pairs + R::slot(it16, jt / F::TP, REV) * F::PARTS * 1024;
-          if constexpr (F::PARTS == 2) {
-            const bf16x4 h = to_bf16(sc[u]);
-            *reinterpret_cast<bf16x4*>(q + 8 * (jt % 2)) = h;
-            *reinterpret_cast<bf16x4*>(q + 8 * (jt % 2) + 1024) = rest_of(sc[u], h);
+          const bool half = R::half(it16, jt / F::TP, REV);
+          char* q = pairs + R::block(it16, jt / F::TP, REV) + (half ? 8 : 16) * lane;
+          if constexpr (F::TP == 2) {
+            bf16x4 part[R::P];
+            parts_of(sc[u], part);
+#pragma unroll
+            for (int i = 0; i < R::P; ++i) *reinterpret_cast<bf16x4*>(q + (half ? 512 * i : 8 * (jt % 2) + 1024 * i)) = part[i];
           } else {
             *reinterpret_cast<floatx4*>(q) = sc[u];
           }
@@ -475,7 +505,7 @@ template <typename T, int KW, bool OUT, bool REV, bool DOTS> __device__ __forcei
   typedef Cells<T, KW> XC;
   typedef Cells<T, SLAB> ZC;
   typedef Room<T, KW, OUT> R;
-  constexpr int C = R::C, NI = R::NI, NJ = R::NJ, NS = KW / F::K, NT = KW / 16, TP = F::TP, PARTS = F::PARTS;
+  constexpr int C = R::C, NI = R::NI, NJ = R::NJ, NS = KW / F::K, NT = KW / 16, TP = F::TP, ZP = parts_of_z<T>(), PP = R::P, SP = parts_of_state<T>(DOTS);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g4 = 4 * (lane >> 4), n0 = k.col0 + 16 * wave;
   const Spot& p = k.p;
   const unsigned lds0 = lds_byte_addr(lds);
@@ -519,26 +549,36 @@ template <typename T, int KW, bool OUT, bool REV, bool DOTS> __device__ __forcei
     wb += w_step;
   };
   if (DOTS && k.nchunk > 0) partners(t0);
+  floatx4 zero = {0.f, 0.f, 0.f, 0.f};  // kept in registers: a constant would be moved into every sum's at every chunk
+  asm volatile("" : "+v"(zero));
   for (int it = 0, at = 0; it < k.nchunk; ++it) {
     const int valid = min(C, p.len - t0);
     const float* f = reinterpret_cast<const float*>(lds + R::FACTORS) + 256 * (it & 1);
     const unsigned xr = xa + at, yc = ya + at, zc = za + at;
-    const char* pairs = lds + R::PAIRS + (it & 1) * R::PAIRB + 16 * lane;
+    const char* pairs = lds + R::PAIRS + (it & 1) * R::PAIRB;
     // What LDS holds is read well ahead of its use: two steps of x, all pairs, four tiles of y
-    Frag zf[NJ], zh[NJ], zl[NJ], x[3][NI], hi[2], lo[2], pf[R::SLOTS > 0 ? R::SLOTS : 1][PARTS], yf[4][NJ];
-    floatx4 acc[NI], in[NI], cf[NJ][TP];
+    Frag zf[NJ], zs[NJ][ZP], x[3][NI], sp[2][SP], pf[PP][R::SLOTS], yf[4][NJ];
+    floatx4 acc[NI], low[NI], in[NI], cf[NJ][TP];  // low: of the state's lower parts, summed apart so that their sums are not rounded at the whole's
     const auto read_x = [&](int s) {
 #pragma unroll
       for (int t = 0; t < NI; ++t) x[s % 3][t] = XC::by_row(xr, 16 * t * XC::ROWB, s);
     };
-    const auto read_pairs = [&](int half) {
+    const auto pair_block = [&](int t, int j, int part) -> Frag {
+      const char* q = pairs + R::block(t, j, REV);
+      if constexpr (TP == 2) {
+        if (R::half(t, j, REV)) {
+          const bf16x4 there = *reinterpret_cast<const bf16x4*>(q + 512 * part + 8 * lane), none = {};
+          return REV ? Mma16::join(none, there) : Mma16::join(there, none);
+        }
+      }
+      return *reinterpret_cast<const Frag*>(q + 1024 * part + 16 * lane);
+    };
+    const auto read_pairs = [&](int part) {
 #pragma unroll
       for (int t = 0; t < NI; ++t)
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
-          if (R::needed(t, j, REV) && (half < 0 || (t < (NI + 1) / 2) == (half == 0)))
-#pragma unroll
-            for (int part = 0; part < PARTS; ++part) pf[R::slot(t, j, REV)][part] = *reinterpret_cast<const Frag*>(pairs + (R::slot(t, j, REV) * PARTS + part) * 1024);
+          if (R::needed(t, j, REV)) pf[part][R::slot(t, j, REV)] = pair_block(t, j, part);
     };
     const auto read_y = [&](int i) {
 #pragma unroll
@@ -548,23 +588,22 @@ template <typename T, int KW, bool OUT, bool REV, bool DOTS> __device__ __forcei
       floatx4 v[TP];
 #pragma unroll
       for (int t = 0; t < TP; ++t) v[t] = st[TP * s + t];
-      split(v, hi[s & 1], lo[s & 1]);
+      split(v, sp[s & 1]);
     };
     const auto from_state = [&](int s) {  // rows of the result are columns of z, its column is i
 #pragma unroll
-      for (int t = 0; t < NI; ++t) F::mma(acc[t], hi[s & 1], x[s % 3][t]);
-      if (PARTS == 2)
+      for (int part = 0; part < SP; ++part)
 #pragma unroll
-        for (int t = 0; t < NI; ++t) F::mma(acc[t], lo[s & 1], x[s % 3][t]);
+        for (int t = 0; t < NI; ++t) F::mma(SP == 3 && part ? low[t] : acc[t], sp[s & 1][part], x[s % 3][t]);
     };
     const auto from_pairs = [&] {
 #pragma unroll
-      for (int part = 0; part < PARTS; ++part)
+      for (int part = 0; part < PP; ++part)
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
           for (int t = 0; t < NI; ++t)
-            if (R::needed(t, j, REV)) F::mma(in[t], zf[j], pf[R::slot(t, j, REV)][part]);
+            if (R::needed(t, j, REV)) F::mma(in[t], zf[j], pf[part][R::slot(t, j, REV)]);
     };
     // z with each token's factor, as an operand
     const auto scaled = [&](auto guard) {
@@ -578,7 +617,7 @@ template <typename T, int KW, bool OUT, bool REV, bool DOTS> __device__ __forcei
             const bool there = !decltype(guard)::value || F::K * j + 16 * t + g4 + r < valid;  // (0 times what is not finite)
             v[t][r] = rounded(there ? F::get(zf[j], t, r) * cf[j][t][r] : 0.f);
           }
-        split(v, zh[j], zl[j]);
+        split(v, zs[j]);
       }
     };
     if constexpr (OUT) {
@@ -600,16 +639,16 @@ template <typename T, int KW, bool OUT, bool REV, bool DOTS> __device__ __forcei
     if constexpr (OUT) {
       // ---- what the state gives
 #pragma unroll
-      for (int t = 0; t < NI; ++t) acc[t] = in[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+      for (int t = 0; t < NI; ++t) acc[t] = low[t] = in[t] = zero;
       split_state(0);
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
         if (s + 2 < NS) read_x(s + 2);
-        else read_pairs(NS == 1 ? -1 : s + 2 - NS);
+        else if (s + 2 - NS < PP) read_pairs(s + 2 - NS);
         __builtin_amdgcn_sched_barrier(0);
         if (s + 1 < NS) split_state(s + 1);
         from_state(s);
-        interleave<T, 0, PARTS * NI, 3>();
+        interleave<T, 0, SP * NI, 3>();
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -619,7 +658,7 @@ template <typename T, int KW, bool OUT, bool REV, bool DOTS> __device__ __forcei
     // ---- what the chunk's pairs give
     if constexpr (OUT) from_pairs();
     scaled(std::false_type{});
-    if constexpr (OUT) interleave<T, 0, R::SLOTS * PARTS, 9>();
+    if constexpr (OUT) interleave<T, 0, R::SLOTS * PP, 9>();
     if (__builtin_expect(odd, 0)) {
       scaled(std::true_type{});
       if constexpr (OUT) {
@@ -635,10 +674,10 @@ template <typename T, int KW, bool OUT, bool REV, bool DOTS> __device__ __forcei
         for (int t = 0; t < NI; ++t) {
           in[t] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int part = 0; part < PARTS; ++part)
+          for (int part = 0; part < PP; ++part)
 #pragma unroll
             for (int j = 0; j < NJ; ++j)
-              if (R::needed(t, j, REV)) F::mma(in[t], zf[j], *reinterpret_cast<const Frag*>(pairs + (R::slot(t, j, REV) * PARTS + part) * 1024));
+              if (R::needed(t, j, REV)) F::mma(in[t], zf[j], pair_block(t, j, part));
         }
         const T* zp = head_of<T>(ro.z, p, k.h) + n0 + g4;
 #pragma unroll 1
@@ -649,8 +688,11 @@ template <typename T, int KW, bool OUT, bool REV, bool DOTS> __device__ __forcei
           for (int t = 0; t < NI; ++t) {
             const int i = 16 * t + l16;
             if (REV ? j < i : j > i) continue;
-            const T* q = reinterpret_cast<const T*>(pairs + R::slot(t, j / F::K, REV) * PARTS * 1024 + 16 * (16 * from + l16 - lane)) + 4 * tile + e;
-            const float w = to_f32(q[0]) + (PARTS == 2 ? to_f32(q[1024 / sizeof(T)]) : 0.f);
+            const bool half = R::half(t, j / F::K, REV);
+            const T* q = reinterpret_cast<const T*>(pairs + R::block(t, j / F::K, REV) + (half ? 8 : 16) * (16 * from + l16)) + (half ? 0 : 4 * tile) + e;
+            float w = 0.f;
+#pragma unroll
+            for (int part = 0; part < PP; ++part) w += to_f32(q[part * (half ? 512 : 1024) / sizeof(T)]);
 #pragma unroll
             for (int r = 0; r < 4; ++r)
               if (!is_finite(z[r])) in[t][r] += w * z[r];
@@ -668,16 +710,16 @@ template <typename T, int KW, bool OUT, bool REV, bool DOTS> __device__ __forcei
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) F::mma(st[i], yf[i & 3][j], zh[j]);
-      if (PARTS == 2)
+      for (int part = 0; part < ZP; ++part)
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) F::mma(st[i], yf[i & 3][j], zl[j]);
+        for (int j = 0; j < NJ; ++j) F::mma(st[i], yf[i & 3][j], zs[j][part]);
       if (i + 4 < NT) read_y(i + 4);
     }
     if constexpr (OUT) {
       float d[2 * NI];  // what w makes of them: by the state, by the pairs
 #pragma unroll
       for (int t = 0; t < NI; ++t) {
+        if (SP == 3) acc[t] += low[t];
         acc[t] *= rf[t];
         if constexpr (DOTS) {
           d[t] = d[NI + t] = 0.f;
@@ -734,7 +776,7 @@ template <typename T, int KW, bool OUT, bool REV, bool DOTS> __device__ __forcei
   }
 }
 
-template <typename T, int KW, bool OUT> __global__ __launch_bounds__(WALK_THREADS) void decay_walk_kernel(Walk a) {
+template <typename T, int KW, bool OUT, bool BWD> __global__ __launch_bounds__(WALK_THREADS) void decay_walk_kernel(Walk a) {
   typedef Room<T, KW, OUT> R;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   // workgroups of one (slot, head) follow each other on one XCD, whose L2 then holds what they share
@@ -764,9 +806,9 @@ template <typename T, int KW, bool OUT> __global__ __launch_bounds__(WALK_THREAD
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) - 4;
     if (ro.rev) pair_wave<T, KW, OUT, true>(wave, a, ro, k, lds);
     else pair_wave<T, KW, OUT, false>(wave, a, ro, k, lds);
-  } else if (OUT && ro.dots) {
-    if (ro.rev) walk_state<T, KW, OUT, true, OUT>(a, ro, k, lds);
-    else walk_state<T, KW, OUT, false, OUT>(a, ro, k, lds);
+  } else if (BWD && ro.dots) {
+    if (ro.rev) walk_state<T, KW, OUT, true, BWD>(a, ro, k, lds);
+    else walk_state<T, KW, OUT, false, BWD>(a, ro, k, lds);
   } else {
     if (ro.rev) walk_state<T, KW, OUT, true, false>(a, ro, k, lds);
     else walk_state<T, KW, OUT, false, false>(a, ro, k, lds);
@@ -1065,8 +1107,8 @@ Walk walk(const lnx_decay_args* a, const Layout& l) {
   return k;
 }
 
-template <typename T, int KW, bool OUT> int start(const Walk& k, const char* name, hipStream_t st) {
-  const auto kernel = decay_walk_kernel<T, KW, OUT>;
+template <typename T, int KW, bool OUT, bool BWD> int start(const Walk& k, const char* name, hipStream_t st) {
+  const auto kernel = decay_walk_kernel<T, KW, OUT, BWD>;
   constexpr int bytes = Room<T, KW, OUT>::BYTES;
   static_assert(bytes <= 160 * 1024, "LDS of a CU");
   if (int rc = lnx_lds_limit(reinterpret_cast<const void*>(kernel), bytes)) return rc;
@@ -1074,13 +1116,13 @@ template <typename T, int KW, bool OUT> int start(const Walk& k, const char* nam
   hipLaunchKernelGGL(kernel, dim3((unsigned)((int64_t)k.units * k.per)), dim3(WALK_THREADS), bytes, st, k);
   return LNX_OK;
 }
-template <typename T, bool OUT> int start(Walk& k, int roles, const char* name, hipStream_t st) {
+template <typename T, bool OUT, bool BWD> int start(Walk& k, int roles, const char* name, hipStream_t st) {
   k.per = 0;
   int kw = 0;  // the widest of the launch's keys
   for (int i = 0; i < roles; ++i) k.per += k.role[i].slabs, kw = kw < k.role[i].kw ? k.role[i].kw : kw;
-  if (kw <= 64) return start<T, 64, OUT>(k, name, st);
-  if (kw <= 128) return start<T, 128, OUT>(k, name, st);
-  return start<T, 256, OUT>(k, name, st);
+  if (kw <= 64) return start<T, 64, OUT, BWD>(k, name, st);
+  if (kw <= 128) return start<T, 128, OUT, BWD>(k, name, st);
+  return start<T, 256, OUT, BWD>(k, name, st);
 }
 
 void join(const lnx_decay_args* a, const Layout& l, float* states, const float* whole, const float* init, bool rev, hipStream_t st) {
@@ -1100,13 +1142,13 @@ template <typename T> int forward(const lnx_decay_args* a, hipStream_t st) {
     k.whole = reinterpret_cast<float*>(ws);
     k.role[0] = r;
     k.role[0].fin = states;
-    if (int rc = start<T, false>(k, 1, "decay_local", st)) return rc;
+    if (int rc = start<T, false, false>(k, 1, "decay_local", st)) return rc;
     join(a, l, states, k.whole, a->initial_state, false, st);
     r.init = states;
   }
   r.fin = a->final_state;
   k.role[0] = r;
-  return start<T, true>(k, 1, "decay_fwd", st);
+  return start<T, true, false>(k, 1, "decay_fwd", st);
 }
 
 template <typename T> int backward(const lnx_decay_args* a, hipStream_t st) {
@@ -1124,7 +1166,7 @@ template <typename T> int backward(const lnx_decay_args* a, hipStream_t st) {
     k.whole = reinterpret_cast<float*>(ws + ceil_div(l.dots + l.part, 16) * 16);
     k.role[0] = v;
     k.role[0].fin = states;
-    if (int rc = start<T, false>(k, 1, "decay_local", st)) return rc;
+    if (int rc = start<T, false, false>(k, 1, "decay_local", st)) return rc;
     join(a, l, states, k.whole, a->d_final_state, true, st);
     kk.init = v.init = states;
   }
@@ -1133,11 +1175,11 @@ template <typename T> int backward(const lnx_decay_args* a, hipStream_t st) {
   const auto step = [](int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; };
   k.role[0] = q, k.role[1] = kk, k.role[2] = v;
   if (step(wide) == step(narrow)) {
-    if (int rc = start<T, true>(k, 3, "decay_bwd", st)) return rc;
+    if (int rc = start<T, true, true>(k, 3, "decay_bwd", st)) return rc;
   } else {
-    if (int rc = start<T, true>(k, 2, "decay_bwd_qk", st)) return rc;
+    if (int rc = start<T, true, true>(k, 2, "decay_bwd_qk", st)) return rc;
     k.role[0] = v;
-    if (int rc = start<T, true>(k, 1, "decay_bwd_v", st)) return rc;
+    if (int rc = start<T, true, false>(k, 1, "decay_bwd_v", st)) return rc;
   }
   GateGrad d{};
   d.dots_q = q.dots, d.dots_k = kk.dots, d.fin = a->final_state, d.d_fin = a->d_final_state, d.cu = a->cu_seqlens;
