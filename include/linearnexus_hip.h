@@ -577,8 +577,8 @@ int lnx_attn_step_paged(const lnx_attn_step_paged_args* a, void* hip_stream);
  * d_g is dense [B, H, T], or [H], the sums over rows and tokens, with g_per_head.  States [B, H, dk, dv] ([nseq, H, dk, dv] packed) dense fp32;
  * initial_state, d_final_state (zeros) and d_initial_state may be NULL.  The forward call leaves in `kept` what the backward call reads (NULL:
  * no backward pass will follow; lnx_decay_kept_bytes may be 0); the backward call reads the forward call's inputs, `kept`, and final_state where d_final_state
- * is given.  The workspace (16-byte aligned, may be NULL where its size is 0; the forward size depends on whether kept is set) holds nothing between
- * calls.  No atomics.
+ * is given.  The workspace (16-byte aligned, may be NULL where its size is 0; the forward size depends on whether kept is set, the backward
+ * size on whether initial_state and d_initial_state are) holds nothing between calls.  No atomics.
  */
 typedef struct lnx_decay_args {
   int32_t B, H, T, dk, dv, nseq, dtype, g_per_head;

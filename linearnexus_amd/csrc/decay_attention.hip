@@ -219,7 +219,7 @@ struct Spot {
   int64_t tok;
   bool on, first, last;
 };
-__device__ __forceinline__ Spot spot(const Walk& a, int slot) {
+template <typename A> __device__ __forceinline__ Spot spot(const A& a, int slot) {
   Spot s;
   if (!a.nseq) {
     s.b = s.row = slot / a.nseg;
@@ -859,36 +859,45 @@ __global__ __launch_bounds__(JOIN_THREADS) void decay_join_kernel(Join a) {
 //   dg_t = sum_{s >= t} (x_s + u_s) + sum_{r < t} y_r + Z     Z = W - sum y     W before the chunk = Z + sum x
 // x: what a token's outputs took from the state before the chunk, y: what its key hands to the state behind it, u: its pairs as a query less those as
 // a key.  A strong decay makes x, y and Z small, and they are summed apart from the pairs, which cancel over a chunk.
+// W is known at both ends of a segment, from the states there.  Walked from its end the sums miss it at its beginning by what their terms were off, which
+// for a slow decay is a drift; that is taken back evenly over the tokens (H8 T4096 d128: dg off by 1.1e-6 -> 3.4e-7 against 64 bits).
 struct GateGrad {
   const float *dots_q, *dots_k;  // [inter, pairs][slab][B H][T]
-  const float *fin, *d_fin;
+  const float *init, *d_init, *fin, *d_fin;  // of rows, or NULL
+  const float *before, *behind;  // of segments: the state before each, the state's gradient behind it
   const int32_t* cu;
-  float *dg, *part;  // part: sums over a row, [row][H]
-  int B, H, T, nseq, slabs;
+  float *dg, *part;  // part: sums over a segment, [slot][H]
+  int B, H, T, nseq, slabs, seg, nseg;
   int64_t step, size;
 };
 template <int C> __global__ __launch_bounds__(GATE_THREADS) void decay_gate_grad_kernel(GateGrad a) {
-  constexpr int NC = GATE_THREADS / C;
-  __shared__ float chunk[2][NC], red[16];
-  const int row = blockIdx.x / a.H, h = blockIdx.x % a.H, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, in = lane % C, mine = threadIdx.x / C;
-  int from = 0, len = a.T;
-  if (a.nseq) from = seq_first(a.cu, row, a.T), len = seq_end(a.cu, row, a.T) - from;
-  const int64_t base = (int64_t)((a.nseq ? 0 : row) * a.H + h) * a.T + from;
-  const auto block_sum = [&](float x) {
-    x = wave_sum(x);
+  constexpr int NC = GATE_THREADS / C, U = 4;  // chunks of a turn; turns whose dots are fetched together
+  __shared__ double chunk[2][NC], red[16];
+  const int slot = blockIdx.x / a.H, h = blockIdx.x % a.H, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, in = lane % C, mine = threadIdx.x / C;
+  const Spot p = spot(a, slot);
+  if (!p.on) {
+    if (a.part && threadIdx.x == 0) a.part[(int64_t)slot * a.H + h] = 0.f;
+    return;
+  }
+  const int len = p.len;
+  const int64_t base = (int64_t)(p.b * a.H + h) * a.T + p.tok;
+  const auto block_sum = [&](double x) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o, LNX_WAVE);
     __syncthreads();
     if (lane == 0) red[wave] = x;
     __syncthreads();
-    float s = 0.f;
+    double s = 0.;
     for (int i = 0; i < 16; ++i) s += red[i];
     return s;
   };
-  float W = 0.f;
-  if (a.d_fin) {
-    const int64_t at = ((int64_t)row * a.H + h) * a.size;
-    for (int64_t i = threadIdx.x; i < a.size; i += GATE_THREADS) W += a.fin[at + i] * a.d_fin[at + i];
-    W = block_sum(W);
-  }
+  const auto product = [&](const float* s, const float* d, int64_t i, int64_t j) {  // of two states, this thread's part
+    float w = 0.f;
+    if (s && d)
+      for (int64_t e = threadIdx.x; e < a.size; e += GATE_THREADS) w += s[(i * a.H + h) * a.size + e] * d[(j * a.H + h) * a.size + e];
+    return (double)w;
+  };
+  float x[U], y[U], u[U];
   const auto get = [&](int t, float& x, float& y, float& u) {
     x = y = u = 0.f;
     if (t < 0 || t >= len) return;
@@ -898,39 +907,63 @@ template <int C> __global__ __launch_bounds__(GATE_THREADS) void decay_gate_grad
       u += a.dots_q[(a.slabs + s) * a.step + base + t] - a.dots_k[(a.slabs + s) * a.step + base + t];
     }
   };
-  float sum = 0.f, x, y, u, nx, ny, nu;
-  int t = (len - 1) / GATE_THREADS * GATE_THREADS + threadIdx.x;
-  get(t, x, y, u);
-  for (int turn = 0; t > -GATE_THREADS + (int)threadIdx.x; t -= GATE_THREADS, turn ^= 1) {
-    get(t - GATE_THREADS, nx, ny, nu);
-    float sx = x, su = u, py = y;
+  const auto fetch = [&](int t) {
 #pragma unroll
-    for (int o = 1; o < C; o <<= 1) {
-      const float bx = __shfl_down(sx, o, LNX_WAVE), bu = __shfl_down(su, o, LNX_WAVE), by = __shfl_up(py, o, LNX_WAVE);
-      if (in + o < C) sx += bx, su += bu;
-      if (in >= o) py += by;
+    for (int i = 0; i < U; ++i) get(t - i * GATE_THREADS, x[i], y[i], u[i]);
+  };
+  const int top = len > 0 ? (len - 1) / GATE_THREADS * GATE_THREADS + (int)threadIdx.x : (int)threadIdx.x;
+  fetch(top);
+  double off = 0.;
+#pragma unroll
+  for (int i = 0; i < U; ++i) off += x[i] - y[i];
+  for (int t = top - U * GATE_THREADS; t >= 0; t -= GATE_THREADS) {
+    float nx, ny, nu;
+    get(t, nx, ny, nu);
+    off += nx - ny;
+  }
+  const double end = p.last ? product(a.fin, a.d_fin, p.row, p.row) : product(a.before, a.behind, slot + 1, slot);
+  const double begin = p.first ? product(a.init, a.d_init, p.row, p.row) : product(a.before, a.behind, slot, slot - 1);
+  double W = block_sum(end);
+  off = block_sum(off + end - begin);
+  if (!is_finite((float)off)) off = 0.;
+  const double drift = len > 0 ? off / len : 0.;
+  float sum = 0.f;
+  for (int t = top, turn = 0; t - (int)threadIdx.x >= 0 || turn == 0; t -= U * GATE_THREADS) {
+    if (turn) fetch(t);
+#pragma unroll
+    for (int i = 0; i < U; ++i, ++turn) {
+      const int ti = t - i * GATE_THREADS;
+      if (ti - (int)threadIdx.x < 0) break;  // (of the workgroup)
+      float sx = x[i], su = u[i], py = y[i];
+#pragma unroll
+      for (int o = 1; o < C; o <<= 1) {
+        const float bx = __shfl_down(sx, o, LNX_WAVE), bu = __shfl_down(su, o, LNX_WAVE), by = __shfl_up(py, o, LNX_WAVE);
+        if (in + o < C) sx += bx, su += bu;
+        if (in >= o) py += by;
+      }
+      const float X = __shfl(sx, lane - in, LNX_WAVE), Y = __shfl(py, lane - in + C - 1, LNX_WAVE);
+      if (in == 0) chunk[turn & 1][mine] = (double)X - Y;
+      __syncthreads();
+      double behind = W;
+#pragma unroll 8
+      for (int j = NC - 1; j >= 0; --j) {
+        if (j == mine) behind = W;
+        W += chunk[turn & 1][j];
+      }
+      const float Z = (float)(behind - max(0, len - (ti - in + C)) * drift - Y);
+      const float d = sx + su + (py - y[i]) + Z;
+      if (ti < len) {
+        if (a.dg) a.dg[base + ti] = d;
+        sum += d;
+      }
     }
-    const float X = __shfl(sx, lane - in, LNX_WAVE), Y = __shfl(py, lane - in + C - 1, LNX_WAVE);
-    if (in == 0) chunk[turn][mine] = X - Y;
-    __syncthreads();
-    float behind = W;
-    for (int i = NC - 1; i >= 0; --i) {
-      if (i == mine) behind = W;
-      W += chunk[turn][i];
-    }
-    const float d = sx + su + (py - y) + (behind - Y);
-    if (t < len) {
-      if (a.dg) a.dg[base + t] = d;
-      sum += d;
-    }
-    x = nx, y = ny, u = nu;
   }
   if (a.part) {
-    sum = block_sum(sum);
-    if (threadIdx.x == 0) a.part[(int64_t)row * a.H + h] = sum;
+    const double s = block_sum(sum);
+    if (threadIdx.x == 0) a.part[(int64_t)slot * a.H + h] = (float)s;
   }
 }
-// dg[h] = sum of the rows' sums
+// dg[h] = sum of the segments' sums
 __global__ __launch_bounds__(256) void decay_gate_sum_kernel(const float* part, int64_t rows, int H, float* dg) {
   __shared__ float red[4];
   float s = 0.f;
@@ -1033,7 +1066,8 @@ int segment(const lnx_decay_args* a) {
 }
 struct Layout {
   int seg, nseg;
-  int64_t slots, states, factors, dots, part, rows;  // bytes: states of all segments, their factors, the walks' dots, rows' sums
+  int64_t slots, rows;
+  int64_t states, factors, dots, part, d_init;  // bytes: states of all segments, their factors, the walks' dots, segments' sums, gradients of the initial states that the caller does not want
 };
 Layout layout(const lnx_decay_args* a) {
   Layout l{};
@@ -1044,7 +1078,8 @@ Layout layout(const lnx_decay_args* a) {
   l.slots = a->nseq ? a->T / l.seg + a->nseq : (int64_t)a->B * l.nseg;
   if (s) l.states = l.slots * a->H * a->dk * a->dv * 4, l.factors = ceil_div(l.slots * a->H * 4, 16) * 16;
   l.dots = ceil_div(4 * ceil_div(a->dk, SLAB) * a->B * a->H * (int64_t)a->T * 4, 16) * 16;
-  l.part = l.rows * a->H * 4;
+  l.part = l.slots * a->H * 4;
+  if (a->initial_state && !a->d_initial_state) l.d_init = l.rows * a->H * a->dk * a->dv * 4;
   return l;
 }
 
@@ -1061,7 +1096,7 @@ int check(const char* what, const lnx_decay_args* a, bool bwd) {
   if (a->B == 0) return LNX_OK;
   const Layout l = layout(a);
   const int64_t walks = l.slots * a->H * (bwd ? 2 * ceil_div(a->dk, SLAB) + ceil_div(a->dv, SLAB) : ceil_div(a->dv, SLAB));
-  if (walks > MAX_GRID / WALK_THREADS || l.rows * a->H > MAX_GRID / (bwd ? GATE_THREADS : JOIN_THREADS)) return lnx_set_error(LNX_ERR_SHAPE, "%s: too many rows", what);
+  if (walks > MAX_GRID / WALK_THREADS || (bwd ? l.slots * a->H > MAX_GRID / GATE_THREADS : l.rows * a->H > MAX_GRID / JOIN_THREADS)) return lnx_set_error(LNX_ERR_SHAPE, "%s: too many rows", what);
   if (!bwd && !a->final_state) return lnx_set_error(LNX_ERR_NULL, "%s: final_state is required", what);
   if (bwd && a->d_final_state && !a->final_state) return lnx_set_error(LNX_ERR_NULL, "%s: d_final_state needs final_state", what);
   if (bwd && !a->d_g) return lnx_set_error(LNX_ERR_NULL, "%s: d_g is required", what);
@@ -1161,16 +1196,18 @@ template <typename T> int backward(const lnx_decay_args* a, hipStream_t st) {
   q.dots = reinterpret_cast<float*>(ws), kk.dots = q.dots + 2 * q.slabs * k.dots_step;
   q.init = l.states ? a->kept : a->initial_state;
   kk.init = v.init = a->d_final_state;
+  int64_t at = ceil_div(l.dots + l.part, 16) * 16;
+  float* states = nullptr;
   if (l.states) {
-    float* states = reinterpret_cast<float*>(ws + ceil_div(l.dots + l.part, 16) * 16 + l.factors);
-    k.whole = reinterpret_cast<float*>(ws + ceil_div(l.dots + l.part, 16) * 16);
+    k.whole = reinterpret_cast<float*>(ws + at), at += l.factors;
+    states = reinterpret_cast<float*>(ws + at), at += l.states;
     k.role[0] = v;
     k.role[0].fin = states;
     if (int rc = start<T, false, false>(k, 1, "decay_local", st)) return rc;
     join(a, l, states, k.whole, a->d_final_state, true, st);
     kk.init = v.init = states;
   }
-  v.fin = a->d_initial_state;
+  v.fin = l.d_init ? reinterpret_cast<float*>(ws + at) : a->d_initial_state;
   const int wide = a->dk > a->dv ? a->dk : a->dv, narrow = a->dk + a->dv - wide;
   const auto step = [](int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; };
   k.role[0] = q, k.role[1] = kk, k.role[2] = v;
@@ -1182,17 +1219,18 @@ template <typename T> int backward(const lnx_decay_args* a, hipStream_t st) {
     if (int rc = start<T, true, false>(k, 1, "decay_bwd_v", st)) return rc;
   }
   GateGrad d{};
-  d.dots_q = q.dots, d.dots_k = kk.dots, d.fin = a->final_state, d.d_fin = a->d_final_state, d.cu = a->cu_seqlens;
+  d.dots_q = q.dots, d.dots_k = kk.dots, d.init = a->initial_state, d.d_init = v.fin, d.fin = a->final_state, d.d_fin = a->d_final_state, d.cu = a->cu_seqlens;
+  d.before = a->kept, d.behind = states, d.seg = l.seg, d.nseg = l.nseg;
   if (a->g_per_head) d.part = reinterpret_cast<float*>(ws + l.dots);
   else d.dg = a->d_g;
   d.B = a->B, d.H = a->H, d.T = a->T, d.nseq = a->nseq, d.slabs = q.slabs, d.step = k.dots_step, d.size = (int64_t)a->dk * a->dv;
   lnx_profile_mark("decay_gate_grad", st);
-  const dim3 rows((unsigned)(l.rows * a->H));
-  if (q.kw <= 128) decay_gate_grad_kernel<chunk_of<T, 128>()><<<rows, GATE_THREADS, 0, st>>>(d);
-  else decay_gate_grad_kernel<chunk_of<T, 256>()><<<rows, GATE_THREADS, 0, st>>>(d);
+  const dim3 grid((unsigned)(l.slots * a->H));
+  if (q.kw <= 128) decay_gate_grad_kernel<chunk_of<T, 128>()><<<grid, GATE_THREADS, 0, st>>>(d);
+  else decay_gate_grad_kernel<chunk_of<T, 256>()><<<grid, GATE_THREADS, 0, st>>>(d);
   if (a->g_per_head) {
     lnx_profile_mark("decay_gate_sum", st);
-    decay_gate_sum_kernel<<<dim3((unsigned)a->H), 256, 0, st>>>(d.part, l.rows, a->H, a->d_g);
+    decay_gate_sum_kernel<<<dim3((unsigned)a->H), 256, 0, st>>>(d.part, l.slots, a->H, a->d_g);
   }
   return LNX_OK;
 }
@@ -1219,7 +1257,7 @@ extern "C" uint64_t lnx_decay_fwd_workspace_bytes(const lnx_decay_args* a) {
 extern "C" uint64_t lnx_decay_bwd_workspace_bytes(const lnx_decay_args* a) {
   if (!sizes(a)) return 0;
   const Layout l = layout(a);
-  return ceil_div(l.dots + l.part, 16) * 16 + l.factors + l.states;
+  return ceil_div(l.dots + l.part, 16) * 16 + l.factors + l.states + l.d_init;
 }
 extern "C" int lnx_decay_fwd(const lnx_decay_args* a, void* hip_stream) {
   if (int rc = check("decay_fwd", a, false)) return rc;
