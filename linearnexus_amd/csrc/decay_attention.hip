@@ -269,21 +269,21 @@ template <typename T> __device__ __forceinline__ const T* head_of(const Side& s,
   return static_cast<const T*>(s.p) + p.b * s.sb + h * s.sh + p.tok * s.st;
 }
 
-// bf16 parts of an operand that is not one of the inputs.  What a token adds to the state: three, exact as fp32 is.  The state as an operand: three
-// where dg is taken from the results, two where they are rounded to bf16.  Pairs: two.  (Errors against 64 bits at H8 T4096 d128, everything
-// in two parts -> thus: states 2.4e-6 -> 2.2e-7, dg 8.8e-6 -> 1.0e-6; pairs in three too: dg 1.0e-6.  B8 H16 T4096, us: forward 151 -> 165,
-// backward 530 -> 620, 650 with the pairs.)
+// bf16 parts of an operand that is not one of the inputs.  What a token adds to the state: three, exact as fp32 is.  The state as an operand and the
+// pairs: three where dg is taken from the results, two where they are rounded to bf16.  (Errors against 64 bits, all in two parts -> thus: states
+// of H8 T4096 d128 2.4e-6 -> 2.2e-7, dg 1.4e-6 -> 2.2e-7 by the state's; dg per head of B10 H3 T40 6.3e-6 -> 2.9e-7 by the pairs'.  B8 H16 T4096, us:
+// forward 151 -> 165, backward 530 -> 650, 575 without the state's third part, 620 without the pairs'.)
 template <typename T> constexpr int parts_of_z() { return sizeof(T) == 2 ? 3 : 1; }
 template <typename T> constexpr int parts_of_state(bool dots) { return sizeof(T) == 2 ? (dots ? 3 : 2) : 1; }
-template <typename T> constexpr int parts_of_pairs() { return sizeof(T) == 2 ? 2 : 1; }
+template <typename T> constexpr int parts_of_pairs(bool dots) { return sizeof(T) == 2 ? (dots ? 3 : 2) : 1; }
 
-// LDS of a walk.  OUT: false for the local walks of segments, which leave what a segment adds to the state and nothing else.
-template <typename T, int KW, bool OUT> struct Room {
+// LDS of a walk.  OUT: false for the local walks of segments, which leave what a segment adds to the state and nothing else.  BWD: walks with dots among them.
+template <typename T, int KW, bool OUT, bool BWD> struct Room {
   static constexpr int C = chunk_of<T, KW>(), NI = C / 16, NJ = C / Form<T>::K;
   // Pairs lie in LDS as operands, in blocks of 16 rows x K: those that have any, of bf16 in half a block where only one of its two tiles has
   static constexpr bool needed(int i, int j, bool rev) { return rev ? Form<T>::K * (j + 1) > 16 * i : Form<T>::K * j <= 16 * i + 15; }
   static constexpr bool half(int i, int j, bool rev) { return Form<T>::TP == 2 && (rev ? 2 * j < i : 2 * j + 1 > i); }
-  static constexpr int P = parts_of_pairs<T>();
+  static constexpr int P = parts_of_pairs<T>(BWD);
   static constexpr int block(int i, int j, bool rev) {  // where block (i, j) begins
     int at = 0;
     for (int b = 0; b < i * NJ + j; ++b)
@@ -334,11 +334,11 @@ template <typename T, int READS, int MFMAS, int VALUS> __device__ __forceinline_
 
 // Four of a walk's eight waves: they bring chunk c + 1 to LDS and form the decays and the pairs of chunk c, one tile of 16 rows each, while
 // the others walk chunk c - 1.  One barrier a chunk.
-template <typename T, int KW, bool OUT, bool REV, int W> __device__ __forceinline__ void walk_pairs(const Walk& a, const Role& ro, const Task& k, char* lds) {
+template <typename T, int KW, bool OUT, bool REV, bool BWD, int W> __device__ __forceinline__ void walk_pairs(const Walk& a, const Role& ro, const Task& k, char* lds) {
   typedef Form<T> F;
   typedef typename F::Frag Frag;
   typedef Cells<T, KW> XC;
-  typedef Room<T, KW, OUT> R;
+  typedef Room<T, KW, OUT, BWD> R;
   constexpr int C = R::C, NS = KW / F::K;
   constexpr int wave = W, UNITS = R::units(W);
   const int lane = threadIdx.x & 63, l16 = lane & 15, g4 = 4 * (lane >> 4);
@@ -491,21 +491,21 @@ template <typename T, int KW, bool OUT, bool REV, int W> __device__ __forceinlin
   if (!OUT && k.item == 0 && threadIdx.x == 448) a.whole[(int64_t)k.slot * a.H + k.h] = between(whole_h, whole_l, 0.f, 0.f);
 }
 
-template <typename T, int KW, bool OUT, bool REV> __device__ __forceinline__ void pair_wave(int wave, const Walk& a, const Role& ro, const Task& k, char* lds) {
-  if (wave == 0) walk_pairs<T, KW, OUT, REV, 0>(a, ro, k, lds);
-  else if (wave == 1) walk_pairs<T, KW, OUT, REV, 1>(a, ro, k, lds);
-  else if (wave == 2) walk_pairs<T, KW, OUT, REV, 2>(a, ro, k, lds);
-  else walk_pairs<T, KW, OUT, REV, 3>(a, ro, k, lds);
+template <typename T, int KW, bool OUT, bool REV, bool BWD> __device__ __forceinline__ void pair_wave(int wave, const Walk& a, const Role& ro, const Task& k, char* lds) {
+  if (wave == 0) walk_pairs<T, KW, OUT, REV, BWD, 0>(a, ro, k, lds);
+  else if (wave == 1) walk_pairs<T, KW, OUT, REV, BWD, 1>(a, ro, k, lds);
+  else if (wave == 2) walk_pairs<T, KW, OUT, REV, BWD, 2>(a, ro, k, lds);
+  else walk_pairs<T, KW, OUT, REV, BWD, 3>(a, ro, k, lds);
 }
 
 // The other four: 16 columns of the state and of the results each.
-template <typename T, int KW, bool OUT, bool REV, bool DOTS> __device__ __forceinline__ void walk_state(const Walk& a, const Role& ro, const Task& k, char* lds) {
+template <typename T, int KW, bool OUT, bool REV, bool BWD, bool DOTS> __device__ __forceinline__ void walk_state(const Walk& a, const Role& ro, const Task& k, char* lds) {
   typedef Form<T> F;
   typedef typename F::Frag Frag;
   typedef Cells<T, KW> XC;
   typedef Cells<T, SLAB> ZC;
-  typedef Room<T, KW, OUT> R;
-  constexpr int C = R::C, NI = R::NI, NJ = R::NJ, NS = KW / F::K, NT = KW / 16, TP = F::TP, ZP = parts_of_z<T>(), PP = R::P, SP = parts_of_state<T>(DOTS);
+  typedef Room<T, KW, OUT, BWD> R;
+  constexpr int C = R::C, NI = R::NI, NJ = R::NJ, NS = KW / F::K, NT = KW / 16, TP = F::TP, ZP = parts_of_z<T>(), PP = parts_of_pairs<T>(DOTS), SP = parts_of_state<T>(DOTS);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g4 = 4 * (lane >> 4), n0 = k.col0 + 16 * wave;
   const Spot& p = k.p;
   const unsigned lds0 = lds_byte_addr(lds);
@@ -556,8 +556,8 @@ template <typename T, int KW, bool OUT, bool REV, bool DOTS> __device__ __forcei
     const float* f = reinterpret_cast<const float*>(lds + R::FACTORS) + 256 * (it & 1);
     const unsigned xr = xa + at, yc = ya + at, zc = za + at;
     const char* pairs = lds + R::PAIRS + (it & 1) * R::PAIRB;
-    // What LDS holds is read well ahead of its use: two steps of x, all pairs, four tiles of y
-    Frag zf[NJ], zs[NJ][ZP], x[3][NI], sp[2][SP], pf[PP][R::SLOTS], yf[4][NJ];
+    // What LDS holds is read well ahead of its use: two steps of x, two parts of the pairs, four tiles of y
+    Frag zf[NJ], zs[NJ][ZP], x[3][NI], sp[2][SP], pf[2][R::SLOTS], yf[4][NJ];
     floatx4 acc[NI], low[NI], in[NI], cf[NJ][TP];  // low: of the state's lower parts, summed apart so that their sums are not rounded at the whole's
     const auto read_x = [&](int s) {
 #pragma unroll
@@ -578,7 +578,7 @@ template <typename T, int KW, bool OUT, bool REV, bool DOTS> __device__ __forcei
       for (int t = 0; t < NI; ++t)
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
-          if (R::needed(t, j, REV)) pf[part][R::slot(t, j, REV)] = pair_block(t, j, part);
+          if (R::needed(t, j, REV)) pf[part % 2][R::slot(t, j, REV)] = pair_block(t, j, part);
     };
     const auto read_y = [&](int i) {
 #pragma unroll
@@ -598,12 +598,14 @@ template <typename T, int KW, bool OUT, bool REV, bool DOTS> __device__ __forcei
     };
     const auto from_pairs = [&] {
 #pragma unroll
-      for (int part = 0; part < PP; ++part)
+      for (int part = 0; part < PP; ++part) {
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
           for (int t = 0; t < NI; ++t)
-            if (R::needed(t, j, REV)) F::mma(in[t], zf[j], pf[part][R::slot(t, j, REV)]);
+            if (R::needed(t, j, REV)) F::mma(in[t], zf[j], pf[part % 2][R::slot(t, j, REV)]);
+        if (part + 2 < PP) read_pairs(part + 2);
+      }
     };
     // z with each token's factor, as an operand
     const auto scaled = [&](auto guard) {
@@ -777,7 +779,7 @@ template <typename T, int KW, bool OUT, bool REV, bool DOTS> __device__ __forcei
 }
 
 template <typename T, int KW, bool OUT, bool BWD> __global__ __launch_bounds__(WALK_THREADS) void decay_walk_kernel(Walk a) {
-  typedef Room<T, KW, OUT> R;
+  typedef Room<T, KW, OUT, BWD> R;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   // workgroups of one (slot, head) follow each other on one XCD, whose L2 then holds what they share
   const int w = blockIdx.x;
@@ -804,14 +806,14 @@ template <typename T, int KW, bool OUT, bool BWD> __global__ __launch_bounds__(W
   }
   if (threadIdx.x >= 256) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) - 4;
-    if (ro.rev) pair_wave<T, KW, OUT, true>(wave, a, ro, k, lds);
-    else pair_wave<T, KW, OUT, false>(wave, a, ro, k, lds);
+    if (ro.rev) pair_wave<T, KW, OUT, true, BWD>(wave, a, ro, k, lds);
+    else pair_wave<T, KW, OUT, false, BWD>(wave, a, ro, k, lds);
   } else if (BWD && ro.dots) {
-    if (ro.rev) walk_state<T, KW, OUT, true, BWD>(a, ro, k, lds);
-    else walk_state<T, KW, OUT, false, BWD>(a, ro, k, lds);
+    if (ro.rev) walk_state<T, KW, OUT, true, BWD, BWD>(a, ro, k, lds);
+    else walk_state<T, KW, OUT, false, BWD, BWD>(a, ro, k, lds);
   } else {
-    if (ro.rev) walk_state<T, KW, OUT, true, false>(a, ro, k, lds);
-    else walk_state<T, KW, OUT, false, false>(a, ro, k, lds);
+    if (ro.rev) walk_state<T, KW, OUT, true, BWD, false>(a, ro, k, lds);
+    else walk_state<T, KW, OUT, false, BWD, false>(a, ro, k, lds);
   }
 }
 
@@ -860,7 +862,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void decay_join_kernel(Join a) {
 // x: what a token's outputs took from the state before the chunk, y: what its key hands to the state behind it, u: its pairs as a query less those as
 // a key.  A strong decay makes x, y and Z small, and they are summed apart from the pairs, which cancel over a chunk.
 // W is known at both ends of a segment, from the states there.  Walked from its end the sums miss it at its beginning by what their terms were off, which
-// for a slow decay is a drift; that is taken back evenly over the tokens (H8 T4096 d128: dg off by 1.1e-6 -> 3.4e-7 against 64 bits).
+// for a slow decay is a drift; that is taken back evenly over the tokens (H8 T4096 d128: dg off by 1.1e-6 -> 2.2e-7 against 64 bits).
 struct GateGrad {
   const float *dots_q, *dots_k;  // [inter, pairs][slab][B H][T]
   const float *init, *d_init, *fin, *d_fin;  // of rows, or NULL
@@ -1144,7 +1146,7 @@ Walk walk(const lnx_decay_args* a, const Layout& l) {
 
 template <typename T, int KW, bool OUT, bool BWD> int start(const Walk& k, const char* name, hipStream_t st) {
   const auto kernel = decay_walk_kernel<T, KW, OUT, BWD>;
-  constexpr int bytes = Room<T, KW, OUT>::BYTES;
+  constexpr int bytes = Room<T, KW, OUT, BWD>::BYTES;
   static_assert(bytes <= 160 * 1024, "LDS of a CU");
   if (int rc = lnx_lds_limit(reinterpret_cast<const void*>(kernel), bytes)) return rc;
   lnx_profile_mark(name, st);
