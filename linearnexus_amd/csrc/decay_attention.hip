@@ -836,23 +836,31 @@ __global__ __launch_bounds__(JOIN_THREADS) void decay_join_kernel(Join a) {
   }
   const int64_t e0 = ((int64_t)blockIdx.y * JOIN_THREADS + threadIdx.x) * 4;
   const int many = (int)min((int64_t)4, a.size - e0);
-  float s[4], add[4], next[4];
-  const auto at = [&](int i) { return a.states + ((slot + (a.rev ? n - 1 - i : i)) * a.H + h) * a.size + e0; };
+  constexpr int U = 4;  // segments fetched together
+  float s[4], add[U][4], f[U];
+  const auto segment = [&](int i) { return slot + (a.rev ? n - 1 - i : i); };
   const auto get = [&](float (&x)[4], const float* q) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = q && e < many ? q[e] : 0.f;
   };
   get(s, a.init ? a.init + ((int64_t)row * a.H + h) * a.size + e0 : nullptr);
-  get(add, n > 1 ? at(0) : nullptr);
-  for (int i = 0; i < n; ++i) {
-    get(next, i + 2 < n ? at(i + 1) : nullptr);
-    const float f = i + 1 < n ? a.whole[(slot + (a.rev ? n - 1 - i : i)) * a.H + h] : 0.f;
-    float* q = at(i);
+  for (int i0 = 0; i0 < n; i0 += U) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (e < many) q[e] = s[e];
-      s[e] = f * s[e] + add[e];
-      add[e] = next[e];
+    for (int u = 0; u < U; ++u) {
+      const bool on = i0 + u + 1 < n;  // nothing walks on from the last one, which left nothing
+      const int64_t at = on ? segment(i0 + u) * a.H + h : 0;
+      get(add[u], on ? a.states + at * a.size + e0 : nullptr);
+      f[u] = on ? a.whole[at] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i0 + u >= n) break;
+      float* q = a.states + (segment(i0 + u) * a.H + h) * a.size + e0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (e < many) q[e] = s[e];
+        s[e] = f[u] * s[e] + add[u][e];
+      }
     }
   }
 }
@@ -895,8 +903,11 @@ template <int C> __global__ __launch_bounds__(GATE_THREADS) void decay_gate_grad
   };
   const auto product = [&](const float* s, const float* d, int64_t i, int64_t j) {  // of two states, this thread's part
     float w = 0.f;
-    if (s && d)
-      for (int64_t e = threadIdx.x; e < a.size; e += GATE_THREADS) w += s[(i * a.H + h) * a.size + e] * d[(j * a.H + h) * a.size + e];
+    if (s && d) {
+      s += (i * a.H + h) * a.size, d += (j * a.H + h) * a.size;
+#pragma unroll 8
+      for (int e = threadIdx.x; e < (int)a.size; e += GATE_THREADS) w += s[e] * d[e];
+    }
     return (double)w;
   };
   float x[U], y[U], u[U];
@@ -929,7 +940,7 @@ template <int C> __global__ __launch_bounds__(GATE_THREADS) void decay_gate_grad
   off = block_sum(off + end - begin);
   if (!is_finite((float)off)) off = 0.;
   const double drift = len > 0 ? off / len : 0.;
-  float sum = 0.f;
+  double sum = 0.;
   for (int t = top, turn = 0; t - (int)threadIdx.x >= 0 || turn == 0; t -= U * GATE_THREADS) {
     if (turn) fetch(t);
 #pragma unroll
