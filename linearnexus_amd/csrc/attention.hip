@@ -18,6 +18,7 @@
 // are busy 44, 45 and 36 % of the time, vector instructions 50, 33 and 26 %.
 // No atomics: dk and dv are summed over the group's query heads by the workgroup that owns the keys, dq by a kernel of its own.
 #include "lnx_common.h"
+#include "lds_direct.h"
 #include "mma_tiles.h"
 #include "packed_slots.h"
 

@@ -14,6 +14,7 @@
 #include <type_traits>
 
 #include "lnx_common.h"
+#include "lds_direct.h"
 #include "mma_tiles.h"
 #include "packed_slots.h"
 

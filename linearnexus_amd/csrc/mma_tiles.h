@@ -255,11 +255,6 @@ __device__ __forceinline__ unsigned lds_byte_addr(const void* p) { return (unsig
 __device__ __forceinline__ void dma16(const void* src, unsigned dst) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(__builtin_amdgcn_readfirstlane(dst)) : "memory", "m0");
 }
-// 16 bytes a lane from `base` + off bytes straight to LDS, lane l at dst + 16 l; the base is the wave's, so a tile's loads cost no
-// vector arithmetic
-__device__ __forceinline__ void dma16_at(const void* base, unsigned off, unsigned dst) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(__builtin_amdgcn_readfirstlane(dst)) : "memory", "m0");
-}
 // The same with four bytes per lane: 256 consecutive bytes of LDS
 __device__ __forceinline__ void dma4(const void* src, unsigned dst) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(__builtin_amdgcn_readfirstlane(dst)) : "memory", "m0");
