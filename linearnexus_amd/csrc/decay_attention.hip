@@ -11,6 +11,9 @@
 // by their own rounding alone, states like fp32's, and dg, a running difference of x . out and y . out over a whole sequence, keeps its digits.
 // Exponents are differences of sums over a chunk: the sums are held as a multiple of 1/64 and a rest, so that a difference is exact to a unit
 // however far the sums have run (a decay of e^-100 beside one of 1).
+// Measured at d128 in bf16: B8 H16 T4096 forward 158 us (537 MB, 3.4 TB/s), backward 638 (its three walks read and write 1.82 GB) and 21 for dg; one
+// prompt of H16 T65000 147 + 8 + 306; a token at B256 H32 211 us, 5.1 TB/s.  A walk's bound is what a SIMD issues: a chunk of 64 tokens is some 350 vector
+// instructions of each of its two waves, 92 to 156 matrix instructions of 16 cycles and a quarter of 280 KB of LDS, in 5000 to 6500 cycles.
 #include <type_traits>
 
 #include "lnx_common.h"
@@ -298,8 +301,8 @@ template <typename T, int KW, bool OUT, bool BWD> struct Room {
   }
   static constexpr int SLOTS = slot(NI, 0, false);
   static constexpr int XB = C * KW * sizeof(T), ZB = C * SLAB * sizeof(T), BUF = (OUT ? 2 : 1) * XB + ZB, PAIRB = OUT ? block(NI, 0, false) : 0;
-  static constexpr int RING = OUT ? 3 : 6, AHEAD = RING - 2;  // chunks in LDS; how far ahead of the pairs' chunk they are fetched
-  static constexpr int PAIRS = RING * BUF, FACTORS = PAIRS + 2 * PAIRB, SUMS = FACTORS + 2 * 1024, RAW = SUMS + 4 * 512, DOTS = RAW + RING * 256;
+  static constexpr int RING = OUT ? 3 : 6, AHEAD = RING - 1;  // chunks in LDS; how far ahead they are fetched (their gates one more)
+  static constexpr int PAIRS = RING * BUF, FACTORS = PAIRS + PAIRB, SUMS = FACTORS + 2 * 1024, RAW = SUMS + 4 * 512, DOTS = RAW + (RING + 1) * 256;
   static constexpr int BYTES = DOTS + (OUT ? 2 * 4 * 2 * C * 4 : 0);
   // The 16 x 16 tiles of pairs, ten of a chunk of 64, in four nearly equal shares: tile u of wave w
   static constexpr int units(int w) { return NI == 4 ? (w < 2 ? 2 : 3) : w < NI * (NI + 1) / 2; }
@@ -320,11 +323,10 @@ struct Task {
 };
 template <bool REV> __device__ __forceinline__ int chunk_at(const Task& k, int it) { return REV ? k.nchunk - 1 - it : it; }
 
-// Scheduling of a stretch of MFMAS matrix instructions: READS reads of LDS first, then VALUS vector instructions behind each of them.  Left to itself
-// the compiler puts what can run beside a matrix instruction (16 cycles) before or behind the whole run.
-template <typename T, int READS, int MFMAS, int VALUS> __device__ __forceinline__ void interleave() {
+// Scheduling of a stretch of MFMAS matrix instructions: VALUS vector instructions behind each of them.  Left to itself the compiler puts what can run
+// beside a matrix instruction (16 cycles) before or behind the whole run.
+template <typename T, int MFMAS, int VALUS> __device__ __forceinline__ void interleave() {
   if constexpr (sizeof(T) == 2) {
-    if constexpr (READS > 0) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
 #pragma unroll
     for (int i = 0; i < MFMAS; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
@@ -333,8 +335,9 @@ template <typename T, int READS, int MFMAS, int VALUS> __device__ __forceinline_
   }
 }
 
-// Four of a walk's eight waves: they bring chunk c + 1 to LDS and form the decays and the pairs of chunk c, one tile of 16 rows each, while
-// the others walk chunk c - 1.  One barrier a chunk.
+// Four of a walk's eight waves.  While the others take what the state gives, they form the chunk's pairs, a share of the tiles each; while the others
+// take what the pairs give and move the state on, they send for the chunk after next and form the next one's decays.  Two barriers a chunk.  (With one, the
+// pairs a chunk ahead of the state and the loads one chunk ahead of them: B8 H16 T4096 d128 forward 162 us -> 159, backward 644 -> 638.)
 template <typename T, int KW, bool OUT, bool REV, bool BWD, int W> __device__ __forceinline__ void walk_pairs(const Walk& a, const Role& ro, const Task& k, char* lds) {
   typedef Form<T> F;
   typedef typename F::Frag Frag;
@@ -353,12 +356,13 @@ template <typename T, int KW, bool OUT, bool REV, bool BWD, int W> __device__ __
   const T* zp = head_of<T>(ro.z, p, k.h) + k.col0 + first * ro.z.st;
   const int64_t x_step = OUT ? dir * ro.x.st : 0, y_step = dir * ro.y.st, z_step = dir * ro.z.st, g_step = dir * a.gt;
   const float* gp = a.g + p.b * a.gb + k.h * a.gh + (p.tok + first + min(lane, C - 1)) * a.gt;
+  int g_next = first, raw_next = 0;  // the next chunk of gates: its first token, its place
   const Mover<T, KW, C> mx(OUT ? ro.x.st : 0, wave, lane), my(ro.y.st, wave, lane);
   const Mover<T, SLAB, C> mz(ro.z.st, wave, lane);
   const bool wide = ro.kw >= KW && k.vw == SLAB;
   int t_next = first;  // the next chunk's first token
   // A chunk's loads, ten of a wave at KW = 128, all at once: a CU takes 64 bytes a cycle, for which these waves wait (of 40 KB 640 cycles), but
-  // handed out between the steps of their work the last ones came too late for the next chunk (forward at B8 H16 T4096 d128 157 us -> 178 - 210)
+  // handed out between the steps of their work they kept the last ones from the next chunk (forward at B8 H16 T4096 d128, one chunk ahead, 157 us -> 178 - 210)
   constexpr int NX = OUT ? decltype(mx)::N : 0, NY = decltype(my)::N, NZ = decltype(mz)::N;
   const auto fetch = [&](int buf) {
     const int valid = min(C, p.len - t_next);
@@ -370,14 +374,16 @@ template <typename T, int KW, bool OUT, bool REV, bool BWD, int W> __device__ __
         else if (i < NY + NX) mx.one(OUT ? i - NY : 0, tiles + R::XB + R::ZB, xp, wave);
         else mz.one(i - NY - NX, tiles + R::XB, zp, wave);
       }
-      if (wave == 0) dma4(gp, lds0 + R::RAW + 256 * buf);
     } else {
       my.edge(tiles, yp, ro.y.st, valid, ro.kw, wave, lane);
       if constexpr (OUT) mx.edge(tiles + R::XB + R::ZB, xp, ro.x.st, valid, ro.kw, wave, lane);
       mz.edge(tiles + R::XB, zp, ro.z.st, valid, k.vw, wave, lane);
-      if (wave == 0) dma4(gp - max(0, min(lane, C - 1) - (valid - 1)) * a.gt, lds0 + R::RAW + 256 * buf);
     }
-    yp += y_step, xp += x_step, zp += z_step, gp += g_step, t_next += (int)dir;
+    yp += y_step, xp += x_step, zp += z_step, t_next += (int)dir;
+  };
+  const auto fetch_gates = [&] {
+    if (wave == 0) dma4(gp - max(0, min(lane, C - 1) - (min(C, p.len - g_next) - 1)) * a.gt, lds0 + R::RAW + 256 * raw_next);
+    gp += g_step, g_next += (int)dir, raw_next = raw_next == R::RING ? 0 : raw_next + 1;
   };
   // the dots of the chunk before the one that is walked: thread = (kind, token)
   const float* red = reinterpret_cast<const float*>(lds + R::DOTS);
@@ -393,64 +399,65 @@ template <typename T, int KW, bool OUT, bool REV, bool BWD, int W> __device__ __
     dot_p += dot_p ? dir : 0;
     dot_t += (int)dir;
   };
-  __builtin_amdgcn_s_setprio(1);  // they have the longer way to the barrier: forward at B8 H16 T4096 d128 166 us -> 154
   float* sums = reinterpret_cast<float*>(lds + R::SUMS) + 128 * wave;  // of this wave: multiples, rests
   const float* raw = reinterpret_cast<const float*>(lds + R::RAW);
   float whole_h = 0.f, whole_l = 0.f;
-  // until chunk `it` is there: all but the loads of those behind it, which are whole ones if they are to be counted
+  // until chunk `it` is there: all but the loads of those behind it, where all of these are counted
   const auto arrived = [&](int it) {
     constexpr int N = (R::AHEAD - 1) * (NY + NX + NZ);
-    if (R::AHEAD > 1 && wide && it + R::AHEAD < k.nchunk) {
-      if (wave == 0) dma_wait<N + R::AHEAD - 1>();
-      else dma_wait<N>();
-    } else {
-      dma_wait<0>();
+    if (wide && it + R::AHEAD < k.nchunk) dma_wait<wave == 0 ? N + R::AHEAD - 1 : N>();
+    else dma_wait<0>();
+  };
+  const auto decays = [&](int it, int raw_at, int t0) {  // lane = token
+    const int valid = min(C, p.len - t0);
+    float gv = lane < valid ? raw[64 * raw_at + lane] * LOG2E : 0.f;
+    gv = gv < -200.f ? -200.f : gv;  // e^-138 is nothing
+    const float gm = rounded(rintf(gv * 64.f) * (1.f / 64.f)), H = running_sum(gm), L = running_sum(gv - gm), HT = lane_value(H, 63), LT = lane_value(L, 63);
+    sums[lane] = H;
+    sums[64 + lane] = L;
+    if (wave == 3) {
+      const float head = between(H, L, 0.f, 0.f), tail = between(HT, LT, H, L);
+      float* f = reinterpret_cast<float*>(lds + R::FACTORS) + 256 * (it & 1);
+      f[lane] = (REV ? tail : head) * ro.row_scale;
+      f[64 + lane] = lane < valid ? (REV ? head : tail) * ro.col_scale : 0.f;
+      f[128 + lane] = between(HT, LT, 0.f, 0.f);
+      if (!OUT) whole_h += HT, whole_l += LT;
     }
   };
+  for (int i = 0; i <= R::AHEAD && i < k.nchunk; ++i) fetch_gates();
   for (int i = 0; i < R::AHEAD && i < k.nchunk; ++i) fetch(i);
-  arrived(0);
+  dma_wait<0>();
   lds_barrier();
-  for (int it = 0, buf = 0, t0 = first; it <= k.nchunk; ++it) {
-    const int next = buf == R::RING - 1 ? 0 : buf + 1;
-    const bool on = it < k.nchunk;
-    // the next chunk on its way, then the operands of this one's pairs
-    if (it + R::AHEAD < k.nchunk) fetch(buf + R::AHEAD < R::RING ? buf + R::AHEAD : buf + R::AHEAD - R::RING);
-    constexpr bool TWO_ROWS = UNITS > 1 && R::unit_row(W, 0, REV) != R::unit_row(W, UNITS > 1, REV);  // (wave 0's)
-    Frag x[1 + TWO_ROWS][NS], y[UNITS > 0 ? UNITS : 1][NS];
-    if (OUT && UNITS > 0 && on) {
-      const unsigned xr = lds0 + buf * R::BUF + R::XB + R::ZB + XC::rows(lane), yr = lds0 + buf * R::BUF + XC::rows(lane);
+  if (k.nchunk > 0) decays(0, 0, first);
+  lds_barrier();
+  for (int it = 0, buf = 0, raw_at = 0, t0 = first; it < k.nchunk; ++it) {
+    if (dots && it >= 1) leave_dots(it - 1);  // (ahead of the loads: whoever waits for these does not wait for it)
+    if constexpr (OUT) {
+      if constexpr (UNITS > 0) {
+        // ---- pairs: rows of a result are j, its column is i
+        constexpr bool TWO_ROWS = UNITS > 1 && R::unit_row(W, 0, REV) != R::unit_row(W, UNITS > 1, REV);  // (wave 0's)
+        Frag x[1 + TWO_ROWS][NS], y[UNITS][NS];
+        const unsigned xr = lds0 + buf * R::BUF + R::XB + R::ZB + XC::rows(lane), yr = lds0 + buf * R::BUF + XC::rows(lane);
 #pragma unroll
-      for (int s = 0; s < NS; ++s) {
+        for (int s = 0; s < NS; ++s) {
+#pragma unroll
+          for (int u = 0; u < UNITS; ++u) {
+            if (u <= TWO_ROWS) x[u][s] = XC::by_row(xr, R::unit_row(W, u, REV) * 16 * XC::ROWB, s);
+            y[u][s] = XC::by_row(yr, R::unit_col(W, u, REV) * 16 * XC::ROWB, s);
+          }
+        }
+        const int valid = min(C, p.len - t0);
+        char* pairs = lds + R::PAIRS;
+        floatx4 sc[UNITS], w[UNITS];
+        // what the decays make of them is formed beside the reads
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {
-          if (u <= TWO_ROWS) x[u][s] = XC::by_row(xr, R::unit_row(W, u, REV) * 16 * XC::ROWB, s);
-          y[u][s] = XC::by_row(yr, R::unit_col(W, u, REV) * 16 * XC::ROWB, s);
+          const int i = 16 * R::unit_row(W, u, REV) + l16, j0 = 16 * R::unit_col(W, u, REV) + g4;
+          const float hi_ = sums[i], li_ = sums[64 + i];
+          const floatx4 hj = load4(sums + j0), lj = load4(sums + 64 + j0);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) w[u][r] = REV ? between(hj[r], lj[r], hi_, li_) : between(hi_, li_, hj[r], lj[r]);
         }
-      }
-    }
-    const int valid = min(C, p.len - t0);
-    if (on) {
-      // ---- the chunk's decays: lane = token
-      float gv = lane < valid ? raw[64 * buf + lane] * LOG2E : 0.f;
-      gv = gv < -200.f ? -200.f : gv;  // e^-138 is nothing
-      const float gm = rounded(rintf(gv * 64.f) * (1.f / 64.f)), H = running_sum(gm), L = running_sum(gv - gm), HT = lane_value(H, 63), LT = lane_value(L, 63);
-      sums[lane] = H;
-      sums[64 + lane] = L;
-      if (wave == 3) {
-        const float head = between(H, L, 0.f, 0.f), tail = between(HT, LT, H, L);
-        float* f = reinterpret_cast<float*>(lds + R::FACTORS) + 256 * (it & 1);
-        f[lane] = (REV ? tail : head) * ro.row_scale;
-        f[64 + lane] = lane < valid ? (REV ? head : tail) * ro.col_scale : 0.f;
-        f[128 + lane] = between(HT, LT, 0.f, 0.f);
-        if (!OUT) whole_h += HT, whole_l += LT;
-      }
-    }
-    if (dots && it >= 2) leave_dots(it - 2);
-    if constexpr (OUT) {
-      if (UNITS > 0 && on) {
-        // ---- pairs: rows of a result are j, its column is i
-        char* pairs = lds + R::PAIRS + (it & 1) * R::PAIRB;
-        floatx4 sc[UNITS > 0 ? UNITS : 1];
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) sc[u] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -460,10 +467,8 @@ template <typename T, int KW, bool OUT, bool REV, bool BWD, int W> __device__ __
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {
           const int it16 = R::unit_row(W, u, REV), jt = R::unit_col(W, u, REV), i = 16 * it16 + l16, j0 = 16 * jt + g4;
-          const float hi_ = sums[i], li_ = sums[64 + i];
-          const floatx4 hj = load4(sums + j0), lj = load4(sums + 64 + j0);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) sc[u][r] *= REV ? between(hj[r], lj[r], hi_, li_) : between(hi_, li_, hj[r], lj[r]);
+          for (int r = 0; r < 4; ++r) sc[u][r] *= w[u][r];
           if (it16 == jt || (REV && valid < C)) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) sc[u][r] = (REV ? j0 + r >= i && j0 + r < valid : j0 + r <= i) ? sc[u][r] : 0.f;
@@ -482,11 +487,16 @@ template <typename T, int KW, bool OUT, bool REV, bool BWD, int W> __device__ __
           }
         }
       }
+      lds_barrier();
     }
+    if (it + R::AHEAD < k.nchunk) fetch(buf == 0 ? R::RING - 1 : buf - 1);
+    if (it + R::AHEAD + 1 < k.nchunk) fetch_gates();
+    buf = buf == R::RING - 1 ? 0 : buf + 1;
+    raw_at = raw_at == R::RING ? 0 : raw_at + 1;
+    t0 += (int)dir;
+    if (it + 1 < k.nchunk) decays(it + 1, raw_at, t0);
     arrived(it + 1);
     lds_barrier();
-    buf = next;
-    t0 += (int)dir;
   }
   if (dots && k.nchunk > 0) leave_dots(k.nchunk - 1);
   if (!OUT && k.item == 0 && threadIdx.x == 448) a.whole[(int64_t)k.slot * a.H + k.h] = between(whole_h, whole_l, 0.f, 0.f);
@@ -506,7 +516,7 @@ template <typename T, int KW, bool OUT, bool REV, bool BWD, bool DOTS> __device_
   typedef Cells<T, KW> XC;
   typedef Cells<T, SLAB> ZC;
   typedef Room<T, KW, OUT, BWD> R;
-  constexpr int C = R::C, NI = R::NI, NJ = R::NJ, NS = KW / F::K, NT = KW / 16, TP = F::TP, ZP = parts_of_z<T>(), PP = parts_of_pairs<T>(DOTS), SP = parts_of_state<T>(DOTS);
+  constexpr int C = R::C, NI = R::NI, NJ = R::NJ, NS = KW / F::K, NT = KW / 16, TP = F::TP, NZT = NJ * TP, ZP = parts_of_z<T>(), PP = parts_of_pairs<T>(DOTS), SP = parts_of_state<T>(DOTS);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g4 = 4 * (lane >> 4), n0 = k.col0 + 16 * wave;
   const Spot& p = k.p;
   const unsigned lds0 = lds_byte_addr(lds);
@@ -536,7 +546,7 @@ template <typename T, int KW, bool OUT, bool REV, bool BWD, bool DOTS> __device_
 #pragma unroll
   for (int i = 0; i < NT; ++i) asm volatile("" : "+v"(st[i]));
   lds_barrier();  // the first chunk's tiles
-  lds_barrier();  // its pairs
+  lds_barrier();  // its decays
   const int dir = REV ? -C : C;
   int t0 = chunk_at<REV>(k, 0) * C;
   T* ob = op + t0 * (OUT ? ro.out.st : 0);
@@ -556,7 +566,7 @@ template <typename T, int KW, bool OUT, bool REV, bool BWD, bool DOTS> __device_
     const int valid = min(C, p.len - t0);
     const float* f = reinterpret_cast<const float*>(lds + R::FACTORS) + 256 * (it & 1);
     const unsigned xr = xa + at, yc = ya + at, zc = za + at;
-    const char* pairs = lds + R::PAIRS + (it & 1) * R::PAIRB;
+    const char* pairs = lds + R::PAIRS;
     // What LDS holds is read well ahead of its use: two steps of x, two parts of the pairs, four tiles of y
     Frag zf[NJ], zs[NJ][ZP], x[3][NI], sp[2][SP], pf[2][R::SLOTS], yf[4][NJ];
     floatx4 acc[NI], low[NI], in[NI], cf[NJ][TP];  // low: of the state's lower parts, summed apart so that their sums are not rounded at the whole's
@@ -608,19 +618,23 @@ template <typename T, int KW, bool OUT, bool REV, bool BWD, bool DOTS> __device_
         if (part + 2 < PP) read_pairs(part + 2);
       }
     };
-    // z with each token's factor, as an operand
-    const auto scaled = [&](auto guard) {
+    // z with each token's factor, as an operand: one tile
+    const auto scaled = [&](auto guard, int j, int t) {
+      floatx4 v;
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        floatx4 v[TP];
+      for (int r = 0; r < 4; ++r) {
+        const bool there = !decltype(guard)::value || F::K * j + 16 * t + g4 + r < valid;  // (0 times what is not finite)
+        v[r] = rounded(there ? F::get(zf[j], t, r) * cf[j][t][r] : 0.f);
+      }
+      if constexpr (TP == 2) {
+        bf16x4 part[ZP];
+        parts_of(v, part);
 #pragma unroll
-        for (int t = 0; t < TP; ++t)
+        for (int i = 0; i < ZP; ++i)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const bool there = !decltype(guard)::value || F::K * j + 16 * t + g4 + r < valid;  // (0 times what is not finite)
-            v[t][r] = rounded(there ? F::get(zf[j], t, r) * cf[j][t][r] : 0.f);
-          }
-        split(v, zs[j]);
+          for (int r = 0; r < 4; ++r) zs[j][i][4 * t + r] = part[i][r];
+      } else {
+        zs[j][0] = v;
       }
     };
     if constexpr (OUT) {
@@ -647,23 +661,33 @@ template <typename T, int KW, bool OUT, bool REV, bool BWD, bool DOTS> __device_
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
         if (s + 2 < NS) read_x(s + 2);
-        else if (s + 2 - NS < PP) read_pairs(s + 2 - NS);
         __builtin_amdgcn_sched_barrier(0);
         if (s + 1 < NS) split_state(s + 1);
+#pragma unroll
+        for (int i = s * NZT / NS; i < (s + 1) * NZT / NS; ++i) scaled(std::false_type{}, i / TP, i % TP);
         from_state(s);
-        interleave<T, 0, SP * NI, 3>();
+        interleave<T, SP * NI, 6>();
         __builtin_amdgcn_sched_barrier(0);
       }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NZT; ++i) scaled(std::false_type{}, i / TP, i % TP);
     }
 #pragma unroll
     for (int i = 0; i < 4 && i < NT; ++i) read_y(i);
-    __builtin_amdgcn_sched_barrier(0);
     // ---- what the chunk's pairs give
+    if constexpr (OUT) {
+      lds_barrier();
+      read_pairs(0);
+      if (PP > 1) read_pairs(1);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < NT; ++i) st[i] *= total;
     if constexpr (OUT) from_pairs();
-    scaled(std::false_type{});
-    if constexpr (OUT) interleave<T, 0, R::SLOTS * PP, 9>();
     if (__builtin_expect(odd, 0)) {
-      scaled(std::true_type{});
+#pragma unroll
+      for (int i = 0; i < NZT; ++i) scaled(std::true_type{}, i / TP, i % TP);
       if constexpr (OUT) {
         // A masked pair would be 0 times such a value: they are taken out of the product and added pair by pair
 #pragma unroll
@@ -708,8 +732,6 @@ template <typename T, int KW, bool OUT, bool REV, bool BWD, bool DOTS> __device_
     if constexpr (OUT)
 #pragma unroll
       for (int t = 0; t < NI; ++t) rf[t] = f[16 * t + l16];
-#pragma unroll
-    for (int i = 0; i < NT; ++i) st[i] *= total;
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
 #pragma unroll
@@ -1067,8 +1089,8 @@ int64_t ceil_div(int64_t x, int64_t y) { return (x + y - 1) / y; }
 constexpr int MAX_D = 256;
 
 // Tokens of a segment, a multiple of 64, or 0: rows are walked whole.  Segments read keys and values (queries and gradients) once more, so they
-// are for rows and heads that leave CUs without a workgroup: as many as give every CU one (H16 T65000 d128: 290 us and 125 on the local walks; with
-// two a CU 310 and 138), of four chunks and more, for rows of more than eight (us of forward alone and with backward, chunks of 64, eight and
+// are for rows and heads that leave CUs without a workgroup: as many as give every CU one (H16 T65000 d128, with two bf16 parts of what a token adds: 290 us
+// and 125 on the local walks, with two a CU 310 and 138; with three parts 306 and 147), of four chunks and more, for rows of more than eight (us of forward alone and with backward, chunks of 64, eight and
 // more -> four: H8 T1000 d128 35, 79 -> 27, 62; H16 T700 34, 77 -> 25, 68; of two 25, 70 and 23, 74; H16 T500 d64 whole 15, 37, in two 20, 45).
 // The rows of a packed batch are taken for one: their lengths are not known here, and sequences of one segment are walked once whatever its size.
 int segment(const lnx_decay_args* a) {
