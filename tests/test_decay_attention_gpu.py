@@ -459,3 +459,39 @@ def test_refusals():
     with torch.autograd.forward_ad.dual_level():
         with pytest.raises(NotImplementedError):
             f(torch.autograd.forward_ad.make_dual(q, q), k, v, g)
+
+
+@pytest.mark.parametrize("per_head", [False, True])
+@pytest.mark.parametrize("T", [40, 600])
+def test_states_and_gates_gradients_of_bf16_are_as_exact_as_fp32(T, per_head):
+    """By norms.  A state is T / 64 chunks, each a scaling and six products into one sum: 7 T / 64 roundings of 2^-24, in no step with each other, and factors
+    good to three units of 2^-23: 3 2^-23 + (7 T / 64)^(1/2) 2^-24 < 2^-20.  dg is made of two such states' dots, whose own sums are as long: 2^-19.  Operands in two parts
+    would leave 2^-18 and 2^-17."""
+    t, do, ds = _inputs(2, 3, T, 128, 128, "bf16", per_head=per_head, decay=0.02, seed=31)
+    leaves = {n: x.detach().requires_grad_() for n, x in t.items()}
+    o, sT = la.decay_linear_attention(leaves["q"], leaves["k"], leaves["v"], leaves["g"], None, leaves["s0"])
+    dg, d0 = torch.autograd.grad([o, sT], [leaves["g"], leaves["s0"]], [do, ds])
+    want = {"state": torch.empty_like(sT, dtype=torch.float64), "dstate": torch.empty_like(sT, dtype=torch.float64), "dg": torch.zeros_like(dg, dtype=torch.float64)}
+    for b in range(2):
+        for h in range(3):
+            g = t["g"][h].expand(T) if per_head else t["g"][b, h]
+            r = _formulas(*(t[n][b, h].double() for n in ("q", "k", "v")), g.double(), t["s0"][b, h].double(), 128 ** -0.5, do[b, h].double(), ds[b, h].double(), 64)
+            want["state"][b, h], want["dstate"][b, h] = r["state"], r["dstate"]
+            if per_head:
+                want["dg"][h] += r["dg"].sum()
+            else:
+                want["dg"][b, h] = r["dg"]
+    for what, got, tol in (("state", sT, 2.0 ** -20), ("dstate", d0, 2.0 ** -20), ("dg", dg, 2.0 ** -19)):
+        off = float((got.detach().double() - want[what]).norm() / want[what].norm())
+        assert off < tol, f"{what}: {off:.2g}"
+
+
+@pytest.mark.parametrize("T", [100, 700])
+def test_gates_gradient_does_not_depend_on_who_wants_the_states(T):
+    t, do, ds = _inputs(1, 2, T, 64, 64, "bf16", seed=32)
+    grads = []
+    for wanted in (True, False):
+        g, s0 = t["g"].detach().requires_grad_(), t["s0"].detach().requires_grad_(wanted)
+        o, sT = la.decay_linear_attention(t["q"], t["k"], t["v"], g, None, s0)
+        grads.append(torch.autograd.grad([o, sT], [g, s0] if wanted else [g], [do, ds])[0])
+    assert torch.equal(*grads)

@@ -120,6 +120,12 @@ def test_decay_sizes():
         a.kept = _ptr()
         assert fwd(a) == n * 4
         assert bwd(a) >= 4 * 4096 * 4 + kept(a) + n * 4
+    a = _decay()  # the gradient of an initial state is formed, whether the caller wants it or not
+    small = bwd(a)
+    a.initial_state = _ptr()
+    assert bwd(a) == small + 4 * 64 * 64 * 4
+    a.d_initial_state = _ptr()
+    assert bwd(a) == small
     assert kept(_decay(H=1, T=512)) == 0 and kept(_decay(H=1, T=513)) == 3 * 64 * 64 * 4
     assert kept(_decay(H=2, T=4096, nseq=5)) == (4096 // 256 + 5) * 2 * 64 * 64 * 4  # a slot more for every sequence
     for bad in (dict(B=0), dict(H=0), dict(dk=0), dict(dv=300), dict(T=-1), dict(nseq=-1)):
