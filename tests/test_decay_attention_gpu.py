@@ -495,3 +495,27 @@ def test_gates_gradient_does_not_depend_on_who_wants_the_states(T):
         o, sT = la.decay_linear_attention(t["q"], t["k"], t["v"], g, None, s0)
         grads.append(torch.autograd.grad([o, sT], [g, s0] if wanted else [g], [do, ds])[0])
     assert torch.equal(*grads)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("H,T,dv", [(130, 9001, 8), (64, 17100, 40), (3, 8193, 256)])
+def test_gates_gradients_over_segments_of_more_than_4096_tokens(H, T, dv, dtype):
+    """By norms, as above: at most nine roundings a chunk of 32, 3 2^-23 + (9 T / 32)^(1/2) 2^-24 < 2^-17 of a state, twice that of dg.  The definition token by token."""
+    t, do, ds = _inputs(1, H, T, 8, dv, dtype, state=False, decay=0.02, seed=33)
+    g = t["g"].detach().requires_grad_()
+    o, sT = la.decay_linear_attention(t["q"], t["k"], t["v"], g)
+    got = torch.autograd.grad([o, sT], [g], [do, ds])[0]
+    q, k, v, d = (x[0].transpose(0, 1).double() for x in (t["q"], t["k"], t["v"], do))  # [T, H, .]
+    e = torch.exp(t["g"][0].double()).T[:, :, None, None]
+    kv, qd = k[..., :, None] * v[..., None, :], 8 ** -0.5 * q[..., :, None] * d[..., None, :]
+    before, s = torch.empty_like(kv), torch.zeros_like(kv[0])
+    for i in range(T):
+        before[i] = s
+        s = e[i] * s + kv[i]
+    want, back = torch.empty(T, H, dtype=torch.float64, device=DEV), ds[0].double()
+    for i in range(T - 1, -1, -1):
+        back = back + qd[i]  # of the state behind token i
+        want[i] = (e[i] * back * before[i]).sum((1, 2))
+        back = e[i] * back
+    off = float((got[0].T.double() - want).norm() / want.norm())
+    assert off < 2.0 ** -16, f"{off:.2g}"
