@@ -1131,6 +1131,10 @@ int check(const char* what, const lnx_decay_args* a, bool bwd) {
   if (a->dtype != LNX_F32 && a->dtype != LNX_BF16) return lnx_set_error(LNX_ERR_DTYPE, "%s: dtype %d", what, a->dtype);
   if (!(a->scale == a->scale) || a->scale - a->scale != 0.f) return lnx_set_error(LNX_ERR_SHAPE, "%s: scale must be finite", what);
   if (a->nseq && !a->cu_seqlens) return lnx_set_error(LNX_ERR_NULL, "%s: nseq without cu_seqlens", what);
+  if (bwd && a->g_per_head) {  // written whether there are rows or not
+    if (!a->d_g) return lnx_set_error(LNX_ERR_NULL, "%s: d_g is required", what);
+    if (a->H > MAX_GRID / 256) return lnx_set_error(LNX_ERR_SHAPE, "%s: too many heads", what);
+  }
   if (a->B == 0) return LNX_OK;
   const Layout l = layout(a);
   const int64_t walks = l.slots * a->H * (bwd ? 2 * ceil_div(a->dk, SLAB) + ceil_div(a->dv, SLAB) : ceil_div(a->dv, SLAB));
@@ -1224,6 +1228,11 @@ template <typename T> int forward(const lnx_decay_args* a, hipStream_t st) {
   return start<T, true, false>(k, 1, "decay_fwd", st);
 }
 
+void gate_sum(const lnx_decay_args* a, const float* part, int64_t rows, hipStream_t st) {
+  lnx_profile_mark("decay_gate_sum", st);
+  decay_gate_sum_kernel<<<dim3((unsigned)a->H), 256, 0, st>>>(part, rows, a->H, a->d_g);
+}
+
 template <typename T> int backward(const lnx_decay_args* a, hipStream_t st) {
   const Layout l = layout(a);
   Walk k = walk(a, l);
@@ -1266,10 +1275,7 @@ template <typename T> int backward(const lnx_decay_args* a, hipStream_t st) {
   const dim3 grid((unsigned)(l.slots * a->H));
   if (q.kw <= 128) decay_gate_grad_kernel<chunk_of<T, 128>()><<<grid, GATE_THREADS, 0, st>>>(d);
   else decay_gate_grad_kernel<chunk_of<T, 256>()><<<grid, GATE_THREADS, 0, st>>>(d);
-  if (a->g_per_head) {
-    lnx_profile_mark("decay_gate_sum", st);
-    decay_gate_sum_kernel<<<dim3((unsigned)a->H), 256, 0, st>>>(d.part, l.slots, a->H, a->d_g);
-  }
+  if (a->g_per_head) gate_sum(a, d.part, l.slots, st);
   return LNX_OK;
 }
 
@@ -1305,8 +1311,12 @@ extern "C" int lnx_decay_fwd(const lnx_decay_args* a, void* hip_stream) {
 }
 extern "C" int lnx_decay_bwd(const lnx_decay_args* a, void* hip_stream) {
   if (int rc = check("decay_bwd", a, true)) return rc;
-  if (a->B == 0) return LNX_OK;
   hipStream_t st = static_cast<hipStream_t>(hip_stream);
+  if (a->B == 0) {
+    if (!a->g_per_head) return LNX_OK;
+    gate_sum(a, nullptr, 0, st);  // sums over no rows are zeros
+    return finish("decay_bwd", LNX_OK, st);
+  }
   return finish("decay_bwd", a->dtype == LNX_BF16 ? backward<bf16_t>(a, st) : backward<float>(a, st), st);
 }
 extern "C" int lnx_decay_step(const lnx_decay_step_args* a, void* hip_stream) {
