@@ -1141,7 +1141,7 @@ int check(const char* what, const lnx_decay_args* a, bool bwd) {
   if (walks > MAX_GRID / WALK_THREADS || (bwd ? l.slots * a->H > MAX_GRID / GATE_THREADS : l.rows * a->H > MAX_GRID / JOIN_THREADS)) return lnx_set_error(LNX_ERR_SHAPE, "%s: too many rows", what);
   if (!bwd && !a->final_state) return lnx_set_error(LNX_ERR_NULL, "%s: final_state is required", what);
   if (bwd && a->d_final_state && !a->final_state) return lnx_set_error(LNX_ERR_NULL, "%s: d_final_state needs final_state", what);
-  if (bwd && !a->d_g) return lnx_set_error(LNX_ERR_NULL, "%s: d_g is required", what);
+  if (bwd && a->T && !a->d_g) return lnx_set_error(LNX_ERR_NULL, "%s: d_g is required", what);
   const lnx_tensor4* ts[] = {&a->q, &a->k, &a->v, &a->o, &a->d_o, &a->d_q, &a->d_k, &a->d_v};
   const int64_t size = a->dtype == LNX_BF16 ? 2 : 4;
   const auto fits = [&](int extent, int64_t stride) { return extent <= 1 || stride * size % 16 == 0; };
