@@ -91,6 +91,31 @@ void refuse_tangents(const char* op, const variable_list& ts) {
   for (const Tensor& t : ts) refuse_tangents(op, {&t});
 }
 
+// Gradients as they leave a backward pass: the kernels have none of their own, so under create_graph, where they would come back as constants
+// whose part of a second derivative is silently absent, whatever asks for it is told so.  The node lies before what the op's inputs and the
+// incoming gradients come from, as one that had the derivative would.
+struct NoDerivative : torch::autograd::Node {
+  const std::string op;
+  NoDerivative(const char* op, torch::autograd::edge_list&& edges) : Node(std::move(edges)), op(op) {}
+  variable_list apply(variable_list&&) override { TORCH_CHECK_NOT_IMPLEMENTED(false, op, " has no second derivative"); }
+};
+variable_list first_order(const char* op, const variable_list& incoming, variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  torch::autograd::edge_list edges;
+  if (const auto self = torch::autograd::get_current_node())
+    for (const torch::autograd::Edge& e : self->next_edges())
+      if (e.is_valid()) edges.push_back(e);
+  for (const Tensor& g : incoming)
+    if (g.defined() && g.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(g));
+  const auto node = std::make_shared<NoDerivative>(op, std::move(edges));
+  for (Tensor& g : grads) {
+    if (!g.defined()) continue;
+    g = g.detach();
+    torch::autograd::create_gradient_edge(g, node);
+  }
+  return grads;
+}
+
 Tensor work_area(const Tensor& like, uint64_t bytes) { return at::empty({(int64_t)std::max<uint64_t>(bytes, 1)}, like.options().dtype(at::kByte)); }
 
 std::string shape_text(const Tensor& t) {
@@ -1018,7 +1043,7 @@ struct LayerNormFn : Function<LayerNormFn> {
     const c10::DeviceGuard guard(x.device());
     check_status(lnx_layer_norm_bwd(&a, stream_of(x)), "lnx_layer_norm_bwd");
     auto to = [](const Tensor& t, int64_t type) { return t.defined() ? t.to((at::ScalarType)type) : t; };
-    return {dx, to(dw, m[1]), to(db, m[2]), Tensor(), Tensor()};
+    return first_order("layer_norm", grads, {dx, to(dw, m[1]), to(db, m[2]), Tensor(), Tensor()});
   }
 };
 
@@ -1823,7 +1848,8 @@ struct DecayFn : Function<DecayFn> {
     a.workspace = ptr(ws);
     const c10::DeviceGuard guard(q.device());
     check_status(lnx_decay_bwd(&a, stream_of(q)), "lnx_decay_bwd");
-    return {decay_cut(dq, s.dk), decay_cut(dk, s.dk), decay_cut(dv, s.dv), dg.to((at::ScalarType)m[8]), d0.defined() ? d0.to((at::ScalarType)m[10]) : d0, Tensor(), Tensor()};
+    return first_order("decay_linear_attention", grads, {decay_cut(dq, s.dk), decay_cut(dk, s.dk), decay_cut(dv, s.dv), dg.to((at::ScalarType)m[8]),
+                                                  d0.defined() ? d0.to((at::ScalarType)m[10]) : d0, Tensor(), Tensor()});
   }
 };
 

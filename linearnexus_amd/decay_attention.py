@@ -6,7 +6,7 @@ erasing (the scans of linear_attn.py), for prompts, training and decoding.
 o in q's dtype and memory order, the state ``[B,H,dk,dv]`` in float32.  ``[B,T,H,d]`` tensors are passed as ``x.transpose(1, 2)`` views and nothing is
 copied.  ``g`` holds log-decays (<= 0; -inf drops everything before the token): ``[B,H,T]``, any strides, or one constant for each head, ``[H]``.
 Packed batches pass B = 1, ``cu_seqlens`` and states ``[nseq,H,dk,dv]``, like the chunked ops.  Differentiable with respect to q, k, v, g and the
-initial state; states and sums are float32 whatever q is.
+initial state, once: asking for a second derivative raises; states and sums are float32 whatever q is.
 ``decay_linear_attention_step(q, k, v, g, state, scale=None, *, inplace=False)`` is one decode token on ``[B,H,d]`` tensors, in place on request (not
 differentiable then).  There is no other code path: the ops raise if the library is missing.
 """

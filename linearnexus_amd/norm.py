@@ -45,5 +45,5 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
 
     ``x [..., d]`` and the result are float32 or bfloat16; sums are float32.  ``weight`` and ``bias`` are ``[d]``, or ``[heads, d]`` for
     ``x [..., heads, d]``: every head is a row of its own with its own weights (the norm behind a linear-attention mixer).  ``None``: ones, zeros.
-    Differentiable with respect to all three."""
+    Differentiable with respect to all three, once: asking for a second derivative raises."""
     return _lib.host().layer_norm(x, weight, bias, eps)
