@@ -896,6 +896,9 @@ __global__ __launch_bounds__(JOIN_THREADS) void decay_join_kernel(Join a) {
 // a key.  A strong decay makes x, y and Z small, and they are summed apart from the pairs, which cancel over a chunk.
 // W is known at both ends of a segment, from the states there.  Walked from its end the sums miss it at its beginning by what their terms were off, which
 // for a slow decay is a drift; that is taken back evenly over the tokens (H8 T4096 d128: dg off by 1.1e-6 -> 2.2e-7 against 64 bits).
+// Where a term is not finite the sums from the end are not either, from its token down; a key's or a value's leaves its own dg and the earlier ones be,
+// which then come from the segment's beginning:
+//   dg_t = sum_{r < t} (y_r - x_r - u_r) + W before the chunk     W behind the chunk = W before + sum (y - x)
 struct GateGrad {
   const float *dots_q, *dots_k;  // [inter, pairs][slab][B H][T]
   const float *init, *d_init, *fin, *d_fin;  // of rows, or NULL
@@ -963,7 +966,25 @@ template <int C> __global__ __launch_bounds__(GATE_THREADS) void decay_gate_grad
   const double begin = p.first ? product(a.init, a.d_init, p.row, p.row) : product(a.before, a.behind, slot, slot - 1);
   double W = block_sum(end);
   off = block_sum(off + end - begin);
-  if (!is_finite((float)off)) off = 0.;
+  int good = -1;  // tokens up to here: from the beginning
+  double B = 0.;
+  if (!is_finite((float)off)) {
+    off = 0.;
+    int bad = len;
+    for (int t = threadIdx.x; t < bad; t += GATE_THREADS) {
+      float ax, ay, au;
+      get(t, ax, ay, au);
+      if (!is_finite(ax + ay + au)) bad = t;
+    }
+    B = block_sum(begin);
+#pragma unroll
+    for (int o = 32; o; o >>= 1) bad = min(bad, __shfl_xor(bad, o, LNX_WAVE));
+    __syncthreads();
+    if (lane == 0) red[wave] = bad;
+    __syncthreads();
+    for (int i = 0; i < 16; ++i) bad = min(bad, (int)red[i]);
+    if (is_finite((float)B)) good = min(bad, len - 1);
+  }
   const double drift = len > 0 ? off / len : 0.;
   double sum = 0.;
   for (int t = top, turn = 0; t - (int)threadIdx.x >= 0 || turn == 0; t -= U * GATE_THREADS) {
@@ -990,10 +1011,35 @@ template <int C> __global__ __launch_bounds__(GATE_THREADS) void decay_gate_grad
       }
       const float Z = (float)(behind - max(0, len - (ti - in + C)) * drift - Y);
       const float d = sx + su + (py - y[i]) + Z;
-      if (ti < len) {
+      if (ti < len && ti > good) {
         if (a.dg) a.dg[base + ti] = d;
         sum += d;
       }
+    }
+  }
+  __syncthreads();
+  for (int t = threadIdx.x, turn = 0; t - (int)threadIdx.x <= good; t += GATE_THREADS, ++turn) {
+    float ax, ay, au;
+    get(t < good ? t : -1, ax, ay, au);
+    const float own = ay - ax - au;
+    float before = own, all = ay - ax;
+#pragma unroll
+    for (int o = 1; o < C; o <<= 1) {
+      const float bb = __shfl_up(before, o, LNX_WAVE), ba = __shfl_up(all, o, LNX_WAVE);
+      if (in >= o) before += bb, all += ba;
+    }
+    if (in == C - 1) chunk[turn & 1][mine] = all;
+    __syncthreads();
+    double from = B;
+#pragma unroll 8
+    for (int j = 0; j < NC; ++j) {
+      if (j == mine) from = B;
+      B += chunk[turn & 1][j];
+    }
+    if (t <= good) {
+      const float d = (float)from + (before - own);
+      if (a.dg) a.dg[base + t] = d;
+      sum += d;
     }
   }
   if (a.part) {

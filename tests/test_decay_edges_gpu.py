@@ -6,6 +6,7 @@ import torch
 
 import linearnexus_amd as la
 from linearnexus_amd import _lib
+from test_decay_attention_gpu import CHUNK, DT, _close, _formulas, _inputs
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -42,3 +43,64 @@ def test_rows_without_tokens_have_gradients(packed, per_head):
     assert torch.equal(s, s0) and o.shape == z.shape
     dz, dg, d0 = torch.autograd.grad([o, s], [z, g, s0], [torch.zeros_like(o), ds])
     assert dz.shape == z.shape and dg.shape == g.shape and bool((dg == 0).all()) and torch.equal(d0, ds)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("per_head", [False, True])
+@pytest.mark.parametrize("which", ["q", "k", "v", "do"])
+@pytest.mark.parametrize("T,at", [(1, 0), (100, 0), (100, 63), (100, 99), (150, 70), (1100, 0), (1100, 300), (1100, 1099), (2600, 1700)])
+def test_gates_gradients_beside_values_that_are_not_finite(T, at, which, per_head, dtype):
+    """dg_t = e^g <dS_t, S_{t-1}> takes keys and values of earlier tokens and queries and gradients of t and later ones: the others' dg is what it is
+    without the value, within the bound of the terms that it is summed from; other heads' is the same bit for bit.  (1100 tokens and more: in segments.)"""
+    for value in (float("nan"), float("inf")):
+        t, do, ds = _inputs(1, 2, T, 64, 64, dtype, per_head=per_head, decay=0.1, seed=41)
+        leaves = {n: x.detach().requires_grad_() for n, x in t.items()}
+        bad = {**{n: t[n].clone() for n in ("q", "k", "v")}, "do": do.clone()}
+        bad[which][0, 1, at, 5] = value
+        grads = []
+        for x in ({**t, "do": do}, bad):
+            g = t["g"].detach().requires_grad_()
+            o, sT = la.decay_linear_attention(x["q"], x["k"], x["v"], g, None, t["s0"])
+            grads.append(torch.autograd.grad([o, sT], g, [x["do"], ds])[0])
+        E = (2.0 ** -15 if dtype == "bf16" else 0.0) + (T + 192) * 2.0 ** -23 + 17 * 2.0 ** -20
+        x = [t[n][0, 1].double() for n in ("q", "k", "v")]
+        gg = (t["g"][1].expand(T) if per_head else t["g"][0, 1]).double()
+        back = [do[0, 1].double(), ds[0, 1].double()]
+        ref = _formulas(*x, gg, t["s0"][0, 1].double(), 64 ** -0.5, *back, CHUNK[DT[dtype]])["dg"]
+        mag = _formulas(*(y.abs() for y in x), gg, t["s0"][0, 1].double().abs(), 64 ** -0.5, *(y.abs() for y in back), CHUNK[DT[dtype]])["dg sums"]
+        tokens = torch.arange(T, device=DEV)
+        fine = tokens <= at if which in ("k", "v") else tokens > at
+        if per_head:
+            assert torch.equal(grads[0][0], grads[1][0])
+            if bool(fine.all()):
+                _close(grads[1][1], ref.sum(), (2 * E * mag).sum() + (T + 16) * 2.0 ** -23 * ref.abs().sum(), "dg")
+            else:
+                assert not bool(torch.isfinite(grads[1][1]))
+        else:
+            assert torch.equal(grads[0][0, 0], grads[1][0, 0])
+            _close(grads[1][0, 1][fine], ref[fine], (2 * E * mag)[fine], "dg")
+            assert not bool(torch.isfinite(grads[1][0, 1][~fine]).any())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("at", [100, 1024, 2100, 2221])
+def test_gates_gradients_beside_a_value_that_is_not_finite_in_a_long_row(at, dtype):
+    """Heads enough that rows are walked whole: more tokens than are summed at a time."""
+    H, T = 130, 2222
+    t, do, ds = _inputs(1, H, T, 16, 16, dtype, state=False, decay=0.1, seed=42)
+    v = t["v"].clone()
+    v[0, 7, at, 3] = float("inf")
+    grads = []
+    for x in (t["v"], v):
+        g = t["g"].detach().requires_grad_()
+        o, sT = la.decay_linear_attention(t["q"], t["k"], x, g)
+        grads.append(torch.autograd.grad([o, sT], g, [do, ds])[0][0])
+    others = torch.arange(H, device=DEV) != 7
+    assert torch.equal(grads[0][others], grads[1][others]) and not bool(torch.isfinite(grads[1][7, at + 1 :]).any())
+    x = [t[n][0, 7].double() for n in ("q", "k", "v", "g")]
+    back = [do[0, 7].double(), ds[0, 7].double()]
+    zero = torch.zeros(16, 16, dtype=torch.float64, device=DEV)
+    ref = _formulas(*x, zero, 0.25, *back, CHUNK[DT[dtype]])["dg"]
+    mag = _formulas(*(y.abs() for y in x[:3]), x[3], zero, 0.25, *(y.abs() for y in back), CHUNK[DT[dtype]])["dg sums"]
+    E = (2.0 ** -15 if dtype == "bf16" else 0.0) + (T + 96) * 2.0 ** -23 + 17 * 2.0 ** -20
+    _close(grads[1][7, : at + 1], ref[: at + 1], (2 * E * mag)[: at + 1], "dg")
