@@ -98,5 +98,33 @@ template <int TPR> __device__ __forceinline__ void row_sum2(float& x, float& y, 
 #pragma unroll
   for (int i = 1; i < TPR / 64; ++i) x += red[i], y += red[16 + i];
 }
+// Two or three of them, of rows of a wave and more by fewer exchanges: an exchange of rows of 16 lanes of two values leaves one sum, whose even rows are the
+// first's and whose odd rows the second's, one of the halves of that and the third's the like, so that the last four steps are one value's
+template <int TPR, int N> __device__ __forceinline__ void row_sums(float (&x)[N], float* red) {
+  static_assert(N == 2 || N == 3, "rows of 16 lanes: 0, 1, 0, 1 or 0, 1, 2, 2");
+  if constexpr (TPR < 64) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = lanes_sum<TPR>(x[i]);
+  } else {
+    const auto two = __builtin_amdgcn_permlane16_swap(__float_as_uint(x[0]), __float_as_uint(x[1]), false, false);
+    float s = __uint_as_float(two[0]) + __uint_as_float(two[1]);
+    const auto all = __builtin_amdgcn_permlane32_swap(__float_as_uint(s), __float_as_uint(N == 2 ? s : xor16_sum(x[N - 1])), false, false);
+    s = row16_sum(__uint_as_float(all[0]) + __uint_as_float(all[1]));
+    if constexpr (TPR == 64) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(s), 16 * i));
+    } else {
+      const int lane = threadIdx.x & 63;
+      if (lane % 16 == 0 && lane < 16 * N) red[lane + (threadIdx.x >> 6)] = s;
+      lds_barrier();
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        x[i] = red[16 * i];
+#pragma unroll
+        for (int w = 1; w < TPR / 64; ++w) x[i] += red[16 * i + w];
+      }
+    }
+  }
+}
 
 }  // namespace
