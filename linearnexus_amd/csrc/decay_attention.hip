@@ -435,7 +435,7 @@ template <typename T, int KW, bool OUT, bool REV, bool BWD, int W> __device__ __
   if (k.nchunk > 0) decays(0, 0, first);
   lds_barrier();
   for (int it = 0, buf = 0, raw_at = 0, t0 = first; it < k.nchunk; ++it) {
-    if (dots && it >= 1) leave_dots(it - 1);  // (ahead of the loads: whoever waits for these does not wait for it)
+    if (dots && it >= 1) leave_dots(it - 1);  // (ahead of the loads, so that those still on their way at the wait below are loads alone: it is waited for there)
     if constexpr (OUT) {
       if constexpr (UNITS > 0) {
         // ---- pairs: rows of a result are j, its column is i
