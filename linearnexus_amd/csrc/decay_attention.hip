@@ -892,12 +892,45 @@ __global__ __launch_bounds__(JOIN_THREADS) void decay_join_kernel(Join a) {
   }
 }
 
+// Sums over C lanes, in every one of them
+template <int CTRL> __device__ __forceinline__ double from_lane64(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint64_t lo = (unsigned)__builtin_amdgcn_mov_dpp((int)u, CTRL, 0xF, 0xF, true), hi = (unsigned)__builtin_amdgcn_mov_dpp((int)(u >> 32), CTRL, 0xF, 0xF, true);
+  return __builtin_bit_cast(double, hi << 32 | lo);
+}
+template <int C> __device__ __forceinline__ float chunk_sum(float x) {
+  x = row16_sum(x);
+  if constexpr (C >= 32) x = xor16_sum(x);
+  if constexpr (C == 64) x = xor32_sum(x);
+  return x;
+}
+template <int C> __device__ __forceinline__ double chunk_sum(double x) {
+  x += from_lane64<0xB1>(x);
+  x += from_lane64<0x4E>(x);
+  x += from_lane64<0x141>(x);
+  x += from_lane64<0x128>(x);
+  const auto both = [](uint64_t lo, uint64_t hi) { return __builtin_bit_cast(double, hi << 32 | (unsigned)lo); };
+  if constexpr (C >= 32) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const auto lo = __builtin_amdgcn_permlane16_swap((unsigned)u, (unsigned)u, false, false), hi = __builtin_amdgcn_permlane16_swap((unsigned)(u >> 32), (unsigned)(u >> 32), false, false);
+    x = both(lo[0], hi[0]) + both(lo[1], hi[1]);
+  }
+  if constexpr (C == 64) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const auto lo = __builtin_amdgcn_permlane32_swap((unsigned)u, (unsigned)u, false, false), hi = __builtin_amdgcn_permlane32_swap((unsigned)(u >> 32), (unsigned)(u >> 32), false, false);
+    x = both(lo[0], hi[0]) + both(lo[1], hi[1]);
+  }
+  return x;
+}
+
 // dg from the walks' dots.  In a chunk with W = <dS, S> behind it:
 //   dg_t = sum_{s >= t} (x_s + u_s) + sum_{r < t} y_r + Z     Z = W - sum y     W before the chunk = Z + sum x
 // x: what a token's outputs took from the state before the chunk, y: what its key hands to the state behind it, u: its pairs as a query less those as
 // a key.  A strong decay makes x, y and Z small, and they are summed apart from the pairs, which cancel over a chunk.
 // W is known at both ends of a segment, from the states there.  Walked from its end the sums miss it at its beginning by what their terms were off, which
-// for a slow decay is a drift; that is taken back evenly over the tokens (H8 T4096 d128: dg off by 1.1e-6 -> 2.2e-7 against 64 bits).
+// for a slow decay is a drift; that is taken back from the chunks in the proportion of sum |x| + |y| (H8 T4096 d128: dg off by 1.1e-6 -> 2.2e-7 against 64 bits),
+// so that a quiet part of a row has no share in what a loud one is off by (H130 T4096 d64, the half of a row whose other half's values are a thousand times its own:
+// 2e-4 - 1.6e-3 of its norm if evenly, at most 3e-6 thus; the kernel 21.0 us -> 22.2 at B8 H16 T4096 d128).  A chunk's sum is of the same differences as the row's, in double.
 // Where a term is not finite the sums from the end are not either, from its token down; a key's or a value's leaves its own dg and the earlier ones be,
 // which then come from the segment's beginning:
 //   dg_t = sum_{r < t} (y_r - x_r - u_r) + W before the chunk     W behind the chunk = W before + sum (y - x)
@@ -956,13 +989,13 @@ template <int C> __global__ __launch_bounds__(GATE_THREADS) void decay_gate_grad
   };
   const int top = len > 0 ? (len - 1) / GATE_THREADS * GATE_THREADS + (int)threadIdx.x : (int)threadIdx.x;
   fetch(top);
-  double off = 0.;
+  double off = 0., loud = 0.;
 #pragma unroll
-  for (int i = 0; i < U; ++i) off += x[i] - y[i];
+  for (int i = 0; i < U; ++i) off += x[i] - y[i], loud += fabsf(x[i]) + fabsf(y[i]);
   for (int t = top - U * GATE_THREADS; t >= 0; t -= GATE_THREADS) {
     float nx, ny, nu;
     get(t, nx, ny, nu);
-    off += nx - ny;
+    off += nx - ny, loud += fabsf(nx) + fabsf(ny);
   }
   const double end = p.last ? product(a.fin, a.d_fin, p.row, p.row) : product(a.before, a.behind, slot + 1, slot);
   const double begin = p.first ? product(a.init, a.d_init, p.row, p.row) : product(a.before, a.behind, slot, slot - 1);
@@ -987,7 +1020,8 @@ template <int C> __global__ __launch_bounds__(GATE_THREADS) void decay_gate_grad
     for (int i = 0; i < 16; ++i) bad = min(bad, (int)red[i]);
     if (is_finite((float)B)) good = min(bad, len - 1);
   }
-  const double drift = len > 0 ? off / len : 0.;
+  loud = block_sum(loud);
+  const double drift = loud > 0. && off != 0. ? off / loud : 0.;
   double sum = 0.;
   for (int t = top, turn = 0; t - (int)threadIdx.x >= 0 || turn == 0; t -= U * GATE_THREADS) {
     if (turn) fetch(t);
@@ -1002,8 +1036,10 @@ template <int C> __global__ __launch_bounds__(GATE_THREADS) void decay_gate_grad
         if (in + o < C) sx += bx, su += bu;
         if (in >= o) py += by;
       }
-      const float X = __shfl(sx, lane - in, LNX_WAVE), Y = __shfl(py, lane - in + C - 1, LNX_WAVE);
-      if (in == 0) chunk[turn & 1][mine] = (double)X - Y;
+      const float Y = __shfl(py, lane - in + C - 1, LNX_WAVE);
+      const double step = chunk_sum<C>((double)(x[i] - y[i]));  // as the sum over the row took them
+      const float weight = chunk_sum<C>(fabsf(x[i]) + fabsf(y[i]));
+      if (in == 0) chunk[turn & 1][mine] = step - weight * drift;
       __syncthreads();
       double behind = W;
 #pragma unroll 8
@@ -1011,7 +1047,7 @@ template <int C> __global__ __launch_bounds__(GATE_THREADS) void decay_gate_grad
         if (j == mine) behind = W;
         W += chunk[turn & 1][j];
       }
-      const float Z = (float)(behind - max(0, len - (ti - in + C)) * drift - Y);
+      const float Z = (float)(behind - Y);
       const float d = sx + su + (py - y[i]) + Z;
       if (ti < len && ti > good) {
         if (a.dg) a.dg[base + ti] = d;

@@ -104,3 +104,27 @@ def test_gates_gradients_beside_a_value_that_is_not_finite_in_a_long_row(at, dty
     mag = _formulas(*(y.abs() for y in x[:3]), x[3], zero, 0.25, *(y.abs() for y in back), CHUNK[DT[dtype]])["dg sums"]
     E = (2.0 ** -15 if dtype == "bf16" else 0.0) + (T + 96) * 2.0 ** -23 + 17 * 2.0 ** -20
     _close(grads[1][7, : at + 1], ref[: at + 1], (2 * E * mag)[: at + 1], "dg")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("loud", ["first", "second"])
+def test_gates_gradients_of_a_quiet_half_beside_a_loud_one(loud, dtype):
+    """One half's values are a thousand times the other's, a reset between them, in rows that are walked whole: the quiet half's dg is what it is alone.  By
+    norms: at most nine roundings of a state for each chunk of 32, 3 2^-23 + (9 T / 32)^(1/2) 2^-24 < 2^-18 of it, twice that of dg, and as much again for its
+    share in what the row's sums miss: 2^-16."""
+    B, H, T, d = 2, 66, 4096, 16
+    t, do, _ = _inputs(B, H, T, d, d, dtype, state=False, decay=0.002, seed=43)
+    half = {"first": slice(0, T // 2), "second": slice(T // 2, T)}
+    t["v"][:, :, half[loud]] *= 1000.0
+    t["g"][:, :, T // 2] = -float("inf")
+    g = t["g"].detach().requires_grad_()
+    o, _ = la.decay_linear_attention(t["q"], t["k"], t["v"], g)
+    got = torch.autograd.grad(o, g, do)[0]
+    quiet = half["second" if loud == "first" else "first"]
+    zero = torch.zeros(d, d, dtype=torch.float64, device=DEV)
+    for b, h in ((0, 0), (0, 37), (1, 65)):
+        x = [y[b, h, quiet].double() for y in (t["q"], t["k"], t["v"], t["g"])]
+        x[3] = x[3].clamp_min(-60.0)  # (the reset is the first of the second half, whose own state is empty)
+        want = _formulas(*x, zero, d ** -0.5, do[b, h, quiet].double(), zero, CHUNK[DT[dtype]])["dg"]
+        off = float((got[b, h, quiet].double() - want).norm() / want.norm())
+        assert off < 2.0 ** -16, f"{off:.2g}"
