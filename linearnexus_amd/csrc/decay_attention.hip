@@ -1006,10 +1006,10 @@ template <int C> __global__ __launch_bounds__(GATE_THREADS) void decay_gate_grad
   if (!is_finite((float)off)) {
     off = 0.;
     int bad = len;
-    for (int t = threadIdx.x; t < bad; t += GATE_THREADS) {
+    for (int64_t t = threadIdx.x; t < bad; t += GATE_THREADS) {  // (rows may end within GATE_THREADS of 2^31)
       float ax, ay, au;
-      get(t, ax, ay, au);
-      if (!is_finite(ax + ay + au)) bad = t;
+      get((int)t, ax, ay, au);
+      if (!is_finite(ax + ay + au)) bad = (int)t;
     }
     B = block_sum(begin);
 #pragma unroll
@@ -1056,9 +1056,10 @@ template <int C> __global__ __launch_bounds__(GATE_THREADS) void decay_gate_grad
     }
   }
   __syncthreads();
-  for (int t = threadIdx.x, turn = 0; t - (int)threadIdx.x <= good; t += GATE_THREADS, ++turn) {
+  int turn = 0;
+  for (int64_t t = threadIdx.x; t - (int)threadIdx.x <= good; t += GATE_THREADS, ++turn) {
     float ax, ay, au;
-    get(t < good ? t : -1, ax, ay, au);
+    get(t < good ? (int)t : -1, ax, ay, au);
     const float own = ay - ax - au;
     float before = own, all = ay - ax;
 #pragma unroll
