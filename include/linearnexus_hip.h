@@ -574,7 +574,8 @@ int lnx_attn_step_paged(const lnx_attn_step_paged_args* a, void* hip_stream);
  * q, k, d_q, d_k are [B, H, T, dk], v, o, d_o, d_v [B, H, T, dv] in `dtype`, each with its own strides like the tensors of causal
  * attention above; dk, dv <= 256.  Rows are whole numbers of 16 bytes: columns behind dk and dv up to the next multiple of 8 (bf16) or 4 (fp32)
  * exist and hold zeros in the inputs.  g [B, H, T] fp32 with its own strides (any; 0 for a constant), <= 0, -inf drops what came before the token;
- * d_g is dense [B, H, T], or [H], the sums over rows and tokens (zeros where there are none), with g_per_head.  States [B, H, dk, dv] ([nseq, H, dk, dv] packed) dense fp32;
+ * d_g is dense [B, H, T], or [H], the sums over rows and tokens (zeros where there are none), with g_per_head; it may be NULL where it has
+ * no elements.  States [B, H, dk, dv] ([nseq, H, dk, dv] packed) dense fp32;
  * initial_state, d_final_state (zeros) and d_initial_state may be NULL.  The forward call leaves in `kept` what the backward call reads (NULL:
  * no backward pass will follow; lnx_decay_kept_bytes may be 0); the backward call reads the forward call's inputs, `kept`, and final_state where d_final_state
  * is given.  The workspace (16-byte aligned, may be NULL where its size is 0; the forward size depends on whether kept is set, the backward

@@ -12,7 +12,7 @@
 // Exponents are differences of sums over a chunk: the sums are held as a multiple of 1/64 and a rest, so that a difference is exact to a unit
 // however far the sums have run (a decay of e^-100 beside one of 1).
 // Measured at d128 in bf16: B8 H16 T4096 forward 141 - 165 us (537 MB, 3.3 - 3.8 TB/s), backward 577 - 640 (its three walks read 1.41 GB and write
-// 0.41) and 21 for dg; one prompt of H16 T65000 147 + 8 + 306; a token at B256 H32 210 us, 5.1 TB/s.  A walk's bound is what its eight waves issue:
+// 0.41) and 22 for dg; one prompt of H16 T65000 147 + 8 + 306; a token at B256 H32 210 us, 5.1 TB/s.  A walk's bound is what its eight waves issue:
 // of a chunk's 5400 cycles (7200 where dg is taken) vector instructions hold a SIMD for 49 %, the matrix cores for 30 (26), and a CU, whose LDS one
 // workgroup fills, has two waves a SIMD to put between each other.
 

@@ -6,7 +6,7 @@
 // what their own mean misses is taken off (rows of 768 around 10^4 with a deviation of 2: y off by 4.8e-4 -> 4.3e-7, dx 5e-5 -> 4e-7; a per cent of the backward
 // pass's time).  The backward pass forms mean and rho again from x, which it needs anyway: nothing is kept.  Its sums over the rows stay in registers over all rows of a workgroup, which are rows of one head, and
 // leave as one partial row each; a second launch adds them (no atomics, the same from run to run).
-// 32768 rows of 2048 in bf16: forward 57 - 60 us, 4.5 - 4.7 TB/s, backward 85 - 92 (403 MB) and 7 for the sums; 32768 x 16 heads of 128: 46 - 48, 79 - 81,
+// 32768 rows of 2048 in bf16: forward 57 - 60 us, 4.5 - 4.7 TB/s, backward 82 - 93 (403 MB) and 7 for the sums; 32768 x 16 heads of 128: 46 - 49, 80 - 82,
 // 5.  A group of TPR lanes takes four rows at a time where there are workgroups enough (heads of 128: forward 55 us with one row).
 #include "lnx_common.h"
 #include "mma_tiles.h"
