@@ -1819,7 +1819,10 @@ struct DecayFn : Function<DecayFn> {
     const Tensor q = decay_rows(q0), k = decay_rows(k0), v = decay_rows(v0), g = g0.to(at::kFloat), si = f32(undef(s0));
     Tensor kept;
     auto [o, sT] = decay_forward(s, q, k, v, g, si, undef(cu), &kept);
-    ctx->save_for_backward({q, k, v, g, si, undef(cu), kept, sT});
+    ctx->save_for_backward({q, k, v, g, si, undef(cu), kept});
+    // read where its gradient is given, and only then held to what it was: decode steps may go on from it in place
+    ctx->saved_data["state"] = sT.detach();
+    ctx->saved_data["version"] = (int64_t)sT._version();
     ctx->saved_data["i"] = std::vector<int64_t>{s.B, s.H, s.T, s.dk, s.dv, s.nseq, s.rows, s.per_head, (int64_t)g0.scalar_type(), s0.has_value() && s0->requires_grad(),
                                                 (int64_t)(s0.has_value() ? s0->scalar_type() : at::kFloat)};
     ctx->saved_data["d"] = s.scale;
@@ -1841,7 +1844,10 @@ struct DecayFn : Function<DecayFn> {
     Tensor d0;
     if (m[9]) d0 = at::empty({s.rows, s.H, s.dk, s.dv}, fo);
     a.d_o = tensor4(d_o), a.d_q = tensor4(dq), a.d_k = tensor4(dk), a.d_v = tensor4(dv), a.d_g = fptr(dg), a.d_final_state = fptr(ds), a.d_initial_state = fptr(d0);
-    a.final_state = fptr(sv[7]);
+    const Tensor last = ctx->saved_data["state"].toTensor();
+    TORCH_CHECK(!ds.defined() || (int64_t)last._version() == ctx->saved_data["version"].toInt(),
+                "the gradient of decay_linear_attention: the final state, whose gradient is given, has been modified by an inplace operation");
+    a.final_state = fptr(last);
     if (kept.numel()) a.kept = fptr(kept);
     a.workspace_bytes = lnx_decay_bwd_workspace_bytes(&a);
     const Tensor ws = work_area(q, a.workspace_bytes);

@@ -128,3 +128,16 @@ def test_gates_gradients_of_a_quiet_half_beside_a_loud_one(loud, dtype):
         want = _formulas(*x, zero, d ** -0.5, do[b, h, quiet].double(), zero, CHUNK[DT[dtype]])["dg"]
         off = float((got[b, h, quiet].double() - want).norm() / want.norm())
         assert off < 2.0 ** -16, f"{off:.2g}"
+
+
+@pytest.mark.parametrize("T", [40, 1100])
+def test_decode_steps_go_on_from_a_prompts_state_in_place(T):
+    """The prompt's gradient needs its last state only where that has a gradient: otherwise a step may write over it, and its gradient is refused."""
+    t, do, ds = _inputs(1, 2, T, 64, 64, "f32", seed=44)
+    leaves = [t[n].detach().requires_grad_() for n in ("q", "k", "v", "g")]
+    o, s = la.decay_linear_attention(*leaves)
+    want = torch.autograd.grad(o, leaves, do, retain_graph=True)
+    la.decay_linear_attention_step(*(t[n][:, :, 0] for n in ("q", "k", "v", "g")), s.detach(), inplace=True)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(o, leaves, do, retain_graph=True), want))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad([o, s], leaves, [do, ds])
